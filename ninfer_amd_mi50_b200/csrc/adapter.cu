@@ -38,6 +38,7 @@ adapter_shrink_kernel(const T* __restrict__ x, const T* __restrict__ A, const fl
                       float* __restrict__ h, int K, int SR, int n, int whole) {
   __shared__ float xs[kShrinkK];
   chain_wait(x, A, scale, ids);
+  chain_release_late();                  // a product launched behind this may begin: what came before is complete
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int a = adapter_of(ids, t, n);
   if (a < 0) return;
@@ -73,6 +74,21 @@ adapter_shrink_kernel(const T* __restrict__ x, const T* __restrict__ A, const fl
       if (lane == 0 && j + q < SR) h[(size_t)t * SR + j + q] = v * scale[a];
     }
   }
+}
+
+template <typename T>
+static void launch_shrink(const void* x, const void* A, const float* scale, const int* ids, float* h, int rows, int K, int SR, int n,
+                          cudaStream_t stream) {
+  const int whole = (K * (int)sizeof(T)) % 16 == 0;
+  launch_chained(adapter_shrink_kernel<T>, dim3(rows, (SR + 2 * kShrinkWarps - 1) / (2 * kShrinkWarps)), dim3(32 * kShrinkWarps), 0, stream,
+                 (const T*)x, (const T*)A, scale, ids, h, K, SR, n, whole);
+}
+
+// The bfloat16 form alone, for adapter_tc.cu.
+int adapter_shrink_simt(const void* x, const void* A, const float* scale, const int* ids, float* h, int rows, int K, int SR, int n,
+                        cudaStream_t stream) {
+  launch_shrink<__nv_bfloat16>(x, A, scale, ids, h, rows, K, SR, n, stream);
+  return check_launch("adapter_shrink");
 }
 
 struct AdapterSlices {                    // features below end[s] belong to slice s
@@ -126,9 +142,7 @@ template <typename T>
 static int launch_adapter(const void* x, const void* A, const void* B, const float* scale, const int* ids, const float* z, float* h,
                           void* y, int rows, int N, int K, int R, int n, const AdapterSlices& slices, cudaStream_t stream) {
   const int SR = slices.n * R;
-  const int whole = (K * (int)sizeof(T)) % 16 == 0;
-  launch_chained(adapter_shrink_kernel<T>, dim3(rows, (SR + 2 * kShrinkWarps - 1) / (2 * kShrinkWarps)), dim3(32 * kShrinkWarps), 0, stream,
-                 (const T*)x, (const T*)A, scale, ids, h, K, SR, n, whole);
+  launch_shrink<T>(x, A, scale, ids, h, rows, K, SR, n, stream);
   launch_chained(adapter_expand_kernel<T>, dim3((N + 255) / 256, (rows + kExpandRows - 1) / kExpandRows), dim3(256), 0, stream, z,
                  (const float*)h, (const T*)B, ids, (T*)y, rows, N, R, SR, n, slices);
   return check_launch("adapter_add");

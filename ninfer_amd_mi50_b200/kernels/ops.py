@@ -123,6 +123,7 @@ TUNING = {
     "moe_stream_shared": 1,
     "moe_stream_shared_max_tokens": 16,
     "moe_stream_smem_kb": 192,
+    "adapter": "auto",            # "simt" | "auto": adapters beside a bfloat16 projection
 }
 
 SUPPORTED_HEAD_DIMS = tuple(range(16, 257, 16))

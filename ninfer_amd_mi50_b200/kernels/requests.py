@@ -10,7 +10,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import lib as _lib
-from .ops import _chk, _dt, _p, _stream, c_int, linear
+from .ops import TUNING, _chk, _dt, _p, _stream, c_int, linear
 
 __all__ = ["ADAPTER_RANKS", "MAX_ADAPTER_SLICES", "adapter_linear", "adapter_rank", "adjust_logits", "append_history",
            "request_status"]
@@ -74,6 +74,13 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         e += v
         ends.append(e)
     ends = (c_int * S)(*ends)
+    if x.dtype == torch.bfloat16 and K % 8 == 0 and TUNING["adapter"] == "auto":
+        lib = _lib.load()
+        h = torch.empty((lib.nf_adapter_parts(c_int(T), c_int(K)), T, S * R), dtype=torch.float32, device=x.device)
+        _lib.call("nf_adapter_linear", _p(x), _p(w), _p(a), _p(b), _p(scale), _p(ids), _p(h), _p(out), c_int(T), c_int(N), c_int(K),
+                  c_int(R), c_int(n), c_int(S), ends, _stream())
+        return out
+    # float32, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
     h = torch.empty((T, S * R), dtype=torch.float32, device=x.device)
     z = linear(x, w, out_dtype=torch.float32)
     _lib.call("nf_adapter_add", _p(x), _p(a), _p(b), _p(scale), _p(ids), _p(z), _p(h), _p(out), c_int(T), c_int(N), c_int(K),
@@ -168,8 +175,8 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
 
 
 def request_status() -> int:
-    """0, or what these kernels found outside their operands since the last call: 1 + a row whose adapter was outside the
-    pool, 1000000 + 1 + a row whose log or mask did not fit.  Synchronises the device."""
+    """0, or what these kernels met since the last call: 1 to 14 a bounded wait that ran out, 101 + a row whose adapter was
+    outside the pool, 10000001 + a row whose log or mask did not fit.  Synchronises the device."""
     lib = _lib.load()
-    ad, ru = int(lib.nf_adapter_index_status()), int(lib.nf_rules_index_status())
-    return ad if ad else (1000000 + ru if ru else 0)
+    tc, ad, ru = int(lib.nf_adapter_tc_status()), int(lib.nf_adapter_index_status()), int(lib.nf_rules_index_status())
+    return tc if tc else (100 + ad if ad else (10000000 + ru if ru else 0))
