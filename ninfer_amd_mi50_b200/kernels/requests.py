@@ -1,22 +1,63 @@
 """Python faces of the kernels for what a request brings of its own to a step that it shares: a low-rank adapter beside a
 projection, and penalties, biases and a mask on its logits.  Everything is indexed by the step's rows on the device, so
 that a step captured into a graph serves whichever requests its index tensors name.
+
+These calls come many times a step and take a few microseconds on the device, so the host's part is kept short: one
+condition over all operands, and a second look, for the message, only where it fails.
 """
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import lib as _lib
-from .ops import TUNING, _chk, _dt, _p, _stream, c_int, linear
+from .ops import TUNING, _chk, _dt, linear
 
 __all__ = ["ADAPTER_RANKS", "MAX_ADAPTER_SLICES", "adapter_linear", "adapter_rank", "adjust_logits", "append_history",
            "request_status"]
 
 ADAPTER_RANKS = (16, 32, 64, 128)       # ranks that adapters are laid out for; a smaller one is padded with zeros
 MAX_ADAPTER_SLICES = 8
+
+_I, _P = ctypes.c_int, ctypes.c_void_p
+_SIGNATURES = {
+    "nf_adapter_add": [_P] * 8 + [_I] * 6 + [_P, _I, _P],
+    "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _P],
+    "nf_append_history": [_P] * 4 + [_I] * 3 + [_P],
+    "nf_logit_rules": [_P] * 11 + [_I] + [_P] * 2 + [_I] * 7 + [_P],
+    "nf_adapter_parts": [_I] * 2,
+}
+_functions = {}
+_used = False           # whether any of these kernels was called: until then there is no status to read
+
+
+def _function(name: str):
+    f = _functions.get(name)
+    if f is None:
+        f = getattr(_lib.load(), name)
+        f.argtypes = _SIGNATURES[name]
+        _functions[name] = f
+    return f
+
+
+def _call(name: str, *args) -> None:
+    global _used
+    _used = True
+    rc = _function(name)(*args)
+    _lib.count_launches(1)
+    if rc != 0:
+        raise _lib.KernelError(f"{name}: {_lib.load().nf_last_error().decode(errors='replace')}")
+
+
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def adapter_rank(rank: int) -> int:
@@ -25,6 +66,39 @@ def adapter_rank(rank: int) -> int:
         if 1 <= rank <= r:
             return r
     raise ValueError(f"adapter rank {rank} is not supported (1..{ADAPTER_RANKS[-1]})")
+
+
+def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
+    """Says what is wrong with the operands of adapter_linear."""
+    _chk(x, "x")
+    for t, name in ((w, "w"), (a, "a"), (b, "b"), (scale, "scale"), (ids, "ids"), (out, "out")):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"adapter_linear: {name} lies on {t.device}, x on {x.device}")
+    _chk(w, "w", x.dtype); _chk(a, "a", x.dtype); _chk(b, "b", x.dtype)
+    _chk(scale, "scale", torch.float32); _chk(ids, "ids", torch.int32)
+    _dt(x)
+    if x.dim() != 2 or w.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError("adapter_linear takes x [T, K], w [N, K], a [n, slices * R, K] and b [n, N, R]")
+    T, K = x.shape
+    N, n, R, S = w.shape[0], b.shape[0], b.shape[2], len(widths)
+    if w.shape[1] != K:
+        raise ValueError(f"adapter_linear: x has {K} columns, w has {w.shape[1]}")
+    if not 1 <= S <= MAX_ADAPTER_SLICES or min(widths) < 1 or sum(widths) != N:
+        raise ValueError(f"adapter_linear: widths {list(widths)} are not 1 to {MAX_ADAPTER_SLICES} positive parts of {N} features")
+    if R not in ADAPTER_RANKS:
+        raise ValueError(f"adapter_linear: rank {R} is not one of {ADAPTER_RANKS}; pad with zeros")
+    if n < 1 or K < 1 or a.shape != (n, S * R, K) or b.shape[1] != N:
+        raise ValueError(f"adapter_linear: a {tuple(a.shape)} and b {tuple(b.shape)} do not fit {S} parts, rank {R} and w "
+                         f"{tuple(w.shape)}")
+    if scale.shape != (n,) or ids.shape != (T,):
+        raise ValueError(f"adapter_linear: scale {tuple(scale.shape)} and ids {tuple(ids.shape)} for {n} adapters and {T} rows")
+    if out is not None:
+        _chk(out, "out", x.dtype)
+        if out.shape != (T, N):
+            raise ValueError(f"adapter_linear: out is {tuple(out.shape)}, not {(T, N)}")
+    for t, name in ((x, "x"), (w, "w"), (a, "a"), (b, "b"), (out, "out")):
+        if t is not None and t.data_ptr() % 16:
+            raise ValueError(f"adapter_linear: {name} does not start on a 16-byte boundary")
 
 
 def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, ids: torch.Tensor,
@@ -36,55 +110,46 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     `widths`: the parts that the N features are stacked of (query, key and value, say), each with rows of `a` of its own;
     [N] if left out.  a [n, len(widths) * R, K] (the parts' rows one after the other), b [n, N, R], R one of
     `ADAPTER_RANKS`, scale float32 [n], ids int32 [T].  Sums are float32 and rounded once, to x's type.  An id outside
-    [-1, n) is served like -1 and reported by `check_status`.  The weights of all adapters have to be finite: rows of
-    several requests share a product, in which another request's adapter is multiplied by zero."""
-    for t, name in ((x, "x"), (w, "w"), (a, "a"), (b, "b"), (scale, "scale"), (ids, "ids")):
-        if t.device != x.device:
-            raise ValueError(f"adapter_linear: {name} lies on {t.device}, x on {x.device}")
-    _chk(x, "x"); _chk(w, "w", x.dtype); _chk(a, "a", x.dtype); _chk(b, "b", x.dtype)
-    _chk(scale, "scale", torch.float32); _chk(ids, "ids", torch.int32)
-    dt = _dt(x)
-    if x.dim() != 2 or w.dim() != 2 or a.dim() != 3 or b.dim() != 3:
-        raise ValueError("adapter_linear takes x [T, K], w [N, K], a [n, slices * R, K] and b [n, N, R]")
-    T, K = x.shape
-    N = w.shape[0]
-    widths = [N] if widths is None else [int(v) for v in widths]
-    n, R, S = b.shape[0], b.shape[2], len(widths)
-    if w.shape[1] != K:
-        raise ValueError(f"adapter_linear: x has {K} columns, w has {w.shape[1]}")
-    if not 1 <= S <= MAX_ADAPTER_SLICES or min(widths) < 1 or sum(widths) != N:
-        raise ValueError(f"adapter_linear: widths {widths} are not 1 to {MAX_ADAPTER_SLICES} positive parts of {N} features")
-    if R not in ADAPTER_RANKS:
-        raise ValueError(f"adapter_linear: rank {R} is not one of {ADAPTER_RANKS}; pad with zeros")
-    if n < 1 or a.shape != (n, S * R, K) or b.shape[1] != N:
-        raise ValueError(f"adapter_linear: a {tuple(a.shape)} and b {tuple(b.shape)} do not fit {S} parts, rank {R} and w "
-                         f"{tuple(w.shape)}")
-    if scale.shape != (n,) or ids.shape != (T,):
-        raise ValueError(f"adapter_linear: scale {tuple(scale.shape)} and ids {tuple(ids.shape)} for {n} adapters and {T} rows")
+    [-1, n) is served like -1 and, from n on, reported by `check_status`.  The weights of all adapters have to be finite:
+    rows of several requests share a product, in which another request's adapter is multiplied by zero."""
+    if widths is None:
+        widths = (w.shape[0],)
+    dtype, dev = x.dtype, x.get_device()
+    xs, ws, bs = x.shape, w.shape, b.shape
+    S = len(widths)
+    if not (dev >= 0 and len(xs) == 2 and len(ws) == 2 and len(bs) == 3 and (dtype is torch.bfloat16 or dtype is torch.float32)
+            and w.dtype is dtype and a.dtype is dtype and b.dtype is dtype and scale.dtype is torch.float32
+            and ids.dtype is torch.int32 and w.get_device() == dev and a.get_device() == dev and b.get_device() == dev
+            and scale.get_device() == dev and ids.get_device() == dev and x.is_contiguous() and w.is_contiguous()
+            and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous() and ids.is_contiguous()):
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
+    T, K = xs
+    N, (n, _, R) = ws[0], bs
+    if not (K > 0 and ws[1] == K and n > 0 and bs[1] == N and R in ADAPTER_RANKS and 1 <= S <= MAX_ADAPTER_SLICES
+            and min(widths) > 0 and sum(widths) == N and a.shape == (n, S * R, K) and scale.shape == (n,) and ids.shape == (T,)):
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     if out is None:
-        out = torch.empty((T, N), dtype=x.dtype, device=x.device)
-    else:
-        _chk(out, "out", x.dtype)
-        if out.shape != (T, N) or out.device != x.device:
-            raise ValueError(f"adapter_linear: out is {tuple(out.shape)} on {out.device}, not {(T, N)} on {x.device}")
+        out = x.new_empty((T, N))
+    elif not (out.dtype is dtype and out.get_device() == dev and out.is_contiguous() and out.shape == (T, N)):
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     if T == 0:
         return out
-    ends, e = [], 0
-    for v in widths:
+    px, pw, pa, pb, po = x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), out.data_ptr()
+    if (px | pw | pa | pb | po) & 15:
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
+    ends, e = (_I * S)(), 0
+    for i, v in enumerate(widths):
         e += v
-        ends.append(e)
-    ends = (c_int * S)(*ends)
-    if x.dtype == torch.bfloat16 and K % 8 == 0 and TUNING["adapter"] == "auto":
-        lib = _lib.load()
-        h = torch.empty((lib.nf_adapter_parts(c_int(T), c_int(K)), T, S * R), dtype=torch.float32, device=x.device)
-        _lib.call("nf_adapter_linear", _p(x), _p(w), _p(a), _p(b), _p(scale), _p(ids), _p(h), _p(out), c_int(T), c_int(N), c_int(K),
-                  c_int(R), c_int(n), c_int(S), ends, _stream())
+        ends[i] = e
+    if dtype is torch.bfloat16 and K % 8 == 0 and TUNING["adapter"] == "auto":
+        h = scale.new_empty(_function("nf_adapter_parts")(T, K) * T * S * R)
+        _call("nf_adapter_linear", px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream())
         return out
     # float32, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
-    h = torch.empty((T, S * R), dtype=torch.float32, device=x.device)
+    h = scale.new_empty(T * S * R)
     z = linear(x, w, out_dtype=torch.float32)
-    _lib.call("nf_adapter_add", _p(x), _p(a), _p(b), _p(scale), _p(ids), _p(z), _p(h), _p(out), c_int(T), c_int(N), c_int(K),
-              c_int(R), c_int(n), c_int(S), ends, c_int(dt), _stream())
+    _call("nf_adapter_add", px, pa, pb, scale.data_ptr(), ids.data_ptr(), z.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _dt(x),
+          _stream())
     return out
 
 
@@ -100,8 +165,63 @@ def append_history(history: torch.Tensor, slots: torch.Tensor, positions: torch.
     if history.dim() != 2:
         raise ValueError("append_history: history is [slots, capacity]")
     if tokens.numel():
-        _lib.call("nf_append_history", _p(history), _p(slots), _p(positions), _p(tokens), c_int(tokens.numel()),
-                  c_int(history.shape[0]), c_int(history.shape[1]), _stream())
+        _call("nf_append_history", history.data_ptr(), slots.data_ptr(), positions.data_ptr(), tokens.data_ptr(), tokens.numel(),
+              history.shape[0], history.shape[1], _stream())
+
+
+def _rows_apart(t: torch.Tensor, R: int, V: int) -> int:
+    """Elements between two rows of [R, V], or -1 where the rows are not runs of their own."""
+    step, one = t.stride()
+    if R <= 1:
+        step = V
+    return step if (one == 1 or V <= 1) and step >= V else -1
+
+
+def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out) -> None:
+    """Says what is wrong with the operands of adjust_logits."""
+    _chk(logits, "logits", torch.float32, contiguous=False); _chk(history, "history", torch.int32)
+    if logits.dim() != 2 or history.dim() != 2:
+        raise ValueError("adjust_logits takes logits [R, V] and history [slots, capacity]")
+    R, V = logits.shape
+    _chk(penalties, "penalties", torch.float32)
+    if penalties.shape != (R, 3):
+        raise ValueError(f"adjust_logits: penalties are {tuple(penalties.shape)}, not {(R, 3)}")
+    lists = [(slots, "slots", R), (lengths, "lengths", R), (starts, "starts", R)]
+    if tokens is not None:
+        lists.append((tokens, "tokens", R))
+    others = [history, penalties]
+    if bias is not None:
+        offsets, ids, values = bias
+        lists += [(offsets, "bias offsets", R + 1), (ids, "bias ids", ids.numel())]
+        _chk(values, "bias values", torch.float32)
+        if values.shape != ids.shape:
+            raise ValueError(f"adjust_logits: {tuple(ids.shape)} bias ids, {tuple(values.shape)} values")
+        others.append(values)
+    if mask is not None:
+        bits, index = mask
+        lists.append((index, "mask index", R))
+        _chk(bits, "mask bits", torch.int32)
+        if bits.dim() != 2 or bits.shape[0] < 1 or bits.shape[1] != (V + 31) // 32:
+            raise ValueError(f"adjust_logits: mask bits are {tuple(bits.shape)}, not [M, {(V + 31) // 32}]")
+        others.append(bits)
+    for t, name, n in lists:
+        _chk(t, name, torch.int32)
+        if t.shape != (n,):
+            raise ValueError(f"adjust_logits: {name} are {tuple(t.shape)}, not {(n,)}")
+    if out is not None:
+        _chk(out, "out", torch.float32, contiguous=False)
+        if out.shape != (R, V):
+            raise ValueError(f"adjust_logits: out is {tuple(out.shape)}, not {(R, V)}")
+        others.append(out)
+    for t in others + [v[0] for v in lists]:
+        if t.device != logits.device:
+            raise ValueError(f"adjust_logits: a tensor lies on {t.device}, the logits on {logits.device}")
+    for t, name in ((logits, "logits"), (out, "out")):
+        if t is not None and R and V and _rows_apart(t, R, V) < 0:
+            raise ValueError(f"adjust_logits: the rows of {name} must be runs of their own, got strides {t.stride()}")
+    if history.shape[0] < 1 or history.shape[1] < 4 or history.shape[1] % 4 or history.data_ptr() % 16:
+        raise ValueError(f"adjust_logits: history is {tuple(history.shape)}; its capacity must be a multiple of 4, its start a "
+                         f"16-byte boundary")
 
 
 def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor,
@@ -117,66 +237,73 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
         v = logit;  v = v > 0 ? v / p^c : v p^c;  v -= f g + q [g > 0];  v += bias;  out = allowed ? v : -inf
 
     (1, 0, 0 changes nothing.)  `tokens` int32 [R]: the last token of each row, which is written to its log here, at
-    lengths[r] - 1; left out, the log holds it already.  `bias` = (offsets int32 [R + 1], ids int32, values float32): the
-    entries of row r are those from offsets[r] to offsets[r + 1], each id once.  `mask` = (bits int32 [M, (V + 31) // 32],
-    index int32 [R]): bit i % 32 of word i // 32 of row index[r] is set where token i is allowed; index -1: no mask.  A
-    row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself.  A slot, a length or a mask row
-    outside its tensor changes that row as if it had no tokens or no mask, and is reported by `check_status`."""
-    _chk(logits, "logits", torch.float32, contiguous=False); _chk(history, "history", torch.int32)
-    if logits.dim() != 2 or history.dim() != 2:
-        raise ValueError("adjust_logits takes logits [R, V] and history [slots, capacity]")
-    R, V = logits.shape
-    _chk(penalties, "penalties", torch.float32)
-    if penalties.shape != (R, 3):
-        raise ValueError(f"adjust_logits: penalties are {tuple(penalties.shape)}, not {(R, 3)}")
-    lists = [(slots, "slots", R), (lengths, "lengths", R), (starts, "starts", R)]
-    if tokens is not None:
-        lists.append((tokens, "tokens", R))
-    offsets = ids = values = bits = index = None
+    lengths[r] - 1; left out, the log holds it already.  No two rows may write to one slot.  `bias` = (offsets int32
+    [R + 1], ids int32, values float32): the entries of row r are those from offsets[r] to offsets[r + 1], each id once.
+    `mask` = (bits int32 [M, (V + 31) // 32], index int32 [R]): bit i % 32 of word i // 32 of row index[r] is set where
+    token i is allowed; index -1: no mask.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits`
+    itself.  A slot, a length or a mask row outside its tensor changes that row as if it had no tokens or no mask, and is
+    reported by `check_status`."""
+    operands = (logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
+    dev = logits.get_device()
+    ls, hs = logits.shape, history.shape
+    if not (dev >= 0 and len(ls) == 2 and len(hs) == 2 and logits.dtype is torch.float32 and history.dtype is torch.int32
+            and slots.dtype is torch.int32 and lengths.dtype is torch.int32 and starts.dtype is torch.int32
+            and penalties.dtype is torch.float32 and history.get_device() == dev and slots.get_device() == dev
+            and lengths.get_device() == dev and starts.get_device() == dev and penalties.get_device() == dev
+            and history.is_contiguous() and slots.is_contiguous() and lengths.is_contiguous() and starts.is_contiguous()
+            and penalties.is_contiguous()):
+        _refuse_logits(*operands)
+    R, V = ls
+    one = (R,)
+    if not (slots.shape == one and lengths.shape == one and starts.shape == one and penalties.shape == (R, 3) and hs[0] > 0
+            and hs[1] > 0 and hs[1] % 4 == 0 and history.data_ptr() % 16 == 0):
+        _refuse_logits(*operands)
+    if tokens is not None and not (tokens.dtype is torch.int32 and tokens.get_device() == dev and tokens.is_contiguous()
+                                   and tokens.shape == one):
+        _refuse_logits(*operands)
+    p_off = p_ids = p_values = p_bits = p_index = None
+    n_bias = n_masks = 0
     if bias is not None:
         offsets, ids, values = bias
-        lists += [(offsets, "bias offsets", R + 1), (ids, "bias ids", ids.numel())]
-        _chk(values, "bias values", torch.float32)
-        if values.shape != ids.shape:
-            raise ValueError(f"adjust_logits: {tuple(ids.shape)} bias ids, {tuple(values.shape)} values")
+        n_bias = ids.numel()
+        if not (offsets.dtype is torch.int32 and ids.dtype is torch.int32 and values.dtype is torch.float32
+                and offsets.get_device() == dev and ids.get_device() == dev and values.get_device() == dev
+                and offsets.is_contiguous() and ids.is_contiguous() and values.is_contiguous() and offsets.shape == (R + 1,)
+                and ids.shape == (n_bias,) and values.shape == (n_bias,)):
+            _refuse_logits(*operands)
+        p_off, p_ids, p_values = offsets.data_ptr(), ids.data_ptr(), values.data_ptr()
     if mask is not None:
         bits, index = mask
-        lists.append((index, "mask index", R))
-        _chk(bits, "mask bits", torch.int32)
-        if bits.dim() != 2 or bits.shape[0] < 1 or bits.shape[1] != (V + 31) // 32:
-            raise ValueError(f"adjust_logits: mask bits are {tuple(bits.shape)}, not [M, {(V + 31) // 32}]")
-    for t, name, n in lists:
-        _chk(t, name, torch.int32)
-        if t.shape != (n,):
-            raise ValueError(f"adjust_logits: {name} are {tuple(t.shape)}, not {(n,)}")
-    for t in (history, penalties, values, bits, *(v[0] for v in lists)):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"adjust_logits: a tensor lies on {t.device}, the logits on {logits.device}")
+        n_masks = bits.shape[0] if bits.dim() == 2 else 0
+        if not (bits.dtype is torch.int32 and index.dtype is torch.int32 and bits.get_device() == dev and index.get_device() == dev
+                and bits.is_contiguous() and index.is_contiguous() and n_masks > 0 and bits.shape[1] == (V + 31) // 32
+                and index.shape == one):
+            _refuse_logits(*operands)
+        p_bits, p_index = bits.data_ptr(), index.data_ptr()
     if out is None:
-        out = torch.empty((R, V), dtype=torch.float32, device=logits.device)
-    _chk(out, "out", torch.float32, contiguous=False)
-    if out.shape != (R, V) or out.device != logits.device:
-        raise ValueError(f"adjust_logits: out is {tuple(out.shape)} on {out.device}, not {(R, V)} on {logits.device}")
-    strides = []
-    for t, name in ((logits, "logits"), (out, "out")):
-        step = t.stride(0) if R > 1 else V
-        if V > 1 and t.stride(1) != 1 or step < V:
-            raise ValueError(f"adjust_logits: the rows of {name} must be runs of their own, got strides {t.stride()}")
-        strides.append(step)
+        out = history.new_empty((R, V), dtype=torch.float32)
+        apart_out = V
+    else:
+        if not (out.dtype is torch.float32 and out.get_device() == dev and out.shape == ls):
+            _refuse_logits(*operands)
+        apart_out = _rows_apart(out, R, V)
     if R == 0 or V == 0:
         return out
-    if history.shape[0] < 1 or history.shape[1] < 4 or history.shape[1] % 4:
-        raise ValueError(f"adjust_logits: history is {tuple(history.shape)}; its capacity must be a multiple of 4")
-    _lib.call("nf_logit_rules", _p(logits), _p(out), _p(history), _p(slots), _p(lengths), _p(starts), _p(tokens), _p(penalties),
-              _p(offsets), _p(ids), _p(values), c_int(0 if ids is None else ids.numel()), _p(bits), _p(index),
-              c_int(0 if bits is None else bits.shape[0]), c_int(R), c_int(V), c_int(strides[0]), c_int(strides[1]),
-              c_int(history.shape[0]), c_int(history.shape[1]), _stream())
+    apart = _rows_apart(logits, R, V)
+    if apart < 0 or apart_out < 0:
+        _refuse_logits(*operands)
+    _call("nf_logit_rules", logits.data_ptr(), out.data_ptr(), history.data_ptr(), slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
+          _ptr(tokens), penalties.data_ptr(), p_off, p_ids, p_values, n_bias, p_bits, p_index, n_masks, R, V, apart, apart_out, hs[0],
+          hs[1], _stream())
     return out
 
 
 def request_status() -> int:
     """0, or what these kernels met since the last call: 1 to 14 a bounded wait that ran out, 101 + a row whose adapter was
-    outside the pool, 10000001 + a row whose log or mask did not fit.  Synchronises the device."""
+    outside the pool, 10000001 + a row whose log or mask did not fit.  Synchronises the device; where none of them was ever
+    called there is nothing to read."""
+    if not _used:
+        return 0
     lib = _lib.load()
     tc, ad, ru = int(lib.nf_adapter_tc_status()), int(lib.nf_adapter_index_status()), int(lib.nf_rules_index_status())
     return tc if tc else (100 + ad if ad else (10000000 + ru if ru else 0))
