@@ -41,19 +41,95 @@ struct TcSlices {
   int end[8];
 };
 
-// bf16 x bf16 -> f32, both operands K-major, 128 rows, n columns
-__device__ __forceinline__ unsigned ad_instr_desc(int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(kAdM >> 4) << 24);
+// bf16 x bf16 -> f32, both operands K-major, m rows, n columns
+__device__ __forceinline__ unsigned ad_instr_desc(int n, int m) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ unsigned cluster_addr(unsigned local, int rank) {
+  unsigned remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One CTA, or the two of a cluster that work on one tile.  Barriers that the products' issuer waits for are those of the even CTA.
+template <int CTAS>
+__device__ __forceinline__ void tc_alloc(unsigned* base, unsigned cols) {
+  if (CTAS == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void tc_dealloc(unsigned base, unsigned cols) {
+  if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, void* bar) {
+  if (CTAS == 2) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(cluster_addr(smem_u32(bar), 0)) : "memory");
+  } else {
+    tma_load_2d(dst, map, x, y, bar);
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+  if (CTAS == 2) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  } else {
+    tc_mma(d, a, b, idesc, accumulate);
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void commit(void* bar) {
+  if (CTAS == 2) {
+    const unsigned short both = 3;
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(both) : "memory");
+  } else {
+    tc_commit(bar);
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void arrive_leader(void* bar) {
+  if (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(smem_u32(bar), 0)) : "memory");
+  else mbar_arrive(bar);
+}
+// mbar_wait for arrivals that may come from the other CTA of the cluster.
+__device__ __forceinline__ bool mbar_wait_cluster(void* bar, unsigned parity, volatile int* stop, int code) {
+  for (unsigned i = 0; i < kPollLimit; ++i) {
+    unsigned ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 1023u) == 1023u && *stop) return false;
+  }
+  *stop = 1;
+  atomicCAS(&g_adapter_tc_error, 0, code);
+  return false;
 }
 
 // The adapters that occur among a tile's rows, in ascending order: each lane holds four rows' ids (-1: none), the next one
 // is the smallest above the last.
+template <int CTAS>
 struct TileIds {
-  int v[4];
+  int v[4 * CTAS];
   __device__ __forceinline__ void load(const int* ids, int row0, int rows, int n) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * CTAS; ++i) {
       const int t = row0 + lane + 32 * i;
       const int a = t < rows ? ids[t] : -1;
       v[i] = a >= 0 && a < n ? a : -1;
@@ -62,7 +138,7 @@ struct TileIds {
   __device__ __forceinline__ int next(int last) const {
     int m = kNone;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = v[i] > last ? min(m, v[i]) : m;
+    for (int i = 0; i < 4 * CTAS; ++i) m = v[i] > last ? min(m, v[i]) : m;
     return __reduce_min_sync(0xffffffffu, m);
   }
 };
@@ -70,35 +146,65 @@ struct TileIds {
 // ---- h: the adapters' first product ---------------------------------------------------------------------------------------
 
 struct __align__(8) ShrinkBars {
-  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2];
+  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full, acc_empty;
   unsigned tmem_base;
   int stop;
+  unsigned char served[kAdM];           // rows of the tile whose adapter this CTA has taken
 };
 
-// D[j, t] = sum over this CTA's part of k of A[a, j, k] x[t, k], for the adapters a of a tile of up to 128 rows: every
-// gridDim.z-th of those that occur.  Parts of k are left beside one another in h [parts, rows, SR], for whoever reads them to add.
-// 192 threads: producer, MMA, four epilogue warps.  grid: (parts of k, row tiles * tiles of 128 j, adapters in turn).
+// CTAs of a cluster wait for one another, and an allocation of tensor memory waits for the SM's other CTAs: whatever of these
+// kernels may meet on an SM, from several streams too, has to find its columns at once.  One CTA of this kernel (256 columns, more
+// than half of the shared memory) beside those of adapter_rows_kernel (64 each, that split k 36 KB each) do; the wide kernel, and
+// all others that take all columns, leave no shared memory for either.
+constexpr size_t kShrinkSmemLeast = 120 * 1024;
+constexpr int kShrinkCols = 256;        // columns of an accumulator: numbers of h of all adapters of a pass
+
+// Writes 8 numbers of h: as they are, or as the nearest bfloat16 and what that leaves, SR numbers behind one another.
+__device__ __forceinline__ void put_h(float* h, int t, int SR, int j, const float* v, bool split) {
+  if (!split) {
+    store4(h + (size_t)t * SR + j, v);
+    store4(h + (size_t)t * SR + j + 4, v + 4);
+    return;
+  }
+  __nv_bfloat162 hi[4], lo[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    const float2 back = __bfloat1622float2(hi[e]);
+    // (of an infinity nothing is left)
+    lo[e] = __floats2bfloat162_rn(isinf(back.x) ? 0.f : v[2 * e] - back.x, isinf(back.y) ? 0.f : v[2 * e + 1] - back.y);
+  }
+  __nv_bfloat16* row = reinterpret_cast<__nv_bfloat16*>(h) + (size_t)t * 2 * SR + j;
+  *reinterpret_cast<uint4*>(row) = *reinterpret_cast<uint4*>(hi);
+  *reinterpret_cast<uint4*>(row + SR) = *reinterpret_cast<uint4*>(lo);
+}
+
+// D[t, (adapter, j)] over a tile of up to 128 rows: x is the 128-row operand, the rows of A of up to `group` of the adapters
+// that occur in the tile the other, so that x is read once for all of them.  The CTAs of a cluster split k; each leaves every
+// row's own numbers in `part` [members, rows, SR], and after the cluster's barrier adds up, scales and writes a share of rows.
+// 192 threads: producer, MMA, four epilogue warps (a thread a row).  grid: (members, row tiles * j tiles, groups in turn).
 __global__ void __launch_bounds__(192, 1)
 adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ scale,
-                         const int* __restrict__ ids, float* __restrict__ h, int rows, int K, int SR, int n, int row_tiles, int NT,
-                         int a_box, int stages) {
+                         const int* __restrict__ ids, float* part, float* h, int rows, int K, int SR, int n, int row_tiles, int x_box, int JW,
+                         int group, int stages, int split) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   ShrinkBars* bars = reinterpret_cast<ShrinkBars*>(smem);
   unsigned char* stage0 = smem + 1024;
-  const int stage_bytes = kAdTile + NT * 128;
+  const int stage_bytes = kAdTile + group * JW * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int members = gridDim.x, member = blockIdx.x;
   volatile int* stop = &bars->stop;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&bars->acc_full[b], 1); mbar_init(&bars->acc_empty[b], 4); }
+    mbar_init(&bars->acc_full, 1);
+    mbar_init(&bars->acc_empty, 4);
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(256) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (threadIdx.x < kAdM) bars->served[threadIdx.x] = 0;
+  __syncwarp();
+  if (warp == 1) tc_alloc<1>(&bars->tmem_base, kShrinkCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -106,123 +212,161 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   chain_wait(ids, scale);
   chain_release_late();               // the product behind this may begin: what came before is complete
   const int tile = blockIdx.y % row_tiles, jt = blockIdx.y / row_tiles;
-  const int row0 = tile * kAdM, j0 = jt * kAdM;
+  const int row0 = tile * kAdM, j0 = jt * JW, jn = min(JW, SR - j0);
   const int steps = (K + kAdK - 1) / kAdK;
-  const int k_first = (int)((long long)blockIdx.x * steps / gridDim.x), k_last = (int)((long long)(blockIdx.x + 1) * steps / gridDim.x);
-  TileIds tids;
+  const int k_first = (int)((long long)member * steps / members), k_last = (int)((long long)(member + 1) * steps / members);
+  TileIds<1> tids;
   tids.load(ids, row0, rows, n);
+  // the next group of adapters: lane g holds the g-th; returns how many
+  int last = -1;
+  auto next_group = [&](int& mine) {
+    int count = 0;
+    while (count < group) {
+      const int a = tids.next(last);
+      if (a == kNone) break;
+      if (lane == count) mine = a;
+      last = a;
+      ++count;
+    }
+    return count;
+  };
 
   if (warp == 0) {
-    int it = 0, turn = 0, issued = 0;
+    int it = 0, issued = 0, mine = 0;
     bool ok = true;
-    for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a), ++turn) {
+    for (int turn = 0;; ++turn) {
+      const int count = next_group(mine);
+      if (!count || !ok) break;
       if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
-      if (lane == 0) {
-        for (int ks = k_first; ks < k_last; ++ks, ++it) {
-          const int s = it % stages;
-          if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1, &g_adapter_tc_error)) { ok = false; break; }
-          unsigned char* st = stage0 + (size_t)s * stage_bytes;
-          mbar_expect_tx(&bars->full[s], a_box * 128 + NT * 128);
-          tma_load_2d(st, &map_a, ks * kAdK, a * SR + j0, &bars->full[s]);
-          tma_load_2d(st + kAdTile, &map_x, ks * kAdK, row0, &bars->full[s]);
-          issued = it + 1;
+      for (int ks = k_first; ks < k_last; ++ks, ++it) {
+        const int s = it % stages;
+        if (!warp_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1)) { ok = false; break; }
+        unsigned char* st = stage0 + (size_t)s * stage_bytes;
+        if (lane == 0) {
+          mbar_expect_tx(&bars->full[s], x_box * 128 + count * JW * 128);
+          tma_load_2d(st, &map_x, ks * kAdK, row0, &bars->full[s]);
         }
+        __syncwarp();
+        if (lane < count) tma_load_2d(st + kAdTile + lane * JW * 128, &map_a, ks * kAdK, mine * SR + j0, &bars->full[s]);
+        issued = it + 1;
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
     if (!ok && lane == 0) {
       for (int j = max(0, issued - stages); j < issued; ++j)
         for (unsigned i = 0; i < (1u << 20); ++i)
           if (mbar_try(&bars->full[j % stages], (j / stages) & 1)) break;
     }
+    __syncwarp();
   } else if (warp == 1) {
-    int it = 0, turn = 0, done = 0;
+    int it = 0, done = 0, mine = 0;
     bool ok = true;
-    const unsigned idesc = ad_instr_desc(NT);
-    for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a), ++turn) {
+    for (int turn = 0;; ++turn) {
+      const int count = next_group(mine);
+      if (!count || !ok) break;
       if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
       if (lane == 0) {
-        const int ab = done & 1;
-        if (!mbar_wait(&bars->acc_empty[ab], ((done >> 1) & 1) ^ 1, stop, 2, &g_adapter_tc_error)) ok = false;
+        const unsigned idesc = ad_instr_desc(count * JW, kAdM);
+        if (!mbar_wait(&bars->acc_empty, (done & 1) ^ 1, stop, 2, &g_adapter_tc_error)) ok = false;
         tc_fence_after();
         for (int ks = k_first; ks < k_last && ok; ++ks, ++it) {
           const int s = it % stages;
           if (!mbar_wait(&bars->full[s], (it / stages) & 1, stop, 3, &g_adapter_tc_error)) { ok = false; break; }
           tc_fence_after();
           unsigned char* st = stage0 + (size_t)s * stage_bytes;
-          const unsigned long long da = smem_desc(st), db = smem_desc(st + kAdTile);
+          const unsigned long long dx = smem_desc(st), da = smem_desc(st + kAdTile);
 #pragma unroll
-          for (int kk = 0; kk < kAdK / 16; ++kk) tc_mma(tmem + ab * 128, da + 2 * kk, db + 2 * kk, idesc, ks > k_first || kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < kAdK / 16; ++kk)
+            tc_mma(tmem, dx + 2 * kk, da + 2 * kk, idesc, ks > k_first || kk > 0 ? 1u : 0u);
           tc_commit(&bars->empty[s]);
         }
-        if (ok) tc_commit(&bars->acc_full[ab]);
+        if (ok) tc_commit(&bars->acc_full);
       }
       ++done;
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
   } else {
-    const int quad = warp & 3, j = j0 + quad * 32 + lane;
-    int turn = 0, done = 0;
-    float* part = h + (size_t)blockIdx.x * rows * SR;
-    for (int a = tids.next(-1); a != kNone; a = tids.next(a), ++turn) {
+    const int quad = warp & 3, r = quad * 32 + lane, t = row0 + r;
+    const int own = t < rows ? ids[t] : -1;
+    int done = 0, mine = 0;
+    float* to = part + ((size_t)member * rows + t) * SR + j0;
+    for (int turn = 0;; ++turn) {
+      const int count = next_group(mine);
+      if (!count) break;
       if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
-      const int ab = done & 1;
-      if (!warp_wait(&bars->acc_full[ab], (done >> 1) & 1, stop, 4)) break;
+      if (!warp_wait(&bars->acc_full, done & 1, stop, 4)) break;
       tc_fence_after();
-      const float sc = scale[a];
-      const unsigned at = tmem + ab * 128 + ((unsigned)(quad * 32) << 16);
-#pragma unroll 1
-      for (int q = 0; q * 32 < NT; ++q) {
-        const int id = q == 0 ? tids.v[0] : q == 1 ? tids.v[1] : q == 2 ? tids.v[2] : tids.v[3];
-        const unsigned mine = __ballot_sync(0xffffffffu, id == a);      // this tile's rows 32 q .. 32 q + 31 with adapter a
-        if (!mine) continue;
-        unsigned v[32];
-        if (q * 32 + 32 <= NT) tc_ld32(at + q * 32, v);
-        else tc_ld16(at + q * 32, v);                  // (NT is a multiple of 16)
-        tc_wait_ld();
-        if (j < SR) {
+      for (int g = 0; g < count; ++g) {
+        const int a = __shfl_sync(0xffffffffu, mine, g);       // (every lane, before any condition on its own row)
+        const bool is = own == a;
+        if (!__any_sync(0xffffffffu, is)) continue;
+        const unsigned at = tmem + g * JW + ((unsigned)(quad * 32) << 16);
+        for (int c = 0; c < jn; c += 16) {
+          unsigned v[16];
+          tc_ld16(at + c, v);
+          tc_wait_ld();
+          if (is) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (mine & (1u << c)) part[(size_t)(row0 + q * 32 + c) * SR + j] = __uint_as_float(v[c]) * sc;
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(to + c + e) = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]),
+                                                                   __uint_as_float(v[e + 3]));
+          }
         }
+        if (is) bars->served[r] = 1;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+      if (lane == 0) mbar_arrive(&bars->acc_empty);
       ++done;
     }
+  }
+  __syncwarp();
+  cluster_barrier();                  // every member's part is there
+  const int r_first = member * kAdM / members, r_count = (member + 1) * kAdM / members - r_first, pieces = jn >> 3;
+  for (int i = threadIdx.x; i < r_count * pieces; i += blockDim.x) {
+    const int r = r_first + i / pieces, j = j0 + (i % pieces) * 8, t = row0 + r;
+    if (!bars->served[r]) continue;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < members; ++m) {
+      const float4* p = reinterpret_cast<const float4*>(part + ((size_t)m * rows + t) * SR + j);
+      const float4 a = __ldcg(p), b = __ldcg(p + 1);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    const float sc = scale[ids[t]];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= sc;
+    put_h(h, t, SR, j, v, split != 0);
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
+    tc_dealloc<1>(tmem, kShrinkCols);
   }
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------
 
 struct __align__(8) WideBars {
-  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full, h_empty;
+  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full[2], h_empty[2];
   unsigned tmem_base;
   int stop;
 };
 
 constexpr int kWideEpilogueWarps = 8;
 constexpr int kWideThreads = 32 * (2 + 4 + kWideEpilogueWarps);
-constexpr int kWideHead = 1024, kWideH = 2 * kAdTile;      // barriers; the two parts of a tile's rows of h
+constexpr int kWideHead = 1024, kWideH = 2 * kAdTile;      // barriers; rows of h
 constexpr int kWideSmem = 225 * 1024;
 
 struct WideTile {
   int row0, f0, width, slice;
 };
 // Tile i: features vary fastest, so that the CTAs that run together share rows of x and go through W side by side.
-__device__ __forceinline__ WideTile wide_tile(int i, int f_tiles, int BN, const TcSlices& sl) {
+__device__ __forceinline__ WideTile wide_tile(int i, int f_tiles, int tile_rows, int BN, const TcSlices& sl) {
   WideTile w;
   const int m = i / f_tiles;
   int f = i - m * f_tiles, begin = 0;
-  w.row0 = m * kAdM;
-  w.slice = 0;
+  w.row0 = m * tile_rows;
   for (int s = 0;; ++s) {
     const int tiles = (sl.end[s] - begin + BN - 1) / BN;
     if (f < tiles || s + 1 >= sl.n) {
@@ -236,55 +380,64 @@ __device__ __forceinline__ WideTile wide_tile(int i, int f_tiles, int BN, const 
   }
 }
 
+// CTAS 1: a CTA a tile of 128 rows x BN features.  CTAS 2: two CTAs of a cluster a tile of 256 x BN; each holds its own 128 rows of x
+// and half of the features' rows of W, and the even one issues products over both (`cta_group::2`): half of W's bytes a CTA.
 // Warps: 0 producer, 1 MMA and tensor memory, 2..5 rows of h (a thread a row), 6..13 epilogue.
+template <int CTAS>
 __global__ void __launch_bounds__(kWideThreads, 1)
 adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_b,
-                    const int* __restrict__ ids, const float* __restrict__ h, int parts, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
+                    const int* __restrict__ ids, const __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
                     int R, int n, const __grid_constant__ TcSlices slices, int f_tiles, int n_tiles, int BN, int stages) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   WideBars* bars = reinterpret_cast<WideBars*>(smem);
   unsigned char* h_tile = smem + kWideHead;
   unsigned char* stage0 = h_tile + kWideH;
-  const int stage_bytes = kAdTile + BN * 128;
+  const int w_bytes = BN / CTAS * 128, stage_bytes = kAdTile + w_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
   volatile int* stop = &bars->stop;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&bars->acc_full[b], 1); mbar_init(&bars->acc_empty[b], kWideEpilogueWarps); }
-    mbar_init(&bars->h_full, 4);
-    mbar_init(&bars->h_empty, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->acc_full[b], 1);
+      mbar_init(&bars->acc_empty[b], kWideEpilogueWarps * CTAS);
+      mbar_init(&bars->h_full[b], 4 * CTAS);
+      mbar_init(&bars->h_empty[b], 1);
+    }
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  __syncwarp();
+  if (warp == 1) tc_alloc<CTAS>(&bars->tmem_base, 512);
   tc_fence_before();
+  if (CTAS == 2) cluster_barrier();
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = bars->tmem_base;
   const int steps = (K + kAdK - 1) / kAdK;
   const int r_steps = (R + kAdK - 1) / kAdK;          // steps of up to 64 ranks an adapter
   const int r_here = min(R, kAdK);                    // ranks of one such step (R is 16, 32, 64 or 128)
-  TileIds tids;
+  // Rows of h lie 128 bytes apart.  Up to 32 ranks both parts fit into that, and there is room for two adapters' rows.
+  const int h_bufs = R <= 32 ? 2 : 1, lo_at = R <= 32 ? 64 : kAdTile;
+  TileIds<CTAS> tids;
 
   if (warp == 0) {
-    // ---- producer: x and W (the kernel before the first launch wrote x: complete, see chain_release_late there) ----------
+    // ---- producer: x and W (what wrote x is complete, see chain_release_late in the kernels that make h) ------------------
     int it = 0, issued = 0;
     bool ok = true;
-    for (int i = blockIdx.x; i < n_tiles && ok; i += gridDim.x) {
-      const WideTile w = wide_tile(i, f_tiles, BN, slices);
+    for (int i = first; i < n_tiles && ok; i += stride) {
+      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
+      const int x_row = w.row0 + rank * kAdM, w_row = w.f0 + rank * (BN / CTAS);
       if (lane == 0) {
         for (int ks = 0; ks < steps; ++ks, ++it) {
           const int s = it % stages;
           if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1, &g_adapter_tc_error)) { ok = false; break; }
           unsigned char* st = stage0 + (size_t)s * stage_bytes;
-          mbar_expect_tx(&bars->full[s], stage_bytes);
-          tma_load_2d(st, &map_x, ks * kAdK, w.row0, &bars->full[s]);
-          tma_load_2d(st + kAdTile, &map_w, ks * kAdK, w.f0, &bars->full[s]);
+          if (rank == 0) mbar_expect_tx(&bars->full[s], CTAS * stage_bytes);
+          tma_load<CTAS>(st, &map_x, ks * kAdK, x_row, &bars->full[s]);
+          tma_load<CTAS>(st + kAdTile, &map_w, ks * kAdK, w_row, &bars->full[s]);
           issued = it + 1;
         }
       }
@@ -294,31 +447,33 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             const int s = it % stages;
             if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1, &g_adapter_tc_error)) { ok = false; break; }
             unsigned char* st = stage0 + (size_t)s * stage_bytes;
-            mbar_expect_tx(&bars->full[s], BN * 128);
-            tma_load_2d(st + kAdTile, &map_b, rs * kAdK, a * N + w.f0, &bars->full[s]);
+            if (rank == 0) mbar_expect_tx(&bars->full[s], CTAS * w_bytes);
+            tma_load<CTAS>(st + kAdTile, &map_b, rs * kAdK, a * N + w_row, &bars->full[s]);
             issued = it + 1;
           }
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (!ok && lane == 0) {
+    // copies still on their way land in this CTA's shared memory (the even CTA's barriers count both CTAs' bytes)
+    if (!ok && lane == 0 && rank == 0) {
       for (int j = max(0, issued - stages); j < issued; ++j)
         for (unsigned i = 0; i < (1u << 20); ++i)
           if (mbar_try(&bars->full[j % stages], (j / stages) & 1)) break;
     }
-  } else if (warp == 1) {
+    __syncwarp();
+  } else if (warp == 1 && rank == 0) {
     // ---- MMA ----------------------------------------------------------------------------------------------------------------
     int it = 0, done = 0, ht = 0;
     bool ok = true;
-    const unsigned idesc = ad_instr_desc(BN);
-    for (int i = blockIdx.x; i < n_tiles && ok; i += gridDim.x, ++done) {
-      const WideTile w = wide_tile(i, f_tiles, BN, slices);
+    const unsigned idesc = ad_instr_desc(BN, kAdM * CTAS);
+    for (int i = first; i < n_tiles && ok; i += stride, ++done) {
+      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int ab = done & 1;
       const unsigned acc = tmem + ab * 256;
       if (lane == 0) {
-        if (!mbar_wait(&bars->acc_empty[ab], ((done >> 1) & 1) ^ 1, stop, 2, &g_adapter_tc_error)) ok = false;
+        if (!mbar_wait_cluster(&bars->acc_empty[ab], ((done >> 1) & 1) ^ 1, stop, 2)) ok = false;
         tc_fence_after();
         for (int ks = 0; ks < steps && ok; ++ks, ++it) {
           const int s = it % stages;
@@ -327,88 +482,78 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           unsigned char* st = stage0 + (size_t)s * stage_bytes;
           const unsigned long long da = smem_desc(st), db = smem_desc(st + kAdTile);
 #pragma unroll
-          for (int kk = 0; kk < kAdK / 16; ++kk) tc_mma(acc, da + 2 * kk, db + 2 * kk, idesc, ks > 0 || kk > 0 ? 1u : 0u);
-          tc_commit(&bars->empty[s]);
+          for (int kk = 0; kk < kAdK / 16; ++kk) mma<CTAS>(acc, da + 2 * kk, db + 2 * kk, idesc, ks > 0 || kk > 0 ? 1u : 0u);
+          commit<CTAS>(&bars->empty[s]);
         }
       }
       for (int a = tids.next(-1); a != kNone; a = tids.next(a)) {
         if (lane == 0 && ok) {
           for (int rs = 0; rs < r_steps; ++rs, ++it, ++ht) {
-            const int s = it % stages;
-            if (!mbar_wait(&bars->h_full, ht & 1, stop, 5, &g_adapter_tc_error) ||
+            const int s = it % stages, hb = ht % h_bufs;
+            if (!mbar_wait_cluster(&bars->h_full[hb], (ht / h_bufs) & 1, stop, 5) ||
                 !mbar_wait(&bars->full[s], (it / stages) & 1, stop, 3, &g_adapter_tc_error)) { ok = false; break; }
             tc_fence_after();
-            const unsigned long long hi = smem_desc(h_tile), lo = smem_desc(h_tile + kAdTile);
+            const unsigned long long hi = smem_desc(h_tile + hb * kAdTile), lo = hi + (lo_at >> 4);
             const unsigned long long db = smem_desc(stage0 + (size_t)s * stage_bytes + kAdTile);
             for (int kk = 0; kk < r_here / 16; ++kk) {
-              tc_mma(acc, hi + 2 * kk, db + 2 * kk, idesc, 1u);
-              tc_mma(acc, lo + 2 * kk, db + 2 * kk, idesc, 1u);
+              mma<CTAS>(acc, hi + 2 * kk, db + 2 * kk, idesc, 1u);
+              mma<CTAS>(acc, lo + 2 * kk, db + 2 * kk, idesc, 1u);
             }
-            tc_commit(&bars->empty[s]);
-            tc_commit(&bars->h_empty);
+            commit<CTAS>(&bars->empty[s]);
+            commit<CTAS>(&bars->h_empty[hb]);
           }
         }
       }
-      if (lane == 0 && ok) tc_commit(&bars->acc_full[ab]);
+      if (lane == 0 && ok) commit<CTAS>(&bars->acc_full[ab]);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-  } else if (warp < 6) {
-    // ---- rows of h: this thread's row of the tile, in the operand's swizzled image --------------------------------------------
+  } else if (warp >= 2 && warp < 6) {
+    // ---- rows of h: this thread's row of the tile, in the operand's swizzled image; zeros for another adapter ---------------
     chain_wait(h);
-    const int r = (warp - 2) * 32 + lane, SR = slices.n * R;
+    const int r = (warp - 2) * 32 + lane, SR = slices.n * R, n_pieces = r_here >> 3;
     int ht = 0;
     bool ok = true;
-    for (int i = blockIdx.x; i < n_tiles && ok; i += gridDim.x) {
-      const WideTile w = wide_tile(i, f_tiles, BN, slices);
+    for (int i = first; i < n_tiles && ok; i += stride) {
+      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
-      const int t = w.row0 + r;
+      const int t = w.row0 + rank * kAdM + r;
       const int own = t < rows ? ids[t] : -1;
       if (w.f0 == 0 && own >= n) atomicCAS(&g_adapter_tc_index, 0, t + 1);
       for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
         for (int rs = 0; rs < r_steps; ++rs, ++ht) {
-          if (!warp_wait(&bars->h_empty, (ht & 1) ^ 1, stop, 6)) { ok = false; break; }
-          const float* src = h + (size_t)t * SR + w.slice * R + rs * kAdK;
-          for (int j = 0; j < r_here / 8; ++j) {
-            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-            if (own == a) {
-              float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-              for (int p = 0; p < parts; ++p) {
-                float u[8];
-                load8(src + (size_t)p * rows * SR + 8 * j, u);
+          const int hb = ht % h_bufs;
+          uint4 hi[8], lo[8];
+          const uint4* src = reinterpret_cast<const uint4*>(h + (size_t)t * 2 * SR + w.slice * R + rs * kAdK);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += u[e];
-              }
-              __nv_bfloat162 a2[4], b2[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                a2[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                const float2 back = __bfloat1622float2(a2[e]);
-                // (of an infinity nothing is left)
-                b2[e] = __floats2bfloat162_rn(isinf(back.x) ? 0.f : v[2 * e] - back.x, isinf(back.y) ? 0.f : v[2 * e + 1] - back.y);
-              }
-              hi = *reinterpret_cast<uint4*>(a2);
-              lo = *reinterpret_cast<uint4*>(b2);
-            }
-            const int at = r * 128 + ((j ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4*>(h_tile + at) = hi;
-            *reinterpret_cast<uint4*>(h_tile + kAdTile + at) = lo;
+          for (int j = 0; j < 8; ++j) {
+            hi[j] = lo[j] = make_uint4(0, 0, 0, 0);
+            if (own == a && j < n_pieces) { hi[j] = src[j]; lo[j] = src[j + (SR >> 3)]; }
           }
+          if (!warp_wait(&bars->h_empty[hb], ((ht / h_bufs) & 1) ^ 1, stop, 6)) { ok = false; break; }
+          unsigned char* row = h_tile + hb * kAdTile + r * 128;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < n_pieces) {
+              *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) = hi[j];
+              if (h_bufs == 2) *reinterpret_cast<uint4*>(row + (((j + 4) ^ (r & 7)) << 4)) = lo[j];
+              else *reinterpret_cast<uint4*>(row + kAdTile + ((j ^ (r & 7)) << 4)) = lo[j];
+            }
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->h_full);
+          if (lane == 0) arrive_leader<CTAS>(&bars->h_full[hb]);
         }
       }
     }
-  } else {
+  } else if (warp >= 6) {
     // ---- epilogue: tensor-memory lanes 32 * (warp % 4) .. + 31, every other run of 32 columns --------------------------------
     const int quad = warp & 3, half = (warp - 6) >> 2;
     int done = 0;
-    for (int i = blockIdx.x; i < n_tiles; i += gridDim.x, ++done) {
-      const WideTile w = wide_tile(i, f_tiles, BN, slices);
+    for (int i = first; i < n_tiles; i += stride, ++done) {
+      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       const int ab = done & 1;
       if (!warp_wait(&bars->acc_full[ab], (done >> 1) & 1, stop, 4)) break;
       tc_fence_after();
-      const int t = w.row0 + quad * 32 + lane;
+      const int t = w.row0 + rank * kAdM + quad * 32 + lane;
       __nv_bfloat16* out = y + (size_t)t * N + w.f0;
       const bool whole = N % 8 == 0 && w.f0 % 8 == 0;
       for (int c0 = half * 32; c0 < BN; c0 += 64) {
@@ -420,7 +565,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (c0 + 64 >= BN) {                      // the last this warp reads of the accumulator
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+          if (lane == 0) arrive_leader<CTAS>(&bars->acc_empty[ab]);
         }
         if (c0 >= w.width || t >= rows) continue;
         if (whole && c0 + 32 <= w.width) {
@@ -439,11 +584,13 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   }
+  __syncwarp();
   tc_fence_before();
+  if (CTAS == 2) cluster_barrier();       // the even CTA's products read the odd one's shared memory
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    tc_dealloc<CTAS>(tmem, 512);
   }
 }
 
@@ -457,16 +604,10 @@ struct __align__(8) RowsBars {
   int stop;
 };
 
-__device__ __forceinline__ unsigned cluster_addr(unsigned local, int rank) {
-  unsigned remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-  return remote;
-}
-
 // grid: (members of the cluster, feature tiles).  192 threads: producer, MMA, four epilogue warps (a thread a feature).
 __global__ void __launch_bounds__(192)
 adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const int* __restrict__ ids,
-                    const float* __restrict__ h, int parts, const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows,
+                    const float* __restrict__ h, const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows,
                     int N, int K, int R, int n, const __grid_constant__ TcSlices slices, int NT, int stages) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -482,23 +623,21 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(64) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  __syncwarp();
+  if (warp == 1) tc_alloc<1>(&bars->tmem_base, 64);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = bars->tmem_base;
-  const WideTile w = wide_tile(blockIdx.y, gridDim.y, kAdM, slices);
+  const WideTile w = wide_tile(blockIdx.y, gridDim.y, kAdM, kAdM, slices);
   const int steps = (K + kAdK - 1) / kAdK;
   const int k_first = (int)((long long)member * steps / members), k_last = (int)((long long)(member + 1) * steps / members);
   float* sums = reinterpret_cast<float*>(stage0);              // [NT][128], in the stages once they are read
-  bool fine = true;
 
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0;
+      bool fine = true;
       for (int it = 0; it < k_last - k_first; ++it) {
         const int s = it % stages;
         if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 11, &g_adapter_tc_error)) { fine = false; break; }
@@ -513,10 +652,10 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           for (unsigned i = 0; i < (1u << 20); ++i)
             if (mbar_try(&bars->full[j % stages], (j / stages) & 1)) break;
     }
-    __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const unsigned idesc = ad_instr_desc(NT);
+      const unsigned idesc = ad_instr_desc(NT, kAdM);
+      bool fine = true;
       for (int it = 0; it < k_last - k_first; ++it) {
         const int s = it % stages;
         if (!mbar_wait(&bars->full[s], (it / stages) & 1, stop, 13, &g_adapter_tc_error)) { fine = false; break; }
@@ -529,7 +668,6 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
       if (fine) tc_commit(&bars->acc_full);
     }
-    __syncwarp();
   } else {
     const int quad = warp & 3;
     if (warp_wait(&bars->acc_full, 0, stop, 14)) {
@@ -544,50 +682,65 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
     tc_fence_before();
   }
-  // the members' sums are all there
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncwarp();
+  cluster_barrier();                   // the members' sums are all there
   if (warp >= 2) {
     const int d = (warp & 3) * 32 + lane, f = w.f0 + d, SR = slices.n * R;
     const int t_first = (int)((long long)member * rows / members), t_last = (int)((long long)(member + 1) * rows / members);
     const unsigned local = smem_u32(sums + d);
     chain_wait(h);
-    for (int t = t_first; t < t_last; ++t) {
-      float sum = 0.f;
-      for (int m = 0; m < members; ++m) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(local + t * kAdM * 4, m)) : "memory");
-        sum += v;
-      }
-      const int a = ids[t];
-      if (a >= n && blockIdx.y == 0 && d == 0) atomicCAS(&g_adapter_tc_index, 0, t + 1);
-      if (a >= 0 && a < n && d < w.width) {
-        const __nv_bfloat16* b = B + ((size_t)a * N + f) * R;
-        const float* hr = h + (size_t)t * SR + w.slice * R;
-        for (int j = 0; j < R; j += 8) {
-          float bv[8], hv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          load8(b + j, bv);
-          for (int p = 0; p < parts; ++p) {
-            float u[8];
-            load8(hr + (size_t)p * rows * SR + j, u);
+    constexpr int U = 4;               // rows of x at a time
+    for (int t0 = t_first; t0 < t_last; t0 += U) {
+      float sum[U];
+      int a[U];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) hv[e] += u[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum = fmaf(hv[e], bv[e], sum);
+      for (int i = 0; i < U; ++i) {
+        const int t = min(t0 + i, t_last - 1);
+        a[i] = ids[t];
+        if (a[i] >= n && blockIdx.y == 0 && d == 0) atomicCAS(&g_adapter_tc_index, 0, t + 1);
+        if (a[i] >= n || d >= w.width) a[i] = -1;
+        sum[i] = 0.f;
+        for (int m = 0; m < members; ++m) {
+          float v;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(local + t * kAdM * 4, m)));
+          sum[i] += v;
         }
       }
-      if (d < w.width) y[(size_t)t * N + f] = __float2bfloat16_rn(sum);
+      for (int j = 0; j < R; j += 16) {
+        uint4 raw[U][2];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          if (a[i] >= 0) {
+            const uint4* b = reinterpret_cast<const uint4*>(B + ((size_t)a[i] * N + f) * R + j);
+            raw[i][0] = b[0];
+            raw[i][1] = b[1];
+          }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          if (a[i] >= 0) {
+            const float* hr = h + (size_t)min(t0 + i, t_last - 1) * SR + w.slice * R + j;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float bv[8], hv[8];
+              unpack8(raw[i][c], bv);
+              load8(hr + 8 * c, hv);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) sum[i] = fmaf(hv[e], bv[e], sum[i]);
+            }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (t0 + i < t_last && d < w.width) y[(size_t)(t0 + i) * N + f] = __float2bfloat16_rn(sum[i]);
     }
   }
-  // nobody reads another's shared memory any more
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncwarp();
+  cluster_barrier();                   // nobody reads another's shared memory any more
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(64) : "memory");
+    tc_dealloc<1>(tmem, 64);
   }
 }
 
@@ -629,19 +782,20 @@ int adapter_shrink_simt(const void* x, const void* A, const float* scale, const 
 
 using namespace nf;
 
-// Parts of k that the first product of `rows` rows is cut into: h takes parts * rows * n_slices * R floats.
-extern "C" int nf_adapter_parts(int rows, int K) {
-  const int tiles = (rows + kAdM - 1) / kAdM, steps = (K + kAdK - 1) / kAdK;
-  if (rows <= 16) return 1;
+static int shrink_members(int rows, int K, int SR) {
+  const int tiles = ((rows + kAdM - 1) / kAdM) * (SR > kShrinkCols ? (SR + kAdM - 1) / kAdM : 1), steps = (K + kAdK - 1) / kAdK;
   int p = 1;
   while (p < 8 && 2 * p * tiles <= sm_count() && steps >= 4 * p) p *= 2;
   return p;
 }
 
+// Floats of scratch that `rows` rows take for every number of h (n_slices * R a row).
+extern "C" int nf_adapter_parts(int rows, int K, int SR) { return rows <= 16 ? 1 : 1 + shrink_members(rows, K, SR); }
+
 // y = x W^T + the adapters' part (see the head of this file): x [rows, K], W [N, K], A [n, n_slices * R, K], B [n, N, R], y
-// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h float32 [nf_adapter_parts(rows, K), rows, n_slices * R].  ends: the
-// n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or 128, bases
-// 16-byte aligned.
+// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h float32 [nf_adapter_parts(rows, K, n_slices * R), rows, n_slices * R]
+// of scratch.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or
+// 128, bases 16-byte aligned.
 extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h,
                                  void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;
@@ -658,26 +812,35 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     NF_REQUIRE(ends[i] > (i ? ends[i - 1] : 0), "adapter_linear: slice %d ends at %d", i, ends[i]);
   }
   NF_REQUIRE(ends[n_slices - 1] == N, "adapter_linear: the slices end at %d of %d features", ends[n_slices - 1], N);
-  const int SR = n_slices * R, parts = nf_adapter_parts(rows, K), steps = (K + kAdK - 1) / kAdK;
+  const int SR = n_slices * R, steps = (K + kAdK - 1) / kAdK;
+  const int row_tiles = (rows + kAdM - 1) / kAdM;
 
   // ---- h
   if (rows <= 16) {
     if (int rc = adapter_shrink_simt(x, A, scale, ids, h, rows, K, SR, n, stream)) return rc;
   } else {
-    const int tiles = (rows + kAdM - 1) / kAdM, j_tiles = (SR + kAdM - 1) / kAdM;
-    const int NT = rows >= kAdM ? kAdM : (rows + 15) & ~15, a_box = SR < kAdM ? SR : kAdM;
+    const int members = shrink_members(rows, K, SR);
+    const int JW = SR > kShrinkCols ? kAdM : SR, j_tiles = (SR + JW - 1) / JW;
+    const int most = n < kAdM ? (n < rows ? n : rows) : (rows < kAdM ? rows : kAdM);      // adapters that a tile's rows may have
+    const int group = kShrinkCols / JW < most ? kShrinkCols / JW : most;
+    const int x_box = rows >= kAdM ? kAdM : (rows + 7) & ~7;
     CUtensorMap ma, mx;
-    if (int rc = make_map(&ma, A, (long long)n * SR, K, a_box)) return rc;
-    if (int rc = make_map(&mx, x, rows, K, NT)) return rc;
-    const int stage = kAdTile + NT * 128, stages = 6;
-    const size_t smem = 2048 + (size_t)stages * stage;
-    static int asked = room_for(adapter_shrink_tc_kernel, 2048 + 6 * (size_t)(2 * kAdTile));
+    if (int rc = make_map(&ma, A, (long long)n * SR, K, JW)) return rc;
+    if (int rc = make_map(&mx, x, rows, K, x_box)) return rc;
+    const int stage = kAdTile + group * JW * 128, here = (steps + members - 1) / members;
+    int stages = (200 * 1024) / stage;
+    stages = stages > 8 ? 8 : stages;
+    stages = stages > here && group >= most ? here : stages;
+    size_t smem = 2048 + (size_t)stages * stage;
+    smem = smem < kShrinkSmemLeast ? kShrinkSmemLeast : smem;
+    static int asked = room_for(adapter_shrink_tc_kernel, 204 * 1024);
     if (asked) return asked;
-    int turns = sm_count() / (parts * tiles * j_tiles);          // CTAs that take a tile's adapters in turn
-    const int most = n < NT ? n : NT;
-    turns = turns < 1 ? 1 : turns > most ? most : turns;
-    launch_chained(adapter_shrink_tc_kernel, dim3(parts, tiles * j_tiles, turns), dim3(192), smem, stream, ma, mx, scale, ids, h, rows, K, SR,
-                   n, tiles, NT, a_box, stages);
+    const int passes = (most + group - 1) / group;
+    int turns = sm_count() / (members * row_tiles * j_tiles);          // CTAs that take a tile's groups of adapters in turn
+    turns = turns < 1 ? 1 : turns > passes ? passes : turns;
+    NF_REQUIRE(row_tiles * j_tiles <= 65535, "adapter_linear: %d rows are too many", rows);
+    launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, row_tiles * j_tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
+                           ids, h + (size_t)rows * SR, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, rows > kRowsMost ? 1 : 0);
     if (int rc = check_launch("adapter_shrink")) return rc;
   }
 
@@ -698,33 +861,41 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     static int asked = room_for(adapter_rows_kernel, 108 * 1024);
     if (asked) return asked;
     NF_REQUIRE(tiles <= 65535, "adapter_linear: %d features are too many", N);
-    launch_chained_cluster(adapter_rows_kernel, dim3(members, tiles), dim3(192), smem, stream, members, mw, mx, ids, (const float*)h, parts,
+    launch_chained_cluster(adapter_rows_kernel, dim3(members, tiles), dim3(192), smem, stream, members, mw, mx, ids, (const float*)h,
                            (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows, N, K, R, n, sl, NT, stages);
     return check_launch("adapter_rows");
   }
-  // The width of a tile: the one whose rounds of tiles take the least, a round's time being that of its widest operand.
-  const int m_tiles = (rows + kAdM - 1) / kAdM;
-  int BN = 256;
+  // The tile: the one whose rounds take the least, a round's time being that of the products or of the operands' way into
+  // shared memory (64 bytes a cycle), whichever is the longer.
+  int BN = 256, ctas = 2;
   long long best = -1;
-  for (int c = 256; c >= 64; c -= 32) {
-    const long long tiles = (long long)m_tiles * feature_tiles(sl, c);
-    const long long cost = ((tiles + sm_count() - 1) / sm_count()) * (c > 112 ? c : 112);
-    if (best < 0 || cost < best) { best = cost; BN = c; }
+  for (int g = 2; g >= 1; --g) {
+    const int m_tiles = (rows + kAdM * g - 1) / (kAdM * g), at_once = sm_count() / g;
+    for (int c = 256; c >= 64; c -= 64) {
+      const long long tiles = (long long)m_tiles * feature_tiles(sl, c);
+      const int loads = (kAdTile + c / g * 128) / 64, step = 2 * c > loads ? 2 * c : loads;
+      const long long cost = ((tiles + at_once - 1) / at_once) * step;
+      if (best < 0 || cost < best) { best = cost; BN = c; ctas = g; }
+    }
   }
   CUtensorMap mb;
   if (int rc = make_map(&mx, x, rows, K, kAdM)) return rc;
-  if (int rc = make_map(&mw, W, N, K, BN)) return rc;
-  if (int rc = make_map(&mb, B, (long long)n * N, R, BN)) return rc;
+  if (int rc = make_map(&mw, W, N, K, BN / ctas)) return rc;
+  if (int rc = make_map(&mb, B, (long long)n * N, R, BN / ctas)) return rc;
   const int f_tiles = feature_tiles(sl, BN);
-  const long long n_tiles = (long long)f_tiles * m_tiles;
-  NF_REQUIRE(n_tiles < (1ll << 31), "adapter_linear: %d rows of %d features are too many", rows, N);
-  int stages = (kWideSmem - kWideHead - kWideH) / (kAdTile + BN * 128);
+  const long long n_tiles = (long long)f_tiles * ((rows + kAdM * ctas - 1) / (kAdM * ctas));
+  NF_REQUIRE(n_tiles < (1ll << 30), "adapter_linear: %d rows of %d features are too many", rows, N);
+  int stages = (kWideSmem - kWideHead - kWideH) / (kAdTile + BN / ctas * 128);
   stages = stages > kAdMaxStages ? kAdMaxStages : stages;
-  static int asked = room_for(adapter_wide_kernel, kWideSmem + 1024);
-  if (asked) return asked;
-  const int grid = n_tiles < sm_count() ? (int)n_tiles : sm_count();
-  launch_chained(adapter_wide_kernel, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, mx, mw, mb, ids, (const float*)h, parts,
-                 (__nv_bfloat16*)y, rows, N, K, R, n, sl, f_tiles, (int)n_tiles, BN, stages);
+  static int asked1 = room_for(adapter_wide_kernel<1>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2>, kWideSmem + 1024);
+  if (asked1 || asked2) return 1;
+  const int at_once = sm_count() / ctas, grid = ctas * (n_tiles < at_once ? (int)n_tiles : at_once);
+  if (ctas == 2)
+    launch_chained_cluster(adapter_wide_kernel<2>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, 2, mx, mw, mb, ids,
+                           (const __nv_bfloat16*)h, (__nv_bfloat16*)y, rows, N, K, R, n, sl, f_tiles, (int)n_tiles, BN, stages);
+  else
+    launch_chained(adapter_wide_kernel<1>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, mx, mw, mb, ids,
+                   (const __nv_bfloat16*)h, (__nv_bfloat16*)y, rows, N, K, R, n, sl, f_tiles, (int)n_tiles, BN, stages);
   return check_launch("adapter_wide");
 }
 
