@@ -31,6 +31,14 @@ constexpr int kNone = 0x7fffffff;
 __device__ int g_adapter_tc_error = 0;               // code of the first wait that was given up on
 __device__ int g_adapter_tc_index = 0;               // 1 + a row whose adapter lies outside the pool
 
+// One lane of a whole warp, the same one every time.  The warps that issue products run their loops as a whole and elect a lane
+// for each step: behind a condition on the lane number, which the compiler does not know to leave a single thread, a step's four
+// products took 800 cycles however small they were.
+__device__ __forceinline__ bool elect_one() {
+  unsigned is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
+}
 // A wait of a whole warp: all of its lanes go on, or none does.
 __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile int* stop, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, code, &g_adapter_tc_error));
@@ -106,15 +114,15 @@ __device__ __forceinline__ void arrive_leader(void* bar) {
   if (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(smem_u32(bar), 0)) : "memory");
   else mbar_arrive(bar);
 }
-// mbar_wait for arrivals that may come from the other CTA of the cluster.
-__device__ __forceinline__ bool mbar_wait_cluster(void* bar, unsigned parity, volatile int* stop, int code) {
+// warp_wait for arrivals that may come from the other CTA of the cluster.
+__device__ __forceinline__ bool warp_wait_cluster(void* bar, unsigned parity, volatile int* stop, int code) {
   for (unsigned i = 0; i < kPollLimit; ++i) {
     unsigned ok;
     asm volatile(
         "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (ok) return true;
-    if ((i & 1023u) == 1023u && *stop) return false;
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if ((i & 1023u) == 1023u && __any_sync(0xffffffffu, *stop)) return false;
   }
   *stop = 1;
   atomicCAS(&g_adapter_tc_error, 0, code);
@@ -140,6 +148,15 @@ struct TileIds {
 #pragma unroll
     for (int i = 0; i < 4 * CTAS; ++i) m = v[i] > last ? min(m, v[i]) : m;
     return __reduce_min_sync(0xffffffffu, m);
+  }
+};
+
+// The stage of a ring and the parity of its present use, step after step (no division by the number of stages).
+struct Ring {
+  int s = 0;
+  unsigned phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) { s = 0; phase ^= 1; }
   }
 };
 
@@ -180,21 +197,23 @@ __device__ __forceinline__ void put_h(float* h, int t, int SR, int j, const floa
 }
 
 // D[t, (adapter, j)] over a tile of up to 128 rows: x is the 128-row operand, the rows of A of up to `group` of the adapters
-// that occur in the tile the other, so that x is read once for all of them.  The CTAs of a cluster split k; each leaves every
-// row's own numbers in `part` [members, rows, SR], and after the cluster's barrier adds up, scales and writes a share of rows.
+// that occur in the tile the other, so that x is read once for all of them.  The CTAs of a cluster split k; each sends every row's
+// own numbers to the member that owns the row, which adds them up in the members' order, scales and writes them.
 // 192 threads: producer, MMA, four epilogue warps (a thread a row).  grid: (members, row tiles * j tiles, groups in turn).
 __global__ void __launch_bounds__(192, 1)
 adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ scale,
-                         const int* __restrict__ ids, float* part, float* h, int rows, int K, int SR, int n, int row_tiles, int x_box, int JW,
+                         const int* __restrict__ ids, float* __restrict__ h, int rows, int K, int SR, int n, int row_tiles, int x_box, int JW,
                          int group, int stages, int split) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   ShrinkBars* bars = reinterpret_cast<ShrinkBars*>(smem);
   unsigned char* stage0 = smem + 1024;
   const int stage_bytes = kAdTile + group * JW * 128;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int members = gridDim.x, member = blockIdx.x;
+  float* sums = reinterpret_cast<float*>(stage0 + (size_t)stages * stage_bytes);      // [members][share of rows][JW], written by all members
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int members = gridDim.x, member = blockIdx.x, share = kAdM / members;          // (a power of two up to 8)
   volatile int* stop = &bars->stop;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this member is there
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
     mbar_init(&bars->acc_full, 1);
@@ -232,15 +251,16 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   };
 
   if (warp == 0) {
-    int it = 0, issued = 0, mine = 0;
+    int issued = 0, mine = 0;
     bool ok = true;
+    Ring ring;
     for (int turn = 0;; ++turn) {
       const int count = next_group(mine);
       if (!count || !ok) break;
       if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
-      for (int ks = k_first; ks < k_last; ++ks, ++it) {
-        const int s = it % stages;
-        if (!warp_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1)) { ok = false; break; }
+      for (int ks = k_first; ks < k_last; ++ks, ring.next(stages), ++issued) {
+        const int s = ring.s;
+        if (!warp_wait(&bars->empty[s], ring.phase ^ 1, stop, 1)) { ok = false; break; }
         unsigned char* st = stage0 + (size_t)s * stage_bytes;
         if (lane == 0) {
           mbar_expect_tx(&bars->full[s], x_box * 128 + count * JW * 128);
@@ -248,7 +268,6 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         __syncwarp();
         if (lane < count) tma_load_2d(st + kAdTile + lane * JW * 128, &map_a, ks * kAdK, mine * SR + j0, &bars->full[s]);
-        issued = it + 1;
       }
     }
     if (!ok && lane == 0) {
@@ -258,37 +277,38 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     }
     __syncwarp();
   } else if (warp == 1) {
-    int it = 0, done = 0, mine = 0;
+    int done = 0, mine = 0;
     bool ok = true;
+    Ring ring;
     for (int turn = 0;; ++turn) {
       const int count = next_group(mine);
       if (!count || !ok) break;
       if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
-      if (lane == 0) {
-        const unsigned idesc = ad_instr_desc(count * JW, kAdM);
-        if (!mbar_wait(&bars->acc_empty, (done & 1) ^ 1, stop, 2, &g_adapter_tc_error)) ok = false;
+      const unsigned idesc = ad_instr_desc(count * JW, kAdM);
+      if (!warp_wait(&bars->acc_empty, (done & 1) ^ 1, stop, 2)) break;
+      tc_fence_after();
+      for (int ks = k_first; ks < k_last; ++ks) {
+        if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
         tc_fence_after();
-        for (int ks = k_first; ks < k_last && ok; ++ks, ++it) {
-          const int s = it % stages;
-          if (!mbar_wait(&bars->full[s], (it / stages) & 1, stop, 3, &g_adapter_tc_error)) { ok = false; break; }
-          tc_fence_after();
-          unsigned char* st = stage0 + (size_t)s * stage_bytes;
-          const unsigned long long dx = smem_desc(st), da = smem_desc(st + kAdTile);
+        unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+        const unsigned long long dx = smem_desc(st), da = smem_desc(st + kAdTile);
+        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kAdK / 16; ++kk)
-            tc_mma(tmem, dx + 2 * kk, da + 2 * kk, idesc, ks > k_first || kk > 0 ? 1u : 0u);
-          tc_commit(&bars->empty[s]);
+          for (int kk = 0; kk < kAdK / 16; ++kk) tc_mma(tmem, dx + 2 * kk, da + 2 * kk, idesc, ks > k_first || kk > 0 ? 1u : 0u);
+          tc_commit(&bars->empty[ring.s]);
+          if (ks + 1 == k_last) tc_commit(&bars->acc_full);
         }
-        if (ok) tc_commit(&bars->acc_full);
+        __syncwarp();
+        ring.next(stages);
       }
       ++done;
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
   } else {
     const int quad = warp & 3, r = quad * 32 + lane, t = row0 + r;
     const int own = t < rows ? ids[t] : -1;
     int done = 0, mine = 0;
-    float* to = part + ((size_t)member * rows + t) * SR + j0;
+    const unsigned to = cluster_addr(smem_u32(sums + ((size_t)member * share + r % share) * JW), r / share);
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // every member is there: its shared memory may be written
     for (int turn = 0;; ++turn) {
       const int count = next_group(mine);
       if (!count) break;
@@ -307,8 +327,8 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
           if (is) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(to + c + e) = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]),
-                                                                   __uint_as_float(v[e + 3]));
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c + e) * 4), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]),
+                           "r"(v[e + 3]) : "memory");
           }
         }
         if (is) bars->served[r] = 1;
@@ -320,22 +340,23 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     }
   }
   __syncwarp();
+  if (warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   cluster_barrier();                  // every member's part is there
-  const int r_first = member * kAdM / members, r_count = (member + 1) * kAdM / members - r_first, pieces = jn >> 3;
-  for (int i = threadIdx.x; i < r_count * pieces; i += blockDim.x) {
-    const int r = r_first + i / pieces, j = j0 + (i % pieces) * 8, t = row0 + r;
+  const int pieces = jn >> 3;
+  for (int i = threadIdx.x; i < share * pieces; i += blockDim.x) {
+    const int rl = i / pieces, r = member * share + rl, j = (i - rl * pieces) * 8, t = row0 + r;
     if (!bars->served[r]) continue;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int m = 0; m < members; ++m) {
-      const float4* p = reinterpret_cast<const float4*>(part + ((size_t)m * rows + t) * SR + j);
-      const float4 a = __ldcg(p), b = __ldcg(p + 1);
-      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      float u[8];
+      load8(sums + ((size_t)m * share + rl) * JW + j, u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += u[e];
     }
     const float sc = scale[ids[t]];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= sc;
-    put_h(h, t, SR, j, v, split != 0);
+    put_h(h, t, SR, j0 + j, v, split != 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -348,14 +369,15 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 // ---- many rows -------------------------------------------------------------------------------------------------------------
 
 struct __align__(8) WideBars {
-  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full[2], h_empty[2];
+  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full[4], h_empty[4];
   unsigned tmem_base;
   int stop;
 };
 
 constexpr int kWideEpilogueWarps = 8;
 constexpr int kWideThreads = 32 * (2 + 4 + kWideEpilogueWarps);
-constexpr int kWideHead = 1024, kWideH = 2 * kAdTile;      // barriers; rows of h
+constexpr int kWideHead = 1024;                            // barriers
+constexpr int wide_h_bytes(int ctas) { return 2 * ctas * kAdTile; }      // rows of h
 constexpr int kWideSmem = 225 * 1024;
 
 struct WideTile {
@@ -392,9 +414,9 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   WideBars* bars = reinterpret_cast<WideBars*>(smem);
   unsigned char* h_tile = smem + kWideHead;
-  unsigned char* stage0 = h_tile + kWideH;
+  unsigned char* stage0 = h_tile + wide_h_bytes(CTAS);
   const int w_bytes = BN / CTAS * 128, stage_bytes = kAdTile + w_bytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
   volatile int* stop = &bars->stop;
   if (threadIdx.x == 0) {
@@ -402,9 +424,8 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->acc_full[b], 1);
       mbar_init(&bars->acc_empty[b], kWideEpilogueWarps * CTAS);
-      mbar_init(&bars->h_full[b], 4 * CTAS);
-      mbar_init(&bars->h_empty[b], 1);
     }
+    for (int b = 0; b < 4; ++b) { mbar_init(&bars->h_full[b], 4 * CTAS); mbar_init(&bars->h_empty[b], 1); }
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -418,42 +439,41 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int steps = (K + kAdK - 1) / kAdK;
   const int r_steps = (R + kAdK - 1) / kAdK;          // steps of up to 64 ranks an adapter
   const int r_here = min(R, kAdK);                    // ranks of one such step (R is 16, 32, 64 or 128)
-  // Rows of h lie 128 bytes apart.  Up to 32 ranks both parts fit into that, and there is room for two adapters' rows.
-  const int h_bufs = R <= 32 ? 2 : 1, lo_at = R <= 32 ? 64 : kAdTile;
+  // Rows of h lie 128 bytes apart; up to 32 ranks both parts fit into that.  Several adapters' rows are under way at a time: from
+  // one thread's store to the issuer and back is longer than the products take.
+  const int h_bufs = R <= 32 ? 2 * CTAS : CTAS, lo_at = R <= 32 ? 64 : kAdTile, h_bytes = R <= 32 ? kAdTile : 2 * kAdTile;
   TileIds<CTAS> tids;
 
   if (warp == 0) {
     // ---- producer: x and W (what wrote x is complete, see chain_release_late in the kernels that make h) ------------------
-    int it = 0, issued = 0;
+    int issued = 0;
     bool ok = true;
+    Ring ring;
     for (int i = first; i < n_tiles && ok; i += stride) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int x_row = w.row0 + rank * kAdM, w_row = w.f0 + rank * (BN / CTAS);
-      if (lane == 0) {
-        for (int ks = 0; ks < steps; ++ks, ++it) {
-          const int s = it % stages;
-          if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1, &g_adapter_tc_error)) { ok = false; break; }
-          unsigned char* st = stage0 + (size_t)s * stage_bytes;
-          if (rank == 0) mbar_expect_tx(&bars->full[s], CTAS * stage_bytes);
-          tma_load<CTAS>(st, &map_x, ks * kAdK, x_row, &bars->full[s]);
-          tma_load<CTAS>(st + kAdTile, &map_w, ks * kAdK, w_row, &bars->full[s]);
-          issued = it + 1;
+      for (int ks = 0; ks < steps; ++ks, ++issued, ring.next(stages)) {
+        if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 1)) { ok = false; break; }
+        unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(&bars->full[ring.s], CTAS * stage_bytes);
+          tma_load<CTAS>(st, &map_x, ks * kAdK, x_row, &bars->full[ring.s]);
+          tma_load<CTAS>(st + kAdTile, &map_w, ks * kAdK, w_row, &bars->full[ring.s]);
         }
+        __syncwarp();
       }
-      for (int a = tids.next(-1); a != kNone; a = tids.next(a)) {
-        if (lane == 0 && ok) {
-          for (int rs = 0; rs < r_steps; ++rs, ++it) {
-            const int s = it % stages;
-            if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 1, &g_adapter_tc_error)) { ok = false; break; }
-            unsigned char* st = stage0 + (size_t)s * stage_bytes;
-            if (rank == 0) mbar_expect_tx(&bars->full[s], CTAS * w_bytes);
-            tma_load<CTAS>(st + kAdTile, &map_b, rs * kAdK, a * N + w_row, &bars->full[s]);
-            issued = it + 1;
+      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
+        for (int rs = 0; rs < r_steps; ++rs, ++issued, ring.next(stages)) {
+          if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 1)) { ok = false; break; }
+          unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+          if (elect_one()) {
+            if (rank == 0) mbar_expect_tx(&bars->full[ring.s], CTAS * w_bytes);
+            tma_load<CTAS>(st + kAdTile, &map_b, rs * kAdK, a * N + w_row, &bars->full[ring.s]);
           }
+          __syncwarp();
         }
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
     // copies still on their way land in this CTA's shared memory (the even CTA's barriers count both CTAs' bytes)
     if (!ok && lane == 0 && rank == 0) {
@@ -464,79 +484,88 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     __syncwarp();
   } else if (warp == 1 && rank == 0) {
     // ---- MMA ----------------------------------------------------------------------------------------------------------------
-    int it = 0, done = 0, ht = 0;
+    int done = 0;
     bool ok = true;
+    Ring ring, hring;
     const unsigned idesc = ad_instr_desc(BN, kAdM * CTAS);
     for (int i = first; i < n_tiles && ok; i += stride, ++done) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int ab = done & 1;
       const unsigned acc = tmem + ab * 256;
-      if (lane == 0) {
-        if (!mbar_wait_cluster(&bars->acc_empty[ab], ((done >> 1) & 1) ^ 1, stop, 2)) ok = false;
+      if (!warp_wait_cluster(&bars->acc_empty[ab], ((done >> 1) & 1) ^ 1, stop, 2)) break;
+      tc_fence_after();
+      for (int ks = 0; ks < steps; ++ks, ring.next(stages)) {
+        if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
         tc_fence_after();
-        for (int ks = 0; ks < steps && ok; ++ks, ++it) {
-          const int s = it % stages;
-          if (!mbar_wait(&bars->full[s], (it / stages) & 1, stop, 3, &g_adapter_tc_error)) { ok = false; break; }
-          tc_fence_after();
-          unsigned char* st = stage0 + (size_t)s * stage_bytes;
-          const unsigned long long da = smem_desc(st), db = smem_desc(st + kAdTile);
+        unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+        const unsigned long long da = smem_desc(st), db = smem_desc(st + kAdTile);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kAdK / 16; ++kk) mma<CTAS>(acc, da + 2 * kk, db + 2 * kk, idesc, ks > 0 || kk > 0 ? 1u : 0u);
-          commit<CTAS>(&bars->empty[s]);
+          commit<CTAS>(&bars->empty[ring.s]);
         }
+        __syncwarp();
       }
-      for (int a = tids.next(-1); a != kNone; a = tids.next(a)) {
-        if (lane == 0 && ok) {
-          for (int rs = 0; rs < r_steps; ++rs, ++it, ++ht) {
-            const int s = it % stages, hb = ht % h_bufs;
-            if (!mbar_wait_cluster(&bars->h_full[hb], (ht / h_bufs) & 1, stop, 5) ||
-                !mbar_wait(&bars->full[s], (it / stages) & 1, stop, 3, &g_adapter_tc_error)) { ok = false; break; }
-            tc_fence_after();
-            const unsigned long long hi = smem_desc(h_tile + hb * kAdTile), lo = hi + (lo_at >> 4);
-            const unsigned long long db = smem_desc(stage0 + (size_t)s * stage_bytes + kAdTile);
+      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
+        for (int rs = 0; rs < r_steps; ++rs, ring.next(stages), hring.next(h_bufs)) {
+          if (!warp_wait_cluster(&bars->h_full[hring.s], hring.phase, stop, 5) ||
+              !warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
+          tc_fence_after();
+          const unsigned long long hi = smem_desc(h_tile + hring.s * h_bytes), lo = hi + (lo_at >> 4);
+          const unsigned long long db = smem_desc(stage0 + (size_t)ring.s * stage_bytes + kAdTile);
+          if (elect_one()) {
             for (int kk = 0; kk < r_here / 16; ++kk) {
               mma<CTAS>(acc, hi + 2 * kk, db + 2 * kk, idesc, 1u);
               mma<CTAS>(acc, lo + 2 * kk, db + 2 * kk, idesc, 1u);
             }
-            commit<CTAS>(&bars->empty[s]);
-            commit<CTAS>(&bars->h_empty[hb]);
+            commit<CTAS>(&bars->empty[ring.s]);
+            commit<CTAS>(&bars->h_empty[hring.s]);
           }
+          __syncwarp();
         }
       }
-      if (lane == 0 && ok) commit<CTAS>(&bars->acc_full[ab]);
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (ok && elect_one()) commit<CTAS>(&bars->acc_full[ab]);
+      __syncwarp();
     }
   } else if (warp >= 2 && warp < 6) {
     // ---- rows of h: this thread's row of the tile, in the operand's swizzled image; zeros for another adapter ---------------
     chain_wait(h);
     const int r = (warp - 2) * 32 + lane, SR = slices.n * R, n_pieces = r_here >> 3;
-    int ht = 0;
     bool ok = true;
+    Ring hring;
     for (int i = first; i < n_tiles && ok; i += stride) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int t = w.row0 + rank * kAdM + r;
       const int own = t < rows ? ids[t] : -1;
       if (w.f0 == 0 && own >= n) atomicCAS(&g_adapter_tc_index, 0, t + 1);
-      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
-        for (int rs = 0; rs < r_steps; ++rs, ++ht) {
-          const int hb = ht % h_bufs;
-          uint4 hi[8], lo[8];
-          const uint4* src = reinterpret_cast<const uint4*>(h + (size_t)t * 2 * SR + w.slice * R + rs * kAdK);
+      const bool has = own >= 0 && own < n;
+      uint4 hi[8], lo[8];                       // this row's numbers, read once a tile (beyond 64 ranks: a step)
+      auto read = [&](int rs) {
+        const uint4* src = reinterpret_cast<const uint4*>(h + (size_t)t * 2 * SR + w.slice * R + rs * kAdK);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            hi[j] = lo[j] = make_uint4(0, 0, 0, 0);
-            if (own == a && j < n_pieces) { hi[j] = src[j]; lo[j] = src[j + (SR >> 3)]; }
-          }
-          if (!warp_wait(&bars->h_empty[hb], ((ht / h_bufs) & 1) ^ 1, stop, 6)) { ok = false; break; }
-          unsigned char* row = h_tile + hb * kAdTile + r * 128;
+        for (int j = 0; j < 8; ++j) {
+          hi[j] = lo[j] = make_uint4(0, 0, 0, 0);
+          if (has && j < n_pieces) { hi[j] = src[j]; lo[j] = src[j + (SR >> 3)]; }
+        }
+      };
+      read(0);
+      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
+        const unsigned keep = own == a ? 0xffffffffu : 0u;
+        for (int rs = 0; rs < r_steps; ++rs, hring.next(h_bufs)) {
+          const int hb = hring.s;
+          if (rs > 0 && own == a) read(rs);
+          if (!warp_wait(&bars->h_empty[hb], hring.phase ^ 1, stop, 6)) { ok = false; break; }
+          unsigned char* row = h_tile + hb * h_bytes + r * 128;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (j < n_pieces) {
-              *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) = hi[j];
-              if (h_bufs == 2) *reinterpret_cast<uint4*>(row + (((j + 4) ^ (r & 7)) << 4)) = lo[j];
-              else *reinterpret_cast<uint4*>(row + kAdTile + ((j ^ (r & 7)) << 4)) = lo[j];
+              const uint4 u = make_uint4(hi[j].x & keep, hi[j].y & keep, hi[j].z & keep, hi[j].w & keep);
+              const uint4 v = make_uint4(lo[j].x & keep, lo[j].y & keep, lo[j].z & keep, lo[j].w & keep);
+              *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) = u;
+              if (R <= 32) *reinterpret_cast<uint4*>(row + (((j + 4) ^ (r & 7)) << 4)) = v;
+              else *reinterpret_cast<uint4*>(row + kAdTile + ((j ^ (r & 7)) << 4)) = v;
             }
           fence_async_smem();
           __syncwarp();
@@ -604,8 +633,12 @@ struct __align__(8) RowsBars {
   int stop;
 };
 
-// grid: (members of the cluster, feature tiles).  192 threads: producer, MMA, four epilogue warps (a thread a feature).
-__global__ void __launch_bounds__(192)
+// grid: (members of the cluster, feature tiles).  320 threads: producer, MMA, eight epilogue warps (two threads a feature, rows of
+// x in turn).
+constexpr int kRowsThreads = 320;
+constexpr int kRowsAtOnce = 4;             // rows of x whose rows of B a thread has under way
+
+__global__ void __launch_bounds__(kRowsThreads, 2)
 adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const int* __restrict__ ids,
                     const float* __restrict__ h, const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows,
                     int N, int K, int R, int n, const __grid_constant__ TcSlices slices, int NT, int stages) {
@@ -614,9 +647,12 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   RowsBars* bars = reinterpret_cast<RowsBars*>(smem);
   unsigned char* stage0 = smem + 1024;
   const int stage_bytes = kAdTile + NT * 128;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* sums = reinterpret_cast<float*>(stage0 + (size_t)stages * stage_bytes);      // [members][share of rows][128], written by all members
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int members = gridDim.x, member = blockIdx.x;          // the cluster is the grid's first dimension
+  const int share = (rows + members - 1) / members;            // rows of x that a member adds up: [member * share, ...)
   volatile int* stop = &bars->stop;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this member is there
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
     mbar_init(&bars->acc_full, 1);
@@ -632,93 +668,123 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const WideTile w = wide_tile(blockIdx.y, gridDim.y, kAdM, kAdM, slices);
   const int steps = (K + kAdK - 1) / kAdK;
   const int k_first = (int)((long long)member * steps / members), k_last = (int)((long long)(member + 1) * steps / members);
-  float* sums = reinterpret_cast<float*>(stage0);              // [NT][128], in the stages once they are read
+  const int quad = warp & 3, turn = warp >= 6 ? 1 : 0;         // (epilogue warps)
+  const int d = quad * 32 + lane, f = w.f0 + d;
+  const int t_first = member * share, t_last = min(rows, t_first + share);
+
+  // a thread's rows of x: t_first + turn, + 2, ...; their adapters and rows of B
+  int a[kRowsAtOnce];
+  uint4 raw[kRowsAtOnce][2];
+  auto ask = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      const int t = t0 + 2 * i;
+      a[i] = t < t_last ? ids[t] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      if (a[i] >= n && blockIdx.y == 0 && d == 0) atomicCAS(&g_adapter_tc_index, 0, t0 + 2 * i + 1);
+      if (a[i] >= n || d >= w.width) a[i] = -1;
+      if (a[i] >= 0) {
+        const uint4* b = reinterpret_cast<const uint4*>(B + ((size_t)a[i] * N + f) * R);
+        raw[i][0] = b[0];
+        raw[i][1] = b[1];
+      }
+    }
+  };
 
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      bool fine = true;
-      for (int it = 0; it < k_last - k_first; ++it) {
-        const int s = it % stages;
-        if (!mbar_wait(&bars->empty[s], ((it / stages) & 1) ^ 1, stop, 11, &g_adapter_tc_error)) { fine = false; break; }
-        unsigned char* st = stage0 + (size_t)s * stage_bytes;
-        mbar_expect_tx(&bars->full[s], stage_bytes);
-        tma_load_2d(st, &map_w, (k_first + it) * kAdK, w.f0, &bars->full[s]);
-        tma_load_2d(st + kAdTile, &map_x, (k_first + it) * kAdK, 0, &bars->full[s]);
-        issued = it + 1;
+    Ring ring;
+    int it = 0;
+    const int count = k_last - k_first;
+    for (; it < count; ++it, ring.next(stages)) {
+      if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 11)) break;
+      unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+      if (elect_one()) {
+        mbar_expect_tx(&bars->full[ring.s], stage_bytes);
+        tma_load_2d(st, &map_w, (k_first + it) * kAdK, w.f0, &bars->full[ring.s]);
+        tma_load_2d(st + kAdTile, &map_x, (k_first + it) * kAdK, 0, &bars->full[ring.s]);
       }
-      if (!fine)
-        for (int j = max(0, issued - stages); j < issued; ++j)
-          for (unsigned i = 0; i < (1u << 20); ++i)
-            if (mbar_try(&bars->full[j % stages], (j / stages) & 1)) break;
+      __syncwarp();
     }
+    if (it < count)
+      for (int j = max(0, it - stages); j < it; ++j)
+        for (unsigned i = 0; i < (1u << 20); ++i)
+          if (mbar_try(&bars->full[j % stages], (j / stages) & 1)) break;
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else if (warp == 1) {
-    if (lane == 0) {
-      const unsigned idesc = ad_instr_desc(NT, kAdM);
-      bool fine = true;
-      for (int it = 0; it < k_last - k_first; ++it) {
-        const int s = it % stages;
-        if (!mbar_wait(&bars->full[s], (it / stages) & 1, stop, 13, &g_adapter_tc_error)) { fine = false; break; }
-        tc_fence_after();
-        unsigned char* st = stage0 + (size_t)s * stage_bytes;
-        const unsigned long long dw = smem_desc(st), dx = smem_desc(st + kAdTile);
+    Ring ring;
+    const unsigned idesc = ad_instr_desc(NT, kAdM);
+    const int count = k_last - k_first;
+    for (int it = 0; it < count; ++it, ring.next(stages)) {
+      if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 13)) break;
+      tc_fence_after();
+      unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+      const unsigned long long dw = smem_desc(st), dx = smem_desc(st + kAdTile);
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kAdK / 16; ++kk) tc_mma(tmem, dw + 2 * kk, dx + 2 * kk, idesc, it > 0 || kk > 0 ? 1u : 0u);
-        tc_commit(&bars->empty[s]);
+        tc_commit(&bars->empty[ring.s]);
+        if (it + 1 == count) tc_commit(&bars->acc_full);
       }
-      if (fine) tc_commit(&bars->acc_full);
+      __syncwarp();
     }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
-    const int quad = warp & 3;
+    ask(t_first + turn);
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // every member is there: its shared memory may be written
     if (warp_wait(&bars->acc_full, 0, stop, 14)) {
       tc_fence_after();
-      for (int c0 = 0; c0 < NT; c0 += 16) {
+      // this CTA's sums go to the members that own the rows
+      for (int c0 = 16 * turn; c0 < NT; c0 += 32) {
         unsigned v[16];
         tc_ld16(tmem + ((unsigned)(quad * 32) << 16) + c0, v);
         tc_wait_ld();
+        int to = c0 / share, tl = c0 - to * share;
+        const unsigned mine = smem_u32(sums + (size_t)member * share * kAdM + d);
+        unsigned at = cluster_addr(mine, min(to, members - 1));
 #pragma unroll
-        for (int c = 0; c < 16; ++c) sums[(c0 + c) * kAdM + quad * 32 + lane] = __uint_as_float(v[c]);
+        for (int c = 0; c < 16; ++c) {
+          if (c0 + c < rows) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at + tl * kAdM * 4), "r"(v[c]) : "memory");
+          if (++tl == share) { tl = 0; ++to; at = cluster_addr(mine, min(to, members - 1)); }
+        }
       }
     }
     tc_fence_before();
   }
   __syncwarp();
-  cluster_barrier();                   // the members' sums are all there
+  cluster_barrier();                   // all sums are there, and nothing of tensor memory is still to be read
+  if (warp == 1) {
+    tc_fence_after();
+    tc_dealloc<1>(tmem, 64);
+  }
   if (warp >= 2) {
-    const int d = (warp & 3) * 32 + lane, f = w.f0 + d, SR = slices.n * R;
-    const int t_first = (int)((long long)member * rows / members), t_last = (int)((long long)(member + 1) * rows / members);
-    const unsigned local = smem_u32(sums + d);
+    const int SR = slices.n * R;
     chain_wait(h);
-    constexpr int U = 4;               // rows of x at a time
-    for (int t0 = t_first; t0 < t_last; t0 += U) {
-      float sum[U];
-      int a[U];
+    for (int t0 = t_first + turn; t0 < t_last; t0 += 2 * kRowsAtOnce) {
+      if (t0 != t_first + turn) ask(t0);
+      float sum[kRowsAtOnce];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int t = min(t0 + i, t_last - 1);
-        a[i] = ids[t];
-        if (a[i] >= n && blockIdx.y == 0 && d == 0) atomicCAS(&g_adapter_tc_index, 0, t + 1);
-        if (a[i] >= n || d >= w.width) a[i] = -1;
+      for (int i = 0; i < kRowsAtOnce; ++i) {
+        const int tl = min(t0 + 2 * i, t_last - 1) - t_first;
         sum[i] = 0.f;
-        for (int m = 0; m < members; ++m) {
-          float v;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(local + t * kAdM * 4, m)));
-          sum[i] += v;
-        }
+        for (int m = 0; m < members; ++m) sum[i] += sums[((size_t)m * share + tl) * kAdM + d];
       }
       for (int j = 0; j < R; j += 16) {
-        uint4 raw[U][2];
+        if (j > 0) {
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-          if (a[i] >= 0) {
-            const uint4* b = reinterpret_cast<const uint4*>(B + ((size_t)a[i] * N + f) * R + j);
-            raw[i][0] = b[0];
-            raw[i][1] = b[1];
-          }
+          for (int i = 0; i < kRowsAtOnce; ++i)
+            if (a[i] >= 0) {
+              const uint4* b = reinterpret_cast<const uint4*>(B + ((size_t)a[i] * N + f) * R + j);
+              raw[i][0] = b[0];
+              raw[i][1] = b[1];
+            }
+        }
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+        for (int i = 0; i < kRowsAtOnce; ++i)
           if (a[i] >= 0) {
-            const float* hr = h + (size_t)min(t0 + i, t_last - 1) * SR + w.slice * R + j;
+            const float* hr = h + (size_t)(t0 + 2 * i) * SR + w.slice * R + j;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               float bv[8], hv[8];
@@ -730,17 +796,9 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           }
       }
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (t0 + i < t_last && d < w.width) y[(size_t)(t0 + i) * N + f] = __float2bfloat16_rn(sum[i]);
+      for (int i = 0; i < kRowsAtOnce; ++i)
+        if (t0 + 2 * i < t_last && d < w.width) y[(size_t)(t0 + 2 * i) * N + f] = __float2bfloat16_rn(sum[i]);
     }
-  }
-  __syncwarp();
-  cluster_barrier();                   // nobody reads another's shared memory any more
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tc_dealloc<1>(tmem, 64);
   }
 }
 
@@ -783,18 +841,15 @@ int adapter_shrink_simt(const void* x, const void* A, const float* scale, const 
 using namespace nf;
 
 static int shrink_members(int rows, int K, int SR) {
-  const int tiles = ((rows + kAdM - 1) / kAdM) * (SR > kShrinkCols ? (SR + kAdM - 1) / kAdM : 1), steps = (K + kAdK - 1) / kAdK;
+  const int tiles = ((rows + kAdM - 1) / kAdM) * ((SR + kAdM - 1) / kAdM), steps = (K + kAdK - 1) / kAdK;
   int p = 1;
   while (p < 8 && 2 * p * tiles <= sm_count() && steps >= 4 * p) p *= 2;
   return p;
 }
 
-// Floats of scratch that `rows` rows take for every number of h (n_slices * R a row).
-extern "C" int nf_adapter_parts(int rows, int K, int SR) { return rows <= 16 ? 1 : 1 + shrink_members(rows, K, SR); }
-
 // y = x W^T + the adapters' part (see the head of this file): x [rows, K], W [N, K], A [n, n_slices * R, K], B [n, N, R], y
-// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h float32 [nf_adapter_parts(rows, K, n_slices * R), rows, n_slices * R]
-// of scratch.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or
+// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h float32 [rows, n_slices * R] of
+// scratch.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or
 // 128, bases 16-byte aligned.
 extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h,
                                  void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, cudaStream_t stream) {
@@ -820,18 +875,17 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     if (int rc = adapter_shrink_simt(x, A, scale, ids, h, rows, K, SR, n, stream)) return rc;
   } else {
     const int members = shrink_members(rows, K, SR);
-    const int JW = SR > kShrinkCols ? kAdM : SR, j_tiles = (SR + JW - 1) / JW;
+    const int JW = SR < kAdM ? SR : kAdM, j_tiles = (SR + JW - 1) / JW;
     const int most = n < kAdM ? (n < rows ? n : rows) : (rows < kAdM ? rows : kAdM);      // adapters that a tile's rows may have
     const int group = kShrinkCols / JW < most ? kShrinkCols / JW : most;
     const int x_box = rows >= kAdM ? kAdM : (rows + 7) & ~7;
     CUtensorMap ma, mx;
     if (int rc = make_map(&ma, A, (long long)n * SR, K, JW)) return rc;
     if (int rc = make_map(&mx, x, rows, K, x_box)) return rc;
-    const int stage = kAdTile + group * JW * 128, here = (steps + members - 1) / members;
-    int stages = (200 * 1024) / stage;
+    const int stage = kAdTile + group * JW * 128, sums = kAdM * JW * 4;
+    int stages = (200 * 1024 - sums) / stage;
     stages = stages > 8 ? 8 : stages;
-    stages = stages > here && group >= most ? here : stages;
-    size_t smem = 2048 + (size_t)stages * stage;
+    size_t smem = 2048 + (size_t)stages * stage + sums;
     smem = smem < kShrinkSmemLeast ? kShrinkSmemLeast : smem;
     static int asked = room_for(adapter_shrink_tc_kernel, 204 * 1024);
     if (asked) return asked;
@@ -840,7 +894,7 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     turns = turns < 1 ? 1 : turns > passes ? passes : turns;
     NF_REQUIRE(row_tiles * j_tiles <= 65535, "adapter_linear: %d rows are too many", rows);
     launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, row_tiles * j_tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
-                           ids, h + (size_t)rows * SR, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, rows > kRowsMost ? 1 : 0);
+                           ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, rows > kRowsMost ? 1 : 0);
     if (int rc = check_launch("adapter_shrink")) return rc;
   }
 
@@ -852,16 +906,15 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     while (members < 8 && 2 * members * tiles <= 2 * sm_count() && steps >= 4 * members) members *= 2;
     if (int rc = make_map(&mw, W, N, K, kAdM)) return rc;
     if (int rc = make_map(&mx, x, rows, K, NT)) return rc;
-    const int stage = kAdTile + NT * 128, here = (steps + members - 1) / members;
-    int stages = (104 * 1024) / stage;
+    const int stage = kAdTile + NT * 128, here = (steps + members - 1) / members, share = (rows + members - 1) / members;
+    const int sums = members * share * kAdM * 4;
+    int stages = (104 * 1024 - sums) / stage;
     stages = stages > here ? here : stages;
-    const int least = (NT * kAdM * 4 + stage - 1) / stage;       // the sums take the stages' place
-    stages = stages < least ? least : stages;
-    const size_t smem = 2048 + (size_t)stages * stage;
+    const size_t smem = 2048 + (size_t)stages * stage + sums;
     static int asked = room_for(adapter_rows_kernel, 108 * 1024);
     if (asked) return asked;
     NF_REQUIRE(tiles <= 65535, "adapter_linear: %d features are too many", N);
-    launch_chained_cluster(adapter_rows_kernel, dim3(members, tiles), dim3(192), smem, stream, members, mw, mx, ids, (const float*)h,
+    launch_chained_cluster(adapter_rows_kernel, dim3(members, tiles), dim3(kRowsThreads), smem, stream, members, mw, mx, ids, (const float*)h,
                            (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows, N, K, R, n, sl, NT, stages);
     return check_launch("adapter_rows");
   }
@@ -885,7 +938,7 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
   const int f_tiles = feature_tiles(sl, BN);
   const long long n_tiles = (long long)f_tiles * ((rows + kAdM * ctas - 1) / (kAdM * ctas));
   NF_REQUIRE(n_tiles < (1ll << 30), "adapter_linear: %d rows of %d features are too many", rows, N);
-  int stages = (kWideSmem - kWideHead - kWideH) / (kAdTile + BN / ctas * 128);
+  int stages = (kWideSmem - kWideHead - wide_h_bytes(ctas)) / (kAdTile + BN / ctas * 128);
   stages = stages > kAdMaxStages ? kAdMaxStages : stages;
   static int asked1 = room_for(adapter_wide_kernel<1>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2>, kWideSmem + 1024);
   if (asked1 || asked2) return 1;

@@ -28,7 +28,6 @@ _SIGNATURES = {
     "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _P],
     "nf_append_history": [_P] * 4 + [_I] * 3 + [_P],
     "nf_logit_rules": [_P] * 11 + [_I] + [_P] * 2 + [_I] * 7 + [_P],
-    "nf_adapter_parts": [_I] * 3,
 }
 _functions = {}
 _used = False           # whether any of these kernels was called: until then there is no status to read
@@ -142,7 +141,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         e += v
         ends[i] = e
     if dtype is torch.bfloat16 and K % 8 == 0 and TUNING["adapter"] == "auto":
-        h = scale.new_empty(_function("nf_adapter_parts")(T, K, S * R) * T * S * R)
+        h = scale.new_empty(T * S * R)
         _call("nf_adapter_linear", px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream())
         return out
     # float32, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
