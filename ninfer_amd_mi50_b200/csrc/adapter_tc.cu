@@ -229,7 +229,7 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   tc_fence_after();
   const unsigned tmem = bars->tmem_base;
   chain_wait(ids, scale);
-  chain_release_late();               // the product behind this may begin: what came before is complete
+  chain_release_late();
   const int tile = blockIdx.y % row_tiles, jt = blockIdx.y / row_tiles;
   const int row0 = tile * kAdM, j0 = jt * JW, jn = min(JW, SR - j0);
   const int steps = (K + kAdK - 1) / kAdK;
@@ -270,6 +270,8 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         if (lane < count) tma_load_2d(st + kAdTile + lane * JW * 128, &map_a, ks * kAdK, mine * SR + j0, &bars->full[s]);
       }
     }
+    // The product behind this may begin: what came before is complete.  Not sooner, or W's rows, which it asks for at once, would
+    // come before the adapters'.
     if (!ok && lane == 0) {
       for (int j = max(0, issued - stages); j < issued; ++j)
         for (unsigned i = 0; i < (1u << 20); ++i)
@@ -378,6 +380,7 @@ constexpr int kWideEpilogueWarps = 8;
 constexpr int kWideThreads = 32 * (2 + 4 + kWideEpilogueWarps);
 constexpr int kWideHead = 1024;                            // barriers
 constexpr int wide_h_bytes(int ctas) { return 2 * ctas * kAdTile; }      // rows of h
+constexpr int kTurnRow = 34, kTurnBytes = 32 * kTurnRow * 2;             // a warp's 32 x 32 results, where rows of y are not 16-byte pieces
 constexpr int kWideSmem = 225 * 1024;
 
 struct WideTile {
@@ -402,6 +405,11 @@ __device__ __forceinline__ WideTile wide_tile(int i, int f_tiles, int tile_rows,
   }
 }
 
+// The tile a CTA (or pair) takes after `i`: rounds of as many tiles as there are CTAs, the first dealt forwards, the others backwards.
+// The engine puts decoded rows first, so a step's first tiles have the most adapters, and the CTAs with those get none of the last,
+// shorter round.
+__device__ __forceinline__ int next_tile(int i, int first, int stride) { return i < stride ? 2 * stride - 1 - first : i + stride; }
+
 // CTAS 1: a CTA a tile of 128 rows x BN features.  CTAS 2: two CTAs of a cluster a tile of 256 x BN; each holds its own 128 rows of x
 // and half of the features' rows of W, and the even one issues products over both (`cta_group::2`): half of W's bytes a CTA.
 // Warps: 0 producer, 1 MMA and tensor memory, 2..5 rows of h (a thread a row), 6..13 epilogue.
@@ -410,7 +418,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_b,
                     const int* __restrict__ ids, const __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
                     int R, int n, const __grid_constant__ TcSlices slices, int f_tiles, int n_tiles, int BN, int stages) {
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ unsigned char smem_raw[];      // [barriers | rows of h | stages | where N % 8: results on their way]
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   WideBars* bars = reinterpret_cast<WideBars*>(smem);
   unsigned char* h_tile = smem + kWideHead;
@@ -439,9 +447,10 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int steps = (K + kAdK - 1) / kAdK;
   const int r_steps = (R + kAdK - 1) / kAdK;          // steps of up to 64 ranks an adapter
   const int r_here = min(R, kAdK);                    // ranks of one such step (R is 16, 32, 64 or 128)
-  // Rows of h lie 128 bytes apart; up to 32 ranks both parts fit into that.  Several adapters' rows are under way at a time: from
-  // one thread's store to the issuer and back is longer than the products take.
-  const int h_bufs = R <= 32 ? 2 * CTAS : CTAS, lo_at = R <= 32 ? 64 : kAdTile, h_bytes = R <= 32 ? kAdTile : 2 * kAdTile;
+  // Rows of h lie 128 bytes apart; up to 32 ranks both parts fit into that, beyond they come one after the other.  Several are under
+  // way at a time: from one thread's store to the issuer and back is longer than the products take.
+  constexpr int h_bufs = 2 * CTAS;
+  const int h_parts = R <= 32 ? 1 : 2;
   TileIds<CTAS> tids;
 
   if (warp == 0) {
@@ -449,7 +458,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     int issued = 0;
     bool ok = true;
     Ring ring;
-    for (int i = first; i < n_tiles && ok; i += stride) {
+    for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride)) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int x_row = w.row0 + rank * kAdM, w_row = w.f0 + rank * (BN / CTAS);
@@ -488,7 +497,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     bool ok = true;
     Ring ring, hring;
     const unsigned idesc = ad_instr_desc(BN, kAdM * CTAS);
-    for (int i = first; i < n_tiles && ok; i += stride, ++done) {
+    for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride), ++done) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int ab = done & 1;
@@ -508,21 +517,23 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         __syncwarp();
       }
       for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
-        for (int rs = 0; rs < r_steps; ++rs, ring.next(stages), hring.next(h_bufs)) {
-          if (!warp_wait_cluster(&bars->h_full[hring.s], hring.phase, stop, 5) ||
-              !warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
-          tc_fence_after();
-          const unsigned long long hi = smem_desc(h_tile + hring.s * h_bytes), lo = hi + (lo_at >> 4);
+        for (int rs = 0; rs < r_steps && ok; ++rs, ring.next(stages)) {
+          if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
           const unsigned long long db = smem_desc(stage0 + (size_t)ring.s * stage_bytes + kAdTile);
-          if (elect_one()) {
-            for (int kk = 0; kk < r_here / 16; ++kk) {
-              mma<CTAS>(acc, hi + 2 * kk, db + 2 * kk, idesc, 1u);
-              mma<CTAS>(acc, lo + 2 * kk, db + 2 * kk, idesc, 1u);
+          for (int part = 0; part < h_parts; ++part, hring.next(h_bufs)) {
+            if (!warp_wait_cluster(&bars->h_full[hring.s], hring.phase, stop, 5)) { ok = false; break; }
+            tc_fence_after();
+            const unsigned long long dh = smem_desc(h_tile + hring.s * kAdTile);
+            if (elect_one()) {
+              for (int kk = 0; kk < r_here / 16; ++kk) {
+                mma<CTAS>(acc, dh + 2 * kk, db + 2 * kk, idesc, 1u);
+                if (h_parts == 1) mma<CTAS>(acc, dh + (64 >> 4) + 2 * kk, db + 2 * kk, idesc, 1u);
+              }
+              commit<CTAS>(&bars->h_empty[hring.s]);
+              if (part + 1 == h_parts) commit<CTAS>(&bars->empty[ring.s]);
             }
-            commit<CTAS>(&bars->empty[ring.s]);
-            commit<CTAS>(&bars->h_empty[hring.s]);
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
       if (ok && elect_one()) commit<CTAS>(&bars->acc_full[ab]);
@@ -534,7 +545,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const int r = (warp - 2) * 32 + lane, SR = slices.n * R, n_pieces = r_here >> 3;
     bool ok = true;
     Ring hring;
-    for (int i = first; i < n_tiles && ok; i += stride) {
+    for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride)) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int t = w.row0 + rank * kAdM + r;
@@ -553,23 +564,23 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       read(0);
       for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
         const unsigned keep = own == a ? 0xffffffffu : 0u;
-        for (int rs = 0; rs < r_steps; ++rs, hring.next(h_bufs)) {
-          const int hb = hring.s;
+        for (int rs = 0; rs < r_steps && ok; ++rs) {
           if (rs > 0 && own == a) read(rs);
-          if (!warp_wait(&bars->h_empty[hb], hring.phase ^ 1, stop, 6)) { ok = false; break; }
-          unsigned char* row = h_tile + hb * h_bytes + r * 128;
+          for (int part = 0; part < h_parts; ++part, hring.next(h_bufs)) {
+            if (!warp_wait(&bars->h_empty[hring.s], hring.phase ^ 1, stop, 6)) { ok = false; break; }
+            unsigned char* row = h_tile + hring.s * kAdTile + r * 128;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < n_pieces) {
-              const uint4 u = make_uint4(hi[j].x & keep, hi[j].y & keep, hi[j].z & keep, hi[j].w & keep);
-              const uint4 v = make_uint4(lo[j].x & keep, lo[j].y & keep, lo[j].z & keep, lo[j].w & keep);
-              *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) = u;
-              if (R <= 32) *reinterpret_cast<uint4*>(row + (((j + 4) ^ (r & 7)) << 4)) = v;
-              else *reinterpret_cast<uint4*>(row + kAdTile + ((j ^ (r & 7)) << 4)) = v;
-            }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) arrive_leader<CTAS>(&bars->h_full[hb]);
+            for (int j = 0; j < 8; ++j)
+              if (j < n_pieces) {
+                const uint4 p = part ? lo[j] : hi[j];
+                *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) = make_uint4(p.x & keep, p.y & keep, p.z & keep, p.w & keep);
+                if (j < 4 && h_parts == 1)
+                  *reinterpret_cast<uint4*>(row + (((j + 4) ^ (r & 7)) << 4)) = make_uint4(lo[j].x & keep, lo[j].y & keep, lo[j].z & keep, lo[j].w & keep);
+              }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_leader<CTAS>(&bars->h_full[hring.s]);
+          }
         }
       }
     }
@@ -577,7 +588,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     // ---- epilogue: tensor-memory lanes 32 * (warp % 4) .. + 31, every other run of 32 columns --------------------------------
     const int quad = warp & 3, half = (warp - 6) >> 2;
     int done = 0;
-    for (int i = first; i < n_tiles; i += stride, ++done) {
+    for (int i = first; i < n_tiles; i = next_tile(i, first, stride), ++done) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       const int ab = done & 1;
       if (!warp_wait(&bars->acc_full[ab], (done >> 1) & 1, stop, 4)) break;
@@ -585,6 +596,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const int t = w.row0 + rank * kAdM + quad * 32 + lane;
       __nv_bfloat16* out = y + (size_t)t * N + w.f0;
       const bool whole = N % 8 == 0 && w.f0 % 8 == 0;
+      unsigned short* turned = reinterpret_cast<unsigned short*>(stage0 + (size_t)stages * stage_bytes + (warp - 6) * kTurnBytes);
       for (int c0 = half * 32; c0 < BN; c0 += 64) {
         unsigned v[32];
         if (c0 < w.width) {
@@ -596,8 +608,27 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           __syncwarp();
           if (lane == 0) arrive_leader<CTAS>(&bars->acc_empty[ab]);
         }
-        if (c0 >= w.width || t >= rows) continue;
-        if (whole && c0 + 32 <= w.width) {
+        if (c0 >= w.width) continue;
+        if (!whole) {
+          // a thread's row would be 32 stores of 2 bytes, each to a line of its own: the warp's results change hands, and a store
+          // is 64 bytes of one row
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const __nv_bfloat162 o = __floats2bfloat162_rn(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+            *reinterpret_cast<__nv_bfloat162*>(turned + lane * kTurnRow + c) = o;
+          }
+          __syncwarp();
+          const int t0 = w.row0 + rank * kAdM + quad * 32, count = min(32, rows - t0);
+          if (c0 + lane < w.width) {
+            unsigned short* to = reinterpret_cast<unsigned short*>(y) + (size_t)t0 * N + w.f0 + c0 + lane;
+#pragma unroll 8
+            for (int r = 0; r < count; ++r) to[(size_t)r * N] = turned[r * kTurnRow + lane];
+          }
+          continue;
+        }
+        if (t >= rows) continue;
+        if (c0 + 32 <= w.width) {
 #pragma unroll
           for (int c = 0; c < 32; c += 8) {
             __nv_bfloat162 o[4];
@@ -938,7 +969,10 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
   const int f_tiles = feature_tiles(sl, BN);
   const long long n_tiles = (long long)f_tiles * ((rows + kAdM * ctas - 1) / (kAdM * ctas));
   NF_REQUIRE(n_tiles < (1ll << 30), "adapter_linear: %d rows of %d features are too many", rows, N);
-  int stages = (kWideSmem - kWideHead - wide_h_bytes(ctas)) / (kAdTile + BN / ctas * 128);
+  bool whole = N % 8 == 0;
+  for (int i = 0; i < n_slices; ++i) whole = whole && ends[i] % 8 == 0;
+  const int turned = whole ? 0 : kWideEpilogueWarps * kTurnBytes;
+  int stages = (kWideSmem - kWideHead - wide_h_bytes(ctas) - turned) / (kAdTile + BN / ctas * 128);
   stages = stages > kAdMaxStages ? kAdMaxStages : stages;
   static int asked1 = room_for(adapter_wide_kernel<1>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2>, kWideSmem + 1024);
   if (asked1 || asked2) return 1;
