@@ -30,121 +30,251 @@ struct RuleArgs {
   int V, ld_in, ld_out, n_slots, capacity, n_bias, mask_rows, words;
 };
 
-constexpr int kRuleThreads = 256;
+constexpr int kRuleThreads = 512;
+template <int V> struct Int { static constexpr int value = V; };
 
-// PIECES: runs of four logits a thread; a CTA's piece of the vocabulary is kRuleThreads * 4 * PIECES of them, counted from the
-// last 16-byte boundary at or before the row's start.
-template <int PIECES>
-__global__ void __launch_bounds__(kRuleThreads)
+// Occurrences of one token: in the prompt, and among the generated ones.  A log of up to 65,535 tokens has both in one word.
+template <bool WORD> struct Counts;
+template <> struct Counts<true> {
+  static constexpr int kWords = 1;
+  __device__ static void add(unsigned* n, int, unsigned d, bool made) { atomicAdd(n + d, made ? 0x10000u : 1u); }
+  __device__ static uint4 any(const unsigned* n, int, int d) { return *reinterpret_cast<const uint4*>(n + d); }
+  __device__ static void clear(unsigned* n, int, int d) { n[d] = 0; }
+  __device__ static void get(const unsigned* n, int, int d, unsigned& all, unsigned& made) {
+    made = n[d] >> 16;
+    all = (n[d] & 0xffffu) + made;
+  }
+};
+template <> struct Counts<false> {
+  static constexpr int kWords = 2;
+  __device__ static void add(unsigned* n, int C, unsigned d, bool made) { atomicAdd(n + d + (made ? C : 0), 1u); }
+  __device__ static uint4 any(const unsigned* n, int C, int d) {
+    const uint4 u = *reinterpret_cast<const uint4*>(n + d), v = *reinterpret_cast<const uint4*>(n + C + d);
+    return make_uint4(u.x | v.x, u.y | v.y, u.z | v.z, u.w | v.w);
+  }
+  __device__ static void clear(unsigned* n, int C, int d) { n[d] = n[C + d] = 0; }
+  __device__ static void get(const unsigned* n, int C, int d, unsigned& all, unsigned& made) {
+    made = n[C + d];
+    all = n[d] + made;
+  }
+};
+
+// What a piece of the vocabulary, tokens [lo, lo + C), has of a row's log: the places [from, end) of it, those from `start` on
+// generated.  (Additions whose results nobody waits for: with the first occurrence of a token noticed by what its addition returns,
+// logs of 131,072 tokens took 18.6 us instead of 11.)
+template <bool WORD>
+struct PieceLog {
+  static constexpr int U = 4;   // runs of four tokens a thread has under way
+  unsigned* counts;             // [kWords * C]
+  int lo, C;
+  const int4* quads;
+  int from, start, end;
+  __device__ __forceinline__ void one(int t, bool made) {
+    const unsigned d = (unsigned)t - (unsigned)lo;
+    if (d < (unsigned)C) Counts<WORD>::add(counts, C, d, made);
+  }
+  __device__ __forceinline__ void ask(int q0, int4* t) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (4 * (q0 + u * kRuleThreads) < end) t[u] = quads[q0 + u * kRuleThreads];
+  }
+  __device__ __forceinline__ void take(int q0, const int4* t) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int p = 4 * (q0 + u * kRuleThreads);
+      if (p >= end) break;
+      const int n[4] = {t[u].x, t[u].y, t[u].z, t[u].w};
+      if (p >= from && p + 4 <= end) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) one(n[e], p + e >= start);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (p + e >= from && p + e < end) one(n[e], p + e >= start);
+      }
+    }
+  }
+};
+
+// A CTA takes a piece of WALK * PIECES * 4 * kRuleThreads tokens of one row, counted from the last 16-byte boundary at or before the
+// row's start.  It copies the piece's logits under the mask, WALK steps of PIECES runs of four a thread, and then does what is left to
+// do at the biased tokens and at those that occur in the log, one thread each.  (Done where the logits are copied, the powers and
+// quotients of the few tokens that occur held up nearly every warp: 204 instructions a run of four, 256 rows of 151936 99 us.)
+// What bounds it: 256 rows of 151936 take 69 us, of which the copy alone, as it runs without rules, 49 (6.3 TB/s); the rest is a CTA's
+// chain from a row's numbers to its log to the counts to the list.  So everything that does not wait for anything is asked for first,
+// the log's loads are under way while the logits are copied, a walked piece's logits are brought into L2 meanwhile, and a walked
+// piece leaves room for three CTAs on an SM (with two 76 us).  One row of 151936 and a short log 3.1 us: the chain and the launch.
+template <int PIECES, int WALK, bool WORD>
+__global__ void __launch_bounds__(kRuleThreads, WALK > 1 ? 3 : 2)
 logit_rules_kernel(RuleArgs a) {
-  constexpr int C = kRuleThreads * 4 * PIECES;
-  extern __shared__ __align__(16) unsigned rule_smem[];
-  unsigned* all = rule_smem;                  // [C] occurrences anywhere
-  unsigned* made = all + C;                   // [C] among the generated ones
-  float* add = reinterpret_cast<float*>(made + C);   // [C] biases (where there are any)
+  constexpr int STEP = kRuleThreads * 4 * PIECES, C = STEP * WALK;
+  extern __shared__ __align__(16) unsigned rule_smem[];   // [counts | list]
+  __shared__ int listed;
+  __shared__ unsigned mask[C / 32 + 2];                   // the piece's words of the row's mask
   chain_wait();
   const int r = blockIdx.y, tid = threadIdx.x;
   const float* row = a.logits + (size_t)r * a.ld_in;
   float* out = a.out + (size_t)r * a.ld_out;
+  const bool in_place = a.logits == a.out;
   const int pad = (int)(((uintptr_t)row >> 2) & 3);
   const int lo = (int)blockIdx.x * C - pad;   // the token of place 0
   const bool pairs = (((uintptr_t)out >> 2) & 3) == (unsigned)pad;       // runs of four are aligned on both sides
 
-  float v[PIECES][4];
-#pragma unroll
-  for (int p = 0; p < PIECES; ++p) {
-    const int i = lo + 4 * (tid + p * kRuleThreads);
-    if (i >= 0 && i + 4 <= a.V) {
-      load4(row + i, v[p]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[p][e] = i + e >= 0 && i + e < a.V ? row[i + e] : 0.f;
-    }
-  }
-  for (int i = tid; i < 2 * C / 4; i += kRuleThreads) reinterpret_cast<uint4*>(all)[i] = make_uint4(0, 0, 0, 0);
-  const bool biased = a.bias_offsets != nullptr;
-  if (biased)
-    for (int i = tid; i < C / 4; i += kRuleThreads) reinterpret_cast<float4*>(add)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  __syncthreads();
-
-  // ---- the log's tokens that lie in this piece
-  const float rep = a.penalties[3 * r], freq = a.penalties[3 * r + 1], pres = a.penalties[3 * r + 2];
-  const int slot = a.slots[r];
+  // everything that does not wait for anything is asked for first
+  const int slot = a.slots[r], m = a.mask ? a.mask_index[r] : -1, last_token = a.tokens ? a.tokens[r] : 0;
   int len = a.lengths[r], start = a.starts[r];
-  const bool fits = slot >= 0 && slot < a.n_slots && len >= (a.tokens ? 1 : 0) && len <= a.capacity;
-  if (!fits || start < 0) {
-    if (tid == 0) atomicCAS(&g_rules_error, 0, r + 1);
-    start = max(start, 0);
-    if (!fits) len = 0;
-  }
-  if (len > 0) {
-    int* log = a.history + (size_t)slot * a.capacity;
-    int from = rep != 1.f ? 0 : start;                 // earlier tokens count for the repetition penalty only
-    if (rep == 1.f && freq == 0.f && pres == 0.f) from = len;
-    const int end = a.tokens ? len - 1 : len;
-    for (int i = (from & ~3) + 4 * tid; i < end; i += 4 * kRuleThreads) {
-      const int4 t4 = *reinterpret_cast<const int4*>(log + i);
-      const int t[4] = {t4.x, t4.y, t4.z, t4.w};
+  const float rep = a.penalties[3 * r], freq = a.penalties[3 * r + 1], pres = a.penalties[3 * r + 2];
+  int b0 = 0, b1 = 0;
+  if (a.bias_offsets) { b0 = a.bias_offsets[r]; b1 = a.bias_offsets[r + 1]; }
+  float v[PIECES][4];
+  auto fetch = [&](int w) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned d = (unsigned)(t[e] - lo);
-        if (i + e >= from && i + e < end && d < (unsigned)C) {
-          atomicAdd(&all[d], 1u);
-          if (i + e >= start) atomicAdd(&made[d], 1u);
-        }
+    for (int p = 0; p < PIECES; ++p) {
+      const int i0 = lo + w * STEP + 4 * (tid + p * kRuleThreads);
+      if (i0 >= 0 && i0 + 4 <= a.V) {
+        load4(row + i0, v[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[p][e] = i0 + e >= 0 && i0 + e < a.V ? row[i0 + e] : 0.f;
       }
     }
-    if (a.tokens && tid == 0) {
-      const int t = a.tokens[r];
-      const unsigned d = (unsigned)(t - lo);
-      if (len - 1 >= from && d < (unsigned)C) {
-        atomicAdd(&all[d], 1u);
-        if (len - 1 >= start) atomicAdd(&made[d], 1u);
-      }
-      if (blockIdx.x == 0) log[len - 1] = t;
+  };
+  if (!in_place) {
+    if (WALK > 1 && tid == 0) {                            // the later steps' logits into L2 (whole 16-byte runs of this row)
+      const int first = lo + STEP, count = (min(lo + C, a.V) - first) & ~3;
+      if (count > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row + first), "r"(count * 4));
     }
+    fetch(0);
   }
-  if (biased) {
-    const int b0 = max(a.bias_offsets[r], 0), b1 = min(a.bias_offsets[r + 1], a.n_bias);
-    for (int i = b0 + tid; i < b1; i += kRuleThreads) {
-      const unsigned d = (unsigned)(a.bias_ids[i] - lo);
-      if (d < (unsigned)C) atomicAdd(&add[d], a.bias_values[i]);
-    }
+  const bool generated = freq != 0.f || pres != 0.f || rep != 1.f;
+  const bool fits = slot >= 0 && slot < a.n_slots && len >= (a.tokens ? 1 : 0) && len <= a.capacity;
+  if (tid == 0 && (!fits || start < 0 || (a.mask && m >= a.mask_rows))) atomicCAS(&g_rules_error, 0, r + 1);
+  if (!fits) len = 0;
+  start = max(start, 0);
+  int* log = a.history + (size_t)(fits ? slot : 0) * a.capacity;
+  // earlier tokens count for the repetition penalty only; the log holds all but the last of the row where that comes with the call
+  PieceLog<WORD> piece{rule_smem, lo, C, reinterpret_cast<const int4*>(log), rep != 1.f ? 0 : start, start,
+                       generated ? (a.tokens ? len - 1 : len) : 0};
+  unsigned short* list = reinterpret_cast<unsigned short*>(rule_smem + Counts<WORD>::kWords * C);      // [C] places that occur, in any order
+  const int q_first = (piece.from >> 2) + tid;
+  int4 held[PieceLog<WORD>::U];
+  piece.ask(q_first, held);
+  const unsigned* bits = m >= 0 && m < a.mask_rows ? a.mask + (size_t)m * a.words : nullptr;
+  const int first = max(lo, 0), last = min(lo + C, a.V);    // this piece's tokens
+  const int word0 = first >> 5, words = ((last + 31) >> 5) - word0;
+  if (bits)
+    for (int i = tid; i < words; i += kRuleThreads) mask[i] = bits[word0 + i];
+  b0 = max(b0, 0);
+  b1 = min(b1, a.n_bias);
+  int bias_id = -1;                                        // this thread's entry; those beyond as many as threads are read later
+  float bias = 0.f, biased = 0.f;
+  if (b0 + tid < b1) {
+    bias_id = a.bias_ids[b0 + tid];
+    bias = a.bias_values[b0 + tid];
+    if (bias_id >= first && bias_id < last) biased = row[bias_id];
   }
-  const int m = a.mask ? a.mask_index[r] : -1;
-  if (a.mask && m >= a.mask_rows && tid == 0) atomicCAS(&g_rules_error, 0, r + 1);
-  const unsigned* bits = a.mask && m >= 0 && m < a.mask_rows ? a.mask + (size_t)m * a.words : nullptr;
+  if (generated)
+    for (int i = tid; i < Counts<WORD>::kWords * C / 4; i += kRuleThreads) reinterpret_cast<uint4*>(piece.counts)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) listed = 0;
   __syncthreads();
 
+  // the piece's logits under the mask
+#pragma unroll 1
+  for (int w = 0; w < WALK; ++w) {
+    if (lo + w * STEP >= a.V) break;
+    if (in_place && !bits) break;                           // nothing changes but at single tokens
+    if (w > 0 && !in_place) fetch(w);
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) {
-    const int d0 = 4 * (tid + p * kRuleThreads), i0 = lo + d0;
-    if (i0 + 4 <= 0 || i0 >= a.V) continue;
-    const uint4 c4 = *reinterpret_cast<const uint4*>(all + d0), g4 = *reinterpret_cast<const uint4*>(made + d0);
-    const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w};
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (biased) load4(add + d0, b);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = i0 + e;
-      if (i < 0 || i >= a.V) continue;
-      float x = v[p][e];
-      if (c[e] && rep != 1.f && x != 0.f && !isinf(x)) {       // (0 and the infinities stay what they are, whatever p^c is)
-        const float times = powf(rep, (float)c[e]);
-        x = x > 0.f ? x / times : x * times;
+    for (int p = 0; p < PIECES; ++p) {
+      const int i0 = lo + w * STEP + 4 * (tid + p * kRuleThreads);
+      if (i0 + 4 <= 0 || i0 >= a.V) continue;
+      const bool inside = i0 >= 0 && i0 + 4 <= a.V;
+      unsigned on = 0xfu;                                   // tokens that the mask allows
+      if (bits) {
+        const int from = max(i0, 0), word = (from >> 5) - word0, sh = from & 31;
+        unsigned x = mask[word] >> sh;
+        if (sh > 28 && word + 1 < words) x |= mask[word + 1] << (32 - sh);
+        on &= x << (from - i0);
       }
-      if (g[e]) x = x - (float)g[e] * freq - pres;
-      if (biased) x += b[e];
-      if (bits && !((bits[i >> 5] >> (i & 31)) & 1u)) x = -INFINITY;
-      v[p][e] = x;
-    }
-    if (pairs && i0 >= 0 && i0 + 4 <= a.V) {
-      store4(out + i0, v[p]);
-    } else {
+      if (in_place) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = v[p][e];
+        for (int e = 0; e < 4; ++e)
+          if (!(on & (1u << e)) && i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = -INFINITY;
+        continue;
+      }
+      if (on != 0xfu) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[p][e] = on & (1u << e) ? v[p][e] : -INFINITY;
+      }
+      if (pairs && inside) {
+        store4(out + i0, v[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = v[p][e];
+      }
     }
+  }
+  // the log
+  if (generated) {
+    piece.take(q_first, held);
+    for (int q = q_first + PieceLog<WORD>::U * kRuleThreads; 4 * q < piece.end; q += PieceLog<WORD>::U * kRuleThreads) {
+      piece.ask(q, held);
+      piece.take(q, held);
+    }
+  }
+  if (a.tokens && tid == 0 && len > 0) {
+    if (generated && len - 1 >= piece.from) piece.one(last_token, len - 1 >= start);
+    if (blockIdx.x == 0) log[len - 1] = last_token;
+  }
+
+  // the rules of one token that the mask allows, from its logit
+  auto rules = [&](float x, unsigned c, unsigned g) {
+    if (c && rep != 1.f && x != 0.f && !isinf(x)) {        // (0 and the infinities stay what they are, whatever p^c is)
+      const float times = powf(rep, (float)c);
+      x = x > 0.f ? x / times : x * times;
+    }
+    return g ? x - (float)g * freq - pres : x;
+  };
+  auto allowed = [&](int i) { return !bits || (mask[(i >> 5) - word0] >> (i & 31)) & 1u; };
+  __syncthreads();                                          // the counts are complete, the piece is written
+  // biased tokens: all of their rules, and they are off the list of the others
+  if (b0 < b1) {
+    for (int i = b0 + tid; i < b1; i += kRuleThreads) {
+      if (i >= b0 + kRuleThreads) {
+        bias_id = a.bias_ids[i];
+        bias = a.bias_values[i];
+        if (bias_id >= first && bias_id < last) biased = row[bias_id];
+      }
+      if (bias_id < first || bias_id >= last || !allowed(bias_id)) continue;
+      unsigned c = 0, g = 0;
+      if (generated) {
+        Counts<WORD>::get(piece.counts, C, bias_id - lo, c, g);
+        Counts<WORD>::clear(piece.counts, C, bias_id - lo);
+      }
+      out[bias_id] = rules(biased, c, g) + bias;
+    }
+    __syncthreads();
+  }
+  // the other tokens that occur
+  if (!generated) return;
+  for (int d = 4 * tid; d < C; d += 4 * kRuleThreads) {
+    const uint4 n = Counts<WORD>::any(piece.counts, C, d);
+    if (n.x | n.y | n.z | n.w) {
+      int at = atomicAdd(&listed, (n.x != 0) + (n.y != 0) + (n.z != 0) + (n.w != 0));
+      if (n.x) list[at++] = (unsigned short)d;
+      if (n.y) list[at++] = (unsigned short)(d + 1);
+      if (n.z) list[at++] = (unsigned short)(d + 2);
+      if (n.w) list[at++] = (unsigned short)(d + 3);
+    }
+  }
+  __syncthreads();
+  for (int k = tid; k < listed; k += kRuleThreads) {
+    const int d = list[k], i = lo + d;
+    if (i < 0 || i >= a.V || !allowed(i)) continue;
+    unsigned c, g;
+    Counts<WORD>::get(piece.counts, C, d, c, g);
+    out[i] = rules(row[i], c, g);
   }
 }
 
@@ -190,9 +320,31 @@ extern "C" int nf_logit_rules(const float* logits, float* out, int* history, con
              "logit_rules: a log of %d slots with %d tokens (a multiple of 4), 16-byte aligned", n_slots, capacity);
   const RuleArgs a{logits, out, history, slots, lengths, starts, tokens, penalties, bias_offsets, bias_ids, bias_values, mask,
                    mask_index, V, ld_in, ld_out, n_slots, capacity, n_bias, mask_rows, (V + 31) / 32};
-  constexpr int P = 2, C = kRuleThreads * 4 * P;
-  const size_t smem = (size_t)C * 4 * (bias_offsets ? 3 : 2);
-  launch_chained(logit_rules_kernel<P>, dim3((V + 3 + C - 1) / C, rows), dim3(kRuleThreads), smem, stream, a);
+  // A piece of the vocabulary costs a reading of the log, a table to clear and to look through: the largest that still make several
+  // CTAs a SM.  Rows of 151936 with logs of up to 4,000 tokens, us in pieces of 16384, 8192 and 4096: 16 rows 9.8 (4096) and 8.3
+  // (8192), 32 rows 14.3, 13.3 and 17.5, 64 rows 27.0, 25.4 and 39.1 (logs of up to 8,192), 96 and 128 rows the same in the first two.
+  const auto ctas = [&](int piece) { return (long long)rows * ((V + 3 + piece - 1) / piece); };
+  const bool word = capacity < 65536;
+  const auto run = [&](auto pieces, auto walk, auto packed) {
+    constexpr int P = decltype(pieces)::value, L = decltype(walk)::value, C = kRuleThreads * 4 * P * L;
+    constexpr bool W = decltype(packed)::value;
+    constexpr int most = C * (4 * Counts<W>::kWords + 2);
+    const int bytes = C * 4 * Counts<W>::kWords + 2 * (C < capacity ? C : capacity);      // (the list has a place for every token of a log)
+    if (most > 40 * 1024) {
+      static const cudaError_t asked = cudaFuncSetAttribute(logit_rules_kernel<P, L, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (asked != cudaSuccess) note_launch_error(asked);
+    }
+    launch_chained(logit_rules_kernel<P, L, W>, dim3((V + 3 + C - 1) / C, rows), dim3(kRuleThreads), (size_t)bytes, stream, a);
+  };
+  if (ctas(16384) >= 6 * 148) {
+    if (word) run(Int<2>{}, Int<4>{}, Int<1>{}); else run(Int<2>{}, Int<2>{}, Int<0>{});
+  } else if (ctas(8192) >= 2 * 148) {
+    if (word) run(Int<2>{}, Int<2>{}, Int<1>{}); else run(Int<2>{}, Int<2>{}, Int<0>{});
+  } else if (ctas(4096) >= 2 * 148) {
+    if (word) run(Int<2>{}, Int<1>{}, Int<1>{}); else run(Int<2>{}, Int<1>{}, Int<0>{});
+  } else {
+    if (word) run(Int<1>{}, Int<1>{}, Int<1>{}); else run(Int<1>{}, Int<1>{}, Int<0>{});
+  }
   return check_launch("logit_rules");
 }
 

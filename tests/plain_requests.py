@@ -2,6 +2,7 @@
 projection, penalties, biases and masks on logits; and bounds for what the kernels may be off."""
 
 import math
+from collections import Counter
 
 import torch
 
@@ -51,10 +52,11 @@ def plain_rules(logits, history, slots, lengths, starts, penalties, tokens=None,
             h[slot, n - 1] = int(tokens[r])
         log = h[slot, :n].tolist()
         p, f, q = (float(v) for v in penalties[r].cpu().double())
-        for i in sorted(set(log)):
+        every, made = Counter(log), Counter(log[max(start, 0):])
+        for i in every:
             if not 0 <= i < V:
                 continue
-            c, g, v = log.count(i), log[max(start, 0):].count(i), float(l[r, i])
+            c, g, v = every[i], made[i], float(l[r, i])
             err = 0.0
             if v != 0 and not math.isinf(v) and not math.isnan(v) and p != 1.0:
                 e = c * math.log(p)
@@ -69,10 +71,9 @@ def plain_rules(logits, history, slots, lengths, starts, penalties, tokens=None,
                 off[r, i] += 2 * HALF_F32 * (abs(float(l[r, i])) + abs(v)) if math.isfinite(float(l[r, i])) and math.isfinite(v) else 0.0
                 l[r, i] += v
         if mask is not None and int(mask[1][r]) >= 0:
-            words = mask[0][int(mask[1][r])].tolist()
-            for i in range(V):
-                if not (words[i // 32] >> (i % 32)) & 1:
-                    l[r, i], off[r, i] = -math.inf, 0.0
+            words, i = mask[0][int(mask[1][r])].cpu().long(), torch.arange(V)
+            left_out = (words[i // 32] >> (i % 32)) & 1 == 0
+            l[r, left_out], off[r, left_out] = -math.inf, 0.0
     most = torch.finfo(torch.float32).max
     l[l > most], l[l < -most] = math.inf, -math.inf
     return l, off, h

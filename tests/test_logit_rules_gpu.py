@@ -56,7 +56,8 @@ def same(got, want, off):
 
 @pytest.mark.parametrize("R,V,capacity,longest,few", [
     (1, 1, 4, 1, None), (1, 3, 4, 4, None), (2, 31, 16, 9, None), (3, 33, 8, 8, 5), (5, 1000, 64, 50, 20), (2, 2048, 64, 64, None),
-    (4, 2049, 512, 512, 30), (3, 4099, 2048, 2047, 300), (1, 32003, 1024, 1000, None), (2, 151936, 128, 100, None)])
+    (4, 2049, 512, 512, 30), (3, 4099, 2048, 2047, 300), (1, 32003, 1024, 1000, None), (2, 151936, 128, 100, None),
+    (40, 131075, 64, 60, 30), (75, 16385, 128, 128, 50), (20, 131071, 65536, 300, 40), (3, 5000, 65536, 66000 - 465, 700)])
 @pytest.mark.parametrize("what", ["penalties", "bias", "mask", "all"])
 def test_against_the_plain_form(R, V, capacity, longest, few, what):
     from ninfer_amd_mi50_b200 import kernels
