@@ -123,7 +123,8 @@ TUNING = {
     "moe_stream_shared": 1,
     "moe_stream_shared_max_tokens": 16,
     "moe_stream_smem_kb": 192,
-    "adapter": "auto",            # "simt" | "auto": adapters beside a bfloat16 projection
+    "adapter": "auto",            # "simt" | "auto": "simt" takes the shared product apart from the adapters
+    "adapter_f32_max_rows": 64,   # float32 rows that the kernel with the shared product in it serves
 }
 
 SUPPORTED_HEAD_DIMS = tuple(range(16, 257, 16))

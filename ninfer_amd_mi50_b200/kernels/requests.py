@@ -26,6 +26,7 @@ _I, _P = ctypes.c_int, ctypes.c_void_p
 _SIGNATURES = {
     "nf_adapter_add": [_P] * 8 + [_I] * 6 + [_P, _I, _P],
     "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _P],
+    "nf_adapter_rows_f32": [_P] * 8 + [_I] * 6 + [_P, _P],
     "nf_append_history": [_P] * 4 + [_I] * 3 + [_P],
     "nf_logit_rules": [_P] * 11 + [_I] + [_P] * 2 + [_I] * 7 + [_P],
 }
@@ -140,11 +141,12 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     for i, v in enumerate(widths):
         e += v
         ends[i] = e
-    if dtype is torch.bfloat16 and K % 8 == 0 and TUNING["adapter"] == "auto":
+    bf16 = dtype is torch.bfloat16
+    if TUNING["adapter"] == "auto" and (K % 8 == 0 if bf16 else K % 4 == 0 and T <= TUNING["adapter_f32_max_rows"]):
         h = scale.new_empty(T * S * R)
-        _call("nf_adapter_linear", px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream())
+        _call("nf_adapter_linear" if bf16 else "nf_adapter_rows_f32", px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream())
         return out
-    # float32, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
+    # many float32 rows, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
     h = scale.new_empty(T * S * R)
     z = linear(x, w, out_dtype=torch.float32)
     _call("nf_adapter_add", px, pa, pb, scale.data_ptr(), ids.data_ptr(), z.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _dt(x),

@@ -59,7 +59,9 @@ def test_against_the_plain_form(T, K, widths, n, R, pattern):
     kernels.check_status("adapter")
 
 
-@pytest.mark.parametrize("T,K,widths,n,R", [(1, 64, [64], 1, 16), (5, 200, [100, 28, 3], 4, 64), (40, 513, [130], 7, 16), (130, 96, [65], 3, 32)])
+@pytest.mark.parametrize("T,K,widths,n,R", [(1, 64, [64], 1, 16), (5, 200, [100, 28, 3], 4, 64), (40, 513, [130], 7, 16), (130, 96, [65], 3, 32),
+                                             (4, 2048, [33], 3, 16), (8, 1028, [40, 7], 4, 128), (9, 4, [1], 2, 16), (17, 3000, [66], 5, 32),
+                                             (64, 8192, [30, 31], 40, 16), (65, 1024, [64], 6, 16)])
 def test_float32(T, K, widths, n, R):
     from ninfer_amd_mi50_b200 import kernels
     args = make(T, K, widths, n, R, torch.float32, seed=T)
