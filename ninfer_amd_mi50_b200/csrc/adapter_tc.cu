@@ -379,8 +379,8 @@ struct __align__(8) WideBars {
 constexpr int kWideEpilogueWarps = 8;
 constexpr int kWideThreads = 32 * (2 + 4 + kWideEpilogueWarps);
 constexpr int kWideHead = 1024;                            // barriers
-constexpr int wide_h_bytes(int ctas) { return 2 * ctas * kAdTile; }      // rows of h
-constexpr int kTurnRow = 34, kTurnBytes = 32 * kTurnRow * 2;             // a warp's 32 x 32 results, where rows of y are not 16-byte pieces
+constexpr int wide_h_bytes(int ctas) { return 2 * kAdTile; }      // rows of h
+constexpr int kTurnRow = 80, kTurnBytes = 32 * kTurnRow;                 // a warp's 32 x 32 results, rows 80 bytes apart (no bank twice)
 constexpr int kWideSmem = 225 * 1024;
 
 struct WideTile {
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_b,
                     const int* __restrict__ ids, const __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
                     int R, int n, const __grid_constant__ TcSlices slices, int f_tiles, int n_tiles, int BN, int stages) {
-  extern __shared__ unsigned char smem_raw[];      // [barriers | rows of h | stages | where N % 8: results on their way]
+  extern __shared__ unsigned char smem_raw[];      // [barriers | rows of h | stages | results on their way]
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   WideBars* bars = reinterpret_cast<WideBars*>(smem);
   unsigned char* h_tile = smem + kWideHead;
@@ -449,7 +449,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int r_here = min(R, kAdK);                    // ranks of one such step (R is 16, 32, 64 or 128)
   // Rows of h lie 128 bytes apart; up to 32 ranks both parts fit into that, beyond they come one after the other.  Several are under
   // way at a time: from one thread's store to the issuer and back is longer than the products take.
-  constexpr int h_bufs = 2 * CTAS;
+  constexpr int h_bufs = 2;
   const int h_parts = R <= 32 ? 1 : 2;
   TileIds<CTAS> tids;
 
@@ -593,10 +593,9 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const int ab = done & 1;
       if (!warp_wait(&bars->acc_full[ab], (done >> 1) & 1, stop, 4)) break;
       tc_fence_after();
-      const int t = w.row0 + rank * kAdM + quad * 32 + lane;
-      __nv_bfloat16* out = y + (size_t)t * N + w.f0;
-      const bool whole = N % 8 == 0 && w.f0 % 8 == 0;
-      unsigned short* turned = reinterpret_cast<unsigned short*>(stage0 + (size_t)stages * stage_bytes + (warp - 6) * kTurnBytes);
+      const int t0 = w.row0 + rank * kAdM + quad * 32, count = min(32, rows - t0);
+      const bool whole = N % 8 == 0 && w.f0 % 8 == 0 && w.width % 8 == 0;
+      unsigned char* turned = stage0 + (size_t)stages * stage_bytes + (warp - 6) * kTurnBytes;
       for (int c0 = half * 32; c0 < BN; c0 += 64) {
         unsigned v[32];
         if (c0 < w.width) {
@@ -609,37 +608,30 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           if (lane == 0) arrive_leader<CTAS>(&bars->acc_empty[ab]);
         }
         if (c0 >= w.width) continue;
-        if (!whole) {
-          // a thread's row would be 32 stores of 2 bytes, each to a line of its own: the warp's results change hands, and a store
-          // is 64 bytes of one row
-          __syncwarp();
+        // A lane has 64 bytes of a row of its own: stored from there, every store of a warp goes to 32 lines.  The results change hands
+        // in shared memory, and a store covers 64 bytes of eight rows (5537 rows of 824 x 7392 93 -> 78 us), or, where rows of y are not
+        // 16-byte pieces, of one.
+        __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const __nv_bfloat162 o = __floats2bfloat162_rn(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-            *reinterpret_cast<__nv_bfloat162*>(turned + lane * kTurnRow + c) = o;
-          }
-          __syncwarp();
-          const int t0 = w.row0 + rank * kAdM + quad * 32, count = min(32, rows - t0);
-          if (c0 + lane < w.width) {
-            unsigned short* to = reinterpret_cast<unsigned short*>(y) + (size_t)t0 * N + w.f0 + c0 + lane;
-#pragma unroll 8
-            for (int r = 0; r < count; ++r) to[(size_t)r * N] = turned[r * kTurnRow + lane];
-          }
-          continue;
+        for (int c = 0; c < 32; c += 8) {
+          __nv_bfloat162 o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __floats2bfloat162_rn(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
+          *reinterpret_cast<uint4*>(turned + lane * kTurnRow + 2 * c) = *reinterpret_cast<uint4*>(o);
         }
-        if (t >= rows) continue;
-        if (c0 + 32 <= w.width) {
+        __syncwarp();
+        if (whole) {
+          const int c = c0 + 8 * (lane & 3);
+          __nv_bfloat16* to = y + (size_t)t0 * N + w.f0 + c;
+          if (c < w.width) {                      // (whole: widths are multiples of 8)
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            __nv_bfloat162 o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = __floats2bfloat162_rn(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
-            *reinterpret_cast<uint4*>(out + c0 + c) = *reinterpret_cast<uint4*>(o);
+            for (int r = lane >> 2; r < 32; r += 8)
+              if (r < count) *reinterpret_cast<uint4*>(to + (size_t)r * N) = *reinterpret_cast<const uint4*>(turned + r * kTurnRow + 16 * (lane & 3));
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (c0 + c < w.width) out[c0 + c] = __float2bfloat16_rn(__uint_as_float(v[c]));
+        } else if (c0 + lane < w.width) {
+          unsigned short* to = reinterpret_cast<unsigned short*>(y) + (size_t)t0 * N + w.f0 + c0 + lane;
+#pragma unroll 8
+          for (int r = 0; r < count; ++r) to[(size_t)r * N] = *reinterpret_cast<const unsigned short*>(turned + r * kTurnRow + 2 * lane);
         }
       }
     }
@@ -969,10 +961,7 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
   const int f_tiles = feature_tiles(sl, BN);
   const long long n_tiles = (long long)f_tiles * ((rows + kAdM * ctas - 1) / (kAdM * ctas));
   NF_REQUIRE(n_tiles < (1ll << 30), "adapter_linear: %d rows of %d features are too many", rows, N);
-  bool whole = N % 8 == 0;
-  for (int i = 0; i < n_slices; ++i) whole = whole && ends[i] % 8 == 0;
-  const int turned = whole ? 0 : kWideEpilogueWarps * kTurnBytes;
-  int stages = (kWideSmem - kWideHead - wide_h_bytes(ctas) - turned) / (kAdTile + BN / ctas * 128);
+  int stages = (kWideSmem - kWideHead - wide_h_bytes(ctas) - kWideEpilogueWarps * kTurnBytes) / (kAdTile + BN / ctas * 128);
   stages = stages > kAdMaxStages ? kAdMaxStages : stages;
   static int asked1 = room_for(adapter_wide_kernel<1>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2>, kWideSmem + 1024);
   if (asked1 || asked2) return 1;
