@@ -143,6 +143,11 @@ struct TileIds {
       v[i] = a >= 0 && a < n ? a : -1;
     }
   }
+  // Leaves the adapters that are `turn` modulo `turns`.
+  __device__ __forceinline__ void keep(int turn, int turns) {
+#pragma unroll
+    for (int i = 0; i < 4 * CTAS; ++i) v[i] = v[i] >= 0 && v[i] % turns == turn ? v[i] : -1;
+  }
   __device__ __forceinline__ int next(int last) const {
     int m = kNone;
 #pragma unroll
@@ -173,7 +178,7 @@ struct __align__(8) ShrinkBars {
 // kernels may meet on an SM, from several streams too, has to find its columns at once.  One CTA of this kernel (256 columns, more
 // than half of the shared memory) beside those of adapter_rows_kernel (64 each, that split k 36 KB each) do; the wide kernel, and
 // all others that take all columns, leave no shared memory for either.
-constexpr size_t kShrinkSmemLeast = 120 * 1024;
+constexpr size_t kShrinkSmemLeast = 118 * 1024;
 constexpr int kShrinkCols = 256;        // columns of an accumulator: numbers of h of all adapters of a pass
 
 // Writes 8 numbers of h: as they are, or as the nearest bfloat16 and what that leaves, SR numbers behind one another.
@@ -199,7 +204,8 @@ __device__ __forceinline__ void put_h(float* h, int t, int SR, int j, const floa
 // D[t, (adapter, j)] over a tile of up to 128 rows: x is the 128-row operand, the rows of A of up to `group` of the adapters
 // that occur in the tile the other, so that x is read once for all of them.  The CTAs of a cluster split k; each sends every row's
 // own numbers to the member that owns the row, which adds them up in the members' order, scales and writes them.
-// 192 threads: producer, MMA, four epilogue warps (a thread a row).  grid: (members, row tiles * j tiles, groups in turn).
+// gridDim.z CTAs take the adapters of a tile in turn, by their number.
+// 192 threads: producer, MMA, four epilogue warps (a thread a row).  grid: (members, row tiles * j tiles, adapters in turn).
 __global__ void __launch_bounds__(192, 1)
 adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ scale,
                          const int* __restrict__ ids, float* __restrict__ h, int rows, int K, int SR, int n, int row_tiles, int x_box, int JW,
@@ -209,9 +215,10 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   ShrinkBars* bars = reinterpret_cast<ShrinkBars*>(smem);
   unsigned char* stage0 = smem + 1024;
   const int stage_bytes = kAdTile + group * JW * 128;
-  float* sums = reinterpret_cast<float*>(stage0 + (size_t)stages * stage_bytes);      // [members][share of rows][JW], written by all members
+  float* sums = reinterpret_cast<float*>(stage0 + (size_t)stages * stage_bytes);      // [members][share of rows][JW + 4], written by all members
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int members = gridDim.x, member = blockIdx.x, share = kAdM / members;          // (a power of two up to 8)
+  const int JP = JW + 4;              // numbers between two rows of sums: threads store rows side by side, no bank twice
   volatile int* stop = &bars->stop;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this member is there
   if (threadIdx.x == 0) {
@@ -236,6 +243,7 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   const int k_first = (int)((long long)member * steps / members), k_last = (int)((long long)(member + 1) * steps / members);
   TileIds<1> tids;
   tids.load(ids, row0, rows, n);
+  tids.keep(blockIdx.z, gridDim.z);
   // the next group of adapters: lane g holds the g-th; returns how many
   int last = -1;
   auto next_group = [&](int& mine) {
@@ -254,10 +262,9 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     int issued = 0, mine = 0;
     bool ok = true;
     Ring ring;
-    for (int turn = 0;; ++turn) {
+    for (;;) {
       const int count = next_group(mine);
       if (!count || !ok) break;
-      if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
       for (int ks = k_first; ks < k_last; ++ks, ring.next(stages), ++issued) {
         const int s = ring.s;
         if (!warp_wait(&bars->empty[s], ring.phase ^ 1, stop, 1)) { ok = false; break; }
@@ -282,10 +289,9 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     int done = 0, mine = 0;
     bool ok = true;
     Ring ring;
-    for (int turn = 0;; ++turn) {
+    for (;;) {
       const int count = next_group(mine);
       if (!count || !ok) break;
-      if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
       const unsigned idesc = ad_instr_desc(count * JW, kAdM);
       if (!warp_wait(&bars->acc_empty, (done & 1) ^ 1, stop, 2)) break;
       tc_fence_after();
@@ -309,12 +315,11 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const int quad = warp & 3, r = quad * 32 + lane, t = row0 + r;
     const int own = t < rows ? ids[t] : -1;
     int done = 0, mine = 0;
-    const unsigned to = cluster_addr(smem_u32(sums + ((size_t)member * share + r % share) * JW), r / share);
+    const unsigned to = cluster_addr(smem_u32(sums + ((size_t)member * share + r % share) * JP), r / share);
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // every member is there: its shared memory may be written
-    for (int turn = 0;; ++turn) {
+    for (;;) {
       const int count = next_group(mine);
       if (!count) break;
-      if (turn % (int)gridDim.z != (int)blockIdx.z) continue;
       if (!warp_wait(&bars->acc_full, done & 1, stop, 4)) break;
       tc_fence_after();
       for (int g = 0; g < count; ++g) {
@@ -351,7 +356,7 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int m = 0; m < members; ++m) {
       float u[8];
-      load8(sums + ((size_t)m * share + rl) * JW + j, u);
+      load8(sums + ((size_t)m * share + rl) * JP + j, u);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += u[e];
     }
@@ -371,7 +376,7 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 // ---- many rows -------------------------------------------------------------------------------------------------------------
 
 struct __align__(8) WideBars {
-  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full[4], h_empty[4];
+  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full[4], h_peer[4], h_empty[4];
   unsigned tmem_base;
   int stop;
 };
@@ -433,7 +438,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       mbar_init(&bars->acc_full[b], 1);
       mbar_init(&bars->acc_empty[b], kWideEpilogueWarps * CTAS);
     }
-    for (int b = 0; b < 4; ++b) { mbar_init(&bars->h_full[b], 4 * CTAS); mbar_init(&bars->h_empty[b], 1); }
+    for (int b = 0; b < 4; ++b) { mbar_init(&bars->h_full[b], 4); mbar_init(&bars->h_peer[b], 1); mbar_init(&bars->h_empty[b], 1); }
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -521,7 +526,8 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
           const unsigned long long db = smem_desc(stage0 + (size_t)ring.s * stage_bytes + kAdTile);
           for (int part = 0; part < h_parts; ++part, hring.next(h_bufs)) {
-            if (!warp_wait_cluster(&bars->h_full[hring.s], hring.phase, stop, 5)) { ok = false; break; }
+            if (!warp_wait(&bars->h_full[hring.s], hring.phase, stop, 5) ||
+                (CTAS == 2 && !warp_wait_cluster(&bars->h_peer[hring.s], hring.phase, stop, 5))) { ok = false; break; }
             tc_fence_after();
             const unsigned long long dh = smem_desc(h_tile + hring.s * kAdTile);
             if (elect_one()) {
@@ -538,6 +544,22 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
       if (ok && elect_one()) commit<CTAS>(&bars->acc_full[ab]);
       __syncwarp();
+    }
+  } else if (CTAS == 2 && warp == 1) {
+    // ---- the odd CTA's rows of h, passed on to the even one.  (Arriving there, with what was written before, takes a thread a thousand
+    // cycles: four warps that write the next rows meanwhile do not wait for it.  777 rows of 2048 x 11264 with 12 adapters of
+    // rank 64 in the first tile 61 -> 59.5 us, 244 of 128 x 3743 with 34 of rank 16 41 -> 36.)
+    bool ok = true;
+    Ring hring;
+    for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride)) {
+      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
+      tids.load(ids, w.row0, rows, n);
+      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a))
+        for (int e = 0; e < r_steps * h_parts; ++e, hring.next(h_bufs)) {
+          if (!warp_wait(&bars->h_full[hring.s], hring.phase, stop, 7)) { ok = false; break; }
+          if (elect_one()) arrive_leader<CTAS>(&bars->h_peer[hring.s]);
+          __syncwarp();
+        }
     }
   } else if (warp >= 2 && warp < 6) {
     // ---- rows of h: this thread's row of the tile, in the operand's swizzled image; zeros for another adapter ---------------
@@ -579,7 +601,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
               }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) arrive_leader<CTAS>(&bars->h_full[hring.s]);
+            if (lane == 0) mbar_arrive(&bars->h_full[hring.s]);
           }
         }
       }
@@ -851,6 +873,8 @@ template <typename F>
 int room_for(F* kernel, size_t smem) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   NF_REQUIRE(e == cudaSuccess, "adapter_linear: cannot have %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+  // An SM that runs one kernel with a part of its memory as shared memory takes no CTA of the next one that needs more.
+  cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   return 0;
 }
 
@@ -900,21 +924,23 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     const int members = shrink_members(rows, K, SR);
     const int JW = SR < kAdM ? SR : kAdM, j_tiles = (SR + JW - 1) / JW;
     const int most = n < kAdM ? (n < rows ? n : rows) : (rows < kAdM ? rows : kAdM);      // adapters that a tile's rows may have
-    const int group = kShrinkCols / JW < most ? kShrinkCols / JW : most;
+    // CTAs that take a tile's adapters in turn.  Behind few rows comes a product that streams W: a third of the SMs is enough for what
+    // it would otherwise wait for (64 rows of 3584 x 3584, 48 adapters of rank 32: on all of them 24.7 us, on a third 22.5).
+    const bool few = rows <= kRowsMost;
+    int turns = sm_count() / (members * row_tiles * j_tiles * (few ? 3 : 1));
+    turns = turns < 1 ? 1 : turns > most ? most : turns;
+    const int each = (most + turns - 1) / turns, group = kShrinkCols / JW < each ? kShrinkCols / JW : each;
     const int x_box = rows >= kAdM ? kAdM : (rows + 7) & ~7;
     CUtensorMap ma, mx;
     if (int rc = make_map(&ma, A, (long long)n * SR, K, JW)) return rc;
     if (int rc = make_map(&mx, x, rows, K, x_box)) return rc;
-    const int stage = kAdTile + group * JW * 128, sums = kAdM * JW * 4;
-    int stages = (200 * 1024 - sums) / stage;
-    stages = stages > 8 ? 8 : stages;
+    const int stage = kAdTile + group * JW * 128, sums = kAdM * (JW + 4) * 4;
+    int stages = ((few ? (int)kShrinkSmemLeast - 2048 : 200 * 1024) - sums) / stage;
+    stages = stages > 8 ? 8 : stages < 2 ? 2 : stages;
     size_t smem = 2048 + (size_t)stages * stage + sums;
     smem = smem < kShrinkSmemLeast ? kShrinkSmemLeast : smem;
     static int asked = room_for(adapter_shrink_tc_kernel, 204 * 1024);
     if (asked) return asked;
-    const int passes = (most + group - 1) / group;
-    int turns = sm_count() / (members * row_tiles * j_tiles);          // CTAs that take a tile's groups of adapters in turn
-    turns = turns < 1 ? 1 : turns > passes ? passes : turns;
     NF_REQUIRE(row_tiles * j_tiles <= 65535, "adapter_linear: %d rows are too many", rows);
     launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, row_tiles * j_tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
                            ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, rows > kRowsMost ? 1 : 0);
@@ -975,7 +1001,7 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
   return check_launch("adapter_wide");
 }
 
-// 0, or the code of the first wait that one of these kernels gave up on since the last call (1 to 6 the wide form and the
+// 0, or the code of the first wait that one of these kernels gave up on since the last call (1 to 7 the wide form and the
 // first product, 11 to 14 the form for few rows); 100 + 1 + a row whose adapter lay outside the pool.  Synchronises.
 extern "C" int nf_adapter_tc_status() {
   int v[2] = {0, 0}, zero = 0;
