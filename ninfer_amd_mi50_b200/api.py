@@ -29,7 +29,7 @@ from .config.engine_options import EngineOptions
 from .engine.batch import StepEntry
 from .engine.engine import Engine
 from .sampling.params import SamplingParams
-from .sampling.sampler import sample_reference, uniform_draw
+from .sampling.sampler import check_rules, sample_reference, uniform_draw
 
 
 class NinferError(RuntimeError):
@@ -39,8 +39,9 @@ class NinferError(RuntimeError):
 class Session:
     """One request's place in the cache: a state slot, pages, a length."""
 
-    def __init__(self, engine: "Ninfer", key: int):
+    def __init__(self, engine: "Ninfer", key: int, adapter: Optional[str] = None):
         self._engine, self._key = engine, key
+        self._adapter = engine._engine.adapter_slot(adapter)
         self._open = True
         engine._runner.open(key)
 
@@ -79,11 +80,11 @@ class Session:
         for i in range(0, len(tokens), chunk):
             part = list(tokens[i:i + chunk])
             last = i + chunk >= len(tokens)
-            out = self._engine._runner.step([StepEntry(self._key, part, [len(part) - 1] if last else [])])
+            out = self._engine._runner.step([StepEntry(self._key, part, [len(part) - 1] if last else [], self._adapter)])
         return out[0].cpu().numpy()
 
     def decode(self, token: int) -> np.ndarray:
-        return self._engine._runner.step([StepEntry(self._key, [int(token)], [0])])[0].cpu().numpy()
+        return self._engine._runner.step([StepEntry(self._key, [int(token)], [0], self._adapter)])[0].cpu().numpy()
 
     def close(self) -> None:
         if self._open:
@@ -96,13 +97,13 @@ class Ninfer:
                  prefill_chunk: int = 2048, num_sequences: int = 1, *, dtype: str = "bfloat16",
                  page_size: int = 64, cache_tokens: Optional[int] = None,
                  max_batched_tokens: Optional[int] = None, use_graph: bool = True,
-                 run_ahead: bool = True,
+                 run_ahead: bool = True, adapters: int = 0, adapter_rank: int = 16,
                  config: Optional[Dict[str, Any]] = None, random_weights: Optional[int] = None,
                  device: str = "cuda:0"):
         opts = EngineOptions(dtype=dtype, max_context=max_context, prefill_chunk=prefill_chunk,
                              num_sequences=num_sequences, page_size=page_size, cache_tokens=cache_tokens,
                              max_batched_tokens=max_batched_tokens, use_graph=use_graph, run_ahead=run_ahead,
-                             device=device)
+                             adapters=adapters, adapter_rank=adapter_rank, device=device)
         self._engine = Engine(model_dir, config=config, random_seed=random_weights, options=opts)
         self._runner = self._engine.runner
         self.vocab = self._engine.vocab_size
@@ -151,10 +152,19 @@ class Ninfer:
     def detokenize(self, ids: Sequence[int]) -> str:
         return self._tok().decode(ids)
 
+    # ---- adapters ----
+    def load_adapter(self, name: str, weights, scale: float = 1.0) -> None:
+        """Load a low-rank adapter: names of the checkpoint's tensors -> (A [r, in], B [out, r]), or the path of a folder
+        with ``adapter_config.json`` and ``adapter_model.safetensors``."""
+        self._engine.load_adapter(name, weights, scale)
+
+    def drop_adapter(self, name: str) -> None:
+        self._engine.drop_adapter(name)
+
     # ---- sessions ----
-    def session(self) -> Session:
+    def session(self, adapter: Optional[str] = None) -> Session:
         try:
-            return Session(self, ("session", next(self._keys)))
+            return Session(self, ("session", next(self._keys)), adapter)
         except Exception as e:
             raise NinferError(f"session: {e}") from None
 
@@ -162,34 +172,40 @@ class Ninfer:
         """One step for N live requests, one token each -> logits [N, vocab]."""
         if len(sessions) != len(tokens):
             raise NinferError("decode_batch: sessions and tokens differ in length")
-        out = self._runner.step([StepEntry(s._key, [int(t)], [0]) for s, t in zip(sessions, tokens)])
+        out = self._runner.step([StepEntry(s._key, [int(t)], [0], s._adapter) for s, t in zip(sessions, tokens)])
         return out.cpu().numpy()
 
     def step(self, entries: Sequence[tuple]) -> np.ndarray:
         """A mixed batch: ``(session, tokens, want)`` triples -> logits [wanted rows, vocab]."""
-        out = self._runner.step([StepEntry(s._key, list(t), list(w)) for s, t, w in entries])
+        out = self._runner.step([StepEntry(s._key, list(t), list(w), s._adapter) for s, t, w in entries])
         return out.cpu().numpy()
 
     # ---- sampling (ninfer_sample, ninfer_c_api.cpp:248-260) ----
     def sample(self, logits, temperature: float = 0.7, top_k: int = 50, top_p: float = 0.95,
-               repetition_penalty: float = 1.0, seed: int = 0, recent: Sequence[int] = ()) -> int:
-        p = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed)
-        return sample_reference(np.asarray(logits, dtype=np.float32), p, recent, uniform_draw(seed, 0))
+               repetition_penalty: float = 1.0, seed: int = 0, recent: Sequence[int] = (), prompt_length: int = 0,
+               **rules) -> int:
+        """`rules`: frequency_penalty, presence_penalty, logit_bias, allowed_tokens, as in `SamplingParams`;
+        `recent[prompt_length:]` are the generated ids."""
+        p = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, **rules)
+        check_rules(p, self.vocab)
+        return sample_reference(np.asarray(logits, dtype=np.float32), p, recent, uniform_draw(seed, 0), prompt_length)
 
     # ---- whole generations through the scheduler ----
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 512,
                  temperature: float = 0.7, top_k: int = 50, top_p: float = 0.95,
                  repetition_penalty: float = 1.0, seed: int = 0,
-                 stop_ids: Iterable[int] = ()) -> List[List[int]]:
-        p = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, max_new_tokens)
-        return self._engine.generate(prompts, p, stop_ids)
+                 stop_ids: Iterable[int] = (), adapter=None, **rules) -> List[List[int]]:
+        """`adapter`: the name of a loaded adapter, or a name (or None) for each prompt; `rules`: frequency_penalty,
+        presence_penalty, logit_bias, allowed_tokens, as in `SamplingParams`."""
+        p = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, max_new_tokens, **rules)
+        return self._engine.generate(prompts, p, stop_ids, adapter)
 
     def stream(self, prompt: Sequence[int], max_new_tokens: int = 512, temperature: float = 0.7,
                top_k: int = 50, top_p: float = 0.95, repetition_penalty: float = 1.0, seed: int = 0,
-               stop_ids: Iterable[int] = ()):
+               stop_ids: Iterable[int] = (), adapter: Optional[str] = None, **rules):
         """Token ids of one generation, each as soon as it exists."""
-        p = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, max_new_tokens)
-        return self._engine.stream(prompt, p, stop_ids)
+        p = SamplingParams(temperature, top_k, top_p, repetition_penalty, seed, max_new_tokens, **rules)
+        return self._engine.stream(prompt, p, stop_ids, adapter)
 
     def close(self) -> None:
         self._engine = None

@@ -47,6 +47,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", type=int, default=50)
     ap.add_argument("--top-p", type=float, default=0.95, help="nucleus probability")
     ap.add_argument("--repeat-penalty", type=float, default=1.05, help="repetition penalty")
+    ap.add_argument("--frequency-penalty", type=float, default=0.0, help="taken from a logit for every time its token was generated")
+    ap.add_argument("--presence-penalty", type=float, default=0.0, help="taken from the logits of tokens that were generated")
+    ap.add_argument("--adapter", metavar="DIR", help="a low-rank adapter to generate with (adapter_config.json, adapter_model.safetensors)")
+    ap.add_argument("--adapter-rank", type=int, default=64, help="largest rank that there is room for with --adapter")
     ap.add_argument("--seed", type=int, default=0, help="sampling seed (0 = 1234 for a one-shot run)")
     ap.add_argument("--graph", action="store_true", default=True, help="CUDA-graph decode (default on)")
     ap.add_argument("--no-graph", dest="graph", action="store_false")
@@ -119,9 +123,16 @@ def main(argv=None, stdin=None, stdout=None) -> int:
                  prefill_chunk=args.prefill_chunk, num_sequences=n_seq, dtype=args.dtype,
                  page_size=args.page_size, cache_tokens=args.cache_tokens,
                  max_batched_tokens=args.max_batched_tokens, use_graph=args.graph,
-                 random_weights=args.random_weights, device=args.device)
+                 random_weights=args.random_weights, device=args.device, adapters=1 if args.adapter else 0,
+                 adapter_rank=args.adapter_rank)
+    if args.adapter:
+        eng.load_adapter("adapter", args.adapter)
     sampling = dict(max_new_tokens=args.max_new, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                     repetition_penalty=args.repeat_penalty)
+    # (named only where given: a caller's engine need not know them)
+    sampling.update({k: v for k, v in (("frequency_penalty", args.frequency_penalty), ("presence_penalty", args.presence_penalty)) if v})
+    if args.adapter:
+        sampling["adapter"] = "adapter"
 
     def say(ids: List[int], seed: int) -> str:
         """One generation from text-derived ids, printed as it comes; returns the answer."""

@@ -30,6 +30,8 @@ class EngineOptions:
     run_ahead: bool = True           # launch the next decode step before reading this one's tokens
     status_every: int = 64           # decode steps between two reads of the kernels' status flags
     clear_reused_pages: bool = True  # zero a cache page when it is handed out a second time
+    adapters: int = 0                # low-rank adapters that requests may choose from, at most; 0: none
+    adapter_rank: int = 16           # largest rank of one (pools are laid out for the next of 16, 32, 64, 128)
     device: str = "cuda:0"
 
     def __post_init__(self) -> None:
@@ -50,6 +52,8 @@ class EngineOptions:
             self.cache_tokens = self.num_sequences * self.pages_for(self.max_context) * self.page_size
         if self.max_batched_tokens is None:
             self.max_batched_tokens = max(self.prefill_chunk, self.num_sequences)
+        if self.adapters < 0:
+            raise ValueError("adapters must not be negative")
         if self.max_batched_tokens < 1:
             raise ValueError("max_batched_tokens must be at least 1")
 

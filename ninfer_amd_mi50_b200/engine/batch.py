@@ -25,6 +25,7 @@ class StepEntry:
     req: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = ()      # indices into `tokens` whose logits are asked for
+    adapter: int = -1             # slot of the request's adapter, -1: none
 
 
 class BatchError(ValueError):
@@ -61,9 +62,10 @@ def validate_entries(entries: Sequence[StepEntry], cache: CacheManager, vocab_si
 
 def pack_step(entries: Sequence[StepEntry], cache: CacheManager, dtype: torch.dtype,
               device: torch.device, *, table_width: Optional[int] = None,
-              arrays: Optional[Sequence[np.ndarray]] = None) -> StepContext:
+              arrays: Optional[Sequence[np.ndarray]] = None, adapted: bool = False) -> StepContext:
     """Build the step's metadata.  Pages for the new tokens must be reserved already.  `arrays`: the entries' tokens
-    as `validate_entries` returned them (a list of thousands is turned into an array once a step)."""
+    as `validate_entries` returned them (a list of thousands is turned into an array once a step).  `adapted`: some entry has
+    an adapter, the rows' slots go along."""
     S = len(entries)
     # numpy pieces, not Python lists: a 2,048-token portion was 0.85 ms of list building here
     pieces_tok, pieces_pos, pieces_seg = [], [], []
@@ -97,10 +99,12 @@ def pack_step(entries: Sequence[StepEntry], cache: CacheManager, dtype: torch.dt
             tbl = np.pad(tbl, ((0, 0), (0, width - tbl.shape[1])), constant_values=-1)
         tables.append((g.index, width, tbl.reshape(-1)))
     sizes = [T, T, T, S + 1, S, S, len(logit_rows)] + [S * w for _, w, _ in tables]
+    slots = [np.repeat(np.asarray([e.adapter for e in entries], dtype=np.int32), seg_len)] if adapted else []
+    sizes += [T] * len(slots)
     small = lambda v: np.asarray(v, dtype=np.int32)
     flat_all = np.concatenate(pieces_tok + pieces_pos + pieces_seg +
                               [small(seg_row0), small(seg_pos0), small(seg_slot), small(logit_rows)] +
-                              [f for _, _, f in tables])
+                              [f for _, _, f in tables] + slots)
     buf = torch.from_numpy(flat_all)
     host_bytes = buf.numel() * 4
     if device.type == "cuda":
@@ -114,6 +118,8 @@ def pack_step(entries: Sequence[StepEntry], cache: CacheManager, dtype: torch.dt
         max_rows_per_seg=max(seg_len) if seg_len else 0,
         max_context=max((p + n for p, n in zip(seg_pos0, seg_len)), default=0))
     ctx.scratch["h2d_bytes"] = host_bytes
+    if adapted:
+        ctx.row_adapter = parts.pop()
     for (gi, width, _), t in zip(tables, parts[7:]):
         ctx.block_tables[gi] = t.view(S, width)
     return ctx

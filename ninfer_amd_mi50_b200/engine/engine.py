@@ -13,7 +13,7 @@ import torch
 
 from ..config.engine_options import EngineOptions
 from ..sampling.params import SamplingParams
-from ..sampling.sampler import Sampler, check_params
+from ..sampling.sampler import Sampler, check_allowed, check_params
 from .loading import load_runner
 from .scheduler import Request, Scheduler
 
@@ -42,8 +42,11 @@ class Engine:
 
     # ---- requests ---------------------------------------------------------------------
     def submit(self, prompt: Sequence[int], params: Optional[SamplingParams] = None,
-               stop_ids: Iterable[int] = (), request_id: Optional[Hashable] = None) -> Hashable:
+               stop_ids: Iterable[int] = (), request_id: Optional[Hashable] = None,
+               adapter: Optional[str] = None) -> Hashable:
+        """Queue a request; `adapter`: the name of a loaded adapter that it is served with."""
         params = params or SamplingParams()
+        slot = self.adapter_slot(adapter)
         check_params(params, self.vocab_size)
         for t in prompt:
             if not 0 <= int(t) < self.vocab_size:
@@ -55,10 +58,36 @@ class Engine:
         rid = request_id if request_id is not None else f"req-{next(self._ids)}"
         if rid in self.requests and self.requests[rid].status != "finished":
             raise ValueError(f"request id {rid!r} is in use")
-        req = Request(rid, [int(t) for t in prompt], params, set(int(s) for s in stop_ids))
+        req = Request(rid, [int(t) for t in prompt], params, set(int(s) for s in stop_ids), adapter=slot)
         self.scheduler.add(req)
         self.requests[rid] = req
         return rid
+
+    # ---- adapters ---------------------------------------------------------------------
+    def adapter_slot(self, name: Optional[str]) -> int:
+        if name is not None and self.runner.adapters is None:
+            raise ValueError("this engine keeps no adapters (EngineOptions.adapters)")
+        return self.runner.adapters.slot(name) if name is not None else -1
+
+    def load_adapter(self, name: str, weights, scale: float = 1.0) -> None:
+        """Load a low-rank adapter that requests can then name: `weights` maps names of the checkpoint's tensors to
+        (A [r, in], B [out, r]), or is the path of a folder as `weights.read_adapter` takes it (`scale` multiplies the
+        folder's own)."""
+        if self.runner.adapters is None:
+            raise ValueError("this engine keeps no adapters (EngineOptions.adapters)")
+        if isinstance(weights, str):
+            from ..weights import read_adapter
+            weights, own = read_adapter(weights)
+            scale = scale * own
+        self.runner.adapters.load(name, weights, scale)
+
+    def drop_adapter(self, name: str) -> None:
+        """Give an adapter's slot back.  Refused while a request that names it is not finished."""
+        slot = self.adapter_slot(name)
+        users = [r.id for r in self.requests.values() if r.adapter == slot and r.status != "finished"]
+        if users:
+            raise ValueError(f"adapter {name!r} is in use by {users}")
+        self.runner.adapters.drop(name)
 
     # ---- stepping ---------------------------------------------------------------------
     def step(self) -> List[Request]:
@@ -80,8 +109,14 @@ class Engine:
             done = list(self.scheduler.finished[before:])      # finished without running (out of cache)
             if not batch:
                 return done
+            try:
+                allowed = self._allowed(batch)          # (a caller's function: before anything has run)
+            except Exception:
+                for s in batch:
+                    self.cache.truncate(s.request.id)
+                raise
             logits = self.runner.step(self.scheduler.entries(batch))
-            picked = self._sample(batch, logits, ahead=False)
+            picked = self._sample(batch, logits, ahead=False, allowed=allowed)
         tokens: List[int] = []
         if picked is not None:
             landing = self._start_readback(picked)
@@ -90,7 +125,28 @@ class Engine:
             tokens = self._finish_readback(landing)
             self.d2h_bytes += picked.numel() * 4
         self._check_kernels(batch)
-        return done + self.scheduler.update(batch, tokens)
+        ended = done + self.scheduler.update(batch, tokens)
+        for req in ended:
+            self.sampler.forget(req.id)
+        return ended
+
+    def _allowed(self, batch) -> Optional[List[Optional[Sequence[int]]]]:
+        """The tokens that may follow, for each request of the batch that samples; None where there is no such rule.  A
+        request that nothing may follow ends with this step."""
+        sampling = [s.request for s in batch if s.sample]
+        if all(r.params.allowed_tokens is None for r in sampling):
+            return None
+        out: List[Optional[Sequence[int]]] = []
+        for r in sampling:
+            r.ended = False
+            ids = r.params.allowed(r.generated)
+            if ids is not None and callable(r.params.allowed_tokens):
+                ids = [int(t) for t in ids]
+                check_allowed(ids, self.vocab_size)
+                if not ids:
+                    r.ended, ids = True, None
+            out.append(ids)
+        return out
 
     def _check_kernels(self, batch) -> None:
         """Read the kernels' status flags (a bounded wait that ran out, an index outside its
@@ -138,7 +194,8 @@ class Engine:
             landed.synchronize()
         return host.tolist()
 
-    def _sample(self, batch, logits: torch.Tensor, ahead: bool) -> Optional[torch.Tensor]:
+    def _sample(self, batch, logits: torch.Tensor, ahead: bool,
+                allowed: Optional[List[Optional[Sequence[int]]]] = None) -> Optional[torch.Tensor]:
         sampling = [s for s in batch if s.sample]
         if not sampling:
             return None
@@ -147,7 +204,8 @@ class Engine:
         return self.sampler.sample(
             logits, [s.request.params for s in sampling],
             recent=[s.request.tokens for s in sampling],
-            counters=[len(s.request.generated) + extra for s in sampling])
+            counters=[len(s.request.generated) + extra for s in sampling],
+            prompt_lengths=[len(s.request.prompt) for s in sampling], keys=[s.request.id for s in sampling], allowed=allowed)
 
     def _launch_ahead(self, batch, picked: torch.Tensor):
         """Launch the step after `batch` on the tokens in `picked` (still on the device), if the
@@ -180,20 +238,24 @@ class Engine:
 
     def generate(self, prompts: Sequence[Sequence[int]],
                  params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
-                 stop_ids: Iterable[int] = ()) -> List[List[int]]:
-        """Generate for every prompt (token ids in, token ids out), batched by the scheduler."""
+                 stop_ids: Iterable[int] = (), adapter: Union[str, Sequence[Optional[str]], None] = None) -> List[List[int]]:
+        """Generate for every prompt (token ids in, token ids out), batched by the scheduler.  `adapter`: the name of an
+        adapter for all prompts, or a name (or None) for each."""
         if params is None or isinstance(params, SamplingParams):
             params = [params or SamplingParams()] * len(prompts)
-        ids = [self.submit(p, sp, stop_ids) for p, sp in zip(prompts, params)]
+        adapters = [adapter] * len(prompts) if adapter is None or isinstance(adapter, str) else list(adapter)
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(prompts)} prompts, {len(adapters)} adapters")
+        ids = [self.submit(p, sp, stop_ids, adapter=a) for p, sp, a in zip(prompts, params, adapters)]
         self.run_until_idle()
         return [list(self.requests[i].generated) for i in ids]
 
     def stream(self, prompt: Sequence[int], params: Optional[SamplingParams] = None,
-               stop_ids: Iterable[int] = ()):
+               stop_ids: Iterable[int] = (), adapter: Optional[str] = None):
         """Generate for one prompt and yield each token id as soon as its step has been read
         back (the reference's CLI prints text as it comes, src/apps/ninfer.cpp:121-138).  Other
         requests that are live meanwhile keep running in the same steps."""
-        rid = self.submit(prompt, params, stop_ids)
+        rid = self.submit(prompt, params, stop_ids, adapter=adapter)
         req = self.requests[rid]
         sent = 0
         while True:

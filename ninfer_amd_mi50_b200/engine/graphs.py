@@ -91,12 +91,13 @@ class Staging:
 
 
 class DecodeGraph:
-    def __init__(self, runner, staging: Staging, rows: int, context_bound: int):
+    def __init__(self, runner, staging: Staging, rows: int, context_bound: int, adapted: bool = False):
         self.runner, self.staging, self.S, self.context_bound = runner, staging, rows, context_bound
         cache, dev = runner.cache, runner.device
         S = rows
         self.width = cache.max_pages_per_request
-        sizes = [S, S, S, S + 1, S, S, S] + [S * self.width for _ in cache.groups]
+        self.adapted = adapted               # rows have adapters: their slots are the last index data
+        sizes = [S, S, S, S + 1, S, S, S] + [S * self.width for _ in cache.groups] + [S] * adapted
         self.offsets = np.cumsum([0] + sizes).tolist()
         total = self.offsets[-1]
         self.dev = torch.zeros((total,), dtype=torch.int32, device=dev)
@@ -105,7 +106,7 @@ class DecodeGraph:
             dtype=runner.dtype, device=dev, T=S, S=S, token_ids=parts[0], positions=parts[1],
             row_seg=parts[2], seg_row0=parts[3], seg_pos0=parts[4], seg_slot=parts[5],
             logit_rows=parts[6], seg_len_host=[1] * S, seg_pos0_host=None, max_rows_per_seg=1,
-            max_context=context_bound, graph_mode=True)
+            max_context=context_bound, graph_mode=True, row_adapter=parts[-1] if adapted else None)
         for gi, g in enumerate(cache.groups):
             self.ctx.block_tables[g.index] = parts[7 + gi].view(S, self.width)
         # a row is its own segment, and its logits are wanted: row_seg, seg_row0 and logit_rows of every step
@@ -159,6 +160,9 @@ class DecodeGraph:
                 tbl[:n] = cache.block_rows(g.index, slots, self.width)
             tbl[n:, 0] = g.null_page
             tbl[n:, 1:] = -1
+        if self.adapted:
+            a[o[-2]:o[-2] + n] = [e.adapter for e in entries]
+            a[o[-2] + n:o[-1]] = -1
 
     def run(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Pages for the new tokens are reserved already.  Returns logits [S, vocab] that stay
@@ -182,7 +186,7 @@ class DecodeGraphs:
     def __init__(self, runner, max_rows: int):
         self.runner, self.max_rows = runner, max_rows
         self.staging = Staging()
-        self.graphs: Dict[Tuple[int, int], DecodeGraph] = {}
+        self.graphs: Dict[Tuple[int, ...], DecodeGraph] = {}      # by rows, context bound, and whether rows have adapters
 
     def eligible(self, entries: Sequence[StepEntry]) -> bool:
         return 0 < len(entries) <= self.max_rows and all(len(e.tokens) == 1 for e in entries)
@@ -191,7 +195,9 @@ class DecodeGraphs:
         cache = self.runner.cache
         rows = row_bucket(len(entries))
         longest = max(cache.length(e.req) for e in entries) + 1
-        key = (rows, context_bucket(longest, cache.max_context))
+        key: Tuple[int, ...] = (rows, context_bucket(longest, cache.max_context))
+        if any(e.adapter >= 0 for e in entries):
+            key += (True,)
         if key not in self.graphs:
             self.graphs[key] = DecodeGraph(self.runner, self.staging, *key)
         return self.graphs[key]

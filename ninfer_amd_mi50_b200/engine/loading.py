@@ -15,6 +15,7 @@ from .. import log
 from ..cache.manager import CacheManager
 from ..config.engine_options import EngineOptions
 from ..config.model_config import read_config_json
+from ..parts.adapters import AdapterBank
 from ..parts.model import DecoderModel
 from ..registry import architecture_of
 from ..weights.loader import ENGINE_DTYPES, CheckpointSource, RandomSource, load_model
@@ -54,6 +55,9 @@ def load_runner(model_dir: Optional[str] = None, *, config: Optional[Dict[str, A
                          max_context=options.max_context, dtype=dtype, device=device,
                          clear_reused_pages=options.clear_reused_pages)
     runner = ModelRunner(model, cache, dtype, device, use_graph=options.use_graph)
+    if options.adapters > 0:
+        runner.adapters = AdapterBank(model, options.adapters, options.adapter_rank, dtype, device)
+        log.info(f"room for {options.adapters} adapters of rank {runner.adapters.rank}: {runner.adapters.nbytes() / 2**20:.1f} MiB")
     runner.config = typed
     runner.options = options
     log.info(f"ready: weights {model.weight_bytes() / 2**20:.1f} MiB, cache "

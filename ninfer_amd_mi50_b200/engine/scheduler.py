@@ -37,6 +37,8 @@ class Request:
     finish_reason: Optional[str] = None  # length | stop | context | out_of_cache
     preemptions: int = 0
     computed: int = 0                    # tokens of (prompt + generated) that are in the cache
+    adapter: int = -1                    # slot of its adapter, -1: none
+    ended: bool = False                  # no token may follow: the one that this step draws is dropped
 
     @property
     def tokens(self) -> List[int]:
@@ -145,7 +147,7 @@ class Scheduler:
         to receive - decided before that token is known, so that the next step can be launched
         while the host still waits for this one.  Only when nothing else could be in that
         batch: every running request decodes in `batch`, nobody waits, no request's sampling
-        looks at earlier tokens (repetition penalty).  Requests that will finish by length or
+        looks at earlier tokens (penalties, a function that says which tokens may follow).  Requests that will finish by length or
         context with the coming token are left out; a request that stops on a stop token after
         all has run one token for nothing, which `update` is told to ignore.  Holds the pages
         of the returned batch; returns None (holding nothing) if running ahead is not possible.
@@ -157,7 +159,7 @@ class Scheduler:
             req = s.request
             if not s.sample or len(s.tokens) != 1 or req.status != "running" or req.remaining != 1:
                 return None
-            if req.params.repetition_penalty != 1.0:
+            if req.params.looks_back:
                 return None
             after = len(req.generated) + 1                       # generated tokens once this step's is in
             if after >= req.params.max_new_tokens or len(req.prompt) + after >= self.max_context:
@@ -234,7 +236,7 @@ class Scheduler:
     @staticmethod
     def entries(batch: Sequence[Scheduled]) -> List[StepEntry]:
         """The batch as step entries: logits are wanted at the last row of portions that sample."""
-        return [StepEntry(s.request.id, s.tokens, [len(s.tokens) - 1] if s.sample else [])
+        return [StepEntry(s.request.id, s.tokens, [len(s.tokens) - 1] if s.sample else [], s.request.adapter)
                 for s in batch]
 
     # ---- after the step ----------------------------------------------------------------
@@ -259,6 +261,10 @@ class Scheduler:
             if not s.sample:
                 continue
             tok = int(next(it))
+            if req.ended:
+                self._finish(req, "stop")
+                done.append(req)
+                continue
             req.generated.append(tok)
             reason = None
             if tok in req.stop_ids:

@@ -26,6 +26,7 @@ class ModelRunner:
         self.model, self.cache, self.dtype = model, cache, dtype
         self.device = torch.device(device)
         self.graphs = None
+        self.adapters = None          # the bank of adapters, where the engine keeps one
         if use_graph and self.device.type == "cuda" and model.graph_safe:
             from .graphs import DecodeGraphs
             self.graphs = DecodeGraphs(self, cache.max_requests)
@@ -63,6 +64,12 @@ class ModelRunner:
         if not entries:
             return torch.empty((0, self.model.vocab_size), dtype=torch.float32, device=self.device)
         arrays = validate_entries(entries, self.cache, self.model.vocab_size)
+        adapted = False
+        for e in entries:
+            if e.adapter != -1:
+                if self.adapters is None or e.adapter not in self.adapters.slots.values():
+                    raise BatchError(f"request {e.req!r}: no adapter in slot {e.adapter}")
+                adapted = True
         self.reserve(entries)
         try:
             if self.graphs is not None and self.graphs.eligible(entries):
@@ -70,7 +77,7 @@ class ModelRunner:
             elif device_tokens is not None:
                 raise ValueError("token ids on the device can only feed a step that is replayed from a graph")
             else:
-                ctx = pack_step(entries, self.cache, self.dtype, self.device, arrays=arrays)
+                ctx = pack_step(entries, self.cache, self.dtype, self.device, arrays=arrays, adapted=adapted)
                 logits, moved = self.run(ctx), ctx.scratch.get("h2d_bytes", 0)
         except Exception:
             for e in entries:

@@ -20,6 +20,7 @@ import torch
 from .. import kernels
 from ..config.model_config import PartSpec
 from ..registry import build_part, register_part
+from .adapters import Projection
 from .base import CacheSpec, CacheView, Fetch, Mixer, StepContext, TensorSpec
 
 
@@ -66,6 +67,12 @@ class PagedGqaAttention(Mixer):
         n = self.w_qkv.numel() * self.w_qkv.element_size() + self.w_o.numel() * self.w_o.element_size()
         return n + (self.b_qkv.numel() * 4 if self.b_qkv is not None else 0)
 
+    def projections(self):
+        p = self.prefix
+        return {"qkv": Projection((p + "q_proj.weight", p + "k_proj.weight", p + "v_proj.weight"),
+                                  (self.q_width, self.kv_width, self.kv_width), self.hidden_size),
+                "o": Projection((p + "o_proj.weight",), (self.hidden_size,), self.q_width)}
+
     # ---- cache ------------------------------------------------------------------------
     def cache_spec(self) -> CacheSpec:
         kind = "window" if self.window else "full"
@@ -83,7 +90,7 @@ class PagedGqaAttention(Mixer):
         bias = self.b_qkv
         if table is None:
             # an encoding that is not a half-split rotation: bias first, then its own hook
-            qkv = kernels.linear(x, self.w_qkv)
+            qkv = self.project("qkv", x, self.w_qkv, ctx)
             if bias is not None:
                 qkv.add_(bias.to(qkv.dtype))
                 bias = None
@@ -91,6 +98,12 @@ class PagedGqaAttention(Mixer):
             k = qkv[:, self.q_width:self.q_width + self.kv_width].unflatten(1, (Hkv, D))
             self.position.apply(q, k, ctx.positions)
             kernels.rope_append(qkv, None, ctx.positions, ctx.row_seg, None, 0, Hq, Hkv, D,
+                                cache.pages, cache.block_table, cache.page_size, cache.append)
+        elif self.adapter_pool("qkv", ctx) is not None:
+            # the adapters' part comes before the rotation
+            inv_freq, rot = table
+            qkv = self.project("qkv", x, self.w_qkv, ctx)
+            kernels.rope_append(qkv, bias, ctx.positions, ctx.row_seg, inv_freq, rot, Hq, Hkv, D,
                                 cache.pages, cache.block_table, cache.page_size, cache.append)
         else:
             # projection, bias, rotation and the write of k, v at (request, position): one kernel
@@ -101,4 +114,4 @@ class PagedGqaAttention(Mixer):
                                              cache.append)
         out = kernels.paged_attention(qkv, Hq, Hkv, D, cache.pages, cache.block_table,
                                       cache.page_size, ctx, self.window or 0, self.scale)
-        return kernels.linear(out, self.w_o)
+        return self.project("o", out, self.w_o, ctx)

@@ -15,9 +15,12 @@ from __future__ import annotations
 import bisect
 import itertools
 from dataclasses import dataclass, field
-from typing import Callable, Dict, List, Optional, Sequence, Tuple
+from typing import TYPE_CHECKING, Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
+
+if TYPE_CHECKING:
+    from .adapters import Projection, ProjectionAdapters
 
 
 # --------------------------------------------------------------------------------------
@@ -132,6 +135,7 @@ class StepContext:
     max_rows_per_seg: int = 1
     max_context: int = 0           # bound on pos0 + rows over the segments of this step
     graph_mode: bool = False
+    row_adapter: Optional[torch.Tensor] = None     # [T] adapter slot of each row, -1: none; None: no row has one
     scratch: Dict[str, torch.Tensor] = field(default_factory=dict)
     _tiles: Dict[object, Tuple[torch.Tensor, int]] = field(default_factory=dict)
 
@@ -379,6 +383,24 @@ class Part:
     # True if `forward` only launches work on the current stream from device-side data
     # (no host reads of the step's contents), so that a step may be captured in a CUDA graph.
     graph_safe = False
+
+    # pools of adapters by projection, where the engine keeps any (see adapters.py)
+    adapters: Dict[str, "ProjectionAdapters"] = {}
+
+    def projections(self) -> Dict[str, "Projection"]:
+        """The weight matrices of this part that take adapters."""
+        return {}
+
+    def adapter_pool(self, which: str, ctx: "StepContext") -> Optional["ProjectionAdapters"]:
+        """The pool of a projection if a row of this step has an adapter; None: the projection alone."""
+        pool = self.adapters.get(which)
+        return pool if pool is not None and ctx.row_adapter is not None else None
+
+    def project(self, which: str, x: torch.Tensor, w: torch.Tensor, ctx: "StepContext") -> torch.Tensor:
+        """x w^T, with the rows' adapters beside it."""
+        from .. import kernels
+        pool = self.adapter_pool(which, ctx)
+        return kernels.linear(x, w) if pool is None else pool.linear(x, w, ctx.row_adapter)
 
     def tensor_specs(self) -> List[TensorSpec]:
         return []

@@ -22,6 +22,7 @@ import torch
 
 from .. import kernels
 from ..registry import register_part
+from .adapters import Projection
 from .base import BiasedOutput, FeedForward, Fetch, RoutedSum, StepContext, TensorSpec
 
 
@@ -102,7 +103,17 @@ class DenseSwiglu(FeedForward):
     def weight_bytes(self) -> int:
         return (self.w_gate_up.numel() + self.w_down.numel()) * self.w_down.element_size()
 
+    def projections(self):
+        if self.has_bias:                 # (a bias that is added to float32 sums: not together with adapters)
+            return {}
+        H, I = self.hidden_size, self.intermediate_size
+        return {"gate_up": Projection((self._n("gate"), self._n("up")), (I, I), H), "down": Projection((self._n("down"),), (H,), I)}
+
     def forward(self, x: torch.Tensor, ctx: StepContext):
+        if self.adapter_pool("gate_up", ctx) is not None:
+            gu = self.project("gate_up", x, self.w_gate_up, ctx)
+            act = kernels.silu_mul(gu) if self.activation is None else kernels.gated_bias_act(gu, None, self.activation, x.dtype)
+            return self.project("down", act, self.w_down, ctx)
         if not self.has_bias and (self.activation is None or self.activation == kernels.ACT_GELU_TANH):
             # an activation without constants of its own sits where silu does: in the first product's epilogue
             act = {} if self.activation is None else {"act": self.activation}

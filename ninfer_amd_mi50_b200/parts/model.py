@@ -69,6 +69,10 @@ class DecoderModel:
         self.embedding: Optional[torch.Tensor] = None
         self.head: Optional[torch.Tensor] = None
 
+    def parts(self):
+        """The parts of all blocks, in the order of the layers."""
+        return [p for b in self.blocks for p in b.parts()]
+
     # ---- what the model needs ---------------------------------------------------------
     def tensor_specs(self) -> List[TensorSpec]:
         V, H = self.vocab_size, self.hidden_size

@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Callable, Dict, Optional, Sequence, Union
 
 
 @dataclass
@@ -14,7 +15,34 @@ class SamplingParams:
     repetition_penalty: float = 1.0   # 1: off (the CLI's default is 1.05, as in the reference)
     seed: int = 0                     # 0: a fresh seed per request
     max_new_tokens: int = 512
+    # what the reference does not have: penalties on what was generated (each occurrence, and once), values added to
+    # single tokens' logits, and the tokens that may follow: a set, or a function from the generated ids to one (None: any
+    # token; an empty answer ends the request)
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None
+    allowed_tokens: Union[Sequence[int], Callable[[Sequence[int]], Optional[Sequence[int]]], None] = None
 
     @property
     def greedy(self) -> bool:
         return self.temperature <= 0.0
+
+    @property
+    def has_rules(self) -> bool:
+        """Whether logits pass through more than the repetition penalty."""
+        return (self.frequency_penalty != 0.0 or self.presence_penalty != 0.0 or bool(self.logit_bias)
+                or self.allowed_tokens is not None)
+
+    @property
+    def penalises(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
+
+    @property
+    def looks_back(self) -> bool:
+        """Whether the next token depends on earlier ones by more than the model."""
+        return self.penalises or callable(self.allowed_tokens)
+
+    def allowed(self, generated: Sequence[int]) -> Optional[Sequence[int]]:
+        """The tokens that may follow `generated`; None: any."""
+        a = self.allowed_tokens
+        return a(list(generated)) if callable(a) else a

@@ -14,13 +14,15 @@ engine.cpp:166-169; the idea is the same, the generator is not.)
 
 from __future__ import annotations
 
+import math
 from collections import Counter
-from typing import List, Optional, Sequence
+from typing import Hashable, List, Optional, Sequence
 
 import torch
 
 from .. import kernels
 from .params import SamplingParams
+from .rules import RuleRow, TokenLogs, apply_rules
 
 _MASK = (1 << 64) - 1
 
@@ -34,7 +36,32 @@ def uniform_draw(seed: int, counter: int) -> float:
     return (z >> 40) / float(1 << 24)
 
 
+def check_allowed(ids: Sequence[int], vocab: int) -> None:
+    for t in ids:
+        if not 0 <= int(t) < vocab:
+            raise ValueError(f"allowed token {t} outside [0, {vocab})")
+
+
+def check_rules(p: SamplingParams, vocab: int) -> None:
+    """Raises ValueError for penalties, biases or allowed tokens that make no sense."""
+    if p.has_rules and not p.repetition_penalty > 0:
+        raise ValueError("repetition_penalty must be positive")
+    for what in ("frequency_penalty", "presence_penalty"):
+        if not math.isfinite(getattr(p, what)):
+            raise ValueError(f"{what}={getattr(p, what)} must be finite")
+    for t, v in (p.logit_bias or {}).items():
+        if not 0 <= int(t) < vocab:
+            raise ValueError(f"logit_bias names token {t} outside [0, {vocab})")
+        if math.isnan(float(v)) or float(v) == math.inf:
+            raise ValueError(f"logit_bias of token {t} is {v}: finite, or -inf for a token that is never drawn")
+    if p.allowed_tokens is not None and not callable(p.allowed_tokens):
+        if len(p.allowed_tokens) == 0:
+            raise ValueError("allowed_tokens allows nothing")
+        check_allowed(p.allowed_tokens, vocab)
+
+
 def check_params(p: SamplingParams, vocab: int) -> None:
+    check_rules(p, vocab)
     if p.greedy:
         return
     k = min(max(p.top_k, 1), vocab)
@@ -47,14 +74,26 @@ def check_params(p: SamplingParams, vocab: int) -> None:
 
 
 def sample_reference(logits: Sequence[float], p: SamplingParams, recent: Sequence[int] = (),
-                     draw: float = 0.0) -> int:
-    """Host twin: same policy, same tie rules, same draw."""
+                     draw: float = 0.0, prompt_length: int = 0) -> int:
+    """Host twin: same policy, same tie rules, same draw.  `recent[prompt_length:]` are the generated ids."""
     l = torch.as_tensor(logits, dtype=torch.float32).clone()
     V = l.numel()
     if p.repetition_penalty != 1.0:
         for tok in recent:
             if 0 <= tok < V:
                 l[tok] = l[tok] / p.repetition_penalty if l[tok] > 0 else l[tok] * p.repetition_penalty
+    if p.has_rules:
+        generated = list(recent[prompt_length:])
+        for tok, n in Counter(generated).items():
+            if 0 <= tok < V:
+                l[tok] = l[tok] - n * p.frequency_penalty - p.presence_penalty
+        for tok, v in (p.logit_bias or {}).items():
+            l[tok] += v
+        allowed = p.allowed(generated)
+        if allowed is not None:
+            left_out = torch.ones(V, dtype=torch.bool)
+            left_out[torch.as_tensor(list(allowed), dtype=torch.long)] = False
+            l[left_out] = -math.inf
     if p.greedy:
         return int(torch.argmax(l))          # first maximum
     l = l * torch.tensor(1.0 / p.temperature, dtype=torch.float32)
@@ -90,20 +129,32 @@ class Sampler:
 
     def __init__(self, vocab_size: int, device):
         self.vocab_size, self.device = vocab_size, torch.device(device)
+        self.logs = TokenLogs(self.device)
+
+    def forget(self, key: Hashable) -> None:
+        """A request is done: its log of tokens may be given to another."""
+        self.logs.forget(key)
 
     def sample(self, logits: torch.Tensor, params: Sequence[SamplingParams],
                recent: Optional[Sequence[Sequence[int]]] = None,
-               counters: Optional[Sequence[int]] = None) -> torch.Tensor:
+               counters: Optional[Sequence[int]] = None, prompt_lengths: Optional[Sequence[int]] = None,
+               keys: Optional[Sequence[Hashable]] = None,
+               allowed: Optional[Sequence[Optional[Sequence[int]]]] = None) -> torch.Tensor:
         """logits float32 [R, V] on the device -> int32 [R] on the device.
 
-        `recent[r]` are the ids the repetition penalty looks at (prompt and generated);
-        `counters[r]` is the index of the token being drawn, the RNG counter."""
+        `recent[r]` are the ids the penalties look at (prompt and generated), of which the first
+        `prompt_lengths[r]` are the prompt's (0 if left out);
+        `counters[r]` is the index of the token being drawn, the RNG counter; `keys[r]` names the request whose tokens
+        these are, so that only new ones are sent; `allowed[r]` is what `params[r].allowed` says of the generated ids, where
+        the caller has asked already."""
         R = logits.shape[0]
         if R == 0:
             return torch.empty((0,), dtype=torch.int32, device=self.device)
         dev = self.device
         # repetition penalty on a copy (the caller may still want the raw logits)
-        pen_rows = [r for r in range(R) if params[r].repetition_penalty != 1.0 and recent and recent[r]]
+        rule_rows = [r for r in range(R) if params[r].has_rules]
+        pen_rows = [r for r in range(R) if params[r].repetition_penalty != 1.0 and recent and recent[r] and not params[r].has_rules]
+        own = bool(pen_rows)
         if pen_rows:
             logits = logits.clone()
             ids, counts, row_of = [], [], []
@@ -114,6 +165,14 @@ class Sampler:
             pen = mk([p.repetition_penalty for p in params], torch.float32)
             kernels.repetition_penalty(logits, mk(ids, torch.int32), mk(counts, torch.int32),
                                        mk(row_of, torch.int32), pen)
+        if rule_rows:
+            rows = []
+            for r in rule_rows:
+                tokens = list(recent[r]) if recent else []
+                prompt = prompt_lengths[r] if prompt_lengths else 0
+                ids = allowed[r] if allowed is not None else params[r].allowed(tokens[prompt:])
+                rows.append(RuleRow(r, params[r], tokens, prompt, keys[r] if keys else None, ids))
+            logits = apply_rules(logits, rows, self.logs, out=logits if own else None)
         if all(p.greedy for p in params):
             return kernels.argmax_rows(logits)
         out = kernels.argmax_rows(logits)

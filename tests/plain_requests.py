@@ -77,3 +77,36 @@ def plain_rules(logits, history, slots, lengths, starts, penalties, tokens=None,
     most = torch.finfo(torch.float32).max
     l[l > most], l[l < -most] = math.inf, -math.inf
     return l, off, h
+
+
+# ---- twins of the kernels, for CPU tests of the engine's logic --------------------------------------------------------------
+
+def adapter_linear(x, w, a, b, scale, ids, widths=None, out=None):
+    y = x.float() @ w.float().t()
+    R = b.shape[2]
+    for t, i in enumerate(ids.tolist()):
+        lo = 0
+        for j, width in enumerate(widths or [w.shape[0]]):
+            if i >= 0:
+                h = (a[i, j * R:(j + 1) * R].float() @ x[t].float()) * scale[i]
+                y[t, lo:lo + width] += b[i, lo:lo + width].float() @ h
+            lo += width
+    return y.to(x.dtype)
+
+
+def append_history(history, slots, positions, tokens):
+    history[slots.long(), positions.long()] = tokens
+
+
+def adjust_logits(logits, history, slots, lengths, starts, penalties, tokens=None, bias=None, mask=None, out=None):
+    y, _, h = plain_rules(logits, history, slots, lengths, starts, penalties, tokens, bias, mask)
+    history.copy_(h)
+    if out is not None:
+        return out.copy_(y)
+    return y.float()
+
+
+def install(monkeypatch):
+    import ninfer_amd_mi50_b200.kernels as K
+    for name in ("adapter_linear", "append_history", "adjust_logits"):
+        monkeypatch.setattr(K, name, globals()[name])
