@@ -31,6 +31,7 @@ _SIGNATURES = {
     "nf_logit_rules": [_P] * 11 + [_I] + [_P] * 2 + [_I] * 7 + [_P],
 }
 _functions = {}
+_slices = {}            # widths -> (their ends for the C call, how many, their sum)
 _used = False           # whether any of these kernels was called: until then there is no status to read
 
 
@@ -54,6 +55,22 @@ def _call(name: str, *args) -> None:
 
 def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _parts(widths: Sequence[int]) -> Tuple[ctypes.Array, int, int]:
+    """The ends of stacked parts as the kernels take them, their number and the last end; no parts where a width is none."""
+    key = tuple(widths)
+    got = _slices.get(key)
+    if got is None:
+        ends, e = (_I * max(1, len(key)))(), 0
+        ok = all(int(v) > 0 for v in key)
+        for i, v in enumerate(key if ok else ()):
+            e += int(v)
+            ends[i] = e
+        got = (ends, len(key) if ok else 0, e)
+        if len(_slices) < 1024:
+            _slices[key] = got
+    return got
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -90,7 +107,7 @@ def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
     if n < 1 or K < 1 or a.shape != (n, S * R, K) or b.shape[1] != N:
         raise ValueError(f"adapter_linear: a {tuple(a.shape)} and b {tuple(b.shape)} do not fit {S} parts, rank {R} and w "
                          f"{tuple(w.shape)}")
-    if scale.shape != (n,) or ids.shape != (T,):
+    if scale.numel() != n or ids.numel() != T:
         raise ValueError(f"adapter_linear: scale {tuple(scale.shape)} and ids {tuple(ids.shape)} for {n} adapters and {T} rows")
     if out is not None:
         _chk(out, "out", x.dtype)
@@ -116,7 +133,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         widths = (w.shape[0],)
     dtype, dev = x.dtype, x.get_device()
     xs, ws, bs = x.shape, w.shape, b.shape
-    S = len(widths)
+    ends, S, total = _parts(widths)
     if not (dev >= 0 and len(xs) == 2 and len(ws) == 2 and len(bs) == 3 and (dtype is torch.bfloat16 or dtype is torch.float32)
             and w.dtype is dtype and a.dtype is dtype and b.dtype is dtype and scale.dtype is torch.float32
             and ids.dtype is torch.int32 and w.get_device() == dev and a.get_device() == dev and b.get_device() == dev
@@ -124,9 +141,9 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
             and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous() and ids.is_contiguous()):
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     T, K = xs
-    N, (n, _, R) = ws[0], bs
-    if not (K > 0 and ws[1] == K and n > 0 and bs[1] == N and R in ADAPTER_RANKS and 1 <= S <= MAX_ADAPTER_SLICES
-            and min(widths) > 0 and sum(widths) == N and a.shape == (n, S * R, K) and scale.shape == (n,) and ids.shape == (T,)):
+    N, (n, b_rows, R) = ws[0], bs
+    if not (K > 0 and ws[1] == K and n > 0 and b_rows == N and R in ADAPTER_RANKS and 1 <= S <= MAX_ADAPTER_SLICES
+            and total == N and a.shape == (n, S * R, K) and scale.numel() == n and ids.numel() == T):
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     if out is None:
         out = x.new_empty((T, N))
@@ -137,10 +154,6 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     px, pw, pa, pb, po = x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), out.data_ptr()
     if (px | pw | pa | pb | po) & 15:
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
-    ends, e = (_I * S)(), 0
-    for i, v in enumerate(widths):
-        e += v
-        ends[i] = e
     bf16 = dtype is torch.bfloat16
     if TUNING["adapter"] == "auto" and (K % 8 == 0 if bf16 else K % 4 == 0 and T <= TUNING["adapter_f32_max_rows"]):
         h = scale.new_empty(T * S * R)
@@ -185,7 +198,7 @@ def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, b
         raise ValueError("adjust_logits takes logits [R, V] and history [slots, capacity]")
     R, V = logits.shape
     _chk(penalties, "penalties", torch.float32)
-    if penalties.shape != (R, 3):
+    if penalties.numel() != 3 * R:
         raise ValueError(f"adjust_logits: penalties are {tuple(penalties.shape)}, not {(R, 3)}")
     lists = [(slots, "slots", R), (lengths, "lengths", R), (starts, "starts", R)]
     if tokens is not None:
@@ -195,7 +208,7 @@ def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, b
         offsets, ids, values = bias
         lists += [(offsets, "bias offsets", R + 1), (ids, "bias ids", ids.numel())]
         _chk(values, "bias values", torch.float32)
-        if values.shape != ids.shape:
+        if values.numel() != ids.numel():
             raise ValueError(f"adjust_logits: {tuple(ids.shape)} bias ids, {tuple(values.shape)} values")
         others.append(values)
     if mask is not None:
@@ -207,7 +220,7 @@ def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, b
         others.append(bits)
     for t, name, n in lists:
         _chk(t, name, torch.int32)
-        if t.shape != (n,):
+        if t.numel() != n:
             raise ValueError(f"adjust_logits: {name} are {tuple(t.shape)}, not {(n,)}")
     if out is not None:
         _chk(out, "out", torch.float32, contiguous=False)
@@ -244,56 +257,52 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     token i is allowed; index -1: no mask.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits`
     itself.  A slot, a length or a mask row outside its tensor changes that row as if it had no tokens or no mask, and is
     reported by `check_status`."""
-    operands = (logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
     dev = logits.get_device()
     ls, hs = logits.shape, history.shape
-    if not (dev >= 0 and len(ls) == 2 and len(hs) == 2 and logits.dtype is torch.float32 and history.dtype is torch.int32
+    good = (dev >= 0 and len(ls) == 2 and len(hs) == 2 and logits.dtype is torch.float32 and history.dtype is torch.int32
             and slots.dtype is torch.int32 and lengths.dtype is torch.int32 and starts.dtype is torch.int32
             and penalties.dtype is torch.float32 and history.get_device() == dev and slots.get_device() == dev
             and lengths.get_device() == dev and starts.get_device() == dev and penalties.get_device() == dev
             and history.is_contiguous() and slots.is_contiguous() and lengths.is_contiguous() and starts.is_contiguous()
-            and penalties.is_contiguous()):
-        _refuse_logits(*operands)
-    R, V = ls
-    one = (R,)
-    if not (slots.shape == one and lengths.shape == one and starts.shape == one and penalties.shape == (R, 3) and hs[0] > 0
-            and hs[1] > 0 and hs[1] % 4 == 0 and history.data_ptr() % 16 == 0):
-        _refuse_logits(*operands)
-    if tokens is not None and not (tokens.dtype is torch.int32 and tokens.get_device() == dev and tokens.is_contiguous()
-                                   and tokens.shape == one):
-        _refuse_logits(*operands)
+            and penalties.is_contiguous())
+    R, V = ls if good else (0, 0)
+    p_history = history.data_ptr()
+    good = (good and slots.numel() == R and lengths.numel() == R and starts.numel() == R and penalties.numel() == 3 * R
+            and hs[0] > 0 and hs[1] > 0 and hs[1] % 4 == 0 and p_history % 16 == 0)
+    if good and tokens is not None:
+        good = tokens.dtype is torch.int32 and tokens.get_device() == dev and tokens.is_contiguous() and tokens.numel() == R
     p_off = p_ids = p_values = p_bits = p_index = None
     n_bias = n_masks = 0
-    if bias is not None:
+    if good and bias is not None:
         offsets, ids, values = bias
         n_bias = ids.numel()
-        if not (offsets.dtype is torch.int32 and ids.dtype is torch.int32 and values.dtype is torch.float32
+        good = (offsets.dtype is torch.int32 and ids.dtype is torch.int32 and values.dtype is torch.float32
                 and offsets.get_device() == dev and ids.get_device() == dev and values.get_device() == dev
-                and offsets.is_contiguous() and ids.is_contiguous() and values.is_contiguous() and offsets.shape == (R + 1,)
-                and ids.shape == (n_bias,) and values.shape == (n_bias,)):
-            _refuse_logits(*operands)
+                and offsets.is_contiguous() and ids.is_contiguous() and values.is_contiguous() and offsets.numel() == R + 1
+                and values.numel() == n_bias)
         p_off, p_ids, p_values = offsets.data_ptr(), ids.data_ptr(), values.data_ptr()
-    if mask is not None:
+    if good and mask is not None:
         bits, index = mask
         n_masks = bits.shape[0] if bits.dim() == 2 else 0
-        if not (bits.dtype is torch.int32 and index.dtype is torch.int32 and bits.get_device() == dev and index.get_device() == dev
+        good = (bits.dtype is torch.int32 and index.dtype is torch.int32 and bits.get_device() == dev and index.get_device() == dev
                 and bits.is_contiguous() and index.is_contiguous() and n_masks > 0 and bits.shape[1] == (V + 31) // 32
-                and index.shape == one):
-            _refuse_logits(*operands)
+                and index.numel() == R)
         p_bits, p_index = bits.data_ptr(), index.data_ptr()
+    if good and out is not None:
+        good = out.dtype is torch.float32 and out.get_device() == dev and out.shape == ls
+    if not good:
+        _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
     if out is None:
-        out = history.new_empty((R, V), dtype=torch.float32)
+        out = penalties.new_empty((R, V))
         apart_out = V
     else:
-        if not (out.dtype is torch.float32 and out.get_device() == dev and out.shape == ls):
-            _refuse_logits(*operands)
         apart_out = _rows_apart(out, R, V)
     if R == 0 or V == 0:
         return out
     apart = _rows_apart(logits, R, V)
     if apart < 0 or apart_out < 0:
-        _refuse_logits(*operands)
-    _call("nf_logit_rules", logits.data_ptr(), out.data_ptr(), history.data_ptr(), slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
+        _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
+    _call("nf_logit_rules", logits.data_ptr(), out.data_ptr(), p_history, slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
           _ptr(tokens), penalties.data_ptr(), p_off, p_ids, p_values, n_bias, p_bits, p_index, n_masks, R, V, apart, apart_out, hs[0],
           hs[1], _stream())
     return out
