@@ -8,10 +8,11 @@
 //
 // `adapter_wide_kernel`, many rows: a persistent CTA an SM, tiles of 128 rows x up to 256 features, k in steps of 64 through a
 // ring of TMA stages, two accumulators in tensor memory so that a tile's epilogue runs under the next tile's products.  Behind
-// the last step over k a tile takes one step more for each adapter that occurs among its 128 rows: rows of h of that adapter,
-// zeros for the others, times the adapter's rows of B.  h enters as two bfloat16 numbers, the nearest and what it leaves
-// (2^-17 of h is lost), both against the same rows of B: the adapters' part is then as good as the float32 sum it is added to.
-// Tiles never reach over the end of a slice, so a tile needs one slice's columns of h.
+// the last step over k a tile takes a step or a few more for each adapter that occurs among its rows: rows of h of that adapter,
+// zeros for the others, times the adapter's rows of B.  The kernel that makes h lays it out so, a block of 128 rows for every
+// adapter of a row tile, and these steps go through the ring like all others.  h enters as two bfloat16 numbers, the nearest and
+// what it leaves (2^-17 of h is lost), both against the same rows of B: the adapters' part is then as good as the float32 sum it is
+// added to.  Tiles never reach over the end of a slice, so a tile needs one slice's columns of h.
 //
 // `adapter_rows_kernel`, few rows: the time is that of reading W once.  W is the 128-row operand, the rows of x the other; the
 // CTAs of a cluster share a tile of 128 features and split k; their sums meet through distributed shared memory, each CTA
@@ -171,7 +172,8 @@ struct __align__(8) ShrinkBars {
   unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full, acc_empty;
   unsigned tmem_base;
   int stop;
-  unsigned char served[kAdM];           // rows of the tile whose adapter this CTA has taken
+  int id[kAdM];                         // the rows' adapters, -1: none
+  unsigned char first[kAdM], place[kAdM];      // whether a row is the first with its adapter; that adapter's place among the tile's
 };
 
 // CTAs of a cluster wait for one another, and an allocation of tensor memory waits for the SM's other CTAs: whatever of these
@@ -181,35 +183,31 @@ struct __align__(8) ShrinkBars {
 constexpr size_t kShrinkSmemLeast = 118 * 1024;
 constexpr int kShrinkCols = 256;        // columns of an accumulator: numbers of h of all adapters of a pass
 
-// Writes 8 numbers of h: as they are, or as the nearest bfloat16 and what that leaves, SR numbers behind one another.
-__device__ __forceinline__ void put_h(float* h, int t, int SR, int j, const float* v, bool split) {
-  if (!split) {
-    store4(h + (size_t)t * SR + j, v);
-    store4(h + (size_t)t * SR + j + 4, v + 4);
-    return;
-  }
-  __nv_bfloat162 hi[4], lo[4];
+// 8 numbers of h as the nearest bfloat16 and what that leaves.
+__device__ __forceinline__ void split_h(const float* v, uint4& hi, uint4& lo) {
+  __nv_bfloat162 a[4], b[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    hi[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-    const float2 back = __bfloat1622float2(hi[e]);
+    a[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    const float2 back = __bfloat1622float2(a[e]);
     // (of an infinity nothing is left)
-    lo[e] = __floats2bfloat162_rn(isinf(back.x) ? 0.f : v[2 * e] - back.x, isinf(back.y) ? 0.f : v[2 * e + 1] - back.y);
+    b[e] = __floats2bfloat162_rn(isinf(back.x) ? 0.f : v[2 * e] - back.x, isinf(back.y) ? 0.f : v[2 * e + 1] - back.y);
   }
-  __nv_bfloat16* row = reinterpret_cast<__nv_bfloat16*>(h) + (size_t)t * 2 * SR + j;
-  *reinterpret_cast<uint4*>(row) = *reinterpret_cast<uint4*>(hi);
-  *reinterpret_cast<uint4*>(row + SR) = *reinterpret_cast<uint4*>(lo);
+  hi = *reinterpret_cast<uint4*>(a);
+  lo = *reinterpret_cast<uint4*>(b);
 }
 
 // D[t, (adapter, j)] over a tile of up to 128 rows: x is the 128-row operand, the rows of A of up to `group` of the adapters
 // that occur in the tile the other, so that x is read once for all of them.  The CTAs of a cluster split k; each sends every row's
 // own numbers to the member that owns the row, which adds them up in the members' order, scales and writes them.
-// gridDim.z CTAs take the adapters of a tile in turn, by their number.
+// gridDim.z CTAs take the adapters of a tile in turn, by their number.  What is written: `places` 0, a row's numbers as they are, [rows,
+// SR] float32; otherwise blocks of 128 rows, [row tile][place of the adapter among the tile's, `places` of them][slice][128][2 R]
+// bfloat16, R numbers rounded and R of what that leaves, zeros in the rows of other adapters.
 // 192 threads: producer, MMA, four epilogue warps (a thread a row).  grid: (members, row tiles * j tiles, adapters in turn).
 __global__ void __launch_bounds__(192, 1)
 adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ scale,
                          const int* __restrict__ ids, float* __restrict__ h, int rows, int K, int SR, int n, int row_tiles, int x_box, int JW,
-                         int group, int stages, int split) {
+                         int group, int stages, int places, int R) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   ShrinkBars* bars = reinterpret_cast<ShrinkBars*>(smem);
@@ -228,7 +226,6 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (threadIdx.x < kAdM) bars->served[threadIdx.x] = 0;
   __syncwarp();
   if (warp == 1) tc_alloc<1>(&bars->tmem_base, kShrinkCols);
   tc_fence_before();
@@ -313,7 +310,23 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     }
   } else {
     const int quad = warp & 3, r = quad * 32 + lane, t = row0 + r;
-    const int own = t < rows ? ids[t] : -1;
+    int own = t < rows ? ids[t] : -1;
+    if (own >= n) {
+      if (member == 0 && jt == 0 && blockIdx.z == 0) atomicCAS(&g_adapter_tc_index, 0, t + 1);
+      own = -1;
+    }
+    bars->id[r] = own = max(own, -1);
+    if (places) {
+      // the place of the row's adapter among the tile's in ascending order: how many first rows of smaller ones there are
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      int earlier = 0;
+      for (int o = 0; o < r; ++o) earlier |= bars->id[o] == own;
+      bars->first[r] = own >= 0 && !earlier;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      int place = 0;
+      for (int o = 0; o < kAdM; ++o) place += bars->first[o] && bars->id[o] < own;
+      bars->place[r] = (unsigned char)place;
+    }
     int done = 0, mine = 0;
     const unsigned to = cluster_addr(smem_u32(sums + ((size_t)member * share + r % share) * JP), r / share);
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // every member is there: its shared memory may be written
@@ -324,7 +337,7 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       tc_fence_after();
       for (int g = 0; g < count; ++g) {
         const int a = __shfl_sync(0xffffffffu, mine, g);       // (every lane, before any condition on its own row)
-        const bool is = own == a;
+        const bool is = own == a;          // (a is none of the marks for no adapter)
         if (!__any_sync(0xffffffffu, is)) continue;
         const unsigned at = tmem + g * JW + ((unsigned)(quad * 32) << 16);
         for (int c = 0; c < jn; c += 16) {
@@ -338,7 +351,6 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                            "r"(v[e + 3]) : "memory");
           }
         }
-        if (is) bars->served[r] = 1;
       }
       tc_fence_before();
       __syncwarp();
@@ -350,20 +362,50 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   if (warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   cluster_barrier();                  // every member's part is there
   const int pieces = jn >> 3;
-  for (int i = threadIdx.x; i < share * pieces; i += blockDim.x) {
-    const int rl = i / pieces, r = member * share + rl, j = (i - rl * pieces) * 8, t = row0 + r;
-    if (!bars->served[r]) continue;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto numbers = [&](int rl, int j, float* v) {                // 8 numbers of this member's row rl, from j on
+    const float sc = scale[bars->id[member * share + rl]];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
     for (int m = 0; m < members; ++m) {
       float u[8];
       load8(sums + ((size_t)m * share + rl) * JP + j, u);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += u[e];
     }
-    const float sc = scale[ids[t]];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= sc;
-    put_h(h, t, SR, j0 + j, v, split != 0);
+  };
+  if (!places) {
+    for (int i = threadIdx.x; i < share * pieces; i += blockDim.x) {
+      const int rl = i / pieces, j = (i - rl * pieces) * 8, id = bars->id[member * share + rl];
+      if (id < 0 || id % (int)gridDim.z != (int)blockIdx.z) continue;
+      float v[8];
+      numbers(rl, j, v);
+      float* to = h + (size_t)(row0 + member * share + rl) * SR + j0 + j;
+      store4(to, v);
+      store4(to + 4, v + 4);
+    }
+  } else {
+    for (int a = tids.next(-1); a != kNone; a = tids.next(a)) {
+      int place = -1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tids.v[i] == a) place = bars->place[lane + 32 * i];
+      place = __reduce_max_sync(0xffffffffu, place);
+      __nv_bfloat16* block = reinterpret_cast<__nv_bfloat16*>(h) + ((size_t)tile * places + place) * kAdM * 2 * SR;
+      for (int i = threadIdx.x; i < share * pieces; i += blockDim.x) {
+        const int rl = i / pieces, j = j0 + (i - rl * pieces) * 8, r = member * share + rl, slice = j / R;
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (bars->id[r] == a) {
+          float v[8];
+          numbers(rl, j - j0, v);
+          split_h(v, hi, lo);
+        }
+        __nv_bfloat16* to = block + ((size_t)slice * kAdM + r) * 2 * R + (j - slice * R);
+        *reinterpret_cast<uint4*>(to) = hi;
+        *reinterpret_cast<uint4*>(to + R) = lo;
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -376,15 +418,14 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 // ---- many rows -------------------------------------------------------------------------------------------------------------
 
 struct __align__(8) WideBars {
-  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2], h_full[4], h_peer[4], h_empty[4];
+  unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full[2], acc_empty[2];
   unsigned tmem_base;
   int stop;
 };
 
 constexpr int kWideEpilogueWarps = 8;
-constexpr int kWideThreads = 32 * (2 + 4 + kWideEpilogueWarps);
+constexpr int kWideThreads = 32 * (2 + kWideEpilogueWarps);
 constexpr int kWideHead = 1024;                            // barriers
-constexpr int wide_h_bytes(int ctas) { return 2 * kAdTile; }      // rows of h
 constexpr int kTurnRow = 80, kTurnBytes = 32 * kTurnRow;                 // a warp's 32 x 32 results, rows 80 bytes apart (no bank twice)
 constexpr int kWideSmem = 225 * 1024;
 
@@ -417,17 +458,16 @@ __device__ __forceinline__ int next_tile(int i, int first, int stride) { return 
 
 // CTAS 1: a CTA a tile of 128 rows x BN features.  CTAS 2: two CTAs of a cluster a tile of 256 x BN; each holds its own 128 rows of x
 // and half of the features' rows of W, and the even one issues products over both (`cta_group::2`): half of W's bytes a CTA.
-// Warps: 0 producer, 1 MMA and tensor memory, 2..5 rows of h (a thread a row), 6..13 epilogue.
+// Warps: 0 producer, 1 MMA and tensor memory, 2..9 epilogue.  map_h: h as the first product lays it out, `places` blocks a row tile.
 template <int CTAS>
 __global__ void __launch_bounds__(kWideThreads, 1)
 adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_b,
-                    const int* __restrict__ ids, const __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
-                    int R, int n, const __grid_constant__ TcSlices slices, int f_tiles, int n_tiles, int BN, int stages) {
-  extern __shared__ unsigned char smem_raw[];      // [barriers | rows of h | stages | results on their way]
+                    const __grid_constant__ CUtensorMap map_h, const int* __restrict__ ids, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
+                    int R, int n, int places, const __grid_constant__ TcSlices slices, int f_tiles, int n_tiles, int BN, int stages) {
+  extern __shared__ unsigned char smem_raw[];      // [barriers | stages | results on their way]
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   WideBars* bars = reinterpret_cast<WideBars*>(smem);
-  unsigned char* h_tile = smem + kWideHead;
-  unsigned char* stage0 = h_tile + wide_h_bytes(CTAS);
+  unsigned char* stage0 = smem + kWideHead;
   const int w_bytes = BN / CTAS * 128, stage_bytes = kAdTile + w_bytes;
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
@@ -438,7 +478,6 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       mbar_init(&bars->acc_full[b], 1);
       mbar_init(&bars->acc_empty[b], kWideEpilogueWarps * CTAS);
     }
-    for (int b = 0; b < 4; ++b) { mbar_init(&bars->h_full[b], 4); mbar_init(&bars->h_peer[b], 1); mbar_init(&bars->h_empty[b], 1); }
     bars->stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -450,45 +489,46 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tc_fence_after();
   const unsigned tmem = bars->tmem_base;
   const int steps = (K + kAdK - 1) / kAdK;
-  const int r_steps = (R + kAdK - 1) / kAdK;          // steps of up to 64 ranks an adapter
-  const int r_here = min(R, kAdK);                    // ranks of one such step (R is 16, 32, 64 or 128)
-  // Rows of h lie 128 bytes apart; up to 32 ranks both parts fit into that, beyond they come one after the other.  Several are under
-  // way at a time: from one thread's store to the issuer and back is longer than the products take.
-  constexpr int h_bufs = 2;
-  const int h_parts = R <= 32 ? 1 : 2;
+  // An adapter's steps: up to 32 ranks one, with both parts of h beside one another; beyond, 64 numbers of a part each.
+  const int r_steps = (R + kAdK - 1) / kAdK, h_steps = R <= 32 ? 1 : 2 * r_steps;
   TileIds<CTAS> tids;
 
   if (warp == 0) {
-    // ---- producer: x and W (what wrote x is complete, see chain_release_late in the kernels that make h) ------------------
+    // ---- producer: x and W (what wrote x is complete, see chain_release_late in the kernels that make h), then h and B ----
     int issued = 0;
-    bool ok = true;
+    bool ok = true, waited = false;
     Ring ring;
+    auto step = [&](const CUtensorMap* mx, int kx, int x_row, const CUtensorMap* mw, int kw, int w_row) {
+      if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 1)) { ok = false; return; }
+      unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+      if (elect_one()) {
+        if (rank == 0) mbar_expect_tx(&bars->full[ring.s], CTAS * stage_bytes);
+        tma_load<CTAS>(st, mx, kx, x_row, &bars->full[ring.s]);
+        tma_load<CTAS>(st + kAdTile, mw, kw, w_row, &bars->full[ring.s]);
+      }
+      __syncwarp();
+      ++issued;
+      ring.next(stages);
+    };
     for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride)) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
       tids.load(ids, w.row0, rows, n);
       const int x_row = w.row0 + rank * kAdM, w_row = w.f0 + rank * (BN / CTAS);
-      for (int ks = 0; ks < steps; ++ks, ++issued, ring.next(stages)) {
-        if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 1)) { ok = false; break; }
-        unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
-        if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(&bars->full[ring.s], CTAS * stage_bytes);
-          tma_load<CTAS>(st, &map_x, ks * kAdK, x_row, &bars->full[ring.s]);
-          tma_load<CTAS>(st + kAdTile, &map_w, ks * kAdK, w_row, &bars->full[ring.s]);
-        }
-        __syncwarp();
-      }
+      for (int ks = 0; ks < steps && ok; ++ks) step(&map_x, ks * kAdK, x_row, &map_w, ks * kAdK, w_row);
+      if (!waited) { chain_wait(); waited = true; }
+      int place = 0;                            // of the adapter among this CTA's own rows
       for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
-        for (int rs = 0; rs < r_steps; ++rs, ++issued, ring.next(stages)) {
-          if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 1)) { ok = false; break; }
-          unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
-          if (elect_one()) {
-            if (rank == 0) mbar_expect_tx(&bars->full[ring.s], CTAS * w_bytes);
-            tma_load<CTAS>(st + kAdTile, &map_b, rs * kAdK, a * N + w_row, &bars->full[ring.s]);
-          }
-          __syncwarp();
-        }
+        bool here = false;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) here |= (rank ? tids.v[4 * (CTAS - 1) + v] : tids.v[v]) == a;
+        here = __any_sync(0xffffffffu, here);
+        // (the other CTA's alone: rows behind the last block, which read as zeros)
+        const int h_row = here ? ((x_row / kAdM * places + place) * slices.n + w.slice) * kAdM : (rows + kAdM - 1) / kAdM * places * slices.n * kAdM;
+        for (int e = 0; e < h_steps && ok; ++e) step(&map_h, e * kAdK, h_row, &map_b, e % r_steps * kAdK, a * N + w_row);
+        place += here;
       }
     }
+    if (!waited) chain_wait();
     // copies still on their way land in this CTA's shared memory (the even CTA's barriers count both CTAs' bytes)
     if (!ok && lane == 0 && rank == 0) {
       for (int j = max(0, issued - stages); j < issued; ++j)
@@ -500,7 +540,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     // ---- MMA ----------------------------------------------------------------------------------------------------------------
     int done = 0;
     bool ok = true;
-    Ring ring, hring;
+    Ring ring;
     const unsigned idesc = ad_instr_desc(BN, kAdM * CTAS);
     for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride), ++done) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
@@ -522,93 +562,28 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         __syncwarp();
       }
       for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
-        for (int rs = 0; rs < r_steps && ok; ++rs, ring.next(stages)) {
+        for (int e = 0; e < h_steps; ++e, ring.next(stages)) {
           if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 3)) { ok = false; break; }
-          const unsigned long long db = smem_desc(stage0 + (size_t)ring.s * stage_bytes + kAdTile);
-          for (int part = 0; part < h_parts; ++part, hring.next(h_bufs)) {
-            if (!warp_wait(&bars->h_full[hring.s], hring.phase, stop, 5) ||
-                (CTAS == 2 && !warp_wait_cluster(&bars->h_peer[hring.s], hring.phase, stop, 5))) { ok = false; break; }
-            tc_fence_after();
-            const unsigned long long dh = smem_desc(h_tile + hring.s * kAdTile);
-            if (elect_one()) {
-              for (int kk = 0; kk < r_here / 16; ++kk) {
-                mma<CTAS>(acc, dh + 2 * kk, db + 2 * kk, idesc, 1u);
-                if (h_parts == 1) mma<CTAS>(acc, dh + (64 >> 4) + 2 * kk, db + 2 * kk, idesc, 1u);
-              }
-              commit<CTAS>(&bars->h_empty[hring.s]);
-              if (part + 1 == h_parts) commit<CTAS>(&bars->empty[ring.s]);
+          tc_fence_after();
+          unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+          const unsigned long long dh = smem_desc(st), db = smem_desc(st + kAdTile);
+          const int n_kk = min(R, kAdK) / 16;
+          if (elect_one()) {
+            for (int kk = 0; kk < n_kk; ++kk) {
+              mma<CTAS>(acc, dh + 2 * kk, db + 2 * kk, idesc, 1u);
+              if (R <= 32) mma<CTAS>(acc, dh + 2 * (n_kk + kk), db + 2 * kk, idesc, 1u);
             }
-            __syncwarp();
+            commit<CTAS>(&bars->empty[ring.s]);
           }
+          __syncwarp();
         }
       }
       if (ok && elect_one()) commit<CTAS>(&bars->acc_full[ab]);
       __syncwarp();
     }
-  } else if (CTAS == 2 && warp == 1) {
-    // ---- the odd CTA's rows of h, passed on to the even one.  (Arriving there, with what was written before, takes a thread a thousand
-    // cycles: four warps that write the next rows meanwhile do not wait for it.  777 rows of 2048 x 11264 with 12 adapters of
-    // rank 64 in the first tile 61 -> 59.5 us, 244 of 128 x 3743 with 34 of rank 16 41 -> 36.)
-    bool ok = true;
-    Ring hring;
-    for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride)) {
-      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
-      tids.load(ids, w.row0, rows, n);
-      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a))
-        for (int e = 0; e < r_steps * h_parts; ++e, hring.next(h_bufs)) {
-          if (!warp_wait(&bars->h_full[hring.s], hring.phase, stop, 7)) { ok = false; break; }
-          if (elect_one()) arrive_leader<CTAS>(&bars->h_peer[hring.s]);
-          __syncwarp();
-        }
-    }
-  } else if (warp >= 2 && warp < 6) {
-    // ---- rows of h: this thread's row of the tile, in the operand's swizzled image; zeros for another adapter ---------------
-    chain_wait(h);
-    const int r = (warp - 2) * 32 + lane, SR = slices.n * R, n_pieces = r_here >> 3;
-    bool ok = true;
-    Ring hring;
-    for (int i = first; i < n_tiles && ok; i = next_tile(i, first, stride)) {
-      const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
-      tids.load(ids, w.row0, rows, n);
-      const int t = w.row0 + rank * kAdM + r;
-      const int own = t < rows ? ids[t] : -1;
-      if (w.f0 == 0 && own >= n) atomicCAS(&g_adapter_tc_index, 0, t + 1);
-      const bool has = own >= 0 && own < n;
-      uint4 hi[8], lo[8];                       // this row's numbers, read once a tile (beyond 64 ranks: a step)
-      auto read = [&](int rs) {
-        const uint4* src = reinterpret_cast<const uint4*>(h + (size_t)t * 2 * SR + w.slice * R + rs * kAdK);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          hi[j] = lo[j] = make_uint4(0, 0, 0, 0);
-          if (has && j < n_pieces) { hi[j] = src[j]; lo[j] = src[j + (SR >> 3)]; }
-        }
-      };
-      read(0);
-      for (int a = tids.next(-1); a != kNone && ok; a = tids.next(a)) {
-        const unsigned keep = own == a ? 0xffffffffu : 0u;
-        for (int rs = 0; rs < r_steps && ok; ++rs) {
-          if (rs > 0 && own == a) read(rs);
-          for (int part = 0; part < h_parts; ++part, hring.next(h_bufs)) {
-            if (!warp_wait(&bars->h_empty[hring.s], hring.phase ^ 1, stop, 6)) { ok = false; break; }
-            unsigned char* row = h_tile + hring.s * kAdTile + r * 128;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j < n_pieces) {
-                const uint4 p = part ? lo[j] : hi[j];
-                *reinterpret_cast<uint4*>(row + ((j ^ (r & 7)) << 4)) = make_uint4(p.x & keep, p.y & keep, p.z & keep, p.w & keep);
-                if (j < 4 && h_parts == 1)
-                  *reinterpret_cast<uint4*>(row + (((j + 4) ^ (r & 7)) << 4)) = make_uint4(lo[j].x & keep, lo[j].y & keep, lo[j].z & keep, lo[j].w & keep);
-              }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->h_full[hring.s]);
-          }
-        }
-      }
-    }
-  } else if (warp >= 6) {
+  } else if (warp >= 2) {
     // ---- epilogue: tensor-memory lanes 32 * (warp % 4) .. + 31, every other run of 32 columns --------------------------------
-    const int quad = warp & 3, half = (warp - 6) >> 2;
+    const int quad = warp & 3, half = (warp - 2) >> 2;
     int done = 0;
     for (int i = first; i < n_tiles; i = next_tile(i, first, stride), ++done) {
       const WideTile w = wide_tile(i, f_tiles, kAdM * CTAS, BN, slices);
@@ -617,7 +592,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       tc_fence_after();
       const int t0 = w.row0 + rank * kAdM + quad * 32, count = min(32, rows - t0);
       const bool whole = N % 8 == 0 && w.f0 % 8 == 0 && w.width % 8 == 0;
-      unsigned char* turned = stage0 + (size_t)stages * stage_bytes + (warp - 6) * kTurnBytes;
+      unsigned char* turned = stage0 + (size_t)stages * stage_bytes + (warp - 2) * kTurnBytes;
       for (int c0 = half * 32; c0 < BN; c0 += 64) {
         unsigned v[32];
         if (c0 < w.width) {
@@ -894,28 +869,32 @@ static int shrink_members(int rows, int K, int SR) {
   return p;
 }
 
-// y = x W^T + the adapters' part (see the head of this file): x [rows, K], W [N, K], A [n, n_slices * R, K], B [n, N, R], y
-// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h float32 [rows, n_slices * R] of
-// scratch.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or
-// 128, bases 16-byte aligned.
-extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h,
-                                 void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, cudaStream_t stream) {
-  if (rows == 0 || N == 0) return 0;
-  NF_REQUIRE(rows > 0 && N > 0 && K > 0 && n > 0, "adapter_linear: bad sizes rows=%d N=%d K=%d n=%d", rows, N, K, n);
-  NF_REQUIRE(K % 8 == 0, "adapter_linear: K=%d must be a multiple of 8", K);
-  NF_REQUIRE(R == 16 || R == 32 || R == 64 || R == 128, "adapter_linear: rank %d is not 16, 32, 64 or 128", R);
-  NF_REQUIRE(n_slices >= 1 && n_slices <= 8, "adapter_linear: %d slices, 1 to 8", n_slices);
-  NF_REQUIRE((long long)n * N < (1ll << 31) && (long long)n * n_slices * R < (1ll << 31), "adapter_linear: %d adapters of %d features are too many", n, N);
-  NF_REQUIRE((uintptr_t)x % 16 == 0 && (uintptr_t)W % 16 == 0 && (uintptr_t)A % 16 == 0 && (uintptr_t)B % 16 == 0 && (uintptr_t)h % 16 == 0 &&
-             (uintptr_t)y % 16 == 0, "adapter_linear: operands must be 16-byte aligned");
-  TcSlices sl{n_slices, {}};
-  for (int i = 0; i < n_slices; ++i) {
-    sl.end[i] = ends[i];
-    NF_REQUIRE(ends[i] > (i ? ends[i - 1] : 0), "adapter_linear: slice %d ends at %d", i, ends[i]);
-  }
-  NF_REQUIRE(ends[n_slices - 1] == N, "adapter_linear: the slices end at %d of %d features", ends[n_slices - 1], N);
-  const int SR = n_slices * R, steps = (K + kAdK - 1) / kAdK;
-  const int row_tiles = (rows + kAdM - 1) / kAdM;
+// Blocks of 128 rows of h that a row tile may need: the adapters that may occur in it.
+static int adapter_places(int rows, int n) {
+  const int most = rows < kAdM ? rows : kAdM;
+  return n < most ? n : most;
+}
+
+// Rows that one pass serves: all, unless h would take more than kScratchBytes (many adapters, many ranks, many rows).
+constexpr long long kScratchBytes = 256ll << 20;
+static int rows_a_pass(int rows, int SR, int n) {
+  if (rows <= kRowsMost) return rows;
+  const long long tile = (long long)adapter_places(rows, n) * kAdM * SR * 4;
+  long long pairs = kScratchBytes / (2 * tile);
+  if (pairs < 1) pairs = 1;
+  return 2 * kAdM * pairs < rows ? (int)(2 * kAdM * pairs) : rows;
+}
+
+// Floats of scratch that nf_adapter_linear needs for `rows` rows, SR numbers of h a row, a pool of n adapters.
+extern "C" long long nf_adapter_scratch(int rows, int SR, int n) {
+  if (rows <= kRowsMost) return (long long)rows * SR;
+  return (long long)((rows_a_pass(rows, SR, n) + kAdM - 1) / kAdM) * adapter_places(rows, n) * kAdM * SR;
+}
+
+static int adapter_pass(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h, void* y, int rows,
+                        int N, int K, int R, int n, const TcSlices& sl, cudaStream_t stream) {
+  const int SR = sl.n * R, steps = (K + kAdK - 1) / kAdK, n_slices = sl.n;
+  const int row_tiles = (rows + kAdM - 1) / kAdM, places = adapter_places(rows, n);
 
   // ---- h
   if (rows <= 16) {
@@ -943,7 +922,7 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
     if (asked) return asked;
     NF_REQUIRE(row_tiles * j_tiles <= 65535, "adapter_linear: %d rows are too many", rows);
     launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, row_tiles * j_tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
-                           ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, rows > kRowsMost ? 1 : 0);
+                           ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, few ? 0 : places, R);
     if (int rc = check_launch("adapter_shrink")) return rc;
   }
 
@@ -980,28 +959,58 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
       if (best < 0 || cost < best) { best = cost; BN = c; ctas = g; }
     }
   }
-  CUtensorMap mb;
+  CUtensorMap mb, mh;
   if (int rc = make_map(&mx, x, rows, K, kAdM)) return rc;
   if (int rc = make_map(&mw, W, N, K, BN / ctas)) return rc;
   if (int rc = make_map(&mb, B, (long long)n * N, R, BN / ctas)) return rc;
+  if (int rc = make_map(&mh, h, (long long)row_tiles * places * n_slices * kAdM, 2 * R, kAdM)) return rc;
   const int f_tiles = feature_tiles(sl, BN);
   const long long n_tiles = (long long)f_tiles * ((rows + kAdM * ctas - 1) / (kAdM * ctas));
   NF_REQUIRE(n_tiles < (1ll << 30), "adapter_linear: %d rows of %d features are too many", rows, N);
-  int stages = (kWideSmem - kWideHead - wide_h_bytes(ctas) - kWideEpilogueWarps * kTurnBytes) / (kAdTile + BN / ctas * 128);
+  int stages = (kWideSmem - kWideHead - kWideEpilogueWarps * kTurnBytes) / (kAdTile + BN / ctas * 128);
   stages = stages > kAdMaxStages ? kAdMaxStages : stages;
   static int asked1 = room_for(adapter_wide_kernel<1>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2>, kWideSmem + 1024);
   if (asked1 || asked2) return 1;
   const int at_once = sm_count() / ctas, grid = ctas * (n_tiles < at_once ? (int)n_tiles : at_once);
   if (ctas == 2)
-    launch_chained_cluster(adapter_wide_kernel<2>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, 2, mx, mw, mb, ids,
-                           (const __nv_bfloat16*)h, (__nv_bfloat16*)y, rows, N, K, R, n, sl, f_tiles, (int)n_tiles, BN, stages);
+    launch_chained_cluster(adapter_wide_kernel<2>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, 2, mx, mw, mb, mh, ids,
+                           (__nv_bfloat16*)y, rows, N, K, R, n, places, sl, f_tiles, (int)n_tiles, BN, stages);
   else
-    launch_chained(adapter_wide_kernel<1>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, mx, mw, mb, ids,
-                   (const __nv_bfloat16*)h, (__nv_bfloat16*)y, rows, N, K, R, n, sl, f_tiles, (int)n_tiles, BN, stages);
+    launch_chained(adapter_wide_kernel<1>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, mx, mw, mb, mh, ids,
+                   (__nv_bfloat16*)y, rows, N, K, R, n, places, sl, f_tiles, (int)n_tiles, BN, stages);
   return check_launch("adapter_wide");
 }
 
-// 0, or the code of the first wait that one of these kernels gave up on since the last call (1 to 7 the wide form and the
+// y = x W^T + the adapters' part (see the head of this file): x [rows, K], W [N, K], A [n, n_slices * R, K], B [n, N, R], y
+// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h: scratch of
+// nf_adapter_scratch(rows, n_slices * R, n) floats.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or
+// 128, bases 16-byte aligned.
+extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h,
+                                 void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, cudaStream_t stream) {
+  if (rows == 0 || N == 0) return 0;
+  NF_REQUIRE(rows > 0 && N > 0 && K > 0 && n > 0, "adapter_linear: bad sizes rows=%d N=%d K=%d n=%d", rows, N, K, n);
+  NF_REQUIRE(K % 8 == 0, "adapter_linear: K=%d must be a multiple of 8", K);
+  NF_REQUIRE(R == 16 || R == 32 || R == 64 || R == 128, "adapter_linear: rank %d is not 16, 32, 64 or 128", R);
+  NF_REQUIRE(n_slices >= 1 && n_slices <= 8, "adapter_linear: %d slices, 1 to 8", n_slices);
+  NF_REQUIRE((long long)n * N < (1ll << 31) && (long long)n * n_slices * R < (1ll << 31), "adapter_linear: %d adapters of %d features are too many", n, N);
+  NF_REQUIRE((uintptr_t)x % 16 == 0 && (uintptr_t)W % 16 == 0 && (uintptr_t)A % 16 == 0 && (uintptr_t)B % 16 == 0 && (uintptr_t)h % 16 == 0 &&
+             (uintptr_t)y % 16 == 0, "adapter_linear: operands must be 16-byte aligned");
+  TcSlices sl{n_slices, {}};
+  for (int i = 0; i < n_slices; ++i) {
+    sl.end[i] = ends[i];
+    NF_REQUIRE(ends[i] > (i ? ends[i - 1] : 0), "adapter_linear: slice %d ends at %d", i, ends[i]);
+  }
+  NF_REQUIRE(ends[n_slices - 1] == N, "adapter_linear: the slices end at %d of %d features", ends[n_slices - 1], N);
+  const int pass = rows_a_pass(rows, n_slices * R, n);
+  for (int t = 0; t < rows; t += pass) {
+    const int now = rows - t < pass ? rows - t : pass;
+    if (int rc = adapter_pass((const __nv_bfloat16*)x + (size_t)t * K, W, A, B, scale, ids + t, h, (__nv_bfloat16*)y + (size_t)t * N, now, N, K, R, n,
+                              sl, stream)) return rc;
+  }
+  return 0;
+}
+
+// 0, or the code of the first wait that one of these kernels gave up on since the last call (1 to 4 the wide form and the
 // first product, 11 to 14 the form for few rows); 100 + 1 + a row whose adapter lay outside the pool.  Synchronises.
 extern "C" int nf_adapter_tc_status() {
   int v[2] = {0, 0}, zero = 0;

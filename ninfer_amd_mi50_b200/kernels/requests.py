@@ -28,6 +28,7 @@ _SIGNATURES = {
     "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _P],
     "nf_adapter_rows_f32": [_P] * 8 + [_I] * 6 + [_P, _P],
     "nf_append_history": [_P] * 4 + [_I] * 3 + [_P],
+    "nf_adapter_scratch": [_I] * 3,
     "nf_logit_rules": [_P] * 11 + [_I] + [_P] * 2 + [_I] * 7 + [_P],
 }
 _functions = {}
@@ -40,6 +41,8 @@ def _function(name: str):
     if f is None:
         f = getattr(_lib.load(), name)
         f.argtypes = _SIGNATURES[name]
+        if name == "nf_adapter_scratch":
+            f.restype = ctypes.c_longlong
         _functions[name] = f
     return f
 
@@ -156,7 +159,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     bf16 = dtype is torch.bfloat16
     if TUNING["adapter"] == "auto" and (K % 8 == 0 if bf16 else K % 4 == 0 and T <= TUNING["adapter_f32_max_rows"]):
-        h = scale.new_empty(T * S * R)
+        h = scale.new_empty(_function("nf_adapter_scratch")(T, S * R, n) if bf16 else T * S * R)
         _call("nf_adapter_linear" if bf16 else "nf_adapter_rows_f32", px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream())
         return out
     # many float32 rows, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
