@@ -908,7 +908,8 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     const bool few = rows <= kRowsMost;
     int turns = sm_count() / (members * row_tiles * j_tiles * (few ? 3 : 1));
     turns = turns < 1 ? 1 : turns > most ? most : turns;
-    const int each = (most + turns - 1) / turns, group = kShrinkCols / JW < each ? kShrinkCols / JW : each;
+    const int each = (most + turns - 1) / turns, cols = few ? kShrinkCols : kShrinkCols / 2;
+    const int group = cols / JW < each ? cols / JW : each;
     const int x_box = rows >= kAdM ? kAdM : (rows + 7) & ~7;
     CUtensorMap ma, mx;
     if (int rc = make_map(&ma, A, (long long)n * SR, K, JW)) return rc;

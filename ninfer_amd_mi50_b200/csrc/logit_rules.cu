@@ -167,11 +167,10 @@ logit_rules_kernel(RuleArgs a) {
   b0 = max(b0, 0);
   b1 = min(b1, a.n_bias);
   int bias_id = -1;                                        // this thread's entry; those beyond as many as threads are read later
-  float bias = 0.f, biased = 0.f;
+  float bias = 0.f;
   if (b0 + tid < b1) {
     bias_id = a.bias_ids[b0 + tid];
     bias = a.bias_values[b0 + tid];
-    if (bias_id >= first && bias_id < last) biased = row[bias_id];
   }
   if (generated)
     for (int i = tid; i < Counts<WORD>::kWords * C / 4; i += kRuleThreads) reinterpret_cast<uint4*>(piece.counts)[i] = make_uint4(0, 0, 0, 0);
@@ -215,6 +214,8 @@ logit_rules_kernel(RuleArgs a) {
       }
     }
   }
+  // (not before: it would hold up the copy for a trip to memory; in place, before anything but the mask has changed it)
+  float biased = bias_id >= first && bias_id < last ? row[bias_id] : 0.f;
   // the log
   if (generated) {
     piece.take(q_first, held);
