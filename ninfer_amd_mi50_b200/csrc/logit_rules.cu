@@ -30,7 +30,6 @@ struct RuleArgs {
   int V, ld_in, ld_out, n_slots, capacity, n_bias, mask_rows, words;
 };
 
-constexpr int kRuleThreads = 512;
 template <int V> struct Int { static constexpr int value = V; };
 
 // Occurrences of one token: in the prompt, and among the generated ones.  A log of up to 65,535 tokens has both in one word.
@@ -62,7 +61,7 @@ template <> struct Counts<false> {
 // What a piece of the vocabulary, tokens [lo, lo + C), has of a row's log: the places [from, end) of it, those from `start` on
 // generated.  (Additions whose results nobody waits for: with the first occurrence of a token noticed by what its addition returns,
 // logs of 131,072 tokens took 18.6 us instead of 11.)
-template <bool WORD>
+template <int THREADS, bool WORD>
 struct PieceLog {
   static constexpr int U = 4;   // runs of four tokens a thread has under way
   unsigned* counts;             // [kWords * C]
@@ -76,12 +75,12 @@ struct PieceLog {
   __device__ __forceinline__ void ask(int q0, int4* t) const {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (4 * (q0 + u * kRuleThreads) < end) t[u] = quads[q0 + u * kRuleThreads];
+      if (4 * (q0 + u * THREADS) < end) t[u] = quads[q0 + u * THREADS];
   }
   __device__ __forceinline__ void take(int q0, const int4* t) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int p = 4 * (q0 + u * kRuleThreads);
+      const int p = 4 * (q0 + u * THREADS);
       if (p >= end) break;
       const int n[4] = {t[u].x, t[u].y, t[u].z, t[u].w};
       if (p >= from && p + 4 <= end) {
@@ -96,7 +95,7 @@ struct PieceLog {
   }
 };
 
-// A CTA takes a piece of WALK * PIECES * 4 * kRuleThreads tokens of one row, counted from the last 16-byte boundary at or before the
+// A CTA takes a piece of WALK * PIECES * 4 * THREADS tokens of one row, counted from the last 16-byte boundary at or before the
 // row's start.  It copies the piece's logits under the mask, WALK steps of PIECES runs of four a thread, and then does what is left to
 // do at the biased tokens and at those that occur in the log, one thread each.  (Done where the logits are copied, the powers and
 // quotients of the few tokens that occur held up nearly every warp: 204 instructions a run of four, 256 rows of 151936 99 us.)
@@ -104,10 +103,10 @@ struct PieceLog {
 // chain from a row's numbers to its log to the counts to the list.  So everything that does not wait for anything is asked for first,
 // the log's loads are under way while the logits are copied, a walked piece's logits are brought into L2 meanwhile, and a walked
 // piece leaves room for three CTAs on an SM (with two 76 us).  One row of 151936 and a short log 3.1 us: the chain and the launch.
-template <int PIECES, int WALK, bool WORD>
-__global__ void __launch_bounds__(kRuleThreads, WALK > 1 ? 3 : 2)
+template <int THREADS, int PIECES, int WALK, bool WORD>
+__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : WALK > 1 ? 3 : 2)
 logit_rules_kernel(RuleArgs a) {
-  constexpr int STEP = kRuleThreads * 4 * PIECES, C = STEP * WALK;
+  constexpr int STEP = THREADS * 4 * PIECES, C = STEP * WALK;
   extern __shared__ __align__(16) unsigned rule_smem[];   // [counts | list]
   __shared__ int listed;
   __shared__ unsigned mask[C / 32 + 2];                   // the piece's words of the row's mask
@@ -130,7 +129,7 @@ logit_rules_kernel(RuleArgs a) {
   auto fetch = [&](int w) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int i0 = lo + w * STEP + 4 * (tid + p * kRuleThreads);
+      const int i0 = lo + w * STEP + 4 * (tid + p * THREADS);
       if (i0 >= 0 && i0 + 4 <= a.V) {
         load4(row + i0, v[p]);
       } else {
@@ -153,17 +152,17 @@ logit_rules_kernel(RuleArgs a) {
   start = max(start, 0);
   int* log = a.history + (size_t)(fits ? slot : 0) * a.capacity;
   // earlier tokens count for the repetition penalty only; the log holds all but the last of the row where that comes with the call
-  PieceLog<WORD> piece{rule_smem, lo, C, reinterpret_cast<const int4*>(log), rep != 1.f ? 0 : start, start,
+  PieceLog<THREADS, WORD> piece{rule_smem, lo, C, reinterpret_cast<const int4*>(log), rep != 1.f ? 0 : start, start,
                        generated ? (a.tokens ? len - 1 : len) : 0};
   unsigned short* list = reinterpret_cast<unsigned short*>(rule_smem + Counts<WORD>::kWords * C);      // [C] places that occur, in any order
   const int q_first = (piece.from >> 2) + tid;
-  int4 held[PieceLog<WORD>::U];
+  int4 held[PieceLog<THREADS, WORD>::U];
   piece.ask(q_first, held);
   const unsigned* bits = m >= 0 && m < a.mask_rows ? a.mask + (size_t)m * a.words : nullptr;
   const int first = max(lo, 0), last = min(lo + C, a.V);    // this piece's tokens
   const int word0 = first >> 5, words = ((last + 31) >> 5) - word0;
   if (bits)
-    for (int i = tid; i < words; i += kRuleThreads) mask[i] = bits[word0 + i];
+    for (int i = tid; i < words; i += THREADS) mask[i] = bits[word0 + i];
   b0 = max(b0, 0);
   b1 = min(b1, a.n_bias);
   int bias_id = -1;                                        // this thread's entry; those beyond as many as threads are read later
@@ -173,7 +172,7 @@ logit_rules_kernel(RuleArgs a) {
     bias = a.bias_values[b0 + tid];
   }
   if (generated)
-    for (int i = tid; i < Counts<WORD>::kWords * C / 4; i += kRuleThreads) reinterpret_cast<uint4*>(piece.counts)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < Counts<WORD>::kWords * C / 4; i += THREADS) reinterpret_cast<uint4*>(piece.counts)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) listed = 0;
   __syncthreads();
 
@@ -185,7 +184,7 @@ logit_rules_kernel(RuleArgs a) {
     if (w > 0 && !in_place) fetch(w);
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int i0 = lo + w * STEP + 4 * (tid + p * kRuleThreads);
+      const int i0 = lo + w * STEP + 4 * (tid + p * THREADS);
       if (i0 + 4 <= 0 || i0 >= a.V) continue;
       const bool inside = i0 >= 0 && i0 + 4 <= a.V;
       unsigned on = 0xfu;                                   // tokens that the mask allows
@@ -219,7 +218,7 @@ logit_rules_kernel(RuleArgs a) {
   // the log
   if (generated) {
     piece.take(q_first, held);
-    for (int q = q_first + PieceLog<WORD>::U * kRuleThreads; 4 * q < piece.end; q += PieceLog<WORD>::U * kRuleThreads) {
+    for (int q = q_first + PieceLog<THREADS, WORD>::U * THREADS; 4 * q < piece.end; q += PieceLog<THREADS, WORD>::U * THREADS) {
       piece.ask(q, held);
       piece.take(q, held);
     }
@@ -241,8 +240,8 @@ logit_rules_kernel(RuleArgs a) {
   __syncthreads();                                          // the counts are complete, the piece is written
   // biased tokens: all of their rules, and they are off the list of the others
   if (b0 < b1) {
-    for (int i = b0 + tid; i < b1; i += kRuleThreads) {
-      if (i >= b0 + kRuleThreads) {
+    for (int i = b0 + tid; i < b1; i += THREADS) {
+      if (i >= b0 + THREADS) {
         bias_id = a.bias_ids[i];
         bias = a.bias_values[i];
         if (bias_id >= first && bias_id < last) biased = row[bias_id];
@@ -259,7 +258,7 @@ logit_rules_kernel(RuleArgs a) {
   }
   // the other tokens that occur
   if (!generated) return;
-  for (int d = 4 * tid; d < C; d += 4 * kRuleThreads) {
+  for (int d = 4 * tid; d < C; d += 4 * THREADS) {
     const uint4 n = Counts<WORD>::any(piece.counts, C, d);
     if (n.x | n.y | n.z | n.w) {
       int at = atomicAdd(&listed, (n.x != 0) + (n.y != 0) + (n.z != 0) + (n.w != 0));
@@ -270,7 +269,7 @@ logit_rules_kernel(RuleArgs a) {
     }
   }
   __syncthreads();
-  for (int k = tid; k < listed; k += kRuleThreads) {
+  for (int k = tid; k < listed; k += THREADS) {
     const int d = list[k], i = lo + d;
     if (i < 0 || i >= a.V || !allowed(i)) continue;
     unsigned c, g;
@@ -326,25 +325,25 @@ extern "C" int nf_logit_rules(const float* logits, float* out, int* history, con
   // (8192), 32 rows 14.3, 13.3 and 17.5, 64 rows 27.0, 25.4 and 39.1 (logs of up to 8,192), 96 and 128 rows the same in the first two.
   const auto ctas = [&](int piece) { return (long long)rows * ((V + 3 + piece - 1) / piece); };
   const bool word = capacity < 65536;
-  const auto run = [&](auto pieces, auto walk, auto packed) {
-    constexpr int P = decltype(pieces)::value, L = decltype(walk)::value, C = kRuleThreads * 4 * P * L;
+  const auto run = [&](auto threads, auto pieces, auto walk, auto packed) {
+    constexpr int T = decltype(threads)::value, P = decltype(pieces)::value, L = decltype(walk)::value, C = T * 4 * P * L;
     constexpr bool W = decltype(packed)::value;
     constexpr int most = C * (4 * Counts<W>::kWords + 2);
     const int bytes = C * 4 * Counts<W>::kWords + 2 * (C < capacity ? C : capacity);      // (the list has a place for every token of a log)
     if (most > 40 * 1024) {
-      static const cudaError_t asked = cudaFuncSetAttribute(logit_rules_kernel<P, L, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      static const cudaError_t asked = cudaFuncSetAttribute(logit_rules_kernel<T, P, L, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (asked != cudaSuccess) note_launch_error(asked);
     }
-    launch_chained(logit_rules_kernel<P, L, W>, dim3((V + 3 + C - 1) / C, rows), dim3(kRuleThreads), (size_t)bytes, stream, a);
+    launch_chained(logit_rules_kernel<T, P, L, W>, dim3((V + 3 + C - 1) / C, rows), dim3(T), (size_t)bytes, stream, a);
   };
   if (ctas(16384) >= 6 * 148) {
-    if (word) run(Int<2>{}, Int<4>{}, Int<1>{}); else run(Int<2>{}, Int<2>{}, Int<0>{});
+    if (word) run(Int<512>{}, Int<2>{}, Int<4>{}, Int<1>{}); else run(Int<512>{}, Int<2>{}, Int<2>{}, Int<0>{});
   } else if (ctas(8192) >= 2 * 148) {
-    if (word) run(Int<2>{}, Int<2>{}, Int<1>{}); else run(Int<2>{}, Int<2>{}, Int<0>{});
+    if (word) run(Int<512>{}, Int<2>{}, Int<2>{}, Int<1>{}); else run(Int<512>{}, Int<2>{}, Int<2>{}, Int<0>{});
   } else if (ctas(4096) >= 2 * 148) {
-    if (word) run(Int<2>{}, Int<1>{}, Int<1>{}); else run(Int<2>{}, Int<1>{}, Int<0>{});
+    if (word) run(Int<512>{}, Int<2>{}, Int<1>{}, Int<1>{}); else run(Int<512>{}, Int<2>{}, Int<1>{}, Int<0>{});
   } else {
-    if (word) run(Int<1>{}, Int<1>{}, Int<1>{}); else run(Int<1>{}, Int<1>{}, Int<0>{});
+    if (word) run(Int<512>{}, Int<1>{}, Int<1>{}, Int<1>{}); else run(Int<1024>{}, Int<1>{}, Int<1>{}, Int<0>{});
   }
   return check_launch("logit_rules");
 }
