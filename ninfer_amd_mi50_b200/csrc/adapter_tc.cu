@@ -180,7 +180,7 @@ struct __align__(8) ShrinkBars {
 // kernels may meet on an SM, from several streams too, has to find its columns at once.  One CTA of this kernel (256 columns, more
 // than half of the shared memory) beside those of adapter_rows_kernel (64 each, that split k 36 KB each) do; the wide kernel, and
 // all others that take all columns, leave no shared memory for either.
-constexpr size_t kShrinkSmemLeast = 118 * 1024;
+constexpr size_t kShrinkSmemLeast = 118 * 1024, kShrinkSmemMost = 204 * 1024;
 constexpr int kShrinkCols = 256;        // columns of an accumulator: numbers of h of all adapters of a pass
 
 // 8 numbers of h as the nearest bfloat16 and what that leaves.
@@ -274,8 +274,6 @@ adapter_shrink_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         if (lane < count) tma_load_2d(st + kAdTile + lane * JW * 128, &map_a, ks * kAdK, mine * SR + j0, &bars->full[s]);
       }
     }
-    // The product behind this may begin: what came before is complete.  Not sooner, or W's rows, which it asks for at once, would
-    // come before the adapters'.
     if (!ok && lane == 0) {
       for (int j = max(0, issued - stages); j < issued; ++j)
         for (unsigned i = 0; i < (1u << 20); ++i)
@@ -646,6 +644,7 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 // ---- few rows ----------------------------------------------------------------------------------------------------------------
 
 constexpr int kRowsMost = 64;              // rows that adapter_rows_kernel takes
+constexpr int kStagedLeast = 128;          // numbers of h of a member's rows and a slice from which they are fetched at once
 
 struct __align__(8) RowsBars {
   unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full;
@@ -658,6 +657,9 @@ struct __align__(8) RowsBars {
 constexpr int kRowsThreads = 320;
 constexpr int kRowsAtOnce = 4;             // rows of x whose rows of B a thread has under way
 
+// STAGED: a member fetches h of its rows at once, into the stages, which nothing uses any more by then; read where it is used, every row
+// and 16 ranks are a trip to L2 in turn (64 rows of 2048 x 9216 and rank 16 21.1 us instead of 24.2; a single row 8.1 instead of 7.1).
+template <bool STAGED>
 __global__ void __launch_bounds__(kRowsThreads, 2)
 adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const int* __restrict__ ids,
                     const float* __restrict__ h, const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows,
@@ -781,16 +783,31 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
   if (warp >= 2) {
     const int SR = slices.n * R;
-    chain_wait(h);
-    for (int t0 = t_first + turn; t0 < t_last; t0 += 2 * kRowsAtOnce) {
-      if (t0 != t_first + turn) ask(t0);
-      float sum[kRowsAtOnce];
+    float* hs = reinterpret_cast<float*>(stage0);
+    float sum[kRowsAtOnce];
+    auto add_up = [&](int t0) {          // the members' sums, in their order
 #pragma unroll
       for (int i = 0; i < kRowsAtOnce; ++i) {
         const int tl = min(t0 + 2 * i, t_last - 1) - t_first;
         sum[i] = 0.f;
         for (int m = 0; m < members; ++m) sum[i] += sums[((size_t)m * share + tl) * kAdM + d];
       }
+    };
+    if (STAGED && t_first < t_last) add_up(t_first + turn);
+    chain_wait(h);
+    if (STAGED) {
+      const int pieces = R >> 2;
+      for (int i = threadIdx.x - 64; i < (t_last - t_first) * pieces; i += kRowsThreads - 64) {
+        const int tl = i / pieces;
+        float v[4];
+        load4(h + (size_t)(t_first + tl) * SR + w.slice * R + 4 * (i - tl * pieces), v);
+        store4(hs + 4 * i, v);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    for (int t0 = t_first + turn; t0 < t_last; t0 += 2 * kRowsAtOnce) {
+      if (t0 != t_first + turn) ask(t0);
+      if (!STAGED || t0 != t_first + turn) add_up(t0);
       for (int j = 0; j < R; j += 16) {
         if (j > 0) {
 #pragma unroll
@@ -804,12 +821,12 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 #pragma unroll
         for (int i = 0; i < kRowsAtOnce; ++i)
           if (a[i] >= 0) {
-            const float* hr = h + (size_t)(t0 + 2 * i) * SR + w.slice * R + j;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               float bv[8], hv[8];
               unpack8(raw[i][c], bv);
-              load8(hr + 8 * c, hv);
+              if (STAGED) load8(hs + (t0 + 2 * i - t_first) * R + j + 8 * c, hv);
+              else load8(h + (size_t)(t0 + 2 * i) * SR + w.slice * R + j + 8 * c, hv);
 #pragma unroll
               for (int e = 0; e < 8; ++e) sum[i] = fmaf(hv[e], bv[e], sum[i]);
             }
@@ -853,6 +870,28 @@ int room_for(F* kernel, size_t smem) {
   return 0;
 }
 
+// Clusters of `members` (1, 2, 4 or 8) CTAs that run at once.  A cluster lies within a part of the device, whose SMs are no multiple of
+// 4 or 8 (of a CTA that fills an SM 74 clusters of two, 33 of four, 15 of eight), and clusters beyond that begin when others end.
+template <typename F>
+int clusters_at_once(F* kernel, int threads, size_t smem, int members) {
+  static int known[4] = {};
+  int& n = known[members == 8 ? 3 : members >> 1];
+  if (!n) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(members);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = members;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+  }
+  return n;
+}
+
 }  // namespace
 
 int adapter_shrink_simt(const void* x, const void* A, const float* scale, const int* ids, float* h, int rows, int K, int SR, int n,
@@ -861,13 +900,6 @@ int adapter_shrink_simt(const void* x, const void* A, const float* scale, const 
 }  // namespace nf
 
 using namespace nf;
-
-static int shrink_members(int rows, int K, int SR) {
-  const int tiles = ((rows + kAdM - 1) / kAdM) * ((SR + kAdM - 1) / kAdM), steps = (K + kAdK - 1) / kAdK;
-  int p = 1;
-  while (p < 8 && 2 * p * tiles <= sm_count() && steps >= 4 * p) p *= 2;
-  return p;
-}
 
 // Blocks of 128 rows of h that a row tile may need: the adapters that may occur in it.
 static int adapter_places(int rows, int n) {
@@ -900,16 +932,33 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
   if (rows <= 16) {
     if (int rc = adapter_shrink_simt(x, A, scale, ids, h, rows, K, SR, n, stream)) return rc;
   } else {
-    const int members = shrink_members(rows, K, SR);
-    const int JW = SR < kAdM ? SR : kAdM, j_tiles = (SR + JW - 1) / JW;
+    static int asked = room_for(adapter_shrink_tc_kernel, kShrinkSmemMost);
+    if (asked) return asked;
+    const int JW = SR < kAdM ? SR : kAdM, j_tiles = (SR + JW - 1) / JW, tiles = row_tiles * j_tiles;
     const int most = n < kAdM ? (n < rows ? n : rows) : (rows < kAdM ? rows : kAdM);      // adapters that a tile's rows may have
-    // CTAs that take a tile's adapters in turn.  Behind few rows comes a product that streams W: a third of the SMs is enough for what
-    // it would otherwise wait for (64 rows of 3584 x 3584, 48 adapters of rank 32: on all of them 24.7 us, on a third 22.5).
+    // How many members split k, and how many CTAs take a tile's adapters in turn: the least time by a simple account in cycles of what a CTA
+    // and a group of adapters cost however short, of a step's bytes and of rounds of clusters, for tiles with as many adapters as may be and
+    // for tiles with two (1024 rows of 2048 x 4608, 24 adapters of rank 16 among all rows: 8 members, 2 in turn 57 us, 4 and 4 38).  Behind
+    // few rows comes a product that streams W: two SMs of five are enough for what it would otherwise wait for (64 rows of 3584 x 3584, 48
+    // adapters of rank 32: 19.7 us, on all of them 25.3).
     const bool few = rows <= kRowsMost;
-    int turns = sm_count() / (members * row_tiles * j_tiles * (few ? 3 : 1));
-    turns = turns < 1 ? 1 : turns > most ? most : turns;
-    const int each = (most + turns - 1) / turns, cols = few ? kShrinkCols : kShrinkCols / 2;
-    const int group = cols / JW < each ? cols / JW : each;
+    const int cols = few ? kShrinkCols : kShrinkCols / 2;
+    int members = 1, turns = 1;
+    long long best = -1;
+    for (int m = 1; m <= 8 && (m == 1 || steps >= 2 * m); m *= 2) {
+      int at_once = clusters_at_once(adapter_shrink_tc_kernel, 192, kShrinkSmemMost, m);
+      if (few) at_once = at_once * 2 / 5;
+      const int z_most = at_once / tiles < 1 ? 1 : at_once / tiles > most ? most : at_once / tiles;
+      for (int z = 1; z <= z_most; ++z) {
+        const auto time = [&](int adapters) {
+          const int each = (adapters + z - 1) / z, group = cols / JW < each ? cols / JW : each;
+          return 6000 + (each + group - 1) / group * (2000 + (steps + m - 1) / m * (kAdTile + group * JW * 128) / 48);
+        };
+        const long long cost = (long long)((tiles * z + at_once - 1) / at_once) * (time(most) + time(most < 2 ? most : 2));
+        if (best < 0 || cost < best) { best = cost; members = m; turns = z; }
+      }
+    }
+    const int each = (most + turns - 1) / turns, group = cols / JW < each ? cols / JW : each;
     const int x_box = rows >= kAdM ? kAdM : (rows + 7) & ~7;
     CUtensorMap ma, mx;
     if (int rc = make_map(&ma, A, (long long)n * SR, K, JW)) return rc;
@@ -919,10 +968,8 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     stages = stages > 8 ? 8 : stages < 2 ? 2 : stages;
     size_t smem = 2048 + (size_t)stages * stage + sums;
     smem = smem < kShrinkSmemLeast ? kShrinkSmemLeast : smem;
-    static int asked = room_for(adapter_shrink_tc_kernel, 204 * 1024);
-    if (asked) return asked;
-    NF_REQUIRE(row_tiles * j_tiles <= 65535, "adapter_linear: %d rows are too many", rows);
-    launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, row_tiles * j_tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
+    NF_REQUIRE(tiles <= 65535, "adapter_linear: %d rows are too many", rows);
+    launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
                            ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, few ? 0 : places, R);
     if (int rc = check_launch("adapter_shrink")) return rc;
   }
@@ -931,20 +978,26 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
   CUtensorMap mx, mw;
   if (rows <= kRowsMost) {
     const int NT = (rows + 15) & ~15, tiles = feature_tiles(sl, kAdM);
+    // As many members as have all clusters begin at once, two CTAs an SM, one where the first product runs; clusters of 4 and 8 leave SMs
+    // over (8 rows of 2048 x 4608: 8 members, of whose 36 clusters some came late, 12.5 us, 4 members 9.7; 64 rows 19.0 and 14.9).
+    const int slots = 2 * sm_count() - (rows > 16 ? sm_count() / 24 * 8 : 0);
+    const auto fit = [&](int m) { return m * tiles <= (m == 2 ? 2 * sm_count() : slots - 8 * (m - 1)); };
     int members = 1;
-    while (members < 8 && 2 * members * tiles <= 2 * sm_count() && steps >= 4 * members) members *= 2;
+    while (members < 8 && steps >= 4 * members && fit(2 * members)) members *= 2;
     if (int rc = make_map(&mw, W, N, K, kAdM)) return rc;
     if (int rc = make_map(&mx, x, rows, K, NT)) return rc;
     const int stage = kAdTile + NT * 128, here = (steps + members - 1) / members, share = (rows + members - 1) / members;
     const int sums = members * share * kAdM * 4;
     int stages = (104 * 1024 - sums) / stage;
     stages = stages > here ? here : stages;
+    while (stages * stage < share * R * 4) ++stages;      // (h of a member's rows takes their place)
     const size_t smem = 2048 + (size_t)stages * stage + sums;
-    static int asked = room_for(adapter_rows_kernel, 108 * 1024);
-    if (asked) return asked;
+    static int asked = room_for(adapter_rows_kernel<false>, 108 * 1024), asked_staged = room_for(adapter_rows_kernel<true>, 108 * 1024);
+    if (asked || asked_staged) return 1;
     NF_REQUIRE(tiles <= 65535, "adapter_linear: %d features are too many", N);
-    launch_chained_cluster(adapter_rows_kernel, dim3(members, tiles), dim3(kRowsThreads), smem, stream, members, mw, mx, ids, (const float*)h,
-                           (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows, N, K, R, n, sl, NT, stages);
+    launch_chained_cluster(share * R >= kStagedLeast ? adapter_rows_kernel<true> : adapter_rows_kernel<false>, dim3(members, tiles),
+                           dim3(kRowsThreads), smem, stream, members, mw, mx, ids, (const float*)h, (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows,
+                           N, K, R, n, sl, NT, stages);
     return check_launch("adapter_rows");
   }
   // The tile: the one whose rounds take the least, a round's time being that of the products or of the operands' way into
