@@ -16,8 +16,9 @@
 //
 // `adapter_rows_kernel`, few rows: the time is that of reading W once.  W is the 128-row operand, the rows of x the other; the
 // CTAs of a cluster share a tile of 128 features and split k; their sums meet through distributed shared memory, each CTA
-// adding up the rows it owns, in the order of the CTAs, and adding the adapters' part: a thread a feature, whose row of B it
-// reads from memory once for each row of x with another adapter than the one before.
+// adding up the rows it owns, in the order of the CTAs.  The adapters' part is added there, a thread a feature, whose row of B it
+// reads from memory once for each row of x with another adapter than the one before; or, where that is much (many rows or ranks),
+// it is a few more steps of the product, as in the wide kernel, an adapter's steps taken by one CTA of the cluster.
 #define NF_CHAIN_CLASS 0x40
 #include "tcgen05.cuh"
 
@@ -178,8 +179,8 @@ struct __align__(8) ShrinkBars {
 
 // CTAs of a cluster wait for one another, and an allocation of tensor memory waits for the SM's other CTAs: whatever of these
 // kernels may meet on an SM, from several streams too, has to find its columns at once.  One CTA of this kernel (256 columns, more
-// than half of the shared memory) beside those of adapter_rows_kernel (64 each, that split k 36 KB each) do; the wide kernel, and
-// all others that take all columns, leave no shared memory for either.
+// than half of the shared memory) beside those of adapter_rows_kernel (64 each, that split k 36 KB each; of more than 64 rows 128, and nearly
+// all of the shared memory) do; the wide kernel, and all others that take all columns, leave no shared memory for either.
 constexpr size_t kShrinkSmemLeast = 118 * 1024, kShrinkSmemMost = 204 * 1024;
 constexpr int kShrinkCols = 256;        // columns of an accumulator: numbers of h of all adapters of a pass
 
@@ -643,8 +644,8 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------
 
-constexpr int kRowsMost = 64;              // rows that adapter_rows_kernel takes
-constexpr int kStagedLeast = 128;          // numbers of h of a member's rows and a slice from which they are fetched at once
+constexpr int kRowsMost = 64;              // rows that adapter_rows_kernel takes whatever the other sizes
+constexpr int kStagedLeast = 128, kBlocksAbove = 512;      // numbers of h of a member's rows and a slice: see RowsForm
 
 struct __align__(8) RowsBars {
   unsigned long long full[kAdMaxStages], empty[kAdMaxStages], acc_full;
@@ -655,15 +656,25 @@ struct __align__(8) RowsBars {
 // grid: (members of the cluster, feature tiles).  320 threads: producer, MMA, eight epilogue warps (two threads a feature, rows of
 // x in turn).
 constexpr int kRowsThreads = 320;
+enum RowsForm { kRowsPlain, kRowsStaged, kRowsBlocks };
 constexpr int kRowsAtOnce = 4;             // rows of x whose rows of B a thread has under way
 
-// STAGED: a member fetches h of its rows at once, into the stages, which nothing uses any more by then; read where it is used, every row
-// and 16 ranks are a trip to L2 in turn (64 rows of 2048 x 9216 and rank 16 21.1 us instead of 24.2; a single row 8.1 instead of 7.1).
-template <bool STAGED>
+// The adapters' part, by FORM.  kRowsPlain: added up by a thread a feature, which reads its row of B while W is read, and h.
+// kRowsStaged: a member fetches h of its rows at once, into the stages, which nothing uses any more by then; read where it is used, every
+// row and 16 ranks are a trip to L2 in turn (64 rows of 2048 x 9216 and rank 16 21.1 us instead of 22.5; a single row 8.1 instead of 7.1).
+// kRowsBlocks: steps of the product, h in the blocks of the wide kernel, rows of B brought into L2 while W is read.  64 rows of 2048 x
+// 3584, 24 adapters: rank 16 18.3 us instead of 12.2, the products, their sums and their way to the owners now come behind h; rank 64 23.1
+// instead of 36.1, rank 128 35.6 instead of 62.8.
+// What bounds it: one row of 2048 x 2048 takes 7.1 us, its 8.4 MB 1.3: launch, the first loads, the members' sums, h and the rows of y,
+// one after the other.  64 rows of 3584 x 3584 with 48 adapters of rank 32 take 19.6 us, their 43 MB 6.7: h is there after 12, W's sums
+// by then, and the adapters' part takes 4.
+template <RowsForm FORM>
 __global__ void __launch_bounds__(kRowsThreads, 2)
-adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const int* __restrict__ ids,
-                    const float* __restrict__ h, const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows,
-                    int N, int K, int R, int n, const __grid_constant__ TcSlices slices, int NT, int stages) {
+adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b,
+                    const __grid_constant__ CUtensorMap map_h, const int* __restrict__ ids, const float* __restrict__ h,
+                    const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows, int N, int K, int R, int n,
+                    const __grid_constant__ TcSlices slices, int NT, int stages) {
+  constexpr bool STAGED = FORM == kRowsStaged, BLOCKS = FORM == kRowsBlocks;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   RowsBars* bars = reinterpret_cast<RowsBars*>(smem);
@@ -682,7 +693,8 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
-  if (warp == 1) tc_alloc<1>(&bars->tmem_base, 64);
+  const unsigned columns = NT > 64 ? 128 : 64;
+  if (warp == 1) tc_alloc<1>(&bars->tmem_base, columns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -715,22 +727,47 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
   };
 
+  // BLOCKS: this member's adapters, those whose place among the rows' is the member's modulo the members; an adapter's steps as in the
+  // wide kernel
+  const int r_steps = (R + kAdK - 1) / kAdK, h_steps = R <= 32 ? 1 : 2 * r_steps;
+  TileIds<1> tids;
+  if (BLOCKS && warp < 3) tids.load(ids, 0, rows, n);
+  auto own_adapters = [&](auto each) {         // each(adapter, place) until it says no
+    int place = 0;
+    for (int a = tids.next(-1); a != kNone; a = tids.next(a), ++place)
+      if (place % members == member && !each(a, place)) break;
+  };
+
   if (warp == 0) {
     Ring ring;
-    int it = 0;
+    int issued = 0;
     const int count = k_last - k_first;
-    for (; it < count; ++it, ring.next(stages)) {
-      if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 11)) break;
+    auto step = [&](const CUtensorMap* mw, int kw, int w_row, const CUtensorMap* mx, int kx, int x_row) {
+      if (!warp_wait(&bars->empty[ring.s], ring.phase ^ 1, stop, 11)) return false;
       unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
       if (elect_one()) {
         mbar_expect_tx(&bars->full[ring.s], stage_bytes);
-        tma_load_2d(st, &map_w, (k_first + it) * kAdK, w.f0, &bars->full[ring.s]);
-        tma_load_2d(st + kAdTile, &map_x, (k_first + it) * kAdK, 0, &bars->full[ring.s]);
+        tma_load_2d(st, mw, kw, w_row, &bars->full[ring.s]);
+        tma_load_2d(st + kAdTile, mx, kx, x_row, &bars->full[ring.s]);
       }
       __syncwarp();
+      ++issued;
+      ring.next(stages);
+      return true;
+    };
+    bool ok = true;
+    for (int it = 0; it < count && ok; ++it) ok = step(&map_w, (k_first + it) * kAdK, w.f0, &map_x, (k_first + it) * kAdK, 0);
+    if (BLOCKS) {
+      chain_wait();
+      if (ok)
+        own_adapters([&](int a, int place) {
+          for (int e = 0; e < h_steps && ok; ++e)
+            ok = step(&map_b, e % r_steps * kAdK, a * N + w.f0, &map_h, e * kAdK, (place * slices.n + w.slice) * kAdM);
+          return ok;
+        });
     }
-    if (it < count)
-      for (int j = max(0, it - stages); j < it; ++j)
+    if (!ok)
+      for (int j = max(0, issued - stages); j < issued; ++j)
         for (unsigned i = 0; i < (1u << 20); ++i)
           if (mbar_try(&bars->full[j % stages], (j / stages) & 1)) break;
     __syncwarp();
@@ -739,8 +776,9 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     Ring ring;
     const unsigned idesc = ad_instr_desc(NT, kAdM);
     const int count = k_last - k_first;
+    bool ok = true;
     for (int it = 0; it < count; ++it, ring.next(stages)) {
-      if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 13)) break;
+      if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 13)) { ok = false; break; }
       tc_fence_after();
       unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
       const unsigned long long dw = smem_desc(st), dx = smem_desc(st + kAdTile);
@@ -748,13 +786,46 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 #pragma unroll
         for (int kk = 0; kk < kAdK / 16; ++kk) tc_mma(tmem, dw + 2 * kk, dx + 2 * kk, idesc, it > 0 || kk > 0 ? 1u : 0u);
         tc_commit(&bars->empty[ring.s]);
-        if (it + 1 == count) tc_commit(&bars->acc_full);
+        if (!BLOCKS && it + 1 == count) tc_commit(&bars->acc_full);
       }
+      __syncwarp();
+    }
+    if (BLOCKS && ok) {
+      const int n_kk = min(R, kAdK) / 16;
+      own_adapters([&](int, int) {
+        for (int e = 0; e < h_steps; ++e, ring.next(stages)) {
+          if (!warp_wait(&bars->full[ring.s], ring.phase, stop, 13)) return ok = false;
+          tc_fence_after();
+          unsigned char* st = stage0 + (size_t)ring.s * stage_bytes;
+          const unsigned long long db = smem_desc(st), dh = smem_desc(st + kAdTile);
+          if (elect_one()) {
+            for (int kk = 0; kk < n_kk; ++kk) {
+              tc_mma(tmem, db + 2 * kk, dh + 2 * kk, idesc, 1u);
+              if (R <= 32) tc_mma(tmem, db + 2 * kk, dh + 2 * (n_kk + kk), idesc, 1u);
+            }
+            tc_commit(&bars->empty[ring.s]);
+          }
+          __syncwarp();
+        }
+        return true;
+      });
+      if (ok && elect_one()) tc_commit(&bars->acc_full);
       __syncwarp();
     }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
-    ask(t_first + turn);
+    if (BLOCKS) {
+      // rows of B into L2 while W is read: the steps that fetch them wait for h
+      if (warp == 2)
+        own_adapters([&](int a, int) {
+          if (lane == 0)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(B + ((size_t)a * N + w.f0) * R), "r"(w.width * R * 2) : "memory");
+          return true;
+        });
+    } else {
+      ask(t_first + turn);
+    }
+    __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // every member is there: its shared memory may be written
     if (warp_wait(&bars->acc_full, 0, stop, 14)) {
       tc_fence_after();
@@ -779,7 +850,7 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   cluster_barrier();                   // all sums are there, and nothing of tensor memory is still to be read
   if (warp == 1) {
     tc_fence_after();
-    tc_dealloc<1>(tmem, 64);
+    tc_dealloc<1>(tmem, columns);
   }
   if (warp >= 2) {
     const int SR = slices.n * R;
@@ -793,6 +864,15 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         for (int m = 0; m < members; ++m) sum[i] += sums[((size_t)m * share + tl) * kAdM + d];
       }
     };
+    if (BLOCKS) {
+      for (int t0 = t_first + turn; t0 < t_last; t0 += 2 * kRowsAtOnce) {
+        add_up(t0);
+#pragma unroll
+        for (int i = 0; i < kRowsAtOnce; ++i)
+          if (t0 + 2 * i < t_last && d < w.width) y[(size_t)(t0 + 2 * i) * N + f] = __float2bfloat16_rn(sum[i]);
+      }
+      return;
+    }
     if (STAGED && t_first < t_last) add_up(t_first + turn);
     chain_wait(h);
     if (STAGED) {
@@ -919,14 +999,32 @@ static int rows_a_pass(int rows, int SR, int n) {
 
 // Floats of scratch that nf_adapter_linear needs for `rows` rows, SR numbers of h a row, a pool of n adapters.
 extern "C" long long nf_adapter_scratch(int rows, int SR, int n) {
-  if (rows <= kRowsMost) return (long long)rows * SR;
+  if (rows <= 16) return (long long)rows * SR;
   return (long long)((rows_a_pass(rows, SR, n) + kAdM - 1) / kAdM) * adapter_places(rows, n) * kAdM * SR;
 }
 
+// One pass; the rows that an error names are counted from its first.
 static int adapter_pass(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h, void* y, int rows,
                         int N, int K, int R, int n, const TcSlices& sl, cudaStream_t stream) {
   const int SR = sl.n * R, steps = (K + kAdK - 1) / kAdK, n_slices = sl.n;
   const int row_tiles = (rows + kAdM - 1) / kAdM, places = adapter_places(rows, n);
+
+  // ---- which kernel the product is, and how it is split
+  const int NT = (rows + 15) & ~15, f_tiles128 = feature_tiles(sl, kAdM);
+  int parts = 1, share = rows;              // members of a cluster of adapter_rows_kernel, rows of x that each adds up
+  bool blocks = false;
+  if (rows <= kAdM) {
+    // As many members as have all clusters begin at once: two CTAs an SM, one where the first product runs (of more than 64 rows one, and
+    // none); clusters of 4 and 8 leave SMs over (8 rows of 2048 x 4608: 8 members, of whose 36 clusters some came late, 12.5 us, 4 members
+    // 9.7; 64 rows 19.0 and 14.9).
+    const int slots = (rows > kRowsMost ? 1 : 2) * sm_count() - (rows > 16 ? sm_count() / 24 * 8 : 0);
+    const auto fit = [&](int m) { return m * f_tiles128 <= (m == 2 && rows <= kRowsMost ? 2 * sm_count() : slots - 8 * (m - 1)); };
+    while (parts < 8 && steps >= 4 * parts && fit(2 * parts)) parts *= 2;
+    share = (rows + parts - 1) / parts;
+    // (between them: a thread's numbers of h, of all the rows that it adds up; of more than 64 rows the other way is the wide kernel, which
+    // splits no k: 100 rows of 3584 x 3584 and rank 16 24 us instead of 36, of 3584 x 7168, where no two members have room, 44 instead of 37)
+    blocks = rows > 16 && (rows > kRowsMost ? parts > 1 : share * R > kBlocksAbove);
+  }
 
   // ---- h
   if (rows <= 16) {
@@ -942,12 +1040,14 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     // few rows comes a product that streams W: two SMs of five are enough for what it would otherwise wait for (64 rows of 3584 x 3584, 48
     // adapters of rank 32: 19.7 us, on all of them 25.3).
     const bool few = rows <= kRowsMost;
-    const int cols = few ? kShrinkCols : kShrinkCols / 2;
+    const int cols = few || blocks ? kShrinkCols : kShrinkCols / 2;
     int members = 1, turns = 1;
     long long best = -1;
     for (int m = 1; m <= 8 && (m == 1 || steps >= 2 * m); m *= 2) {
       int at_once = clusters_at_once(adapter_shrink_tc_kernel, 192, kShrinkSmemMost, m);
       if (few) at_once = at_once * 2 / 5;
+      else if (blocks) at_once = at_once * (sm_count() - parts * f_tiles128) / sm_count();
+      if (at_once < 1) continue;
       const int z_most = at_once / tiles < 1 ? 1 : at_once / tiles > most ? most : at_once / tiles;
       for (int z = 1; z <= z_most; ++z) {
         const auto time = [&](int adapters) {
@@ -970,34 +1070,36 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     smem = smem < kShrinkSmemLeast ? kShrinkSmemLeast : smem;
     NF_REQUIRE(tiles <= 65535, "adapter_linear: %d rows are too many", rows);
     launch_chained_cluster(adapter_shrink_tc_kernel, dim3(members, tiles, turns), dim3(192), smem, stream, members, ma, mx, scale,
-                           ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, few ? 0 : places, R);
+                           ids, h, rows, K, SR, n, row_tiles, x_box, JW, group, stages, few && !blocks ? 0 : places, R);
     if (int rc = check_launch("adapter_shrink")) return rc;
   }
 
   // ---- the shared product and the adapters' part
-  CUtensorMap mx, mw;
-  if (rows <= kRowsMost) {
-    const int NT = (rows + 15) & ~15, tiles = feature_tiles(sl, kAdM);
-    // As many members as have all clusters begin at once, two CTAs an SM, one where the first product runs; clusters of 4 and 8 leave SMs
-    // over (8 rows of 2048 x 4608: 8 members, of whose 36 clusters some came late, 12.5 us, 4 members 9.7; 64 rows 19.0 and 14.9).
-    const int slots = 2 * sm_count() - (rows > 16 ? sm_count() / 24 * 8 : 0);
-    const auto fit = [&](int m) { return m * tiles <= (m == 2 ? 2 * sm_count() : slots - 8 * (m - 1)); };
-    int members = 1;
-    while (members < 8 && steps >= 4 * members && fit(2 * members)) members *= 2;
+  CUtensorMap mx, mw, mb, mh;
+  if (rows <= kRowsMost || blocks) {
     if (int rc = make_map(&mw, W, N, K, kAdM)) return rc;
     if (int rc = make_map(&mx, x, rows, K, NT)) return rc;
-    const int stage = kAdTile + NT * 128, here = (steps + members - 1) / members, share = (rows + members - 1) / members;
-    const int sums = members * share * kAdM * 4;
-    int stages = (104 * 1024 - sums) / stage;
-    stages = stages > here ? here : stages;
-    while (stages * stage < share * R * 4) ++stages;      // (h of a member's rows takes their place)
+    const int stage = kAdTile + NT * 128, here = (steps + parts - 1) / parts, sums = parts * share * kAdM * 4;
+    int stages = ((NT > 64 ? 200 : 104) * 1024 - sums) / stage;
+    if (!blocks) {
+      stages = stages > here ? here : stages;
+      while (stages * stage < share * R * 4) ++stages;      // (h of a member's rows takes their place)
+    }
+    stages = stages > kAdMaxStages ? kAdMaxStages : stages;
     const size_t smem = 2048 + (size_t)stages * stage + sums;
-    static int asked = room_for(adapter_rows_kernel<false>, 108 * 1024), asked_staged = room_for(adapter_rows_kernel<true>, 108 * 1024);
-    if (asked || asked_staged) return 1;
-    NF_REQUIRE(tiles <= 65535, "adapter_linear: %d features are too many", N);
-    launch_chained_cluster(share * R >= kStagedLeast ? adapter_rows_kernel<true> : adapter_rows_kernel<false>, dim3(members, tiles),
-                           dim3(kRowsThreads), smem, stream, members, mw, mx, ids, (const float*)h, (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows,
-                           N, K, R, n, sl, NT, stages);
+    static int asked = room_for(adapter_rows_kernel<kRowsPlain>, 108 * 1024), asked_staged = room_for(adapter_rows_kernel<kRowsStaged>, 108 * 1024),
+               asked_blocks = room_for(adapter_rows_kernel<kRowsBlocks>, 204 * 1024);
+    if (asked || asked_staged || asked_blocks) return 1;
+    NF_REQUIRE(f_tiles128 <= 65535, "adapter_linear: %d features are too many", N);
+    mb = mh = mw;
+    if (blocks) {
+      if (int rc = make_map(&mb, B, (long long)n * N, R, kAdM)) return rc;
+      if (int rc = make_map(&mh, h, (long long)places * n_slices * kAdM, 2 * R, NT)) return rc;
+    }
+    const auto kernel = blocks ? adapter_rows_kernel<kRowsBlocks>
+                               : share * R >= kStagedLeast ? adapter_rows_kernel<kRowsStaged> : adapter_rows_kernel<kRowsPlain>;
+    launch_chained_cluster(kernel, dim3(parts, f_tiles128), dim3(kRowsThreads), smem, stream, parts, mw, mx, mb, mh, ids, (const float*)h,
+                           (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows, N, K, R, n, sl, NT, stages);
     return check_launch("adapter_rows");
   }
   // The tile: the one whose rounds take the least, a round's time being that of the products or of the operands' way into
@@ -1013,7 +1115,6 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
       if (best < 0 || cost < best) { best = cost; BN = c; ctas = g; }
     }
   }
-  CUtensorMap mb, mh;
   if (int rc = make_map(&mx, x, rows, K, kAdM)) return rc;
   if (int rc = make_map(&mw, W, N, K, BN / ctas)) return rc;
   if (int rc = make_map(&mb, B, (long long)n * N, R, BN / ctas)) return rc;
@@ -1036,9 +1137,9 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
 }
 
 // y = x W^T + the adapters' part (see the head of this file): x [rows, K], W [N, K], A [n, n_slices * R, K], B [n, N, R], y
-// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h: scratch of
-// nf_adapter_scratch(rows, n_slices * R, n) floats.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64 or
-// 128, bases 16-byte aligned.
+// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h: scratch of nf_adapter_scratch(rows, n_slices * R, n)
+// floats.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64
+// or 128, bases 16-byte aligned.
 extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h,
                                  void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;

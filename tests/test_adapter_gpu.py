@@ -47,6 +47,11 @@ SIZES = [
     (64, 1024, [300, 44], 9, 16), (65, 136, [256, 256], 3, 64), (127, 192, [80], 128, 16), (128, 320, [130], 2, 128),
     (129, 320, [272, 16], 5, 16), (200, 640, [520], 6, 32), (257, 1032, [144, 300], 3, 64), (300, 128, [40, 40, 600], 11, 16),
     (513, 456, [1030], 4, 16),
+    # the adapters' part as steps of a product that splits k: all members, an uneven share of rows, adapters and ranks
+    (24, 520, [700], 5, 128), (41, 1000, [130, 6], 12, 64), (64, 512, [300, 140], 64, 128), (66, 1032, [1000, 72], 66, 16),
+    (97, 2048, [640], 7, 32), (128, 96, [200], 3, 32), (128, 1024, [24, 8, 256], 128, 128),
+    # many rows, adapters and ranks: passes of 512 rows, the last of 88 and of 28
+    (600, 64, [16] * 8, 128, 128), (540, 64, [16] * 8, 128, 128),
 ]
 
 
