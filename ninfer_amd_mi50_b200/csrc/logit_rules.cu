@@ -32,6 +32,8 @@ struct RuleArgs {
 
 template <int V> struct Int { static constexpr int value = V; };
 
+constexpr int kSharedLog = 16384;      // tokens of a log from which a cluster shares it out
+
 // Occurrences of one token: in the prompt, and among the generated ones.  A log of up to 65,535 tokens has both in one word.
 template <bool WORD> struct Counts;
 template <> struct Counts<true> {
@@ -58,19 +60,19 @@ template <> struct Counts<false> {
   }
 };
 
-// What a piece of the vocabulary, tokens [lo, lo + C), has of a row's log: the places [from, end) of it, those from `start` on
+// What tokens [lo, lo + span) of the vocabulary have of a row's log: the places [from, end) of it, those from `start` on
 // generated.  (Additions whose results nobody waits for: with the first occurrence of a token noticed by what its addition returns,
-// logs of 131,072 tokens took 18.6 us instead of 11.)
+// long logs took 1.7 times as long.)
 template <int THREADS, bool WORD>
 struct PieceLog {
   static constexpr int U = 4;   // runs of four tokens a thread has under way
-  unsigned* counts;             // [kWords * C]
-  int lo, C;
+  unsigned* counts;             // [kWords][plane]
+  int plane, lo, span;
   const int4* quads;
   int from, start, end;
   __device__ __forceinline__ void one(int t, bool made) {
     const unsigned d = (unsigned)t - (unsigned)lo;
-    if (d < (unsigned)C) Counts<WORD>::add(counts, C, d, made);
+    if (d < (unsigned)span) Counts<WORD>::add(counts, plane, d, made);
   }
   __device__ __forceinline__ void ask(int q0, int4* t) const {
 #pragma unroll
@@ -103,11 +105,13 @@ struct PieceLog {
 // chain from a row's numbers to its log to the counts to the list.  So everything that does not wait for anything is asked for first,
 // the log's loads are under way while the logits are copied, a walked piece's logits are brought into L2 meanwhile, and a walked
 // piece leaves room for three CTAs on an SM (with two 76 us).  One row of 151936 and a short log 3.1 us: the chain and the launch.
-template <int THREADS, int PIECES, int WALK, bool WORD>
-__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : WALK > 1 ? 3 : 2)
+// SPLIT: CTAs of a cluster, with a piece each.  A long log is shared out: each CTA counts a part of it for all SPLIT pieces, and adds up what
+// the others have for its own.
+template <int THREADS, int PIECES, int WALK, bool WORD, int SPLIT>
+__global__ void __launch_bounds__(THREADS, WALK > 1 ? 3 : 2)
 logit_rules_kernel(RuleArgs a) {
-  constexpr int STEP = THREADS * 4 * PIECES, C = STEP * WALK;
-  extern __shared__ __align__(16) unsigned rule_smem[];   // [counts | list]
+  constexpr int STEP = THREADS * 4 * PIECES, C = STEP * WALK, CC = C * SPLIT;      // tokens of a piece, tokens that are counted
+  extern __shared__ __align__(16) unsigned rule_smem[];   // [counts of CC tokens | list]
   __shared__ int listed;
   __shared__ unsigned mask[C / 32 + 2];                   // the piece's words of the row's mask
   chain_wait();
@@ -116,7 +120,8 @@ logit_rules_kernel(RuleArgs a) {
   float* out = a.out + (size_t)r * a.ld_out;
   const bool in_place = a.logits == a.out;
   const int pad = (int)(((uintptr_t)row >> 2) & 3);
-  const int lo = (int)blockIdx.x * C - pad;   // the token of place 0
+  const int lo = (int)blockIdx.x * C - pad;   // the token of the piece's place 0
+  const int member = SPLIT > 1 ? (int)blockIdx.x % SPLIT : 0, own = member * C;      // own: where the piece's counts begin
   const bool pairs = (((uintptr_t)out >> 2) & 3) == (unsigned)pad;       // runs of four are aligned on both sides
 
   // everything that does not wait for anything is asked for first
@@ -152,10 +157,14 @@ logit_rules_kernel(RuleArgs a) {
   start = max(start, 0);
   int* log = a.history + (size_t)(fits ? slot : 0) * a.capacity;
   // earlier tokens count for the repetition penalty only; the log holds all but the last of the row where that comes with the call
-  PieceLog<THREADS, WORD> piece{rule_smem, lo, C, reinterpret_cast<const int4*>(log), rep != 1.f ? 0 : start, start,
-                       generated ? (a.tokens ? len - 1 : len) : 0};
-  unsigned short* list = reinterpret_cast<unsigned short*>(rule_smem + Counts<WORD>::kWords * C);      // [C] places that occur, in any order
-  const int q_first = (piece.from >> 2) + tid;
+  const int from = rep != 1.f ? 0 : start, end = generated ? (a.tokens ? len - 1 : len) : 0;
+  const bool shared = SPLIT > 1 && end - from >= kSharedLog;      // (the members of a cluster have the same row)
+  PieceLog<THREADS, WORD> piece{rule_smem + (shared ? 0 : own), CC, shared ? lo - own : lo, shared ? CC : C,
+                                reinterpret_cast<const int4*>(log), from, start, end};
+  unsigned* counts = rule_smem + own;                      // of this CTA's piece
+  unsigned short* list = reinterpret_cast<unsigned short*>(rule_smem + Counts<WORD>::kWords * CC);      // [C] places that occur, in any order
+  constexpr int RUN = PieceLog<THREADS, WORD>::U * THREADS;
+  const int q_first = (from >> 2) + (shared ? member * RUN : 0) + tid, q_step = shared ? SPLIT * RUN : RUN;
   int4 held[PieceLog<THREADS, WORD>::U];
   piece.ask(q_first, held);
   const unsigned* bits = m >= 0 && m < a.mask_rows ? a.mask + (size_t)m * a.words : nullptr;
@@ -172,7 +181,9 @@ logit_rules_kernel(RuleArgs a) {
     bias = a.bias_values[b0 + tid];
   }
   if (generated)
-    for (int i = tid; i < Counts<WORD>::kWords * C / 4; i += THREADS) reinterpret_cast<uint4*>(piece.counts)[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < Counts<WORD>::kWords; ++w)
+      for (int i = tid; i < piece.span / 4; i += THREADS) reinterpret_cast<uint4*>(piece.counts + w * CC)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) listed = 0;
   __syncthreads();
 
@@ -218,13 +229,13 @@ logit_rules_kernel(RuleArgs a) {
   // the log
   if (generated) {
     piece.take(q_first, held);
-    for (int q = q_first + PieceLog<THREADS, WORD>::U * THREADS; 4 * q < piece.end; q += PieceLog<THREADS, WORD>::U * THREADS) {
+    for (int q = q_first + q_step; 4 * q < end; q += q_step) {
       piece.ask(q, held);
       piece.take(q, held);
     }
   }
   if (a.tokens && tid == 0 && len > 0) {
-    if (generated && len - 1 >= piece.from) piece.one(last_token, len - 1 >= start);
+    if (generated && (member == 0 || !shared) && len - 1 >= from) piece.one(last_token, len - 1 >= start);
     if (blockIdx.x == 0) log[len - 1] = last_token;
   }
 
@@ -237,6 +248,23 @@ logit_rules_kernel(RuleArgs a) {
     return g ? x - (float)g * freq - pres : x;
   };
   auto allowed = [&](int i) { return !bits || (mask[(i >> 5) - word0] >> (i & 31)) & 1u; };
+  if (shared) {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    for (int i = tid; i < Counts<WORD>::kWords * C / 4; i += THREADS) {
+      unsigned* n = counts + i / (C / 4) * CC + i % (C / 4) * 4;      // (which only this thread reads here, and nobody elsewhere)
+      uint4 sum = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < SPLIT; ++m) {
+        unsigned at;
+        uint4 v;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(n)), "r"(m));
+        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+        sum = make_uint4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+      }
+      *reinterpret_cast<uint4*>(n) = sum;
+    }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // this thread reads the others' counts no more
+  }
   __syncthreads();                                          // the counts are complete, the piece is written
   // biased tokens: all of their rules, and they are off the list of the others
   if (b0 < b1) {
@@ -249,8 +277,8 @@ logit_rules_kernel(RuleArgs a) {
       if (bias_id < first || bias_id >= last || !allowed(bias_id)) continue;
       unsigned c = 0, g = 0;
       if (generated) {
-        Counts<WORD>::get(piece.counts, C, bias_id - lo, c, g);
-        Counts<WORD>::clear(piece.counts, C, bias_id - lo);
+        Counts<WORD>::get(counts, CC, bias_id - lo, c, g);
+        Counts<WORD>::clear(counts, CC, bias_id - lo);
       }
       out[bias_id] = rules(biased, c, g) + bias;
     }
@@ -259,7 +287,7 @@ logit_rules_kernel(RuleArgs a) {
   // the other tokens that occur
   if (!generated) return;
   for (int d = 4 * tid; d < C; d += 4 * THREADS) {
-    const uint4 n = Counts<WORD>::any(piece.counts, C, d);
+    const uint4 n = Counts<WORD>::any(counts, CC, d);
     if (n.x | n.y | n.z | n.w) {
       int at = atomicAdd(&listed, (n.x != 0) + (n.y != 0) + (n.z != 0) + (n.w != 0));
       if (n.x) list[at++] = (unsigned short)d;
@@ -273,11 +301,13 @@ logit_rules_kernel(RuleArgs a) {
     const int d = list[k], i = lo + d;
     if (i < 0 || i >= a.V || !allowed(i)) continue;
     unsigned c, g;
-    Counts<WORD>::get(piece.counts, C, d, c, g);
+    Counts<WORD>::get(counts, CC, d, c, g);
     out[i] = rules(row[i], c, g);
   }
+  if (shared) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // nobody reads this CTA's counts any more
 }
 
+// A thread an entry: 64 entries are a launch and two trips to memory in turn, 2 us; no entry is read twice, nothing to tile.
 __global__ void __launch_bounds__(256)
 append_history_kernel(int* __restrict__ history, const int* __restrict__ slots, const int* __restrict__ positions,
                       const int* __restrict__ tokens, int n, int n_slots, int capacity) {
@@ -323,27 +353,34 @@ extern "C" int nf_logit_rules(const float* logits, float* out, int* history, con
   // A piece of the vocabulary costs a reading of the log, a table to clear and to look through: the largest that still make several
   // CTAs a SM.  Rows of 151936 with logs of up to 4,000 tokens, us in pieces of 16384, 8192 and 4096: 16 rows 9.8 (4096) and 8.3
   // (8192), 32 rows 14.3, 13.3 and 17.5, 64 rows 27.0, 25.4 and 39.1 (logs of up to 8,192), 96 and 128 rows the same in the first two.
+  // Few rows whose logs may be long: pieces of 2048 in clusters of four, which share out a log of kSharedLog tokens and more (alone and in
+  // clusters, us: 5 rows of 32003 and logs of 131,072 tokens 17.5 and 10.6, one of 151936 20.6 and 10.5, with a log of 2,000 3.2 and 3.4).
+  // More rows read their logs faster in pieces of 4096 and 8192 (16 rows of 151936 and logs of 131,072 tokens 29, in clusters 39).
   const auto ctas = [&](int piece) { return (long long)rows * ((V + 3 + piece - 1) / piece); };
   const bool word = capacity < 65536;
-  const auto run = [&](auto threads, auto pieces, auto walk, auto packed) {
-    constexpr int T = decltype(threads)::value, P = decltype(pieces)::value, L = decltype(walk)::value, C = T * 4 * P * L;
+  const auto run = [&](auto threads, auto pieces, auto walk, auto packed, auto split) {
+    constexpr int T = decltype(threads)::value, P = decltype(pieces)::value, L = decltype(walk)::value, S = decltype(split)::value;
+    constexpr int C = T * 4 * P * L, CC = C * S;
     constexpr bool W = decltype(packed)::value;
-    constexpr int most = C * (4 * Counts<W>::kWords + 2);
-    const int bytes = C * 4 * Counts<W>::kWords + 2 * (C < capacity ? C : capacity);      // (the list has a place for every token of a log)
+    constexpr int most = 4 * Counts<W>::kWords * CC + 2 * C;
+    const int bytes = 4 * Counts<W>::kWords * CC + 2 * (C < capacity ? C : capacity);      // (the list has a place for every token of a log)
     if (most > 40 * 1024) {
-      static const cudaError_t asked = cudaFuncSetAttribute(logit_rules_kernel<T, P, L, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      static const cudaError_t asked = cudaFuncSetAttribute(logit_rules_kernel<T, P, L, W, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (asked != cudaSuccess) note_launch_error(asked);
     }
-    launch_chained(logit_rules_kernel<T, P, L, W>, dim3((V + 3 + C - 1) / C, rows), dim3(T), (size_t)bytes, stream, a);
+    const dim3 grid((V + 3 + CC - 1) / CC * S, rows);
+    if (S > 1) launch_chained_cluster(logit_rules_kernel<T, P, L, W, S>, grid, dim3(T), (size_t)bytes, stream, S, a);
+    else launch_chained(logit_rules_kernel<T, P, L, W, S>, grid, dim3(T), (size_t)bytes, stream, a);
   };
+  const Int<512> threads;
   if (ctas(16384) >= 6 * 148) {
-    if (word) run(Int<512>{}, Int<2>{}, Int<4>{}, Int<1>{}); else run(Int<512>{}, Int<2>{}, Int<2>{}, Int<0>{});
+    if (word) run(threads, Int<2>{}, Int<4>{}, Int<1>{}, Int<1>{}); else run(threads, Int<2>{}, Int<2>{}, Int<0>{}, Int<1>{});
   } else if (ctas(8192) >= 2 * 148) {
-    if (word) run(Int<512>{}, Int<2>{}, Int<2>{}, Int<1>{}); else run(Int<512>{}, Int<2>{}, Int<2>{}, Int<0>{});
+    if (word) run(threads, Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}); else run(threads, Int<2>{}, Int<2>{}, Int<0>{}, Int<1>{});
   } else if (ctas(4096) >= 2 * 148) {
-    if (word) run(Int<512>{}, Int<2>{}, Int<1>{}, Int<1>{}); else run(Int<512>{}, Int<2>{}, Int<1>{}, Int<0>{});
+    if (word) run(threads, Int<2>{}, Int<1>{}, Int<1>{}, Int<1>{}); else run(threads, Int<2>{}, Int<1>{}, Int<0>{}, Int<1>{});
   } else {
-    if (word) run(Int<512>{}, Int<1>{}, Int<1>{}, Int<1>{}); else run(Int<1024>{}, Int<1>{}, Int<1>{}, Int<0>{});
+    if (word) run(threads, Int<1>{}, Int<1>{}, Int<1>{}, Int<1>{}); else run(threads, Int<1>{}, Int<1>{}, Int<0>{}, Int<4>{});
   }
   return check_launch("logit_rules");
 }

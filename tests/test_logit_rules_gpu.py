@@ -57,7 +57,8 @@ def same(got, want, off):
 @pytest.mark.parametrize("R,V,capacity,longest,few", [
     (1, 1, 4, 1, None), (1, 3, 4, 4, None), (2, 31, 16, 9, None), (3, 33, 8, 8, 5), (5, 1000, 64, 50, 20), (2, 2048, 64, 64, None),
     (4, 2049, 512, 512, 30), (3, 4099, 2048, 2047, 300), (1, 32003, 1024, 1000, None), (2, 151936, 128, 100, None),
-    (40, 131075, 64, 60, 30), (75, 16385, 128, 128, 50), (20, 131071, 65536, 300, 40), (3, 5000, 65536, 66000 - 465, 700)])
+    (40, 131075, 64, 60, 30), (75, 16385, 128, 128, 50), (20, 131071, 65536, 300, 40), (3, 5000, 65536, 66000 - 465, 700),
+    (2, 40001, 70000, 70000, None), (3, 8189, 65536, 16384, 8000), (1, 8195, 65540, 16385, None), (4, 151936, 65536, 40000, 30000)])
 @pytest.mark.parametrize("what", ["penalties", "bias", "mask", "all"])
 def test_against_the_plain_form(R, V, capacity, longest, few, what):
     from ninfer_amd_mi50_b200 import kernels
@@ -89,6 +90,20 @@ def test_the_last_tokens_go_into_the_log(R, V):
     same(got, want, off)
     assert torch.equal(args[1].cpu(), log)
     assert torch.equal(kernels.adjust_logits(*args), got)       # the log holds them now
+
+
+@pytest.mark.parametrize("length", [16384, 16385, 30001])
+def test_the_last_token_of_a_long_log(length):
+    from ninfer_amd_mi50_b200 import kernels
+    args = make(2, 20003, 65536, length, seed=length, few=15000)
+    args[3][1] = length - 7
+    tokens = torch.tensor([14999, 8191], dtype=torch.int32).cuda()
+    full = args[1].clone()
+    full[args[2].long(), args[3].long() - 1] = tokens
+    want, off, _ = plain_rules(args[0], full, *args[2:])
+    got = kernels.adjust_logits(*args, tokens=tokens)
+    same(got, want, off)
+    assert torch.equal(args[1], full)
 
 
 def test_append_history():
