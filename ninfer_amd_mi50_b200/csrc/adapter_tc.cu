@@ -1026,6 +1026,27 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     blocks = rows > 16 && (rows > kRowsMost ? parts > 1 : share * R > kBlocksAbove);
   }
 
+  // The wide kernel's tile: the one whose rounds take the least, a round's time being that of the products or of the operands' way into
+  // shared memory (64 bytes a cycle), whichever is the longer; below 128 features only where they leave the first product its SMs (200 rows
+  // of 2048 x 5632: tiles of 64 32 us, of 128 27).
+  int BN = 256, ctas = 2, wide_grid = sm_count();
+  long long least = -1;
+  for (int g = 2; g >= 1; --g) {
+    const int m_tiles = (rows + kAdM * g - 1) / (kAdM * g), at_once = sm_count() / g;
+    for (int c = 256; c >= 64; c -= 32) {
+      const long long tiles = (long long)m_tiles * feature_tiles(sl, c);
+      const int loads = (kAdTile + c / g * 128) / 64, step = 2 * c > loads ? 2 * c : loads;
+      const long long cost = ((tiles + at_once - 1) / at_once) * step;
+      if (c < 128 && 4 * tiles * g > sm_count()) break;
+      if (least < 0 || cost < least) {
+        least = cost;
+        BN = c;
+        ctas = g;
+        wide_grid = tiles < at_once ? (int)tiles * g : at_once * g;
+      }
+    }
+  }
+
   // ---- h
   if (rows <= 16) {
     if (int rc = adapter_shrink_simt(x, A, scale, ids, h, rows, K, SR, n, stream)) return rc;
@@ -1041,23 +1062,35 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     // adapters of rank 32: 19.7 us, on all of them 25.3).
     const bool few = rows <= kRowsMost;
     const int cols = few || blocks ? kShrinkCols : kShrinkCols / 2;
-    int members = 1, turns = 1;
-    long long best = -1;
-    for (int m = 1; m <= 8 && (m == 1 || steps >= 2 * m); m *= 2) {
-      int at_once = clusters_at_once(adapter_shrink_tc_kernel, 192, kShrinkSmemMost, m);
-      if (few) at_once = at_once * 2 / 5;
-      else if (blocks) at_once = at_once * (sm_count() - parts * f_tiles128) / sm_count();
-      if (at_once < 1) continue;
-      const int z_most = at_once / tiles < 1 ? 1 : at_once / tiles > most ? most : at_once / tiles;
-      for (int z = 1; z <= z_most; ++z) {
-        const auto time = [&](int adapters) {
-          const int each = (adapters + z - 1) / z, group = cols / JW < each ? cols / JW : each;
-          return 6000 + (each + group - 1) / group * (2000 + (steps + m - 1) / m * (kAdTile + group * JW * 128) / 48);
-        };
-        const long long cost = (long long)((tiles * z + at_once - 1) / at_once) * (time(most) + time(most < 2 ? most : 2));
-        if (best < 0 || cost < best) { best = cost; members = m; turns = z; }
+    struct Split {
+      int members, turns;
+      long long cost;
+    };
+    const auto split = [&](int sms) {
+      Split best{1, 1, -1};
+      for (int m = 1; m <= 8 && (m == 1 || steps >= 2 * m); m *= 2) {
+        const int at_once = clusters_at_once(adapter_shrink_tc_kernel, 192, kShrinkSmemMost, m) * sms / sm_count();
+        if (at_once < 1) continue;
+        const int z_most = at_once / tiles < 1 ? 1 : at_once / tiles > most ? most : at_once / tiles;
+        for (int z = 1; z <= z_most; ++z) {
+          const auto time = [&](int adapters) {
+            const int each = (adapters + z - 1) / z, group = cols / JW < each ? cols / JW : each;
+            return 6000 + (each + group - 1) / group * (2000 + (steps + m - 1) / m * (kAdTile + group * JW * 128) / 48);
+          };
+          const long long cost = (long long)((tiles * z + at_once - 1) / at_once) * (time(most) + time(most < 2 ? most : 2));
+          if (best.cost < 0 || cost < best.cost) best = {m, z, cost};
+        }
       }
+      return best;
+    };
+    const int least_room = sm_count() * 2 / 5;
+    Split plan = split(few ? least_room : blocks ? sm_count() - parts * f_tiles128 : sm_count());
+    // A wide kernel that needs few SMs runs beside the first product where that is not much longer for it (512 rows of 2048 x 2048 34 -> 26 us).
+    if (!few && !blocks && 4 * wide_grid <= 3 * sm_count()) {
+      const Split beside = split(sm_count() - wide_grid > least_room ? sm_count() - wide_grid : least_room);
+      if (4 * beside.cost <= 5 * plan.cost) plan = beside;
     }
+    const int members = plan.members, turns = plan.turns;
     const int each = (most + turns - 1) / turns, group = cols / JW < each ? cols / JW : each;
     const int x_box = rows >= kAdM ? kAdM : (rows + 7) & ~7;
     CUtensorMap ma, mx;
@@ -1101,19 +1134,6 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     launch_chained_cluster(kernel, dim3(parts, f_tiles128), dim3(kRowsThreads), smem, stream, parts, mw, mx, mb, mh, ids, (const float*)h,
                            (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows, N, K, R, n, sl, NT, stages);
     return check_launch("adapter_rows");
-  }
-  // The tile: the one whose rounds take the least, a round's time being that of the products or of the operands' way into
-  // shared memory (64 bytes a cycle), whichever is the longer.
-  int BN = 256, ctas = 2;
-  long long best = -1;
-  for (int g = 2; g >= 1; --g) {
-    const int m_tiles = (rows + kAdM * g - 1) / (kAdM * g), at_once = sm_count() / g;
-    for (int c = 256; c >= 64; c -= 64) {
-      const long long tiles = (long long)m_tiles * feature_tiles(sl, c);
-      const int loads = (kAdTile + c / g * 128) / 64, step = 2 * c > loads ? 2 * c : loads;
-      const long long cost = ((tiles + at_once - 1) / at_once) * step;
-      if (best < 0 || cost < best) { best = cost; BN = c; ctas = g; }
-    }
   }
   if (int rc = make_map(&mx, x, rows, K, kAdM)) return rc;
   if (int rc = make_map(&mw, W, N, K, BN / ctas)) return rc;
