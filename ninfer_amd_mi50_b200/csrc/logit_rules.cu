@@ -101,10 +101,10 @@ struct PieceLog {
 // row's start.  It copies the piece's logits under the mask, WALK steps of PIECES runs of four a thread, and then does what is left to
 // do at the biased tokens and at those that occur in the log, one thread each.  (Done where the logits are copied, the powers and
 // quotients of the few tokens that occur held up nearly every warp: 204 instructions a run of four, 256 rows of 151936 99 us.)
-// What bounds it: 256 rows of 151936 take 69 us, of which the copy alone, as it runs without rules, 49 (6.3 TB/s); the rest is a CTA's
+// What bounds it: 256 rows of 151936 take 64 us, of which the copy alone, as it runs without rules, 49 (6.3 TB/s); the rest is a CTA's
 // chain from a row's numbers to its log to the counts to the list.  So everything that does not wait for anything is asked for first,
 // the log's loads are under way while the logits are copied, a walked piece's logits are brought into L2 meanwhile, and a walked
-// piece leaves room for three CTAs on an SM (with two 76 us).  One row of 151936 and a short log 3.1 us: the chain and the launch.
+// piece leaves room for three CTAs on an SM (two: a tenth longer).  One row of 151936 and a short log 2.6 us: the chain and the launch.
 // SPLIT: CTAs of a cluster, with a piece each.  A long log is shared out: each CTA counts a part of it for all SPLIT pieces, and adds up what
 // the others have for its own.
 template <int THREADS, int PIECES, int WALK, bool WORD, int SPLIT>
@@ -188,39 +188,61 @@ logit_rules_kernel(RuleArgs a) {
   __syncthreads();
 
   // the piece's logits under the mask
+  // (whole and aligned on both sides, with nothing to look after: 256 rows 63.9 us, by the other way 68.0, where the copy's instructions show)
+  if (!in_place && pairs && lo >= 0 && lo + C <= a.V) {
 #pragma unroll 1
-  for (int w = 0; w < WALK; ++w) {
-    if (lo + w * STEP >= a.V) break;
-    if (in_place && !bits) break;                           // nothing changes but at single tokens
-    if (w > 0 && !in_place) fetch(w);
+    for (int w = 0; w < WALK; ++w) {
+      if (w > 0) {
 #pragma unroll
-    for (int p = 0; p < PIECES; ++p) {
-      const int i0 = lo + w * STEP + 4 * (tid + p * THREADS);
-      if (i0 + 4 <= 0 || i0 >= a.V) continue;
-      const bool inside = i0 >= 0 && i0 + 4 <= a.V;
-      unsigned on = 0xfu;                                   // tokens that the mask allows
-      if (bits) {
-        const int from = max(i0, 0), word = (from >> 5) - word0, sh = from & 31;
-        unsigned x = mask[word] >> sh;
-        if (sh > 28 && word + 1 < words) x |= mask[word + 1] << (32 - sh);
-        on &= x << (from - i0);
+        for (int p = 0; p < PIECES; ++p) load4(row + lo + w * STEP + 4 * (tid + p * THREADS), v[p]);
       }
-      if (in_place) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!(on & (1u << e)) && i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = -INFINITY;
-        continue;
-      }
-      if (on != 0xfu) {
+      for (int p = 0; p < PIECES; ++p) {
+        const int i0 = lo + w * STEP + 4 * (tid + p * THREADS);
+        if (bits) {
+          const int word = (i0 >> 5) - word0;
+          const unsigned on = __funnelshift_r(mask[word], mask[word + 1], i0);      // (by i0 modulo 32)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[p][e] = on & (1u << e) ? v[p][e] : -INFINITY;
-      }
-      if (pairs && inside) {
+          for (int e = 0; e < 4; ++e) v[p][e] = on & (1u << e) ? v[p][e] : -INFINITY;
+        }
         store4(out + i0, v[p]);
-      } else {
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int w = 0; w < WALK; ++w) {
+      if (lo + w * STEP >= a.V) break;
+      if (in_place && !bits) break;                           // nothing changes but at single tokens
+      if (w > 0 && !in_place) fetch(w);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = v[p][e];
+      for (int p = 0; p < PIECES; ++p) {
+        const int i0 = lo + w * STEP + 4 * (tid + p * THREADS);
+        if (i0 + 4 <= 0 || i0 >= a.V) continue;
+        const bool inside = i0 >= 0 && i0 + 4 <= a.V;
+        unsigned on = 0xfu;                                   // tokens that the mask allows
+        if (bits) {
+          const int from = max(i0, 0), word = (from >> 5) - word0, sh = from & 31;
+          unsigned x = mask[word] >> sh;
+          if (sh > 28 && word + 1 < words) x |= mask[word + 1] << (32 - sh);
+          on &= x << (from - i0);
+        }
+        if (in_place) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(on & (1u << e)) && i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = -INFINITY;
+          continue;
+        }
+        if (on != 0xfu) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[p][e] = on & (1u << e) ? v[p][e] : -INFINITY;
+        }
+        if (pairs && inside) {
+          store4(out + i0, v[p]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = v[p][e];
+        }
       }
     }
   }
