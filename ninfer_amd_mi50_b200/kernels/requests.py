@@ -47,17 +47,20 @@ def _function(name: str):
     return f
 
 
-def _call(name: str, *args) -> None:
+def _begin(name: str):
+    """The C function, about to be called."""
     global _used
     _used = True
-    rc = _function(name)(*args)
     _lib.count_launches(1)
-    if rc != 0:
-        raise _lib.KernelError(f"{name}: {_lib.load().nf_last_error().decode(errors='replace')}")
+    return _functions.get(name) or _function(name)
 
 
-def _stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+def _failed(name: str) -> None:
+    raise _lib.KernelError(f"{name}: {_lib.load().nf_last_error().decode(errors='replace')}")
+
+
+def _stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _parts(widths: Sequence[int]) -> Tuple[ctypes.Array, int, int]:
@@ -74,10 +77,6 @@ def _parts(widths: Sequence[int]) -> Tuple[ctypes.Array, int, int]:
         if len(_slices) < 1024:
             _slices[key] = got
     return got
-
-
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
 
 
 def adapter_rank(rank: int) -> int:
@@ -159,14 +158,18 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     bf16 = dtype is torch.bfloat16
     if TUNING["adapter"] == "auto" and (K % 8 == 0 if bf16 else K % 4 == 0 and T <= TUNING["adapter_f32_max_rows"]):
-        h = scale.new_empty(_function("nf_adapter_scratch")(T, S * R, n) if bf16 else T * S * R)
-        _call("nf_adapter_linear" if bf16 else "nf_adapter_rows_f32", px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream())
+        # (h of a few rows lies row by row, see nf_adapter_scratch)
+        h = scale.new_empty(_function("nf_adapter_scratch")(T, S * R, n) if bf16 and T > 16 else T * S * R)
+        name = "nf_adapter_linear" if bf16 else "nf_adapter_rows_f32"
+        if _begin(name)(px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream(dev)):
+            _failed(name)
         return out
     # many float32 rows, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
     h = scale.new_empty(T * S * R)
     z = linear(x, w, out_dtype=torch.float32)
-    _call("nf_adapter_add", px, pa, pb, scale.data_ptr(), ids.data_ptr(), z.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _dt(x),
-          _stream())
+    if _begin("nf_adapter_add")(px, pa, pb, scale.data_ptr(), ids.data_ptr(), z.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _dt(x),
+                                _stream(dev)):
+        _failed("nf_adapter_add")
     return out
 
 
@@ -181,9 +184,9 @@ def append_history(history: torch.Tensor, slots: torch.Tensor, positions: torch.
                              f"one length on {history.device}")
     if history.dim() != 2:
         raise ValueError("append_history: history is [slots, capacity]")
-    if tokens.numel():
-        _call("nf_append_history", history.data_ptr(), slots.data_ptr(), positions.data_ptr(), tokens.data_ptr(), tokens.numel(),
-              history.shape[0], history.shape[1], _stream())
+    if tokens.numel() and _begin("nf_append_history")(history.data_ptr(), slots.data_ptr(), positions.data_ptr(), tokens.data_ptr(),
+                                                      tokens.numel(), history.shape[0], history.shape[1], _stream(history.get_device())):
+        _failed("nf_append_history")
 
 
 def _rows_apart(t: torch.Tensor, R: int, V: int) -> int:
@@ -305,9 +308,10 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     apart = _rows_apart(logits, R, V)
     if apart < 0 or apart_out < 0:
         _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
-    _call("nf_logit_rules", logits.data_ptr(), out.data_ptr(), p_history, slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
-          _ptr(tokens), penalties.data_ptr(), p_off, p_ids, p_values, n_bias, p_bits, p_index, n_masks, R, V, apart, apart_out, hs[0],
-          hs[1], _stream())
+    if _begin("nf_logit_rules")(logits.data_ptr(), out.data_ptr(), p_history, slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
+                                None if tokens is None else tokens.data_ptr(), penalties.data_ptr(), p_off, p_ids, p_values, n_bias, p_bits,
+                                p_index, n_masks, R, V, apart, apart_out, hs[0], hs[1], _stream(dev)):
+        _failed("nf_logit_rules")
     return out
 
 
