@@ -42,8 +42,10 @@ class Session:
     def __init__(self, engine: "Ninfer", key: int, adapter: Optional[str] = None):
         self._engine, self._key = engine, key
         self._adapter = engine._engine.adapter_slot(adapter)
-        self._open = True
         engine._runner.open(key)
+        self._open = True
+        if self._adapter >= 0:
+            engine._runner.adapters.hold(self._adapter)
 
     def __enter__(self):
         return self
@@ -90,6 +92,8 @@ class Session:
         if self._open:
             self._engine._runner.close(self._key)
             self._open = False
+            if self._adapter >= 0:
+                self._engine._runner.adapters.release(self._adapter)
 
 
 class Ninfer:
@@ -159,6 +163,7 @@ class Ninfer:
         self._engine.load_adapter(name, weights, scale)
 
     def drop_adapter(self, name: str) -> None:
+        """Give an adapter's place to others.  Refused while a session with it is open or a request with it is not finished."""
         self._engine.drop_adapter(name)
 
     # ---- sessions ----

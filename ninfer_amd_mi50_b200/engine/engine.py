@@ -82,7 +82,7 @@ class Engine:
         self.runner.adapters.load(name, weights, scale)
 
     def drop_adapter(self, name: str) -> None:
-        """Give an adapter's slot back.  Refused while a request that names it is not finished."""
+        """Give an adapter's slot back.  Refused while a request that names it is not finished or a session with it is open."""
         slot = self.adapter_slot(name)
         users = [r.id for r in self.requests.values() if r.adapter == slot and r.status != "finished"]
         if users:

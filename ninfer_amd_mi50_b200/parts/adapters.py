@@ -64,6 +64,7 @@ class AdapterBank:
         self.all: List[ProjectionAdapters] = []
         self.pools: Dict[str, List[ProjectionAdapters]] = {}       # by tensor name (layers may share a tensor)
         self.slots: Dict[str, int] = {}                      # by adapter name
+        self.held = [0] * self.capacity                      # holders of each slot beside the scheduler's requests
         for part in model.parts():
             pools = {what: ProjectionAdapters(p, self.capacity, self.rank, dtype, device, self.scale)
                      for what, p in part.projections().items()}
@@ -82,6 +83,14 @@ class AdapterBank:
         if name not in self.slots:
             raise AdapterError(f"no adapter {name!r}; loaded: {sorted(self.slots)}")
         return self.slots[name]
+
+    def hold(self, slot: int) -> None:
+        """An adapter is not dropped before whoever held its slot has released it: a slot's number says nothing of whose
+        weights it has by then."""
+        self.held[slot] += 1
+
+    def release(self, slot: int) -> None:
+        self.held[slot] -= 1
 
     def nbytes(self) -> int:
         return sum(p.nbytes() for p in self.all)
@@ -125,5 +134,7 @@ class AdapterBank:
 
     def drop(self, name: str) -> None:
         """Give a slot back (its weights stay until another adapter takes it; no row names it any more)."""
-        self.slot(name)
+        slot = self.slot(name)
+        if self.held[slot]:
+            raise AdapterError(f"adapter {name!r} is in use by {self.held[slot]} open session(s)")
         del self.slots[name]
