@@ -13,6 +13,10 @@
 // first), exactly as above.  With no top-k limit (k >= vocab) and top_p >= 1 the draw walks
 // the vocabulary in id order instead of sorted order: the same distribution, without a
 // sort of the whole vocabulary.
+//
+// A token of probability 0 (its logit -inf: masked) is never drawn, whatever the draw and the
+// roundings of the running sum: a draw of 0 takes the first token that has any, a draw that the
+// running sum rounds short of the last.  Only a row in which none has any gives one of those.
 #include "common.cuh"
 
 namespace nf {
@@ -140,7 +144,7 @@ sample_rows_kernel(const float* __restrict__ logits, int V, const float* __restr
   __shared__ int cand_i[kMaxK];
   __shared__ float red[33];
   __shared__ unsigned s_prefix, s_remaining;
-  __shared__ int s_n_gt, s_n_eq, s_result;
+  __shared__ int s_n_gt, s_n_eq, s_result, s_last;
   __shared__ float scan[1024];
   __shared__ int warp_cnt[32];
   const int r = blockIdx.x, tid = threadIdx.x;
@@ -170,9 +174,10 @@ sample_rows_kernel(const float* __restrict__ logits, int V, const float* __restr
     sum = block_sum(sum, red);
     const float target = u * sum;
     // chunks of blockDim.x ids in order; inclusive scan inside a chunk; the pick is the
-    // lowest id whose running sum reaches the target
+    // lowest id of those with a probability whose running sum reaches the target
     float base = 0.f;
-    if (tid == 0) s_result = 0x7fffffff;
+    int last = -1;                         // this thread's last id that has a probability
+    if (tid == 0) { s_result = 0x7fffffff; s_last = -1; }
     __syncthreads();
     for (int c0 = 0; c0 < V; c0 += blockDim.x) {
       const int i = c0 + tid;
@@ -185,13 +190,20 @@ sample_rows_kernel(const float* __restrict__ logits, int V, const float* __restr
         scan[tid] += add;
         __syncthreads();
       }
-      if (i < V && base + scan[tid] >= target) atomicMin(&s_result, i);
+      if (p > 0.f) {
+        last = i;
+        if (base + scan[tid] >= target) atomicMin(&s_result, i);
+      }
       __syncthreads();
       if (s_result != 0x7fffffff) break;
       base += scan[blockDim.x - 1];
       __syncthreads();
     }
-    if (tid == 0) out[r] = s_result != 0x7fffffff ? s_result : V - 1;
+    if (s_result == 0x7fffffff) {          // (the same for every thread)
+      if (last >= 0) atomicMax(&s_last, last);
+      __syncthreads();
+    }
+    if (tid == 0) out[r] = s_result != 0x7fffffff ? s_result : s_last >= 0 ? s_last : V - 1;
     return;
   }
 
@@ -295,8 +307,12 @@ sample_rows_kernel(const float* __restrict__ logits, int V, const float* __restr
     float cum = 0.f;
     int pick = cand_i[keep - 1];
     for (int i = 0; i < keep; ++i) {
-      cum += expf(cand_v[i] - m) / sum / s2;
-      if (u <= cum) { pick = cand_i[i]; break; }
+      const float p = expf(cand_v[i] - m) / sum / s2;
+      cum += p;
+      if (p > 0.f) {
+        pick = cand_i[i];
+        if (u <= cum) break;
+      }
     }
     out[r] = pick;
   }

@@ -101,8 +101,10 @@ def sample_reference(logits: Sequence[float], p: SamplingParams, recent: Sequenc
     if k >= V and p.top_p >= 1.0:
         e = torch.exp(l - l.max())
         cum = torch.cumsum(e, 0)
-        hit = torch.nonzero(cum >= draw * e.sum())
-        return int(hit[0]) if len(hit) else V - 1
+        # (a token of probability 0 is never drawn, here and below)
+        hit = torch.nonzero((cum >= draw * e.sum()) & (e > 0))
+        some = torch.nonzero(e > 0)
+        return int(hit[0]) if len(hit) else int(some[-1]) if len(some) else V - 1
     order = sorted(range(V), key=lambda i: (-float(l[i]), i))[:k]
     vals = l[order]
     prob = torch.exp(vals - vals[0])
@@ -116,12 +118,14 @@ def sample_reference(logits: Sequence[float], p: SamplingParams, recent: Sequenc
                 keep = i + 1
                 break
     prob = prob[:keep] / prob[:keep].sum()
-    cum = 0.0
+    cum, pick = 0.0, order[keep - 1]
     for i in range(keep):
         cum += float(prob[i])
-        if draw <= cum:
-            return order[i]
-    return order[keep - 1]
+        if prob[i] > 0:
+            pick = order[i]
+            if draw <= cum:
+                break
+    return pick
 
 
 class Sampler:
