@@ -143,7 +143,7 @@ class Engine:
             if ids is not None and callable(r.params.allowed_tokens):
                 ids = [int(t) for t in ids]
                 check_allowed(ids, self.vocab_size)
-                if not ids:
+                if not r.params.leaves(ids):
                     r.ended, ids = True, None
             out.append(ids)
         return out

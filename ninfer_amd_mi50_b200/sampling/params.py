@@ -3,6 +3,7 @@
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Callable, Dict, Optional, Sequence, Union
 
@@ -17,7 +18,7 @@ class SamplingParams:
     max_new_tokens: int = 512
     # what the reference does not have: penalties on what was generated (each occurrence, and once), values added to
     # single tokens' logits, and the tokens that may follow: a set, or a function from the generated ids to one (None: any
-    # token; an empty answer ends the request)
+    # token; an answer that is empty, or all of whose tokens have a bias of -inf, ends the request)
     frequency_penalty: float = 0.0
     presence_penalty: float = 0.0
     logit_bias: Optional[Dict[int, float]] = None
@@ -46,3 +47,8 @@ class SamplingParams:
         """The tokens that may follow `generated`; None: any."""
         a = self.allowed_tokens
         return a(list(generated)) if callable(a) else a
+
+    def leaves(self, ids: Sequence[int]) -> bool:
+        """Whether a token of `ids` may be drawn: one without a bias of -inf."""
+        never = {int(t) for t, v in (self.logit_bias or {}).items() if v == -math.inf}
+        return any(int(t) not in never for t in ids)

@@ -42,6 +42,11 @@ def check_allowed(ids: Sequence[int], vocab: int) -> None:
             raise ValueError(f"allowed token {t} outside [0, {vocab})")
 
 
+def check_leaves(p: SamplingParams, ids: Sequence[int]) -> None:
+    if not p.leaves(ids):
+        raise ValueError("the allowed tokens and biases of -inf leave no token to draw")
+
+
 def check_rules(p: SamplingParams, vocab: int) -> None:
     """Raises ValueError for penalties, biases or allowed tokens that make no sense."""
     if p.has_rules and not p.repetition_penalty > 0:
@@ -58,6 +63,8 @@ def check_rules(p: SamplingParams, vocab: int) -> None:
         if len(p.allowed_tokens) == 0:
             raise ValueError("allowed_tokens allows nothing")
         check_allowed(p.allowed_tokens, vocab)
+    if p.logit_bias:
+        check_leaves(p, range(vocab) if p.allowed_tokens is None or callable(p.allowed_tokens) else p.allowed_tokens)
 
 
 def check_params(p: SamplingParams, vocab: int) -> None:
@@ -91,8 +98,10 @@ def sample_reference(logits: Sequence[float], p: SamplingParams, recent: Sequenc
             l[tok] += v
         allowed = p.allowed(generated)
         if allowed is not None:
+            allowed = list(allowed)
+            check_leaves(p, allowed)
             left_out = torch.ones(V, dtype=torch.bool)
-            left_out[torch.as_tensor(list(allowed), dtype=torch.long)] = False
+            left_out[torch.as_tensor(allowed, dtype=torch.long)] = False
             l[left_out] = -math.inf
     if p.greedy:
         return int(torch.argmax(l))          # first maximum
@@ -174,7 +183,13 @@ class Sampler:
             for r in rule_rows:
                 tokens = list(recent[r]) if recent else []
                 prompt = prompt_lengths[r] if prompt_lengths else 0
-                ids = allowed[r] if allowed is not None else params[r].allowed(tokens[prompt:])
+                if allowed is not None:
+                    ids = allowed[r]
+                else:
+                    ids = params[r].allowed(tokens[prompt:])
+                    if ids is not None:
+                        ids = list(ids) if callable(params[r].allowed_tokens) else ids
+                        check_leaves(params[r], ids)
                 rows.append(RuleRow(r, params[r], tokens, prompt, keys[r] if keys else None, ids))
             logits = apply_rules(logits, rows, self.logs, out=logits if own else None)
         if all(p.greedy for p in params):

@@ -10,7 +10,9 @@ import plain_requests
 from adapter_models import merged, random_adapter
 from tiny_configs import CONFIGS, random_tokens
 
+from ninfer_amd_mi50_b200 import kernels
 from ninfer_amd_mi50_b200.api import Ninfer, NinferError
+from ninfer_amd_mi50_b200.sampling import Sampler, SamplingParams, sample_reference
 from ninfer_amd_mi50_b200.weights import write_random_model
 
 CFG, SEED = CONFIGS["B"]
@@ -23,6 +25,7 @@ def ninfer(tmp_path, monkeypatch):
     write_random_model(CFG, SEED, d)
     plain_kernels.install(monkeypatch)
     plain_requests.install(monkeypatch)
+    monkeypatch.setattr(kernels, "sample_rows", lambda logits, *a: kernels.argmax_rows(logits), raising=False)      # (some draw)
     return Ninfer(d, max_context=128, prefill_chunk=16, num_sequences=3, dtype="float32", device="cpu", page_size=16, adapters=1,
                   adapter_rank=9), plain_model.read_model_folder(d)
 
@@ -59,3 +62,41 @@ def test_an_adapter_stays_while_a_session_has_it(ninfer):
     eng.drop_adapter("b")
     for f in full:
         f.close()
+
+
+# ---- rules that together leave no token ---------------------------------------------------------------------------------------
+
+INF = float("inf")
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_a_fixed_set_that_its_biases_empty_is_refused(ninfer, temperature):
+    eng, _ = ninfer
+    for rules in (dict(allowed_tokens=[7], logit_bias={7: -INF}), dict(allowed_tokens=[7, 7, 9], logit_bias={7: -INF, 9: -INF, 8: 1.0}),
+                  dict(logit_bias={i: -INF for i in range(V)})):
+        with pytest.raises(ValueError, match="leave"):
+            eng.generate([[1, 2]], 3, temperature, **rules)
+        with pytest.raises(ValueError, match="leave"):
+            eng.sample([0.0] * V, temperature, **rules)
+    drawn = eng.generate([[1, 2]], 3, temperature, allowed_tokens=[7, 9], logit_bias={7: -INF}, seed=3)
+    assert drawn == [[9, 9, 9]]
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_an_answer_that_the_biases_empty_ends_the_request(ninfer, temperature):
+    eng, _ = ninfer
+
+    def answer(generated):
+        return (t for t in ([5, 6] if len(generated) < 2 else [6]))
+
+    p = SamplingParams(temperature, allowed_tokens=answer, logit_bias={6: -INF}, max_new_tokens=6, seed=1)
+    rid = eng._engine.submit([1, 2, 3], p)
+    eng._engine.run_until_idle()
+    assert eng._engine.requests[rid].generated == [5, 5] and eng._engine.requests[rid].finish_reason == "stop"
+    # by themselves, the sampler and its host twin say so instead of drawing what is not allowed
+    with pytest.raises(ValueError, match="leave"):
+        sample_reference([0.0] * V, p, [5, 5])
+    with pytest.raises(ValueError, match="leave"):
+        Sampler(V, "cpu").sample(torch.zeros(1, V), [p], recent=[[5, 5]])
+    with pytest.raises(ValueError, match="leave"):
+        Sampler(V, "cpu").sample(torch.zeros(1, V), [SamplingParams(temperature, allowed_tokens=lambda g: [])], recent=[[5, 5]])
