@@ -14,7 +14,8 @@
 
 namespace nf {
 
-// set by a row whose slot, length or start does not fit the log: 1 + the row; read by nf_rules_index_status
+// set by a row whose slot, length or start does not fit the log, or whose mask or biases do not fit theirs: 1 + the row; read by
+// nf_rules_index_status
 __device__ int g_rules_error = 0;
 
 struct RuleArgs {
@@ -152,9 +153,13 @@ logit_rules_kernel(RuleArgs a) {
   }
   const bool generated = freq != 0.f || pres != 0.f || rep != 1.f;
   const bool fits = slot >= 0 && slot < a.n_slots && len >= (a.tokens ? 1 : 0) && len <= a.capacity;
-  if (tid == 0 && (!fits || start < 0 || (a.mask && m >= a.mask_rows))) atomicCAS(&g_rules_error, 0, r + 1);
+  if (tid == 0 && (!fits || start < 0 || start > len || (a.mask && m >= a.mask_rows) || b0 < 0 || b0 > b1 || b1 > a.n_bias))
+    atomicCAS(&g_rules_error, 0, r + 1);
   if (!fits) len = 0;
-  start = max(start, 0);
+  // (places of the log and of the lists are walked in steps beyond them: none of these may begin near the end of an int)
+  start = min(max(start, 0), len);
+  b1 = min(max(b1, 0), a.n_bias);
+  b0 = min(max(b0, 0), b1);
   int* log = a.history + (size_t)(fits ? slot : 0) * a.capacity;
   // earlier tokens count for the repetition penalty only; the log holds all but the last of the row where that comes with the call
   const int from = rep != 1.f ? 0 : start, end = generated ? (a.tokens ? len - 1 : len) : 0;
@@ -172,8 +177,6 @@ logit_rules_kernel(RuleArgs a) {
   const int word0 = first >> 5, words = ((last + 31) >> 5) - word0;
   if (bits)
     for (int i = tid; i < words; i += THREADS) mask[i] = bits[word0 + i];
-  b0 = max(b0, 0);
-  b1 = min(b1, a.n_bias);
   int bias_id = -1;                                        // this thread's entry; those beyond as many as threads are read later
   float bias = 0.f;
   if (b0 + tid < b1) {
@@ -360,7 +363,7 @@ extern "C" int nf_append_history(int* history, const int* slots, const int* posi
 // out[r] from logits[r] (rows ld_in and ld_out floats apart; out may be logits).  tokens: the last token of every row, written
 // to its log's place lengths[r] - 1 and counted with it, or null (the log holds it already).  bias: ids and values of row r at
 // [bias_offsets[r], bias_offsets[r + 1]), each id once a row, or null.  mask: bit i & 31 of word i >> 5 of row
-// mask_index[r] is set where token i is allowed.  capacity: a multiple of 4; history 16-byte aligned.
+// mask_index[r] is set where token i is allowed.  capacity: a multiple of 4, up to 2^30; history 16-byte aligned.
 extern "C" int nf_logit_rules(const float* logits, float* out, int* history, const int* slots, const int* lengths, const int* starts,
                               const int* tokens, const float* penalties, const int* bias_offsets, const int* bias_ids,
                               const float* bias_values, int n_bias, const unsigned* mask, const int* mask_index, int mask_rows,
@@ -368,8 +371,9 @@ extern "C" int nf_logit_rules(const float* logits, float* out, int* history, con
   if (rows == 0) return 0;
   NF_REQUIRE(rows > 0 && rows <= 65535 && V > 0 && V <= (1 << 30), "logit_rules: bad sizes rows=%d V=%d", rows, V);
   NF_REQUIRE(ld_in >= V && ld_out >= V, "logit_rules: rows %d and %d apart for %d logits", ld_in, ld_out, V);
-  NF_REQUIRE(n_slots > 0 && capacity > 0 && capacity % 4 == 0 && (uintptr_t)history % 16 == 0,
-             "logit_rules: a log of %d slots with %d tokens (a multiple of 4), 16-byte aligned", n_slots, capacity);
+  NF_REQUIRE(n_slots > 0 && capacity > 0 && capacity % 4 == 0 && capacity <= (1 << 30) && (uintptr_t)history % 16 == 0,
+             "logit_rules: a log of %d slots with %d tokens (a multiple of 4, up to 2^30), 16-byte aligned", n_slots, capacity);
+  NF_REQUIRE(n_bias >= 0 && n_bias <= (1 << 30), "logit_rules: %d biases", n_bias);
   const RuleArgs a{logits, out, history, slots, lengths, starts, tokens, penalties, bias_offsets, bias_ids, bias_values, mask,
                    mask_index, V, ld_in, ld_out, n_slots, capacity, n_bias, mask_rows, (V + 31) / 32};
   // A piece of the vocabulary costs a reading of the log, a table to clear and to look through: the largest that still make several
@@ -407,7 +411,7 @@ extern "C" int nf_logit_rules(const float* logits, float* out, int* history, con
   return check_launch("logit_rules");
 }
 
-// 0, or 1 + a row (or an appended entry) whose slot, length, start or mask did not fit since the last call.  Synchronises.
+// 0, or 1 + a row (or an appended entry) whose slot, length, start, mask or biases did not fit since the last call.  Synchronises.
 extern "C" int nf_rules_index_status() {
   int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, g_rules_error, sizeof(int)) != cudaSuccess) return -1;

@@ -261,8 +261,8 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     [R + 1], ids int32, values float32): the entries of row r are those from offsets[r] to offsets[r + 1], each id once.
     `mask` = (bits int32 [M, (V + 31) // 32], index int32 [R]): bit i % 32 of word i // 32 of row index[r] is set where
     token i is allowed; index -1: no mask.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits`
-    itself.  A slot, a length or a mask row outside its tensor changes that row as if it had no tokens or no mask, and is
-    reported by `check_status`."""
+    itself.  A slot, a length or a mask row outside its tensor changes that row as if it had no tokens or no mask; a start
+    counts as the nearest place from 0 to the length, an offset as the nearest entry: all are reported by `check_status`."""
     dev = logits.get_device()
     ls, hs = logits.shape, history.shape
     good = (dev >= 0 and len(ls) == 2 and len(hs) == 2 and logits.dtype is torch.float32 and history.dtype is torch.int32
@@ -317,7 +317,7 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
 
 def request_status() -> int:
     """0, or what these kernels met since the last call: 1 to 14 a bounded wait that ran out, 101 + a row whose adapter was
-    outside the pool, 10000001 + a row whose log or mask did not fit.  Synchronises the device; where none of them was ever
+    outside the pool, 10000001 + a row whose log, mask or biases did not fit.  Synchronises the device; where none of them was ever
     called there is nothing to read."""
     if not _used:
         return 0
