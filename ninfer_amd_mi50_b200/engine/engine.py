@@ -39,6 +39,7 @@ class Engine:
         self._landing = [None, None]     # pinned buffers the drawn tokens land in, used in turn
         self._landing_turn = 0
         self._steps_since_check = 0
+        self._reported = 0      # finished requests that `step` has returned
 
     # ---- requests ---------------------------------------------------------------------
     def submit(self, prompt: Sequence[int], params: Optional[SamplingParams] = None,
@@ -60,6 +61,7 @@ class Engine:
             raise ValueError(f"request id {rid!r} is in use")
         req = Request(rid, [int(t) for t in prompt], params, set(int(s) for s in stop_ids), adapter=slot)
         self.scheduler.add(req)
+        self.sampler.forget(rid)       # (of an earlier request of this name, if no step has returned it yet)
         self.requests[rid] = req
         return rid
 
@@ -97,18 +99,15 @@ class Engine:
         With `run_ahead`, a pure decode step launches its successor before the host reads the
         tokens it drew (they are handed on inside the device), so the device does not idle
         while the host schedules; that successor is picked up by the next call."""
-        done: List[Request] = []
         if self._ahead is not None and not any(s.request.status == "running" for s in self._ahead[0]):
             self._ahead = None          # every request of that step has stopped meanwhile: nothing to record
         if self._ahead is not None:
             batch, picked = self._ahead
             self._ahead = None
         else:
-            before = len(self.scheduler.finished)
             batch = self.scheduler.schedule()
-            done = list(self.scheduler.finished[before:])      # finished without running (out of cache)
             if not batch:
-                return done
+                return self._ended()
             try:
                 allowed = self._allowed(batch)          # (a caller's function: before anything has run)
             except Exception:
@@ -125,7 +124,14 @@ class Engine:
             tokens = self._finish_readback(landing)
             self.d2h_bytes += picked.numel() * 4
         self._check_kernels(batch)
-        ended = done + self.scheduler.update(batch, tokens)
+        self.scheduler.update(batch, tokens)
+        return self._ended()
+
+    def _ended(self) -> List[Request]:
+        """The requests that have finished since this was last asked (also those that finished without running, out of cache, and
+        in a step that failed).  The sampler keeps nothing of them: another request may come under the same name."""
+        ended = self.scheduler.finished[self._reported:]
+        self._reported += len(ended)
         for req in ended:
             self.sampler.forget(req.id)
         return ended

@@ -100,3 +100,38 @@ def test_an_answer_that_the_biases_empty_ends_the_request(ninfer, temperature):
         Sampler(V, "cpu").sample(torch.zeros(1, V), [p], recent=[[5, 5]])
     with pytest.raises(ValueError, match="leave"):
         Sampler(V, "cpu").sample(torch.zeros(1, V), [SamplingParams(temperature, allowed_tokens=lambda g: [])], recent=[[5, 5]])
+
+
+# ---- logs of tokens of requests that come and go ------------------------------------------------------------------------------
+
+def test_a_request_that_ran_out_of_cache_leaves_no_tokens_to_the_next_of_its_name(tmp_path, monkeypatch):
+    d = str(tmp_path / "B")
+    write_random_model(CFG, SEED, d)
+    plain_kernels.install(monkeypatch)
+    plain_requests.install(monkeypatch)
+    eng = Ninfer(d, max_context=64, prefill_chunk=64, num_sequences=2, dtype="float32", device="cpu", page_size=16, cache_tokens=64)
+    pcfg, weights = plain_model.read_model_folder(d)
+    rules = SamplingParams(0.0, presence_penalty=100.0, frequency_penalty=1.0, max_new_tokens=30)
+    s = eng.session()
+    s.prefill(random_tokens(40, V, 1))                       # three of four pages
+    first = eng._engine.submit(random_tokens(10, V, 2), rules, request_id="x")
+    ended = []
+    while not eng._engine.scheduler.idle:
+        ended += eng._engine.step()
+    assert [r.id for r in ended] == [first] and ended[0].finish_reason == "out_of_cache" and ended[0].generated
+    assert not eng._engine.sampler.logs.slots
+    s.close()
+    # a prompt whose first tokens alone hold the token that the repetition penalty keeps from being drawn
+    for seed in range(50):
+        p = random_tokens(30, V, 3 + seed)
+        a = p[0]
+        p = [a] * 8 + [t for t in p if t != a][:22]
+        row = plain_model.plain_forward(pcfg, weights, p)[-1]
+        if row[a] < 0 and a not in ended[0].tokens:
+            break
+    rules = SamplingParams(0.0, repetition_penalty=10.0, presence_penalty=0.5, allowed_tokens=[a, int(row.argmin())], max_new_tokens=1)
+    want = sample_reference(row, rules, p, prompt_length=len(p))
+    assert want != a == sample_reference(row, rules, [], prompt_length=0)
+    eng._engine.submit(p, rules, request_id="x")
+    eng._engine.run_until_idle()
+    assert eng._engine.requests["x"].generated == [want]
