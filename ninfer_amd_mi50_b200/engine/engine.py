@@ -114,6 +114,8 @@ class Engine:
                 for s in batch:
                     self.cache.truncate(s.request.id)
                 raise
+            if not batch:
+                return self._ended()
             logits = self.runner.step(self.scheduler.entries(batch))
             picked = self._sample(batch, logits, ahead=False, allowed=allowed)
         tokens: List[int] = []
@@ -138,19 +140,30 @@ class Engine:
 
     def _allowed(self, batch) -> Optional[List[Optional[Sequence[int]]]]:
         """The tokens that may follow, for each request of the batch that samples; None where there is no such rule.  A
-        request that nothing may follow ends with this step."""
+        request that nothing may follow ends with this step.
+
+        A function that fails, or answers what makes no sense, fails the step for its caller, once; the next step asks it
+        again, and if it fails then too its request ends and leaves the batch: the other requests go on."""
         sampling = [s.request for s in batch if s.sample]
         if all(r.params.allowed_tokens is None for r in sampling):
             return None
         out: List[Optional[Sequence[int]]] = []
         for r in sampling:
             r.ended = False
-            ids = r.params.allowed(r.generated)
-            if ids is not None and callable(r.params.allowed_tokens):
-                ids = [int(t) for t in ids]
-                check_allowed(ids, self.vocab_size)
-                if not r.params.leaves(ids):
-                    r.ended, ids = True, None
+            try:
+                ids = r.params.allowed(r.generated)
+                if ids is not None and callable(r.params.allowed_tokens):
+                    ids = [int(t) for t in ids]
+                    check_allowed(ids, self.vocab_size)
+            except Exception as e:
+                again, r.error = r.error is not None, e
+                if not again:
+                    raise
+                self.scheduler.fail(r, batch)
+                continue
+            r.error = None
+            if ids is not None and callable(r.params.allowed_tokens) and not r.params.leaves(ids):
+                r.ended, ids = True, None
             out.append(ids)
         return out
 

@@ -34,11 +34,12 @@ class Request:
     stop_ids: Set[int] = field(default_factory=set)
     generated: List[int] = field(default_factory=list)
     status: str = "waiting"              # waiting | running | finished
-    finish_reason: Optional[str] = None  # length | stop | context | out_of_cache
+    finish_reason: Optional[str] = None  # length | stop | context | out_of_cache | error
     preemptions: int = 0
     computed: int = 0                    # tokens of (prompt + generated) that are in the cache
     adapter: int = -1                    # slot of its adapter, -1: none
     ended: bool = False                  # no token may follow: the one that this step draws is dropped
+    error: Optional[Exception] = None    # what its function of allowed tokens last raised, None once it has answered
 
     @property
     def tokens(self) -> List[int]:
@@ -232,6 +233,12 @@ class Scheduler:
         self.stats.finished += 1
         if reason == "out_of_cache":
             self.stats.out_of_cache += 1
+
+    def fail(self, req: Request, batch: List[Scheduled]) -> None:
+        """End a running request that has been scheduled and cannot go on (`req.error` says why): its pages are given back, the
+        rest of the batch stays as it is."""
+        batch[:] = [s for s in batch if s.request is not req]
+        self._finish(req, "error")
 
     @staticmethod
     def entries(batch: Sequence[Scheduled]) -> List[StepEntry]:

@@ -135,3 +135,70 @@ def test_a_request_that_ran_out_of_cache_leaves_no_tokens_to_the_next_of_its_nam
     eng._engine.submit(p, rules, request_id="x")
     eng._engine.run_until_idle()
     assert eng._engine.requests["x"].generated == [want]
+
+
+# ---- functions that fail ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", ["raises", "outside", "no list"])
+def test_a_function_that_keeps_failing_ends_its_request_alone(ninfer, bad):
+    eng, (pcfg, weights) = ninfer
+    eng, asked = eng._engine, []
+
+    def fails(generated):
+        asked.append(len(generated))
+        if len(generated) < 2:
+            return [3, 4]
+        if bad == "raises":
+            raise RuntimeError("grammar")
+        return [V] if bad == "outside" else 7
+
+    kind = {"raises": RuntimeError, "outside": ValueError, "no list": TypeError}[bad]
+    p = random_tokens(6, V, 2)
+    rid = eng.submit(p, SamplingParams(0.0, allowed_tokens=fails, max_new_tokens=9))
+    beside = eng.submit(p, SamplingParams(0.0, max_new_tokens=9))
+    turn = eng.submit(p, SamplingParams(0.0, allowed_tokens=lambda g: [10 + len(g)], max_new_tokens=9))
+    raised, ended = 0, []
+    for _ in range(40):
+        try:
+            ended += eng.step()
+        except kind:
+            raised += 1
+        if eng.scheduler.idle:
+            break
+    req = eng.requests[rid]
+    assert raised == 1 and asked == [0, 1, 2, 2]             # the caller hears of it once, the function is asked once more
+    assert req.finish_reason == "error" and isinstance(req.error, kind) and len(req.generated) == 2
+    assert sorted(r.id for r in ended) == sorted([rid, beside, turn])
+    assert eng.requests[beside].generated == plain_model.plain_greedy(pcfg, weights, p, 9)
+    assert eng.requests[turn].generated == list(range(10, 19))
+    assert not eng.cache.is_open(rid) and eng.submit(p, SamplingParams(0.0, max_new_tokens=1), request_id=rid) == rid
+    eng.run_until_idle()
+
+
+def test_two_functions_that_fail_and_one_that_recovers(ninfer):
+    eng = ninfer[0]._engine
+    count = [0]
+
+    def recovers(generated):
+        count[0] += 1
+        if count[0] % 2 == 0:
+            raise RuntimeError("now and then")
+        return [5]
+
+    def fails(generated):
+        raise KeyError("always")
+
+    ids = [eng.submit([1, 2], SamplingParams(0.0, allowed_tokens=f, max_new_tokens=4)) for f in (fails, recovers, fails)]
+    for _ in range(40):
+        try:
+            eng.run_until_idle()
+            break
+        except (RuntimeError, KeyError):
+            pass
+    assert eng.scheduler.idle and [eng.requests[i].finish_reason for i in ids] == ["error", "length", "error"]
+    assert eng.requests[ids[1]].generated == [5] * 4 and eng.requests[ids[1]].error is None
+    # ended alone in its batch
+    rid = eng.submit([1, 2], SamplingParams(0.0, allowed_tokens=fails, max_new_tokens=4))
+    with pytest.raises(KeyError):
+        eng.step()
+    assert [r.id for r in eng.step()] == [rid] and eng.scheduler.idle
