@@ -19,7 +19,10 @@ from .params import SamplingParams
 def mask_words(ids: Sequence[int], vocab: int) -> np.ndarray:
     """int32 words whose bit i % 32 of word i // 32 is set for the given ids."""
     on = np.zeros(((vocab + 31) // 32) * 32, dtype=bool)
-    on[np.asarray(list(ids), dtype=np.int64)] = True
+    ids = np.asarray(list(ids), dtype=np.int64)
+    if ids.size and not (0 <= ids.min() and ids.max() < vocab):
+        raise ValueError(f"allowed tokens from {ids.min()} to {ids.max()} do not lie in [0, {vocab})")
+    on[ids] = True
     return np.packbits(on, bitorder="little").view(np.int32)
 
 
@@ -82,7 +85,7 @@ def apply_rules(logits: torch.Tensor, rows: Sequence[RuleRow], logs: TokenLogs, 
     back = [r for r in rows if r.params.penalises]
     slots, lengths, starts = np.zeros(R, np.int32), np.zeros(R, np.int32), np.zeros(R, np.int32)
     penalties = np.tile(np.array([1.0, 0.0, 0.0], np.float32), (R, 1))
-    tokens = np.zeros(0, np.int32)
+    tokens, held = np.zeros(0, np.int32), {}               # held: slots -> the tokens that their logs have after this
     placed = np.zeros((2, 0), np.int32)
     if back:
         new_tokens, new_slots, new_at = [], [], []
@@ -95,7 +98,7 @@ def apply_rules(logits: torch.Tensor, rows: Sequence[RuleRow], logs: TokenLogs, 
             new_tokens += r.tokens[known:]
             new_slots += [slot] * (n - known)
             new_at += range(known, n)
-            logs.known[slot] = n
+            held[slot] = n
         tokens, placed = np.asarray(new_tokens, np.int32), np.asarray([new_slots, new_at], np.int32)
     else:
         logs.fit(1, 4)
@@ -119,6 +122,8 @@ def apply_rules(logits: torch.Tensor, rows: Sequence[RuleRow], logs: TokenLogs, 
         [len(p) for p in pieces[:10]] + [sum(len(w) for w in words)])
     if len(tokens):
         kernels.append_history(logs.history, placed_d[:len(tokens)], placed_d[len(tokens):], tok_d)
+    for slot, n in held.items():             # (not before: a call that fails on the way has sent nothing)
+        logs.known[slot] = n
     return kernels.adjust_logits(
         logits, logs.history, slots_d, lengths_d, starts_d, pen_d.view(torch.float32).view(R, 3),
         bias=(off_d, ids_d, val_d.view(torch.float32)) if ids else None,

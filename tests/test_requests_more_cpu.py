@@ -202,3 +202,28 @@ def test_two_functions_that_fail_and_one_that_recovers(ninfer):
     with pytest.raises(KeyError):
         eng.step()
     assert [r.id for r in eng.step()] == [rid] and eng.scheduler.idle
+
+
+# ---- a step of the sampler that fails -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("where", ["tokens outside", "a negative token", "append", "adjust"])
+def test_a_call_of_the_sampler_that_fails_loses_no_tokens(where, monkeypatch):
+    plain_kernels.install(monkeypatch)
+    plain_requests.install(monkeypatch)
+    s, p = Sampler(50, "cpu"), SamplingParams(0.0, presence_penalty=100.0)
+    logits = torch.arange(50.0)[None]
+    draw = lambda tokens, params=p: s.sample(logits, [params], recent=[tokens], prompt_lengths=[0], keys=["a"]).tolist()
+    assert draw([49]) == [48]
+    with monkeypatch.context() as m:
+        def broken(*a, **k):
+            raise kernels.KernelError("no room")
+
+        bad = p
+        if where in ("append", "adjust"):
+            m.setattr(kernels, {"append": "append_history", "adjust": "adjust_logits"}[where], broken)
+        else:
+            bad = SamplingParams(0.0, presence_penalty=100.0, allowed_tokens=[3, 300 if where == "tokens outside" else -1])
+        with pytest.raises((kernels.KernelError, ValueError)):
+            draw([49, 48, 47], bad)
+    assert draw([49, 48, 47]) == [46]
+    assert draw([49, 48, 47, 46]) == [45]
