@@ -102,7 +102,7 @@ class AdapterBank:
             raise AdapterError(f"adapter {name!r} is loaded already")
         if not weights:
             raise AdapterError(f"adapter {name!r} adapts nothing")
-        if not abs(float(scale)) < float("inf"):
+        if not torch.isfinite(torch.tensor(float(scale), dtype=torch.float32)):
             raise AdapterError(f"adapter {name!r}: scale {scale} is not finite")
         unknown = sorted(n for n in weights if n not in self.pools)
         if unknown:

@@ -14,6 +14,7 @@ engine.cpp:166-169; the idea is the same, the generator is not.)
 
 from __future__ import annotations
 
+import ctypes
 import math
 from collections import Counter
 from typing import Hashable, List, Optional, Sequence
@@ -36,6 +37,11 @@ def uniform_draw(seed: int, counter: int) -> float:
     return (z >> 40) / float(1 << 24)
 
 
+def float32(v: float) -> float:
+    """The number that the device computes with: an infinity for what float32 has no room for."""
+    return ctypes.c_float(v).value
+
+
 def check_allowed(ids: Sequence[int], vocab: int) -> None:
     for t in ids:
         if not 0 <= int(t) < vocab:
@@ -49,15 +55,15 @@ def check_leaves(p: SamplingParams, ids: Sequence[int]) -> None:
 
 def check_rules(p: SamplingParams, vocab: int) -> None:
     """Raises ValueError for penalties, biases or allowed tokens that make no sense."""
-    if p.has_rules and not p.repetition_penalty > 0:
+    if p.has_rules and not float32(p.repetition_penalty) > 0:
         raise ValueError("repetition_penalty must be positive")
     for what in ("frequency_penalty", "presence_penalty"):
-        if not math.isfinite(getattr(p, what)):
+        if not math.isfinite(float32(getattr(p, what))):
             raise ValueError(f"{what}={getattr(p, what)} must be finite")
     for t, v in (p.logit_bias or {}).items():
         if not 0 <= int(t) < vocab:
             raise ValueError(f"logit_bias names token {t} outside [0, {vocab})")
-        if math.isnan(float(v)) or float(v) == math.inf:
+        if float(v) != -math.inf and not math.isfinite(float32(v)):
             raise ValueError(f"logit_bias of token {t} is {v}: finite, or -inf for a token that is never drawn")
     if p.allowed_tokens is not None and not callable(p.allowed_tokens):
         if len(p.allowed_tokens) == 0:

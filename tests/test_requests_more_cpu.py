@@ -227,3 +227,18 @@ def test_a_call_of_the_sampler_that_fails_loses_no_tokens(where, monkeypatch):
             draw([49, 48, 47], bad)
     assert draw([49, 48, 47]) == [46]
     assert draw([49, 48, 47, 46]) == [45]
+
+
+# ---- numbers that float32 does not hold ---------------------------------------------------------------------------------------
+
+def test_numbers_that_are_infinite_on_the_device_are_refused(ninfer):
+    from ninfer_amd_mi50_b200.sampling import check_params
+    for bad in (dict(frequency_penalty=1e39), dict(presence_penalty=-1e39), dict(logit_bias={3: 1e39}), dict(logit_bias={3: -1e39}),
+                dict(presence_penalty=1.0, repetition_penalty=1e-50)):
+        with pytest.raises(ValueError):
+            check_params(SamplingParams(0.0, **bad), 50)
+    check_params(SamplingParams(0.0, frequency_penalty=3e38, presence_penalty=-3e38, logit_bias={3: 3e38, 4: -INF, 5: -3e38}), 50)
+    eng, _ = ninfer
+    with pytest.raises(ValueError, match="scale"):
+        eng.load_adapter("a", random_adapter(CFG, 1, 9), 1e39)
+    assert not eng._runner.adapters.slots
