@@ -190,11 +190,12 @@ def append_history(history: torch.Tensor, slots: torch.Tensor, positions: torch.
 
 
 def _rows_apart(t: torch.Tensor, R: int, V: int) -> int:
-    """Elements between two rows of [R, V], or -1 where the rows are not runs of their own."""
+    """Elements between two rows of [R, V], or -1 where the rows are not runs of their own, or too far apart for the kernel's
+    32-bit step."""
     step, one = t.stride()
     if R <= 1:
         step = V
-    return step if (one == 1 or V <= 1) and step >= V else -1
+    return step if (one == 1 or V <= 1) and V <= step < 1 << 31 else -1
 
 
 def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out) -> None:
@@ -238,7 +239,7 @@ def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, b
             raise ValueError(f"adjust_logits: a tensor lies on {t.device}, the logits on {logits.device}")
     for t, name in ((logits, "logits"), (out, "out")):
         if t is not None and R and V and _rows_apart(t, R, V) < 0:
-            raise ValueError(f"adjust_logits: the rows of {name} must be runs of their own, got strides {t.stride()}")
+            raise ValueError(f"adjust_logits: the rows of {name} must be runs of their own, less than 2^31 apart, got strides {t.stride()}")
     if history.shape[0] < 1 or history.shape[1] < 4 or history.shape[1] % 4 or history.data_ptr() % 16:
         raise ValueError(f"adjust_logits: history is {tuple(history.shape)}; its capacity must be a multiple of 4, its start a "
                          f"16-byte boundary")
