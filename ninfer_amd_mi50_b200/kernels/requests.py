@@ -87,6 +87,12 @@ def adapter_rank(rank: int) -> int:
     raise ValueError(f"adapter rank {rank} is not supported (1..{ADAPTER_RANKS[-1]})")
 
 
+def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    p, q = s.data_ptr(), t.data_ptr()
+    return p < q + t.numel() * t.element_size() and q < p + s.numel() * s.element_size()
+
+
 def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
     """Says what is wrong with the operands of adapter_linear."""
     _chk(x, "x")
@@ -115,6 +121,8 @@ def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
         _chk(out, "out", x.dtype)
         if out.shape != (T, N):
             raise ValueError(f"adapter_linear: out is {tuple(out.shape)}, not {(T, N)}")
+        if T and _overlap(x, out):
+            raise ValueError("adapter_linear: out shares memory with x")
     for t, name in ((x, "x"), (w, "w"), (a, "a"), (b, "b"), (out, "out")):
         if t is not None and t.data_ptr() % 16:
             raise ValueError(f"adapter_linear: {name} does not start on a 16-byte boundary")
@@ -149,7 +157,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     if out is None:
         out = x.new_empty((T, N))
-    elif not (out.dtype is dtype and out.get_device() == dev and out.is_contiguous() and out.shape == (T, N)):
+    elif not (out.dtype is dtype and out.get_device() == dev and out.is_contiguous() and out.shape == (T, N)) or _overlap(x, out):
         _refuse_adapter(x, w, a, b, scale, ids, widths, out)
     if T == 0:
         return out
@@ -198,6 +206,14 @@ def _rows_apart(t: torch.Tensor, R: int, V: int) -> int:
     return step if (one == 1 or V <= 1) and V <= step < 1 << 31 else -1
 
 
+def _clash(p: int, apart: int, q: int, apart_q: int, R: int, V: int) -> bool:
+    """Whether float32 rows at p and at q share memory otherwise than as the same rows."""
+    if (p == q and (apart == apart_q or R == 1)) or p + 4 * ((R - 1) * apart + V) <= q or q + 4 * ((R - 1) * apart_q + V) <= p:
+        return False
+    between = (q - p) // 4 % apart                    # rows of one tensor may lie between those of the other
+    return apart != apart_q or not V <= between <= apart - V
+
+
 def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out) -> None:
     """Says what is wrong with the operands of adjust_logits."""
     _chk(logits, "logits", torch.float32, contiguous=False); _chk(history, "history", torch.int32)
@@ -240,6 +256,8 @@ def _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, b
     for t, name in ((logits, "logits"), (out, "out")):
         if t is not None and R and V and _rows_apart(t, R, V) < 0:
             raise ValueError(f"adjust_logits: the rows of {name} must be runs of their own, less than 2^31 apart, got strides {t.stride()}")
+    if out is not None and R and V and _clash(logits.data_ptr(), _rows_apart(logits, R, V), out.data_ptr(), _rows_apart(out, R, V), R, V):
+        raise ValueError("adjust_logits: out shares memory with the logits without being the logits")
     if history.shape[0] < 1 or history.shape[1] < 4 or history.shape[1] % 4 or history.data_ptr() % 16:
         raise ValueError(f"adjust_logits: history is {tuple(history.shape)}; its capacity must be a multiple of 4, its start a "
                          f"16-byte boundary")
@@ -262,7 +280,7 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     [R + 1], ids int32, values float32): the entries of row r are those from offsets[r] to offsets[r + 1], each id once.
     `mask` = (bits int32 [M, (V + 31) // 32], index int32 [R]): bit i % 32 of word i // 32 of row index[r] is set where
     token i is allowed; index -1: no mask.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits`
-    itself.  A slot, a length or a mask row outside its tensor changes that row as if it had no tokens or no mask; a start
+    itself, but not overlap it otherwise.  A slot, a length or a mask row outside its tensor changes that row as if it had no tokens or no mask; a start
     counts as the nearest place from 0 to the length, an offset as the nearest entry: all are reported by `check_status`."""
     dev = logits.get_device()
     ls, hs = logits.shape, history.shape
@@ -307,9 +325,10 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
     if R == 0 or V == 0:
         return out
     apart = _rows_apart(logits, R, V)
-    if apart < 0 or apart_out < 0:
+    p_in, p_out = logits.data_ptr(), out.data_ptr()
+    if apart < 0 or apart_out < 0 or _clash(p_in, apart, p_out, apart_out, R, V):
         _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
-    if _begin("nf_logit_rules")(logits.data_ptr(), out.data_ptr(), p_history, slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
+    if _begin("nf_logit_rules")(p_in, p_out, p_history, slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
                                 None if tokens is None else tokens.data_ptr(), penalties.data_ptr(), p_off, p_ids, p_values, n_bias, p_bits,
                                 p_index, n_masks, R, V, apart, apart_out, hs[0], hs[1], _stream(dev)):
         _failed("nf_logit_rules")

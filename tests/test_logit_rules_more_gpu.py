@@ -55,3 +55,32 @@ def test_starts_and_offsets_at_the_ends_are_not_reported():
     want, off, _ = plain_rules(*args, bias=bias, mask=mask)
     same(kernels.adjust_logits(*args, bias=bias, mask=mask), want, off)
     kernels.check_status("test")
+
+
+def test_an_out_that_overlaps_the_logits_is_refused():
+    from ninfer_amd_mi50_b200 import kernels
+    args = make(3, 40, 16, 16)
+    buf = torch.zeros(400).cuda()
+    rows = lambda at, apart: buf.as_strided((3, 40), (apart, 1), at)
+    rest = args[1:]
+    for logits, out in ((rows(0, 40), rows(1, 40)), (rows(0, 40), rows(0, 50)), (rows(0, 50), rows(60, 50)), (rows(40, 100), rows(0, 60))):
+        with pytest.raises(ValueError, match="shares memory"):
+            kernels.adjust_logits(logits, *rest, out=out)
+    for logits, out in ((rows(0, 100), rows(50, 100)), (rows(0, 40), rows(120, 50)), (rows(7, 50), rows(7, 50)), (rows(140, 100), rows(100, 100))):
+        logits.copy_(args[0])
+        want, off, _ = plain_rules(*args)
+        assert kernels.adjust_logits(logits, *rest, out=out) is out
+        same(out, want, off)
+    kernels.check_status("test")
+
+
+def test_an_out_that_overlaps_the_rows_of_a_projection_is_refused():
+    from ninfer_amd_mi50_b200 import kernels
+    for dtype in (torch.float32, torch.bfloat16):
+        zeros = lambda *shape: torch.zeros(shape, dtype=dtype).cuda()
+        buf = zeros(64 * 64 + 64)
+        x, w, a, b = buf[:64 * 64].view(64, 64), zeros(64, 64), zeros(1, 16, 64), zeros(1, 64, 16)
+        scale, ids = torch.ones(1).cuda(), torch.zeros(64, dtype=torch.int32).cuda()
+        for out in (x, buf[64:].view(64, 64)):
+            with pytest.raises(ValueError, match="shares memory"):
+                kernels.adapter_linear(x, w, a, b, scale, ids, out=out)
