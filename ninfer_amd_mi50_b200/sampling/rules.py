@@ -106,7 +106,7 @@ def apply_rules(logits: torch.Tensor, rows: Sequence[RuleRow], logs: TokenLogs, 
     for r in sorted(rows, key=lambda r: r.row):
         bias = r.params.logit_bias or {}
         offsets[r.row + 1] = len(bias)
-        ids += bias.keys()
+        ids += (int(t) for t in bias)
         values += bias.values()
     offsets = np.cumsum(offsets, dtype=np.int32)
     index, words = np.full(R, -1, np.int32), []

@@ -70,6 +70,8 @@ def check_rules(p: SamplingParams, vocab: int) -> None:
             raise ValueError("allowed_tokens allows nothing")
         check_allowed(p.allowed_tokens, vocab)
     if p.logit_bias:
+        if len({int(t) for t in p.logit_bias}) < len(p.logit_bias):
+            raise ValueError("logit_bias names a token twice")
         check_leaves(p, range(vocab) if p.allowed_tokens is None or callable(p.allowed_tokens) else p.allowed_tokens)
 
 
@@ -101,7 +103,7 @@ def sample_reference(logits: Sequence[float], p: SamplingParams, recent: Sequenc
             if 0 <= tok < V:
                 l[tok] = l[tok] - n * p.frequency_penalty - p.presence_penalty
         for tok, v in (p.logit_bias or {}).items():
-            l[tok] += v
+            l[int(tok)] += v
         allowed = p.allowed(generated)
         if allowed is not None:
             allowed = list(allowed)

@@ -242,3 +242,12 @@ def test_numbers_that_are_infinite_on_the_device_are_refused(ninfer):
     with pytest.raises(ValueError, match="scale"):
         eng.load_adapter("a", random_adapter(CFG, 1, 9), 1e39)
     assert not eng._runner.adapters.slots
+
+
+def test_a_token_that_two_biases_name_is_refused():
+    from ninfer_amd_mi50_b200.sampling import check_params
+    with pytest.raises(ValueError, match="twice"):
+        check_params(SamplingParams(0.0, logit_bias={5: 1.0, "5": 2.0}), 50)
+    p = SamplingParams(0.0, logit_bias={"5": 99.0})
+    check_params(p, 50)
+    assert sample_reference([0.0] * 50, p) == 5
