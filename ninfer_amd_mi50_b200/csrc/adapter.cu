@@ -115,10 +115,10 @@ constexpr int kExpandRows = 8;
 // R numbers a feature; rank in pieces of 16 numbers so that a feature's row stays in registers.  What bounds it: z in and y out, 512 rows
 // of 2048 in float32 8.4 MB, 1.3 us; 16 under the profiler, since 512 CTAs wait for one trip to memory after the other (ids, z, B, h).
 // It serves what is not worth more: float32 beyond 64 rows, where the product before it takes 142, and rows that TMA cannot fetch.
-template <typename T>
+template <typename T, typename TY>
 __global__ void __launch_bounds__(256)
 adapter_expand_kernel(const float* __restrict__ z, const float* __restrict__ h, const T* __restrict__ B, const int* __restrict__ ids,
-                      T* __restrict__ y, int rows, int N, int R, int SR, int n, AdapterSlices slices) {
+                      TY* __restrict__ y, int rows, int N, int R, int SR, int n, AdapterSlices slices) {
   chain_wait(z, h, B, ids);
   const int f = blockIdx.x * blockDim.x + threadIdx.x, t0 = blockIdx.y * kExpandRows;
   if (f >= N) return;
@@ -151,7 +151,7 @@ adapter_expand_kernel(const float* __restrict__ z, const float* __restrict__ h, 
   }
 #pragma unroll
   for (int i = 0; i < kExpandRows; ++i)
-    if (t0 + i < rows) y[(size_t)(t0 + i) * N + f] = from_float<T>(sum[i]);
+    if (t0 + i < rows) y[(size_t)(t0 + i) * N + f] = from_float<TY>(sum[i]);
 }
 
 // ---- few float32 rows: the shared product with the adapters' part in its epilogue ----------------------------------------------
@@ -275,13 +275,13 @@ static void launch_rows_f32(const void* x, const void* W, const void* A, const v
                  (const float*)x, (const float*)W, (const float*)h, (const float*)B, ids, (float*)y, rows, N, K, R, SR, n, slices);
 }
 
-template <typename T>
+template <typename T, typename TY>
 static int launch_adapter(const void* x, const void* A, const void* B, const float* scale, const int* ids, const float* z, float* h,
                           void* y, int rows, int N, int K, int R, int n, const AdapterSlices& slices, cudaStream_t stream) {
   const int SR = slices.n * R;
   launch_shrink<T>(x, A, scale, ids, h, rows, K, SR, n, stream);
-  launch_chained(adapter_expand_kernel<T>, dim3((N + 255) / 256, (rows + kExpandRows - 1) / kExpandRows), dim3(256), 0, stream, z,
-                 (const float*)h, (const T*)B, ids, (T*)y, rows, N, R, SR, n, slices);
+  launch_chained(adapter_expand_kernel<T, TY>, dim3((N + 255) / 256, (rows + kExpandRows - 1) / kExpandRows), dim3(256), 0, stream, z,
+                 (const float*)h, (const T*)B, ids, (TY*)y, rows, N, R, SR, n, slices);
   return check_launch("adapter_add");
 }
 
@@ -310,11 +310,11 @@ extern "C" int nf_adapter_rows_f32(const void* x, const void* W, const void* A, 
 }
 
 // y = z + the adapters' part (see the head of this file).  z float32 [rows, N], h float32 scratch [rows, n_slices * R]; x, A
-// [n, n_slices * R, K], B [n, N, R] and y of `dtype`; ends: the n_slices features (host memory) at which the slices end, the
+// [n, n_slices * R, K], B [n, N, R] of `dtype`, y of `y_dtype` (the same, or float32); ends: the n_slices features (host memory) at which the slices end, the
 // last N.  R: a multiple of 16.  All bases 16-byte aligned.
 extern "C" int nf_adapter_add(const void* x, const void* A, const void* B, const float* scale, const int* ids, const float* z,
                               float* h, void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, int dtype,
-                              cudaStream_t stream) {
+                              int y_dtype, cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;
   NF_REQUIRE(rows > 0 && N > 0 && K > 0 && n > 0, "adapter_add: bad sizes rows=%d N=%d K=%d n=%d", rows, N, K, n);
   NF_REQUIRE(R > 0 && R % 16 == 0, "adapter_add: rank %d must be a multiple of 16", R);
@@ -325,8 +325,11 @@ extern "C" int nf_adapter_add(const void* x, const void* A, const void* B, const
   AdapterSlices s{n_slices, {}};
   for (int i = 0; i < n_slices; ++i) s.end[i] = ends[i];
   NF_REQUIRE(s.end[n_slices - 1] == N, "adapter_add: the slices end at %d of %d features", s.end[n_slices - 1], N);
-  if (dtype == kBF16) return launch_adapter<__nv_bfloat16>(x, A, B, scale, ids, z, h, y, rows, N, K, R, n, s, stream);
-  return launch_adapter<float>(x, A, B, scale, ids, z, h, y, rows, N, K, R, n, s, stream);
+  NF_REQUIRE(y_dtype == dtype || y_dtype == kF32, "adapter_add: the result is float32 or of the operands' type");
+  if (dtype == kBF16 && y_dtype == kBF16)
+    return launch_adapter<__nv_bfloat16, __nv_bfloat16>(x, A, B, scale, ids, z, h, y, rows, N, K, R, n, s, stream);
+  if (dtype == kBF16) return launch_adapter<__nv_bfloat16, float>(x, A, B, scale, ids, z, h, y, rows, N, K, R, n, s, stream);
+  return launch_adapter<float, float>(x, A, B, scale, ids, z, h, y, rows, N, K, R, n, s, stream);
 }
 
 // 0, or 1 + a row whose adapter lay outside the pool since the last call (it was served without one).  Synchronises.

@@ -461,13 +461,14 @@ __device__ __forceinline__ int next_tile(int i, int first, int stride) { return 
 // CTAS 1: a CTA a tile of 128 rows x BN features.  CTAS 2: two CTAs of a cluster a tile of 256 x BN; each holds its own 128 rows of x
 // and half of the features' rows of W, and the even one issues products over both (`cta_group::2`): half of W's bytes a CTA.
 // Warps: 0 producer, 1 MMA and tensor memory, 2..9 epilogue.  map_h: h as the first product lays it out, `places` blocks a row tile.
+// TY: the type of y, bfloat16, or float32 for a caller that has more to do with the sums.
 // What bounds it: the tensor cores (73 % busy under the profiler at 2048 rows of 2048 x 6144) and the operands' way into shared memory,
 // which at 256 x 256 a pair takes as long as the products: 512 cycles a step, 600 to 700 measured.  8192 rows of 3584 x 4608 take 190 us
 // with h, 1.43 PFLOP/s; the library's product without adapters 172.
-template <int CTAS>
+template <int CTAS, typename TY>
 __global__ void __launch_bounds__(kWideThreads, 1)
 adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_b,
-                    const __grid_constant__ CUtensorMap map_h, const int* __restrict__ ids, __nv_bfloat16* __restrict__ y, int rows, int N, int K,
+                    const __grid_constant__ CUtensorMap map_h, const int* __restrict__ ids, TY* __restrict__ y, int rows, int N, int K,
                     int R, int n, int places, const __grid_constant__ TcSlices slices, int f_tiles, int n_tiles, int BN, int stages) {
   extern __shared__ unsigned char smem_raw[];      // [barriers | stages | results on their way]
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -596,7 +597,8 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (!warp_wait(&bars->acc_full[ab], (done >> 1) & 1, stop, 4)) break;
       tc_fence_after();
       const int t0 = w.row0 + rank * kAdM + quad * 32, count = min(32, rows - t0);
-      const bool whole = N % 8 == 0 && w.f0 % 8 == 0 && w.width % 8 == 0;
+      constexpr int P = 16 / (int)sizeof(TY);              // numbers of a 16-byte piece
+      const bool whole = N % P == 0 && w.f0 % P == 0 && w.width % P == 0;
       unsigned char* turned = stage0 + (size_t)stages * stage_bytes + (warp - 2) * kTurnBytes;
       for (int c0 = half * 32; c0 < BN; c0 += 64) {
         unsigned v[32];
@@ -610,30 +612,48 @@ adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           if (lane == 0) arrive_leader<CTAS>(&bars->acc_empty[ab]);
         }
         if (c0 >= w.width) continue;
-        // A lane has 64 bytes of a row of its own: stored from there, every store of a warp goes to 32 lines.  The results change hands
-        // in shared memory, and a store covers 64 bytes of eight rows (5537 rows of 824 x 7392 93 -> 78 us), or, where rows of y are not
-        // 16-byte pieces, of one.
-        __syncwarp();
+        if constexpr (P == 4) {
+          // A lane's 32 sums are a whole line of its row: stored from here.
+          if (lane < count) {
+            float* to = y + (size_t)(t0 + lane) * N + w.f0 + c0;
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
-          __nv_bfloat162 o[4];
+            for (int c = 0; c < 32; c += 4) {
+              if (whole) {
+                if (c0 + c < w.width) *reinterpret_cast<uint4*>(to + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+              } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __floats2bfloat162_rn(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
-          *reinterpret_cast<uint4*>(turned + lane * kTurnRow + 2 * c) = *reinterpret_cast<uint4*>(o);
-        }
-        __syncwarp();
-        if (whole) {
-          const int c = c0 + 8 * (lane & 3);
-          __nv_bfloat16* to = y + (size_t)t0 * N + w.f0 + c;
-          if (c < w.width) {                      // (whole: widths are multiples of 8)
-#pragma unroll
-            for (int r = lane >> 2; r < 32; r += 8)
-              if (r < count) *reinterpret_cast<uint4*>(to + (size_t)r * N) = *reinterpret_cast<const uint4*>(turned + r * kTurnRow + 16 * (lane & 3));
+                for (int e = c; e < c + 4; ++e)
+                  if (c0 + e < w.width) to[e] = __uint_as_float(v[e]);
+              }
+            }
           }
-        } else if (c0 + lane < w.width) {
-          unsigned short* to = reinterpret_cast<unsigned short*>(y) + (size_t)t0 * N + w.f0 + c0 + lane;
+          __syncwarp();
+        } else {
+          // A lane has 64 bytes of a row of its own: stored from there, every store of a warp goes to 32 lines.  The results change hands
+          // in shared memory, and a store covers 64 bytes of eight rows (5537 rows of 824 x 7392 93 -> 78 us), or, where rows of y are not
+          // 16-byte pieces, of one.
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            __nv_bfloat162 o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __floats2bfloat162_rn(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
+            *reinterpret_cast<uint4*>(turned + lane * kTurnRow + 2 * c) = *reinterpret_cast<uint4*>(o);
+          }
+          __syncwarp();
+          if (whole) {
+            const int c = c0 + 8 * (lane & 3);
+            __nv_bfloat16* to = y + (size_t)t0 * N + w.f0 + c;
+            if (c < w.width) {                      // (whole: widths are multiples of 8)
+#pragma unroll
+              for (int r = lane >> 2; r < 32; r += 8)
+                if (r < count) *reinterpret_cast<uint4*>(to + (size_t)r * N) = *reinterpret_cast<const uint4*>(turned + r * kTurnRow + 16 * (lane & 3));
+            }
+          } else if (c0 + lane < w.width) {
+            unsigned short* to = reinterpret_cast<unsigned short*>(y) + (size_t)t0 * N + w.f0 + c0 + lane;
 #pragma unroll 8
-          for (int r = 0; r < count; ++r) to[(size_t)r * N] = *reinterpret_cast<const unsigned short*>(turned + r * kTurnRow + 2 * lane);
+            for (int r = 0; r < count; ++r) to[(size_t)r * N] = *reinterpret_cast<const unsigned short*>(turned + r * kTurnRow + 2 * lane);
+          }
         }
       }
     }
@@ -674,11 +694,11 @@ constexpr int kRowsAtOnce = 4;             // rows of x whose rows of B a thread
 // What bounds it: one row of 2048 x 2048 takes 7.1 us, its 8.4 MB 1.3: launch, the first loads, the members' sums, h and the rows of y,
 // one after the other.  64 rows of 3584 x 3584 with 48 adapters of rank 32 take 19.6 us, their 43 MB 6.7: h is there after 12, W's sums
 // by then, and the adapters' part takes 4.
-template <RowsForm FORM>
+template <RowsForm FORM, typename TY>
 __global__ void __launch_bounds__(kRowsThreads, 2)
 adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_h, const int* __restrict__ ids, const float* __restrict__ h,
-                    const __nv_bfloat16* __restrict__ B, __nv_bfloat16* __restrict__ y, int rows, int N, int K, int R, int n,
+                    const __nv_bfloat16* __restrict__ B, TY* __restrict__ y, int rows, int N, int K, int R, int n,
                     const __grid_constant__ TcSlices slices, int NT, int stages) {
   constexpr bool STAGED = FORM == kRowsStaged, BLOCKS = FORM == kRowsBlocks;
   extern __shared__ unsigned char smem_raw[];
@@ -875,7 +895,7 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         add_up(t0);
 #pragma unroll
         for (int i = 0; i < kRowsAtOnce; ++i)
-          if (t0 + 2 * i < t_last && d < w.width) y[(size_t)(t0 + 2 * i) * N + f] = __float2bfloat16_rn(sum[i]);
+          if (t0 + 2 * i < t_last && d < w.width) y[(size_t)(t0 + 2 * i) * N + f] = from_float<TY>(sum[i]);
       }
       return;
     }
@@ -920,7 +940,7 @@ adapter_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
 #pragma unroll
       for (int i = 0; i < kRowsAtOnce; ++i)
-        if (t0 + 2 * i < t_last && d < w.width) y[(size_t)(t0 + 2 * i) * N + f] = __float2bfloat16_rn(sum[i]);
+        if (t0 + 2 * i < t_last && d < w.width) y[(size_t)(t0 + 2 * i) * N + f] = from_float<TY>(sum[i]);
     }
   }
 }
@@ -1010,7 +1030,8 @@ extern "C" long long nf_adapter_scratch(int rows, int SR, int n) {
 }
 
 // One pass; the rows that an error names are counted from its first.
-static int adapter_pass(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h, void* y, int rows,
+template <typename TY>
+static int adapter_pass(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h, TY* y, int rows,
                         int N, int K, int R, int n, const TcSlices& sl, cudaStream_t stream) {
   const int SR = sl.n * R, steps = (K + kAdK - 1) / kAdK, n_slices = sl.n;
   const int row_tiles = (rows + kAdM - 1) / kAdM, places = adapter_places(rows, n);
@@ -1126,8 +1147,8 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
     }
     stages = stages > kAdMaxStages ? kAdMaxStages : stages;
     const size_t smem = 2048 + (size_t)stages * stage + sums;
-    static int asked = room_for(adapter_rows_kernel<kRowsPlain>, 108 * 1024), asked_staged = room_for(adapter_rows_kernel<kRowsStaged>, 108 * 1024),
-               asked_blocks = room_for(adapter_rows_kernel<kRowsBlocks>, 204 * 1024);
+    static int asked = room_for(adapter_rows_kernel<kRowsPlain, TY>, 108 * 1024), asked_staged = room_for(adapter_rows_kernel<kRowsStaged, TY>, 108 * 1024),
+               asked_blocks = room_for(adapter_rows_kernel<kRowsBlocks, TY>, 204 * 1024);
     if (asked || asked_staged || asked_blocks) return 1;
     NF_REQUIRE(f_tiles128 <= 65535, "adapter_linear: %d features are too many", N);
     mb = mh = mw;
@@ -1135,10 +1156,10 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
       if (int rc = make_map(&mb, B, (long long)n * N, R, kAdM)) return rc;
       if (int rc = make_map(&mh, h, (long long)places * n_slices * kAdM, 2 * R, NT)) return rc;
     }
-    const auto kernel = blocks ? adapter_rows_kernel<kRowsBlocks>
-                               : share * R >= kStagedLeast ? adapter_rows_kernel<kRowsStaged> : adapter_rows_kernel<kRowsPlain>;
+    const auto kernel = blocks ? adapter_rows_kernel<kRowsBlocks, TY>
+                               : share * R >= kStagedLeast ? adapter_rows_kernel<kRowsStaged, TY> : adapter_rows_kernel<kRowsPlain, TY>;
     launch_chained_cluster(kernel, dim3(parts, f_tiles128), dim3(kRowsThreads), smem, stream, parts, mw, mx, mb, mh, ids, (const float*)h,
-                           (const __nv_bfloat16*)B, (__nv_bfloat16*)y, rows, N, K, R, n, sl, NT, stages);
+                           (const __nv_bfloat16*)B, y, rows, N, K, R, n, sl, NT, stages);
     return check_launch("adapter_rows");
   }
   if (int rc = make_map(&mx, x, rows, K, kAdM)) return rc;
@@ -1150,24 +1171,24 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
   NF_REQUIRE(n_tiles < (1ll << 30), "adapter_linear: %d rows of %d features are too many", rows, N);
   int stages = (kWideSmem - kWideHead - kWideEpilogueWarps * kTurnBytes) / (kAdTile + BN / ctas * 128);
   stages = stages > kAdMaxStages ? kAdMaxStages : stages;
-  static int asked1 = room_for(adapter_wide_kernel<1>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2>, kWideSmem + 1024);
+  static int asked1 = room_for(adapter_wide_kernel<1, TY>, kWideSmem + 1024), asked2 = room_for(adapter_wide_kernel<2, TY>, kWideSmem + 1024);
   if (asked1 || asked2) return 1;
   const int at_once = sm_count() / ctas, grid = ctas * (n_tiles < at_once ? (int)n_tiles : at_once);
   if (ctas == 2)
-    launch_chained_cluster(adapter_wide_kernel<2>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, 2, mx, mw, mb, mh, ids,
-                           (__nv_bfloat16*)y, rows, N, K, R, n, places, sl, f_tiles, (int)n_tiles, BN, stages);
+    launch_chained_cluster(adapter_wide_kernel<2, TY>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, 2, mx, mw, mb, mh, ids,
+                           y, rows, N, K, R, n, places, sl, f_tiles, (int)n_tiles, BN, stages);
   else
-    launch_chained(adapter_wide_kernel<1>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, mx, mw, mb, mh, ids,
-                   (__nv_bfloat16*)y, rows, N, K, R, n, places, sl, f_tiles, (int)n_tiles, BN, stages);
+    launch_chained(adapter_wide_kernel<1, TY>, dim3(grid), dim3(kWideThreads), (size_t)kWideSmem + 1024, stream, mx, mw, mb, mh, ids,
+                   y, rows, N, K, R, n, places, sl, f_tiles, (int)n_tiles, BN, stages);
   return check_launch("adapter_wide");
 }
 
 // y = x W^T + the adapters' part (see the head of this file): x [rows, K], W [N, K], A [n, n_slices * R, K], B [n, N, R], y
-// [rows, N] bfloat16; scale float32 [n]; ids [rows], -1 for none; h: scratch of nf_adapter_scratch(rows, n_slices * R, n)
+// [rows, N] bfloat16 (y float32 where y_dtype says so); scale float32 [n]; ids [rows], -1 for none; h: scratch of nf_adapter_scratch(rows, n_slices * R, n)
 // floats.  ends: the n_slices features (host memory) at which the slices end, the last N.  K a multiple of 8, R 16, 32, 64
 // or 128, bases 16-byte aligned.
 extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, const void* B, const float* scale, const int* ids, float* h,
-                                 void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, cudaStream_t stream) {
+                                 void* y, int rows, int N, int K, int R, int n, int n_slices, const int* ends, int y_dtype, cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;
   NF_REQUIRE(rows > 0 && N > 0 && K > 0 && n > 0, "adapter_linear: bad sizes rows=%d N=%d K=%d n=%d", rows, N, K, n);
   NF_REQUIRE(K % 8 == 0, "adapter_linear: K=%d must be a multiple of 8", K);
@@ -1185,8 +1206,10 @@ extern "C" int nf_adapter_linear(const void* x, const void* W, const void* A, co
   const int pass = rows_a_pass(rows, n_slices * R, n);
   for (int t = 0; t < rows; t += pass) {
     const int now = rows - t < pass ? rows - t : pass;
-    if (int rc = adapter_pass((const __nv_bfloat16*)x + (size_t)t * K, W, A, B, scale, ids + t, h, (__nv_bfloat16*)y + (size_t)t * N, now, N, K, R, n,
-                              sl, stream)) return rc;
+    const auto pass_to = [&](auto* to) {
+      return adapter_pass((const __nv_bfloat16*)x + (size_t)t * K, W, A, B, scale, ids + t, h, to + (size_t)t * N, now, N, K, R, n, sl, stream);
+    };
+    if (int rc = y_dtype == kF32 ? pass_to((float*)y) : pass_to((__nv_bfloat16*)y)) return rc;
   }
   return 0;
 }

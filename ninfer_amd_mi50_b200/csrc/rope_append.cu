@@ -80,8 +80,12 @@ rope_append_kernel(T* __restrict__ qkv, const float* __restrict__ bias,
 
 // bfloat16, rotation over the whole head (rot == D, D % 16 == 0): a thread owns 8 consecutive
 // dims of the low half and the 8 matching dims of the high half of one head, 16 bytes each way.
+// SUMS: the projection comes as float32 sums [T, W] and is rounded once, after the rotation; of
+// qkv the query columns are written.  (16 rows of 16 + 2 x 16 heads of 128 read 393 KB instead of
+// 197: under what the launch takes.)
+template <bool SUMS>
 __global__ void __launch_bounds__(256)
-rope_append_bf16x8_kernel(__nv_bfloat16* __restrict__ qkv, const float* __restrict__ bias,
+rope_append_bf16x8_kernel(const float* __restrict__ sums, __nv_bfloat16* __restrict__ qkv, const float* __restrict__ bias,
                           const int* __restrict__ positions, const int* __restrict__ row_seg,
                           const float* __restrict__ inv_freq, int Hq, int Hkv, int D,
                           __nv_bfloat16* __restrict__ pages, const int* __restrict__ block_table,
@@ -90,10 +94,11 @@ rope_append_bf16x8_kernel(__nv_bfloat16* __restrict__ qkv, const float* __restri
   const int t = blockIdx.x;
   const int half = D / 2;
   chain_release();
-  chain_wait(qkv, positions, row_seg, block_table);
+  chain_wait(sums, qkv, positions, row_seg, block_table);
   const int pos = positions[t];
   const int W = (Hq + 2 * Hkv) * D;
   __nv_bfloat16* x = qkv + (size_t)t * W;
+  const float* xs = SUMS ? sums + (size_t)t * W : nullptr;
   const int groups = half / 8;             // 8-dim groups per half head
   const int heads = append ? Hq + 2 * Hkv : Hq;
   const int n_items = heads * groups;
@@ -104,6 +109,7 @@ rope_append_bf16x8_kernel(__nv_bfloat16* __restrict__ qkv, const float* __restri
   // and the page lookup are worked out while they are on their way.
   for (int idx0 = threadIdx.x; idx0 - (int)threadIdx.x < n_items; idx0 += 2 * blockDim.x) {
     uint4 ra[2], rb[2];
+    float fa[2][8], fb[2][8];
     int head[2], gi[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -111,9 +117,14 @@ rope_append_bf16x8_kernel(__nv_bfloat16* __restrict__ qkv, const float* __restri
       head[u] = idx / groups;
       gi[u] = idx - head[u] * groups;
       if (idx < n_items) {
-        const __nv_bfloat16* src = x + (size_t)head[u] * D + gi[u] * 8;
-        ra[u] = *reinterpret_cast<const uint4*>(src);
-        rb[u] = *reinterpret_cast<const uint4*>(src + half);
+        const size_t at = (size_t)head[u] * D + gi[u] * 8;
+        if (SUMS) {
+          load8(xs + at, fa[u]);
+          load8(xs + at + half, fb[u]);
+        } else {
+          ra[u] = *reinterpret_cast<const uint4*>(x + at);
+          rb[u] = *reinterpret_cast<const uint4*>(x + at + half);
+        }
       }
     }
     if (!have_table) {
@@ -140,8 +151,13 @@ rope_append_bf16x8_kernel(__nv_bfloat16* __restrict__ qkv, const float* __restri
       const size_t base = (size_t)head[u] * D;
       const int i0 = gi[u] * 8, i1 = half + gi[u] * 8;
       float a[8], b[8];
-      unpack8(ra[u], a);
-      unpack8(rb[u], b);
+      if (SUMS) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { a[e] = fa[u][e]; b[e] = fb[u][e]; }
+      } else {
+        unpack8(ra[u], a);
+        unpack8(rb[u], b);
+      }
       if (bias) {
         // 16-byte loads: one float at a time, a warp's loads of a bias touch eight lines each
         float ba[8], bb[8];
@@ -192,7 +208,7 @@ extern "C" int nf_rope_append(void* qkv, const float* bias, const int* positions
   NF_REQUIRE(smem <= 48 * 1024, "rope_append: rotary width %d too large", rot);
   if (dtype == kBF16 && rot == D && D % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)pages % 16 == 0 &&
       (uintptr_t)bias % 16 == 0) {
-    launch_chained(rope_append_bf16x8_kernel, dim3(T), dim3(256), smem, stream, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
+    launch_chained(rope_append_bf16x8_kernel<false>, dim3(T), dim3(256), smem, stream, (const float*)nullptr, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
     return check_launch("rope_append");
   }
   if (dtype == kF32)
@@ -200,4 +216,19 @@ extern "C" int nf_rope_append(void* qkv, const float* bias, const int* positions
   else
     rope_append_kernel<__nv_bfloat16><<<T, 256, smem, stream>>>((__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, rot, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
   return check_launch("rope_append");
+}
+
+// The same from float32 sums [T, W] to bfloat16 qkv (its query columns) and pages; the rotation covers the whole head.
+extern "C" int nf_rope_append_sums(const float* sums, void* qkv, const float* bias, const int* positions, const int* row_seg,
+                                   const float* inv_freq, int T, int Hq, int Hkv, int D, void* pages, const int* block_table,
+                                   int bt_width, int page_size, int num_pages, int append, cudaStream_t stream) {
+  if (T == 0) return 0;
+  NF_REQUIRE(T > 0 && Hq > 0 && Hkv > 0 && D > 0 && D % 16 == 0 && inv_freq, "rope_append_sums: bad sizes T=%d Hq=%d Hkv=%d D=%d", T, Hq, Hkv, D);
+  NF_REQUIRE(Hq + 2 * Hkv <= 65535, "rope_append_sums: too many heads");
+  NF_REQUIRE((uintptr_t)sums % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)pages % 16 == 0 && (uintptr_t)bias % 16 == 0,
+             "rope_append_sums: operands must be 16-byte aligned");
+  const size_t smem = (size_t)D * sizeof(float);
+  NF_REQUIRE(smem <= 48 * 1024, "rope_append_sums: head_dim %d too large", D);
+  launch_chained(rope_append_bf16x8_kernel<true>, dim3(T), dim3(256), smem, stream, sums, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
+  return check_launch("rope_append_sums");
 }

@@ -453,6 +453,11 @@ def linear_relu2(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def swiglu_keeps_sums(x: torch.Tensor) -> bool:
+    """Whether `linear_swiglu` gives its activation the product's float32 sums."""
+    return x.dtype == torch.float32 or _bf16_path(x.shape[0], x.shape[1], "bf16_linear") != "large"
+
+
 def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, act=None) -> torch.Tensor:
     """x [M, K], w [2I, K] (gate rows first) -> silu(x gate^T) * (x up^T)  [M, I]; `act`: another gated
     activation in silu's place (the product kernels' epilogues take it; after a library product it is a
@@ -498,6 +503,35 @@ def rope_append(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: torc
               _stream())
 
 
+def rope_keeps_sums(x: torch.Tensor, inv_freq: Optional[torch.Tensor], rotary_dim: int, D: int) -> bool:
+    """Whether `linear_rope_append` is one kernel, which rounds the projection once only, after the rotation."""
+    T, K = x.shape
+    return bool(TUNING["qkv_rope_fused"] and x.is_cuda and x.dtype == torch.bfloat16 and 0 < T <= min(16, TUNING["skinny_max_rows"])
+                and TUNING["bf16_linear"] == "auto" and K % 8 == 0 and D % 16 == 0 and rotary_dim == D
+                and inv_freq is not None)
+
+
+def rope_append_sums(sums: torch.Tensor, bias: Optional[torch.Tensor], positions: torch.Tensor, row_seg: torch.Tensor,
+                     inv_freq: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Tensor, block_table: torch.Tensor,
+                     page_size: int, append: bool) -> torch.Tensor:
+    """`rope_append` of a projection's float32 sums [T, (Hq + 2 Hkv) D] into bfloat16 pages, with the rotation over whole heads:
+    rounded once, after it.  -> bfloat16, of which the query columns are to be read."""
+    _chk(sums, "sums", torch.float32); _chk(pages, "pages", torch.bfloat16); _chk(inv_freq, "inv_freq", torch.float32)
+    _chk(block_table, "block_table", torch.int32); _chk(positions, "positions", torch.int32); _chk(row_seg, "row_seg", torch.int32)
+    if bias is not None:
+        _chk(bias, "bias", torch.float32)
+    if sums.dim() != 2 or sums.shape[1] != (Hq + 2 * Hkv) * D or inv_freq.numel() != D // 2:
+        raise ValueError("rope_append_sums: the width or the table does not match the head counts")
+    T = sums.shape[0]
+    if positions.numel() != T or row_seg.numel() != T:
+        raise ValueError(f"rope_append_sums: {positions.numel()} positions and {row_seg.numel()} segments for {T} rows")
+    qkv = torch.empty(sums.shape, dtype=pages.dtype, device=sums.device)
+    _lib.call("nf_rope_append_sums", _p(sums), _p(qkv), _p(bias), _p(positions), _p(row_seg), _p(inv_freq),
+              c_int(T), c_int(Hq), c_int(Hkv), c_int(D), _p(pages), _p(block_table), c_int(block_table.shape[1]),
+              c_int(page_size), c_int(pages.shape[0]), c_int(1 if append else 0), _stream())
+    return qkv
+
+
 def linear_rope_append(x: torch.Tensor, w_qkv: torch.Tensor, bias: Optional[torch.Tensor],
                        positions: torch.Tensor, row_seg: torch.Tensor, inv_freq: torch.Tensor,
                        rotary_dim: int, Hq: int, Hkv: int, D: int, pages: torch.Tensor,
@@ -507,9 +541,7 @@ def linear_rope_append(x: torch.Tensor, w_qkv: torch.Tensor, bias: Optional[torc
     cache).  A bfloat16 step of few rows does both in one kernel: the streaming product's
     epilogue adds the bias, rotates and writes keys and values into their cache page."""
     T, K = x.shape
-    if (TUNING["qkv_rope_fused"] and x.is_cuda and x.dtype == torch.bfloat16 and 0 < T <= min(16, TUNING["skinny_max_rows"])
-            and TUNING["bf16_linear"] == "auto" and K % 8 == 0 and D % 16 == 0 and rotary_dim == D
-            and inv_freq is not None):
+    if rope_keeps_sums(x, inv_freq, rotary_dim, D):
         _chk(x, "x"); _chk(w_qkv, "w_qkv", x.dtype); _chk(pages, "pages", x.dtype)
         _chk(block_table, "block_table", torch.int32); _chk(positions, "positions", torch.int32)
         _chk(row_seg, "row_seg", torch.int32); _chk(inv_freq, "inv_freq", torch.float32)

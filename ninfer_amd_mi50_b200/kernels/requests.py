@@ -24,8 +24,8 @@ MAX_ADAPTER_SLICES = 8
 
 _I, _P = ctypes.c_int, ctypes.c_void_p
 _SIGNATURES = {
-    "nf_adapter_add": [_P] * 8 + [_I] * 6 + [_P, _I, _P],
-    "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _P],
+    "nf_adapter_add": [_P] * 8 + [_I] * 6 + [_P, _I, _I, _P],
+    "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _I, _P],
     "nf_adapter_rows_f32": [_P] * 8 + [_I] * 6 + [_P, _P],
     "nf_append_history": [_P] * 4 + [_I] * 3 + [_P],
     "nf_adapter_scratch": [_I] * 3,
@@ -93,7 +93,7 @@ def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
     return p < q + t.numel() * t.element_size() and q < p + s.numel() * s.element_size()
 
 
-def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
+def _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype) -> None:
     """Says what is wrong with the operands of adapter_linear."""
     _chk(x, "x")
     for t, name in ((w, "w"), (a, "a"), (b, "b"), (scale, "scale"), (ids, "ids"), (out, "out")):
@@ -117,8 +117,10 @@ def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
                          f"{tuple(w.shape)}")
     if scale.numel() != n or ids.numel() != T:
         raise ValueError(f"adapter_linear: scale {tuple(scale.shape)} and ids {tuple(ids.shape)} for {n} adapters and {T} rows")
+    if out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"adapter_linear: out_dtype is {out_dtype}, not {x.dtype} or {torch.float32}")
     if out is not None:
-        _chk(out, "out", x.dtype)
+        _chk(out, "out", out_dtype)
         if out.shape != (T, N):
             raise ValueError(f"adapter_linear: out is {tuple(out.shape)}, not {(T, N)}")
         if T and _overlap(x, out):
@@ -129,19 +131,23 @@ def _refuse_adapter(x, w, a, b, scale, ids, widths, out) -> None:
 
 
 def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, ids: torch.Tensor,
-                   widths: Optional[Sequence[int]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   widths: Optional[Sequence[int]] = None, out: Optional[torch.Tensor] = None,
+                   out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [T, K] times w [N, K] transposed, plus every row's adapter -> [T, N]:
 
         out[t] = x[t] w^T + scale[i] (x[t] a[i]^T) b[i]^T,   i = ids[t];   ids[t] = -1: no adapter
 
     `widths`: the parts that the N features are stacked of (query, key and value, say), each with rows of `a` of its own;
     [N] if left out.  a [n, len(widths) * R, K] (the parts' rows one after the other), b [n, N, R], R one of
-    `ADAPTER_RANKS`, scale float32 [n], ids int32 [T].  Sums are float32 and rounded once, to x's type.  An id outside
+    `ADAPTER_RANKS`, scale float32 [n], ids int32 [T].  Sums are float32 and rounded once, to x's type, or
+    left as they are with `out_dtype` float32.  An id outside
     [-1, n) is served like -1 and, from n on, reported by `check_status`.  The weights of all adapters have to be finite:
     rows of several requests share a product, in which another request's adapter is multiplied by zero."""
     if widths is None:
         widths = (w.shape[0],)
     dtype, dev = x.dtype, x.get_device()
+    if out_dtype is None:
+        out_dtype = dtype
     xs, ws, bs = x.shape, w.shape, b.shape
     ends, S, total = _parts(widths)
     if not (dev >= 0 and len(xs) == 2 and len(ws) == 2 and len(bs) == 3 and (dtype is torch.bfloat16 or dtype is torch.float32)
@@ -149,34 +155,36 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
             and ids.dtype is torch.int32 and w.get_device() == dev and a.get_device() == dev and b.get_device() == dev
             and scale.get_device() == dev and ids.get_device() == dev and x.is_contiguous() and w.is_contiguous()
             and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous() and ids.is_contiguous()):
-        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype)
     T, K = xs
     N, (n, b_rows, R) = ws[0], bs
     if not (K > 0 and ws[1] == K and n > 0 and b_rows == N and R in ADAPTER_RANKS and 1 <= S <= MAX_ADAPTER_SLICES
-            and total == N and a.shape == (n, S * R, K) and scale.numel() == n and ids.numel() == T):
-        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
+            and total == N and a.shape == (n, S * R, K) and scale.numel() == n and ids.numel() == T
+            and (out_dtype is dtype or out_dtype is torch.float32)):
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype)
     if out is None:
-        out = x.new_empty((T, N))
-    elif not (out.dtype is dtype and out.get_device() == dev and out.is_contiguous() and out.shape == (T, N)) or _overlap(x, out):
-        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
+        out = x.new_empty((T, N), dtype=out_dtype)
+    elif not (out.dtype is out_dtype and out.get_device() == dev and out.is_contiguous() and out.shape == (T, N)) or _overlap(x, out):
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype)
     if T == 0:
         return out
     px, pw, pa, pb, po = x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), out.data_ptr()
     if (px | pw | pa | pb | po) & 15:
-        _refuse_adapter(x, w, a, b, scale, ids, widths, out)
+        _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype)
     bf16 = dtype is torch.bfloat16
     if TUNING["adapter"] == "auto" and (K % 8 == 0 if bf16 else K % 4 == 0 and T <= TUNING["adapter_f32_max_rows"]):
         # (h of a few rows lies row by row, see nf_adapter_scratch)
         h = scale.new_empty(_function("nf_adapter_scratch")(T, S * R, n) if bf16 and T > 16 else T * S * R)
         name = "nf_adapter_linear" if bf16 else "nf_adapter_rows_f32"
-        if _begin(name)(px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _stream(dev)):
+        more = (_dt(out),) if bf16 else ()
+        if _begin(name)(px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, *more, _stream(dev)):
             _failed(name)
         return out
     # many float32 rows, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
     h = scale.new_empty(T * S * R)
     z = linear(x, w, out_dtype=torch.float32)
     if _begin("nf_adapter_add")(px, pa, pb, scale.data_ptr(), ids.data_ptr(), z.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, _dt(x),
-                                _stream(dev)):
+                                _dt(out), _stream(dev)):
         _failed("nf_adapter_add")
     return out
 

@@ -38,8 +38,9 @@ class ProjectionAdapters:
         self.a = torch.zeros((capacity, n * rank, projection.in_features), dtype=dtype, device=device)
         self.b = torch.zeros((capacity, sum(projection.widths), rank), dtype=dtype, device=device)
 
-    def linear(self, x: torch.Tensor, w: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
-        return kernels.adapter_linear(x, w, self.a, self.b, self.scale, rows, self.projection.widths)
+    def linear(self, x: torch.Tensor, w: torch.Tensor, rows: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        kw = {} if out_dtype in (None, x.dtype) else {"out_dtype": out_dtype}
+        return kernels.adapter_linear(x, w, self.a, self.b, self.scale, rows, self.projection.widths, **kw)
 
     def clear(self, slot: int) -> None:
         self.a[slot].zero_()

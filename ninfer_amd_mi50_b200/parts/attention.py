@@ -100,11 +100,17 @@ class PagedGqaAttention(Mixer):
             kernels.rope_append(qkv, None, ctx.positions, ctx.row_seg, None, 0, Hq, Hkv, D,
                                 cache.pages, cache.block_table, cache.page_size, cache.append)
         elif self.adapter_pool("qkv", ctx) is not None:
-            # the adapters' part comes before the rotation
+            # the adapters' part comes before the rotation.  Rounded where the projection alone is: a row that has no adapter
+            # keeps its roundings beside rows that do
             inv_freq, rot = table
-            qkv = self.project("qkv", x, self.w_qkv, ctx)
-            kernels.rope_append(qkv, bias, ctx.positions, ctx.row_seg, inv_freq, rot, Hq, Hkv, D,
-                                cache.pages, cache.block_table, cache.page_size, cache.append)
+            if kernels.rope_keeps_sums(x, inv_freq, rot, D):
+                sums = self.project("qkv", x, self.w_qkv, ctx, torch.float32)
+                qkv = kernels.rope_append_sums(sums, bias, ctx.positions, ctx.row_seg, inv_freq, Hq, Hkv, D, cache.pages,
+                                               cache.block_table, cache.page_size, cache.append)
+            else:
+                qkv = self.project("qkv", x, self.w_qkv, ctx)
+                kernels.rope_append(qkv, bias, ctx.positions, ctx.row_seg, inv_freq, rot, Hq, Hkv, D,
+                                    cache.pages, cache.block_table, cache.page_size, cache.append)
         else:
             # projection, bias, rotation and the write of k, v at (request, position): one kernel
             # on small bfloat16 steps, two otherwise

@@ -396,11 +396,12 @@ class Part:
         pool = self.adapters.get(which)
         return pool if pool is not None and ctx.row_adapter is not None else None
 
-    def project(self, which: str, x: torch.Tensor, w: torch.Tensor, ctx: "StepContext") -> torch.Tensor:
-        """x w^T, with the rows' adapters beside it."""
+    def project(self, which: str, x: torch.Tensor, w: torch.Tensor, ctx: "StepContext",
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """x w^T, with the rows' adapters beside it; of x's type, or float32 sums with `out_dtype`."""
         from .. import kernels
         pool = self.adapter_pool(which, ctx)
-        return kernels.linear(x, w) if pool is None else pool.linear(x, w, ctx.row_adapter)
+        return kernels.linear(x, w, out_dtype=out_dtype) if pool is None else pool.linear(x, w, ctx.row_adapter, out_dtype)
 
     def tensor_specs(self) -> List[TensorSpec]:
         return []

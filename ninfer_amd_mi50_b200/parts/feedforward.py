@@ -110,11 +110,17 @@ class DenseSwiglu(FeedForward):
         return {"gate_up": Projection((self._n("gate"), self._n("up")), (I, I), H), "down": Projection((self._n("down"),), (H,), I)}
 
     def forward(self, x: torch.Tensor, ctx: StepContext):
+        in_epilogue = not self.has_bias and (self.activation is None or self.activation == kernels.ACT_GELU_TANH)
         if self.adapter_pool("gate_up", ctx) is not None:
-            gu = self.project("gate_up", x, self.w_gate_up, ctx)
-            act = kernels.silu_mul(gu) if self.activation is None else kernels.gated_bias_act(gu, None, self.activation, x.dtype)
-            return self.project("down", act, self.w_down, ctx)
-        if not self.has_bias and (self.activation is None or self.activation == kernels.ACT_GELU_TANH):
+            # rounded where the products without adapters are: a row that has none keeps its roundings beside rows that do
+            sums = not in_epilogue or kernels.swiglu_keeps_sums(x)
+            gu = self.project("gate_up", x, self.w_gate_up, ctx, torch.float32 if sums else None)
+            if self.activation is None and gu.dtype == x.dtype:
+                act = kernels.silu_mul(gu)
+            else:
+                act = kernels.gated_bias_act(gu, None, self.activation, x.dtype)
+            return self.project("down", act, self.w_down, ctx, None if in_epilogue else torch.float32)
+        if in_epilogue:
             # an activation without constants of its own sits where silu does: in the first product's epilogue
             act = {} if self.activation is None else {"act": self.activation}
             return kernels.linear(kernels.linear_swiglu(x, self.w_gate_up, **act), self.w_down)
