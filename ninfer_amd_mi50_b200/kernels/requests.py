@@ -14,7 +14,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import lib as _lib
-from .ops import TUNING, _chk, _dt, linear
+from .ops import TUNING, _DT, _chk, _dt, linear
 
 __all__ = ["ADAPTER_RANKS", "MAX_ADAPTER_SLICES", "adapter_linear", "adapter_rank", "adjust_logits", "append_history",
            "request_status"]
@@ -23,6 +23,7 @@ ADAPTER_RANKS = (16, 32, 64, 128)       # ranks that adapters are laid out for; 
 MAX_ADAPTER_SLICES = 8
 
 _I, _P = ctypes.c_int, ctypes.c_void_p
+_F32, _BF16 = _DT[torch.float32], _DT[torch.bfloat16]
 _SIGNATURES = {
     "nf_adapter_add": [_P] * 8 + [_I] * 6 + [_P, _I, _I, _P],
     "nf_adapter_linear": [_P] * 8 + [_I] * 6 + [_P, _I, _P],
@@ -163,7 +164,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
             and (out_dtype is dtype or out_dtype is torch.float32)):
         _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype)
     if out is None:
-        out = x.new_empty((T, N), dtype=out_dtype)
+        out = x.new_empty((T, N)) if out_dtype is dtype else x.new_empty((T, N), dtype=out_dtype)
     elif not (out.dtype is out_dtype and out.get_device() == dev and out.is_contiguous() and out.shape == (T, N)) or _overlap(x, out):
         _refuse_adapter(x, w, a, b, scale, ids, widths, out, out_dtype)
     if T == 0:
@@ -175,10 +176,13 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     if TUNING["adapter"] == "auto" and (K % 8 == 0 if bf16 else K % 4 == 0 and T <= TUNING["adapter_f32_max_rows"]):
         # (h of a few rows lies row by row, see nf_adapter_scratch)
         h = scale.new_empty(_function("nf_adapter_scratch")(T, S * R, n) if bf16 and T > 16 else T * S * R)
-        name = "nf_adapter_linear" if bf16 else "nf_adapter_rows_f32"
-        more = (_dt(out),) if bf16 else ()
-        if _begin(name)(px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends, *more, _stream(dev)):
-            _failed(name)
+        if bf16:
+            if _begin("nf_adapter_linear")(px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends,
+                                           _BF16 if out_dtype is dtype else _F32, _stream(dev)):
+                _failed("nf_adapter_linear")
+        elif _begin("nf_adapter_rows_f32")(px, pw, pa, pb, scale.data_ptr(), ids.data_ptr(), h.data_ptr(), po, T, N, K, R, n, S, ends,
+                                           _stream(dev)):
+            _failed("nf_adapter_rows_f32")
         return out
     # many float32 rows, or rows that TMA cannot fetch: the shared product by itself, the adapters added to its float32 sums
     h = scale.new_empty(T * S * R)
@@ -325,16 +329,17 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, slots: torch.Tens
         good = out.dtype is torch.float32 and out.get_device() == dev and out.shape == ls
     if not good:
         _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
-    if out is None:
+    given = out is not None
+    if given:
+        apart_out = _rows_apart(out, R, V)
+    else:
         out = penalties.new_empty((R, V))
         apart_out = V
-    else:
-        apart_out = _rows_apart(out, R, V)
     if R == 0 or V == 0:
         return out
     apart = _rows_apart(logits, R, V)
     p_in, p_out = logits.data_ptr(), out.data_ptr()
-    if apart < 0 or apart_out < 0 or _clash(p_in, apart, p_out, apart_out, R, V):
+    if apart < 0 or apart_out < 0 or (given and _clash(p_in, apart, p_out, apart_out, R, V)):
         _refuse_logits(logits, history, slots, lengths, starts, penalties, tokens, bias, mask, out)
     if _begin("nf_logit_rules")(p_in, p_out, p_history, slots.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
                                 None if tokens is None else tokens.data_ptr(), penalties.data_ptr(), p_off, p_ids, p_values, n_bias, p_bits,
