@@ -77,6 +77,11 @@ def check_rules(p: SamplingParams, vocab: int) -> None:
 
 def check_params(p: SamplingParams, vocab: int) -> None:
     check_rules(p, vocab)
+    check_draw(p, vocab)
+
+
+def check_draw(p: SamplingParams, vocab: int) -> None:
+    """Raises ValueError for limits of a draw that the device sampler does not take."""
     if p.greedy:
         return
     k = min(max(p.top_k, 1), vocab)
@@ -205,7 +210,7 @@ class Sampler:
         out = kernels.argmax_rows(logits)
         rows = [r for r in range(R) if not params[r].greedy]
         for r in rows:
-            check_params(params[r], self.vocab_size)
+            (check_params if params[r].has_rules else check_draw)(params[r], self.vocab_size)
         sel = torch.tensor(rows, dtype=torch.long, device=dev)
         sub = logits.index_select(0, sel) if len(rows) < R else logits
         temp = torch.tensor([params[r].temperature for r in rows], dtype=torch.float32).to(dev)
