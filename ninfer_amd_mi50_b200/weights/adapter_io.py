@@ -26,9 +26,14 @@ def read_adapter(folder: str) -> Tuple[Dict[str, Tuple[torch.Tensor, torch.Tenso
         raise SafetensorsError(f"{folder}/adapter_config.json: r and lora_alpha must be numbers") from None
     if r < 1:
         raise SafetensorsError(f"{folder}/adapter_config.json: r={r}")
-    for key in ("rank_pattern", "alpha_pattern", "modules_to_save"):
+    # what would change the product beyond scale B A: scales of single tensors, norms, tokens from which it counts, other base weights
+    for key in ("rank_pattern", "alpha_pattern", "modules_to_save", "use_dora", "alora_invocation_tokens", "trainable_token_indices",
+                "layer_replication"):
         if cfg.get(key):
             raise SafetensorsError(f"{folder}/adapter_config.json: {key} is not supported")
+    start = str(cfg.get("init_lora_weights", True)).lower()
+    if start.startswith(("pissa", "olora", "corda", "loftq")):
+        raise SafetensorsError(f"{folder}/adapter_config.json: init_lora_weights {start!r} goes with base weights of its own")
     found: Dict[str, Dict[str, torch.Tensor]] = {}
     f = SafetensorsFile(os.path.join(folder, "adapter_model.safetensors"))
     try:

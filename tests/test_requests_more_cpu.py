@@ -251,3 +251,17 @@ def test_a_token_that_two_biases_name_is_refused():
     p = SamplingParams(0.0, logit_bias={"5": 99.0})
     check_params(p, 50)
     assert sample_reference([0.0] * 50, p) == 5
+
+
+@pytest.mark.parametrize("key,value", [("use_dora", True), ("alora_invocation_tokens", [1, 2]), ("trainable_token_indices", [3]),
+                                       ("layer_replication", [[0, 2]]), ("init_lora_weights", "pissa"), ("init_lora_weights", "loftq")])
+def test_a_folder_that_says_more_than_a_pair_a_tensor_is_refused(key, value, tmp_path):
+    import json
+    from ninfer_amd_mi50_b200.weights import SafetensorsError, read_adapter, write_safetensors
+    write_safetensors(str(tmp_path / "adapter_model.safetensors"), [("m.lora_A.weight", torch.zeros(2, 4)), ("m.lora_B.weight", torch.zeros(6, 2))])
+    config = {"r": 2, "lora_alpha": 4, "peft_type": "LORA", "init_lora_weights": True, "use_dora": False, "layer_replication": None}
+    (tmp_path / "adapter_config.json").write_text(json.dumps(config))
+    assert read_adapter(str(tmp_path))[1] == 2.0
+    (tmp_path / "adapter_config.json").write_text(json.dumps(dict(config, **{key: value})))
+    with pytest.raises(SafetensorsError, match=key):
+        read_adapter(str(tmp_path))
