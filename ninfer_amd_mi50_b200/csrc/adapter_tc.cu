@@ -463,8 +463,8 @@ __device__ __forceinline__ int next_tile(int i, int first, int stride) { return 
 // Warps: 0 producer, 1 MMA and tensor memory, 2..9 epilogue.  map_h: h as the first product lays it out, `places` blocks a row tile.
 // TY: the type of y, bfloat16, or float32 for a caller that has more to do with the sums.
 // What bounds it: the tensor cores (73 % busy under the profiler at 2048 rows of 2048 x 6144) and the operands' way into shared memory,
-// which at 256 x 256 a pair takes as long as the products: 512 cycles a step, 600 to 700 measured.  8192 rows of 3584 x 4608 take 190 us
-// with h, 1.43 PFLOP/s; the library's product without adapters 172.
+// which at 256 x 256 a pair takes as long as the products: 512 cycles a step, 600 to 700 measured.  8192 rows of 3584 x 4608 take 194 us
+// with h, 1.4 PFLOP/s; the library's product without adapters 172.
 template <int CTAS, typename TY>
 __global__ void __launch_bounds__(kWideThreads, 1)
 adapter_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_b,
@@ -691,7 +691,7 @@ constexpr int kRowsAtOnce = 4;             // rows of x whose rows of B a thread
 // kRowsBlocks: steps of the product, h in the blocks of the wide kernel, rows of B brought into L2 while W is read.  64 rows of 2048 x
 // 3584, 24 adapters: rank 16 18.3 us instead of 12.2, the products, their sums and their way to the owners now come behind h; rank 64 23.1
 // instead of 36.1, rank 128 35.6 instead of 62.8.
-// What bounds it: one row of 2048 x 2048 takes 7.1 us, its 8.4 MB 1.3: launch, the first loads, the members' sums, h and the rows of y,
+// What bounds it: one row of 2048 x 2048 takes 7.5 us, its 8.4 MB 1.3: launch, the first loads, the members' sums, h and the rows of y,
 // one after the other.  64 rows of 3584 x 3584 with 48 adapters of rank 32 take 19.6 us, their 43 MB 6.7: h is there after 12, W's sums
 // by then, and the adapters' part takes 4.
 template <RowsForm FORM, typename TY>
@@ -1075,6 +1075,9 @@ static int adapter_pass(const void* x, const void* W, const void* A, const void*
   }
 
   // ---- h
+  // Few rows: a warp a number.  K 2048, N 3584, 24 adapters of rank 16, the whole call that way and on tensor cores: 17 rows 8.2 and 9.6 us,
+  // 24 rows 8.4 and 10.0, 32 rows 10.2 and 9.6, 64 rows 13.4 and 12.0; K 3584, 48 adapters of rank 32: 17 rows 15.0 and 14.6, 24 rows 15.6 and
+  // 16.8, 32 rows 16.3 and 17.0, 64 rows 21.6 and 19.7; K 2048, N 6144, 16 adapters of rank 16: 17 rows 11.8 and 12.8, 64 rows 16.3 and 17.0.
   if (rows <= 16) {
     if (int rc = adapter_shrink_simt(x, A, scale, ids, h, rows, K, SR, n, stream)) return rc;
   } else {

@@ -102,10 +102,10 @@ struct PieceLog {
 // row's start.  It copies the piece's logits under the mask, WALK steps of PIECES runs of four a thread, and then does what is left to
 // do at the biased tokens and at those that occur in the log, one thread each.  (Done where the logits are copied, the powers and
 // quotients of the few tokens that occur held up nearly every warp: 204 instructions a run of four, 256 rows of 151936 99 us.)
-// What bounds it: 256 rows of 151936 take 64 us, of which the copy alone, as it runs without rules, 49 (6.3 TB/s); the rest is a CTA's
-// chain from a row's numbers to its log to the counts to the list.  So everything that does not wait for anything is asked for first,
+// What bounds it: 256 rows of 151936 take 64 us, of which the copy alone, as it runs without rules, 49 (6.3 TB/s), 64 rows 22.3 of which the
+// copy 13.7 (16.6 under masks); the rest is a CTA's chain from a row's numbers to its log to the counts to the list.  So everything that does not wait for anything is asked for first,
 // the log's loads are under way while the logits are copied, a walked piece's logits are brought into L2 meanwhile, and a walked
-// piece leaves room for three CTAs on an SM (two: a tenth longer).  One row of 151936 and a short log 2.6 us: the chain and the launch.
+// piece leaves room for three CTAs on an SM (two: a tenth longer).  One row of 151936 and a short log 2.9 us: the chain and the launch.
 // SPLIT: CTAs of a cluster, with a piece each.  A long log is shared out: each CTA counts a part of it for all SPLIT pieces, and adds up what
 // the others have for its own.
 template <int THREADS, int PIECES, int WALK, bool WORD, int SPLIT>
@@ -382,6 +382,7 @@ extern "C" int nf_logit_rules(const float* logits, float* out, int* history, con
   // Few rows whose logs may be long: pieces of 2048 in clusters of four, which share out a log of kSharedLog tokens and more (alone and in
   // clusters, us: 5 rows of 32003 and logs of 131,072 tokens 17.5 and 10.6, one of 151936 20.6 and 10.5, with a log of 2,000 3.2 and 3.4).
   // More rows read their logs faster in pieces of 4096 and 8192 (16 rows of 151936 and logs of 131,072 tokens 29, in clusters 39).
+  // (The lengths are on the device: what the host knows of the logs, for this and for the counts' words, is how long they may become.)
   const auto ctas = [&](int piece) { return (long long)rows * ((V + 3 + piece - 1) / piece); };
   const bool word = capacity < 65536;
   const auto run = [&](auto threads, auto pieces, auto walk, auto packed, auto split) {
