@@ -91,7 +91,7 @@ def apply_rules(logits: torch.Tensor, rows: Sequence[RuleRow], logs: TokenLogs, 
         new_tokens, new_slots, new_at = [], [], []
         for r, slot in zip(back, logs.place(back)):
             n, known = len(r.tokens), logs.known[slot]
-            slots[r.row], lengths[r.row], starts[r.row] = slot, n, r.prompt_length
+            slots[r.row], lengths[r.row], starts[r.row] = slot, n, min(r.prompt_length, n)
             penalties[r.row] = r.params.repetition_penalty, r.params.frequency_penalty, r.params.presence_penalty
             if known > n:                                    # a log never shrinks: this is another list of tokens
                 known = 0

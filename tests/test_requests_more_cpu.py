@@ -265,3 +265,15 @@ def test_a_folder_that_says_more_than_a_pair_a_tensor_is_refused(key, value, tmp
     (tmp_path / "adapter_config.json").write_text(json.dumps(dict(config, **{key: value})))
     with pytest.raises(SafetensorsError, match=key):
         read_adapter(str(tmp_path))
+
+
+def test_a_prompt_longer_than_the_tokens_is_all_of_them(monkeypatch):
+    """The device reports a start beyond the log."""
+    plain_kernels.install(monkeypatch)
+    plain_requests.install(monkeypatch)
+    seen, twin = [], kernels.adjust_logits
+    monkeypatch.setattr(kernels, "adjust_logits", lambda l, h, s, lengths, starts, *a, **k: (seen.append((lengths.tolist(), starts.tolist())),
+                                                                                            twin(l, h, s, lengths, starts, *a, **k))[1])
+    p = SamplingParams(0.0, presence_penalty=100.0)
+    out = Sampler(50, "cpu").sample(torch.arange(50.0)[None], [p], recent=[[49, 48]], prompt_lengths=[5], keys=["a"])
+    assert out.tolist() == [49] and seen == [([2], [2])]
