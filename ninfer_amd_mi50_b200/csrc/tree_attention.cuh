@@ -1,0 +1,53 @@
+// What the kernels of tree attention share: a request's rows and keys, which of them a row sees, and the host's side of
+// shared memory beyond 48 KB.
+#pragma once
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace nf {
+
+constexpr int kTreeRows = 16;     // (node, query head) pairs of a CTA on CUDA cores
+
+struct TreeArgs {
+  const int *block_table, *lengths, *row0, *mask;
+  float *ws_acc, *ws_ml;          // [shares][T][Hq][D], [shares][T][Hq][2]
+  long long q_stride;
+  int bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context, chunk, shares;
+  float scale;
+};
+
+struct TreeRequest {
+  int row0, nodes, len, keys;     // its rows, the keys it held, these and its nodes'
+  bool bad;
+};
+
+// What the tensors say of request s, brought into the bounds that the call gave.
+__device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int s) {
+  TreeRequest r;
+  const int begin = a.row0[s], end = a.row0[s + 1], len = a.lengths[s];
+  r.row0 = min(max(begin, 0), a.T);
+  r.nodes = min(min(max(end, r.row0), a.T) - r.row0, 32 * a.words);
+  r.len = min(max(len, 0), a.max_context);
+  r.keys = min(r.len + r.nodes, a.max_context);      // (both below 2^30: see the call)
+  r.bad = begin < 0 || end < begin || end > a.T || end - begin > 32 * a.words || len < 0 || len > a.max_context - r.nodes;
+  return r;
+}
+
+// Whether node i of the request sees key j < r.keys.
+__device__ __forceinline__ bool tree_sees(const TreeArgs& a, const TreeRequest& r, int i, int j) {
+  const int k = j - r.len;
+  return k < 0 || (a.mask[(size_t)(r.row0 + i) * a.words + (k >> 5)] >> (k & 31) & 1);
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device.
+inline int allow_smem(const void* kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  NF_REQUIRE(e == cudaSuccess, "cannot have %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+  return 0;
+}
+
+}  // namespace nf

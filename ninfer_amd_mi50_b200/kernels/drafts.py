@@ -1,0 +1,284 @@
+"""Python faces of the kernels by which a request tries several continuations at once: attention of a tree of drafted
+tokens over its cache, which of them the model's probabilities let stand, the cache's rows of those moved up behind what
+the request held, and pages copied for a request that is forked.
+
+A step's nodes are rows, a request's rows lie together: `row0` int32 [S + 1] says where each request's begin.  Node 0 of a
+request is its tree's root, the newest token that it has; the others are drafted.  Keys and values of node i go into the
+request's pages at position lengths[s] + i, whatever its depth (`rope_append` with these positions and no rotation, after
+one that rotates by the depth and appends nothing).  Everything is on the device, so that a captured step serves any trees.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import lib as _lib
+from .ops import _DT, _chk, _dt, check_head_dim
+
+__all__ = ["MAX_TREE_NODES", "MAX_VERIFY_NODES", "compact_cache", "copy_pages", "draft_status", "tree_attention", "verify_drafts"]
+
+MAX_TREE_NODES = 256          # nodes of a request that tree attention takes
+MAX_VERIFY_NODES = 1024       # ... and verification
+MAX_TREE_CONTEXT = 1 << 30
+
+_I, _L, _P, _F = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_float
+_SIGNATURES = {
+    "nf_tree_attention_chunk": [_I] * 6,
+    "nf_tree_attention": [_P, _L, _P, _P, _I] + [_P] * 3 + [_I] + [_P] * 2 + [_I] * 9 + [_F, _I, _P],
+    "nf_verify_drafts": [_P, _L, _P, _L] + [_P] * 7 + [_I] * 4 + [_P],
+    "nf_compact_cache": [_P, _L] + [_I] * 5 + [_P, _I] + [_P] * 3 + [_I] * 2 + [_P],
+    "nf_copy_pages": [_P, _L] + [_I] * 5 + [_P] * 3 + [_I, _P],
+}
+_functions = {}
+_used = False           # whether any of these kernels was called: until then there is no status to read
+
+
+def _function(name: str):
+    f = _functions.get(name)
+    if f is None:
+        f = getattr(_lib.load(), name)
+        f.argtypes = _SIGNATURES[name]
+        _functions[name] = f
+    return f
+
+
+def _call(name: str, device: int, *args) -> None:
+    """The C function, on the current stream of the tensors' device."""
+    global _used
+    _used = True
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            _call(name, device, *args)
+        return
+    _lib.count_launches(1)
+    if (_functions.get(name) or _function(name))(*args, torch._C._cuda_getCurrentRawStream(device)):
+        raise _lib.KernelError(f"{name}: {_lib.load().nf_last_error().decode(errors='replace')}")
+
+
+def _ints(what: str, device, **tensors) -> None:
+    """Refuses index tensors that are not contiguous int32 ones on `device`."""
+    for name, t in tensors.items():
+        _chk(t, name, torch.int32)
+        if t.device != device:
+            raise ValueError(f"{what}: {name} lies on {t.device}, not on {device}")
+
+
+def _same_memory(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the memory that two tensors span overlaps."""
+    def span(v):
+        return v.data_ptr(), v.data_ptr() + v.element_size() * (1 + sum((n - 1) * d for n, d in zip(v.shape, v.stride())))
+    (a, b), (c, d) = span(s), span(t)
+    return s.numel() > 0 and t.numel() > 0 and a < d and c < b
+
+
+def _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, out) -> None:
+    """Says what is wrong with the operands of tree_attention."""
+    what = "tree_attention"
+    _chk(qkv, "qkv", contiguous=False)
+    _dt(qkv)
+    _chk(pages, "pages", qkv.dtype)
+    check_head_dim(D)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads do not divide into {Hkv} groups")
+    if qkv.dim() != 2 or qkv.shape[1] < Hq * D or qkv.stride(1) != 1 or (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
+        raise ValueError(f"{what}: qkv is {tuple(qkv.shape)} with strides {qkv.stride()}; rows of {Hq} heads of {D} are wanted")
+    if page_size < 1 or pages.dim() != 5 or pages.shape[1:] != (2, Hkv, page_size, D) or not 1 <= pages.shape[0] < 1 << 31:
+        raise ValueError(f"{what}: pages are {tuple(pages.shape)}, not [pages, 2, {Hkv}, {page_size}, {D}]")
+    if pages.device != qkv.device:
+        raise ValueError(f"{what}: pages lie on {pages.device}, qkv on {qkv.device}")
+    _ints(what, qkv.device, block_table=block_table, lengths=lengths, row0=row0, mask=mask)
+    T = qkv.shape[0]
+    if block_table.dim() != 2 or block_table.shape[1] < 1 or lengths.shape != block_table.shape[:1] or row0.shape != (lengths.numel() + 1,):
+        raise ValueError(f"{what}: block table {tuple(block_table.shape)}, lengths {tuple(lengths.shape)} and row0 {tuple(row0.shape)} "
+                         f"are not of one number of requests (row0: one more)")
+    if mask.dim() != 2 or mask.shape[0] != T or not 1 <= mask.shape[1] <= MAX_TREE_NODES // 32:
+        raise ValueError(f"{what}: mask is {tuple(mask.shape)}, not [{T}, 1 to {MAX_TREE_NODES // 32}]")
+    if not 1 <= max_context <= MAX_TREE_CONTEXT:
+        raise ValueError(f"{what}: max_context={max_context} is not within 1 and {MAX_TREE_CONTEXT}")
+    if pages.data_ptr() % 16:
+        raise ValueError(f"{what}: pages do not start on a 16-byte boundary")
+    if out is not None:
+        _chk(out, "out", qkv.dtype)
+        if out.shape != (T, Hq * D) or out.device != qkv.device:
+            raise ValueError(f"{what}: out is {tuple(out.shape)} on {out.device}, not {(T, Hq * D)} on {qkv.device}")
+        for t, name in ((qkv, "qkv"), (pages, "pages")):
+            if _same_memory(out, t):
+                raise ValueError(f"{what}: out shares memory with {name}")
+
+
+def tree_attention(qkv: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Tensor, block_table: torch.Tensor, page_size: int,
+                   lengths: torch.Tensor, row0: torch.Tensor, mask: torch.Tensor, max_context: int, scale: float,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the (rotated) queries of trees of drafted tokens over the cache -> [T, Hq * D].
+
+    qkv [T, at least Hq * D] (rows may lie further apart): queries in the first columns.  Request s holds lengths[s] keys;
+    its rows row0[s] .. row0[s + 1] - 1 are its nodes, whose keys and values are in its pages already, node i's at position
+    lengths[s] + i.  A row sees all keys that the request held, and node k's where bit k % 32 of word k // 32 of its mask
+    (int32 [T, words], words for as many nodes as a request may have) is set: its ancestors and itself, as a rule, but any
+    set will do.  A row that sees nothing is zero.  pages [pages, 2, Hkv, page_size, D], block_table int32 [S, width];
+    `max_context`: what lengths[s] and a request's nodes add up to at most.  All of a page's rows must hold finite numbers,
+    as they do in a cache manager's pool.
+
+    Rows that belong to no request stay as they were in `out`.  Rows, lengths or nodes outside the bounds, and pages outside
+    the pool, count as if they ended there, and are reported by `check_status`."""
+    dtype, dev = qkv.dtype, qkv.get_device()
+    qs, bs, ms = qkv.shape, block_table.shape, mask.shape
+    if not (dev >= 0 and dtype in _DT and pages.dtype is dtype and pages.get_device() == dev and pages.is_contiguous() and len(qs) == 2
+            and len(bs) == 2 and len(ms) == 2 and D % 16 == 0 and 16 <= D <= 256 and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and page_size > 0
+            and qs[1] >= Hq * D and qkv.stride(1) == 1 and (qs[0] <= 1 or qkv.stride(0) >= qs[1]) and 1 <= pages.shape[0] < 1 << 31
+            and pages.shape[1:] == (2, Hkv, page_size, D) and block_table.dtype is torch.int32 and lengths.dtype is torch.int32
+            and row0.dtype is torch.int32 and mask.dtype is torch.int32 and block_table.get_device() == dev and lengths.get_device() == dev
+            and row0.get_device() == dev and mask.get_device() == dev and block_table.is_contiguous() and lengths.is_contiguous()
+            and row0.is_contiguous() and mask.is_contiguous() and bs[1] > 0 and lengths.shape == bs[:1] and row0.shape == (bs[0] + 1,)
+            and ms[0] == qs[0] and 1 <= ms[1] <= MAX_TREE_NODES // 32 and 1 <= max_context <= MAX_TREE_CONTEXT
+            and pages.data_ptr() % 16 == 0):
+        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, out)
+    T, S = qs[0], bs[0]
+    if out is None:
+        out = qkv.new_empty((T, Hq * D))
+    else:
+        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, out)
+    if T == 0 or S == 0:
+        return out
+    chunk = _function("nf_tree_attention_chunk")(S, T, Hq, Hkv, ms[1], max_context)
+    shares = -(-max_context // chunk)
+    ws = torch.empty(shares * T * Hq * (D + 2), dtype=torch.float32, device=qkv.device) if shares > 1 else None
+    _call("nf_tree_attention", dev, qkv.data_ptr(), qkv.stride(0) if T > 1 else qs[1], pages.data_ptr(), block_table.data_ptr(), bs[1],
+          lengths.data_ptr(), row0.data_ptr(), mask.data_ptr(), ms[1], out.data_ptr(), None if ws is None else ws.data_ptr(), S, T, Hq, Hkv, D,
+          page_size, pages.shape[0], max_context, chunk, scale, _DT[dtype])
+    return out
+
+
+def _rows(t: torch.Tensor, name: str, T: int, V: int, device) -> int:
+    """Numbers between two rows of float32 [T, V]; raises where they are not runs of their own."""
+    _chk(t, name, torch.float32, contiguous=False)
+    if t.device != device or t.shape != (T, V):
+        raise ValueError(f"verify_drafts: {name} is {tuple(t.shape)} on {t.device}, not {(T, V)} on {device}")
+    if T <= 1 or V <= 1:
+        step = t.stride(0) if T > 1 else V
+    else:
+        step = t.stride(0)
+    if (V > 1 and t.stride(1) != 1) or step < V:
+        raise ValueError(f"verify_drafts: the rows of {name} must be runs of their own, got strides {t.stride()}")
+    return step
+
+
+def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, row0: torch.Tensor, draws: torch.Tensor, most: int,
+                  draft: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stand, and the token after them -> (accepted int32 [S], path int32 [S, most], said int32
+    [S, most + 1]).
+
+    probs float32 [T, V] (rows may lie further apart): row t is the model's distribution behind node t's token.  Rows
+    row0[s] .. row0[s + 1] - 1 are the nodes of request s (1 to `MAX_VERIFY_NODES`); node i's token is tokens[row0[s] + i],
+    its parent, a node before it, parents[row0[s] + i] (the root's is not read).  draws float32 [T] are uniform numbers in
+    [0, 1).  draft float32 [T, V]: the distributions that the tokens were drawn from, row t that of node t's; left out,
+    drafted tokens stand for themselves (they were looked up, or are a model's likeliest).
+
+    From v = 0 on, with r = probs[v] and z = 1, v's children c are asked in ascending order: where
+    draws[c] z draft[c][x_c] < r[x_c] (left out: draws[c] z < r[x_c]), c is accepted and takes v's place; else
+    r = max(r - z draft[c], 0) and z = sum(r) (left out: z -= r[x_c], r[x_c] = 0).  Where no child is left, or `most` are
+    accepted, the next token is the lowest whose running sum of r passes draws[root] sum(r).  Tokens are then distributed as
+    the model's own, one after the other.  Sums are 64 bits wide.
+
+    `path[s]` lists the accepted nodes, `said[s]` their tokens and the next one, both with -1 behind; accepted[s] counts
+    the drafted ones.  What is no positive number counts as a probability of 0; a row that holds nothing gives -1.  Nodes
+    whose token or parent makes no sense are nobody's children.  Both are reported by `check_status`."""
+    _chk(probs, "probs", torch.float32, contiguous=False)
+    if probs.dim() != 2 or probs.shape[1] < 1:
+        raise ValueError(f"verify_drafts: probs are {tuple(probs.shape)}, not [rows, vocabulary]")
+    T, V = probs.shape
+    dev = probs.device
+    _ints("verify_drafts", dev, tokens=tokens, parents=parents, row0=row0)
+    _chk(draws, "draws", torch.float32)
+    if draws.device != dev:
+        raise ValueError(f"verify_drafts: draws lie on {draws.device}, not on {dev}")
+    for t, name in ((tokens, "tokens"), (parents, "parents"), (draws, "draws")):
+        if t.shape != (T,):
+            raise ValueError(f"verify_drafts: {name} are {tuple(t.shape)}, not {(T,)}")
+    if row0.dim() != 1 or row0.numel() < 1:
+        raise ValueError(f"verify_drafts: row0 is {tuple(row0.shape)}, not [requests + 1]")
+    if not 1 <= most <= MAX_VERIFY_NODES:
+        raise ValueError(f"verify_drafts: most={most} is not within 1 and {MAX_VERIFY_NODES}")
+    probs_ld = _rows(probs, "probs", T, V, dev)
+    draft_ld = 0 if draft is None else _rows(draft, "draft", T, V, dev)
+    S = row0.numel() - 1
+    out = torch.empty(S * (2 * most + 2), dtype=torch.int32, device=dev)
+    accepted, path, said = out[:S], out[S:S * (most + 1)].view(S, most), out[S * (most + 1):].view(S, most + 1)
+    if S and not T:
+        raise ValueError(f"verify_drafts: {S} requests without a row")
+    if S:
+        _call("nf_verify_drafts", probs.get_device(), probs.data_ptr(), probs_ld, None if draft is None else draft.data_ptr(), draft_ld,
+              tokens.data_ptr(), parents.data_ptr(), row0.data_ptr(), draws.data_ptr(), accepted.data_ptr(), path.data_ptr(), said.data_ptr(),
+              S, T, V, most)
+    return accepted, path, said
+
+
+def _shape(what: str, pages: torch.Tensor) -> Tuple[int, ...]:
+    """(address, bytes between two layers, layers, pages, planes, page size, row bytes) of a cache group's pages: one layer's
+    [pages, 2, heads, page_size, D] or [pages, page_size, width], or with the layers before that."""
+    _chk(pages, "pages", contiguous=False)
+    if pages.dim() not in (3, 4, 5, 6):
+        raise ValueError(f"{what}: pages are {tuple(pages.shape)}, not (layers,) pages, (2, heads,) page_size, width")
+    layered = pages if pages.dim() in (4, 6) else pages.unsqueeze(0)
+    L, P, size = layered.shape[0], layered.shape[1], layered.element_size()
+    if layered.numel() == 0:
+        raise ValueError(f"{what}: pages are {tuple(pages.shape)}")
+    if not layered[0].is_contiguous() or (L > 1 and layered.stride(0) < layered[0].numel()):
+        raise ValueError(f"{what}: a layer's pages must be contiguous, got strides {pages.stride()}")
+    planes = layered.shape[2] * layered.shape[3] if layered.dim() == 6 else 1
+    row = layered.shape[-1] * size
+    if row % 2 or max(P, planes, layered.shape[-2], row, L) >= 1 << 31:
+        raise ValueError(f"{what}: rows of {layered.shape[-1]} numbers of {size} bytes, in pages {tuple(pages.shape)}")
+    return layered.data_ptr(), (layered.stride(0) if L > 1 else layered[0].numel()) * size, L, P, planes, layered.shape[-2], row
+
+
+def compact_cache(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
+    """In every layer of `pages`, the cache's rows of the nodes that were kept move up behind what their request held:
+
+        row lengths[s] + 1 + j  takes the place of  row lengths[s] + path[s, j],    j < accepted[s]
+
+    so that they lie as if they alone had been run behind the root, whose row, lengths[s], stays.  pages: a cache group's
+    [layers, pages, 2, heads, page_size, D] or [layers, pages, page_size, width], or one layer's; block_table int32
+    [S, width]; path int32 [S, most] (rising) and accepted int32 [S] as `verify_drafts` gives them.  A request whose path does
+    not rise keeps its rows as they are, a row whose page is not in the pool stays: both are reported by `check_status`."""
+    shape = _shape("compact_cache", pages)
+    _ints("compact_cache", pages.device, block_table=block_table, lengths=lengths, path=path, accepted=accepted)
+    if (block_table.dim() != 2 or block_table.shape[1] < 1 or path.dim() != 2 or lengths.dim() != 1 or lengths.shape != block_table.shape[:1]
+            or accepted.shape != lengths.shape or path.shape[0] != lengths.numel()):
+        raise ValueError(f"compact_cache: block table {tuple(block_table.shape)}, lengths {tuple(lengths.shape)}, path {tuple(path.shape)} and "
+                         f"accepted {tuple(accepted.shape)} are not of one number of requests")
+    S, most = path.shape
+    if S and most:
+        _call("nf_compact_cache", pages.get_device(), *shape, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), path.data_ptr(),
+              accepted.data_ptr(), S, most)
+
+
+def copy_pages(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
+    """In every layer of `pages` (as `compact_cache` takes them), page dst[i] becomes page src[i]: its first rows[i] rows
+    where `rows` is given, the others then stay.  src, dst and rows are int32 lists of one length; no page may be written
+    twice, or be read and written.  An entry that is outside the pool, or has more rows than a page, is left out and
+    reported by `check_status`."""
+    shape = _shape("copy_pages", pages)
+    _ints("copy_pages", pages.device, src=src, dst=dst, **({} if rows is None else {"rows": rows}))
+    if src.dim() != 1 or dst.shape != src.shape or (rows is not None and rows.shape != src.shape):
+        raise ValueError(f"copy_pages: src {tuple(src.shape)}, dst {tuple(dst.shape)}"
+                         + ("" if rows is None else f" and rows {tuple(rows.shape)}") + " are not lists of one length")
+    if src.numel():
+        _call("nf_copy_pages", pages.get_device(), *shape, src.data_ptr(), dst.data_ptr(), None if rows is None else rows.data_ptr(), src.numel())
+
+
+def draft_status() -> int:
+    """0, or what these kernels met since the last call: 1000001 + a request whose lengths, rows or pages did not fit tree
+    attention, 2000001 + one whose tree or probabilities made no sense to verification, 3000001 + a request or an entry whose
+    path or pages did not fit a copy.  Synchronises the device; where none was ever called there is nothing to read."""
+    if not _used:
+        return 0
+    lib = _lib.load()
+    for k, name in enumerate(("nf_tree_attention_status", "nf_verify_drafts_status", "nf_cache_pages_status"), 1):
+        v = int(getattr(lib, name)())
+        if v:
+            return k * 1000000 + v
+    return 0

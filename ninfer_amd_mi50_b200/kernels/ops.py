@@ -390,11 +390,13 @@ def check_status(where: str = "") -> None:
     its operands since the last check: its output is then not to be used.  Synchronises the
     device, so it is called where the host waits anyway (after a step's logits or tokens have
     been read) and every so many decode steps."""
+    from .drafts import draft_status
     from .requests import request_status
     tc = tensor_core_status()
     ix = index_status()
     rq = request_status()
-    if tc or ix or rq:
+    dr = draft_status()
+    if tc or ix or rq or dr:
         what = []
         if tc:
             what.append(f"a tensor-core kernel gave up on a wait (code {tc})")
@@ -402,6 +404,8 @@ def check_status(where: str = "") -> None:
             what.append(f"a kernel met an index outside its operands (code {ix})")
         if rq:
             what.append(f"an adapter, a log of tokens or a mask did not fit its row (code {rq})")
+        if dr:
+            what.append(f"a tree of drafted tokens or a copy of cache rows did not fit its request (code {dr})")
         raise _lib.KernelError((where + ": " if where else "") + "; ".join(what)
                                + "; the results of the steps since the last check are invalid")
 
