@@ -33,14 +33,6 @@ constexpr int kNone = 0x7fffffff;
 __device__ int g_adapter_tc_error = 0;               // code of the first wait that was given up on
 __device__ int g_adapter_tc_index = 0;               // 1 + a row whose adapter lies outside the pool
 
-// One lane of a whole warp, the same one every time.  The warps that issue products run their loops as a whole and elect a lane
-// for each step: behind a condition on the lane number, which the compiler does not know to leave a single thread, a step's four
-// products took 800 cycles however small they were.
-__device__ __forceinline__ bool elect_one() {
-  unsigned is;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
-  return is != 0;
-}
 // A wait of a whole warp: all of its lanes go on, or none does.
 __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile int* stop, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, code, &g_adapter_tc_error));

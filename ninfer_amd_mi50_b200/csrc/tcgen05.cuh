@@ -42,6 +42,14 @@ __device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, volatile i
   atomicCAS(err, 0, code);
   return false;
 }
+// One lane of a whole warp, the same one every time.  The warps that issue products run their loops as a whole and elect a lane
+// for each step: behind a condition on the lane number, which the compiler does not know to leave a single thread, a step's four
+// products took 800 cycles however small they were.
+__device__ __forceinline__ bool elect_one() {
+  unsigned is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
+}
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, void* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"

@@ -144,6 +144,7 @@ template <typename T>
 __global__ void __launch_bounds__(128)
 tree_attention_merge_kernel(TreeArgs a, T* __restrict__ out) {
   const int at = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  chain_wait(a.ws_acc, a.ws_ml, a.lengths, a.row0);
   if (at >= a.T * a.Hq) return;
   const int t = at / a.Hq;
   int lo = 0, hi = a.S;                                      // the last request that begins at or before the row
@@ -154,24 +155,41 @@ tree_attention_merge_kernel(TreeArgs a, T* __restrict__ out) {
   const TreeRequest r = tree_request(a, lo);
   if (t < r.row0 || t >= r.row0 + r.nodes) return;           // a row behind the last request's
   const int shares = (r.keys + a.chunk - 1) / a.chunk;
+  if (shares == 1 && a.whole_written) return;
   const size_t step = (size_t)a.T * a.Hq;
-  float m = -INFINITY, l = 0.f;
-  for (int c = lane; c < shares; c += 32) {
-    const float2 ml = reinterpret_cast<const float2*>(a.ws_ml)[c * step + at];
-    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top;
-    l = l * exp2f(m - base) + ml.y * exp2f(ml.x - base);
-    m = top;
-  }
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + at;
+  float m = -INFINITY;
+  for (int c = lane; c < shares; c += 32) m = fmaxf(m, ml[c * step].x);
   const float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
-  l = warp_sum(l * exp2f(m - base));
-  for (int d = lane; d < a.D; d += 32) {
-    float sum = 0.f;
-    for (int c = 0; c < shares; ++c) {
-      const float w = exp2f(a.ws_ml[2 * (c * step + at)] - base);
-      sum += w ? w * a.ws_acc[(c * step + at) * a.D + d] : 0.f;
+  float l = 0.f, sum[8] = {};
+  for (int c0 = 0; c0 < shares; c0 += 32) {
+    float w = 0.f;                                           // of share c0 + lane
+    if (c0 + lane < shares) {
+      const float2 v = ml[(c0 + lane) * step];
+      w = exp2f(v.x - base);
+      l += w * v.y;
     }
-    out[(size_t)at * a.D + d] = from_float<T>(l > 0.f ? sum / l : (l == 0.f ? 0.f : l));
+    const int n = min(32, shares - c0);
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+      const float wc = __shfl_sync(0xffffffffu, w, c);
+      const float* acc = a.ws_acc + ((c0 + c) * step + at) * a.D;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (128 * i + 4 * lane < a.D) {
+          const float4 v = *reinterpret_cast<const float4*>(acc + 128 * i + 4 * lane);
+          if (wc) sum[4 * i] += wc * v.x, sum[4 * i + 1] += wc * v.y, sum[4 * i + 2] += wc * v.z, sum[4 * i + 3] += wc * v.w;
+        }
+    }
   }
+  l = warp_sum(l);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int d = 128 * i + 4 * lane + k;
+      if (d < a.D) out[(size_t)at * a.D + d] = from_float<T>(l > 0.f ? sum[4 * i + k] / l : (l == 0.f ? 0.f : l));
+    }
 }
 
 template <typename T, int NC>
@@ -182,9 +200,13 @@ int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out
   const dim3 grid(a.shares, a.S * a.Hkv, (pairs + kTreeRows - 1) / kTreeRows);
   NF_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
   tree_attention_rows_kernel<T, NC><<<grid, kThreads, smem, stream>>>(a, (const T*)qkv, (const T*)pages, (T*)out);
-  if (int rc = check_launch("tree_attention_rows")) return rc;
+  return check_launch("tree_attention_rows");
+}
+
+template <typename T>
+int launch_merge(const TreeArgs& a, void* out, cudaStream_t stream) {
   if (a.shares == 1) return 0;
-  tree_attention_merge_kernel<T><<<(a.T * a.Hq + 3) / 4, 128, 0, stream>>>(a, (T*)out);
+  launch_chained(tree_attention_merge_kernel<T>, dim3((a.T * a.Hq + 3) / 4), dim3(128), 0, stream, a, (T*)out);
   return check_launch("tree_attention_merge");
 }
 
@@ -200,8 +222,15 @@ int launch_rows_of(const TreeArgs& a, const void* qkv, const void* pages, void* 
 
 using namespace nf;
 
+// Whether the tensor-core form takes these sizes: bfloat16, heads of 64 or 128, whole pages a block of 128 keys, queries on
+// 16-byte boundaries.
+extern "C" int nf_tree_attention_tensor(int dtype, int Hkv, int D, int page_size, long long num_pages, const void* qkv, long long q_stride) {
+  return dtype == kBF16 && tree_tc_fits(D, page_size, num_pages * 2 * Hkv * page_size) && (uintptr_t)qkv % 16 == 0 && q_stride % 8 == 0;
+}
+
 // Keys a share takes, for calls of these sizes; the workspace is a float for every (share, row, query head, D + 2).
-extern "C" int nf_tree_attention_chunk(int S, int T, int Hq, int Hkv, int words, int max_context) {
+extern "C" int nf_tree_attention_chunk(int S, int T, int Hq, int Hkv, int words, int max_context, int tensor) {
+  if (tensor) return tree_tc_chunk(S, T, Hq, Hkv, words, max_context);
   // shares enough that a few hundred CTAs are under way, of 64 keys at least
   const long long pairs = std::min(32ll * words, (long long)T) * (Hq / Hkv);
   const long long ctas = (long long)S * Hkv * ((pairs + kTreeRows - 1) / kTreeRows);
@@ -216,8 +245,8 @@ extern "C" int nf_tree_attention_chunk(int S, int T, int Hq, int Hkv, int words,
 // where one share takes all keys.
 extern "C" int nf_tree_attention(const void* qkv, long long q_stride, const void* pages, const int* block_table, int bt_width,
                                  const int* lengths, const int* row0, const int* mask, int words, void* out, float* ws, int S, int T,
-                                 int Hq, int Hkv, int D, int page_size, int num_pages, int max_context, int chunk, float scale, int dtype,
-                                 cudaStream_t stream) {
+                                 int Hq, int Hkv, int D, int page_size, int num_pages, int max_context, int chunk, int tensor, float scale,
+                                 int dtype, cudaStream_t stream) {
   if (S == 0 || T == 0) return 0;
   NF_REQUIRE(S > 0 && T > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && D > 0 && D % 16 == 0 && D <= 256 && page_size > 0 && num_pages > 0 &&
                  bt_width > 0 && words > 0 && max_context > 0 && chunk > 0 && q_stride >= (long long)Hq * D && (long long)T * Hq < (1ll << 31),
@@ -228,8 +257,15 @@ extern "C" int nf_tree_attention(const void* qkv, long long q_stride, const void
   NF_REQUIRE(shares == 1 || ws, "tree attention: %d shares of keys want a workspace", shares);
   float* ws_ml = ws ? ws + (size_t)shares * T * Hq * D : nullptr;
   TreeArgs a = {block_table, lengths, row0, mask, ws, ws_ml, q_stride, bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context,
-                chunk, shares, scale};
-  return dtype == kF32 ? launch_rows_of<float>(a, qkv, pages, out, stream) : launch_rows_of<__nv_bfloat16>(a, qkv, pages, out, stream);
+                chunk, shares, tensor, scale};
+  if (tensor) {
+    NF_REQUIRE(nf_tree_attention_tensor(dtype, Hkv, D, page_size, num_pages, qkv, q_stride) && chunk % 128 == 0 && (uintptr_t)out % 16 == 0,
+               "tree attention: sizes the tensor-core form does not take (D=%d page=%d)", D, page_size);
+    if (int rc = launch_tree_tc(a, qkv, pages, out, stream)) return rc;
+  } else if (int rc = dtype == kF32 ? launch_rows_of<float>(a, qkv, pages, out, stream) : launch_rows_of<__nv_bfloat16>(a, qkv, pages, out, stream)) {
+    return rc;
+  }
+  return dtype == kF32 ? launch_merge<float>(a, out, stream) : launch_merge<__nv_bfloat16>(a, out, stream);
 }
 
 // 0, or 1 + a request of which lengths, rows or pages did not fit a call since the last time.  Synchronises.

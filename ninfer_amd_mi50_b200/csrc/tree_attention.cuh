@@ -15,6 +15,7 @@ struct TreeArgs {
   float *ws_acc, *ws_ml;          // [shares][T][Hq][D], [shares][T][Hq][2]
   long long q_stride;
   int bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context, chunk, shares;
+  int whole_written;              // a request with one share has its result from the first kernel
   float scale;
 };
 
@@ -40,6 +41,11 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, const TreeRequest& 
   const int k = j - r.len;
   return k < 0 || (a.mask[(size_t)(r.row0 + i) * a.words + (k >> 5)] >> (k & 31) & 1);
 }
+
+// The tensor-core form (tree_attention_tc.cu).
+bool tree_tc_fits(int D, int page_size, long long page_rows);
+int tree_tc_chunk(int S, int T, int Hq, int Hkv, int words, int max_context);
+int launch_tree_tc(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream);
 
 // Lets a kernel have `bytes` of dynamic shared memory on the current device.
 inline int allow_smem(const void* kernel, size_t bytes) {

@@ -1,0 +1,582 @@
+// Attention of trees of drafted tokens in bfloat16 on the 5th-generation tensor cores (tree_attention.cu says what is
+// computed).  All (node, query head) pairs of a key head read the same keys, so they are the rows of one product, 128 a
+// tile.  A CTA a SM walks its share of the items (request, key head, share of the keys, two tiles of pairs); the copies for
+// an item are on their way while the one before it is worked off.
+//
+//   warps 0, 2   producers of keys and of values: TMA copies (128-byte swizzle), page by page through the block table, in
+//                blocks of 128 keys, into rings
+//   warps 1, 3   issuers of ``tcgen05.mma``, one a softmax group: S = Q K^T (128 x 128) and O += P V, with P out of tensor memory
+//   warps 4-7 and 8-11   two softmax groups, a thread a row: the queries of the item to come, then a reference maximum that is raised only when a score passes it
+//                by 2^8 (O's row is then rescaled), weights 2^(s - m) rounded to bfloat16 in the place of the scores
+//
+// Each group has an S and an O of its own in tensor memory (128 columns each, all 512).  With two tiles of pairs a group
+// takes one of them and both read each block of keys; with one tile they take every other block, and their sums are put
+// together at the end.  Either way one group's exponentials run under the other's products.  A group's products are issued
+// by one thread and run in that order, so the scores of a step are there only when the sums of the step before are, and P,
+// which lies where S did, and O need no signs of their own.  (With one issuer for both groups its waits, 150 cycles each
+// even where there is nothing to wait for, lay between the products.)
+//
+// Only blocks that reach behind the keys that the request held are masked: there a thread shifts its row's mask so that bit
+// i says whether its i-th score counts.  Keys behind the last node are masked and their values set to zero, since whatever
+// a page holds there would be multiplied by a weight of nothing.
+//
+// The weights are rounded to bfloat16 for the second product (an error of 2^-9 of a weight at most, as independent from
+// key to key as the rounding of the result); their sum is of the unrounded ones.  Scores, maxima, sums and O are float32.
+//
+// Every wait is bounded: the one that runs out records a code in `g_tree_tc_error` and sets `stop`, upon which the other
+// waits run out too, the CTA's warps leave, wait (bounded) for copies in flight, and free tensor memory.
+#include "tcgen05.cuh"
+#include "tree_attention.cuh"
+
+namespace nf {
+namespace {
+
+constexpr int kRows = 128;       // pairs of a CTA (MMA M)
+constexpr int kKeys = 128;       // keys per block
+constexpr int kThreads = 384;
+constexpr int kMostRequests = 1024;   // of a launch: their numbers lie in shared memory
+constexpr int kAtom = 128 * 128; // bytes of a swizzle atom column: 128 rows x 64 bf16
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.f;
+
+__device__ int g_tree_tc_error = 0;
+__device__ int g_tree_tc_index = 0;
+
+struct __align__(8) Barriers {
+  unsigned long long q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], o_final[2], o_read;
+  unsigned tmem_base;
+  int stop, quit[2];
+};
+
+struct Requests {
+  int upto[kMostRequests + 1];      // items of the requests before
+  int row0[kMostRequests], nodes[kMostRequests], len[kMostRequests], keys[kMostRequests];
+};
+
+// Descriptor of an MN-major operand with 128-byte swizzle: 64 contiguous MN elements a row, rows = k, the next 64 MN
+// elements `lbo` bytes further.
+__device__ __forceinline__ unsigned long long smem_desc_mn(const void* p, unsigned lbo) {
+  unsigned long long d = 0;
+  d |= (unsigned long long)((smem_u32(p) & 0x3FFFFu) >> 4);
+  d |= (unsigned long long)(lbo >> 4) << 16;
+  d |= (unsigned long long)(1024 >> 4) << 32;
+  d |= (unsigned long long)1 << 46;
+  d |= (unsigned long long)2 << 61;
+  return d;
+}
+// bf16 x bf16 -> f32, M = 128, N = n; b_mn: the B operand is MN-major.
+__device__ __forceinline__ unsigned mma_desc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(kRows >> 4) << 24);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z));
+  return v;
+}
+
+// Two float32 in one register pair, which this architecture multiplies and adds at once.
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ void halves(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
+  unsigned long long v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+  return v;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long x, unsigned long long y) {
+  unsigned long long v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+  return v;
+}
+
+// Scores that are not seen become -inf: their weight is exactly zero.
+__device__ __forceinline__ void hide(unsigned* u, unsigned seen) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!(seen >> i & 1)) u[i] = 0xff800000u;
+}
+
+// A bounded wait of a whole warp: all its lanes go on, or none.
+__device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile int* stop, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, code, &g_tree_tc_error));
+}
+
+// What a CTA works on at a time: share `share` of the keys of (request s, key head g), and `tiles` (1 or 2) tiles of pairs.
+struct Item {
+  int s, g, share, shares, pair0, pairs, tiles, first, last, blocks, row0, len, keys;
+  __device__ __forceinline__ int steps(int group) const { return tiles == 2 ? blocks : (blocks + 1 - group) >> 1; }
+  __device__ __forceinline__ int block(int group, int step) const { return tiles == 2 ? step : 2 * step + group; }
+};
+// Item `at`, which is in request s or a later one; false behind the last.
+__device__ __forceinline__ bool find_item(const TreeArgs& a, const Requests& q, int at, Item& t) {
+  if (at >= q.upto[a.S]) return false;
+  while (at >= q.upto[t.s + 1]) ++t.s;
+  const int G = a.Hq / a.Hkv, local = at - q.upto[t.s];
+  t.row0 = q.row0[t.s], t.len = q.len[t.s], t.keys = q.keys[t.s];
+  t.pairs = q.nodes[t.s] * G;
+  t.shares = (t.keys + a.chunk - 1) / a.chunk;
+  const int twos = (t.pairs + 2 * kRows - 1) / (2 * kRows);
+  t.pair0 = local % twos * 2 * kRows;
+  t.tiles = t.pairs - t.pair0 > kRows ? 2 : 1;
+  t.share = local / twos % t.shares;
+  t.g = local / twos / t.shares;
+  t.first = t.share * a.chunk;
+  t.last = min(t.first + a.chunk, t.keys);
+  t.blocks = (t.last - t.first + kKeys - 1) / kKeys;
+  return true;
+}
+
+// Bits of the 64 keys from `key0` on that row `row` of the request sees.
+__device__ __forceinline__ unsigned long long seen64(const TreeArgs& a, const Item& t, int row, int key0) {
+  const int k0 = key0 - t.len, left = t.keys - key0;
+  if (left <= 0) return 0ull;
+  const unsigned long long real = left >= 64 ? ~0ull : (1ull << left) - 1;
+  if (k0 <= -64) return real;
+  const int* m = a.mask + (size_t)row * a.words;
+  auto word = [&](int w) { return w < a.words ? (unsigned long long)(unsigned)m[w] : 0ull; };
+  unsigned long long v;
+  if (k0 < 0) v = ((word(0) | word(1) << 32) << -k0) | ((1ull << -k0) - 1);
+  else {
+    const int w = k0 >> 5, sh = k0 & 31;
+    v = (word(w) | word(w + 1) << 32) >> sh;
+    if (sh) v |= word(w + 2) << (64 - sh);
+  }
+  return v & real;
+}
+
+__device__ __forceinline__ void tc_st16(unsigned taddr, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ TreeArgs a, const __nv_bfloat16* __restrict__ qkv,
+                         __nv_bfloat16* __restrict__ out) {
+  constexpr int ATOMS = D / 64, KB = ATOMS * kAtom;          // bytes of a tile of queries, and of a block of keys or values
+  constexpr int STAGES = D == 64 ? 4 : 2;
+  constexpr int PIECES = D / 8;                              // 16-byte pieces of a query
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* Qs = smem;                                  // [2 tiles]
+  unsigned char* KV = Qs + 2 * KB;                           // [stages][keys, values]
+  Barriers* bars = reinterpret_cast<Barriers*>(KV + 2 * STAGES * KB);
+  float2* s_stat = reinterpret_cast<float2*>(bars + 1);      // [2 item parities][2 groups][128 rows] (maximum, sum)
+  Requests& reqs = *reinterpret_cast<Requests*>(s_stat + 4 * kRows);
+  volatile int* stop = &bars->stop;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.Hq / a.Hkv;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 8);
+    mbar_init(&bars->q_empty, 2);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&bars->k_full[i], 1);
+      mbar_init(&bars->k_empty[i], 2);
+      mbar_init(&bars->v_full[i], 1);
+      mbar_init(&bars->v_empty[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->o_final[i], 1);
+    }
+    mbar_init(&bars->o_read, 8);
+    bars->stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  chain_wait(qkv);                       // (barriers and tensor memory are this SM's own; everything below was written by earlier kernels)
+  for (int s = threadIdx.x; s < a.S; s += kThreads) {
+    const TreeRequest r = tree_request(a, s);
+    if (r.bad && blockIdx.x == 0) atomicCAS(&g_tree_tc_index, 0, 1 + s);
+    reqs.row0[s] = r.row0, reqs.nodes[s] = r.nodes, reqs.len[s] = r.len, reqs.keys[s] = r.keys;
+    reqs.upto[s + 1] = (r.nodes * G + 2 * kRows - 1) / (2 * kRows) * ((r.keys + a.chunk - 1) / a.chunk) * a.Hkv;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int sum = 0;
+    if (lane == 0) reqs.upto[0] = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 32) {
+      int v = s0 + lane < a.S ? reqs.upto[s0 + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (s0 + lane < a.S) reqs.upto[s0 + lane + 1] = sum + v;
+      sum += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  __syncthreads();
+  Item t;
+  t.s = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = bars->tmem_base;                     // S of group g at columns 128 g, O at 256 + 128 g
+
+  if (warp < 4) {
+    if (warp == 0 || warp == 2) {
+      // ---- producers -------------------------------------------------------------------------------------------------
+      const int kv = warp >> 1, per = kKeys / a.page_size;                // pages a block spans (at most 8)
+      bool ok = true;
+      int gb = 0, issued = -1;
+      for (int at = blockIdx.x; ok && find_item(a, reqs, at, t); at += gridDim.x) {
+        const int* bt = a.block_table + (size_t)t.s * a.bt_width;
+        for (int blk = 0; blk < t.blocks; ++blk, ++gb) {
+          const int st = gb % STAGES;
+          // lane i looks up the block's i-th page
+          const int j = t.first + blk * kKeys + lane * a.page_size;
+          int page = -1;
+          if (lane < per && j < t.last) {
+            const int lp = j / a.page_size;
+            page = lp < a.bt_width ? bt[lp] : -1;
+            if (page < 0 || page >= a.num_pages) {
+              page = -1;
+              atomicCAS(&g_tree_tc_index, 0, 1 + t.s);
+            }
+          }
+          const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+          unsigned char* to = KV + (2 * st + kv) * KB;
+          void* full = kv ? &bars->v_full[st] : &bars->k_full[st];
+          void* empty = kv ? &bars->v_empty[st] : &bars->k_empty[st];
+          if (!warp_wait(empty, ((gb / STAGES) & 1) ^ 1, stop, 2)) { ok = false; break; }
+          if (elect_one()) mbar_expect_tx(full, (unsigned)__popc(there) * a.page_size * D * 2);
+          __syncwarp();
+          for (int i = 0; i < per; ++i) {
+            const int y = ((__shfl_sync(0xffffffffu, page, i) * 2 + kv) * a.Hkv + t.g) * a.page_size;
+            if ((there >> i & 1) && elect_one())
+              for (int x = 0; x < ATOMS; ++x) tma_load_2d(to + x * kAtom + i * a.page_size * 128, &map_kv, 64 * x, y, full);
+          }
+          issued = gb;
+        }
+      }
+      if (!ok && lane == 0)                                  // copies asked for still land in this CTA's shared memory
+        for (int b = max(0, issued - STAGES + 1); b <= issued; ++b) {
+          void* full = kv ? &bars->v_full[b % STAGES] : &bars->k_full[b % STAGES];
+          for (unsigned i = 0; i < (1u << 20); ++i)
+            if (mbar_try(full, (b / STAGES) & 1)) break;
+        }
+    } else {
+      // ---- products of a group ---------------------------------------------------------------------------------------------
+      const unsigned desc_qk = mma_desc(kKeys, false), desc_pv = mma_desc(D, true);
+      const int group = warp >> 1;
+      const unsigned tmem_s = tmem + group * kKeys, tmem_o = tmem + (2 + group) * kKeys;
+      int gb = 0, gi = 0, done = 0;                          // blocks and items before this one, steps of the group
+      bool ok = true;
+      for (int at = blockIdx.x; ok && find_item(a, reqs, at, t); at += gridDim.x, ++gi) {
+        const int n = t.steps(group);
+        const bool alone = t.tiles == 1;                     // a block is one group's: its stage has both groups' signs from this one
+        auto scores = [&](int step) -> bool {
+          const int b = gb + t.block(group, step), st = b % STAGES;
+          if (!warp_wait(&bars->k_full[st], (b / STAGES) & 1, stop, 4)) return false;
+          tc_fence_after();
+          const unsigned long long dq = smem_desc(Qs + (alone ? 0 : group * KB)), dk = smem_desc(KV + 2 * st * KB);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {            // (an atom on: 16,384 bytes, of which a descriptor counts sixteenths)
+              const int off = (kk >> 2) * (kAtom / 16) + 2 * (kk & 3);
+              tc_mma(tmem_s, dq + off, dk + off, desc_qk, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&bars->s_full[group]);
+            tc_commit(&bars->k_empty[st]);
+            if (alone) tc_commit(&bars->k_empty[st]);
+            if (step == n - 1) tc_commit(&bars->q_empty);
+          }
+          __syncwarp();
+          return true;
+        };
+        if (!warp_wait(&bars->q_full, gi & 1, stop, 3)) { ok = false; break; }
+        if (n > 0) {
+          ok = scores(0);
+        } else {                                             // (o_final says what it says of the item before until that has been read)
+          ok = gi == 0 || warp_wait(&bars->o_read, (gi - 1) & 1, stop, 7);
+          if (elect_one()) tc_commit(&bars->q_empty), tc_commit(&bars->o_final[group]);
+          __syncwarp();
+        }
+        for (int step = 0; ok && step < n; ++step) {
+          const int b = gb + t.block(group, step), st = b % STAGES;
+          // (o_read comes first: it says that all values of the item before have been added up.  A stage that the other group used
+          // last might else be waited for two fills ahead, where a parity says nothing)
+          ok = (step > 0 || gi == 0 || warp_wait(&bars->o_read, (gi - 1) & 1, stop, 7)) && warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 5) &&
+               warp_wait(&bars->p_full[group], (done + step) & 1, stop, 6);
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned long long dv = smem_desc_mn(KV + (2 * st + 1) * KB, kAtom);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)          // (16 keys on: 2,048 bytes)
+              tc_mma_ts(tmem_o, tmem_s + 8 * kk, dv + 128 * kk, desc_pv, (step > 0 || kk > 0) ? 1u : 0u);
+            tc_commit(&bars->v_empty[st]);
+            if (alone) tc_commit(&bars->v_empty[st]);
+            if (step == n - 1) tc_commit(&bars->o_final[group]);
+          }
+          __syncwarp();
+          if (step + 1 < n) ok = scores(step + 1);
+        }
+        gb += t.blocks, done += n;
+      }
+    }
+  } else {
+    // ---- softmax -----------------------------------------------------------------------------------------------------------
+    const int group = (warp >> 2) - 1, quad = warp & 3, row = quad * 32 + lane;
+    const unsigned lane_addr = (unsigned)(quad * 32) << 16;
+    const unsigned tmem_s = tmem + lane_addr + group * kKeys, tmem_o = tmem + lane_addr + (2 + group) * kKeys;
+    const float sc2 = a.scale * kLog2e;
+    int gb = 0, gi = 0, done = 0;
+    // An item's queries as the swizzled image has them: with two tiles a thread its row, with one half a row
+    auto load_queries = [&](const Item& t) {
+      const bool two = t.tiles == 2;
+      const int p = t.pair0 + (two ? group * kRows : 0) + row, n = two ? PIECES : PIECES / 2, c0 = two ? 0 : group * n;
+      unsigned char* to = Qs + (two ? group * KB : 0) + row * 128;
+      const bool real = p < t.pairs;
+      const uint4* q = reinterpret_cast<const uint4*>(qkv + (size_t)(real ? t.row0 + p / G : 0) * a.q_stride + (size_t)(t.g * G + p % G) * D);
+#pragma unroll 1
+      for (int h = 0; h < n; h += PIECES / 2) {
+        uint4 v[PIECES / 2];
+#pragma unroll
+        for (int i = 0; i < PIECES / 2; ++i) v[i] = real ? q[c0 + h + i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < PIECES / 2; ++i) {
+          const int c = c0 + h + i;
+          *reinterpret_cast<uint4*>(to + (c >> 3) * kAtom + (((c & 7) ^ (row & 7)) << 4)) = v[i];
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full);
+    };
+    Item next = t;
+    bool more = find_item(a, reqs, blockIdx.x, next);
+    if (more) load_queries(next);
+    for (int at = blockIdx.x; more; at += gridDim.x, ++gi) {
+      t = next;
+      const int tile0 = t.pair0 + (t.tiles == 2 ? group * kRows : 0), p = tile0 + row;
+      const bool real = p < t.pairs, idle = tile0 + quad * 32 >= t.pairs;      // idle: none of the warp's rows is anybody's
+      const int node = real ? t.row0 + p / G : 0, head = t.g * G + p % G, n = t.steps(group);
+      float m_ref = 0.f, l_run = 0.f;
+      bool have = false, ok = true;
+      for (int step = 0; ok && step < n; ++step, ++done) {
+        const int blk = t.block(group, step), kb = t.first + blk * kKeys;
+        if (!warp_wait(&bars->s_full[group], done & 1, stop, 8)) { ok = false; break; }
+        tc_fence_after();
+        if (!idle) {
+          // Twice through the scores, 32 at a time: for the maximum, and for the weights
+          const bool masked = kb + kKeys > t.len;            // (else keys that every row sees)
+          unsigned long long seen[2] = {~0ull, ~0ull};
+          if (masked)
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) (h ? seen[1] : seen[0]) = real ? seen64(a, t, node, kb + 64 * h) : 0ull;
+          auto part = [&](int c) { return (unsigned)((c & 2 ? seen[1] : seen[0]) >> (32 * (c & 1))); };
+          unsigned u[2][32];
+          tc_ld32(tmem_s, u[0]);
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c0 = 0; c0 < 4; c0 += 2)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              tc_wait_ld();
+              tc_ld32(tmem_s + 32 * ((c0 + k + 1) & 3), u[k ^ 1]);           // (at the end the first ones again)
+              if (masked) hide(u[k], part(c0 + k));
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(u[k][i]), __uint_as_float(u[k][i + 1]));
+            }
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc2;
+          float alpha = 1.f;
+          bool raise = false;
+          if (!have) {
+            have = mx != -INFINITY;
+            m_ref = have ? mx : 0.f;
+          } else if (mx > m_ref + kRaise) {
+            raise = true;
+            alpha = exp2f(m_ref - mx);
+            m_ref = mx;
+          }
+          const unsigned long long sc = pair_of(sc2, sc2), low = pair_of(-m_ref, -m_ref);
+          unsigned long long sum[2] = {0ull, 0ull};          // (two pairs of 0.f)
+#pragma unroll 1
+          for (int c0 = 0; c0 < 4; c0 += 2)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              tc_wait_ld();
+              if (c0 + k < 3) tc_ld32(tmem_s + 32 * (c0 + k + 1), u[k ^ 1]);
+              if (masked) hide(u[k], part(c0 + k));
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float x, y;
+                halves(fma2(pair_of(__uint_as_float(u[k][2 * i]), __uint_as_float(u[k][2 * i + 1])), sc, low), x, y);
+                x = ex2(x), y = ex2(y);
+                sum[i & 1] = add2(sum[i & 1], pair_of(x, y));
+                const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+                u[k][i] = *reinterpret_cast<const unsigned*>(&v);
+              }
+              tc_st16(tmem_s + 16 * (c0 + k), u[k]);         // (over scores that have been read for good)
+            }
+          float s0, s1;
+          halves(add2(sum[0], sum[1]), s0, s1);
+          l_run = fmaf(l_run, alpha, s0 + s1);
+          if (__any_sync(0xffffffffu, raise)) {              // (the product of the step before has run: its scores came first)
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              unsigned o[32];
+              tc_ld32(tmem_o + 32 * c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tc_st32(tmem_o + 32 * c, o);
+            }
+          }
+          tc_wait_st();
+        }
+        if (t.last - kb < kKeys) {                           // the request's last block: nothing behind its last key (both groups say so)
+          const int b = gb + blk, st = b % STAGES;
+          if (!warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 9)) { ok = false; break; }
+          unsigned char* v = KV + (2 * st + 1) * KB;
+          for (int i = (t.last - kb) * 8 + row; i < kKeys * 8; i += 128)
+#pragma unroll
+            for (int x = 0; x < ATOMS; ++x) reinterpret_cast<uint4*>(v + x * kAtom)[i] = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[group]);
+      }
+      // the next item's queries, once this one's last scores are there: on their way while its last values are added up
+      more = find_item(a, reqs, at + gridDim.x, next);
+      if (more && ok) {
+        ok = warp_wait(&bars->q_empty, gi & 1, stop, 1);
+        if (ok) load_queries(next);
+      }
+      // ---- the item's rows -----------------------------------------------------------------------------------------------
+      float2* stat = s_stat + (gi & 1) * 2 * kRows;
+      stat[group * kRows + row] = make_float2(have ? m_ref : -INFINITY, l_run);
+      // whether all leave is one thread's word, so that none waits at this barrier alone
+      if (threadIdx.x == 128) bars->quit[gi & 1] = *stop;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (((volatile int*)bars->quit)[gi & 1]) break;
+      ok = ok && warp_wait(&bars->o_final[0], gi & 1, stop, 10) && warp_wait(&bars->o_final[1], gi & 1, stop, 10);
+      tc_fence_after();
+      if (ok && !idle) {
+        // two tiles: each group its own O; one: both groups' O, half of the columns each
+        const bool two = t.tiles == 2, other = !two && t.steps(1) > 0;
+        const float2 mine = stat[(two ? group : 0) * kRows + row], further = other ? stat[kRows + row] : make_float2(-INFINITY, 0.f);
+        const float top = fmaxf(mine.x, further.x), base = top == -INFINITY ? 0.f : top;
+        float w0 = exp2f(mine.x - base), w1 = exp2f(further.x - base);
+        const float l = mine.y * w0 + further.y * w1, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const size_t place = (size_t)node * a.Hq + head, ws = (size_t)t.share * a.T * a.Hq + place;
+        const bool whole = t.shares == 1;
+        if (whole) w0 *= inv, w1 *= inv;
+        const unsigned o0 = tmem + lane_addr + (2 + (two ? group : 0)) * kKeys, o1 = tmem + lane_addr + 3 * kKeys;
+        const int c0 = two ? 0 : group * (D / 2), cn = two ? D : c0 + D / 2;
+#pragma unroll 1
+        for (int c = c0; c < cn; c += 32) {
+          unsigned o[32], x[32];
+          tc_ld32(o0 + c, o);
+          if (other) tc_ld32(o1 + c, x);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float v = __uint_as_float(o[i]) * w0;
+            if (other) v = fmaf(__uint_as_float(x[i]), w1, v);
+            o[i] = __float_as_uint(v);
+          }
+          if (!real) continue;
+          if (!whole) {
+            uint4* to = reinterpret_cast<uint4*>(a.ws_acc + ws * D + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+            uint4* to = reinterpret_cast<uint4*>(out + place * D + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              unsigned w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(o[8 * i + 2 * k]), __uint_as_float(o[8 * i + 2 * k + 1]));
+                w[k] = *reinterpret_cast<const unsigned*>(&v);
+              }
+              to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (real && !whole && (two || group == 0)) reinterpret_cast<float2*>(a.ws_ml)[ws] = make_float2(top, l);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->o_read);
+      gb += t.blocks;
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+template <int D>
+int launch_tc(const CUtensorMap& map, TreeArgs a, const void* qkv, void* out, cudaStream_t stream) {
+  const size_t smem = 1024 + (size_t)(2 + 2 * (D == 64 ? 4 : 2)) * (D / 64) * kAtom + sizeof(Barriers) + 4 * kRows * sizeof(float2) + sizeof(Requests);
+  static_assert(sizeof(Barriers) % 8 == 0, "float2 follow");
+  if (int rc = allow_smem((const void*)tree_attention_tc_kernel<D>, smem)) return rc;
+  const long long twos = (std::min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv) + 2 * kRows - 1) / (2 * kRows);
+  const int S = a.S;
+  for (int s0 = 0; s0 < S; s0 += kMostRequests) {
+    a.S = std::min(kMostRequests, S - s0);
+    const long long items = twos * a.shares * a.Hkv * a.S;
+    NF_REQUIRE(items < (1ll << 31), "tree attention: %lld shares of work are too many", items);
+    launch_chained(tree_attention_tc_kernel<D>, dim3((unsigned)std::min(items, 148ll)), dim3(kThreads), smem, stream, map, a, (const __nv_bfloat16*)qkv,
+                   (__nv_bfloat16*)out);
+    if (int rc = check_launch("tree_attention_tc")) return rc;
+    a.lengths += a.S, a.row0 += a.S, a.block_table += (size_t)a.S * a.bt_width;
+  }
+  return 0;
+}
+
+}  // namespace
+
+bool tree_tc_fits(int D, int page_size, long long page_rows) {
+  return (D == 64 || D == 128) && (page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && page_rows < (1ll << 31);
+}
+
+int tree_tc_chunk(int S, int T, int Hq, int Hkv, int words, int max_context) {
+  const long long twos = (std::min(32ll * words, (long long)T) * (Hq / Hkv) + 2 * kRows - 1) / (2 * kRows), items = twos * S * Hkv;
+  const long long shares = std::max(1ll, (148 * 3 + items - 1) / items);
+  const long long chunk = ((max_context + shares - 1) / shares + kKeys - 1) / kKeys * kKeys;
+  return (int)std::max(256ll, chunk);
+}
+
+int launch_tree_tc(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
+  CUtensorMap map;
+  if (int rc = make_map(&map, pages, (long long)a.num_pages * 2 * a.Hkv * a.page_size, a.D, a.page_size)) return rc;
+  return a.D == 64 ? launch_tc<64>(map, a, qkv, out, stream) : launch_tc<128>(map, a, qkv, out, stream);
+}
+
+}  // namespace nf
+
+using namespace nf;
+
+// 0, or the code of the first wait that ran out since the last time (2 producers, 3-7 issuer, 8-11 softmax), or 100 + a
+// request (from 1 on) whose lengths, rows or pages did not fit.  Synchronises.
+extern "C" int nf_tree_attention_tc_status() {
+  int v = 0, w = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tree_tc_error, sizeof(int)) != cudaSuccess) return -1;
+  if (cudaMemcpyFromSymbol(&w, g_tree_tc_index, sizeof(int)) != cudaSuccess) return -1;
+  if (v) cudaMemcpyToSymbol(g_tree_tc_error, &zero, sizeof(int));
+  if (w) cudaMemcpyToSymbol(g_tree_tc_index, &zero, sizeof(int));
+  return v ? v : (w ? 100 + w : 0);
+}

@@ -11,12 +11,13 @@ one that rotates by the depth and appends nothing).  Everything is on the device
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
 
 from . import lib as _lib
-from .ops import _DT, _chk, _dt, check_head_dim
+from .ops import TUNING, _DT, _chk, _dt, check_head_dim
 
 __all__ = ["MAX_TREE_NODES", "MAX_VERIFY_NODES", "compact_cache", "copy_pages", "draft_status", "tree_attention", "verify_drafts"]
 
@@ -26,8 +27,9 @@ MAX_TREE_CONTEXT = 1 << 30
 
 _I, _L, _P, _F = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_float
 _SIGNATURES = {
-    "nf_tree_attention_chunk": [_I] * 6,
-    "nf_tree_attention": [_P, _L, _P, _P, _I] + [_P] * 3 + [_I] + [_P] * 2 + [_I] * 9 + [_F, _I, _P],
+    "nf_tree_attention_tensor": [_I] * 4 + [_L, _P, _L],
+    "nf_tree_attention_chunk": [_I] * 7,
+    "nf_tree_attention": [_P, _L, _P, _P, _I] + [_P] * 3 + [_I] + [_P] * 2 + [_I] * 10 + [_F, _I, _P],
     "nf_verify_drafts": [_P, _L, _P, _L] + [_P] * 7 + [_I] * 4 + [_P],
     "nf_compact_cache": [_P, _L] + [_I] * 5 + [_P, _I] + [_P] * 3 + [_I] * 2 + [_P],
     "nf_copy_pages": [_P, _L] + [_I] * 5 + [_P] * 3 + [_I, _P],
@@ -74,7 +76,7 @@ def _same_memory(s: torch.Tensor, t: torch.Tensor) -> bool:
     return s.numel() > 0 and t.numel() > 0 and a < d and c < b
 
 
-def _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, out) -> None:
+def _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale, out) -> None:
     """Says what is wrong with the operands of tree_attention."""
     what = "tree_attention"
     _chk(qkv, "qkv", contiguous=False)
@@ -96,6 +98,8 @@ def _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, 
                          f"are not of one number of requests (row0: one more)")
     if mask.dim() != 2 or mask.shape[0] != T or not 1 <= mask.shape[1] <= MAX_TREE_NODES // 32:
         raise ValueError(f"{what}: mask is {tuple(mask.shape)}, not [{T}, 1 to {MAX_TREE_NODES // 32}]")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{what}: scale={scale} must be positive")
     if not 1 <= max_context <= MAX_TREE_CONTEXT:
         raise ValueError(f"{what}: max_context={max_context} is not within 1 and {MAX_TREE_CONTEXT}")
     if pages.data_ptr() % 16:
@@ -133,22 +137,25 @@ def tree_attention(qkv: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Te
             and row0.dtype is torch.int32 and mask.dtype is torch.int32 and block_table.get_device() == dev and lengths.get_device() == dev
             and row0.get_device() == dev and mask.get_device() == dev and block_table.is_contiguous() and lengths.is_contiguous()
             and row0.is_contiguous() and mask.is_contiguous() and bs[1] > 0 and lengths.shape == bs[:1] and row0.shape == (bs[0] + 1,)
-            and ms[0] == qs[0] and 1 <= ms[1] <= MAX_TREE_NODES // 32 and 1 <= max_context <= MAX_TREE_CONTEXT
+            and ms[0] == qs[0] and 1 <= ms[1] <= MAX_TREE_NODES // 32 and 1 <= max_context <= MAX_TREE_CONTEXT and 0.0 < scale < math.inf
             and pages.data_ptr() % 16 == 0):
-        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, out)
+        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale, out)
     T, S = qs[0], bs[0]
     if out is None:
         out = qkv.new_empty((T, Hq * D))
     else:
-        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, out)
+        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale, out)
     if T == 0 or S == 0:
         return out
-    chunk = _function("nf_tree_attention_chunk")(S, T, Hq, Hkv, ms[1], max_context)
+    p_q, step = qkv.data_ptr(), qkv.stride(0) if T > 1 else qs[1]
+    tensor = TUNING["tree_attention"] == "auto" and _function("nf_tree_attention_tensor")(_DT[dtype], Hkv, D, page_size, pages.shape[0], p_q, step) \
+        and out.data_ptr() % 16 == 0
+    chunk = _function("nf_tree_attention_chunk")(S, T, Hq, Hkv, ms[1], max_context, tensor)
     shares = -(-max_context // chunk)
     ws = torch.empty(shares * T * Hq * (D + 2), dtype=torch.float32, device=qkv.device) if shares > 1 else None
-    _call("nf_tree_attention", dev, qkv.data_ptr(), qkv.stride(0) if T > 1 else qs[1], pages.data_ptr(), block_table.data_ptr(), bs[1],
+    _call("nf_tree_attention", dev, p_q, step, pages.data_ptr(), block_table.data_ptr(), bs[1],
           lengths.data_ptr(), row0.data_ptr(), mask.data_ptr(), ms[1], out.data_ptr(), None if ws is None else ws.data_ptr(), S, T, Hq, Hkv, D,
-          page_size, pages.shape[0], max_context, chunk, scale, _DT[dtype])
+          page_size, pages.shape[0], max_context, chunk, tensor, scale, _DT[dtype])
     return out
 
 
@@ -273,11 +280,13 @@ def copy_pages(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, rows: 
 def draft_status() -> int:
     """0, or what these kernels met since the last call: 1000001 + a request whose lengths, rows or pages did not fit tree
     attention, 2000001 + one whose tree or probabilities made no sense to verification, 3000001 + a request or an entry whose
-    path or pages did not fit a copy.  Synchronises the device; where none was ever called there is nothing to read."""
+    path or pages did not fit a copy, 4000000 + a code of tree attention on tensor cores (2 to 11: a bounded wait that ran out,
+    101 + a request that did not fit).  Synchronises the device; where none was ever called there is nothing to read."""
     if not _used:
         return 0
     lib = _lib.load()
-    for k, name in enumerate(("nf_tree_attention_status", "nf_verify_drafts_status", "nf_cache_pages_status"), 1):
+    for k, name in enumerate(("nf_tree_attention_status", "nf_verify_drafts_status", "nf_cache_pages_status",
+                              "nf_tree_attention_tc_status"), 1):
         v = int(getattr(lib, name)())
         if v:
             return k * 1000000 + v

@@ -69,6 +69,27 @@ def test_attention(case, dtype):
     kernels.check_status()
 
 
+@pytest.mark.parametrize("heads,most,page_size", [((8, 8, 128), 40, 64), ((8, 8, 64), 40, 16), ((24, 2, 128), 40, 64), ((24, 2, 64), 30, 32), ((5, 1, 128), 64, 128)])
+def test_many_requests_of_many_lengths(heads, most, page_size):
+    """More work than there are SMs: each goes from request to request, with one tile of rows and with two."""
+    for seed in range(3):
+        rnd = random.Random(seed)
+        sizes = [rnd.randint(0 if s else 1, most) for s in range(30)]
+        lengths = [rnd.choice([0, 1, 127, 128, rnd.randint(0, 900), rnd.randint(0, 300)]) for _ in sizes]
+        lengths[5] = 2000
+        c = make_attention(sizes, lengths, heads, page_size, seed=seed, words=2)
+        c["qkv"], c["pages"] = c["qkv"].bfloat16().float(), c["pages"].bfloat16().float()
+        got = attend(c, heads, page_size, torch.bfloat16, 0.1)
+        kernels.check_status()
+        want = attend(c, heads, page_size, torch.float32, 0.1).double()
+        # (against the float32 form, which the plain one was compared with: a weight's rounding and the result's, of values below 6)
+        assert float((got.double() - want).abs().max()) <= 6 * 2.0 ** -8 * 2 + 1e-4
+        for s in rnd.sample(range(30), 4):        # and some requests against the plain form
+            lo, hi = c["row0"][s:s + 2]
+            one, weight, size = plain_attention(c["qkv"][lo:hi], *heads, c["pages"], c["table"][s:s + 1], page_size, [lengths[s]], [0, hi - lo], c["mask"][lo:hi], 0.1)
+            near(got[lo:hi], one, weight, size, c["longest"], torch.bfloat16, heads[2])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("heads,length", [((4, 2, 64), 0), ((8, 1, 128), 37), ((2, 2, 48), 130), ((16, 1, 128), 600)])
 def test_any_mask_and_rows_that_see_nothing(heads, length, dtype):
@@ -168,7 +189,7 @@ def test_refusals_of_attention():
                     (2, 0), (3, 40), (3, 272), (4, args[4][:, :1]), (4, args[4].transpose(2, 3)), (4, args[4].flatten()[1:1 + 16 * 64 * 4].view(1, 2, 2, 16, 64)),
                     (5, args[5].long()), (5, args[5][:0]), (5, args[5][0]), (5, args[5].cpu()), (6, 32), (6, 0), (7, args[7].repeat(2)), (8, args[8][:1]),
                     (8, args[8].float()), (9, args[9][:3]), (9, args[9][:, :0]), (9, torch.zeros(T, 9, dtype=torch.int32, device="cuda")), (9, args[9].flatten()),
-                    (10, 0), (10, 1 << 31)]:
+                    (10, 0), (10, 1 << 31), (11, 0.0), (11, -1.0), (11, math.nan)]:
         with pytest.raises((ValueError, TypeError, kernels.KernelError)):
             kernels.tree_attention(*args[:at], bad, *args[at + 1:])
     for out in (torch.empty(T, 255, device="cuda"), torch.empty(T, 256), torch.empty(T, 256, device="cuda").bfloat16(), args[0][:, :256],
