@@ -5,16 +5,15 @@
 //
 //   warps 0, 2   producers of keys and of values: TMA copies (128-byte swizzle), page by page through the block table, in
 //                blocks of 128 keys, into rings
-//   warps 1, 3   issuers of ``tcgen05.mma``, one a softmax group: S = Q K^T (128 x 128) and O += P V, with P out of tensor memory
+//   warp 1       issuer of ``tcgen05.mma``: S = Q K^T (128 x 128) and O += P V, with P out of tensor memory
 //   warps 4-7 and 8-11   two softmax groups, a thread a row: the queries of the item to come, then a reference maximum that is raised only when a score passes it
 //                by 2^8 (O's row is then rescaled), weights 2^(s - m) rounded to bfloat16 in the place of the scores
 //
 // Each group has an S and an O of its own in tensor memory (128 columns each, all 512).  With two tiles of pairs a group
 // takes one of them and both read each block of keys; with one tile they take every other block, and their sums are put
-// together at the end.  Either way one group's exponentials run under the other's products.  A group's products are issued
-// by one thread and run in that order, so the scores of a step are there only when the sums of the step before are, and P,
-// which lies where S did, and O need no signs of their own.  (With one issuer for both groups its waits, 150 cycles each
-// even where there is nothing to wait for, lay between the products.)
+// together at the end.  Either way one group's exponentials run under the other's products.  The products are issued by
+// one thread and run in its order, PV(A), QK(A), PV(B), QK(B): the scores of a step are there only when the sums of the step
+// before are, and P, which lies where S did, and O need no signs of their own.
 //
 // Only blocks that reach behind the keys that the request held are masked: there a thread shifts its row's mask so that bit
 // i says whether its i-th score counts.  Keys behind the last node are masked and their values set to zero, since whatever
@@ -179,12 +178,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 8);
-    mbar_init(&bars->q_empty, 2);
+    mbar_init(&bars->q_empty, 1);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bars->k_full[i], 1);
-      mbar_init(&bars->k_empty[i], 2);
+      mbar_init(&bars->k_empty[i], 1);
       mbar_init(&bars->v_full[i], 1);
-      mbar_init(&bars->v_empty[i], 2);
+      mbar_init(&bars->v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
@@ -271,64 +270,69 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
           for (unsigned i = 0; i < (1u << 20); ++i)
             if (mbar_try(full, (b / STAGES) & 1)) break;
         }
-    } else {
-      // ---- products of a group ---------------------------------------------------------------------------------------------
+    } else if (warp == 1) {
+      // ---- products --------------------------------------------------------------------------------------------------------
       const unsigned desc_qk = mma_desc(kKeys, false), desc_pv = mma_desc(D, true);
-      const int group = warp >> 1;
-      const unsigned tmem_s = tmem + group * kKeys, tmem_o = tmem + (2 + group) * kKeys;
-      int gb = 0, gi = 0, done = 0;                          // blocks and items before this one, steps of the group
+      int gb = 0, gi = 0, done[2] = {0, 0};                  // blocks and items before this one, steps of each group
       bool ok = true;
       for (int at = blockIdx.x; ok && find_item(a, reqs, at, t); at += gridDim.x, ++gi) {
-        const int n = t.steps(group);
-        const bool alone = t.tiles == 1;                     // a block is one group's: its stage has both groups' signs from this one
-        auto scores = [&](int step) -> bool {
-          const int b = gb + t.block(group, step), st = b % STAGES;
-          if (!warp_wait(&bars->k_full[st], (b / STAGES) & 1, stop, 4)) return false;
+        const bool two = t.tiles == 2;
+        const int n0 = t.steps(0), n1 = t.steps(1);
+        int to_come = n0 + n1;                               // products of queries and keys
+        // S = Q K^T of a group's step, whose keys are there
+        auto scores = [&](int group, int b) {
+          const int st = b % STAGES;
+          const unsigned long long dq = smem_desc(Qs + (two ? group * KB : 0)), dk = smem_desc(KV + 2 * st * KB);
           tc_fence_after();
-          const unsigned long long dq = smem_desc(Qs + (alone ? 0 : group * KB)), dk = smem_desc(KV + 2 * st * KB);
+          --to_come;
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {            // (an atom on: 16,384 bytes, of which a descriptor counts sixteenths)
               const int off = (kk >> 2) * (kAtom / 16) + 2 * (kk & 3);
-              tc_mma(tmem_s, dq + off, dk + off, desc_qk, kk > 0 ? 1u : 0u);
+              tc_mma(tmem + group * kKeys, dq + off, dk + off, desc_qk, kk > 0 ? 1u : 0u);
             }
             tc_commit(&bars->s_full[group]);
-            tc_commit(&bars->k_empty[st]);
-            if (alone) tc_commit(&bars->k_empty[st]);
-            if (step == n - 1) tc_commit(&bars->q_empty);
+            if (!two || group == 1) tc_commit(&bars->k_empty[st]);
+            if (to_come == 0) tc_commit(&bars->q_empty);
           }
           __syncwarp();
-          return true;
         };
-        if (!warp_wait(&bars->q_full, gi & 1, stop, 3)) { ok = false; break; }
-        if (n > 0) {
-          ok = scores(0);
-        } else {                                             // (o_final says what it says of the item before until that has been read)
-          ok = gi == 0 || warp_wait(&bars->o_read, (gi - 1) & 1, stop, 7);
-          if (elect_one()) tc_commit(&bars->q_empty), tc_commit(&bars->o_final[group]);
-          __syncwarp();
-        }
-        for (int step = 0; ok && step < n; ++step) {
-          const int b = gb + t.block(group, step), st = b % STAGES;
-          // (o_read comes first: it says that all values of the item before have been added up.  A stage that the other group used
-          // last might else be waited for two fills ahead, where a parity says nothing)
-          ok = (step > 0 || gi == 0 || warp_wait(&bars->o_read, (gi - 1) & 1, stop, 7)) && warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 5) &&
-               warp_wait(&bars->p_full[group], (done + step) & 1, stop, 6);
-          if (!ok) break;
-          tc_fence_after();
-          const unsigned long long dv = smem_desc_mn(KV + (2 * st + 1) * KB, kAtom);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)          // (16 keys on: 2,048 bytes)
-              tc_mma_ts(tmem_o, tmem_s + 8 * kk, dv + 128 * kk, desc_pv, (step > 0 || kk > 0) ? 1u : 0u);
-            tc_commit(&bars->v_empty[st]);
-            if (alone) tc_commit(&bars->v_empty[st]);
-            if (step == n - 1) tc_commit(&bars->o_final[group]);
+        auto keys_there = [&](int b) { return warp_wait(&bars->k_full[b % STAGES], (b / STAGES) & 1, stop, 4); };
+        ok = warp_wait(&bars->q_full, gi & 1, stop, 3);
+        for (int group = 0; ok && group < 2; ++group)
+          if (group == 0 || n1 > 0) {
+            const int b = gb + t.block(group, 0);
+            ok = keys_there(b);
+            if (ok) scores(group, b);
           }
-          __syncwarp();
-          if (step + 1 < n) ok = scores(step + 1);
-        }
-        gb += t.blocks, done += n;
+        for (int step = 0; ok && step < n0; ++step)
+          for (int group = 0; ok && group < 2; ++group) {
+            const int n = group ? n1 : n0;
+            if (step >= n) continue;
+            const int b = gb + t.block(group, step), st = b % STAGES, b_next = gb + t.block(group, step + 1);
+            // what is there before the weights are is not asked for between the products
+            ok = (step > 0 || gi == 0 || warp_wait(&bars->o_read, (gi - 1) & 1, stop, 7)) && warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 5);
+            const bool early = step + 1 < n && __all_sync(0xffffffffu, mbar_try(&bars->k_full[b_next % STAGES], (b_next / STAGES) & 1));
+            ok = ok && warp_wait(&bars->p_full[group], (done[group] + step) & 1, stop, 6);
+            if (!ok) break;
+            tc_fence_after();
+            const unsigned long long dv = smem_desc_mn(KV + (2 * st + 1) * KB, kAtom);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)        // (16 keys on: 2,048 bytes)
+                tc_mma_ts(tmem + (2 + group) * kKeys, tmem + group * kKeys + 8 * kk, dv + 128 * kk, desc_pv, (step > 0 || kk > 0) ? 1u : 0u);
+              if (!two || group == 1) tc_commit(&bars->v_empty[st]);
+              if (step == n - 1) tc_commit(&bars->o_final[group]);
+            }
+            __syncwarp();
+            if (step + 1 < n) {
+              ok = early || keys_there(b_next);
+              if (ok) scores(group, b_next);
+            }
+          }
+        if (ok && n1 == 0 && elect_one()) tc_commit(&bars->o_final[1]);
+        __syncwarp();
+        gb += t.blocks, done[0] += n0, done[1] += n1;
       }
     }
   } else {
@@ -442,7 +446,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
           }
           tc_wait_st();
         }
-        if (t.last - kb < kKeys) {                           // the request's last block: nothing behind its last key (both groups say so)
+        if (t.last - kb < kKeys && (t.tiles == 1 || group == 0)) {       // the request's last block: nothing behind its last key
           const int b = gb + blk, st = b % STAGES;
           if (!warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 9)) { ok = false; break; }
           unsigned char* v = KV + (2 * st + 1) * KB;
