@@ -139,63 +139,86 @@ tree_attention_rows_kernel(TreeArgs a, const T* __restrict__ qkv, const T* __res
   }
 }
 
-// One warp a (row, query head): its request's shares in ascending order.
-template <typename T>
+// Adds up a row's shares in ascending order: WARPS warps a (row, query head), warp w shares w, w + WARPS, ..., whose sums
+// then come together.  What a share that the row has not would hold is fetched beside the others and left out: how many it
+// has is known only when the request's numbers have come.
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(128)
 tree_attention_merge_kernel(TreeArgs a, T* __restrict__ out) {
-  const int at = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  chain_wait(a.ws_acc, a.ws_ml, a.lengths, a.row0);
-  if (at >= a.T * a.Hq) return;
+  constexpr int AT_ONCE = 8;
+  __shared__ float part[WARPS > 1 ? 4 : 1][256 + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = WARPS > 1 ? blockIdx.x : blockIdx.x * 4 + warp;
   const int t = at / a.Hq;
-  int lo = 0, hi = a.S;                                      // the last request that begins at or before the row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.row0[mid] <= t) lo = mid; else hi = mid;
-  }
-  const TreeRequest r = tree_request(a, lo);
+  chain_wait(a.ws_acc, a.ws_ml, a.lengths, a.row0);
+  if (at >= a.T * a.Hq) return;                              // (one warp a row: the others go on)
+  const int own = WARPS > 1 ? warp : 0, most = (a.shares - own + WARPS - 1) / WARPS;       // shares that this warp looks at
+  const size_t step = (size_t)a.T * a.Hq;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + at;
+  auto fetch = [&](int c0, float4 (*v)[2]) {
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (c0 + c < most && 128 * i + 4 * lane < a.D)
+          v[c][i] = *reinterpret_cast<const float4*>(a.ws_acc + ((size_t)(own + WARPS * (c0 + c)) * step + at) * a.D + 128 * i + 4 * lane);
+  };
+  float4 v[AT_ONCE][2];
+  fetch(0, v);
+  float2 first = lane < a.shares ? ml[lane * step] : make_float2(-INFINITY, 0.f);          // of all shares, up to 32
+  int s = 0;                                                 // the last request that begins at or before the row
+  for (int s0 = 1; s0 < a.S; s0 += 32) s += __popc(__ballot_sync(0xffffffffu, s0 + lane < a.S && a.row0[s0 + lane] <= t));
+  const TreeRequest r = tree_request(a, s);
   if (t < r.row0 || t >= r.row0 + r.nodes) return;           // a row behind the last request's
   const int shares = (r.keys + a.chunk - 1) / a.chunk;
   if (shares == 1 && a.whole_written) return;
-  const size_t step = (size_t)a.T * a.Hq;
-  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + at;
-  float m = -INFINITY;
-  for (int c = lane; c < shares; c += 32) m = fmaxf(m, ml[c * step].x);
+  float m = lane < shares ? first.x : -INFINITY;
+  for (int c = 32 + lane; c < shares; c += 32) m = fmaxf(m, ml[c * step].x);
   const float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
+  const int n = (shares - own + WARPS - 1) / WARPS;
   float l = 0.f, sum[8] = {};
-  for (int c0 = 0; c0 < shares; c0 += 32) {
-    float w = 0.f;                                           // of share c0 + lane
-    if (c0 + lane < shares) {
-      const float2 v = ml[(c0 + lane) * step];
-      w = exp2f(v.x - base);
-      l += w * v.y;
-    }
-    const int n = min(32, shares - c0);
-#pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-      const float wc = __shfl_sync(0xffffffffu, w, c);
-      const float* acc = a.ws_acc + ((c0 + c) * step + at) * a.D;
+  for (int c0 = 0; c0 < n; c0 += AT_ONCE) {
+    if (c0) fetch(c0, v);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (128 * i + 4 * lane < a.D) {
-          const float4 v = *reinterpret_cast<const float4*>(acc + 128 * i + 4 * lane);
-          if (wc) sum[4 * i] += wc * v.x, sum[4 * i + 1] += wc * v.y, sum[4 * i + 2] += wc * v.z, sum[4 * i + 3] += wc * v.w;
-        }
+    for (int c = 0; c < AT_ONCE; ++c) {
+      if (c0 + c >= n) break;
+      const int share = own + WARPS * (c0 + c);
+      float2 x;
+      if (share < 32) x = make_float2(__shfl_sync(0xffffffffu, first.x, share), __shfl_sync(0xffffffffu, first.y, share));
+      else x = ml[share * step];
+      const float w = exp2f(x.x - base);
+      l += w * x.y;
+      if (w)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          sum[4 * i] += w * v[c][i].x, sum[4 * i + 1] += w * v[c][i].y, sum[4 * i + 2] += w * v[c][i].z, sum[4 * i + 3] += w * v[c][i].w;
     }
   }
-  l = warp_sum(l);
+  if constexpr (WARPS > 1) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int d = 128 * i + 4 * lane + k;
-      if (d < a.D) out[(size_t)at * a.D + d] = from_float<T>(l > 0.f ? sum[4 * i + k] / l : (l == 0.f ? 0.f : l));
+      for (int k = 0; k < 4; ++k)
+        if (128 * i + 4 * lane + k < a.D) part[warp][128 * i + 4 * lane + k] = sum[4 * i + k];
+    if (lane == 0) part[warp][256] = l;
+    __syncthreads();
+    l = (part[0][256] + part[1][256]) + (part[2][256] + part[3][256]);
+    for (int d = threadIdx.x; d < a.D; d += 128) {
+      const float x = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+      out[(size_t)at * a.D + d] = from_float<T>(l > 0.f ? x / l : (l == 0.f ? 0.f : l));
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (128 * i + 4 * lane < a.D) out[(size_t)at * a.D + 128 * i + 4 * lane + k] = from_float<T>(l > 0.f ? sum[4 * i + k] / l : (l == 0.f ? 0.f : l));
+  }
 }
 
 template <typename T, int NC>
 int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
   const size_t smem = ((size_t)kTreeRows * a.D + kTile * (2 * a.D + 4) + 4 * kTile * 4) * sizeof(float);
-  if (int rc = allow_smem((const void*)tree_attention_rows_kernel<T, NC>, smem)) return rc;
+  if (int rc = allow_smem<tree_attention_rows_kernel<T, NC>>(smem)) return rc;
   const int pairs = (int)min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv);
   const dim3 grid(a.shares, a.S * a.Hkv, (pairs + kTreeRows - 1) / kTreeRows);
   NF_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
@@ -206,7 +229,9 @@ int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out
 template <typename T>
 int launch_merge(const TreeArgs& a, void* out, cudaStream_t stream) {
   if (a.shares == 1) return 0;
-  launch_chained(tree_attention_merge_kernel<T>, dim3((a.T * a.Hq + 3) / 4), dim3(128), 0, stream, a, (T*)out);
+  // a warp a row takes eight shares in one trip to memory
+  if (a.shares <= 8) launch_chained(tree_attention_merge_kernel<T, 1>, dim3((a.T * a.Hq + 3) / 4), dim3(128), 0, stream, a, (T*)out);
+  else launch_chained(tree_attention_merge_kernel<T, 4>, dim3(a.T * a.Hq), dim3(128), 0, stream, a, (T*)out);
   return check_launch("tree_attention_merge");
 }
 
@@ -222,32 +247,68 @@ int launch_rows_of(const TreeArgs& a, const void* qkv, const void* pages, void* 
 
 using namespace nf;
 
-// Whether the tensor-core form takes these sizes: bfloat16, heads of 64 or 128, whole pages a block of 128 keys, queries on
-// 16-byte boundaries.
-extern "C" int nf_tree_attention_tensor(int dtype, int Hkv, int D, int page_size, long long num_pages, const void* qkv, long long q_stride) {
-  return dtype == kBF16 && tree_tc_fits(D, page_size, num_pages * 2 * Hkv * page_size) && (uintptr_t)qkv % 16 == 0 && q_stride % 8 == 0;
+static bool form_takes(int form, int dtype, int Hkv, int D, int page_size, long long num_pages, bool aligned) {
+  if (form == 0) return true;
+  return dtype == kBF16 && (D == 64 || D == 128) && aligned && page_size % 16 == 0 && num_pages * 2 * Hkv * page_size < (1ll << 31) &&
+         (form == 2 || (form == 1 && tree_tc_fits(D, page_size, num_pages * 2 * Hkv * page_size)));
 }
 
-// Keys a share takes, for calls of these sizes; the workspace is a float for every (share, row, query head, D + 2).
-extern "C" int nf_tree_attention_chunk(int S, int T, int Hq, int Hkv, int words, int max_context, int tensor) {
-  if (tensor) return tree_tc_chunk(S, T, Hq, Hkv, words, max_context);
+// How a call of these sizes is served: 4 times the keys of a share, plus the form: 0 CUDA cores; 1 tcgen05, 2 mma.sync, both
+// for bfloat16, heads of 64 or 128, pages of a multiple of 16 rows, and queries and results on 16-byte boundaries.  Up to 32 pairs a request and key head on
+// average mma.sync, which is then the faster (TREEFIG); beyond, the other where pages are 16, 32, 64 or 128
+// rows.  `form` from 0 on asks for one; it counts where it takes the sizes.  The workspace is a float for every (share, row,
+// query head, D + 2), where there is more than one share.
+extern "C" long long nf_tree_attention_plan(int form, int dtype, int S, int T, int Hq, int Hkv, int D, int page_size, long long num_pages, int words,
+                                            int max_context, int aligned) {
+  const bool asked = form >= 0 && form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned);
+  if (!asked) {
+    form = form_takes(1, dtype, Hkv, D, page_size, num_pages, aligned) ? 1 : (form_takes(2, dtype, Hkv, D, page_size, num_pages, aligned) ? 2 : 0);
+    if (form == 1 && (long long)T * (Hq / Hkv) <= 32ll * S) form = 2;
+  }
+  if (form == 1) return 4ll * tree_tc_chunk(S, T, Hq, Hkv, words, max_context) + 1;
+  if (form == 2) return 4ll * tree_mma_chunk(S, T, Hq, Hkv, max_context) + 2;
   // shares enough that a few hundred CTAs are under way, of 64 keys at least
   const long long pairs = std::min(32ll * words, (long long)T) * (Hq / Hkv);
   const long long ctas = (long long)S * Hkv * ((pairs + kTreeRows - 1) / kTreeRows);
   const long long shares = std::max(1ll, (148 * 4 + ctas - 1) / ctas);
   const long long chunk = ((max_context + shares - 1) / shares + 63) / 64 * 64;
-  return (int)std::max(64ll, std::min(chunk, 1ll << 20));
+  return 4ll * std::max(64ll, std::min(chunk, 1ll << 20));
 }
+
+// A call's operands, 8 bytes each: a caller that packs them at once spares the host a conversion for every argument.
+struct TreeCall {
+  const void* qkv;
+  long long q_stride;
+  const void* pages;
+  const int* block_table;
+  long long bt_width;
+  const int *lengths, *row0, *mask;
+  long long words;
+  void* out;
+  float* ws;
+  long long S, T, Hq, Hkv, D, page_size, num_pages, max_context, plan;
+  double scale;
+  long long dtype;
+  cudaStream_t stream;
+};
 
 // qkv [T, q_stride] with the queries in its first Hq * D columns; pages [num_pages, 2, Hkv, page_size, D]; block_table int32
 // [S, bt_width]; lengths int32 [S], row0 int32 [S + 1], mask int32 [T, words]; out [T, Hq * D]: rows that no request has
-// stay as they are.  max_context: no request has more keys, its nodes' among them.  ws: see nf_tree_attention_chunk; none
+// stay as they are.  max_context: no request has more keys, its nodes' among them.  plan, ws: see nf_tree_attention_plan; none
 // where one share takes all keys.
-extern "C" int nf_tree_attention(const void* qkv, long long q_stride, const void* pages, const int* block_table, int bt_width,
-                                 const int* lengths, const int* row0, const int* mask, int words, void* out, float* ws, int S, int T,
-                                 int Hq, int Hkv, int D, int page_size, int num_pages, int max_context, int chunk, int tensor, float scale,
-                                 int dtype, cudaStream_t stream) {
+extern "C" int nf_tree_attention(const TreeCall* call) {
+  const TreeCall& c = *call;
+  const void *qkv = c.qkv, *pages = c.pages;
+  void* out = c.out;
+  const long long q_stride = c.q_stride, plan = c.plan;
+  const int *block_table = c.block_table, *lengths = c.lengths, *row0 = c.row0, *mask = c.mask;
+  float* ws = c.ws;
+  const int bt_width = (int)c.bt_width, words = (int)c.words, S = (int)c.S, T = (int)c.T, Hq = (int)c.Hq, Hkv = (int)c.Hkv, D = (int)c.D,
+            page_size = (int)c.page_size, num_pages = (int)c.num_pages, max_context = (int)c.max_context, dtype = (int)c.dtype;
+  const float scale = (float)c.scale;
+  cudaStream_t stream = c.stream;
   if (S == 0 || T == 0) return 0;
+  const int form = (int)(plan & 3), chunk = (int)(plan >> 2);
   NF_REQUIRE(S > 0 && T > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && D > 0 && D % 16 == 0 && D <= 256 && page_size > 0 && num_pages > 0 &&
                  bt_width > 0 && words > 0 && max_context > 0 && chunk > 0 && q_stride >= (long long)Hq * D && (long long)T * Hq < (1ll << 31),
              "tree attention: bad sizes S=%d T=%d Hq=%d Hkv=%d D=%d page=%d", S, T, Hq, Hkv, D, page_size);
@@ -257,11 +318,12 @@ extern "C" int nf_tree_attention(const void* qkv, long long q_stride, const void
   NF_REQUIRE(shares == 1 || ws, "tree attention: %d shares of keys want a workspace", shares);
   float* ws_ml = ws ? ws + (size_t)shares * T * Hq * D : nullptr;
   TreeArgs a = {block_table, lengths, row0, mask, ws, ws_ml, q_stride, bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context,
-                chunk, shares, tensor, scale};
-  if (tensor) {
-    NF_REQUIRE(nf_tree_attention_tensor(dtype, Hkv, D, page_size, num_pages, qkv, q_stride) && chunk % 128 == 0 && (uintptr_t)out % 16 == 0,
-               "tree attention: sizes the tensor-core form does not take (D=%d page=%d)", D, page_size);
-    if (int rc = launch_tree_tc(a, qkv, pages, out, stream)) return rc;
+                chunk, shares, form != 0, scale};
+  if (form) {
+    const bool aligned = (uintptr_t)qkv % 16 == 0 && q_stride % 8 == 0 && (uintptr_t)out % 16 == 0;
+    NF_REQUIRE(form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned) && chunk % 128 == 0,
+               "tree attention: sizes that form %d does not take (D=%d page=%d)", form, D, page_size);
+    if (int rc = form == 1 ? launch_tree_tc(a, qkv, pages, out, stream) : launch_tree_mma(a, qkv, pages, out, stream)) return rc;
   } else if (int rc = dtype == kF32 ? launch_rows_of<float>(a, qkv, pages, out, stream) : launch_rows_of<__nv_bfloat16>(a, qkv, pages, out, stream)) {
     return rc;
   }

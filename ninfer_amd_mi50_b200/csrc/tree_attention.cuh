@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -46,13 +47,23 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, const TreeRequest& 
 bool tree_tc_fits(int D, int page_size, long long page_rows);
 int tree_tc_chunk(int S, int T, int Hq, int Hkv, int words, int max_context);
 int launch_tree_tc(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream);
+// The form for few pairs (tree_attention_mma.cu).
+int tree_mma_chunk(int S, int T, int Hq, int Hkv, int max_context);
+int launch_tree_mma(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream);
 
-// Lets a kernel have `bytes` of dynamic shared memory on the current device.
-inline int allow_smem(const void* kernel, size_t bytes) {
+// Lets KERNEL have `bytes` of dynamic shared memory, asked for once a device (the question takes the host as long as a launch).
+template <auto KERNEL>
+inline int allow_smem(size_t bytes) {
+  static std::atomic<size_t> had[64];
   if (bytes <= 48 * 1024) return 0;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const bool known = e == cudaSuccess && device >= 0 && device < 64;
+  if (known && had[device].load(std::memory_order_relaxed) >= bytes) return 0;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) (void)cudaGetLastError();
   NF_REQUIRE(e == cudaSuccess, "cannot have %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+  if (known) had[device].store(bytes, std::memory_order_relaxed);
   return 0;
 }
 

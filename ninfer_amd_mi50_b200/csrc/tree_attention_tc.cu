@@ -167,7 +167,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
   constexpr int STAGES = D == 64 ? 4 : 2;
   constexpr int PIECES = D / 8;                              // 16-byte pieces of a query
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);          // (an offset, so that what lies here is known to be shared memory)
   unsigned char* Qs = smem;                                  // [2 tiles]
   unsigned char* KV = Qs + 2 * KB;                           // [stages][keys, values]
   Barriers* bars = reinterpret_cast<Barriers*>(KV + 2 * STAGES * KB);
@@ -536,7 +536,7 @@ template <int D>
 int launch_tc(const CUtensorMap& map, TreeArgs a, const void* qkv, void* out, cudaStream_t stream) {
   const size_t smem = 1024 + (size_t)(2 + 2 * (D == 64 ? 4 : 2)) * (D / 64) * kAtom + sizeof(Barriers) + 4 * kRows * sizeof(float2) + sizeof(Requests);
   static_assert(sizeof(Barriers) % 8 == 0, "float2 follow");
-  if (int rc = allow_smem((const void*)tree_attention_tc_kernel<D>, smem)) return rc;
+  if (int rc = allow_smem<tree_attention_tc_kernel<D>>(smem)) return rc;
   const long long twos = (std::min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv) + 2 * kRows - 1) / (2 * kRows);
   const int S = a.S;
   for (int s0 = 0; s0 < S; s0 += kMostRequests) {

@@ -13,9 +13,9 @@
 //
 // A child's test needs three numbers, so those of all nodes are fetched at once and the walk goes over shared memory; what
 // takes time is the vocabulary's row at the walk's end, and one for a rejection of a drafted token.  A cluster of CTAs
-// takes a request: each walks by itself (the same numbers, the same steps), reads its part of such rows, and the parts'
-// sums change hands in shared memory.  A part is summed in segments of 1,024 numbers, so that the drawn token is searched
-// for in one of them.
+// takes a request: each walks by itself (the same numbers, the same steps) and reads its part of such rows, a warp a run of
+// neighbouring numbers; the runs' sums change hands in shared memory.  The drawn token is then in one CTA's part, in one
+// warp's run, which that warp reads once more, a lane a smaller run.
 #include "common.cuh"
 
 namespace nf {
@@ -23,8 +23,8 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kNodes = 1024;            // most nodes of a request
-constexpr int kSegment = 1024;          // numbers a warp sums up
-constexpr int kMaxSegments = 1024;      // of a CTA
+constexpr int kWarps = kThreads / 32;
+constexpr int kCtas = 8;                // of a cluster
 
 __device__ int g_verify_error = 0;
 
@@ -33,7 +33,7 @@ struct VerifyArgs {
   const int *tokens, *parents, *row0;
   int *accepted, *path, *said;
   long long probs_ld, draft_ld;
-  int T, V, most, part;                 // part: numbers of a CTA, a multiple of kSegment
+  int T, V, most, run;                  // run: numbers of a warp, a multiple of 128
 };
 
 struct Shared {
@@ -42,9 +42,9 @@ struct Shared {
   float draw[kNodes];
   int rejected[kNodes];                 // at the present node
   double mass[kNodes];                  // z when it was rejected
-  double segment[kMaxSegments], total[16];
+  double run[kWarps], total[2][kCtas];  // total: of a pass and of the next in turn, as a CTA may have gone on while another still reads
   double z;
-  int node, next, accepted, n_rejected, todo;
+  int node, next, accepted, n_rejected, todo, summed;
 };
 
 __device__ __forceinline__ void cluster_meet() {
@@ -56,11 +56,6 @@ __device__ __forceinline__ unsigned cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ unsigned cluster_size() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void put_cluster_f64(double* local, unsigned cta, double v) {
   unsigned remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(cta));
@@ -69,105 +64,142 @@ __device__ __forceinline__ void put_cluster_f64(double* local, unsigned cta, dou
 // A probability: what is no positive number counts as none.
 __device__ __forceinline__ double mass_of(float p) { return p > 0.f ? (double)p : 0.0; }
 
-// What is left of p[v] at token i after the node's rejections.
-__device__ __forceinline__ double left_at(const VerifyArgs& a, const Shared& sh, int row0, int n_rejected, int i) {
-  double r = mass_of(a.probs[(size_t)(row0 + sh.node) * a.probs_ld + i]);
+// Four neighbouring numbers of a row, of which the first `n` are in it: at once where the row allows it.
+__device__ __forceinline__ float4 four(const float* p, int n, bool vec) {
+  if (vec && n >= 4) return *reinterpret_cast<const float4*>(p);
+  return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+}
+// What is left of p[v] at tokens i .. i + 3 after the node's rejections, `n` of them in the vocabulary.
+__device__ __forceinline__ void left_at(const VerifyArgs& a, const Shared& sh, int row0, int n_rejected, int i, int n, bool vec, double* r) {
+  const float4 p = four(a.probs + (size_t)(row0 + sh.node) * a.probs_ld + i, n, vec);
+  r[0] = mass_of(p.x), r[1] = mass_of(p.y), r[2] = mass_of(p.z), r[3] = mass_of(p.w);
   for (int k = 0; k < n_rejected; ++k) {
     const int c = sh.rejected[k];
-    if (a.draft) r = fmax(r - sh.mass[k] * mass_of(a.draft[(size_t)(row0 + c) * a.draft_ld + i]), 0.0);
-    else if (sh.token[c] == i) r = 0.0;
+    if (a.draft) {
+      const float4 q = four(a.draft + (size_t)(row0 + c) * a.draft_ld + i, n, vec);
+      const double z = sh.mass[k];
+      r[0] = fmax(r[0] - z * mass_of(q.x), 0.0), r[1] = fmax(r[1] - z * mass_of(q.y), 0.0);
+      r[2] = fmax(r[2] - z * mass_of(q.z), 0.0), r[3] = fmax(r[3] - z * mass_of(q.w), 0.0);
+    } else {
+      const int x = sh.token[c] - i;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x == j) r[j] = 0.0;
+    }
   }
-  return r;
+}
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-// The sum of what is left: every CTA's segments, and all CTAs' sums in `total`.
-__device__ double sum_left(const VerifyArgs& a, Shared& sh, int row0, int n_rejected, int begin, int end) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_seg = (end - begin + kSegment - 1) / kSegment;
-  for (int g = warp; g < n_seg; g += kThreads / 32) {
-    const int lo = begin + g * kSegment, hi = min(lo + kSegment, end);
-    double sum = 0.0;
-    for (int i = lo + lane; i < hi; i += 32) sum += left_at(a, sh, row0, n_rejected, i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh.segment[g] = sum;
+// The sum of what is left: every warp's run, and all CTAs' sums in `total`.
+__device__ double sum_left(const VerifyArgs& a, Shared& sh, double* total, int row0, int n_rejected, bool vec) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int begin = (cluster_rank() * kWarps + warp) * a.run, end = min(begin + a.run, a.V);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int i = begin + 4 * lane; i < end; i += 128) {
+    double r[4];
+    left_at(a, sh, row0, n_rejected, i, end - i, vec, r);
+    sum += (r[0] + r[1]) + (r[2] + r[3]);
   }
-  cluster_meet();                       // (also: the sums of the time before have been read by all)
-  if (warp == 0) {
-    double sum = 0.0;
-    if (lane == 0)
-      for (int g = 0; g < n_seg; ++g) sum += sh.segment[g];
-    sum = __shfl_sync(0xffffffffu, sum, 0);
-    if ((unsigned)lane < cluster_size()) put_cluster_f64(&sh.total[cluster_rank()], lane, sum);
+  sum = warp_sum_f64(sum);
+  if (lane == 0) sh.run[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {                      // (the runs in their order; each CTA's sum goes to all)
+    double part = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) part += sh.run[w];
+    if (lane < kCtas) put_cluster_f64(&total[cluster_rank()], lane, part);
   }
   cluster_meet();
   double all = 0.0;
-  for (unsigned c = 0; c < cluster_size(); ++c) all += sh.total[c];
+#pragma unroll
+  for (int c = 0; c < kCtas; ++c) all += total[c];
   return all;
 }
 
-// The lowest token whose running sum passes `draw` times the whole, by the warp that has it; -1 where nothing is left.
-// Called by all threads of all CTAs after sum_left; one thread of the cluster writes `*to`.
-__device__ void draw_token(const VerifyArgs& a, const Shared& sh, int row0, int n_rejected, int begin, int end, double all, double draw, int* to) {
-  if (threadIdx.x >= 32) return;
-  const int lane = threadIdx.x;
+// The lowest token whose running sum passes `draw` times the whole, written to `*to` by the warp that has it; -1 where
+// nothing is left.  Called by all threads of all CTAs after sum_left.  Where rounding keeps the sums of a stretch from what
+// they were as parts, the last token that has anything is taken.
+__device__ void draw_token(const VerifyArgs& a, const Shared& sh, const double* total, int row0, int n_rejected, bool vec, double all, double draw, int* to) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double bound = draw * all;
-  // the CTA, then the segment, where the running sum passes the bound; else the last that has anything
   double run = 0.0, before = 0.0;
-  int cta = -1;
-  for (unsigned c = 0; c < cluster_size(); ++c) {
-    if (sh.total[c] > 0.0) {
-      cta = c, before = run;
-      if (run + sh.total[c] > bound) break;
+  int mine = -1;
+  for (int c = 0; c < kCtas; ++c) {
+    const double t = total[c];
+    if (t > 0.0) {
+      mine = c, before = run;
+      if (run + t > bound) break;
     }
-    run += sh.total[c];
+    run += t;
   }
-  if (cta < 0) {
-    if (cluster_rank() == 0 && lane == 0) *to = -1;
+  if (mine < 0) {
+    if (cluster_rank() == 0 && threadIdx.x == 0) *to = -1;
     return;
   }
-  if ((unsigned)cta != cluster_rank()) return;
+  if ((unsigned)mine != cluster_rank()) return;
   run = before;
-  int seg = -1;
-  const int n_seg = (end - begin + kSegment - 1) / kSegment;
-  for (int g = 0; g < n_seg; ++g) {
-    if (sh.segment[g] > 0.0) {
-      seg = g, before = run;
-      if (run + sh.segment[g] > bound) break;
+  mine = -1;
+  for (int w = 0; w < kWarps; ++w) {
+    const double t = sh.run[w];
+    if (t > 0.0) {
+      mine = w, before = run;
+      if (run + t > bound) break;
     }
-    run += sh.segment[g];
+    run += t;
   }
-  const int lo = begin + seg * kSegment, hi = min(lo + kSegment, end);
-  int last = -1;
-  run = before;
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    const double r = i < hi ? left_at(a, sh, row0, n_rejected, i) : 0.0;
-    double upto = r;
+  if (mine != warp) return;
+  // a lane takes a run of neighbouring numbers
+  const int begin = (cluster_rank() * kWarps + warp) * a.run, end = min(begin + a.run, a.V), each = a.run / 32;
+  const int lo = begin + lane * each, hi = min(lo + each, end);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int i = lo; i < hi; i += 4) {
+    double r[4];
+    left_at(a, sh, row0, n_rejected, i, hi - i, vec, r);
+    sum += (r[0] + r[1]) + (r[2] + r[3]);
+  }
+  double upto = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, r > 0.0), past = __ballot_sync(0xffffffffu, r > 0.0 && run + upto > bound);
-    if (past) {
-      if (lane == 0) *to = i0 + __ffs(past) - 1;
-      return;
-    }
-    if (some) last = i0 + 31 - __clz(some);
-    run += __shfl_sync(0xffffffffu, upto, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const double v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
-  if (lane == 0) *to = last;
+  const unsigned some = __ballot_sync(0xffffffffu, sum > 0.0), past = __ballot_sync(0xffffffffu, sum > 0.0 && before + upto > bound);
+  const int owner = past ? __ffs(past) - 1 : 31 - __clz(some);
+  if (lane != owner) return;
+  run = before + (upto - sum);
+  int last = -1;
+  for (int i = lo; i < hi; i += 4) {
+    double r[4];
+    left_at(a, sh, row0, n_rejected, i, hi - i, vec, r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      run += r[j];
+      if (r[j] > 0.0) {
+        last = i + j;
+        if (run > bound) {
+          *to = last;
+          return;
+        }
+      }
+    }
+  }
+  *to = last;
 }
 
 __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const unsigned rank = cluster_rank();
-  const int s = blockIdx.x / cluster_size();
+  const int s = blockIdx.x / kCtas;
   const int begin0 = a.row0[s], end0 = a.row0[s + 1];
   const int row0 = min(max(begin0, 0), a.T), n = min(min(max(end0, row0), a.T) - row0, kNodes);
   bool bad = begin0 < 0 || end0 <= begin0 || end0 > a.T || end0 - begin0 > kNodes;
-  const int begin = min((int)rank * a.part, a.V), end = min(begin + a.part, a.V);
   int* path = a.path + (size_t)s * a.most;
   int* said = a.said + (size_t)s * (a.most + 1);
   if (rank == 0) {
@@ -185,17 +217,19 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
     sh.have[i] = fits && i > 0 ? a.probs[(size_t)(row0 + parent) * a.probs_ld + token] : 0.f;
   }
   if (bad && rank == 0) atomicCAS(&g_verify_error, 0, 1 + s);
-  if (threadIdx.x == 0) sh.node = 0, sh.next = 1, sh.accepted = 0, sh.n_rejected = 0, sh.z = 1.0;
+  if (threadIdx.x == 0) sh.node = 0, sh.next = 1, sh.accepted = 0, sh.n_rejected = 0, sh.z = 1.0, sh.summed = 0;
   __syncthreads();
   if (n == 0) {                                            // (no root: the whole cluster leaves)
     if (rank == 0 && threadIdx.x == 0) a.accepted[s] = 0;
     return;
   }
+  // rows that can be read four numbers at a time
+  const bool vec = ((uintptr_t)a.probs | (uintptr_t)a.draft) % 16 == 0 && (a.probs_ld | a.draft_ld) % 4 == 0;
   double all = 0.0;
-  bool summed = false;
+  int pass = 0;
   for (;;) {
     if (threadIdx.x == 0) {
-      int v = sh.node, i = sh.next, k = sh.n_rejected, got = sh.accepted;
+      int v = sh.node, i = sh.next, k = sh.n_rejected, got = sh.accepted, summed = sh.summed;
       double z = sh.z;
       bool wait = false;                                   // for the sum of what a rejection has left
       for (; i < n && got < a.most && !wait; ++i) {
@@ -216,22 +250,21 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
           if (a.draft) wait = true;
           else z -= have;
         }
+        summed = 0;
       }
-      sh.node = v, sh.next = i, sh.n_rejected = k, sh.accepted = got, sh.z = z, sh.todo = wait;
+      sh.node = v, sh.next = i, sh.n_rejected = k, sh.accepted = got, sh.z = z, sh.todo = wait, sh.summed = summed;
     }
     __syncthreads();
-    summed = sh.todo;
-    if (!summed) break;
-    all = sum_left(a, sh, row0, sh.n_rejected, begin, end);
-    if (threadIdx.x == 0) sh.z = all;
-    if (sh.next >= n) break;                               // (nothing else to ask: the sums serve the draw)
-    __syncthreads();
+    if (!sh.todo) break;
+    pass ^= 1;
+    all = sum_left(a, sh, sh.total[pass], row0, sh.n_rejected, vec);
+    if (threadIdx.x == 0) sh.z = all, sh.summed = 1;
   }
   int k = sh.n_rejected;
-  if (!summed) all = sum_left(a, sh, row0, k, begin, end);
-  if (!(all > 0.0) && k > 0) k = 0, all = sum_left(a, sh, row0, 0, begin, end);
+  if (!sh.summed) pass ^= 1, all = sum_left(a, sh, sh.total[pass], row0, k, vec);      // (where the last thing was a rejection its sums serve the draw)
+  if (!(all > 0.0) && k > 0) k = 0, pass ^= 1, all = sum_left(a, sh, sh.total[pass], row0, 0, vec);
   if (!(all > 0.0) && rank == 0 && threadIdx.x == 0) atomicCAS(&g_verify_error, 0, 1 + s);
-  draw_token(a, sh, row0, k, begin, end, all, (double)sh.draw[0], said + sh.accepted);
+  draw_token(a, sh, sh.total[pass], row0, k, vec, all, (double)sh.draw[0], said + sh.accepted);
   if (rank == 0 && threadIdx.x == 0) a.accepted[s] = sh.accepted;
   cluster_meet();                                          // (no CTA leaves while another may still write to it)
 }
@@ -249,20 +282,18 @@ extern "C" int nf_verify_drafts(const float* probs, long long probs_ld, const fl
                                 const int* parents, const int* row0, const float* draws, int* accepted, int* path, int* said, int S, int T,
                                 int V, int most, cudaStream_t stream) {
   if (S == 0) return 0;
-  NF_REQUIRE(S > 0 && S <= (1 << 20) && T > 0 && V > 0 && most > 0 && probs_ld >= V && (!draft || draft_ld >= V),
+  NF_REQUIRE(S > 0 && S <= (1 << 20) && T > 0 && V > 0 && V <= (1 << 30) && most > 0 && probs_ld >= V && (!draft || draft_ld >= V),
              "verify drafts: bad sizes S=%d T=%d V=%d most=%d", S, T, V, most);
-  const int ctas = 8;
-  const int part = ((V + ctas - 1) / ctas + kSegment - 1) / kSegment * kSegment;
-  NF_REQUIRE(part / kSegment <= kMaxSegments, "verify drafts: a vocabulary of %d is too large", V);
-  VerifyArgs a = {probs, draft, draws, tokens, parents, row0, accepted, path, said, probs_ld, draft_ld, T, V, most, part};
+  const int run = ((V + kCtas * kWarps - 1) / (kCtas * kWarps) + 127) / 128 * 128;
+  VerifyArgs a = {probs, draft, draws, tokens, parents, row0, accepted, path, said, probs_ld, draft_ld, T, V, most, run};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(S * ctas);
+  cfg.gridDim = dim3(S * kCtas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.x = kCtas;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;

@@ -12,12 +12,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import lib as _lib
-from .ops import TUNING, _DT, _chk, _dt, check_head_dim
+from .ops import TUNING, _chk, _dt, check_head_dim
 
 __all__ = ["MAX_TREE_NODES", "MAX_VERIFY_NODES", "compact_cache", "copy_pages", "draft_status", "tree_attention", "verify_drafts"]
 
@@ -25,15 +26,18 @@ MAX_TREE_NODES = 256          # nodes of a request that tree attention takes
 MAX_VERIFY_NODES = 1024       # ... and verification
 MAX_TREE_CONTEXT = 1 << 30
 
-_I, _L, _P, _F = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_float
+_I, _L, _P = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
 _SIGNATURES = {
-    "nf_tree_attention_tensor": [_I] * 4 + [_L, _P, _L],
-    "nf_tree_attention_chunk": [_I] * 7,
-    "nf_tree_attention": [_P, _L, _P, _P, _I] + [_P] * 3 + [_I] + [_P] * 2 + [_I] * 10 + [_F, _I, _P],
+    "nf_tree_attention_plan": [_I] * 8 + [_L] + [_I] * 3,
+    "nf_tree_attention": [_P],
     "nf_verify_drafts": [_P, _L, _P, _L] + [_P] * 7 + [_I] * 4 + [_P],
     "nf_compact_cache": [_P, _L] + [_I] * 5 + [_P, _I] + [_P] * 3 + [_I] * 2 + [_P],
     "nf_copy_pages": [_P, _L] + [_I] * 5 + [_P] * 3 + [_I, _P],
 }
+_TREE_CALL = struct.Struct("=20qd2q")          # TreeCall of tree_attention.cu
+_plans = {}             # sizes -> how a call of these is served, as nf_tree_attention_plan says
+_int32, _float32 = torch.int32, torch.float32
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _functions = {}
 _used = False           # whether any of these kernels was called: until then there is no status to read
 
@@ -43,21 +47,22 @@ def _function(name: str):
     if f is None:
         f = getattr(_lib.load(), name)
         f.argtypes = _SIGNATURES[name]
+        if name == "nf_tree_attention_plan":
+            f.restype = _L
         _functions[name] = f
     return f
 
 
-def _call(name: str, device: int, *args) -> None:
-    """The C function, on the current stream of the tensors' device."""
+def _begin(name: str):
+    """The C function, about to be called."""
     global _used
     _used = True
-    if device != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
-            _call(name, device, *args)
-        return
     _lib.count_launches(1)
-    if (_functions.get(name) or _function(name))(*args, torch._C._cuda_getCurrentRawStream(device)):
-        raise _lib.KernelError(f"{name}: {_lib.load().nf_last_error().decode(errors='replace')}")
+    return _functions.get(name) or _function(name)
+
+
+def _failed(name: str) -> None:
+    raise _lib.KernelError(f"{name}: {_lib.load().nf_last_error().decode(errors='replace')}")
 
 
 def _ints(what: str, device, **tensors) -> None:
@@ -128,49 +133,91 @@ def tree_attention(qkv: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Te
 
     Rows that belong to no request stay as they were in `out`.  Rows, lengths or nodes outside the bounds, and pages outside
     the pool, count as if they ended there, and are reported by `check_status`."""
-    dtype, dev = qkv.dtype, qkv.get_device()
-    qs, bs, ms = qkv.shape, block_table.shape, mask.shape
-    if not (dev >= 0 and dtype in _DT and pages.dtype is dtype and pages.get_device() == dev and pages.is_contiguous() and len(qs) == 2
-            and len(bs) == 2 and len(ms) == 2 and D % 16 == 0 and 16 <= D <= 256 and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and page_size > 0
-            and qs[1] >= Hq * D and qkv.stride(1) == 1 and (qs[0] <= 1 or qkv.stride(0) >= qs[1]) and 1 <= pages.shape[0] < 1 << 31
-            and pages.shape[1:] == (2, Hkv, page_size, D) and block_table.dtype is torch.int32 and lengths.dtype is torch.int32
-            and row0.dtype is torch.int32 and mask.dtype is torch.int32 and block_table.get_device() == dev and lengths.get_device() == dev
-            and row0.get_device() == dev and mask.get_device() == dev and block_table.is_contiguous() and lengths.is_contiguous()
-            and row0.is_contiguous() and mask.is_contiguous() and bs[1] > 0 and lengths.shape == bs[:1] and row0.shape == (bs[0] + 1,)
-            and ms[0] == qs[0] and 1 <= ms[1] <= MAX_TREE_NODES // 32 and 1 <= max_context <= MAX_TREE_CONTEXT and 0.0 < scale < math.inf
-            and pages.data_ptr() % 16 == 0):
+    dev, dtype = qkv.get_device(), qkv.dtype
+    qs, bs, ms, ps = qkv.shape, block_table.shape, mask.shape, pages.shape
+    good = (dev >= 0 and len(qs) == 2 and len(bs) == 2 and len(ms) == 2 and len(ps) == 5 and (dtype is torch.bfloat16 or dtype is _float32)
+            and pages.dtype is dtype and block_table.dtype is _int32 and lengths.dtype is _int32 and row0.dtype is _int32 and mask.dtype is _int32
+            and pages.get_device() == dev and block_table.get_device() == dev and lengths.get_device() == dev and row0.get_device() == dev
+            and mask.get_device() == dev and pages.is_contiguous() and block_table.is_contiguous() and lengths.is_contiguous()
+            and row0.is_contiguous() and mask.is_contiguous() and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and D % 16 == 0 and 16 <= D <= 256
+            and page_size > 0 and 1 <= max_context <= MAX_TREE_CONTEXT and 0.0 < scale < math.inf)
+    if good:
+        (T, width), (S, table_width), (rows, words), (n_pages, two, heads, size, dim) = qs, bs, ms, ps
+        step, one = qkv.stride()
+        if T <= 1:
+            step = -(-width // 8) * 8
+        p_pages = pages.data_ptr()
+        good = (width >= Hq * D and one == 1 and step >= width and 1 <= n_pages < 1 << 31 and two == 2 and heads == Hkv and size == page_size
+                and dim == D and table_width > 0 and lengths.shape == (S,) and row0.shape == (S + 1,) and rows == T
+                and 1 <= words <= MAX_TREE_NODES // 32 and p_pages % 16 == 0)
+    if not good or out is not None:
         _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale, out)
-    T, S = qs[0], bs[0]
+        if dev != _current_device():
+            with torch.cuda.device(dev):
+                return tree_attention(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale, out)
+    elif dev != _current_device():
+        with torch.cuda.device(dev):
+            return tree_attention(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale)
     if out is None:
         out = qkv.new_empty((T, Hq * D))
-    else:
-        _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, mask, max_context, scale, out)
     if T == 0 or S == 0:
         return out
-    p_q, step = qkv.data_ptr(), qkv.stride(0) if T > 1 else qs[1]
-    tensor = TUNING["tree_attention"] == "auto" and _function("nf_tree_attention_tensor")(_DT[dtype], Hkv, D, page_size, pages.shape[0], p_q, step) \
-        and out.data_ptr() % 16 == 0
-    chunk = _function("nf_tree_attention_chunk")(S, T, Hq, Hkv, ms[1], max_context, tensor)
-    shares = -(-max_context // chunk)
-    ws = torch.empty(shares * T * Hq * (D + 2), dtype=torch.float32, device=qkv.device) if shares > 1 else None
-    _call("nf_tree_attention", dev, p_q, step, pages.data_ptr(), block_table.data_ptr(), bs[1],
-          lengths.data_ptr(), row0.data_ptr(), mask.data_ptr(), ms[1], out.data_ptr(), None if ws is None else ws.data_ptr(), S, T, Hq, Hkv, D,
-          page_size, pages.shape[0], max_context, chunk, tensor, scale, _DT[dtype])
+    p_q, p_out = qkv.data_ptr(), out.data_ptr()
+    code = 1 if dtype is torch.bfloat16 else 0
+    key = (S, T, Hq, Hkv, D, page_size, n_pages, words, max_context, code, (p_q | p_out | 2 * step) & 15 == 0, TUNING["tree_attention"])
+    plan = _plans.get(key)
+    if plan is None:
+        form = key[-1]
+        plan = _function("nf_tree_attention_plan")(-1 if form == "auto" else form, code, S, T, Hq, Hkv, D, page_size, n_pages, words, max_context, key[-2])
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    shares = -(-max_context // (plan >> 2))
+    # (kept until the call has been made; what comes after it on the stream may have the memory)
+    ws = lengths.new_empty(shares * T * Hq * (D + 2)) if shares > 1 else None
+    if _begin("nf_tree_attention")(_TREE_CALL.pack(p_q, step, p_pages, block_table.data_ptr(), table_width, lengths.data_ptr(), row0.data_ptr(),
+                                                   mask.data_ptr(), words, p_out, 0 if ws is None else ws.data_ptr(), S, T, Hq, Hkv, D, page_size,
+                                                   n_pages, max_context, plan, scale, code, _raw_stream(dev))):
+        _failed("nf_tree_attention")
     return out
 
 
-def _rows(t: torch.Tensor, name: str, T: int, V: int, device) -> int:
-    """Numbers between two rows of float32 [T, V]; raises where they are not runs of their own."""
-    _chk(t, name, torch.float32, contiguous=False)
-    if t.device != device or t.shape != (T, V):
-        raise ValueError(f"verify_drafts: {name} is {tuple(t.shape)} on {t.device}, not {(T, V)} on {device}")
-    if T <= 1 or V <= 1:
-        step = t.stride(0) if T > 1 else V
-    else:
-        step = t.stride(0)
-    if (V > 1 and t.stride(1) != 1) or step < V:
-        raise ValueError(f"verify_drafts: the rows of {name} must be runs of their own, got strides {t.stride()}")
-    return step
+def _rows_apart(t: torch.Tensor, T: int, V: int) -> int:
+    """Numbers between two rows of [T, V], or -1 where the rows are not runs of their own."""
+    step, one = t.stride()
+    if T <= 1:
+        step = V
+    return step if (one == 1 or V <= 1) and step >= V else -1
+
+
+def _refuse_verify(probs, tokens, parents, row0, draws, most, draft) -> None:
+    """Says what is wrong with the operands of verify_drafts."""
+    what = "verify_drafts"
+    _chk(probs, "probs", torch.float32, contiguous=False)
+    if probs.dim() != 2 or probs.shape[1] < 1:
+        raise ValueError(f"{what}: probs are {tuple(probs.shape)}, not [rows, vocabulary]")
+    T, V = probs.shape
+    dev = probs.device
+    _ints(what, dev, tokens=tokens, parents=parents, row0=row0)
+    _chk(draws, "draws", torch.float32)
+    if draws.device != dev:
+        raise ValueError(f"{what}: draws lie on {draws.device}, not on {dev}")
+    for t, name in ((tokens, "tokens"), (parents, "parents"), (draws, "draws")):
+        if t.shape != (T,):
+            raise ValueError(f"{what}: {name} are {tuple(t.shape)}, not {(T,)}")
+    if row0.dim() != 1 or row0.numel() < 1:
+        raise ValueError(f"{what}: row0 is {tuple(row0.shape)}, not [requests + 1]")
+    if not 1 <= most <= MAX_VERIFY_NODES:
+        raise ValueError(f"{what}: most={most} is not within 1 and {MAX_VERIFY_NODES}")
+    if draft is not None:
+        _chk(draft, "draft", torch.float32, contiguous=False)
+        if draft.device != dev or draft.shape != (T, V):
+            raise ValueError(f"{what}: draft is {tuple(draft.shape)} on {draft.device}, not {(T, V)} on {dev}")
+    for t, name in ((probs, "probs"), (draft, "draft")):
+        if t is not None and _rows_apart(t, T, V) < 0:
+            raise ValueError(f"{what}: the rows of {name} must be runs of their own, got strides {t.stride()}")
+    if row0.numel() > 1 and not T:
+        raise ValueError(f"{what}: {row0.numel() - 1} requests without a row")
 
 
 def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, row0: torch.Tensor, draws: torch.Tensor, most: int,
@@ -193,53 +240,74 @@ def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
     `path[s]` lists the accepted nodes, `said[s]` their tokens and the next one, both with -1 behind; accepted[s] counts
     the drafted ones.  What is no positive number counts as a probability of 0; a row that holds nothing gives -1.  Nodes
     whose token or parent makes no sense are nobody's children.  Both are reported by `check_status`."""
-    _chk(probs, "probs", torch.float32, contiguous=False)
-    if probs.dim() != 2 or probs.shape[1] < 1:
-        raise ValueError(f"verify_drafts: probs are {tuple(probs.shape)}, not [rows, vocabulary]")
-    T, V = probs.shape
-    dev = probs.device
-    _ints("verify_drafts", dev, tokens=tokens, parents=parents, row0=row0)
-    _chk(draws, "draws", torch.float32)
-    if draws.device != dev:
-        raise ValueError(f"verify_drafts: draws lie on {draws.device}, not on {dev}")
-    for t, name in ((tokens, "tokens"), (parents, "parents"), (draws, "draws")):
-        if t.shape != (T,):
-            raise ValueError(f"verify_drafts: {name} are {tuple(t.shape)}, not {(T,)}")
-    if row0.dim() != 1 or row0.numel() < 1:
-        raise ValueError(f"verify_drafts: row0 is {tuple(row0.shape)}, not [requests + 1]")
-    if not 1 <= most <= MAX_VERIFY_NODES:
-        raise ValueError(f"verify_drafts: most={most} is not within 1 and {MAX_VERIFY_NODES}")
-    probs_ld = _rows(probs, "probs", T, V, dev)
-    draft_ld = 0 if draft is None else _rows(draft, "draft", T, V, dev)
-    S = row0.numel() - 1
-    out = torch.empty(S * (2 * most + 2), dtype=torch.int32, device=dev)
-    accepted, path, said = out[:S], out[S:S * (most + 1)].view(S, most), out[S * (most + 1):].view(S, most + 1)
-    if S and not T:
-        raise ValueError(f"verify_drafts: {S} requests without a row")
-    if S:
-        _call("nf_verify_drafts", probs.get_device(), probs.data_ptr(), probs_ld, None if draft is None else draft.data_ptr(), draft_ld,
-              tokens.data_ptr(), parents.data_ptr(), row0.data_ptr(), draws.data_ptr(), accepted.data_ptr(), path.data_ptr(), said.data_ptr(),
-              S, T, V, most)
-    return accepted, path, said
+    dev, shape = probs.get_device(), probs.shape
+    good = (dev >= 0 and len(shape) == 2 and shape[1] > 0 and probs.dtype is _float32 and draws.dtype is _float32 and tokens.dtype is _int32
+            and parents.dtype is _int32 and row0.dtype is _int32 and tokens.get_device() == dev and parents.get_device() == dev
+            and row0.get_device() == dev and draws.get_device() == dev and tokens.is_contiguous() and parents.is_contiguous()
+            and row0.is_contiguous() and draws.is_contiguous() and row0.dim() == 1 and tokens.dim() == 1 and parents.dim() == 1
+            and draws.dim() == 1 and 1 <= most <= MAX_VERIFY_NODES)
+    if good:
+        T, V = shape
+        S = row0.numel() - 1
+        probs_ld, draft_ld, p_draft = _rows_apart(probs, T, V), 0, None
+        good = tokens.numel() == T and parents.numel() == T and draws.numel() == T and S >= 0 and probs_ld >= 0 and (T > 0 or S == 0)
+        if good and draft is not None:
+            good = draft.dtype is _float32 and draft.get_device() == dev and draft.shape == shape
+            if good:
+                draft_ld, p_draft = _rows_apart(draft, T, V), draft.data_ptr()
+                good = draft_ld >= 0
+    if not good:
+        _refuse_verify(probs, tokens, parents, row0, draws, most, draft)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return verify_drafts(probs, tokens, parents, row0, draws, most, draft)
+    accepted, path, said = tokens.new_empty(S * (2 * most + 2)).split_with_sizes((S, S * most, S * (most + 1)))
+    if S and _begin("nf_verify_drafts")(probs.data_ptr(), probs_ld, p_draft, draft_ld, tokens.data_ptr(), parents.data_ptr(), row0.data_ptr(),
+                                        draws.data_ptr(), accepted.data_ptr(), path.data_ptr(), said.data_ptr(), S, T, V, most, _raw_stream(dev)):
+        _failed("nf_verify_drafts")
+    return accepted, path.view(S, most), said.view(S, most + 1)
 
 
-def _shape(what: str, pages: torch.Tensor) -> Tuple[int, ...]:
-    """(address, bytes between two layers, layers, pages, planes, page size, row bytes) of a cache group's pages: one layer's
-    [pages, 2, heads, page_size, D] or [pages, page_size, width], or with the layers before that."""
+def _refuse_pages(what: str, pages: torch.Tensor) -> None:
+    """Says what is wrong with a cache group's pages."""
     _chk(pages, "pages", contiguous=False)
     if pages.dim() not in (3, 4, 5, 6):
         raise ValueError(f"{what}: pages are {tuple(pages.shape)}, not (layers,) pages, (2, heads,) page_size, width")
     layered = pages if pages.dim() in (4, 6) else pages.unsqueeze(0)
-    L, P, size = layered.shape[0], layered.shape[1], layered.element_size()
     if layered.numel() == 0:
         raise ValueError(f"{what}: pages are {tuple(pages.shape)}")
-    if not layered[0].is_contiguous() or (L > 1 and layered.stride(0) < layered[0].numel()):
+    if not layered[0].is_contiguous() or (layered.shape[0] > 1 and layered.stride(0) < layered[0].numel()):
         raise ValueError(f"{what}: a layer's pages must be contiguous, got strides {pages.stride()}")
-    planes = layered.shape[2] * layered.shape[3] if layered.dim() == 6 else 1
-    row = layered.shape[-1] * size
-    if row % 2 or max(P, planes, layered.shape[-2], row, L) >= 1 << 31:
-        raise ValueError(f"{what}: rows of {layered.shape[-1]} numbers of {size} bytes, in pages {tuple(pages.shape)}")
-    return layered.data_ptr(), (layered.stride(0) if L > 1 else layered[0].numel()) * size, L, P, planes, layered.shape[-2], row
+    raise ValueError(f"{what}: rows of {layered.shape[-1]} numbers of {layered.element_size()} bytes, in pages {tuple(pages.shape)}")
+
+
+def _pages(what: str, pages: torch.Tensor) -> Tuple[int, ...]:
+    """(address, bytes between two layers, layers, pages, planes, page size, row bytes) of a cache group's pages: one layer's
+    [pages, 2, heads, page_size, D] or [pages, page_size, width], or with the layers before that."""
+    shape, size = pages.shape, pages.element_size()
+    n = len(shape)
+    if n == 6 or n == 5:
+        planes = shape[-4] * shape[-3]
+    elif n == 4 or n == 3:
+        planes = 1
+    else:
+        _refuse_pages(what, pages)
+    layers, P = (shape[0], shape[1]) if n % 2 == 0 else (1, shape[0])
+    rows, width = shape[-2], shape[-1]
+    layer = P * planes * rows * width
+    apart = layer
+    if pages.is_contiguous():
+        good = True
+    elif n % 2 == 0:
+        apart = pages.stride(0) if layers > 1 else layer
+        good = layers > 0 and pages[0].is_contiguous() and apart >= layer
+    else:
+        good = False
+    row = width * size
+    if not (good and pages.is_cuda and layer > 0 and layers > 0 and row % 2 == 0 and row < 1 << 31 and P < 1 << 31 and planes < 1 << 31
+            and rows < 1 << 31 and layers < 1 << 31 and planes * rows * row < 1 << 40):
+        _refuse_pages(what, pages)
+    return pages.data_ptr(), apart * size, layers, P, planes, rows, row
 
 
 def compact_cache(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
@@ -251,16 +319,22 @@ def compact_cache(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch
     [layers, pages, 2, heads, page_size, D] or [layers, pages, page_size, width], or one layer's; block_table int32
     [S, width]; path int32 [S, most] (rising) and accepted int32 [S] as `verify_drafts` gives them.  A request whose path does
     not rise keeps its rows as they are, a row whose page is not in the pool stays: both are reported by `check_status`."""
-    shape = _shape("compact_cache", pages)
-    _ints("compact_cache", pages.device, block_table=block_table, lengths=lengths, path=path, accepted=accepted)
-    if (block_table.dim() != 2 or block_table.shape[1] < 1 or path.dim() != 2 or lengths.dim() != 1 or lengths.shape != block_table.shape[:1]
-            or accepted.shape != lengths.shape or path.shape[0] != lengths.numel()):
+    shape, dev = _pages("compact_cache", pages), pages.get_device()
+    ts, ps = block_table.shape, path.shape
+    if not (block_table.dtype is _int32 and lengths.dtype is _int32 and path.dtype is _int32 and accepted.dtype is _int32
+            and block_table.get_device() == dev and lengths.get_device() == dev and path.get_device() == dev and accepted.get_device() == dev
+            and block_table.is_contiguous() and lengths.is_contiguous() and path.is_contiguous() and accepted.is_contiguous() and len(ts) == 2
+            and len(ps) == 2 and ts[1] > 0 and lengths.dim() == 1 and lengths.numel() == ts[0] and accepted.shape == lengths.shape and ps[0] == ts[0]):
+        _ints("compact_cache", pages.device, block_table=block_table, lengths=lengths, path=path, accepted=accepted)
         raise ValueError(f"compact_cache: block table {tuple(block_table.shape)}, lengths {tuple(lengths.shape)}, path {tuple(path.shape)} and "
                          f"accepted {tuple(accepted.shape)} are not of one number of requests")
-    S, most = path.shape
-    if S and most:
-        _call("nf_compact_cache", pages.get_device(), *shape, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), path.data_ptr(),
-              accepted.data_ptr(), S, most)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return compact_cache(pages, block_table, lengths, path, accepted)
+    S, most = ps
+    if S and most and _begin("nf_compact_cache")(*shape, block_table.data_ptr(), ts[1], lengths.data_ptr(), path.data_ptr(), accepted.data_ptr(), S,
+                                                 most, _raw_stream(dev)):
+        _failed("nf_compact_cache")
 
 
 def copy_pages(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
@@ -268,25 +342,30 @@ def copy_pages(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, rows: 
     where `rows` is given, the others then stay.  src, dst and rows are int32 lists of one length; no page may be written
     twice, or be read and written.  An entry that is outside the pool, or has more rows than a page, is left out and
     reported by `check_status`."""
-    shape = _shape("copy_pages", pages)
-    _ints("copy_pages", pages.device, src=src, dst=dst, **({} if rows is None else {"rows": rows}))
-    if src.dim() != 1 or dst.shape != src.shape or (rows is not None and rows.shape != src.shape):
+    shape, dev, n = _pages("copy_pages", pages), pages.get_device(), src.numel()
+    if not (src.dtype is _int32 and dst.dtype is _int32 and src.get_device() == dev and dst.get_device() == dev and src.is_contiguous()
+            and dst.is_contiguous() and src.dim() == 1 and dst.dim() == 1 and dst.numel() == n
+            and (rows is None or (rows.dtype is _int32 and rows.get_device() == dev and rows.is_contiguous() and rows.dim() == 1 and rows.numel() == n))):
+        _ints("copy_pages", pages.device, src=src, dst=dst, **({} if rows is None else {"rows": rows}))
         raise ValueError(f"copy_pages: src {tuple(src.shape)}, dst {tuple(dst.shape)}"
                          + ("" if rows is None else f" and rows {tuple(rows.shape)}") + " are not lists of one length")
-    if src.numel():
-        _call("nf_copy_pages", pages.get_device(), *shape, src.data_ptr(), dst.data_ptr(), None if rows is None else rows.data_ptr(), src.numel())
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return copy_pages(pages, src, dst, rows)
+    if n and _begin("nf_copy_pages")(*shape, src.data_ptr(), dst.data_ptr(), None if rows is None else rows.data_ptr(), n, _raw_stream(dev)):
+        _failed("nf_copy_pages")
 
 
 def draft_status() -> int:
     """0, or what these kernels met since the last call: 1000001 + a request whose lengths, rows or pages did not fit tree
     attention, 2000001 + one whose tree or probabilities made no sense to verification, 3000001 + a request or an entry whose
     path or pages did not fit a copy, 4000000 + a code of tree attention on tensor cores (2 to 11: a bounded wait that ran out,
-    101 + a request that did not fit).  Synchronises the device; where none was ever called there is nothing to read."""
+    101 + a request that did not fit), 5000000 + one of its form for few pairs (1 and 2, 101 + a request).  Synchronises the device; where none was ever called there is nothing to read."""
     if not _used:
         return 0
     lib = _lib.load()
     for k, name in enumerate(("nf_tree_attention_status", "nf_verify_drafts_status", "nf_cache_pages_status",
-                              "nf_tree_attention_tc_status"), 1):
+                              "nf_tree_attention_tc_status", "nf_tree_attention_mma_status"), 1):
         v = int(getattr(lib, name)())
         if v:
             return k * 1000000 + v

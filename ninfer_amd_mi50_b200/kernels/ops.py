@@ -124,7 +124,7 @@ TUNING = {
     "moe_stream_shared_max_tokens": 16,
     "moe_stream_smem_kb": 192,
     "adapter": "auto",            # "simt" | "auto": "simt" takes the shared product apart from the adapters
-    "tree_attention": "auto",     # "simt" | "auto": "simt" keeps bfloat16 trees on the CUDA cores
+    "tree_attention": "auto",     # or the form for every call: 0 CUDA cores, 1 tcgen05, 2 mma.sync
     "adapter_f32_max_rows": 64,   # float32 rows that the kernel with the shared product in it serves
 }
 

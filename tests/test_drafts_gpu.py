@@ -22,6 +22,18 @@ def attend(c, heads, page_size, dtype, scale, out=None, qkv=None):
                                   c["mask"].cuda(), c["longest"], scale, out=out)
 
 
+@pytest.fixture(params=["auto", 1, 2], ids=["auto", "tcgen05", "mma"])
+def form(request):
+    """The forms of the bfloat16 attention, each for every size that it takes."""
+    kernels.TUNING["tree_attention"] = request.param
+    yield request.param
+    kernels.TUNING["tree_attention"] = "auto"
+
+
+def taken(form, heads, page_size, dtype=torch.bfloat16):
+    return form == "auto" or (dtype == torch.bfloat16 and heads[2] in (64, 128) and page_size % 16 == 0 and (form == 2 or page_size in (16, 32, 64, 128)))
+
+
 def near(got, want, weight, size, keys, dtype, D):
     """The result's rounding is half a step of its size.  A weight is off by what its score and the largest one are off by,
     each (D + 2) roundings of half a step of float32 of the sum of |q||k|, by two steps of the exponential, and in bfloat16
@@ -59,8 +71,10 @@ SIZES = [
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("case", range(len(SIZES)))
-def test_attention(case, dtype):
+def test_attention(case, dtype, form):
     sizes, lengths, heads, ps = SIZES[case]
+    if not taken(form, heads, ps, dtype):
+        return
     c = make_attention(sizes, lengths, heads, ps, seed=case, shape="chain" if case % 3 == 0 else "tree", sharp=1.0 + case % 2)
     c["qkv"], c["pages"] = c["qkv"].to(dtype).float(), c["pages"].to(dtype).float()
     scale = 1 / math.sqrt(heads[2])
@@ -70,7 +84,7 @@ def test_attention(case, dtype):
 
 
 @pytest.mark.parametrize("heads,most,page_size", [((8, 8, 128), 40, 64), ((8, 8, 64), 40, 16), ((24, 2, 128), 40, 64), ((24, 2, 64), 30, 32), ((5, 1, 128), 64, 128)])
-def test_many_requests_of_many_lengths(heads, most, page_size):
+def test_many_requests_of_many_lengths(heads, most, page_size, form):
     """More work than there are SMs: each goes from request to request, with one tile of rows and with two."""
     for seed in range(3):
         rnd = random.Random(seed)
@@ -81,7 +95,9 @@ def test_many_requests_of_many_lengths(heads, most, page_size):
         c["qkv"], c["pages"] = c["qkv"].bfloat16().float(), c["pages"].bfloat16().float()
         got = attend(c, heads, page_size, torch.bfloat16, 0.1)
         kernels.check_status()
+        kernels.TUNING["tree_attention"] = "auto"
         want = attend(c, heads, page_size, torch.float32, 0.1).double()
+        kernels.TUNING["tree_attention"] = form
         # (against the float32 form, which the plain one was compared with: a weight's rounding and the result's, of values below 6)
         assert float((got.double() - want).abs().max()) <= 6 * 2.0 ** -8 * 2 + 1e-4
         for s in rnd.sample(range(30), 4):        # and some requests against the plain form
@@ -92,7 +108,9 @@ def test_many_requests_of_many_lengths(heads, most, page_size):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("heads,length", [((4, 2, 64), 0), ((8, 1, 128), 37), ((2, 2, 48), 130), ((16, 1, 128), 600)])
-def test_any_mask_and_rows_that_see_nothing(heads, length, dtype):
+def test_any_mask_and_rows_that_see_nothing(heads, length, dtype, form):
+    if not taken(form, heads, 16, dtype):
+        return
     sizes = [21, 40]
     c = make_attention(sizes, [length, 0], heads, 16, seed=5)
     g = torch.Generator().manual_seed(1)
@@ -107,7 +125,9 @@ def test_any_mask_and_rows_that_see_nothing(heads, length, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("heads,length", [((4, 2, 64), 17), ((8, 1, 128), 700), ((2, 1, 32), 100)])
-def test_rows_without_a_request_stay_and_what_lies_behind_the_nodes_is_not_looked_at(heads, length, dtype):
+def test_rows_without_a_request_stay_and_what_lies_behind_the_nodes_is_not_looked_at(heads, length, dtype, form):
+    if not taken(form, heads, 16, dtype):
+        return
     c = make_attention([5, 9, 3], [length, 3, length], heads, 16, seed=2)
     c["row0"] = [0, 5, 14, 14]                                # the last rows belong to nobody
     c["qkv"], c["pages"] = c["qkv"].to(dtype).float(), c["pages"].to(dtype).float()
@@ -151,14 +171,18 @@ def test_a_loose_bound_and_other_requests_change_little():
 def test_same_bits_every_time():
     heads = (28, 4, 128)
     c = make_attention([33, 60], [3000, 1111], heads, 64, seed=4)
-    for dtype in (torch.float32, torch.bfloat16):
+    for form, dtype in (("auto", torch.float32), (0, torch.bfloat16), (1, torch.bfloat16), (2, torch.bfloat16)):
+        kernels.TUNING["tree_attention"] = form
         first = attend(c, heads, 64, dtype, 0.09)
         assert all(torch.equal(first, attend(c, heads, 64, dtype, 0.09)) for _ in range(5))
+    kernels.TUNING["tree_attention"] = "auto"
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
-def test_pages_outside_the_pool_and_rows_that_do_not_fit_are_reported(dtype):
+def test_pages_outside_the_pool_and_rows_that_do_not_fit_are_reported(dtype, form):
     heads = (4, 2, 64)
+    if not taken(form, heads, 16, dtype):
+        return
     for what in ("page", "page beyond", "context", "row0", "length", "table"):
         c = make_attention([4, 6], [40, 90], heads, 16, seed=6)
         if what == "page":
