@@ -53,9 +53,9 @@ struct __align__(8) Ring {
 };
 
 template <int D> constexpr int stage_bytes() { return 2 * kStageKeys * D * 2; }
-// the ring, at the end the warps' sums [4][rows][D + 4] in its place; queries; maxima and sums; barriers
+// the ring, at the end the warps' sums [4][rows][4 lanes][D / 4 + 4] in its place; queries; maxima and sums; barriers
 template <int D, int MT> constexpr size_t smem_bytes() {
-  const size_t ring = (size_t)kStages * stage_bytes<D>(), sums = (size_t)kGroups * 16 * MT * (D + 4) * 4;
+  const size_t ring = (size_t)kStages * stage_bytes<D>(), sums = (size_t)kGroups * 16 * MT * (D + 16) * 4;
   return 1024 + (ring > sums ? ring : sums) + 16 * MT * D * 2 + kGroups * 16 * MT * sizeof(float2) + sizeof(Ring);
 }
 
@@ -64,7 +64,7 @@ template <int D, int MT>
 __global__ void __launch_bounds__(kThreads, 2)
 tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ TreeArgs a, int box_rows,
                           const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ out) {
-  constexpr int ROWS = 16 * MT, PIECES = D / 8, ATOMS = D / 64, SB = stage_bytes<D>(), OS = D + 4, AB = kStageKeys * 128;     // AB: 64 numbers of the stage's keys
+  constexpr int ROWS = 16 * MT, PIECES = D / 8, ATOMS = D / 64, SB = stage_bytes<D>(), OL = D / 4 + 4, OS = 4 * OL, AB = kStageKeys * 128;     // AB: 64 numbers of the stage's keys
   constexpr size_t kRing = (size_t)kStages * SB, kSums = (size_t)kGroups * ROWS * OS * 4;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);          // (an offset, so that what lies here is known to be shared memory)
@@ -221,17 +221,28 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int h = 0; h < 2; ++h) raise |= top[m][h] * sc2 > m_run[m][h] + kRaise;     // (nothing so far: -inf, which any score passes)
-        if (__any_sync(0xffffffffu, raise)) {                // seldom: once for the first keys, as a rule
+        if (__any_sync(0xffffffffu, raise)) {                // seldom: for the first keys, as a rule, when there is nothing to rescale
+          float keep[MT][2];
+          bool more = false;
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float up = fmaxf(top[m][h] * sc2, m_run[m][h]), keep = up == -INFINITY ? 1.f : ex2(m_run[m][h] - up);
+              const float up = fmaxf(top[m][h] * sc2, m_run[m][h]);
+              more |= l_run[m][h] != 0.f;
+              keep[m][h] = up == -INFINITY ? 1.f : ex2(m_run[m][h] - up);
               m_run[m][h] = up;
-              l_run[m][h] *= keep;
-#pragma unroll
-              for (int n = 0; n < D / 8; ++n) o[m][n][2 * h] *= keep, o[m][n][2 * h + 1] *= keep;
             }
+          if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                l_run[m][h] *= keep[m][h];
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) o[m][n][2 * h] *= keep[m][h], o[m][n][2 * h + 1] *= keep[m][h];
+              }
+          }
         }
         unsigned w[MT][4];
 #pragma unroll
@@ -267,7 +278,8 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
         for (unsigned n = 0; n < (1u << 20); ++n)
           if (mbar_try(&ring->full[i % kStages], (i / kStages) & 1)) break;
   }
-  // the four warps' sums of a row, at its largest reference, one beside the other
+  // the four warps' sums of a row, one beside the other: each lane's numbers together, so that they go in few instructions
+  // (what a CTA runs once costs it the fetch of its code, some 14 cycles an instruction)
   float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -278,47 +290,50 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if (t4 == 0) stat[group * ROWS + 16 * m + quad + 8 * h] = make_float2(m_run[m][h], l);
     }
-  __syncthreads();                                           // (also: all have done with the ring)
+  __syncthreads();                                           // all have done with the ring
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = 16 * m + quad + 8 * h;
-      float top = -INFINITY;
+      const unsigned to = smem_u32(smem) + 4 * ((group * ROWS + 16 * m + quad + 8 * h) * OS + t4 * OL);
 #pragma unroll
-      for (int w = 0; w < kGroups; ++w) top = fmaxf(top, stat[w * ROWS + row].x);
-      const float f = top == -INFINITY ? 0.f : ex2(m_run[m][h] - top);
-      float* to = sums + ((size_t)group * ROWS + row) * OS + 2 * t4;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(to + 8 * n) = make_float2(o[m][n][2 * h] * f, o[m][n][2 * h + 1] * f);
+      for (int n = 0; n < D / 8; n += 2)
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + 8 * n), "f"(o[m][n][2 * h]), "f"(o[m][n][2 * h + 1]), "f"(o[m][n + 1][2 * h]),
+                     "f"(o[m][n + 1][2 * h + 1]) : "memory");
     }
   __syncthreads();
   const bool whole = r.keys <= a.chunk;
-  constexpr int LANES = D / 4;                               // of a row, four numbers each
-#pragma unroll 2
+  constexpr int LANES = D / 4;                               // of a row, four numbers each: two of 16 j + 2 t, two of 8 further on
+  const int ot = threadIdx.x % LANES / (LANES / 4), oj = threadIdx.x % (LANES / 4);
+#pragma unroll 1
   for (int row = threadIdx.x / LANES; row < ROWS; row += kThreads / LANES) {
-    const int p = pair0 + row, d = threadIdx.x % LANES * 4;
+    const int p = pair0 + row, d = 16 * oj + 2 * ot;
     if (p >= pairs) break;
-    float4 v[kGroups];
     float2 st[kGroups];
+    float4 v[kGroups];
 #pragma unroll
     for (int w = 0; w < kGroups; ++w) {
-      v[w] = *reinterpret_cast<const float4*>(sums + ((size_t)w * ROWS + row) * OS + d);
       st[w] = stat[w * ROWS + row];
+      v[w] = *reinterpret_cast<const float4*>(sums + ((size_t)w * ROWS + row) * OS + ot * OL + 4 * oj);
     }
     const float top = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), base = top == -INFINITY ? 0.f : top;
     float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kGroups; ++w) l = fmaf(ex2(st[w].x - base), st[w].y, l);
-    float4 x = make_float4((v[0].x + v[1].x) + (v[2].x + v[3].x), (v[0].y + v[1].y) + (v[2].y + v[3].y), (v[0].z + v[1].z) + (v[2].z + v[3].z),
-                           (v[0].w + v[1].w) + (v[2].w + v[3].w));
+    for (int w = 0; w < kGroups; ++w) {
+      const float f = ex2(st[w].x - base);
+      l = fmaf(f, st[w].y, l);
+      x.x = fmaf(f, v[w].x, x.x), x.y = fmaf(f, v[w].y, x.y), x.z = fmaf(f, v[w].z, x.z), x.w = fmaf(f, v[w].w, x.w);
+    }
     const size_t to = (size_t)(r.row0 + p / G) * a.Hq + g * G + p % G;
     if (whole) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      *reinterpret_cast<uint2*>(out + to * D + d) = make_uint2(pack(x.x * inv, x.y * inv), pack(x.z * inv, x.w * inv));
+      *reinterpret_cast<unsigned*>(out + to * D + d) = pack(x.x * inv, x.y * inv);
+      *reinterpret_cast<unsigned*>(out + to * D + d + 8) = pack(x.z * inv, x.w * inv);
     } else {
       const size_t ws = (size_t)blockIdx.x * a.T * a.Hq + to;
-      *reinterpret_cast<float4*>(a.ws_acc + ws * D + d) = x;
+      *reinterpret_cast<float2*>(a.ws_acc + ws * D + d) = make_float2(x.x, x.y);
+      *reinterpret_cast<float2*>(a.ws_acc + ws * D + d + 8) = make_float2(x.z, x.w);
       if (d == 0) reinterpret_cast<float2*>(a.ws_ml)[ws] = make_float2(top, l);
     }
   }
@@ -343,9 +358,14 @@ int tree_mma_rows(int S, int T, int Hq, int Hkv) { return (long long)T * (Hq / H
 
 int tree_mma_chunk(int S, int T, int Hq, int Hkv, int max_context) {
   const long long pairs = ((long long)T * (Hq / Hkv) + S - 1) / S, rows = tree_mma_rows(S, T, Hq, Hkv);
-  const long long ctas = (pairs + rows - 1) / rows * S * Hkv, shares = std::max(1ll, (148 * 4 + ctas - 1) / ctas);
-  const long long chunk = ((max_context + shares - 1) / shares + 127) / 128 * 128;
-  return (int)chunk;
+  const long long ctas = (pairs + rows - 1) / rows * S * Hkv;
+  const auto keys = [&](long long shares) { return ((max_context + shares - 1) / shares + 127) / 128 * 128; };
+  // as many shares as have room at once, of 384 keys at least: with fewer what a CTA does once is the most of it (one row
+  // of 16 heads behind 8,192 keys in shares of 256, 512 and 1,024 keys: 23.5, 17.7 and 23.2 us).  Long shares in some more,
+  // since requests are not of one length (8 requests of 32 nodes behind up to 8,192 keys in 2, 5 and 8 shares: 99, 89, 96)
+  long long chunk = keys(std::max(1ll, 296 / ctas));
+  if (chunk > 2048) chunk = keys(std::max(1ll, (5 * 148 + ctas - 1) / ctas));
+  return (int)std::max(384ll, chunk);
 }
 
 int launch_tree_mma(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
