@@ -7,7 +7,8 @@ decode_batch(sessions, tokens) / sample(...) / close()`` and ``Session`` with
 ``src/api/ninfer_c_api.h:32-82``.  Names, argument order, defaults and meanings are kept
 (``gpus``, ``quant`` and ``parallel`` are gone: one GPU, no quantisation); logits come back
 as NumPy float32 arrays instead of Python lists.  Added: ``step`` (a mixed batch with
-chosen logit rows), ``generate`` (the scheduler), ``stats``, ``pages_free``.
+chosen logit rows), ``generate`` (the scheduler), ``stats``, ``pages_free``, ``Session.fork``, and ``Session.decode_tree`` with
+``Session.accept`` (several continuations in one step).
 
     from ninfer_amd_mi50_b200.api import Ninfer
     eng = Ninfer("/path/to/Qwen1.5-MoE-A2.7B", num_sequences=4)
@@ -26,7 +27,7 @@ import numpy as np
 import torch
 
 from .config.engine_options import EngineOptions
-from .engine.batch import StepEntry
+from .engine.batch import StepEntry, TreeEntry
 from .engine.engine import Engine
 from .sampling.params import SamplingParams
 from .sampling.sampler import check_rules, sample_reference, uniform_draw
@@ -87,6 +88,29 @@ class Session:
 
     def decode(self, token: int) -> np.ndarray:
         return self._engine._runner.step([StepEntry(self._key, [int(token)], [0], self._adapter)])[0].cpu().numpy()
+
+    def fork(self) -> "Session":
+        """A session that goes on from where this one is, each on its own from here.  Their filled cache pages are shared."""
+        s = Session.__new__(Session)
+        s._engine, s._key, s._adapter = self._engine, ("session", next(self._engine._keys)), self._adapter
+        try:
+            self._engine._runner.fork(self._key, s._key)
+        except Exception as e:
+            s._open, s._adapter = False, -1
+            raise NinferError(f"fork: {e}") from None
+        s._open = True
+        if s._adapter >= 0:
+            self._engine._runner.adapters.hold(s._adapter)
+        return s
+
+    def decode_tree(self, tokens: Sequence[int], parents: Optional[Sequence[int]] = None) -> np.ndarray:
+        """Run a tree of drafted tokens behind the session: tokens[0] is the newest token, tokens[i] hangs on node parents[i]
+        (parents[0] is not read; left out, each on the one before) -> logits [nodes, vocab].  Nothing is kept until `accept`."""
+        return self._engine.decode_trees([(self, tokens, parents)])
+
+    def accept(self, path: Sequence[int] = ()) -> None:
+        """Keep the last tree's root and the nodes of `path` behind it, from the root's child down."""
+        self._engine._runner.accept({self._key: list(path)})
 
     def close(self) -> None:
         if self._open:
@@ -179,6 +203,11 @@ class Ninfer:
             raise NinferError("decode_batch: sessions and tokens differ in length")
         out = self._runner.step([StepEntry(s._key, [int(t)], [0], s._adapter) for s, t in zip(sessions, tokens)])
         return out.cpu().numpy()
+
+    def decode_trees(self, trees: Sequence[tuple]) -> np.ndarray:
+        """One step of trees of drafted tokens, ``(session, tokens, parents)`` each (`Session.decode_tree`) -> logits of all
+        nodes, tree by tree."""
+        return self._runner.tree_step([TreeEntry(s._key, list(t), p, s._adapter) for s, t, p in trees]).cpu().numpy()
 
     def step(self, entries: Sequence[tuple]) -> np.ndarray:
         """A mixed batch: ``(session, tokens, want)`` triples -> logits [wanted rows, vocab]."""

@@ -131,6 +131,48 @@ class CacheManager:
         self.requests[req] = RequestEntry(slot, tables=[[] for _ in self.groups], rows=self._slot_rows[slot])
         return slot
 
+    def fork(self, req: Hashable, new: Hashable) -> int:
+        """Admit `new` as a request that has come as far as `req`: the same length, pages that are filled shared, the one
+        that is filled in part copied (each goes on writing in its own), state slots copied.  Returns the new slot; where a
+        slot or a page is missing nothing has changed.
+
+        A shared page is never written again: a request writes from its length on, and these lie before it."""
+        ent = self.requests[req]
+        full, rest = divmod(ent.length, self.page_size)
+        if rest and any(len(t) > full and t[full] >= 0 and not g.pool.num_free for g, t in zip(self.groups, ent.tables)):
+            raise OutOfPages(f"request {new!r}: no page free for what {req!r} has filled in part")
+        slot = self.open(new)
+        other = self.requests[new]
+        for g, table, to, row in zip(self.groups, ent.tables, other.tables, other.rows):
+            kept = table[:full]
+            g.pool.share([p for p in kept if p >= 0])
+            to.extend(kept)
+            if rest and len(table) > full:
+                if table[full] >= 0:
+                    taken, _ = g.pool.take_marking_reuse(1)
+                    to.extend(taken)
+                    self._copy_page(g, table[full], taken[0])
+                else:
+                    to.append(-1)
+            row[:len(to)] = to
+        other.length = ent.length
+        other.reserved = ent.length
+        for slab in self.state.values():
+            slab[slot].copy_(slab[ent.slot])
+        return slot
+
+    @staticmethod
+    def _copy_page(g: CacheGroup, src: int, dst: int) -> None:
+        """All of it, so that what lies behind the request's last row is finite in the copy too."""
+        if g.pages is None:
+            return
+        if g.pages.is_cuda:
+            from .. import kernels
+            at = torch.tensor([src, dst], dtype=torch.int32).pin_memory().to(g.pages.device, non_blocking=True)
+            kernels.copy_pages(g.pages, at[:1], at[1:])
+        else:
+            g.pages[:, dst] = g.pages[:, src]
+
     def close(self, req: Hashable) -> None:
         """Give back everything the request holds."""
         ent = self.requests.pop(req)
@@ -269,14 +311,19 @@ class CacheManager:
     def check(self) -> None:
         for gi, g in enumerate(self.groups):
             g.pool.check()
-            seen = {}
+            seen: Dict[int, List[Hashable]] = {}
             for req, ent in self.requests.items():
-                for p in ent.tables[gi]:
+                for i, p in enumerate(ent.tables[gi]):
                     if p < 0:
                         continue
-                    if p in seen:
-                        raise AssertionError(f"page {p} of group {gi} held by {seen[p]!r} and {req!r}")
-                    seen[p] = req
+                    seen.setdefault(p, []).append(req)
+                    if len(seen[p]) > g.pool.holders(p):
+                        raise AssertionError(f"page {p} of group {gi} held by {seen[p][0]!r} and {req!r}")
+                    if g.pool.holders(p) > 1 and (i + 1) * self.page_size > ent.length:
+                        raise AssertionError(f"page {p} of group {gi} is shared, and {req!r} may still write to it")
+            for p, who in seen.items():
+                if len(who) != g.pool.holders(p):
+                    raise AssertionError(f"page {p} of group {gi} has {g.pool.holders(p)} holders, {len(who)} found in block tables")
             if len(seen) != g.pool.num_held:
                 raise AssertionError(f"group {gi}: {g.pool.num_held} pages held, "
                                      f"{len(seen)} found in block tables (a page was lost)")

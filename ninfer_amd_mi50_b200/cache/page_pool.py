@@ -3,7 +3,8 @@
 The reference has no pages: each sequence owns a slab of ``max_context`` positions
 (src/runtime/kv_cache.cpp:14-22) and slots are handed out round-robin and never freed
 (src/api/ninfer_c_api.cpp:150).  Here pages are taken and given back one by one; a page
-just freed is the next one handed out, so reuse happens as early as it can.
+just freed is the next one handed out, so reuse happens as early as it can.  A page may have several holders (the pages that
+forked requests share): it is free again when the last has given it back.
 """
 
 from __future__ import annotations
@@ -21,7 +22,7 @@ class PagePool:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = int(num_pages)
         self._free: List[int] = list(range(self.num_pages - 1, -1, -1))  # pop() gives page 0 first
-        self._held = [False] * self.num_pages
+        self._held = [0] * self.num_pages            # holders of each page
         self._used_before = [False] * self.num_pages
 
     @property
@@ -42,7 +43,7 @@ class PagePool:
         for p in out:
             if self._held[p]:
                 raise AssertionError(f"page {p} handed out while held")
-            self._held[p] = True
+            self._held[p] = 1
         return out
 
     def take_marking_reuse(self, n: int):
@@ -54,14 +55,25 @@ class PagePool:
             self._used_before[p] = True
         return out, again
 
+    def share(self, pages) -> None:
+        """One more holder for each of these pages, which are held."""
+        for p in pages:
+            if not (0 <= p < self.num_pages and self._held[p]):
+                raise AssertionError(f"page {p} is shared while nobody holds it")
+            self._held[p] += 1
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
+
     def give_back(self, pages) -> None:
         for p in pages:
             if not 0 <= p < self.num_pages:
                 raise AssertionError(f"page {p} does not belong to this pool")
             if not self._held[p]:
                 raise AssertionError(f"page {p} freed twice")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
 
     def check(self) -> None:
         """Every page is either free or held, never both, never neither."""
@@ -69,5 +81,5 @@ class PagePool:
         if len(free) != len(self._free):
             raise AssertionError("a page is on the free stack twice")
         for p in range(self.num_pages):
-            if self._held[p] == (p in free):
+            if self._held[p] < 0 or bool(self._held[p]) == (p in free):
                 raise AssertionError(f"page {p}: held={self._held[p]} and free={p in free}")

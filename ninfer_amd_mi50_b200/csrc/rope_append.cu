@@ -24,11 +24,11 @@ rope_append_kernel(T* __restrict__ qkv, const float* __restrict__ bias,
                    const int* __restrict__ positions, const int* __restrict__ row_seg,
                    const float* __restrict__ inv_freq, int rot, int Hq, int Hkv, int D,
                    T* __restrict__ pages, const int* __restrict__ block_table, int bt_width,
-                   int page_size, int num_pages, int append) {
+                   int page_size, int num_pages, int append, const int* __restrict__ places) {
   extern __shared__ float cs[];            // [rot/2] cos, [rot/2] sin
   const int t = blockIdx.x;
   const int half = rot / 2;
-  const int pos = positions[t];
+  const int pos = positions[t], place = places ? places[t] : pos;
   const float fpos = (float)pos;
   for (int i = threadIdx.x; i < half; i += blockDim.x) {
     const float angle = fpos * inv_freq[i];
@@ -42,10 +42,10 @@ rope_append_kernel(T* __restrict__ qkv, const float* __restrict__ bias,
   T* kdst = nullptr;
   if (append) {
     const int seg = row_seg[t];
-    const int lp = pos / page_size;
-    const int page = (lp >= 0 && lp < bt_width) ? block_table[(size_t)seg * bt_width + lp] : -1;
+    const int lp = place / page_size;
+    const int page = (lp >= 0 && lp < bt_width && place >= 0) ? block_table[(size_t)seg * bt_width + lp] : -1;
     if (page >= 0 && page < num_pages)       // no page reserved: never write out of bounds
-      kdst = pages + ((size_t)page * 2 * Hkv * page_size + (size_t)(pos - lp * page_size)) * D;
+      kdst = pages + ((size_t)page * 2 * Hkv * page_size + (size_t)(place - lp * page_size)) * D;
   }
   const size_t kv_head_stride = (size_t)page_size * D;
   const int slots = D / 2;
@@ -89,13 +89,13 @@ rope_append_bf16x8_kernel(const float* __restrict__ sums, __nv_bfloat16* __restr
                           const int* __restrict__ positions, const int* __restrict__ row_seg,
                           const float* __restrict__ inv_freq, int Hq, int Hkv, int D,
                           __nv_bfloat16* __restrict__ pages, const int* __restrict__ block_table,
-                          int bt_width, int page_size, int num_pages, int append) {
+                          int bt_width, int page_size, int num_pages, int append, const int* __restrict__ places) {
   extern __shared__ __align__(16) float cs[];            // [D/2] cos, [D/2] sin
   const int t = blockIdx.x;
   const int half = D / 2;
   chain_release();
-  chain_wait(sums, qkv, positions, row_seg, block_table);
-  const int pos = positions[t];
+  chain_wait(sums, qkv, positions, row_seg, block_table, places);
+  const int pos = positions[t], place = places ? places[t] : pos;
   const int W = (Hq + 2 * Hkv) * D;
   __nv_bfloat16* x = qkv + (size_t)t * W;
   const float* xs = SUMS ? sums + (size_t)t * W : nullptr;
@@ -136,10 +136,10 @@ rope_append_bf16x8_kernel(const float* __restrict__ sums, __nv_bfloat16* __restr
       }
       if (append) {
         const int seg = row_seg[t];
-        const int lp = pos / page_size;
-        const int page = (lp >= 0 && lp < bt_width) ? block_table[(size_t)seg * bt_width + lp] : -1;
+        const int lp = place / page_size;
+        const int page = (lp >= 0 && lp < bt_width && place >= 0) ? block_table[(size_t)seg * bt_width + lp] : -1;
         if (page >= 0 && page < num_pages)
-          kdst = pages + ((size_t)page * 2 * Hkv * page_size + (size_t)(pos - lp * page_size)) * D;
+          kdst = pages + ((size_t)page * 2 * Hkv * page_size + (size_t)(place - lp * page_size)) * D;
       }
       __syncthreads();
       have_table = true;
@@ -194,10 +194,12 @@ rope_append_bf16x8_kernel(const float* __restrict__ sums, __nv_bfloat16* __restr
 
 using namespace nf;
 
-extern "C" int nf_rope_append(void* qkv, const float* bias, const int* positions, const int* row_seg,
+// `places` int32 [T] or null: where in the request's cache each row's keys and values go, if not to its position (rows that
+// are a tree are turned by their depth and lie one behind the other).
+static int rope_append_at(void* qkv, const float* bias, const int* positions, const int* row_seg,
                               const float* inv_freq, int rot, int T, int Hq, int Hkv, int D,
                               void* pages, const int* block_table, int bt_width, int page_size,
-                              int num_pages, int append, int dtype, cudaStream_t stream) {
+                              int num_pages, int append, int dtype, const int* places, cudaStream_t stream) {
   if (T == 0) return 0;
   NF_REQUIRE(T > 0 && Hq > 0 && Hkv > 0 && D > 0, "rope_append: bad sizes T=%d Hq=%d Hkv=%d D=%d", T, Hq, Hkv, D);
   NF_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0, "rope_append: rotary width %d must be even and <= head_dim %d", rot, D);
@@ -208,14 +210,28 @@ extern "C" int nf_rope_append(void* qkv, const float* bias, const int* positions
   NF_REQUIRE(smem <= 48 * 1024, "rope_append: rotary width %d too large", rot);
   if (dtype == kBF16 && rot == D && D % 16 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)pages % 16 == 0 &&
       (uintptr_t)bias % 16 == 0) {
-    launch_chained(rope_append_bf16x8_kernel<false>, dim3(T), dim3(256), smem, stream, (const float*)nullptr, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
+    launch_chained(rope_append_bf16x8_kernel<false>, dim3(T), dim3(256), smem, stream, (const float*)nullptr, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append, places);
     return check_launch("rope_append");
   }
   if (dtype == kF32)
-    rope_append_kernel<float><<<T, 256, smem, stream>>>((float*)qkv, bias, positions, row_seg, inv_freq, rot, Hq, Hkv, D, (float*)pages, block_table, bt_width, page_size, num_pages, append);
+    rope_append_kernel<float><<<T, 256, smem, stream>>>((float*)qkv, bias, positions, row_seg, inv_freq, rot, Hq, Hkv, D, (float*)pages, block_table, bt_width, page_size, num_pages, append, places);
   else
-    rope_append_kernel<__nv_bfloat16><<<T, 256, smem, stream>>>((__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, rot, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
+    rope_append_kernel<__nv_bfloat16><<<T, 256, smem, stream>>>((__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, rot, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append, places);
   return check_launch("rope_append");
+}
+
+extern "C" int nf_rope_append(void* qkv, const float* bias, const int* positions, const int* row_seg, const float* inv_freq, int rot, int T,
+                              int Hq, int Hkv, int D, void* pages, const int* block_table, int bt_width, int page_size, int num_pages,
+                              int append, int dtype, cudaStream_t stream) {
+  return rope_append_at(qkv, bias, positions, row_seg, inv_freq, rot, T, Hq, Hkv, D, pages, block_table, bt_width, page_size, num_pages, append,
+                        dtype, nullptr, stream);
+}
+
+extern "C" int nf_rope_append_at(void* qkv, const float* bias, const int* positions, const int* row_seg, const float* inv_freq, int rot, int T,
+                                 int Hq, int Hkv, int D, void* pages, const int* block_table, int bt_width, int page_size, int num_pages,
+                                 int append, int dtype, const int* places, cudaStream_t stream) {
+  return rope_append_at(qkv, bias, positions, row_seg, inv_freq, rot, T, Hq, Hkv, D, pages, block_table, bt_width, page_size, num_pages, append,
+                        dtype, places, stream);
 }
 
 // The same from float32 sums [T, W] to bfloat16 qkv (its query columns) and pages; the rotation covers the whole head.
@@ -229,6 +245,6 @@ extern "C" int nf_rope_append_sums(const float* sums, void* qkv, const float* bi
              "rope_append_sums: operands must be 16-byte aligned");
   const size_t smem = (size_t)D * sizeof(float);
   NF_REQUIRE(smem <= 48 * 1024, "rope_append_sums: head_dim %d too large", D);
-  launch_chained(rope_append_bf16x8_kernel<true>, dim3(T), dim3(256), smem, stream, sums, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append);
+  launch_chained(rope_append_bf16x8_kernel<true>, dim3(T), dim3(256), smem, stream, sums, (__nv_bfloat16*)qkv, bias, positions, row_seg, inv_freq, Hq, Hkv, D, (__nv_bfloat16*)pages, block_table, bt_width, page_size, num_pages, append, (const int*)nullptr);
   return check_launch("rope_append_sums");
 }

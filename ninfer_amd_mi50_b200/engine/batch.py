@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheManager
-from ..parts.base import StepContext
+from ..parts.base import StepContext, TreeRows
 
 
 @dataclass
@@ -26,6 +26,16 @@ class StepEntry:
     tokens: Sequence[int]
     want: Sequence[int] = ()      # indices into `tokens` whose logits are asked for
     adapter: int = -1             # slot of the request's adapter, -1: none
+
+
+@dataclass
+class TreeEntry:
+    """A tree of drafted tokens behind a request's newest one: node 0, whose parent is not read.  Other nodes have parents
+    among the nodes before them; left out, each hangs on the one before."""
+    req: Hashable
+    tokens: Sequence[int]
+    parents: Optional[Sequence[int]] = None
+    adapter: int = -1
 
 
 class BatchError(ValueError):
@@ -123,3 +133,35 @@ def pack_step(entries: Sequence[StepEntry], cache: CacheManager, dtype: torch.dt
     for (gi, width, _), t in zip(tables, parts[7:]):
         ctx.block_tables[gi] = t.view(S, width)
     return ctx
+
+
+def tree_parents(e: TreeEntry, most: int) -> List[int]:
+    """The parents of an entry's nodes, -1 for the root; raises `BatchError` where they are no tree."""
+    n = len(e.tokens)
+    if n > most:
+        raise BatchError(f"request {e.req!r}: a tree of {n} nodes; {most} are the most")
+    parents = [-1] + list(range(n - 1)) if e.parents is None else [-1] + [int(p) for p in e.parents[1:]]
+    if len(parents) != n or any(not 0 <= p < i for i, p in enumerate(parents) if i):
+        raise BatchError(f"request {e.req!r}: {parents} are not the parents of {n} nodes, each after its own")
+    return parents
+
+
+def tree_rows(lengths: Sequence[int], trees: Sequence[Sequence[int]], device: torch.device) -> TreeRows:
+    """Positions by depth and who sees whom, for requests that held `lengths` tokens; one copy to the device."""
+    words = (max(len(p) for p in trees) + 31) // 32
+    positions: List[int] = []
+    masks: List[bytes] = []
+    for held, parents in zip(lengths, trees):
+        depth, seen = [0] * len(parents), [0] * len(parents)
+        for i, p in enumerate(parents):
+            if i:
+                depth[i], seen[i] = depth[p] + 1, seen[p]
+            seen[i] |= 1 << i
+            masks.append(seen[i].to_bytes(4 * words, "little"))
+        positions += [held + d for d in depth]
+    flat = np.concatenate([np.asarray(positions, dtype=np.int32), np.frombuffer(b"".join(masks), dtype="<i4").astype(np.int32)])
+    buf = torch.from_numpy(flat)
+    if device.type == "cuda":
+        buf = buf.pin_memory().to(device, non_blocking=True)
+    T = len(positions)
+    return TreeRows(buf[:T], buf[T:].view(T, words))

@@ -10,14 +10,14 @@ for.  It runs only the tokens it is given; everything earlier comes from the cac
 
 from __future__ import annotations
 
-from typing import Dict, Hashable, List, Optional, Sequence
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import torch
 
 from ..cache.manager import CacheManager
 from ..cache.page_pool import OutOfPages
 from ..parts.model import DecoderModel
-from .batch import BatchError, StepEntry, pack_step, validate_entries
+from .batch import BatchError, StepEntry, TreeEntry, pack_step, tree_parents, tree_rows, validate_entries
 
 
 class ModelRunner:
@@ -27,6 +27,7 @@ class ModelRunner:
         self.device = torch.device(device)
         self.graphs = None
         self.adapters = None          # the bank of adapters, where the engine keeps one
+        self.trees: Dict[Hashable, Tuple[int, List[int]]] = {}        # requests whose last step was a tree: tokens held before it, parents
         if use_graph and self.device.type == "cuda" and model.graph_safe:
             from .graphs import DecodeGraphs
             self.graphs = DecodeGraphs(self, cache.max_requests)
@@ -39,7 +40,12 @@ class ModelRunner:
         return self.cache.open(req)
 
     def close(self, req: Hashable) -> None:
+        self.trees.pop(req, None)
         self.cache.close(req)
+
+    def fork(self, req: Hashable, new: Hashable) -> int:
+        """Admit `new` as a request that goes on from where `req` is (`CacheManager.fork`)."""
+        return self.cache.fork(req, new)
 
     # ---- the step -------------------------------------------------------------------
     def reserve(self, entries: Sequence[StepEntry]) -> None:
@@ -64,12 +70,9 @@ class ModelRunner:
         if not entries:
             return torch.empty((0, self.model.vocab_size), dtype=torch.float32, device=self.device)
         arrays = validate_entries(entries, self.cache, self.model.vocab_size)
-        adapted = False
+        adapted = self._check_adapters(entries)
         for e in entries:
-            if e.adapter != -1:
-                if self.adapters is None or e.adapter not in self.adapters.slots.values():
-                    raise BatchError(f"request {e.req!r}: no adapter in slot {e.adapter}")
-                adapted = True
+            self.trees.pop(e.req, None)        # (a tree that was not accepted: its rows are written over)
         self.reserve(entries)
         try:
             if self.graphs is not None and self.graphs.eligible(entries):
@@ -89,6 +92,78 @@ class ModelRunner:
         self.h2d_bytes += moved
         self.tokens_run += sum(len(e.tokens) for e in entries)
         return logits
+
+    def _check_adapters(self, entries: Sequence[StepEntry]) -> bool:
+        """Whether some entry has an adapter; raises for one that is not there."""
+        adapted = False
+        for e in entries:
+            if e.adapter != -1:
+                if self.adapters is None or e.adapter not in self.adapters.slots.values():
+                    raise BatchError(f"request {e.req!r}: no adapter in slot {e.adapter}")
+                adapted = True
+        return adapted
+
+    # ---- trees of drafted tokens ------------------------------------------------------
+    def tree_step(self, entries: Sequence[TreeEntry]) -> torch.Tensor:
+        """Run every entry's tree -> float32 logits [nodes, vocab], row by row behind each node.
+
+        Nothing is committed: `accept` says which path of the tree stands, and until then another step of the request
+        starts where this one did.  For models whose mixers see all earlier tokens (`DecoderModel.tree_safe`)."""
+        from .. import kernels
+        entries = list(entries)
+        if not self.model.tree_safe:
+            raise BatchError("this model has layers that cannot run a tree of drafted tokens (states, windows or neighbouring tokens)")
+        if not entries:
+            return torch.empty((0, self.model.vocab_size), dtype=torch.float32, device=self.device)
+        steps = [StepEntry(e.req, e.tokens, range(len(e.tokens)), e.adapter) for e in entries]
+        arrays = validate_entries(steps, self.cache, self.model.vocab_size)
+        parents = [tree_parents(e, kernels.MAX_TREE_NODES) for e in entries]
+        adapted = self._check_adapters(steps)
+        for e in entries:
+            self.trees.pop(e.req, None)
+        self.reserve(steps)
+        lengths = [self.cache.length(e.req) for e in entries]
+        try:
+            ctx = pack_step(steps, self.cache, self.dtype, self.device, arrays=arrays, adapted=adapted)
+            ctx.tree = tree_rows(lengths, parents, self.device)
+            logits = self.run(ctx)
+        except Exception:
+            for e in entries:
+                self.cache.truncate(e.req)
+            raise
+        for e, held, p in zip(entries, lengths, parents):
+            self.trees[e.req] = (held, p)
+        self.steps_run += 1
+        self.h2d_bytes += ctx.scratch.get("h2d_bytes", 0) + 4 * (ctx.tree.positions.numel() + ctx.tree.mask.numel())
+        self.tokens_run += sum(len(e.tokens) for e in entries)
+        return logits
+
+    def accept(self, paths: Dict[Hashable, Sequence[int]]) -> None:
+        """Commit, for each request, the root of its last tree and the nodes of `paths[req]` behind it, from the root's child
+        down (none: the root alone).  Their cache entries move up to where they would be had they been run in a line."""
+        from .. import kernels
+        for req, path in paths.items():
+            if req not in self.trees or self.trees[req][0] != self.cache.length(req):
+                raise BatchError(f"request {req!r}: its last step was not a tree")
+            parents, at = self.trees[req][1], 0
+            for node in path:
+                if not 0 < int(node) < len(parents) or parents[int(node)] != at:
+                    raise BatchError(f"request {req!r}: {list(path)} is not a path down its tree")
+                at = int(node)
+        moving = [req for req, path in paths.items() if any(int(p) != j + 1 for j, p in enumerate(path))]
+        if moving:
+            most = max(len(paths[r]) for r in moving)
+            rows = [[self.cache.length(r), len(paths[r])] + [int(p) for p in paths[r]] + [-1] * (most - len(paths[r])) for r in moving]
+            small = torch.tensor(rows, dtype=torch.int32)
+            lengths, accepted, path = (t.contiguous().to(self.device) for t in (small[:, 0], small[:, 1], small[:, 2:]))
+            for g in self.cache.groups:
+                width = max(len(self.cache.block_table(g.index, r)) for r in moving)
+                table = torch.from_numpy(self.cache.block_rows(g.index, [self.cache.slot(r) for r in moving], width)).to(self.device)
+                kernels.compact_cache(g.pages, table, lengths, path, accepted)
+        for req, path in paths.items():
+            del self.trees[req]
+            self.cache.commit(req, self.cache.length(req) + 1 + len(path))
+            self.cache.truncate(req)           # (pages that only nodes left behind had use for)
 
     def can_take_device_tokens(self, n_entries: int) -> bool:
         """Whether a step of `n_entries` single tokens would be replayed from a graph."""

@@ -4,8 +4,8 @@ the request held, and pages copied for a request that is forked.
 
 A step's nodes are rows, a request's rows lie together: `row0` int32 [S + 1] says where each request's begin.  Node 0 of a
 request is its tree's root, the newest token that it has; the others are drafted.  Keys and values of node i go into the
-request's pages at position lengths[s] + i, whatever its depth (`rope_append` with these positions and no rotation, after
-one that rotates by the depth and appends nothing).  Everything is on the device, so that a captured step serves any trees.
+request's pages at position lengths[s] + i, whatever its depth: `rope_append` turns them by their depth and takes these
+positions as `places`.  Everything is on the device, so that a captured step serves any trees.
 """
 
 from __future__ import annotations

@@ -491,8 +491,9 @@ def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, act=None) -> torch.T
 def rope_append(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: torch.Tensor,
                 row_seg: torch.Tensor, inv_freq: Optional[torch.Tensor], rotary_dim: int,
                 Hq: int, Hkv: int, D: int, pages: torch.Tensor, block_table: torch.Tensor,
-                page_size: int, append: bool) -> None:
-    """In place: qkv += bias; rotate q and k heads; write k, v to the cache pages."""
+                page_size: int, append: bool, places: Optional[torch.Tensor] = None) -> None:
+    """In place: qkv += bias; rotate q and k heads; write k, v to the cache pages, at the rows' positions or, where given, at
+    `places` (rows that are a tree of drafted tokens)."""
     _chk(qkv, "qkv"); _chk(pages, "pages", qkv.dtype); _chk(block_table, "block_table", torch.int32)
     _chk(positions, "positions", torch.int32); _chk(row_seg, "row_seg", torch.int32)
     if bias is not None:
@@ -501,6 +502,15 @@ def rope_append(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: torc
         _chk(inv_freq, "inv_freq", torch.float32)
     if qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError("rope_append: qkv width does not match the head counts")
+    if places is not None:
+        _chk(places, "places", torch.int32)
+        if places.numel() != qkv.shape[0]:
+            raise ValueError(f"rope_append: {places.numel()} places for {qkv.shape[0]} rows")
+        _lib.call("nf_rope_append_at", _p(qkv), _p(bias), _p(positions), _p(row_seg), _p(inv_freq),
+                  c_int(rotary_dim if inv_freq is not None else 0), c_int(qkv.shape[0]), c_int(Hq), c_int(Hkv), c_int(D), _p(pages),
+                  _p(block_table), c_int(block_table.shape[1]), c_int(page_size), c_int(pages.shape[0]), c_int(1 if append else 0), c_int(_dt(qkv)),
+                  _p(places), _stream())
+        return
     _lib.call("nf_rope_append", _p(qkv), _p(bias), _p(positions), _p(row_seg), _p(inv_freq),
               c_int(rotary_dim if inv_freq is not None else 0), c_int(qkv.shape[0]), c_int(Hq),
               c_int(Hkv), c_int(D), _p(pages), _p(block_table), c_int(block_table.shape[1]),

@@ -43,6 +43,10 @@ class PagedGqaAttention(Mixer):
         self.kv_width = self.num_kv_heads * self.head_dim
         self.w_qkv = self.b_qkv = self.w_o = None
 
+    @property
+    def tree_safe(self) -> bool:
+        return not self.window
+
     # ---- weights ----------------------------------------------------------------------
     def tensor_specs(self) -> List[TensorSpec]:
         p, H = self.prefix, self.hidden_size
@@ -86,6 +90,8 @@ class PagedGqaAttention(Mixer):
                 state: Optional[torch.Tensor]) -> torch.Tensor:
         assert cache is not None, "attention needs a cache slot"
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        if ctx.tree is not None:
+            return self._forward_tree(x, ctx, cache)
         table = self.position.rotary_table(x.device)
         bias = self.b_qkv
         if table is None:
@@ -120,4 +126,23 @@ class PagedGqaAttention(Mixer):
                                              cache.append)
         out = kernels.paged_attention(qkv, Hq, Hkv, D, cache.pages, cache.block_table,
                                       cache.page_size, ctx, self.window or 0, self.scale)
+        return self.project("o", out, self.w_o, ctx)
+
+    def _forward_tree(self, x: torch.Tensor, ctx: StepContext, cache: CacheView) -> torch.Tensor:
+        """Rows that are trees: rotated by their depth, kept in the cache one after the other, and seen by their descendants."""
+        if self.window:
+            raise ValueError("a window and a tree of drafted tokens do not go together")
+        Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        qkv = self.project("qkv", x, self.w_qkv, ctx)
+        table = self.position.rotary_table(x.device)
+        place = (Hq, Hkv, D, cache.pages, cache.block_table, cache.page_size)
+        if table is None:
+            if self.b_qkv is not None:
+                qkv.add_(self.b_qkv.to(qkv.dtype))
+            self.position.apply(qkv[:, :self.q_width].unflatten(1, (Hq, D)),
+                                qkv[:, self.q_width:self.q_width + self.kv_width].unflatten(1, (Hkv, D)), ctx.tree.positions)
+            kernels.rope_append(qkv, None, ctx.positions, ctx.row_seg, None, 0, *place, cache.append)
+        else:
+            kernels.rope_append(qkv, self.b_qkv, ctx.tree.positions, ctx.row_seg, *table, *place, cache.append, places=ctx.positions)
+        out = kernels.tree_attention(qkv, *place, ctx.seg_pos0, ctx.seg_row0, ctx.tree.mask, ctx.max_context, self.scale)
         return self.project("o", out, self.w_o, ctx)

@@ -109,6 +109,14 @@ class CacheView:
 # --------------------------------------------------------------------------------------
 
 @dataclass
+class TreeRows:
+    """What a step of trees of drafted tokens says of its rows beside `StepContext`, whose `positions` are then the places in
+    the cache that the rows' entries go to, one after the other behind what the request held."""
+    positions: torch.Tensor        # [T] position of each row in its text: what the request held, plus the row's depth
+    mask: torch.Tensor             # [T, words] bit k: the row sees the k-th row of its segment
+
+
+@dataclass
 class StepContext:
     """Everything about a step that is not the hidden state.
 
@@ -136,6 +144,7 @@ class StepContext:
     max_context: int = 0           # bound on pos0 + rows over the segments of this step
     graph_mode: bool = False
     row_adapter: Optional[torch.Tensor] = None     # [T] adapter slot of each row, -1: none; None: no row has one
+    tree: Optional["TreeRows"] = None              # the segments are trees of drafted tokens; None: each goes on in a line
     scratch: Dict[str, torch.Tensor] = field(default_factory=dict)
     _tiles: Dict[object, Tuple[torch.Tensor, int]] = field(default_factory=dict)
 
@@ -608,6 +617,8 @@ class EmbeddingExtra(Part):
 
 
 class Mixer(Part):
+    tree_safe = False              # whether `forward` serves steps of trees (StepContext.tree)
+
     """Mixes information between the tokens of a request (attention here)."""
 
     def cache_spec(self) -> Optional[CacheSpec]:

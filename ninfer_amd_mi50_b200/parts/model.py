@@ -17,7 +17,7 @@ import torch
 from .. import kernels
 from ..config.model_config import LayerCall, ModelPlan
 from ..registry import build_part, part_class
-from .base import (CacheSpec, CacheView, Fetch, NormedUpdate, PairSum, RoutedSum, StateSpec, StepContext, StreamUpdate, TensorSpec,
+from .base import (CacheSpec, CacheView, Fetch, Mixer, NormedUpdate, PairSum, RoutedSum, StateSpec, StepContext, StreamUpdate, TensorSpec,
                    summed)
 
 
@@ -128,6 +128,11 @@ class DecoderModel:
     def graph_safe(self) -> bool:
         return (all(b.graph_safe for b in self.blocks) and self.final_norm.graph_safe
                 and all(e.graph_safe for e in self.embedding_extras))
+
+    @property
+    def tree_safe(self) -> bool:
+        """Whether steps may bring trees of drafted tokens: every mixer serves them and nothing else looks at a row's neighbours."""
+        return not self.embedding_extras and all(p.tree_safe for p in self.parts() if isinstance(p, Mixer))
 
     def check_limits(self, dtype: torch.dtype, max_context: int, page_size: int) -> None:
         for b in self.blocks:
