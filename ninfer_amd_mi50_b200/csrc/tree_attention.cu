@@ -23,28 +23,66 @@ constexpr int kThreads = 128;
 constexpr int kTile = 32;        // keys at a time: one a lane
 
 // Warp w keeps pairs 4 w .. 4 w + 3 of the CTA's 16; a lane has one key's scores, then every 32nd column of the values.
+// Float32 tiles come by asynchronous copies, the next one while one is worked on; bfloat16 ones pass through registers.
 template <typename T, int NC>
 __global__ void __launch_bounds__(kThreads)
 tree_attention_rows_kernel(TreeArgs a, const T* __restrict__ qkv, const T* __restrict__ pages, T* __restrict__ out) {
+  constexpr bool ASYNC = sizeof(T) == 4;
   extern __shared__ __align__(16) float smem[];
   const int D = a.D, G = a.Hq / a.Hkv, KS = D + 4;           // (rows of keys 4 floats apart: 16-byte reads of 8 lanes meet no bank twice)
+  const int tile = kTile * (KS + D);
   float* Qs = smem;                                          // [16][D]
-  float* Ks = Qs + kTreeRows * D;                            // [32][KS]
-  float* Vs = Ks + kTile * KS;                               // [32][D]
-  float* Ps = Vs + kTile * D;                                // [4 warps][32 keys][4 pairs]
-  __shared__ int key_page[kTile];
+  float* Ps = Qs + kTreeRows * D;                            // [4 warps][32 keys][4 pairs]
+  float* KV = Ps + 4 * kTile * 4;                            // [ASYNC ? 2 : 1 tiles][keys [32][KS], values [32][D]]
   const int s = blockIdx.y / a.Hkv, g = blockIdx.y % a.Hkv;
   const TreeRequest r = tree_request(a, s);
   const int pair0 = blockIdx.z * kTreeRows, pairs = r.nodes * G;
   const int first = blockIdx.x * a.chunk, last = min(first + a.chunk, r.keys);
   if (blockIdx.x == 0 && blockIdx.z == 0 && g == 0 && threadIdx.x == 0 && r.bad) atomicCAS(&g_tree_error, 0, 1 + s);
   if (pair0 >= pairs || (first >= last && (first > 0 || a.shares > 1))) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kTreeRows * D; i += kThreads) {
-    const int p = pair0 + i / D;
-    Qs[i] = p < pairs ? to_float(qkv[(size_t)(r.row0 + p / G) * a.q_stride + (size_t)(g * G + p % G) * D + i % D]) : 0.f;
-  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D4 = D / 4;
   const size_t head = (size_t)a.page_size * D, page_stride = 2 * (size_t)a.Hkv * head;
+  // where key `lane` of a tile lies in the pool; -1 for none
+  auto source = [&](int k0) -> long long {
+    const int j = k0 + lane;
+    if (j >= last) return -1;
+    const int lp = j / a.page_size, page = lp < a.bt_width ? a.block_table[(size_t)s * a.bt_width + lp] : -1;
+    if (page < 0 || page >= a.num_pages) {
+      atomicCAS(&g_tree_error, 0, 1 + s);
+      return -1;
+    }
+    return (long long)(page * page_stride + g * head + (size_t)(j - lp * a.page_size) * D);
+  };
+  auto fetch = [&](float* to, long long mine) {
+#pragma unroll 4
+    for (int i0 = 0; i0 < kTile * D4; i0 += kThreads) {      // (D is a multiple of 16: all threads have as many pieces)
+      const int i = i0 + threadIdx.x, k = i / D4, d = (i - k * D4) * 4;
+      const long long from = __shfl_sync(0xffffffffu, mine, k);
+      float *tk = to + k * KS + d, *tv = to + kTile * KS + k * D + d;
+      const T* p = pages + (from < 0 ? 0 : from + d);
+      if constexpr (ASYNC) {
+        cp16_or_zeros(tk, (const float*)p, from >= 0);
+        cp16_or_zeros(tv, (const float*)(p + (from < 0 ? 0 : (size_t)a.Hkv * head)), from >= 0);
+      } else {
+        float kv[2][4] = {};
+        if (from >= 0) {
+          load4(p, kv[0]);
+          load4(p + (size_t)a.Hkv * head, kv[1]);
+        }
+        store4(tk, kv[0]);
+        store4(tv, kv[1]);
+      }
+    }
+  };
+  long long mine = source(first);
+  if constexpr (ASYNC) {
+    fetch(KV, mine);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  for (int i = threadIdx.x; i < kTreeRows * D; i += kThreads) {
+    const int row = i / D, p = pair0 + row;
+    Qs[i] = p < pairs ? to_float(qkv[(size_t)(r.row0 + p / G) * a.q_stride + (size_t)(g * G + p % G) * D + i - row * D]) : 0.f;
+  }
   float acc[4][NC], m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -53,35 +91,22 @@ tree_attention_rows_kernel(TreeArgs a, const T* __restrict__ qkv, const T* __res
     for (int c = 0; c < NC; ++c) acc[i][c] = 0.f;
   }
   const float scale2 = a.scale * 1.4426950408889634f;
-  for (int k0 = first; k0 < last; k0 += kTile) {
-    __syncthreads();                                         // the tile before has been read
-    if (threadIdx.x < kTile) {
-      const int j = k0 + threadIdx.x;
-      int page = -1;
-      if (j < last) {
-        const int lp = j / a.page_size;
-        page = lp < a.bt_width ? a.block_table[(size_t)s * a.bt_width + lp] : -1;
-        if (page < 0 || page >= a.num_pages) {
-          page = -1;
-          atomicCAS(&g_tree_error, 0, 1 + s);
-        }
-      }
-      key_page[threadIdx.x] = page;
+  int turn = 0;
+  for (int k0 = first; k0 < last; k0 += kTile, turn ^= 1) {
+    const long long here = mine;
+    mine = source(k0 + kTile);
+    float* Ks = KV + (ASYNC ? turn * tile : 0);
+    if constexpr (ASYNC) {
+      if (k0 + kTile < last) fetch(KV + (turn ^ 1) * tile, mine);            // (that place has been read: see the end of the loop)
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      fetch(Ks, here);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kTile * D / 4; i += kThreads) {
-      const int k = i / (D / 4), d = i % (D / 4) * 4, page = key_page[k];
-      float kv[2][4] = {};
-      if (page >= 0) {
-        const T* p = pages + (size_t)page * page_stride + (size_t)g * head + (size_t)((k0 + k) % a.page_size) * D + d;
-        load4(p, kv[0]);
-        load4(p + (size_t)a.Hkv * head, kv[1]);
-      }
-      store4(Ks + k * KS + d, kv[0]);
-      store4(Vs + k * D + d, kv[1]);
-    }
-    __syncthreads();
+    const float* Vs = Ks + kTile * KS;
     float x[4] = {};
+#pragma unroll 4
     for (int d = 0; d < D; d += 4) {
       const float4 k = *reinterpret_cast<const float4*>(Ks + lane * KS + d);
 #pragma unroll
@@ -91,33 +116,55 @@ tree_attention_rows_kernel(TreeArgs a, const T* __restrict__ qkv, const T* __res
       }
     }
     const int j = k0 + lane;
+    float v[4], top[4], w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int p = pair0 + 4 * warp + i;
-      const bool seen = p < pairs && key_page[lane] >= 0 && tree_sees(a, r, p / G, j);
-      const float v = seen ? x[i] * scale2 : -INFINITY, top = fmaxf(m[i], warp_max(v));
-      const float base = top == -INFINITY ? 0.f : top, keep = exp2f(m[i] - base);
-      const float w = exp2f(v - base);
-      l[i] = l[i] * keep + w;                                // (a lane's own part)
-      m[i] = top;
+      v[i] = p < pairs && here >= 0 && tree_sees(a, r, p / G, j) ? x[i] * scale2 : -INFINITY;
+      top[i] = v[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float up = fmaxf(m[i], top[i]), base = up == -INFINITY ? 0.f : up, keep = exp2f(m[i] - base);
+      w[i] = exp2f(v[i] - base);
+      l[i] = l[i] * keep + w[i];                             // (a lane's own part)
+      m[i] = up;
 #pragma unroll
       for (int c = 0; c < NC; ++c) acc[i][c] *= keep;
-      Ps[(warp * kTile + lane) * 4 + i] = w;
     }
+    *reinterpret_cast<float4*>(Ps + (warp * kTile + lane) * 4) = make_float4(w[0], w[1], w[2], w[3]);
     __syncwarp();
-    for (int k = 0; k < kTile; ++k) {
-      const float4 w = *reinterpret_cast<const float4*>(Ps + (warp * kTile + k) * 4);
+    if (k0 + kTile <= r.len) {
+#pragma unroll 4
+      for (int k = 0; k < kTile; ++k) {
+        const float4 w = *reinterpret_cast<const float4*>(Ps + (warp * kTile + k) * 4);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int d = lane + 32 * c;
-        // (a value that no pair of the warp sees may be no number: its weight of nothing must not turn the sum into none)
-        const float v = d < D ? Vs[k * D + d] : 0.f;
-        acc[0][c] += w.x ? w.x * v : 0.f;
-        acc[1][c] += w.y ? w.y * v : 0.f;
-        acc[2][c] += w.z ? w.z * v : 0.f;
-        acc[3][c] += w.w ? w.w * v : 0.f;
+        for (int c = 0; c < NC; ++c) {
+          const int d = lane + 32 * c;
+          const float v = d < D ? Vs[k * D + d] : 0.f;
+          acc[0][c] = fmaf(w.x, v, acc[0][c]), acc[1][c] = fmaf(w.y, v, acc[1][c]), acc[2][c] = fmaf(w.z, v, acc[2][c]), acc[3][c] = fmaf(w.w, v, acc[3][c]);
+        }
+      }
+    } else {
+      for (int k = 0; k < kTile; ++k) {
+        const float4 w = *reinterpret_cast<const float4*>(Ps + (warp * kTile + k) * 4);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int d = lane + 32 * c;
+          // (a value that a pair does not see may be no number: its weight of nothing must not turn the sum into none)
+          const float v = d < D ? Vs[k * D + d] : 0.f;
+          acc[0][c] += w.x ? w.x * v : 0.f;
+          acc[1][c] += w.y ? w.y * v : 0.f;
+          acc[2][c] += w.z ? w.z * v : 0.f;
+          acc[3][c] += w.w ? w.w * v : 0.f;
+        }
       }
     }
+    __syncthreads();                                         // the tile has been read
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -217,7 +264,7 @@ tree_attention_merge_kernel(TreeArgs a, T* __restrict__ out) {
 
 template <typename T, int NC>
 int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
-  const size_t smem = ((size_t)kTreeRows * a.D + kTile * (2 * a.D + 4) + 4 * kTile * 4) * sizeof(float);
+  const size_t smem = ((size_t)kTreeRows * a.D + 4 * kTile * 4 + (sizeof(T) == 4 ? 2 : 1) * kTile * (2 * a.D + 4)) * sizeof(float);
   if (int rc = allow_smem<tree_attention_rows_kernel<T, NC>>(smem)) return rc;
   const int pairs = (int)min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv);
   const dim3 grid(a.shares, a.S * a.Hkv, (pairs + kTreeRows - 1) / kTreeRows);

@@ -6,8 +6,10 @@
 // keys.  (A fifth warp for the copies would leave the others 168 registers, too few beside 32 rows of sums.)  A warp's step is the
 // usual flash step: S = Q K^T and O += P V by ``mma.sync.m16n8k16`` with the pairs as the 16 rows, a reference maximum that
 // is raised only when a score passes it by 2^8, weights rounded to bfloat16 in between (an error of 2^-9 of a weight at most,
-// as independent from key to key as the rounding of the result; their sum is of the unrounded ones).  At the end the sums
-// of the four warps are put together in shared memory.
+// as independent from key to key as the rounding of the result, so that the result is 1.4 times as far from the 64-bit one
+// as its own rounding puts it; their sum is of the unrounded ones).  With 16 pairs a CTA a weight goes into the second
+// product as two numbers, its rounding and what that left, which costs 5 % there; with 32 it would be 10 %.  At the end the
+// sums of the four warps are put together in shared memory.
 //
 // The tensor cores' newer form (tree_attention_tc.cu) wants 128 rows at once and a chain of copies, products and softmax a
 // block of 128 keys; with few pairs most of that is waiting.
@@ -47,6 +49,12 @@ __device__ __forceinline__ unsigned pack(float lo, float hi) {
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
+__device__ __forceinline__ unsigned pack_two(float x, float y, unsigned& rest) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  rest = pack(x - __low2float(v), y - __high2float(v));
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+
 struct __align__(8) Ring {
   unsigned long long full[kStages], empty[kStages];
   int stop;
@@ -64,7 +72,7 @@ template <int D, int MT>
 __global__ void __launch_bounds__(kThreads, 2)
 tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ TreeArgs a, int box_rows,
                           const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ out) {
-  constexpr int ROWS = 16 * MT, PIECES = D / 8, ATOMS = D / 64, SB = stage_bytes<D>(), OL = D / 4 + 4, OS = 4 * OL, AB = kStageKeys * 128;     // AB: 64 numbers of the stage's keys
+  constexpr int ROWS = 16 * MT, PIECES = D / 8, ATOMS = D / 64, SB = stage_bytes<D>(), OL = D / 4 + 4, OS = 4 * OL, PARTS = MT == 1 ? 2 : 1, AB = kStageKeys * 128;     // AB: 64 numbers of the stage's keys
   constexpr size_t kRing = (size_t)kStages * SB, kSums = (size_t)kGroups * ROWS * OS * 4;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);          // (an offset, so that what lies here is known to be shared memory)
@@ -244,7 +252,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
               }
           }
         }
-        unsigned w[MT][4];
+        unsigned w[MT][4], rest[MT][4];                      // PARTS == 2: the weights as two bfloat16 numbers, their rounding and what it left
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -253,8 +261,8 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
             const float w0 = ex2(fmaf(c[m][0][2 * h], sc2, -base)), w1 = ex2(fmaf(c[m][0][2 * h + 1], sc2, -base));
             const float w2 = ex2(fmaf(c[m][1][2 * h], sc2, -base)), w3 = ex2(fmaf(c[m][1][2 * h + 1], sc2, -base));
             l_run[m][h] += (w0 + w1) + (w2 + w3);
-            w[m][h] = pack(w0, w1);
-            w[m][2 + h] = pack(w2, w3);
+            w[m][h] = pack_two(w0, w1, rest[m][h]);
+            w[m][2 + h] = pack_two(w2, w3, rest[m][2 + h]);
           }
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
@@ -264,6 +272,10 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
           for (int m = 0; m < MT; ++m) {
             mma(o[m][2 * n], w[m], b[0], b[1]);
             mma(o[m][2 * n + 1], w[m], b[2], b[3]);
+            if (PARTS == 2) {
+              mma(o[m][2 * n], rest[m], b[0], b[1]);
+              mma(o[m][2 * n + 1], rest[m], b[2], b[3]);
+            }
           }
         }
       }

@@ -15,7 +15,7 @@
 // takes time is the vocabulary's row at the walk's end, and one for a rejection of a drafted token.  A cluster of CTAs
 // takes a request: each walks by itself (the same numbers, the same steps) and reads its part of such rows, a warp a run of
 // neighbouring numbers; the runs' sums change hands in shared memory.  The drawn token is then in one CTA's part, in one
-// warp's run, which that warp reads once more, a lane a smaller run.
+// warp's run, which the CTA reads once more.
 #include "common.cuh"
 
 namespace nf {
@@ -44,7 +44,7 @@ struct Shared {
   double mass[kNodes];                  // z when it was rejected
   double run[kWarps], total[2][kCtas];  // total: of a pass and of the next in turn, as a CTA may have gone on while another still reads
   double z;
-  int node, next, accepted, n_rejected, todo, summed;
+  int node, next, accepted, n_rejected, todo, summed, first, last;
 };
 
 __device__ __forceinline__ void cluster_meet() {
@@ -69,14 +69,15 @@ __device__ __forceinline__ float4 four(const float* p, int n, bool vec) {
   if (vec && n >= 4) return *reinterpret_cast<const float4*>(p);
   return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
 }
-// What is left of p[v] at tokens i .. i + 3 after the node's rejections, `n` of them in the vocabulary.
-__device__ __forceinline__ void left_at(const VerifyArgs& a, const Shared& sh, int row0, int n_rejected, int i, int n, bool vec, double* r) {
-  const float4 p = four(a.probs + (size_t)(row0 + sh.node) * a.probs_ld + i, n, vec);
+// What is left of p[v] at tokens i .. i + 3 after the node's rejections: `p` are its numbers there, `q` those of the first
+// rejected draft, `n` tokens are in the vocabulary.
+__device__ __forceinline__ void left_at(const VerifyArgs& a, const Shared& sh, int row0, int n_rejected, int i, int n, bool vec, float4 p, float4 q,
+                                        double* r) {
   r[0] = mass_of(p.x), r[1] = mass_of(p.y), r[2] = mass_of(p.z), r[3] = mass_of(p.w);
   for (int k = 0; k < n_rejected; ++k) {
     const int c = sh.rejected[k];
     if (a.draft) {
-      const float4 q = four(a.draft + (size_t)(row0 + c) * a.draft_ld + i, n, vec);
+      if (k) q = four(a.draft + (size_t)(row0 + c) * a.draft_ld + i, n, vec);
       const double z = sh.mass[k];
       r[0] = fmax(r[0] - z * mass_of(q.x), 0.0), r[1] = fmax(r[1] - z * mass_of(q.y), 0.0);
       r[2] = fmax(r[2] - z * mass_of(q.z), 0.0), r[3] = fmax(r[3] - z * mass_of(q.w), 0.0);
@@ -98,12 +99,25 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 __device__ double sum_left(const VerifyArgs& a, Shared& sh, double* total, int row0, int n_rejected, bool vec) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int begin = (cluster_rank() * kWarps + warp) * a.run, end = min(begin + a.run, a.V);
+  constexpr int AT_ONCE = 5;            // (a run of 152,000 numbers' is 1,280: two trips to memory)
+  const float* p = a.probs + (size_t)(row0 + sh.node) * a.probs_ld;
+  const float* q = a.draft && n_rejected ? a.draft + (size_t)(row0 + sh.rejected[0]) * a.draft_ld : nullptr;
   double sum = 0.0;
-#pragma unroll 4
-  for (int i = begin + 4 * lane; i < end; i += 128) {
-    double r[4];
-    left_at(a, sh, row0, n_rejected, i, end - i, vec, r);
-    sum += (r[0] + r[1]) + (r[2] + r[3]);
+  for (int i0 = begin + 4 * lane; i0 < end; i0 += 128 * AT_ONCE) {
+    float4 x[AT_ONCE], y[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + 128 * u;
+      x[u] = four(p + i, end - i, vec);
+      y[u] = q ? four(q + i, end - i, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + 128 * u;
+      double r[4];
+      left_at(a, sh, row0, i < end ? n_rejected : 0, i, end - i, vec, x[u], y[u], r);
+      sum += (r[0] + r[1]) + (r[2] + r[3]);
+    }
   }
   sum = warp_sum_f64(sum);
   if (lane == 0) sh.run[warp] = sum;
@@ -121,10 +135,10 @@ __device__ double sum_left(const VerifyArgs& a, Shared& sh, double* total, int r
   return all;
 }
 
-// The lowest token whose running sum passes `draw` times the whole, written to `*to` by the warp that has it; -1 where
+// The lowest token whose running sum passes `draw` times the whole, written to `*to` by the CTA that has it; -1 where
 // nothing is left.  Called by all threads of all CTAs after sum_left.  Where rounding keeps the sums of a stretch from what
 // they were as parts, the last token that has anything is taken.
-__device__ void draw_token(const VerifyArgs& a, const Shared& sh, const double* total, int row0, int n_rejected, bool vec, double all, double draw, int* to) {
+__device__ void draw_token(const VerifyArgs& a, Shared& sh, const double* total, int row0, int n_rejected, bool vec, double all, double draw, int* to) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double bound = draw * all;
   double run = 0.0, before = 0.0;
@@ -152,44 +166,47 @@ __device__ void draw_token(const VerifyArgs& a, const Shared& sh, const double* 
     }
     run += t;
   }
-  if (mine != warp) return;
-  // a lane takes a run of neighbouring numbers
-  const int begin = (cluster_rank() * kWarps + warp) * a.run, end = min(begin + a.run, a.V), each = a.run / 32;
-  const int lo = begin + lane * each, hi = min(lo + each, end);
-  double sum = 0.0;
-#pragma unroll 4
-  for (int i = lo; i < hi; i += 4) {
-    double r[4];
-    left_at(a, sh, row0, n_rejected, i, hi - i, vec, r);
-    sum += (r[0] + r[1]) + (r[2] + r[3]);
-  }
-  double upto = sum;
+  // that warp's run, four numbers a thread of the whole CTA
+  const int begin = (cluster_rank() * kWarps + mine) * a.run, end = min(begin + a.run, a.V);
+  const float* p = a.probs + (size_t)(row0 + sh.node) * a.probs_ld;
+  const float* q = a.draft && n_rejected ? a.draft + (size_t)(row0 + sh.rejected[0]) * a.draft_ld : nullptr;
+  if (threadIdx.x == 0) sh.first = 0x7fffffff, sh.last = -1;
+  for (int i0 = begin; i0 < end; i0 += 4 * kThreads) {
+    const int i = i0 + 4 * threadIdx.x;
+    double r[4] = {0.0, 0.0, 0.0, 0.0};
+    if (i < end)
+      left_at(a, sh, row0, n_rejected, i, end - i, vec, four(p + i, end - i, vec), q ? four(q + i, end - i, vec) : make_float4(0.f, 0.f, 0.f, 0.f), r);
+    const double sum = (r[0] + r[1]) + (r[2] + r[3]);
+    double upto = sum;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  const unsigned some = __ballot_sync(0xffffffffu, sum > 0.0), past = __ballot_sync(0xffffffffu, sum > 0.0 && before + upto > bound);
-  const int owner = past ? __ffs(past) - 1 : 31 - __clz(some);
-  if (lane != owner) return;
-  run = before + (upto - sum);
-  int last = -1;
-  for (int i = lo; i < hi; i += 4) {
-    double r[4];
-    left_at(a, sh, row0, n_rejected, i, hi - i, vec, r);
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    __syncthreads();                                       // (all have read sh.run, and the sums of the stretch before)
+    if (lane == 31) sh.run[warp] = upto;
+    __syncthreads();
+    double at = before;
+    for (int w = 0; w < warp; ++w) at += sh.run[w];
+    if (sum > 0.0) {
+      int last = -1, found = -1;
+      double x = at + (upto - sum);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      run += r[j];
-      if (r[j] > 0.0) {
-        last = i + j;
-        if (run > bound) {
-          *to = last;
-          return;
+      for (int j = 0; j < 4; ++j) {
+        x += r[j];
+        if (r[j] > 0.0) {
+          last = i + j;
+          if (found < 0 && x > bound) found = i + j;
         }
       }
+      if (found < 0 && at + upto > bound) found = last;
+      if (found >= 0) atomicMin(&sh.first, found);
+      atomicMax(&sh.last, last);
     }
+    for (int w = 0; w < kWarps; ++w) before += sh.run[w];
   }
-  *to = last;
+  __syncthreads();
+  if (threadIdx.x == 0) *to = sh.first != 0x7fffffff ? sh.first : sh.last;
 }
 
 __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
