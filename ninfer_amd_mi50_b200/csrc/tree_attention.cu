@@ -364,8 +364,10 @@ extern "C" int nf_tree_attention(const TreeCall* call) {
   const int shares = (max_context + chunk - 1) / chunk;
   NF_REQUIRE(shares == 1 || ws, "tree attention: %d shares of keys want a workspace", shares);
   float* ws_ml = ws ? ws + (size_t)shares * T * Hq * D : nullptr;
+  const int G = Hq / Hkv;
+  NF_REQUIRE(G < 4096, "tree attention: %d query heads a key head are too many", G);
   TreeArgs a = {block_table, lengths, row0, mask, ws, ws_ml, q_stride, bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context,
-                chunk, shares, form != 0, scale};
+                chunk, shares, form != 0, scale, G == 1 ? 0u : (unsigned)(((1ull << 32) + G - 1) / G)};
   if (form) {
     const bool aligned = (uintptr_t)qkv % 16 == 0 && q_stride % 8 == 0 && (uintptr_t)out % 16 == 0;
     NF_REQUIRE(form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned) && chunk % 128 == 0,

@@ -18,7 +18,12 @@ struct TreeArgs {
   int bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context, chunk, shares;
   int whole_written;              // a request with one share has its result from the first kernel
   float scale;
+  unsigned inverse_heads;         // 2^32 / (Hq / Hkv), rounded up: see node_of
 };
+
+// Pair p's node, p / (Hq / Hkv).  The inverse is at most 1 too large, which at p below 2^16 stays below 2^-16 of a node; one
+// query head a key head has no inverse in 32 bits.
+__device__ __forceinline__ int node_of(const TreeArgs& a, int p) { return a.inverse_heads ? (int)__umulhi((unsigned)p, a.inverse_heads) : p; }
 
 struct TreeRequest {
   int row0, nodes, len, keys;     // its rows, the keys it held, these and its nodes'

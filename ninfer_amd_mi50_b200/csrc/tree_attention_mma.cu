@@ -70,7 +70,7 @@ template <int D, int MT> constexpr size_t smem_bytes() {
 // MT times 16 pairs; warp w takes the keys 16 w .. of every stage.
 template <int D, int MT>
 __global__ void __launch_bounds__(kThreads, 2)
-tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ TreeArgs a, int box_rows,
+tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ TreeArgs a, int box_rows, int page_shift,
                           const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ out) {
   constexpr int ROWS = 16 * MT, PIECES = D / 8, ATOMS = D / 64, SB = stage_bytes<D>(), OL = D / 4 + 4, OS = 4 * OL, PARTS = MT == 1 ? 2 : 1, AB = kStageKeys * 128;     // AB: 64 numbers of the stage's keys
   constexpr size_t kRing = (size_t)kStages * SB, kSums = (size_t)kGroups * ROWS * OS * 4;
@@ -95,7 +95,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
   // the first pages, on their way beside the request's numbers: lane i that of the i-th box
   int page = -1;
   const auto look_up = [&](int key) {
-    const int lp = key / a.page_size;
+    const int lp = page_shift >= 0 ? key >> page_shift : key / a.page_size;
     return lp < a.bt_width ? bt[lp] : -1;
   };
   if (warp == 0 && (long long)first + box_rows * lane < a.max_context) page = look_up(first + box_rows * lane);
@@ -122,7 +122,8 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
     if (elect_one()) mbar_expect_tx(&ring->full[st], (unsigned)__popc(boxes) * 2 * box_rows * D * 2);
     __syncwarp();
     if (there) {                                             // each lane its box of keys and of values
-      const int y = (page * 2 * a.Hkv + g) * a.page_size + (key0 + at) % a.page_size;
+      const int in_page = page_shift >= 0 ? (key0 + at) & (a.page_size - 1) : (key0 + at) % a.page_size;
+      const int y = (page * 2 * a.Hkv + g) * a.page_size + in_page;
       unsigned char* to = smem + (size_t)st * SB + at * 128;
 #pragma unroll
       for (int x = 0; x < ATOMS; ++x) {
@@ -139,11 +140,15 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
       __syncwarp();
       fetch(issued);
     }
+  {                                                          // queries: [row][D], a row's 16-byte pieces exchanged by its number
+    constexpr int EACH = ROWS * PIECES / kThreads, PER = PIECES / EACH;    // pieces a thread, threads a row
+    const int row = threadIdx.x / PER, c0 = threadIdx.x % PER, p = pair0 + row, node = node_of(a, p);
+    const uint4* q = reinterpret_cast<const uint4*>(qkv + (size_t)(p < pairs ? r.row0 + node : 0) * a.q_stride + (size_t)(g * G + p - node * G) * D);
+    uint4 v[EACH];
 #pragma unroll
-  for (int i = threadIdx.x; i < ROWS * PIECES; i += kThreads) {            // queries: [row][D], a row's 16-byte pieces exchanged by its number
-    const int row = i / PIECES, c = i % PIECES, p = pair0 + row;
-    const uint4* q = reinterpret_cast<const uint4*>(qkv + (size_t)(p < pairs ? r.row0 + p / G : 0) * a.q_stride + (size_t)(g * G + p % G) * D);
-    *reinterpret_cast<uint4*>(Qs + row * D * 2 + ((c ^ (row & 7)) << 4)) = p < pairs ? q[c] : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < EACH; ++i) v[i] = p < pairs ? q[c0 + PER * i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) *reinterpret_cast<uint4*>(Qs + row * D * 2 + (((c0 + PER * i) ^ (row & 7)) << 4)) = v[i];
   }
   __syncthreads();
   float o[MT][D / 8][4], m_run[MT][2], l_run[MT][2];
@@ -194,18 +199,25 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
           }
         }
         if (k0 + 16 > r.len) {                               // (else keys that every row sees)
+          const int from = k0 - r.len;                       // the tree's node at the tile's first key
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int p = pair0 + 16 * m + quad + 8 * h;
+              unsigned seen = 0;                             // bit i: key k0 + i
+              if (p < pairs) {
+                const int* words = a.mask + (size_t)(r.row0 + node_of(a, p)) * a.words;
+                const int w = from >> 5;                     // (-1 for keys that the request held)
+                const unsigned lo = w < 0 ? ~0u : (unsigned)words[w], hi = w + 1 < a.words ? (unsigned)words[w + 1] : 0u;
+                seen = __funnelshift_r(lo, hi, from & 31);
+                if (last - k0 < 16) seen &= (1u << (last - k0)) - 1;
+              }
 #pragma unroll
               for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  const int j = k0 + 8 * n + 2 * t4 + x;
-                  if (p >= pairs || j >= last || !tree_sees(a, r, p / G, j)) c[m][n][2 * h + x] = -INFINITY;
-                }
+                for (int x = 0; x < 2; ++x)
+                  if (!(seen >> (8 * n + 2 * t4 + x) & 1)) c[m][n][2 * h + x] = -INFINITY;
             }
           // values behind the last key: whatever lies there would be multiplied by a weight of nothing
           for (int e = lane; e < 16 * PIECES; e += 32)
@@ -337,7 +349,8 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
       l = fmaf(f, st[w].y, l);
       x.x = fmaf(f, v[w].x, x.x), x.y = fmaf(f, v[w].y, x.y), x.z = fmaf(f, v[w].z, x.z), x.w = fmaf(f, v[w].w, x.w);
     }
-    const size_t to = (size_t)(r.row0 + p / G) * a.Hq + g * G + p % G;
+    const int node = node_of(a, p);
+    const size_t to = (size_t)(r.row0 + node) * a.Hq + g * G + p - node * G;
     if (whole) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       *reinterpret_cast<unsigned*>(out + to * D + d) = pack(x.x * inv, x.y * inv);
@@ -358,7 +371,7 @@ int launch_mma(const CUtensorMap& map, const TreeArgs& a, int box_rows, const vo
   const long long pairs = std::min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv);
   const long long y = (long long)a.S * a.Hkv, z = (pairs + 16 * MT - 1) / (16 * MT);
   NF_REQUIRE(y <= 65535 && z <= 65535, "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
-  launch_chained(tree_attention_mma_kernel<D, MT>, dim3(a.shares, (unsigned)y, (unsigned)z), dim3(kThreads), smem, stream, map, a, box_rows,
+  launch_chained(tree_attention_mma_kernel<D, MT>, dim3(a.shares, (unsigned)y, (unsigned)z), dim3(kThreads), smem, stream, map, a, box_rows, a.page_size & (a.page_size - 1) ? -1 : __builtin_ctz(a.page_size),
                  (const __nv_bfloat16*)qkv, (__nv_bfloat16*)out);
   return check_launch("tree_attention_mma");
 }

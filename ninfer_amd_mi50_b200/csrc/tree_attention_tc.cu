@@ -279,56 +279,54 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         const bool two = t.tiles == 2;
         const int n0 = t.steps(0), n1 = t.steps(1);
         int to_come = n0 + n1;                               // products of queries and keys
-        // S = Q K^T of a group's step, whose keys are there
-        auto scores = [&](int group, int b) {
+        // (one lane waits, issues and waits again: the tensor cores take a product only when they can begin it, so that what
+        // lies between two of them is time that they stand still)
+        auto wait = [&](void* bar, unsigned parity, int code) { return mbar_wait(bar, parity, stop, code, &g_tree_tc_error); };
+        // S = Q K^T of a group's step
+        auto scores = [&](int group, int b, int left) -> bool {
           const int st = b % STAGES;
           const unsigned long long dq = smem_desc(Qs + (two ? group * KB : 0)), dk = smem_desc(KV + 2 * st * KB);
+          if (!wait(&bars->k_full[st], (b / STAGES) & 1, 4)) return false;
           tc_fence_after();
-          --to_come;
-          if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {            // (an atom on: 16,384 bytes, of which a descriptor counts sixteenths)
-              const int off = (kk >> 2) * (kAtom / 16) + 2 * (kk & 3);
-              tc_mma(tmem + group * kKeys, dq + off, dk + off, desc_qk, kk > 0 ? 1u : 0u);
-            }
-            tc_commit(&bars->s_full[group]);
-            if (!two || group == 1) tc_commit(&bars->k_empty[st]);
-            if (to_come == 0) tc_commit(&bars->q_empty);
+          for (int kk = 0; kk < D / 16; ++kk) {              // (an atom on: 16,384 bytes, of which a descriptor counts sixteenths)
+            const int off = (kk >> 2) * (kAtom / 16) + 2 * (kk & 3);
+            tc_mma(tmem + group * kKeys, dq + off, dk + off, desc_qk, kk > 0 ? 1u : 0u);
           }
-          __syncwarp();
+          tc_commit(&bars->s_full[group]);
+          if (!two || group == 1) tc_commit(&bars->k_empty[st]);
+          if (left == 0) tc_commit(&bars->q_empty);
+          return true;
         };
-        auto keys_there = [&](int b) { return warp_wait(&bars->k_full[b % STAGES], (b / STAGES) & 1, stop, 4); };
-        ok = warp_wait(&bars->q_full, gi & 1, stop, 3);
-        for (int group = 0; ok && group < 2; ++group)
-          if (group == 0 || n1 > 0) {
-            const int b = gb + t.block(group, 0);
-            ok = keys_there(b);
-            if (ok) scores(group, b);
-          }
+        bool all = true;
+        if (elect_one()) {
+          all = wait(&bars->q_full, gi & 1, 3) && scores(0, gb + t.block(0, 0), to_come - 1) && (n1 == 0 || scores(1, gb + t.block(1, 0), to_come - 2));
+        }
+        ok = __all_sync(0xffffffffu, all);
+        to_come -= 1 + (n1 > 0);
         for (int step = 0; ok && step < n0; ++step)
+#pragma unroll 1
           for (int group = 0; ok && group < 2; ++group) {
             const int n = group ? n1 : n0;
             if (step >= n) continue;
-            const int b = gb + t.block(group, step), st = b % STAGES, b_next = gb + t.block(group, step + 1);
-            // what is there before the weights are is not asked for between the products
-            ok = (step > 0 || gi == 0 || warp_wait(&bars->o_read, (gi - 1) & 1, stop, 7)) && warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 5);
-            const bool early = step + 1 < n && __all_sync(0xffffffffu, mbar_try(&bars->k_full[b_next % STAGES], (b_next / STAGES) & 1));
-            ok = ok && warp_wait(&bars->p_full[group], (done[group] + step) & 1, stop, 6);
-            if (!ok) break;
-            tc_fence_after();
-            const unsigned long long dv = smem_desc_mn(KV + (2 * st + 1) * KB, kAtom);
+            const int b = gb + t.block(group, step), st = b % STAGES;
+            if (step + 1 < n) --to_come;
+            all = true;
             if (elect_one()) {
+              all = (step > 0 || gi == 0 || wait(&bars->o_read, (gi - 1) & 1, 7)) && wait(&bars->v_full[st], (b / STAGES) & 1, 5) &&
+                    wait(&bars->p_full[group], (done[group] + step) & 1, 6);
+              if (all) {
+                tc_fence_after();
+                const unsigned long long dv = smem_desc_mn(KV + (2 * st + 1) * KB, kAtom);
 #pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)        // (16 keys on: 2,048 bytes)
-                tc_mma_ts(tmem + (2 + group) * kKeys, tmem + group * kKeys + 8 * kk, dv + 128 * kk, desc_pv, (step > 0 || kk > 0) ? 1u : 0u);
-              if (!two || group == 1) tc_commit(&bars->v_empty[st]);
-              if (step == n - 1) tc_commit(&bars->o_final[group]);
+                for (int kk = 0; kk < kKeys / 16; ++kk)      // (16 keys on: 2,048 bytes)
+                  tc_mma_ts(tmem + (2 + group) * kKeys, tmem + group * kKeys + 8 * kk, dv + 128 * kk, desc_pv, (step > 0 || kk > 0) ? 1u : 0u);
+                if (!two || group == 1) tc_commit(&bars->v_empty[st]);
+                if (step == n - 1) tc_commit(&bars->o_final[group]);
+                if (step + 1 < n) all = scores(group, gb + t.block(group, step + 1), to_come);
+              }
             }
-            __syncwarp();
-            if (step + 1 < n) {
-              ok = early || keys_there(b_next);
-              if (ok) scores(group, b_next);
-            }
+            ok = __all_sync(0xffffffffu, all);
           }
         if (ok && n1 == 0 && elect_one()) tc_commit(&bars->o_final[1]);
         __syncwarp();
