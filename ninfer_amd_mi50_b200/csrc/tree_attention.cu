@@ -262,6 +262,70 @@ tree_attention_merge_kernel(TreeArgs a, T* __restrict__ out) {
   }
 }
 
+// The same of shares whose numbers lie [key head][D / 4][pair][4] (tree_attention_tc.cu): a CTA takes 32 pairs of a key head,
+// a lane a pair, and each of its eight warps an eighth of the numbers; they come together in shared memory, out of which
+// rows are written whole.
+__global__ void __launch_bounds__(256)
+tree_attention_merge_turned_kernel(TreeArgs a, __nv_bfloat16* __restrict__ out) {
+  constexpr int AT_ONCE = 4;
+  __shared__ __align__(16) float turned[32][128 + 4];
+  __shared__ int row_of[32];                                 // each pair's (row, query head) in the result; -1 for none
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y, G = a.Hq / a.Hkv, each = a.D / 32;
+  const int pair = blockIdx.x * 32 + lane, t = pair / G;
+  chain_wait(a.ws_acc, a.ws_ml, a.lengths, a.row0);
+  const size_t all = (size_t)a.T * G;
+  const bool in = pair < all;
+  int lo = 0, hi = a.S;                                      // the last request that begins at or before the pair's row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.row0[mid] <= t) lo = mid; else hi = mid;
+  }
+  const TreeRequest r = tree_request(a, lo);
+  const int shares = in && t >= r.row0 && t < r.row0 + r.nodes ? (r.keys + a.chunk - 1) / a.chunk : 0;
+  const bool mine = shares > 1;                              // (one share: its result is there already)
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + (size_t)g * all + pair;
+  float top = -INFINITY;
+  for (int c = 0; c < (mine ? shares : 0); ++c) top = fmaxf(top, ml[(size_t)c * a.Hkv * all].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  float4 sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* acc = reinterpret_cast<const float4*>(a.ws_acc) + ((size_t)g * (a.D / 4) + warp * each) * all + pair;
+#pragma unroll 1
+  for (int c0 = 0; c0 < (mine ? shares : 0); c0 += AT_ONCE) {
+    float4 v[AT_ONCE][4];
+    float2 x[AT_ONCE];
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c) {
+      const bool there = c0 + c < shares;
+      x[c] = there ? ml[(size_t)(c0 + c) * a.Hkv * all] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (there && i < each) v[c][i] = acc[((size_t)(c0 + c) * a.Hkv * (a.D / 4) + i) * all];
+    }
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c) {
+      const float w = exp2f(x[c].x - base);
+      l += w * x[c].y;
+      if (w != 0.f && c0 + c < shares)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < each) sum[i].x += w * v[c][i].x, sum[i].y += w * v[c][i].y, sum[i].z += w * v[c][i].z, sum[i].w += w * v[c][i].w;
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < each) *reinterpret_cast<float4*>(&turned[lane][4 * (warp * each + i)]) = make_float4(sum[i].x * inv, sum[i].y * inv, sum[i].z * inv, sum[i].w * inv);
+  if (warp == 0) row_of[lane] = mine ? t * a.Hq + g * G + pair - t * G : -1;
+  __syncthreads();
+  for (int e = threadIdx.x; e < 32 * (a.D / 4); e += 256) {
+    const int row = e / (a.D / 4), d = e % (a.D / 4) * 4;
+    if (row_of[row] >= 0) store4(out + (size_t)row_of[row] * a.D + d, &turned[row][d]);
+  }
+}
+
 template <typename T, int NC>
 int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
   const size_t smem = ((size_t)kTreeRows * a.D + 4 * kTile * 4 + (sizeof(T) == 4 ? 2 : 1) * kTile * (2 * a.D + 4)) * sizeof(float);
@@ -276,6 +340,10 @@ int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out
 template <typename T>
 int launch_merge(const TreeArgs& a, void* out, cudaStream_t stream) {
   if (a.shares == 1) return 0;
+  if (a.turned) {
+    launch_chained(tree_attention_merge_turned_kernel, dim3((unsigned)(((long long)a.T * (a.Hq / a.Hkv) + 31) / 32), a.Hkv), dim3(256), 0, stream, a, (__nv_bfloat16*)out);
+    return check_launch("tree_attention_merge_turned");
+  }
   // a warp a row takes eight shares in one trip to memory
   if (a.shares <= 8) launch_chained(tree_attention_merge_kernel<T, 1>, dim3((a.T * a.Hq + 3) / 4), dim3(128), 0, stream, a, (T*)out);
   else launch_chained(tree_attention_merge_kernel<T, 4>, dim3(a.T * a.Hq), dim3(128), 0, stream, a, (T*)out);
@@ -310,7 +378,8 @@ extern "C" long long nf_tree_attention_plan(int form, int dtype, int S, int T, i
   const bool asked = form >= 0 && form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned);
   if (!asked) {
     form = form_takes(1, dtype, Hkv, D, page_size, num_pages, aligned) ? 1 : (form_takes(2, dtype, Hkv, D, page_size, num_pages, aligned) ? 2 : 0);
-    if (form == 1 && (long long)T * (Hq / Hkv) <= 32ll * S) form = 2;
+    const long long pairs = ((long long)T * (Hq / Hkv) + S - 1) / S;                 // of a request and key head, on average
+    if (form == 1 && (pairs <= 32 || (pairs + 31) / 32 * S * Hkv * ((max_context + 63) / 64) <= 148 * 16)) form = 2;
   }
   if (form == 1) return 4ll * tree_tc_chunk(S, T, Hq, Hkv, words, max_context) + 1;
   if (form == 2) return 4ll * tree_mma_chunk(S, T, Hq, Hkv, max_context) + 2;
@@ -367,7 +436,7 @@ extern "C" int nf_tree_attention(const TreeCall* call) {
   const int G = Hq / Hkv;
   NF_REQUIRE(G < 4096, "tree attention: %d query heads a key head are too many", G);
   TreeArgs a = {block_table, lengths, row0, mask, ws, ws_ml, q_stride, bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context,
-                chunk, shares, form != 0, scale, G == 1 ? 0u : (unsigned)(((1ull << 32) + G - 1) / G)};
+                chunk, shares, form != 0, form == 1, scale, G == 1 ? 0u : (unsigned)(((1ull << 32) + G - 1) / G)};
   if (form) {
     const bool aligned = (uintptr_t)qkv % 16 == 0 && q_stride % 8 == 0 && (uintptr_t)out % 16 == 0;
     NF_REQUIRE(form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned) && chunk % 128 == 0,

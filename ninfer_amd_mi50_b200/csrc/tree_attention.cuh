@@ -17,6 +17,7 @@ struct TreeArgs {
   long long q_stride;
   int bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context, chunk, shares;
   int whole_written;              // a request with one share has its result from the first kernel
+  int turned;                     // shares lie [shares][Hkv][D / 4][T * (Hq / Hkv)][4], maxima and sums [shares][Hkv][T * (Hq / Hkv)][2]
   float scale;
   unsigned inverse_heads;         // 2^32 / (Hq / Hkv), rounded up: see node_of
 };

@@ -103,6 +103,12 @@ __device__ __forceinline__ void hide(unsigned* u, unsigned seen) {
     if (!(seen >> i & 1)) u[i] = 0xff800000u;
 }
 
+// The items of a CTA: a round's are dealt forth, the next one's back, so that a CTA does not always have the first tiles of
+// the pairs or always the last, which may be one instead of two.
+__device__ __forceinline__ int item_of(int round) {
+  return round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
 // A bounded wait of a whole warp: all its lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile int* stop, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, code, &g_tree_tc_error));
@@ -234,7 +240,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
       const int kv = warp >> 1, per = kKeys / a.page_size;                // pages a block spans (at most 8)
       bool ok = true;
       int gb = 0, issued = -1;
-      for (int at = blockIdx.x; ok && find_item(a, reqs, at, t); at += gridDim.x) {
+      for (int round = 0; ok && find_item(a, reqs, item_of(round), t); ++round) {
         const int* bt = a.block_table + (size_t)t.s * a.bt_width;
         for (int blk = 0; blk < t.blocks; ++blk, ++gb) {
           const int st = gb % STAGES;
@@ -275,7 +281,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
       const unsigned desc_qk = mma_desc(kKeys, false), desc_pv = mma_desc(D, true);
       int gb = 0, gi = 0, done[2] = {0, 0};                  // blocks and items before this one, steps of each group
       bool ok = true;
-      for (int at = blockIdx.x; ok && find_item(a, reqs, at, t); at += gridDim.x, ++gi) {
+      for (; ok && find_item(a, reqs, item_of(gi), t); ++gi) {
         const bool two = t.tiles == 2;
         const int n0 = t.steps(0), n1 = t.steps(1);
         int to_come = n0 + n1;                               // products of queries and keys
@@ -340,22 +346,27 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
     const unsigned tmem_s = tmem + lane_addr + group * kKeys, tmem_o = tmem + lane_addr + (2 + group) * kKeys;
     const float sc2 = a.scale * kLog2e;
     int gb = 0, gi = 0, done = 0;
-    // An item's queries as the swizzled image has them: with two tiles a thread its row, with one half a row
+    // An item's queries as the swizzled image has them: a warp takes 32 rows of its group's tile, or with one tile 16, and
+    // the lanes of a row its 16-byte pieces side by side
     auto load_queries = [&](const Item& t) {
+      constexpr int AT_ONCE = 32 / PIECES;                   // rows
       const bool two = t.tiles == 2;
-      const int p = t.pair0 + (two ? group * kRows : 0) + row, n = two ? PIECES : PIECES / 2, c0 = two ? 0 : group * n;
-      unsigned char* to = Qs + (two ? group * KB : 0) + row * 128;
-      const bool real = p < t.pairs;
-      const uint4* q = reinterpret_cast<const uint4*>(qkv + (size_t)(real ? t.row0 + p / G : 0) * a.q_stride + (size_t)(t.g * G + p % G) * D);
+      const int c = lane % PIECES, n = two ? 32 : 16, r0 = (two ? quad * 32 : (4 * group + quad) * 16) + lane / PIECES;
+      unsigned char* tile = Qs + (two ? group * KB : 0) + (c >> 3) * kAtom;
+      const int p0 = t.pair0 + (two ? group * kRows : 0);
+      const __nv_bfloat16* q = qkv + (size_t)t.row0 * a.q_stride + (size_t)t.g * G * D + 8 * c;
 #pragma unroll 1
-      for (int h = 0; h < n; h += PIECES / 2) {
-        uint4 v[PIECES / 2];
+      for (int h = 0; h < n; h += 8 * AT_ONCE) {
+        uint4 v[8];
 #pragma unroll
-        for (int i = 0; i < PIECES / 2; ++i) v[i] = real ? q[c0 + h + i] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 8; ++i) {
+          const int p = p0 + r0 + h + i * AT_ONCE, node = node_of(a, p);
+          v[i] = p < t.pairs && h + i * AT_ONCE < n ? *reinterpret_cast<const uint4*>(q + (size_t)node * a.q_stride + (size_t)(p - node * G) * D) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-        for (int i = 0; i < PIECES / 2; ++i) {
-          const int c = c0 + h + i;
-          *reinterpret_cast<uint4*>(to + (c >> 3) * kAtom + (((c & 7) ^ (row & 7)) << 4)) = v[i];
+        for (int i = 0; i < 8; ++i) {
+          const int row = r0 + h + i * AT_ONCE;
+          if (h + i * AT_ONCE < n) *reinterpret_cast<uint4*>(tile + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[i];
         }
       }
       fence_async_smem();
@@ -363,13 +374,13 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
       if (lane == 0) mbar_arrive(&bars->q_full);
     };
     Item next = t;
-    bool more = find_item(a, reqs, blockIdx.x, next);
+    bool more = find_item(a, reqs, item_of(0), next);
     if (more) load_queries(next);
-    for (int at = blockIdx.x; more; at += gridDim.x, ++gi) {
+    for (; more; ++gi) {
       t = next;
       const int tile0 = t.pair0 + (t.tiles == 2 ? group * kRows : 0), p = tile0 + row;
       const bool real = p < t.pairs, idle = tile0 + quad * 32 >= t.pairs;      // idle: none of the warp's rows is anybody's
-      const int node = real ? t.row0 + p / G : 0, head = t.g * G + p % G, n = t.steps(group);
+      const int in_tree = node_of(a, p), node = real ? t.row0 + in_tree : 0, head = t.g * G + p - in_tree * G, n = t.steps(group);
       float m_ref = 0.f, l_run = 0.f;
       bool have = false, ok = true;
       for (int step = 0; ok && step < n; ++step, ++done) {
@@ -458,7 +469,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         if (lane == 0) mbar_arrive(&bars->p_full[group]);
       }
       // the next item's queries, once this one's last scores are there: on their way while its last values are added up
-      more = find_item(a, reqs, at + gridDim.x, next);
+      more = find_item(a, reqs, item_of(gi + 1), next);
       if (more && ok) {
         ok = warp_wait(&bars->q_empty, gi & 1, stop, 1);
         if (ok) load_queries(next);
@@ -479,7 +490,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         const float top = fmaxf(mine.x, further.x), base = top == -INFINITY ? 0.f : top;
         float w0 = exp2f(mine.x - base), w1 = exp2f(further.x - base);
         const float l = mine.y * w0 + further.y * w1, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const size_t place = (size_t)node * a.Hq + head, ws = (size_t)t.share * a.T * a.Hq + place;
+        // (a share's numbers lie [key head][D / 4][pair][4]: the pairs of a warp's lanes side by side)
+        const size_t place = (size_t)node * a.Hq + head, all_pairs = (size_t)a.T * G, pair = (size_t)t.row0 * G + p;
+        const size_t share = (size_t)t.share * a.Hkv + t.g;
         const bool whole = t.shares == 1;
         if (whole) w0 *= inv, w1 *= inv;
         const unsigned o0 = tmem + lane_addr + (2 + (two ? group : 0)) * kKeys, o1 = tmem + lane_addr + 3 * kKeys;
@@ -498,9 +511,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
           }
           if (!real) continue;
           if (!whole) {
-            uint4* to = reinterpret_cast<uint4*>(a.ws_acc + ws * D + c);
+            uint4* to = reinterpret_cast<uint4*>(a.ws_acc) + (share * (D / 4) + c / 4) * all_pairs + pair;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 8; ++i) to[i * all_pairs] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           } else {
             uint4* to = reinterpret_cast<uint4*>(out + place * D + c);
 #pragma unroll
@@ -515,7 +528,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
             }
           }
         }
-        if (real && !whole && (two || group == 0)) reinterpret_cast<float2*>(a.ws_ml)[ws] = make_float2(top, l);
+        if (real && !whole && (two || group == 0)) reinterpret_cast<float2*>(a.ws_ml)[share * all_pairs + pair] = make_float2(top, l);
       }
       tc_fence_before();
       __syncwarp();
@@ -557,8 +570,10 @@ bool tree_tc_fits(int D, int page_size, long long page_rows) {
 
 int tree_tc_chunk(int S, int T, int Hq, int Hkv, int words, int max_context) {
   const long long twos = (std::min(32ll * words, (long long)T) * (Hq / Hkv) + 2 * kRows - 1) / (2 * kRows), items = twos * S * Hkv;
-  const long long shares = std::max(1ll, (148 * 3 + items - 1) / items);
-  const long long chunk = ((max_context + shares - 1) / shares + kKeys - 1) / kKeys * kKeys;
+  const auto keys = [&](long long shares) { return ((max_context + shares - 1) / shares + kKeys - 1) / kKeys * kKeys; };
+  // an item a SM, as long as that is no more than 2,048 keys; else three, since requests are not of one length
+  long long chunk = keys(std::max(1ll, 148 / items));
+  if (chunk > 2048) chunk = keys(std::max(1ll, (148 * 3 + items - 1) / items));
   return (int)std::max(256ll, chunk);
 }
 
