@@ -33,7 +33,7 @@ namespace {
 constexpr int kRows = 128;       // pairs of a CTA (MMA M)
 constexpr int kKeys = 128;       // keys per block
 constexpr int kThreads = 384;
-constexpr int kMostRequests = 1024;   // of a launch: their numbers lie in shared memory
+constexpr int kMostRequests = 512;    // of a launch: their numbers lie in shared memory
 constexpr int kAtom = 128 * 128; // bytes of a swizzle atom column: 128 rows x 64 bf16
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.f;
@@ -48,7 +48,8 @@ struct __align__(8) Barriers {
 };
 
 struct Requests {
-  int upto[kMostRequests + 1];      // items of the requests before
+  int upto[4][kMostRequests + 1];   // items of each class of the requests before
+  int base[5];                      // items of the classes before
   int row0[kMostRequests], nodes[kMostRequests], len[kMostRequests], keys[kMostRequests];
 };
 
@@ -115,24 +116,33 @@ __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile i
 }
 
 // What a CTA works on at a time: share `share` of the keys of (request s, key head g), and `tiles` (1 or 2) tiles of pairs.
+// Items come in classes, the longest first: whole shares of two tiles, a request's last share of two tiles, whole shares of
+// one, last ones of one.  Dealt back and forth in that order the CTAs have much the same to do (16 requests of 32 to 64 nodes
+// behind 8,192 to 16,384 keys: DEALFIG).
 struct Item {
-  int s, g, share, shares, pair0, pairs, tiles, first, last, blocks, row0, len, keys;
+  int cls, s, g, share, shares, pair0, pairs, tiles, first, last, blocks, row0, len, keys;
   __device__ __forceinline__ int steps(int group) const { return tiles == 2 ? blocks : (blocks + 1 - group) >> 1; }
   __device__ __forceinline__ int block(int group, int step) const { return tiles == 2 ? step : 2 * step + group; }
 };
-// Item `at`, which is in request s or a later one; false behind the last.
+__device__ __forceinline__ int two_tiles(int pairs) { return (pairs + kRows - 1) / (2 * kRows); }       // items of two tiles a share
+// Item `at`, which is not before the one that `t` is; false behind the last.
 __device__ __forceinline__ bool find_item(const TreeArgs& a, const Requests& q, int at, Item& t) {
-  if (at >= q.upto[a.S]) return false;
-  while (at >= q.upto[t.s + 1]) ++t.s;
-  const int G = a.Hq / a.Hkv, local = at - q.upto[t.s];
+  if (at >= q.base[4]) return false;
+  while (at >= q.base[t.cls + 1]) ++t.cls, t.s = 0;
+  at -= q.base[t.cls];
+  while (at >= q.upto[t.cls][t.s + 1]) ++t.s;
+  int local = at - q.upto[t.cls][t.s];
   t.row0 = q.row0[t.s], t.len = q.len[t.s], t.keys = q.keys[t.s];
-  t.pairs = q.nodes[t.s] * G;
+  t.pairs = q.nodes[t.s] * (a.Hq / a.Hkv);
   t.shares = (t.keys + a.chunk - 1) / a.chunk;
-  const int twos = (t.pairs + 2 * kRows - 1) / (2 * kRows);
-  t.pair0 = local % twos * 2 * kRows;
-  t.tiles = t.pairs - t.pair0 > kRows ? 2 : 1;
-  t.share = local / twos % t.shares;
-  t.g = local / twos / t.shares;
+  const int twos = two_tiles(t.pairs), whole = t.keys / a.chunk;
+  t.tiles = t.cls < 2 ? 2 : 1;
+  int which = twos;
+  if (t.cls < 2) which = local % twos, local /= twos;
+  t.pair0 = which * 2 * kRows;
+  t.share = whole;
+  if (!(t.cls & 1)) t.share = local % whole, local /= whole;
+  t.g = local;
   t.first = t.share * a.chunk;
   t.last = min(t.first + a.chunk, t.keys);
   t.blocks = (t.last - t.first + kKeys - 1) / kKeys;
@@ -209,26 +219,37 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
     const TreeRequest r = tree_request(a, s);
     if (r.bad && blockIdx.x == 0) atomicCAS(&g_tree_tc_index, 0, 1 + s);
     reqs.row0[s] = r.row0, reqs.nodes[s] = r.nodes, reqs.len[s] = r.len, reqs.keys[s] = r.keys;
-    reqs.upto[s + 1] = (r.nodes * G + 2 * kRows - 1) / (2 * kRows) * ((r.keys + a.chunk - 1) / a.chunk) * a.Hkv;
+    const int pairs = r.nodes * G, twos = two_tiles(pairs), one = pairs > twos * 2 * kRows, whole = pairs ? r.keys / a.chunk : 0;
+    const int rest = pairs && r.keys % a.chunk;
+    reqs.upto[0][s + 1] = twos * whole * a.Hkv;
+    reqs.upto[1][s + 1] = twos * rest * a.Hkv;
+    reqs.upto[2][s + 1] = one * whole * a.Hkv;
+    reqs.upto[3][s + 1] = one * rest * a.Hkv;
   }
   __syncthreads();
-  if (warp == 0) {
+  if (warp < 4) {                        // running sums, a warp a class
     int sum = 0;
-    if (lane == 0) reqs.upto[0] = 0;
+    int* upto = reqs.upto[warp];
+    if (lane == 0) upto[0] = 0;
     for (int s0 = 0; s0 < a.S; s0 += 32) {
-      int v = s0 + lane < a.S ? reqs.upto[s0 + lane + 1] : 0;
+      int v = s0 + lane < a.S ? upto[s0 + lane + 1] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
       }
-      if (s0 + lane < a.S) reqs.upto[s0 + lane + 1] = sum + v;
+      if (s0 + lane < a.S) upto[s0 + lane + 1] = sum + v;
       sum += __shfl_sync(0xffffffffu, v, 31);
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0) {
+    reqs.base[0] = 0;
+    for (int c = 0; c < 4; ++c) reqs.base[c + 1] = reqs.base[c] + reqs.upto[c][a.S];
+  }
+  __syncthreads();
   Item t;
-  t.s = 0;
+  t.cls = t.s = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
