@@ -6,8 +6,9 @@
 //   warps 0, 2   producers of keys and of values: TMA copies (128-byte swizzle), page by page through the block table, in
 //                blocks of 128 keys, into rings
 //   warp 1       issuer of ``tcgen05.mma``: S = Q K^T (128 x 128) and O += P V, with P out of tensor memory
-//   warps 4-7 and 8-11   two softmax groups, a thread a row: the queries of the item to come, then a reference maximum that is raised only when a score passes it
-//                by 2^8 (O's row is then rescaled), weights 2^(s - m) rounded to bfloat16 in the place of the scores
+//   warps 4-11   two softmax groups, a thread a row: the queries of the item to come, then 64 scores at a time, a reference
+//                maximum that is raised only when a score passes it by 8 in the exponent (O's row, and the weights of the
+//                step's first half, are then rescaled), weights 2^(s - m) rounded to bfloat16 in the place of the scores
 //
 // Each group has an S and an O of its own in tensor memory (128 columns each, all 512).  With two tiles of pairs a group
 // takes one of them and both read each block of keys; with one tile they take every other block, and their sums are put
@@ -19,8 +20,9 @@
 // i says whether its i-th score counts.  Keys behind the last node are masked and their values set to zero, since whatever
 // a page holds there would be multiplied by a weight of nothing.
 //
-// The weights are rounded to bfloat16 for the second product (an error of 2^-9 of a weight at most, as independent from
-// key to key as the rounding of the result); their sum is of the unrounded ones.  Scores, maxima, sums and O are float32.
+// The weights are rounded to bfloat16 for the second product (an error of 2^-8 of a weight at most, as independent from
+// key to key as the rounding of the result), a second time where the step's second half makes them less than 2^-8 of the
+// largest; their sum is of the unrounded ones.  Scores, maxima, sums and O are float32.
 //
 // Every wait is bounded: the one that runs out records a code in `g_tree_tc_error` and sets `stop`, upon which the other
 // waits run out too, the CTA's warps leave, wait (bounded) for copies in flight, and free tensor memory.
@@ -118,7 +120,7 @@ __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile i
 // What a CTA works on at a time: share `share` of the keys of (request s, key head g), and `tiles` (1 or 2) tiles of pairs.
 // Items come in classes, the longest first: whole shares of two tiles, a request's last share of two tiles, whole shares of
 // one, last ones of one.  Dealt back and forth in that order the CTAs have much the same to do (16 requests of 32 to 64 nodes
-// behind 8,192 to 16,384 keys: DEALFIG).
+// behind 8,192 to 16,384 keys: 272 us in the order in which they come, 247 so, and 238 with the weights of 64 scores following at once).
 struct Item {
   int cls, s, g, share, shares, pair0, pairs, tiles, first, last, blocks, row0, len, keys;
   __device__ __forceinline__ int steps(int group) const { return tiles == 2 ? blocks : (blocks + 1 - group) >> 1; }
@@ -165,14 +167,6 @@ __device__ __forceinline__ unsigned long long seen64(const TreeArgs& a, const It
     if (sh) v |= word(w + 2) << (64 - sh);
   }
   return v & real;
-}
-
-__device__ __forceinline__ void tc_st16(unsigned taddr, const unsigned* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
 }
 
 template <int D>
@@ -409,70 +403,73 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         if (!warp_wait(&bars->s_full[group], done & 1, stop, 8)) { ok = false; break; }
         tc_fence_after();
         if (!idle) {
-          // Twice through the scores, 32 at a time: for the maximum, and for the weights
-          const bool masked = kb + kKeys > t.len;            // (else keys that every row sees)
-          unsigned long long seen[2] = {~0ull, ~0ull};
-          if (masked)
+          // 64 scores at a time, of which the weights follow at once; a later 64 that raise the reference take the earlier ones'
+          // weights along
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h) (h ? seen[1] : seen[0]) = real ? seen64(a, t, node, kb + 64 * h) : 0ull;
-          auto part = [&](int c) { return (unsigned)((c & 2 ? seen[1] : seen[0]) >> (32 * (c & 1))); };
-          unsigned u[2][32];
-          tc_ld32(tmem_s, u[0]);
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c0 = 0; c0 < 4; c0 += 2)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              tc_wait_ld();
-              tc_ld32(tmem_s + 32 * ((c0 + k + 1) & 3), u[k ^ 1]);           // (at the end the first ones again)
-              if (masked) hide(u[k], part(c0 + k));
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(u[k][i]), __uint_as_float(u[k][i + 1]));
+          for (int h = 0; h < 2; ++h) {
+            unsigned u[64];
+            tc_ld32(tmem_s + 64 * h, u);
+            tc_ld32(tmem_s + 64 * h + 32, u + 32);
+            tc_wait_ld();
+            if (kb + 64 * h + 64 > t.len) {                  // (else keys that every row sees)
+              const unsigned long long seen = real ? seen64(a, t, node, kb + 64 * h) : 0ull;
+              hide(u, (unsigned)seen);
+              hide(u + 32, (unsigned)(seen >> 32));
             }
-          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc2;
-          float alpha = 1.f;
-          bool raise = false;
-          if (!have) {
-            have = mx != -INFINITY;
-            m_ref = have ? mx : 0.f;
-          } else if (mx > m_ref + kRaise) {
-            raise = true;
-            alpha = exp2f(m_ref - mx);
-            m_ref = mx;
-          }
-          const unsigned long long sc = pair_of(sc2, sc2), low = pair_of(-m_ref, -m_ref);
-          unsigned long long sum[2] = {0ull, 0ull};          // (two pairs of 0.f)
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc2;
+            float alpha = 1.f;
+            bool raise = false;
+            if (!have) {
+              have = mx != -INFINITY;
+              m_ref = have ? mx : 0.f;
+            } else if (mx > m_ref + kRaise) {
+              raise = true;
+              alpha = exp2f(m_ref - mx);
+              m_ref = mx;
+            }
+            if (__any_sync(0xffffffffu, raise)) {            // (the product of the step before has run: its scores came first)
+              l_run *= alpha;
 #pragma unroll 1
-          for (int c0 = 0; c0 < 4; c0 += 2)
+              for (int c = 0; c < D / 32; ++c) {
+                unsigned o[32];
+                tc_ld32(tmem_o + 32 * c, o);
+                tc_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              tc_wait_ld();
-              if (c0 + k < 3) tc_ld32(tmem_s + 32 * (c0 + k + 1), u[k ^ 1]);
-              if (masked) hide(u[k], part(c0 + k));
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float x, y;
-                halves(fma2(pair_of(__uint_as_float(u[k][2 * i]), __uint_as_float(u[k][2 * i + 1])), sc, low), x, y);
-                x = ex2(x), y = ex2(y);
-                sum[i & 1] = add2(sum[i & 1], pair_of(x, y));
-                const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-                u[k][i] = *reinterpret_cast<const unsigned*>(&v);
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tc_st32(tmem_o + 32 * c, o);
               }
-              tc_st16(tmem_s + 16 * (c0 + k), u[k]);         // (over scores that have been read for good)
-            }
-          float s0, s1;
-          halves(add2(sum[0], sum[1]), s0, s1);
-          l_run = fmaf(l_run, alpha, s0 + s1);
-          if (__any_sync(0xffffffffu, raise)) {              // (the product of the step before has run: its scores came first)
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              unsigned o[32];
-              tc_ld32(tmem_o + 32 * c, o);
-              tc_wait_ld();
+              if (h) {
+                unsigned o[32];
+                tc_wait_st();
+                tc_ld32(tmem_s, o);
+                tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tc_st32(tmem_o + 32 * c, o);
+                for (int i = 0; i < 32; ++i) {
+                  const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&o[i]);
+                  const __nv_bfloat162 w = __floats2bfloat162_rn(__low2float(v) * alpha, __high2float(v) * alpha);
+                  o[i] = *reinterpret_cast<const unsigned*>(&w);
+                }
+                tc_st32(tmem_s, o);
+              }
             }
+            const unsigned long long sc = pair_of(sc2, sc2), low = pair_of(-m_ref, -m_ref);
+            unsigned long long sum[2] = {0ull, 0ull};        // (two pairs of 0.f)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float x, y;
+              halves(fma2(pair_of(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), sc, low), x, y);
+              x = ex2(x), y = ex2(y);
+              sum[i & 1] = add2(sum[i & 1], pair_of(x, y));
+              const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+              u[i] = *reinterpret_cast<const unsigned*>(&v);
+            }
+            tc_st32(tmem_s + 32 * h, u);                     // (over scores that have been read)
+            float s0, s1;
+            halves(add2(sum[0], sum[1]), s0, s1);
+            l_run += s0 + s1;
           }
           tc_wait_st();
         }

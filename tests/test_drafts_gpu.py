@@ -106,6 +106,40 @@ def test_many_requests_of_many_lengths(heads, most, page_size, form):
             near(got[lo:hi], one, weight, size, c["longest"], torch.bfloat16, heads[2])
 
 
+@pytest.mark.parametrize("spikes", [(), (64,), (0, 64), (63, 127), (31, 32, 95, 96), (10, 70, 129, 200, 300, 301)], ids=str)
+@pytest.mark.parametrize("slope", [0.0, 0.25, -0.25])
+def test_scores_that_rise_within_a_block_of_keys(slope, spikes, form):
+    """Scores that climb from key to key, and keys that stand 16 to 48 above the ones before them."""
+    heads, ps = (8, 1, 128), 64
+    c = make_attention([6, 20], [320, 61], heads, ps, seed=3, shape="chain")
+    q, pages = c["qkv"].clone(), c["pages"].clone()
+    q[:, :heads[0] * 128:128] = 4.0                          # the first dimension carries a score of its own
+    for s in range(2):
+        n = c["row0"][s + 1] - c["row0"][s]
+        for j in range(c["lengths"][s] + n):
+            high = slope * j + sum(16.0 * (1 + i % 3) for i, k in enumerate(spikes) if k == j)
+            pages[c["table"][s, j // ps].long(), 0, :, j % ps, 0] = high / 4 / 0.1
+    c["qkv"], c["pages"] = q.bfloat16().float(), pages.bfloat16().float()
+    want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], ps, c["lengths"], c["row0"], c["mask"], 0.1)
+    # A weight that a later key of its block makes less than 2^-8 of the largest may be rounded twice: 64 of them come to at
+    # most a quarter of the sum, so that much of half a step more.
+    near(attend(c, heads, ps, torch.bfloat16, 0.1), want, weight * 1.25, size, c["longest"], torch.bfloat16, 128)
+    kernels.check_status()
+
+
+def test_more_requests_than_a_launch_takes(form):
+    heads, ps, n = (4, 2, 64), 16, 1100
+    rnd = random.Random(4)
+    sizes = [rnd.randint(0, 3) for _ in range(n)]
+    sizes[511], sizes[512], sizes[1099] = 3, 2, 1
+    lengths = [rnd.randint(0, 40) for _ in range(n)]
+    c = make_attention(sizes, lengths, heads, ps, seed=6)
+    c["qkv"], c["pages"] = c["qkv"].bfloat16().float(), c["pages"].bfloat16().float()
+    want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], ps, c["lengths"], c["row0"], c["mask"], 0.2)
+    near(attend(c, heads, ps, torch.bfloat16, 0.2), want, weight, size, c["longest"], torch.bfloat16, 64)
+    kernels.check_status()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("heads,length", [((4, 2, 64), 0), ((8, 1, 128), 37), ((2, 2, 48), 130), ((16, 1, 128), 600)])
 def test_any_mask_and_rows_that_see_nothing(heads, length, dtype, form):
