@@ -262,70 +262,6 @@ tree_attention_merge_kernel(TreeArgs a, T* __restrict__ out) {
   }
 }
 
-// The same of shares whose numbers lie [key head][D / 4][pair][4] (tree_attention_tc.cu): a CTA takes 32 pairs of a key head,
-// a lane a pair, and each of its eight warps an eighth of the numbers; they come together in shared memory, out of which
-// rows are written whole.
-__global__ void __launch_bounds__(256)
-tree_attention_merge_turned_kernel(TreeArgs a, __nv_bfloat16* __restrict__ out) {
-  constexpr int AT_ONCE = 4;
-  __shared__ __align__(16) float turned[32][128 + 4];
-  __shared__ int row_of[32];                                 // each pair's (row, query head) in the result; -1 for none
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y, G = a.Hq / a.Hkv, each = a.D / 32;
-  const int pair = blockIdx.x * 32 + lane, t = pair / G;
-  chain_wait(a.ws_acc, a.ws_ml, a.lengths, a.row0);
-  const size_t all = (size_t)a.T * G;
-  const bool in = pair < all;
-  int lo = 0, hi = a.S;                                      // the last request that begins at or before the pair's row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.row0[mid] <= t) lo = mid; else hi = mid;
-  }
-  const TreeRequest r = tree_request(a, lo);
-  const int shares = in && t >= r.row0 && t < r.row0 + r.nodes ? (r.keys + a.chunk - 1) / a.chunk : 0;
-  const bool mine = shares > 1;                              // (one share: its result is there already)
-  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + (size_t)g * all + pair;
-  float top = -INFINITY;
-  for (int c = 0; c < (mine ? shares : 0); ++c) top = fmaxf(top, ml[(size_t)c * a.Hkv * all].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
-  float4 sum[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float4* acc = reinterpret_cast<const float4*>(a.ws_acc) + ((size_t)g * (a.D / 4) + warp * each) * all + pair;
-#pragma unroll 1
-  for (int c0 = 0; c0 < (mine ? shares : 0); c0 += AT_ONCE) {
-    float4 v[AT_ONCE][4];
-    float2 x[AT_ONCE];
-#pragma unroll
-    for (int c = 0; c < AT_ONCE; ++c) {
-      const bool there = c0 + c < shares;
-      x[c] = there ? ml[(size_t)(c0 + c) * a.Hkv * all] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (there && i < each) v[c][i] = acc[((size_t)(c0 + c) * a.Hkv * (a.D / 4) + i) * all];
-    }
-#pragma unroll
-    for (int c = 0; c < AT_ONCE; ++c) {
-      const float w = exp2f(x[c].x - base);
-      l += w * x[c].y;
-      if (w != 0.f && c0 + c < shares)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < each) sum[i].x += w * v[c][i].x, sum[i].y += w * v[c][i].y, sum[i].z += w * v[c][i].z, sum[i].w += w * v[c][i].w;
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < each) *reinterpret_cast<float4*>(&turned[lane][4 * (warp * each + i)]) = make_float4(sum[i].x * inv, sum[i].y * inv, sum[i].z * inv, sum[i].w * inv);
-  if (warp == 0) row_of[lane] = mine ? t * a.Hq + g * G + pair - t * G : -1;
-  __syncthreads();
-  for (int e = threadIdx.x; e < 32 * (a.D / 4); e += 256) {
-    const int row = e / (a.D / 4), d = e % (a.D / 4) * 4;
-    if (row_of[row] >= 0) store4(out + (size_t)row_of[row] * a.D + d, &turned[row][d]);
-  }
-}
-
 template <typename T, int NC>
 int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
   const size_t smem = ((size_t)kTreeRows * a.D + 4 * kTile * 4 + (sizeof(T) == 4 ? 2 : 1) * kTile * (2 * a.D + 4)) * sizeof(float);
@@ -340,10 +276,6 @@ int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out
 template <typename T>
 int launch_merge(const TreeArgs& a, void* out, cudaStream_t stream) {
   if (a.shares == 1) return 0;
-  if (a.turned) {
-    launch_chained(tree_attention_merge_turned_kernel, dim3((unsigned)(((long long)a.T * (a.Hq / a.Hkv) + 31) / 32), a.Hkv), dim3(256), 0, stream, a, (__nv_bfloat16*)out);
-    return check_launch("tree_attention_merge_turned");
-  }
   // a warp a row takes eight shares in one trip to memory
   if (a.shares <= 8) launch_chained(tree_attention_merge_kernel<T, 1>, dim3((a.T * a.Hq + 3) / 4), dim3(128), 0, stream, a, (T*)out);
   else launch_chained(tree_attention_merge_kernel<T, 4>, dim3(a.T * a.Hq), dim3(128), 0, stream, a, (T*)out);
@@ -368,11 +300,13 @@ static bool form_takes(int form, int dtype, int Hkv, int D, int page_size, long 
          (form == 2 || (form == 1 && tree_tc_fits(D, page_size, num_pages * 2 * Hkv * page_size)));
 }
 
-// How a call of these sizes is served: 4 times the keys of a share, plus the form: 0 CUDA cores; 1 tcgen05, 2 mma.sync, both
-// for bfloat16, heads of 64 or 128, pages of a multiple of 16 rows, and queries and results on 16-byte boundaries.  Up to 32 pairs a request and key head on
-// average mma.sync, which is then the faster (TREEFIG); beyond, the other where pages are 16, 32, 64 or 128
-// rows.  `form` from 0 on asks for one; it counts where it takes the sizes.  The workspace is a float for every (share, row,
-// query head, D + 2), where there is more than one share.
+// How a call of these sizes is served: 4 times the keys of a share (of form 1: the CTAs), plus the form: 0 CUDA cores; 1
+// tcgen05, 2 mma.sync, both for bfloat16, heads of 64 or 128, pages of a multiple of 16 rows, and queries and results on
+// 16-byte boundaries.  Up to 32 pairs a request and key head on average, or where all is little, mma.sync, which is then the
+// faster: 8 requests of up to 32 nodes, 16 key heads, behind 8,192 keys 76 us and 77 to 83 with tcgen05; 32 of 8 nodes, 4
+// query heads a key head, behind 2,000 46 and 53; one of 27 nodes, 7 query heads, behind 4,097 16.4 and 22.5.  Beyond, the
+// other where pages are 16, 32, 64 or 128 rows: 4 requests of up to 64 nodes, 16 key heads, behind 30,000 142 and 305; 16 of
+// them, 7 query heads, behind 16,384 224 and 812.  `form` from 0 on asks for one; it counts where it takes the sizes.
 extern "C" long long nf_tree_attention_plan(int form, int dtype, int S, int T, int Hq, int Hkv, int D, int page_size, long long num_pages, int words,
                                             int max_context, int aligned) {
   const bool asked = form >= 0 && form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned);
@@ -381,7 +315,7 @@ extern "C" long long nf_tree_attention_plan(int form, int dtype, int S, int T, i
     const long long pairs = ((long long)T * (Hq / Hkv) + S - 1) / S;                 // of a request and key head, on average
     if (form == 1 && (pairs <= 32 || (pairs + 31) / 32 * S * Hkv * ((max_context + 63) / 64) <= 148 * 16)) form = 2;
   }
-  if (form == 1) return 4ll * tree_tc_chunk(S, T, Hq, Hkv, words, max_context) + 1;
+  if (form == 1) return 4ll * tree_tc_ctas(S, T, Hq, Hkv, words, max_context) + 1;
   if (form == 2) return 4ll * tree_mma_chunk(S, T, Hq, Hkv, max_context) + 2;
   // shares enough that a few hundred CTAs are under way, of 64 keys at least
   const long long pairs = std::min(32ll * words, (long long)T) * (Hq / Hkv);
@@ -389,6 +323,13 @@ extern "C" long long nf_tree_attention_plan(int form, int dtype, int S, int T, i
   const long long shares = std::max(1ll, (148 * 4 + ctas - 1) / ctas);
   const long long chunk = ((max_context + shares - 1) / shares + 63) / 64 * 64;
   return 4ll * std::max(64ll, std::min(chunk, 1ll << 20));
+}
+
+// Floats of workspace that a call with this plan wants.
+extern "C" long long nf_tree_attention_workspace(long long plan, int S, int T, int Hq, int D, int max_context) {
+  if ((plan & 3) == 1) return tree_tc_workspace((int)(plan >> 2), S, D);
+  const long long shares = (max_context + (plan >> 2) - 1) / (plan >> 2);
+  return shares > 1 ? shares * T * Hq * (D + 2) : 0;
 }
 
 // A call's operands, 8 bytes each: a caller that packs them at once spares the host a conversion for every argument.
@@ -410,8 +351,8 @@ struct TreeCall {
 
 // qkv [T, q_stride] with the queries in its first Hq * D columns; pages [num_pages, 2, Hkv, page_size, D]; block_table int32
 // [S, bt_width]; lengths int32 [S], row0 int32 [S + 1], mask int32 [T, words]; out [T, Hq * D]: rows that no request has
-// stay as they are.  max_context: no request has more keys, its nodes' among them.  plan, ws: see nf_tree_attention_plan; none
-// where one share takes all keys.
+// stay as they are.  max_context: no request has more keys, its nodes' among them.  plan, ws: see nf_tree_attention_plan
+// and nf_tree_attention_workspace.
 extern "C" int nf_tree_attention(const TreeCall* call) {
   const TreeCall& c = *call;
   const void *qkv = c.qkv, *pages = c.pages;
@@ -430,18 +371,19 @@ extern "C" int nf_tree_attention(const TreeCall* call) {
              "tree attention: bad sizes S=%d T=%d Hq=%d Hkv=%d D=%d page=%d", S, T, Hq, Hkv, D, page_size);
   NF_REQUIRE(dtype == kF32 || dtype == kBF16, "tree attention: unknown type %d", dtype);
   NF_REQUIRE((uintptr_t)pages % 16 == 0, "tree attention: pages must be 16-byte aligned");
-  const int shares = (max_context + chunk - 1) / chunk;
-  NF_REQUIRE(shares == 1 || ws, "tree attention: %d shares of keys want a workspace", shares);
+  const int shares = form == 1 ? 1 : (max_context + chunk - 1) / chunk;
+  NF_REQUIRE(form == 1 ? chunk <= 148 && (chunk == 1 || ws) : shares == 1 || ws, "tree attention: shares of keys want a workspace");
   float* ws_ml = ws ? ws + (size_t)shares * T * Hq * D : nullptr;
   const int G = Hq / Hkv;
   NF_REQUIRE(G < 4096, "tree attention: %d query heads a key head are too many", G);
-  TreeArgs a = {block_table, lengths, row0, mask, ws, ws_ml, q_stride, bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context,
-                chunk, shares, form != 0, form == 1, scale, G == 1 ? 0u : (unsigned)(((1ull << 32) + G - 1) / G)};
+  TreeArgs a = {block_table, lengths, row0, mask, ws, ws_ml, nullptr, q_stride, bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context,
+                chunk, shares, form != 0, scale, G == 1 ? 0u : (unsigned)(((1ull << 32) + G - 1) / G)};
   if (form) {
     const bool aligned = (uintptr_t)qkv % 16 == 0 && q_stride % 8 == 0 && (uintptr_t)out % 16 == 0;
-    NF_REQUIRE(form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned) && chunk % 128 == 0,
+    NF_REQUIRE(form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned) && (form == 1 || chunk % 128 == 0),
                "tree attention: sizes that form %d does not take (D=%d page=%d)", form, D, page_size);
-    if (int rc = form == 1 ? launch_tree_tc(a, qkv, pages, out, stream) : launch_tree_mma(a, qkv, pages, out, stream)) return rc;
+    if (form == 1) return launch_tree_tc(a, chunk, ws, qkv, pages, out, stream);
+    if (int rc = launch_tree_mma(a, qkv, pages, out, stream)) return rc;
   } else if (int rc = dtype == kF32 ? launch_rows_of<float>(a, qkv, pages, out, stream) : launch_rows_of<__nv_bfloat16>(a, qkv, pages, out, stream)) {
     return rc;
   }

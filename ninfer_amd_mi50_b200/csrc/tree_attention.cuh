@@ -14,10 +14,10 @@ constexpr int kTreeRows = 16;     // (node, query head) pairs of a CTA on CUDA c
 struct TreeArgs {
   const int *block_table, *lengths, *row0, *mask;
   float *ws_acc, *ws_ml;          // [shares][T][Hq][D], [shares][T][Hq][2]
+  long long* ws_line;             // the tensor-core form's own: see tree_attention_tc.cu
   long long q_stride;
   int bt_width, words, S, T, Hq, Hkv, D, page_size, num_pages, max_context, chunk, shares;
   int whole_written;              // a request with one share has its result from the first kernel
-  int turned;                     // shares lie [shares][Hkv][D / 4][T * (Hq / Hkv)][4], maxima and sums [shares][Hkv][T * (Hq / Hkv)][2]
   float scale;
   unsigned inverse_heads;         // 2^32 / (Hq / Hkv), rounded up: see node_of
 };
@@ -51,8 +51,9 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, const TreeRequest& 
 
 // The tensor-core form (tree_attention_tc.cu).
 bool tree_tc_fits(int D, int page_size, long long page_rows);
-int tree_tc_chunk(int S, int T, int Hq, int Hkv, int words, int max_context);
-int launch_tree_tc(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream);
+int tree_tc_ctas(int S, int T, int Hq, int Hkv, int words, int max_context);
+long long tree_tc_workspace(int ctas, int S, int D);
+int launch_tree_tc(TreeArgs a, int ctas, float* ws, const void* qkv, const void* pages, void* out, cudaStream_t stream);
 // The form for few pairs (tree_attention_mma.cu).
 int tree_mma_chunk(int S, int T, int Hq, int Hkv, int max_context);
 int launch_tree_mma(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream);

@@ -5,7 +5,7 @@
 // asks for them by TMA, page by page (128-byte swizzle), two stages ahead in a ring of three; each warp takes 16 of the 64
 // keys.  (A fifth warp for the copies would leave the others 168 registers, too few beside 32 rows of sums.)  A warp's step is the
 // usual flash step: S = Q K^T and O += P V by ``mma.sync.m16n8k16`` with the pairs as the 16 rows, a reference maximum that
-// is raised only when a score passes it by 2^8, weights rounded to bfloat16 in between (an error of 2^-9 of a weight at most,
+// is raised only when a score passes it by 8 in the exponent, weights rounded to bfloat16 in between (2^-8 of one at most,
 // as independent from key to key as the rounding of the result, so that the result is 1.4 times as far from the 64-bit one
 // as its own rounding puts it; their sum is of the unrounded ones).  With 16 pairs a CTA a weight goes into the second
 // product as two numbers, its rounding and what that left, which costs 5 % there; with 32 it would be 10 %.  At the end the

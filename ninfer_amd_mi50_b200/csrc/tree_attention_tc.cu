@@ -1,7 +1,7 @@
 // Attention of trees of drafted tokens in bfloat16 on the 5th-generation tensor cores (tree_attention.cu says what is
 // computed).  All (node, query head) pairs of a key head read the same keys, so they are the rows of one product, 128 a
-// tile.  A CTA a SM walks its share of the items (request, key head, share of the keys, two tiles of pairs); the copies for
-// an item are on their way while the one before it is worked off.
+// tile.  A CTA a SM walks its items, each some keys of a request's key head and one or two tiles of pairs; the copies for an
+// item are on their way while the one before it is worked off.
 //
 //   warps 0, 2   producers of keys and of values: TMA copies (128-byte swizzle), page by page through the block table, in
 //                blocks of 128 keys, into rings
@@ -23,6 +23,11 @@
 // The weights are rounded to bfloat16 for the second product (an error of 2^-8 of a weight at most, as independent from
 // key to key as the rounding of the result), a second time where the step's second half makes them less than 2^-8 of the
 // largest; their sum is of the unrounded ones.  Scores, maxima, sums and O are float32.
+//
+// What bounds it: 128 x 128 scores take a group some 3,700 cycles, of which the exponentials of both groups are 2,050 on their
+// own pipe and the products 2,060, one behind the other (the first waits for the scores, the second for the weights).  At this
+// rate the GPU draws its 1,000 W and runs at 1.7 instead of 1.97 GHz, so that what shortens the chain gains less than it
+// saves.  16 requests as above: 224 us, 0.63 PFLOP/s of what the formula asks for, a quarter of the rows being padding.
 //
 // Every wait is bounded: the one that runs out records a code in `g_tree_tc_error` and sets `stop`, upon which the other
 // waits run out too, the CTA's warps leave, wait (bounded) for copies in flight, and free tensor memory.
@@ -50,8 +55,8 @@ struct __align__(8) Barriers {
 };
 
 struct Requests {
-  int upto[4][kMostRequests + 1];   // items of each class of the requests before
-  int base[5];                      // items of the classes before
+  long long start[kMostRequests + 1];   // where each request's work begins on the line
+  long long quota;                      // of a CTA
   int row0[kMostRequests], nodes[kMostRequests], len[kMostRequests], keys[kMostRequests];
 };
 
@@ -106,49 +111,75 @@ __device__ __forceinline__ void hide(unsigned* u, unsigned seen) {
     if (!(seen >> i & 1)) u[i] = 0xff800000u;
 }
 
-// The items of a CTA: a round's are dealt forth, the next one's back, so that a CTA does not always have the first tiles of
-// the pairs or always the last, which may be one instead of two.
-__device__ __forceinline__ int item_of(int round) {
-  return round * (int)gridDim.x + (round & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-}
-
 // A bounded wait of a whole warp: all its lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile int* stop, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, code, &g_tree_tc_error));
 }
 
-// What a CTA works on at a time: share `share` of the keys of (request s, key head g), and `tiles` (1 or 2) tiles of pairs.
-// Items come in classes, the longest first: whole shares of two tiles, a request's last share of two tiles, whole shares of
-// one, last ones of one.  Dealt back and forth in that order the CTAs have much the same to do (16 requests of 32 to 64 nodes
-// behind 8,192 to 16,384 keys: 272 us in the order in which they come, 247 so, and 238 with the weights of 64 scores following at once).
+// The work of a launch lies on a line: request after request, their key heads, their units of two tiles of pairs and at the
+// end, where one tile is left, of one; a unit's length is kAround, for what comes before and behind its blocks, and kTwo or
+// kOne for each block of keys (in hundreds of cycles, as measured).  Each CTA takes as much of the line: the end of a unit that
+// another began, units as a whole, and the beginning of one.  (16 requests of 32 to 64 nodes behind 8,192 to 16,384 keys, 28
+// query heads: 224 us, and 241 with shares of one length dealt to CTAs, the longest first; one of 100 nodes behind 65,536
+// keys 130 and 140; four of up to 64 behind 30,000, 16 key heads 142 and 161.)  Block b of a unit that begins at `o` is the CTA's within whose part o + kAround + b * kTwo lies.
+constexpr int kTwo = 37, kOne = 22, kAround = 120;
+constexpr int kLeast = 4 * kOne;          // of a CTA's part: 256 keys and more
+
+__host__ __device__ __forceinline__ int two_tiles(int pairs) { return (pairs + kRows - 1) / (2 * kRows); }       // units of two tiles
+__device__ __forceinline__ int blocks_of(int keys) { return (keys + kKeys - 1) / kKeys; }
+// The units of a request's key head, and their length on the line.
+struct Units {
+  int twos, all, blocks;
+  __device__ __forceinline__ Units(int pairs, int keys) : twos(two_tiles(pairs)), blocks(blocks_of(keys)) { all = twos + (pairs > twos * 2 * kRows); }
+  __device__ __forceinline__ int block(int u) const { return u < twos ? kTwo : kOne; }
+  __device__ __forceinline__ int length(int u) const { return kAround + block(u) * blocks; }      // (below 2^30 / 128 * 37)
+  __device__ __forceinline__ long long head() const { return (long long)twos * length(0) + (all > twos ? length(twos) : 0); }
+};
+
+// What a CTA works on at a time: blocks of keys of a unit, of (request s, key head g), and `tiles` (1 or 2) tiles of pairs.
 struct Item {
-  int cls, s, g, share, shares, pair0, pairs, tiles, first, last, blocks, row0, len, keys;
+  int s, g, unit, pair0, pairs, tiles, first, last, blocks, row0, len, keys;
+  bool begins, whole;                   // has the unit's first block; all of them
+  long long at;                         // where the unit `unit` begins, which is the one after this item's
   __device__ __forceinline__ int steps(int group) const { return tiles == 2 ? blocks : (blocks + 1 - group) >> 1; }
   __device__ __forceinline__ int block(int group, int step) const { return tiles == 2 ? step : 2 * step + group; }
 };
-__device__ __forceinline__ int two_tiles(int pairs) { return (pairs + kRows - 1) / (2 * kRows); }       // items of two tiles a share
-// Item `at`, which is not before the one that `t` is; false behind the last.
-__device__ __forceinline__ bool find_item(const TreeArgs& a, const Requests& q, int at, Item& t) {
-  if (at >= q.base[4]) return false;
-  while (at >= q.base[t.cls + 1]) ++t.cls, t.s = 0;
-  at -= q.base[t.cls];
-  while (at >= q.upto[t.cls][t.s + 1]) ++t.s;
-  int local = at - q.upto[t.cls][t.s];
-  t.row0 = q.row0[t.s], t.len = q.len[t.s], t.keys = q.keys[t.s];
-  t.pairs = q.nodes[t.s] * (a.Hq / a.Hkv);
-  t.shares = (t.keys + a.chunk - 1) / a.chunk;
-  const int twos = two_tiles(t.pairs), whole = t.keys / a.chunk;
-  t.tiles = t.cls < 2 ? 2 : 1;
-  int which = twos;
-  if (t.cls < 2) which = local % twos, local /= twos;
-  t.pair0 = which * 2 * kRows;
-  t.share = whole;
-  if (!(t.cls & 1)) t.share = local % whole, local /= whole;
-  t.g = local;
-  t.first = t.share * a.chunk;
-  t.last = min(t.first + a.chunk, t.keys);
-  t.blocks = (t.last - t.first + kKeys - 1) / kKeys;
-  return true;
+// The beginning of the CTA's part.
+__device__ __forceinline__ void first_item(const TreeArgs& a, const Requests& q, Item& t) {
+  const long long begin = blockIdx.x * q.quota;
+  int lo = 0, hi = a.S;                 // the last request that begins at or before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (q.start[mid] <= begin) lo = mid; else hi = mid;
+  }
+  const long long head = Units(q.nodes[lo] * (a.Hq / a.Hkv), q.keys[lo]).head();
+  t.s = lo, t.g = t.unit = 0, t.at = q.start[lo];
+  while (t.g < a.Hkv - 1 && t.at + head <= begin) ++t.g, t.at += head;
+}
+// The next item; false behind the CTA's last.
+__device__ __forceinline__ bool next_item(const TreeArgs& a, const Requests& q, Item& t) {
+  const long long begin = blockIdx.x * q.quota, end = begin + q.quota;
+  while (t.s < a.S && t.at < end) {
+    t.pairs = q.nodes[t.s] * (a.Hq / a.Hkv), t.keys = q.keys[t.s];
+    const Units units(t.pairs, t.keys);
+    if (t.unit >= units.all) {
+      t.unit = 0;
+      if (units.all == 0 || ++t.g == a.Hkv) t.g = 0, ++t.s;
+      continue;
+    }
+    const int each = units.block(t.unit), length = each * units.blocks;
+    const long long o = t.at + kAround;
+    t.tiles = t.unit < units.twos ? 2 : 1, t.pair0 = t.unit * 2 * kRows;
+    ++t.unit, t.at = o + length;
+    const int from = (int)min(max(begin - o, 0ll), (long long)length), to = (int)min(max(end - o, 0ll), (long long)length);
+    const int b0 = (from + each - 1) / each, b1 = (to + each - 1) / each;
+    if (b0 >= b1) continue;
+    t.row0 = q.row0[t.s], t.len = q.len[t.s];
+    t.begins = b0 == 0, t.whole = t.begins && b1 == units.blocks;
+    t.first = b0 * kKeys, t.last = min(b1 * kKeys, t.keys), t.blocks = b1 - b0;
+    return true;
+  }
+  return false;
 }
 
 // Bits of the 64 keys from `key0` on that row `row` of the request sees.
@@ -213,37 +244,32 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
     const TreeRequest r = tree_request(a, s);
     if (r.bad && blockIdx.x == 0) atomicCAS(&g_tree_tc_index, 0, 1 + s);
     reqs.row0[s] = r.row0, reqs.nodes[s] = r.nodes, reqs.len[s] = r.len, reqs.keys[s] = r.keys;
-    const int pairs = r.nodes * G, twos = two_tiles(pairs), one = pairs > twos * 2 * kRows, whole = pairs ? r.keys / a.chunk : 0;
-    const int rest = pairs && r.keys % a.chunk;
-    reqs.upto[0][s + 1] = twos * whole * a.Hkv;
-    reqs.upto[1][s + 1] = twos * rest * a.Hkv;
-    reqs.upto[2][s + 1] = one * whole * a.Hkv;
-    reqs.upto[3][s + 1] = one * rest * a.Hkv;
+    reqs.start[s + 1] = a.Hkv * Units(r.nodes * G, r.keys).head();
   }
   __syncthreads();
-  if (warp < 4) {                        // running sums, a warp a class
-    int sum = 0;
-    int* upto = reqs.upto[warp];
-    if (lane == 0) upto[0] = 0;
+  if (warp == 0) {                       // running sums
+    long long sum = 0;
+    if (lane == 0) reqs.start[0] = 0;
     for (int s0 = 0; s0 < a.S; s0 += 32) {
-      int v = s0 + lane < a.S ? upto[s0 + lane + 1] : 0;
+      long long v = s0 + lane < a.S ? reqs.start[s0 + lane + 1] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
       }
-      if (s0 + lane < a.S) upto[s0 + lane + 1] = sum + v;
-      sum += __shfl_sync(0xffffffffu, v, 31);
+      v += sum;
+      if (s0 + lane < a.S) reqs.start[s0 + lane + 1] = v;
+      sum = __shfl_sync(0xffffffffu, v, 31);
     }
+    if (lane == 0) reqs.quota = max((long long)kLeast, (sum + gridDim.x - 1) / gridDim.x);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    reqs.base[0] = 0;
-    for (int c = 0; c < 4; ++c) reqs.base[c + 1] = reqs.base[c] + reqs.upto[c][a.S];
+  if (blockIdx.x == 0 && gridDim.x > 1) {          // for the kernel that adds shares up
+    for (int s = threadIdx.x; s < a.S; s += kThreads) a.ws_line[1 + s] = reqs.start[s];
+    if (threadIdx.x == 0) a.ws_line[0] = reqs.quota;
   }
-  __syncthreads();
   Item t;
-  t.cls = t.s = 0;
+  first_item(a, reqs, t);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -255,7 +281,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
       const int kv = warp >> 1, per = kKeys / a.page_size;                // pages a block spans (at most 8)
       bool ok = true;
       int gb = 0, issued = -1;
-      for (int round = 0; ok && find_item(a, reqs, item_of(round), t); ++round) {
+      while (ok && next_item(a, reqs, t)) {
         const int* bt = a.block_table + (size_t)t.s * a.bt_width;
         for (int blk = 0; blk < t.blocks; ++blk, ++gb) {
           const int st = gb % STAGES;
@@ -296,7 +322,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
       const unsigned desc_qk = mma_desc(kKeys, false), desc_pv = mma_desc(D, true);
       int gb = 0, gi = 0, done[2] = {0, 0};                  // blocks and items before this one, steps of each group
       bool ok = true;
-      for (; ok && find_item(a, reqs, item_of(gi), t); ++gi) {
+      for (; ok && next_item(a, reqs, t); ++gi) {
         const bool two = t.tiles == 2;
         const int n0 = t.steps(0), n1 = t.steps(1);
         int to_come = n0 + n1;                               // products of queries and keys
@@ -389,7 +415,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
       if (lane == 0) mbar_arrive(&bars->q_full);
     };
     Item next = t;
-    bool more = find_item(a, reqs, item_of(0), next);
+    bool more = next_item(a, reqs, next);
     if (more) load_queries(next);
     for (; more; ++gi) {
       t = next;
@@ -487,7 +513,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         if (lane == 0) mbar_arrive(&bars->p_full[group]);
       }
       // the next item's queries, once this one's last scores are there: on their way while its last values are added up
-      more = find_item(a, reqs, item_of(gi + 1), next);
+      more = next_item(a, reqs, next);
       if (more && ok) {
         ok = warp_wait(&bars->q_empty, gi & 1, stop, 1);
         if (ok) load_queries(next);
@@ -508,10 +534,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         const float top = fmaxf(mine.x, further.x), base = top == -INFINITY ? 0.f : top;
         float w0 = exp2f(mine.x - base), w1 = exp2f(further.x - base);
         const float l = mine.y * w0 + further.y * w1, inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        // (a share's numbers lie [key head][D / 4][pair][4]: the pairs of a warp's lanes side by side)
-        const size_t place = (size_t)node * a.Hq + head, all_pairs = (size_t)a.T * G, pair = (size_t)t.row0 * G + p;
-        const size_t share = (size_t)t.share * a.Hkv + t.g;
-        const bool whole = t.shares == 1;
+        // (a share's numbers lie [D / 4][row of the unit][4]: the rows of a warp's lanes side by side)
+        const size_t place = (size_t)node * a.Hq + head, slot = 2 * blockIdx.x + t.begins, at = p - t.pair0;
+        const bool whole = t.whole;
         if (whole) w0 *= inv, w1 *= inv;
         const unsigned o0 = tmem + lane_addr + (2 + (two ? group : 0)) * kKeys, o1 = tmem + lane_addr + 3 * kKeys;
         const int c0 = two ? 0 : group * (D / 2), cn = two ? D : c0 + D / 2;
@@ -529,9 +554,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
           }
           if (!real) continue;
           if (!whole) {
-            uint4* to = reinterpret_cast<uint4*>(a.ws_acc) + (share * (D / 4) + c / 4) * all_pairs + pair;
+            uint4* to = reinterpret_cast<uint4*>(a.ws_acc) + (slot * (D / 4) + c / 4) * (2 * kRows) + at;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i * all_pairs] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 8; ++i) to[i * 2 * kRows] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           } else {
             uint4* to = reinterpret_cast<uint4*>(out + place * D + c);
 #pragma unroll
@@ -546,7 +571,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
             }
           }
         }
-        if (real && !whole && (two || group == 0)) reinterpret_cast<float2*>(a.ws_ml)[share * all_pairs + pair] = make_float2(top, l);
+        if (real && !whole && (two || group == 0)) reinterpret_cast<float2*>(a.ws_ml)[slot * 2 * kRows + at] = make_float2(top, l);
       }
       tc_fence_before();
       __syncwarp();
@@ -561,20 +586,97 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
   }
 }
 
+// The CTA within whose part `at` lies.
+__device__ __forceinline__ int part_of(long long at, long long quota) {
+  return (at | quota) >> 32 ? (int)(at / quota) : (int)((unsigned)at / (unsigned)quota);
+}
+
+// Adds up the shares of units that more CTAs than one worked on, in ascending order: a CTA takes 32 pairs of a key head, a lane
+// a pair, and each of its eight warps an eighth of the numbers; they come together in shared memory, out of which rows are
+// written whole.
+__global__ void __launch_bounds__(256)
+tree_attention_merge_units_kernel(TreeArgs a, __nv_bfloat16* __restrict__ out) {
+  constexpr int AT_ONCE = 4;
+  __shared__ __align__(16) float turned[32][128 + 4];
+  __shared__ int row_of[32];                                 // each pair's (row, query head) in the result; -1 for none
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y, G = a.Hq / a.Hkv, each = a.D / 32;
+  const int pair = blockIdx.x * 32 + lane, t = pair / G;
+  chain_wait(a.ws_acc, a.ws_ml, a.ws_line, a.lengths, a.row0);
+  int lo = 0, hi = a.S;                                      // the last request that begins at or before the pair's row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.row0[mid] <= t) lo = mid; else hi = mid;
+  }
+  const TreeRequest r = tree_request(a, lo);
+  int shares = 0, cta = 0, row = 0;
+  if (pair < (long long)a.T * G && t >= r.row0 && t < r.row0 + r.nodes) {
+    const Units units(r.nodes * G, r.keys);
+    const int p = pair - r.row0 * G, u = p / (2 * kRows);
+    const long long at = a.ws_line[1 + lo] + g * units.head() + (long long)u * units.length(0) + kAround, quota = a.ws_line[0];
+    row = p - u * 2 * kRows;
+    cta = part_of(at, quota);
+    shares = part_of(at + (long long)units.block(u) * (units.blocks - 1), quota) - cta + 1;
+  }
+  const bool mine = shares > 1;                              // (one share: its result is there already)
+  const auto slot = [&](int c) { return (size_t)(2 * (cta + c) + (c == 0)); };
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + row;
+  float top = -INFINITY;
+  for (int c = 0; c < (mine ? shares : 0); ++c) top = fmaxf(top, ml[slot(c) * 2 * kRows].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  float4 sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* acc = reinterpret_cast<const float4*>(a.ws_acc) + warp * each * 2 * kRows + row;
+#pragma unroll 1
+  for (int c0 = 0; c0 < (mine ? shares : 0); c0 += AT_ONCE) {
+    float4 v[AT_ONCE][4];
+    float2 x[AT_ONCE];
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c) {
+      const bool there = c0 + c < shares;
+      x[c] = there ? ml[slot(c0 + c) * 2 * kRows] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (there && i < each) v[c][i] = acc[(slot(c0 + c) * (a.D / 4) + i) * 2 * kRows];
+    }
+#pragma unroll
+    for (int c = 0; c < AT_ONCE; ++c) {
+      const float w = exp2f(x[c].x - base);
+      l += w * x[c].y;
+      if (w != 0.f && c0 + c < shares)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < each) sum[i].x += w * v[c][i].x, sum[i].y += w * v[c][i].y, sum[i].z += w * v[c][i].z, sum[i].w += w * v[c][i].w;
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < each) *reinterpret_cast<float4*>(&turned[lane][4 * (warp * each + i)]) = make_float4(sum[i].x * inv, sum[i].y * inv, sum[i].z * inv, sum[i].w * inv);
+  if (warp == 0) row_of[lane] = mine ? t * a.Hq + g * G + pair - t * G : -1;
+  __syncthreads();
+  for (int e = threadIdx.x; e < 32 * (a.D / 4); e += 256) {
+    const int row = e / (a.D / 4), d = e % (a.D / 4) * 4;
+    if (row_of[row] >= 0) store4(out + (size_t)row_of[row] * a.D + d, &turned[row][d]);
+  }
+}
+
 template <int D>
-int launch_tc(const CUtensorMap& map, TreeArgs a, const void* qkv, void* out, cudaStream_t stream) {
+int launch_tc(const CUtensorMap& map, TreeArgs a, int ctas, const void* qkv, void* out, cudaStream_t stream) {
   const size_t smem = 1024 + (size_t)(2 + 2 * (D == 64 ? 4 : 2)) * (D / 64) * kAtom + sizeof(Barriers) + 4 * kRows * sizeof(float2) + sizeof(Requests);
   static_assert(sizeof(Barriers) % 8 == 0, "float2 follow");
   if (int rc = allow_smem<tree_attention_tc_kernel<D>>(smem)) return rc;
-  const long long twos = (std::min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv) + 2 * kRows - 1) / (2 * kRows);
-  const int S = a.S;
+  const int S = a.S, G = a.Hq / a.Hkv;
+  const dim3 merges((unsigned)(((long long)a.T * G + 31) / 32), a.Hkv);
   for (int s0 = 0; s0 < S; s0 += kMostRequests) {
     a.S = std::min(kMostRequests, S - s0);
-    const long long items = twos * a.shares * a.Hkv * a.S;
-    NF_REQUIRE(items < (1ll << 31), "tree attention: %lld shares of work are too many", items);
-    launch_chained(tree_attention_tc_kernel<D>, dim3((unsigned)std::min(items, 148ll)), dim3(kThreads), smem, stream, map, a, (const __nv_bfloat16*)qkv,
-                   (__nv_bfloat16*)out);
+    launch_chained(tree_attention_tc_kernel<D>, dim3(ctas), dim3(kThreads), smem, stream, map, a, (const __nv_bfloat16*)qkv, (__nv_bfloat16*)out);
     if (int rc = check_launch("tree_attention_tc")) return rc;
+    if (ctas > 1) {
+      launch_chained(tree_attention_merge_units_kernel, merges, dim3(256), 0, stream, a, (__nv_bfloat16*)out);
+      if (int rc = check_launch("tree_attention_merge_units")) return rc;
+    }
     a.lengths += a.S, a.row0 += a.S, a.block_table += (size_t)a.S * a.bt_width;
   }
   return 0;
@@ -586,19 +688,21 @@ bool tree_tc_fits(int D, int page_size, long long page_rows) {
   return (D == 64 || D == 128) && (page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && page_rows < (1ll << 31);
 }
 
-int tree_tc_chunk(int S, int T, int Hq, int Hkv, int words, int max_context) {
-  const long long twos = (std::min(32ll * words, (long long)T) * (Hq / Hkv) + 2 * kRows - 1) / (2 * kRows), items = twos * S * Hkv;
-  const auto keys = [&](long long shares) { return ((max_context + shares - 1) / shares + kKeys - 1) / kKeys * kKeys; };
-  // an item a SM, as long as that is no more than 2,048 keys; else three, since requests are not of one length
-  long long chunk = keys(std::max(1ll, 148 / items));
-  if (chunk > 2048) chunk = keys(std::max(1ll, (148 * 3 + items - 1) / items));
-  return (int)std::max(256ll, chunk);
+// CTAs: as many as there are SMs, or as there may be parts of kLeast.
+int tree_tc_ctas(int S, int T, int Hq, int Hkv, int words, int max_context) {
+  const long long pairs = std::min(32ll * words, (long long)T) * (Hq / Hkv), units = (pairs + 2 * kRows - 1) / (2 * kRows) * S * Hkv;
+  return (int)std::min(148ll, units == 1 && max_context <= 2 * kKeys ? 1 : units * ((max_context + 255ll) / 256 + 2));
 }
 
-int launch_tree_tc(const TreeArgs& a, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
+// Floats: two shares a CTA, the line's parts as 64-bit numbers.
+long long tree_tc_workspace(int ctas, int S, int D) { return ctas > 1 ? 2ll * ctas * 2 * kRows * (D + 2) + 2 * (S + 1) : 0; }
+
+int launch_tree_tc(TreeArgs a, int ctas, float* ws, const void* qkv, const void* pages, void* out, cudaStream_t stream) {
   CUtensorMap map;
   if (int rc = make_map(&map, pages, (long long)a.num_pages * 2 * a.Hkv * a.page_size, a.D, a.page_size)) return rc;
-  return a.D == 64 ? launch_tc<64>(map, a, qkv, out, stream) : launch_tc<128>(map, a, qkv, out, stream);
+  a.ws_acc = ws, a.ws_ml = ws + 2ll * ctas * 2 * kRows * a.D;
+  a.ws_line = (long long*)(a.ws_ml + 2ll * ctas * 2 * kRows * 2);
+  return a.D == 64 ? launch_tc<64>(map, a, ctas, qkv, out, stream) : launch_tc<128>(map, a, ctas, qkv, out, stream);
 }
 
 }  // namespace nf

@@ -29,13 +29,14 @@ MAX_TREE_CONTEXT = 1 << 30
 _I, _L, _P = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
 _SIGNATURES = {
     "nf_tree_attention_plan": [_I] * 8 + [_L] + [_I] * 3,
+    "nf_tree_attention_workspace": [_L] + [_I] * 5,
     "nf_tree_attention": [_P],
     "nf_verify_drafts": [_P, _L, _P, _L] + [_P] * 7 + [_I] * 4 + [_P],
     "nf_compact_cache": [_P, _L] + [_I] * 5 + [_P, _I] + [_P] * 3 + [_I] * 2 + [_P],
     "nf_copy_pages": [_P, _L] + [_I] * 5 + [_P] * 3 + [_I, _P],
 }
 _TREE_CALL = struct.Struct("=20qd2q")          # TreeCall of tree_attention.cu
-_plans = {}             # sizes -> how a call of these is served, as nf_tree_attention_plan says
+_plans = {}             # sizes -> how a call of these is served, as nf_tree_attention_plan says, and its workspace
 _int32, _float32 = torch.int32, torch.float32
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _functions = {}
@@ -47,7 +48,7 @@ def _function(name: str):
     if f is None:
         f = getattr(_lib.load(), name)
         f.argtypes = _SIGNATURES[name]
-        if name == "nf_tree_attention_plan":
+        if name in ("nf_tree_attention_plan", "nf_tree_attention_workspace"):
             f.restype = _L
         _functions[name] = f
     return f
@@ -169,12 +170,13 @@ def tree_attention(qkv: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Te
     if plan is None:
         form = key[-1]
         plan = _function("nf_tree_attention_plan")(-1 if form == "auto" else form, code, S, T, Hq, Hkv, D, page_size, n_pages, words, max_context, key[-2])
+        plan = plan, _function("nf_tree_attention_workspace")(plan, S, T, Hq, D, max_context)
         if len(_plans) >= 4096:
             _plans.clear()
         _plans[key] = plan
-    shares = -(-max_context // (plan >> 2))
+    plan, floats = plan
     # (kept until the call has been made; what comes after it on the stream may have the memory)
-    ws = lengths.new_empty(shares * T * Hq * (D + 2)) if shares > 1 else None
+    ws = lengths.new_empty(floats) if floats else None
     if _begin("nf_tree_attention")(_TREE_CALL.pack(p_q, step, p_pages, block_table.data_ptr(), table_width, lengths.data_ptr(), row0.data_ptr(),
                                                    mask.data_ptr(), words, p_out, 0 if ws is None else ws.data_ptr(), S, T, Hq, Hkv, D, page_size,
                                                    n_pages, max_context, plan, scale, code, _raw_stream(dev))):
