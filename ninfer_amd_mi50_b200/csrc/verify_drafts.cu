@@ -47,10 +47,9 @@ struct Shared {
   int node, next, accepted, n_rejected, todo, summed, first, last;
 };
 
-__device__ __forceinline__ void cluster_meet() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_meet() { cluster_arrive(), cluster_wait(); }
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -212,6 +211,7 @@ __device__ void draw_token(const VerifyArgs& a, Shared& sh, const double* total,
 __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
+  cluster_arrive();                                        // (to be there before another CTA writes to this one)
   const unsigned rank = cluster_rank();
   const int s = blockIdx.x / kCtas;
   const int begin0 = a.row0[s], end0 = a.row0[s + 1];
@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
   if (bad && rank == 0) atomicCAS(&g_verify_error, 0, 1 + s);
   if (threadIdx.x == 0) sh.node = 0, sh.next = 1, sh.accepted = 0, sh.n_rejected = 0, sh.z = 1.0, sh.summed = 0;
   __syncthreads();
+  cluster_wait();
   if (n == 0) {                                            // (no root: the whole cluster leaves)
     if (rank == 0 && threadIdx.x == 0) a.accepted[s] = 0;
     return;
