@@ -28,7 +28,7 @@ compact_cache_kernel(PageShape c, const int* __restrict__ block_table, int bt_wi
                      const int* __restrict__ path, const int* __restrict__ accepted, int most) {
   __shared__ long long from[kMoves], to[kMoves];
   __shared__ int moves, wrong;
-  const int s = blockIdx.y, n = accepted[s], len = lengths[s];
+  const int s = blockIdx.x, n = accepted[s], len = lengths[s];
   if (threadIdx.x == 0) wrong = n < 0 || n > most || len < 0;
   __syncthreads();
   const int* p = path + (size_t)s * most;
@@ -36,7 +36,7 @@ compact_cache_kernel(PageShape c, const int* __restrict__ block_table, int bt_wi
     if (p[j] <= j || (j > 0 && p[j] <= p[j - 1])) wrong = 1;
   __syncthreads();
   if (wrong) {                                             // a path that makes no sense moves nothing
-    if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_pages_error, 0, 1 + s);
+    if (blockIdx.y == 0 && threadIdx.x == 0) atomicCAS(&g_pages_error, 0, 1 + s);
     return;
   }
   const int pieces = c.row_bytes / (int)sizeof(P);
@@ -72,7 +72,7 @@ compact_cache_kernel(PageShape c, const int* __restrict__ block_table, int bt_wi
     }
     __syncthreads();
     const int m = moves;
-    for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < all; i += (long long)gridDim.x * kThreads) {
+    for (long long i = blockIdx.y * (long long)kThreads + threadIdx.x; i < all; i += (long long)gridDim.y * kThreads) {
       const long long plane = i / pieces;
       unsigned char* at = c.base + plane / c.planes * c.layer_bytes + plane % c.planes * c.page_size * c.row_bytes + i % pieces * (long long)sizeof(P);
       for (int j = 0; j < m; ++j) *reinterpret_cast<P*>(at + to[j]) = *reinterpret_cast<const P*>(at + from[j]);
@@ -84,9 +84,9 @@ compact_cache_kernel(PageShape c, const int* __restrict__ block_table, int bt_wi
 template <typename P>
 __global__ void __launch_bounds__(kThreads)
 copy_pages_kernel(PageShape c, const int* __restrict__ src, const int* __restrict__ dst, const int* __restrict__ rows) {
-  const int i = blockIdx.y, a = src[i], b = dst[i], n = rows ? rows[i] : c.page_size;
+  const int i = blockIdx.x, a = src[i], b = dst[i], n = rows ? rows[i] : c.page_size;
   if (a < 0 || a >= c.num_pages || b < 0 || b >= c.num_pages || n < 0 || n > c.page_size) {
-    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicCAS(&g_pages_error, 0, 1 + i);
+    if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicCAS(&g_pages_error, 0, 1 + i);
     return;
   }
   if (a == b) return;
@@ -97,7 +97,7 @@ copy_pages_kernel(PageShape c, const int* __restrict__ src, const int* __restric
   for (int layer = blockIdx.z; layer < c.layers; layer += gridDim.z) {
     const unsigned char* from = c.base + layer * c.layer_bytes + a * page_bytes;
     unsigned char* to = c.base + layer * c.layer_bytes + b * page_bytes;
-    for (long long k = blockIdx.x * (long long)kThreads + threadIdx.x; k < all; k += (long long)gridDim.x * kThreads) {
+    for (long long k = blockIdx.y * (long long)kThreads + threadIdx.x; k < all; k += (long long)gridDim.y * kThreads) {
       const long long at = runs == 1 ? k * (long long)sizeof(P) : k / run * plane_bytes + k % run * (long long)sizeof(P);
       *reinterpret_cast<P*>(to + at) = *reinterpret_cast<const P*>(from + at);
     }
@@ -130,11 +130,11 @@ extern "C" int nf_compact_cache(void* pages, long long layer_bytes, int layers, 
   if (S == 0 || most == 0) return 0;
   const PageShape c = {(unsigned char*)pages, layer_bytes, layers, num_pages, planes, page_size, row_bytes};
   if (int rc = check_shape(c)) return rc;
-  NF_REQUIRE(S > 0 && S <= 65535 && most > 0 && bt_width > 0, "compact cache: bad sizes S=%d most=%d", S, most);
+  NF_REQUIRE(S > 0 && most > 0 && bt_width > 0, "compact cache: bad sizes S=%d most=%d", S, most);
   return by_piece(c, [&](auto p) {
     using P = decltype(p);
     const long long all = (long long)layers * planes * (row_bytes / (int)sizeof(P));
-    const dim3 grid((unsigned)((all + kThreads - 1) / kThreads < 1024 ? (all + kThreads - 1) / kThreads : 1024), S);
+    const dim3 grid(S, (unsigned)((all + kThreads - 1) / kThreads < 1024 ? (all + kThreads - 1) / kThreads : 1024));
     compact_cache_kernel<P><<<grid, kThreads, 0, stream>>>(c, block_table, bt_width, lengths, path, accepted, most);
     return check_launch("compact_cache");
   });
@@ -146,12 +146,12 @@ extern "C" int nf_copy_pages(void* pages, long long layer_bytes, int layers, int
   if (n == 0) return 0;
   const PageShape c = {(unsigned char*)pages, layer_bytes, layers, num_pages, planes, page_size, row_bytes};
   if (int rc = check_shape(c)) return rc;
-  NF_REQUIRE(n > 0 && n <= 65535, "copy pages: %d pages in one call are too many", n);
+  NF_REQUIRE(n > 0, "copy pages: bad number of pages %d", n);
   return by_piece(c, [&](auto p) {
     using P = decltype(p);
     const long long all = (long long)planes * page_size * row_bytes / (int)sizeof(P);
     const long long x = (all + kThreads * 8 - 1) / (kThreads * 8);
-    const dim3 grid((unsigned)(x < 64 ? x : 64), n, layers < 65535 ? layers : 65535);
+    const dim3 grid(n, (unsigned)(x < 64 ? x : 64), layers < 65535 ? layers : 65535);
     copy_pages_kernel<P><<<grid, kThreads, 0, stream>>>(c, src, dst, rows);
     return check_launch("copy_pages");
   });

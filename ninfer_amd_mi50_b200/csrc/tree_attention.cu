@@ -34,11 +34,11 @@ tree_attention_rows_kernel(TreeArgs a, const T* __restrict__ qkv, const T* __res
   float* Qs = smem;                                          // [16][D]
   float* Ps = Qs + kTreeRows * D;                            // [4 warps][32 keys][4 pairs]
   float* KV = Ps + 4 * kTile * 4;                            // [ASYNC ? 2 : 1 tiles][keys [32][KS], values [32][D]]
-  const int s = blockIdx.y / a.Hkv, g = blockIdx.y % a.Hkv;
+  const int of = blockIdx.x / a.shares, share = blockIdx.x % a.shares, s = of / a.Hkv, g = of % a.Hkv;
   const TreeRequest r = tree_request(a, s);
   const int pair0 = blockIdx.z * kTreeRows, pairs = r.nodes * G;
-  const int first = blockIdx.x * a.chunk, last = min(first + a.chunk, r.keys);
-  if (blockIdx.x == 0 && blockIdx.z == 0 && g == 0 && threadIdx.x == 0 && r.bad) atomicCAS(&g_tree_error, 0, 1 + s);
+  const int first = share * a.chunk, last = min(first + a.chunk, r.keys);
+  if (share == 0 && blockIdx.z == 0 && g == 0 && threadIdx.x == 0 && r.bad) atomicCAS(&g_tree_error, 0, 1 + s);
   if (pair0 >= pairs || (first >= last && (first > 0 || a.shares > 1))) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D4 = D / 4;
   const size_t head = (size_t)a.page_size * D, page_stride = 2 * (size_t)a.Hkv * head;
@@ -177,7 +177,7 @@ tree_attention_rows_kernel(TreeArgs a, const T* __restrict__ qkv, const T* __res
       for (int c = 0; c < NC; ++c)
         if (lane + 32 * c < D) out[row * D + lane + 32 * c] = from_float<T>(sum > 0.f ? acc[i][c] / sum : (sum == 0.f ? 0.f : sum));
     } else {
-      const size_t at = (size_t)blockIdx.x * a.T * a.Hq + row;
+      const size_t at = (size_t)share * a.T * a.Hq + row;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         if (lane + 32 * c < D) a.ws_acc[at * D + lane + 32 * c] = acc[i][c];
@@ -267,7 +267,9 @@ int launch_rows(const TreeArgs& a, const void* qkv, const void* pages, void* out
   const size_t smem = ((size_t)kTreeRows * a.D + 4 * kTile * 4 + (sizeof(T) == 4 ? 2 : 1) * kTile * (2 * a.D + 4)) * sizeof(float);
   if (int rc = allow_smem<tree_attention_rows_kernel<T, NC>>(smem)) return rc;
   const int pairs = (int)min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv);
-  const dim3 grid(a.shares, a.S * a.Hkv, (pairs + kTreeRows - 1) / kTreeRows);
+  const long long x = (long long)a.S * a.Hkv * a.shares;
+  NF_REQUIRE(x < (1ll << 31), "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
+  const dim3 grid((unsigned)x, 1, (pairs + kTreeRows - 1) / kTreeRows);
   NF_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
   tree_attention_rows_kernel<T, NC><<<grid, kThreads, smem, stream>>>(a, (const T*)qkv, (const T*)pages, (T*)out);
   return check_launch("tree_attention_rows");

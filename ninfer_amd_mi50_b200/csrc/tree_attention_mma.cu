@@ -80,8 +80,8 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
   float2* stat = reinterpret_cast<float2*>(Qs + ROWS * D * 2);
   Ring* ring = reinterpret_cast<Ring*>(stat + kGroups * ROWS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int s = blockIdx.y / a.Hkv, g = blockIdx.y % a.Hkv, G = a.Hq / a.Hkv;
-  const int first = blockIdx.x * a.chunk;
+  const int s = blockIdx.x / a.Hkv, g = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv;
+  const int first = blockIdx.y * a.chunk;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ring->full[i], 1);
@@ -100,7 +100,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
   };
   if (warp == 0 && (long long)first + box_rows * lane < a.max_context) page = look_up(first + box_rows * lane);
   const TreeRequest r = tree_request(a, s);
-  if (r.bad && blockIdx.x == 0 && blockIdx.z == 0 && g == 0 && threadIdx.x == 0) atomicCAS(&g_tree_mma_error, 0, 1 + s);
+  if (r.bad && blockIdx.y == 0 && blockIdx.z == 0 && g == 0 && threadIdx.x == 0) atomicCAS(&g_tree_mma_error, 0, 1 + s);
   const int pair0 = blockIdx.z * ROWS, pairs = r.nodes * G;
   const int last = min(first + a.chunk, r.keys);
   if (pair0 >= pairs || first >= last) return;
@@ -356,7 +356,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
       *reinterpret_cast<unsigned*>(out + to * D + d) = pack(x.x * inv, x.y * inv);
       *reinterpret_cast<unsigned*>(out + to * D + d + 8) = pack(x.z * inv, x.w * inv);
     } else {
-      const size_t ws = (size_t)blockIdx.x * a.T * a.Hq + to;
+      const size_t ws = (size_t)blockIdx.y * a.T * a.Hq + to;
       *reinterpret_cast<float2*>(a.ws_acc + ws * D + d) = make_float2(x.x, x.y);
       *reinterpret_cast<float2*>(a.ws_acc + ws * D + d + 8) = make_float2(x.z, x.w);
       if (d == 0) reinterpret_cast<float2*>(a.ws_ml)[ws] = make_float2(top, l);
@@ -369,10 +369,10 @@ int launch_mma(const CUtensorMap& map, const TreeArgs& a, int box_rows, const vo
   constexpr size_t smem = smem_bytes<D, MT>();
   if (int rc = allow_smem<tree_attention_mma_kernel<D, MT>>(smem)) return rc;
   const long long pairs = std::min(32ll * a.words, (long long)a.T) * (a.Hq / a.Hkv);
-  const long long y = (long long)a.S * a.Hkv, z = (pairs + 16 * MT - 1) / (16 * MT);
-  NF_REQUIRE(y <= 65535 && z <= 65535, "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
-  launch_chained(tree_attention_mma_kernel<D, MT>, dim3(a.shares, (unsigned)y, (unsigned)z), dim3(kThreads), smem, stream, map, a, box_rows, a.page_size & (a.page_size - 1) ? -1 : __builtin_ctz(a.page_size),
-                 (const __nv_bfloat16*)qkv, (__nv_bfloat16*)out);
+  const long long x = (long long)a.S * a.Hkv, z = (pairs + 16 * MT - 1) / (16 * MT);
+  NF_REQUIRE(x < (1ll << 31) && a.shares <= 65535 && z <= 65535, "tree attention: %d requests with %d key heads are too many", a.S, a.Hkv);
+  launch_chained(tree_attention_mma_kernel<D, MT>, dim3((unsigned)x, a.shares, (unsigned)z), dim3(kThreads), smem, stream, map, a, box_rows,
+                 a.page_size & (a.page_size - 1) ? -1 : __builtin_ctz(a.page_size), (const __nv_bfloat16*)qkv, (__nv_bfloat16*)out);
   return check_launch("tree_attention_mma");
 }
 

@@ -617,9 +617,9 @@ class EmbeddingExtra(Part):
 
 
 class Mixer(Part):
-    tree_safe = False              # whether `forward` serves steps of trees (StepContext.tree)
-
     """Mixes information between the tokens of a request (attention here)."""
+
+    tree_safe = False              # whether `forward` serves steps of trees (StepContext.tree)
 
     def cache_spec(self) -> Optional[CacheSpec]:
         return None

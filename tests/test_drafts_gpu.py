@@ -141,6 +141,21 @@ def test_more_requests_than_a_launch_takes(form):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_more_requests_and_heads_than_a_dimension_of_a_grid(dtype, form):
+    heads, ps, n = (8, 8, 64), 16, 9000
+    if not taken(form, heads, ps, dtype):
+        return
+    sizes, lengths = [0] * n, [0] * n
+    for s in (0, 1, 511, 512, 8190, 8191, 8192, 8999):
+        sizes[s], lengths[s] = 1 + s % 3, 5 + s % 40
+    c = make_attention(sizes, lengths, heads, ps, seed=8)
+    c["qkv"], c["pages"] = c["qkv"].to(dtype).float(), c["pages"].to(dtype).float()
+    want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], ps, c["lengths"], c["row0"], c["mask"], 0.2)
+    near(attend(c, heads, ps, dtype, 0.2), want, weight, size, c["longest"], dtype, 64)
+    kernels.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("heads,length", [((4, 2, 64), 0), ((8, 1, 128), 37), ((2, 2, 48), 130), ((16, 1, 128), 600)])
 def test_any_mask_and_rows_that_see_nothing(heads, length, dtype, form):
     if not taken(form, heads, 16, dtype):
@@ -476,6 +491,26 @@ def test_copied_pages(shape, dtype):
         got = pages.cuda()
         kernels.copy_pages(got, ints(src), ints(dst), None if rows is None else ints(rows))
         assert torch.equal(got.cpu(), want)
+    kernels.check_status()
+
+
+def test_more_copies_and_requests_than_a_dimension_of_a_grid():
+    n = 70000
+    pages = torch.arange(2 * n * 8, dtype=torch.int32, device="cuda").view(2 * n, 2, 4)
+    src, dst = torch.randperm(n, generator=torch.Generator().manual_seed(0)).int(), torch.arange(n, 2 * n, dtype=torch.int32)
+    want = pages.clone()
+    want[n:] = want[:n][src.long().cuda()]
+    kernels.copy_pages(pages, src.cuda(), dst.cuda())
+    assert torch.equal(pages, want)
+    # the second row of every request's only page takes the place of the first behind its root's: page_size 3, path [2]
+    rows = torch.arange(n * 6, device="cuda").to(torch.int16).view(n, 3, 2)
+    want = rows.clone()
+    kept = torch.zeros(n, dtype=torch.int32)
+    kept[[0, 65535, 65536, n - 1]] = 1
+    want[[0, 65535, 65536, n - 1], 1] = want[[0, 65535, 65536, n - 1], 2]
+    kernels.compact_cache(rows, torch.arange(n, dtype=torch.int32, device="cuda").view(n, 1), torch.zeros(n, dtype=torch.int32, device="cuda"),
+                          torch.full((n, 1), 2, dtype=torch.int32, device="cuda"), kept.cuda())
+    assert torch.equal(rows, want)
     kernels.check_status()
 
 
