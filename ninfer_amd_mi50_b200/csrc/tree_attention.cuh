@@ -22,8 +22,8 @@ struct TreeArgs {
   unsigned inverse_heads;         // 2^32 / (Hq / Hkv), rounded up: see node_of
 };
 
-// Pair p's node, p / (Hq / Hkv).  The inverse is at most 1 too large, which at p below 2^16 stays below 2^-16 of a node; one
-// query head a key head has no inverse in 32 bits.
+// Pair p's node, p / (Hq / Hkv).  The inverse is at most 1 too large, which at p below 2^20 (256 nodes of 4,095 heads) stays
+// below 2^-12 of a node, less than a pair's part; one query head a key head has no inverse in 32 bits.
 __device__ __forceinline__ int node_of(const TreeArgs& a, int p) { return a.inverse_heads ? (int)__umulhi((unsigned)p, a.inverse_heads) : p; }
 
 struct TreeRequest {
