@@ -207,6 +207,30 @@ def test_queries_of_rows_that_lie_apart(dtype):
         near(attend(c, heads, 32, dtype, 0.125, qkv=view), want, weight, size, c["longest"], dtype, 64)
 
 
+def test_two_calls_at_once_on_streams_of_their_own(form):
+    """Neither waits for the other, and each has the bits that it has alone."""
+    cases = [make_attention([40, 64, 9], [900, 300, 2000], (8, 2, 128), 64, seed=1), make_attention([30, 2], [1500, 700], (8, 2, 128), 64, seed=2)]
+    args = [((c["qkv"].bfloat16().cuda(), 8, 2, 128, c["pages"].bfloat16().cuda(), c["table"].cuda(), 64, ints(c["lengths"]), ints(c["row0"]),
+              c["mask"].cuda(), c["longest"], 0.1)) for c in cases]
+    v = make_verify([5, 40], 30000, True, seed=3)
+    v = {k: x.cuda() if isinstance(x, torch.Tensor) else x for k, x in v.items()}
+    check = lambda: kernels.verify_drafts(v["probs"], v["tokens"], v["parents"], ints(v["row0"]), v["draws"], 8, v["draft"])
+    alone = [kernels.tree_attention(*x) for x in args] + list(check())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(20):
+        got = []
+        for s, x in zip(streams, args):
+            with torch.cuda.stream(s):
+                got.append(kernels.tree_attention(*x))
+        with torch.cuda.stream(streams[2]):
+            got += check()
+        torch.cuda.synchronize()
+        for x, y in zip(got, alone):
+            assert torch.equal(x, y)
+    kernels.check_status()
+
+
 def test_a_loose_bound_and_other_requests_change_little():
     """What max_context allows beyond the real lengths only changes how keys are shared out."""
     heads = (8, 2, 128)
