@@ -207,6 +207,32 @@ def test_queries_of_rows_that_lie_apart(dtype):
         near(attend(c, heads, 32, dtype, 0.125, qkv=view), want, weight, size, c["longest"], dtype, 64)
 
 
+@pytest.mark.parametrize("dtype,heads,pool", [(torch.bfloat16, (4, 2, 128), 80000), (torch.float32, (4, 2, 128), 40000), (torch.bfloat16, (4, 2, 48), 200000)],
+                         ids=["bf16", "f32", "bf16 of 48"])
+def test_pages_more_than_four_gigabytes_apart(dtype, heads, pool, form):
+    if not taken(form, heads, 64, dtype):
+        return
+    c = make_attention([5, 33], [300, 70], heads, 64, seed=9)
+    c["qkv"], c["pages"] = c["qkv"].to(dtype).float(), c["pages"].to(dtype).float()
+    want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], 64, c["lengths"], c["row0"], c["mask"], 0.1)
+    n = c["pages"].shape[0]
+    pages = torch.empty((pool, *c["pages"].shape[1:]), dtype=dtype, device="cuda")
+    assert pages.nbytes > 4 << 30
+    at = torch.cat([torch.arange(n - n // 2) * 2, pool - 1 - torch.arange(n // 2)])         # both ends of the pool
+    pages[at.cuda()] = c["pages"].to(dtype).cuda()
+    table = torch.where(c["table"] >= 0, at[c["table"].long().clamp_min(0)], -1).int().cuda()
+    got = kernels.tree_attention(c["qkv"].to(dtype).cuda(), *heads, pages, table, 64, ints(c["lengths"]), ints(c["row0"]), c["mask"].cuda(), c["longest"], 0.1)
+    near(got, want, weight, size, c["longest"], dtype, heads[2])
+    # and rows and pages copied there
+    first, last = pages[0].clone(), pages[pool - 1].clone()
+    kernels.copy_pages(pages, ints([0, pool - 1]), ints([pool - 2, 2 * n]))
+    assert torch.equal(pages[pool - 2], first) and torch.equal(pages[2 * n], last)
+    kernels.compact_cache(pages, ints([[pool - 1]]), ints([3]), ints([[4, 9]]), ints([2]))
+    last[:, :, 4], last[:, :, 5] = last[:, :, 7].clone(), last[:, :, 12].clone()
+    assert torch.equal(pages[pool - 1], last)
+    kernels.check_status()
+
+
 def test_two_calls_at_once_on_streams_of_their_own(form):
     """Neither waits for the other, and each has the bits that it has alone."""
     cases = [make_attention([40, 64, 9], [900, 300, 2000], (8, 2, 128), 64, seed=1), make_attention([30, 2], [1500, 700], (8, 2, 128), 64, seed=2)]
