@@ -204,6 +204,44 @@ def test_on_a_stream_of_its_own():
     kernels.check_status()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_trees_and_forks_of_sessions_with_adapters(dtype):
+    """Trees of sessions with different adapters and with none, in one step; a fork keeps its adapter in its place."""
+    from adapter_models import random_adapter
+    cfg = CONFIGS["B"]
+    eng = engine(cfg, dtype, adapters=2, adapter_rank=8)
+    eng.load_adapter("a", random_adapter(cfg, 1, 8), 1.5)
+    eng.load_adapter("b", random_adapter(cfg, 2, 5), -0.5)
+    sessions = [eng.session(name) for name in ("a", None, "b")]
+    drafted = [random_tokens(len(PARENTS), cfg["vocab_size"], 30 + i) for i in range(3)]
+    for i, s in enumerate(sessions):
+        s.prefill(random_tokens(20 + 50 * i, cfg["vocab_size"], i))
+    logits = eng.decode_trees([(s, d, PARENTS) for s, d in zip(sessions, drafted)])
+    for i, s in enumerate(sessions):
+        s.accept([1, 4])
+        f = s.fork()
+        with pytest.raises(Exception, match="accept|not a tree"):
+            f.accept([1])
+        f.close()
+    others = [s.fork() for s in sessions]
+    for i, (s, f) in enumerate(zip(sessions, others)):
+        close(s.decode(7), f.decode(7), dtype)
+    # the same paths run in a line by sessions of their own
+    for i, name in enumerate(("a", None, "b")):
+        with eng.session(name) as line:
+            line.prefill(random_tokens(20 + 50 * i, cfg["vocab_size"], i))
+            for node in (0, 1, 4):
+                close(logits[i * len(PARENTS) + node], line.decode(drafted[i][node]), dtype)
+    for s in sessions:
+        s.close()
+    with pytest.raises(Exception, match="in use"):           # (by the fork)
+        eng.drop_adapter("a")
+    for f in others:
+        f.close()
+    eng.drop_adapter("a")
+    eng._runner.cache.check()
+
+
 def test_refusals():
     from ninfer_amd_mi50_b200.api import NinferError
     from ninfer_amd_mi50_b200.engine import BatchError
