@@ -456,10 +456,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
               alpha = exp2f(m_ref - mx);
               m_ref = mx;
             }
-            if (__any_sync(0xffffffffu, raise)) {            // (the product of the step before has run: its scores came first)
+            if (__any_sync(0xffffffffu, raise)) {
               l_run *= alpha;
+              // O: the product of the step before has run, as its scores came first.  At an item's first step there is none of it
+              // yet, and the other group may still be reading what O holds of the item before: only the issuer waits for that
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
+              for (int c = 0; c < (step ? D / 32 : 0); ++c) {
                 unsigned o[32];
                 tc_ld32(tmem_o + 32 * c, o);
                 tc_wait_ld();
