@@ -61,6 +61,7 @@ __device__ __forceinline__ unsigned pack_two(float x, float y, unsigned& rest) {
 
 struct __align__(8) Ring {
   unsigned long long full[kStages], empty[kStages];
+  unsigned here[kStages];               // bit i: the stage's i-th box has a page; in the place of others lies what lay there before
   int stop;
 };
 
@@ -123,7 +124,10 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
     if (wanted && !there) atomicCAS(&g_tree_mma_error, 0, 1 + s);
     const unsigned boxes = __ballot_sync(0xffffffffu, there);
     if (!__all_sync(0xffffffffu, mbar_wait(&ring->empty[st], ((i / kStages) & 1) ^ 1, stop, 1, &g_tree_mma_wait))) return false;
-    if (elect_one()) mbar_expect_tx(&ring->full[st], (unsigned)__popc(boxes) * 2 * box_rows * D * 2);
+    if (elect_one()) {
+      ((volatile Ring*)ring)->here[st] = boxes >> from;
+      mbar_expect_tx(&ring->full[st], (unsigned)__popc(boxes) * 2 * box_rows * D * 2);
+    }
     __syncwarp();
     if (there) {                                             // each lane its box of keys and of values
       const int in_page = page_shift >= 0 ? (key0 + at) & (a.page_size - 1) : (key0 + at) % a.page_size;
@@ -178,6 +182,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
       value_at[k] = smem_u32(smem) + SB / 2 + (16 * group + vr) * 128 + (((2 * k + vc) ^ (vr & 7)) << 4);
       query_at[k] = smem_u32(Qs) + (lane & 15) * D * 2 + (((2 * k + vc) ^ (lane & 7)) << 4);
     }
+    const unsigned own_box = 1u << 16 * group / box_rows;    // of a stage, the one that the warp's 16 keys lie in
     unsigned stage = 0;
     int st = 0;
     unsigned parity = 0;
@@ -189,6 +194,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
       }
       if (!__all_sync(0xffffffffu, mbar_wait(&ring->full[st], parity, stop, 2, &g_tree_mma_wait))) break;
       if (k0 < last) {
+        const bool gone = !(((volatile Ring*)ring)->here[st] & own_box);     // keys without a page: no row sees them
         float c[MT][2][4] = {};
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -202,7 +208,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
             mma(c[m][1], q, b[2], b[3]);
           }
         }
-        if (k0 + 16 > r.len) {                               // (else keys that every row sees)
+        if (k0 + 16 > r.len || gone) {                       // (else keys that every row sees)
           const int from = k0 - r.len;                       // the tree's node at the tile's first key
 #pragma unroll
           for (int m = 0; m < MT; ++m)
@@ -210,7 +216,7 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
             for (int h = 0; h < 2; ++h) {
               const int p = pair0 + 16 * m + quad + 8 * h;
               unsigned seen = 0;                             // bit i: key k0 + i
-              if (p < pairs) {
+              if (p < pairs && !gone) {
                 const int* words = a.mask + (size_t)(r.row0 + node_of(a, p)) * a.words;
                 const int w = from >> 5;                     // (-1 for keys that the request held)
                 const unsigned lo = w < 0 ? ~0u : (unsigned)words[w], hi = w + 1 < a.words ? (unsigned)words[w + 1] : 0u;
@@ -223,10 +229,11 @@ tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_kv, const __gr
                 for (int x = 0; x < 2; ++x)
                   if (!(seen >> (8 * n + 2 * t4 + x) & 1)) c[m][n][2 * h + x] = -INFINITY;
             }
-          // values behind the last key: whatever lies there would be multiplied by a weight of nothing
+          // values behind the last key, or without a page: whatever lies there would be multiplied by a weight of nothing
           for (int e = lane; e < 16 * PIECES; e += 32)
-            if (k0 + e / PIECES >= last)
+            if (k0 + e / PIECES >= last || gone)
               *reinterpret_cast<uint4*>(smem + stage + SB / 2 + (e % PIECES >> 3) * AB + (16 * group + e / PIECES) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          if (gone) fence_async_smem();                      // (a later stage's copy may take their place)
           __syncwarp();
         }
         float top[MT][2];

@@ -132,8 +132,8 @@ def tree_attention(qkv: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Te
     `max_context`: what lengths[s] and a request's nodes add up to at most.  All of a page's rows must hold finite numbers,
     as they do in a cache manager's pool.
 
-    Rows that belong to no request stay as they were in `out`.  Rows, lengths or nodes outside the bounds, and pages outside
-    the pool, count as if they ended there, and are reported by `check_status`."""
+    Rows that belong to no request stay as they were in `out`.  Rows, lengths or nodes outside the bounds count as if they
+    ended there, keys whose page is not in the pool as if no row saw them; both are reported by `check_status`."""
     dev, dtype = qkv.get_device(), qkv.dtype
     qs, bs, ms, ps = qkv.shape, block_table.shape, mask.shape, pages.shape
     good = (dev >= 0 and len(qs) == 2 and len(bs) == 2 and len(ms) == 2 and len(ps) == 5 and (dtype is torch.bfloat16 or dtype is _float32)

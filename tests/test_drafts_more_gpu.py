@@ -49,3 +49,88 @@ def test_one_tile_of_rows_after_the_other_with_keys_that_rise_at_once(heads, ask
     for _ in range(20):
         assert torch.equal(attend(c, heads, 64, torch.bfloat16, 0.1), first)
     kernels.check_status()
+
+
+def without_missing_pages(c, heads, page_size, pool):
+    """What is left of a step (plain_attention's operands, pages of one row) when nobody sees keys whose page is not there."""
+    lengths, table, mask, rows = [], [], c["mask"].clone(), [torch.zeros(2, heads[1], 1, heads[2])]
+    for s, (lo, hi) in enumerate(zip(c["row0"], c["row0"][1:])):
+        at, held = [], 0
+        for j in range(c["lengths"][s] + hi - lo):
+            page = int(c["table"][s, j // page_size]) if j // page_size < c["table"].shape[1] else -1
+            there = 0 <= page < pool
+            if there:
+                rows.append(c["pages"][page, :, :, j % page_size, None])
+            if j < c["lengths"][s]:
+                held += there
+            elif not there:                                    # a node that nobody sees
+                k = j - c["lengths"][s]
+                mask[lo:hi, k // 32] &= ~(1 << k % 32) if k % 32 < 31 else 0x7fffffff
+            if there or j >= c["lengths"][s]:
+                at.append(len(rows) - 1 if there else 0)
+        lengths.append(held)
+        table.append(at)
+    width = max(1, max(len(t) for t in table))
+    return torch.stack(rows), torch.tensor([t + [-1] * (width - len(t)) for t in table], dtype=torch.int32), lengths, mask
+
+
+@pytest.mark.parametrize("form,dtype,heads,page_size,sizes,lengths", [
+    ("auto", torch.float32, (4, 2, 64), 16, [9, 6, 4], [300, 90, 40]),
+    (0, torch.bfloat16, (6, 2, 48), 7, [9, 6, 4], [100, 90, 40]),
+    (2, torch.bfloat16, (4, 2, 64), 16, [9, 6, 4], [300, 90, 40]),
+    (2, torch.bfloat16, (24, 1, 64), 32, [17, 2, 40], [700, 200, 129]),
+    (2, torch.bfloat16, (4, 4, 128), 64, [3, 4, 1], [900, 30, 500]),
+    (2, torch.bfloat16, (16, 2, 128), 128, [40, 9, 33], [900, 30, 500]),
+    (2, torch.bfloat16, (4, 2, 128), 48, [9, 6, 4], [900, 30, 500]),
+], ids=lambda v: f"{len(v)} requests" if isinstance(v, list) else str(v).replace("torch.", ""))
+def test_keys_of_missing_pages_are_not_seen(form, dtype, heads, page_size, sizes, lengths, asked):
+    """Whatever shared memory still holds there: a call whose keys and values are NaN comes before."""
+    asked(form)
+    for what in ("some", "first", "last", "all of a request", "beyond the table"):
+        c = make_attention(sizes, lengths, heads, page_size, seed=7)
+        c["qkv"], c["pages"] = c["qkv"].to(dtype).float(), c["pages"].to(dtype).float()
+        pool, table = c["pages"].shape[0], c["table"]
+        attend({**c, "pages": torch.full_like(c["pages"], float("nan"))}, heads, page_size, dtype, 0.2)
+        kernels.check_status()
+        if what == "some":
+            gone = torch.rand(table.shape, generator=torch.Generator().manual_seed(3)) < 0.3
+            table[gone] = torch.tensor([-1, pool, 10 ** 6, -2 ** 31], dtype=torch.int32).repeat(table.numel())[:int(gone.sum())]
+        if what == "first":
+            table[:, 0] = -1
+        if what == "last":
+            for s, n in enumerate(sizes):
+                table[s, (lengths[s] + n - 1) // page_size] = pool
+        if what == "all of a request":
+            table[0] = -1
+        if what == "beyond the table":
+            c["table"] = table[:, :max(1, table.shape[1] // 2)].contiguous()
+        pages, rows, held, mask = without_missing_pages(c, heads, page_size, pool)
+        want, weight, size = plain_attention(c["qkv"], *heads, pages, rows, 1, held, c["row0"], mask, 0.2)
+        got = attend(c, heads, page_size, dtype, 0.2)
+        assert form == "auto" or form_of(c, heads, page_size) == form
+        near(got, want, weight, size, c["longest"], dtype, heads[2])
+        assert torch.equal(got, attend(c, heads, page_size, dtype, 0.2))
+        with pytest.raises(kernels.KernelError, match="tree of drafted"):
+            kernels.check_status()
+
+
+@pytest.mark.parametrize("form", ["auto", 0, 1, 2])
+def test_rows_and_lengths_outside_their_bounds_count_as_if_they_ended_there(form, asked):
+    asked(form)
+    heads, dtype = (4, 2, 64), torch.float32 if form == "auto" else torch.bfloat16
+    for what in ("context", "row0", "length"):
+        c = make_attention([4, 6], [40, 90], heads, 16, seed=6)
+        c["qkv"], c["pages"] = c["qkv"].to(dtype).float(), c["pages"].to(dtype).float()
+        plain = {**c}
+        if what == "context":                                  # the second request's keys end there, its nodes' with them
+            c["longest"] = 64
+            plain["lengths"], plain["mask"] = [40, 64], c["mask"].clone()
+            plain["mask"][4:] = 0
+        if what == "row0":
+            c["row0"], plain["row0"] = [0, 4, 99], [0, 4, 10]
+        if what == "length":
+            c["lengths"], plain["lengths"] = [-3, 90], [0, 90]
+        want, weight, size = plain_attention(plain["qkv"], *heads, plain["pages"], plain["table"], 16, plain["lengths"], plain["row0"], plain["mask"], 0.2)
+        near(attend(c, heads, 16, dtype, 0.2), want, weight, size, c["longest"], dtype, heads[2])
+        with pytest.raises(kernels.KernelError, match="tree of drafted"):
+            kernels.check_status()
