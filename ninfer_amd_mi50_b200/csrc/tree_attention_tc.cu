@@ -16,9 +16,9 @@
 // one thread and run in its order, PV(A), QK(A), PV(B), QK(B): the scores of a step are there only when the sums of the step
 // before are, and P, which lies where S did, and O need no signs of their own.
 //
-// Only blocks that reach behind the keys that the request held are masked: there a thread shifts its row's mask so that bit
-// i says whether its i-th score counts.  Keys behind the last node are masked and their values set to zero, since whatever
-// a page holds there would be multiplied by a weight of nothing.
+// Only blocks that reach behind the keys that the request held are masked, and those that lack a page: there a thread shifts
+// its row's mask so that bit i says whether its i-th score counts.  Keys behind the last node or without a page are masked and
+// their values set to zero, since whatever lies there would be multiplied by a weight of nothing.
 //
 // The weights are rounded to bfloat16 for the second product (an error of 2^-8 of a weight at most, as independent from
 // key to key as the rounding of the result), a second time where the step's second half makes them less than 2^-8 of the
@@ -51,6 +51,9 @@ __device__ int g_tree_tc_index = 0;
 struct __align__(8) Barriers {
   unsigned long long q_full, q_empty, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], o_final[2], o_read;
   unsigned tmem_base;
+  // Of the last blocks of keys, bit i: the i-th page is missing, and in its place lies what lay there before.  A word is read
+  // until the block's weights are there, by when the producer is at most STAGES + 1 blocks ahead: twice as many words as stages
+  unsigned lacking[8];
   int stop, quit[2];
 };
 
@@ -182,6 +185,15 @@ __device__ __forceinline__ bool next_item(const TreeArgs& a, const Requests& q, 
   return false;
 }
 
+// Bits of the 64 keys of a block's half that have a page.
+__device__ __forceinline__ unsigned long long paged64(unsigned lacking, int half, int page_size) {
+  unsigned long long v = ~0ull;
+#pragma unroll
+  for (int i = 0; i < 64; i += 16)
+    if (lacking >> (64 * half + i) / page_size & 1) v &= ~(0xffffull << i);
+  return v;
+}
+
 // Bits of the 64 keys from `key0` on that row `row` of the request sees.
 __device__ __forceinline__ unsigned long long seen64(const TreeArgs& a, const Item& t, int row, int key0) {
   const int k0 = key0 - t.len, left = t.keys - key0;
@@ -296,12 +308,15 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
               atomicCAS(&g_tree_tc_index, 0, 1 + t.s);
             }
           }
-          const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+          const unsigned there = __ballot_sync(0xffffffffu, page >= 0), wanted = __ballot_sync(0xffffffffu, lane < per && j < t.last);
           unsigned char* to = KV + (2 * st + kv) * KB;
           void* full = kv ? &bars->v_full[st] : &bars->k_full[st];
           void* empty = kv ? &bars->v_empty[st] : &bars->k_empty[st];
           if (!warp_wait(empty, ((gb / STAGES) & 1) ^ 1, stop, 2)) { ok = false; break; }
-          if (elect_one()) mbar_expect_tx(full, (unsigned)__popc(there) * a.page_size * D * 2);
+          if (elect_one()) {
+            if (kv == 0) ((volatile unsigned*)bars->lacking)[gb % (2 * STAGES)] = wanted & ~there;
+            mbar_expect_tx(full, (unsigned)__popc(there) * a.page_size * D * 2);
+          }
           __syncwarp();
           for (int i = 0; i < per; ++i) {
             const int y = ((__shfl_sync(0xffffffffu, page, i) * 2 + kv) * a.Hkv + t.g) * a.page_size;
@@ -428,6 +443,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
         const int blk = t.block(group, step), kb = t.first + blk * kKeys;
         if (!warp_wait(&bars->s_full[group], done & 1, stop, 8)) { ok = false; break; }
         tc_fence_after();
+        const unsigned lacking = ((volatile unsigned*)bars->lacking)[(gb + blk) % (2 * STAGES)];
         if (!idle) {
           // 64 scores at a time, of which the weights follow at once; a later 64 that raise the reference take the earlier ones'
           // weights along
@@ -437,8 +453,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
             tc_ld32(tmem_s + 64 * h, u);
             tc_ld32(tmem_s + 64 * h + 32, u + 32);
             tc_wait_ld();
-            if (kb + 64 * h + 64 > t.len) {                  // (else keys that every row sees)
-              const unsigned long long seen = real ? seen64(a, t, node, kb + 64 * h) : 0ull;
+            if (kb + 64 * h + 64 > t.len || lacking) {       // (else keys that every row sees)
+              unsigned long long seen = real ? seen64(a, t, node, kb + 64 * h) : 0ull;
+              if (lacking) seen &= paged64(lacking, h, a.page_size);
               hide(u, (unsigned)seen);
               hide(u + 32, (unsigned)(seen >> 32));
             }
@@ -501,13 +518,14 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const __gri
           }
           tc_wait_st();
         }
-        if (t.last - kb < kKeys && (t.tiles == 1 || group == 0)) {       // the request's last block: nothing behind its last key
+        if ((t.last - kb < kKeys || lacking) && (t.tiles == 1 || group == 0)) {      // nothing behind the request's last key, or without a page
           const int b = gb + blk, st = b % STAGES;
           if (!warp_wait(&bars->v_full[st], (b / STAGES) & 1, stop, 9)) { ok = false; break; }
           unsigned char* v = KV + (2 * st + 1) * KB;
-          for (int i = (t.last - kb) * 8 + row; i < kKeys * 8; i += 128)
+          for (int i = (lacking ? 0 : (t.last - kb) * 8) + row; i < kKeys * 8; i += 128)
+            if (kb + i / 8 >= t.last || lacking >> i / 8 / a.page_size & 1)
 #pragma unroll
-            for (int x = 0; x < ATOMS; ++x) reinterpret_cast<uint4*>(v + x * kAtom)[i] = make_uint4(0, 0, 0, 0);
+              for (int x = 0; x < ATOMS; ++x) reinterpret_cast<uint4*>(v + x * kAtom)[i] = make_uint4(0, 0, 0, 0);
           fence_async_smem();
         }
         tc_fence_before();

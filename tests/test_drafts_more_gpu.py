@@ -77,6 +77,11 @@ def without_missing_pages(c, heads, page_size, pool):
 @pytest.mark.parametrize("form,dtype,heads,page_size,sizes,lengths", [
     ("auto", torch.float32, (4, 2, 64), 16, [9, 6, 4], [300, 90, 40]),
     (0, torch.bfloat16, (6, 2, 48), 7, [9, 6, 4], [100, 90, 40]),
+    (1, torch.bfloat16, (4, 2, 64), 16, [9, 6, 4], [300, 90, 40]),
+    (1, torch.bfloat16, (24, 1, 64), 32, [17, 2, 40], [700, 200, 129]),
+    (1, torch.bfloat16, (16, 2, 128), 64, [40, 9, 33], [900, 30, 500]),
+    (1, torch.bfloat16, (8, 2, 128), 128, [70, 9, 33], [900, 30, 500]),
+    (1, torch.bfloat16, (4, 4, 128), 16, [9] * 30, [300, 500, 700] * 10),
     (2, torch.bfloat16, (4, 2, 64), 16, [9, 6, 4], [300, 90, 40]),
     (2, torch.bfloat16, (24, 1, 64), 32, [17, 2, 40], [700, 200, 129]),
     (2, torch.bfloat16, (4, 4, 128), 64, [3, 4, 1], [900, 30, 500]),
