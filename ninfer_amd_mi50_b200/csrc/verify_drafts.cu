@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
           if (a.draft) have = fmax(have - sh.mass[j] * mass_of(a.draft[(size_t)(row0 + c) * a.draft_ld + x]), 0.0);
           else if (sh.token[c] == x) have = 0.0;
         }
-        if ((double)sh.draw[i] * z * (double)sh.ask[i] < have) {
+        if ((double)sh.draw[i] * z * mass_of(sh.ask[i]) < have) {
           if (rank == 0) path[got] = i, said[got] = x;
           ++got;
           v = i, k = 0, z = 1.0;

@@ -6,8 +6,8 @@ import torch
 
 from ninfer_amd_mi50_b200 import kernels
 from ninfer_amd_mi50_b200.kernels import drafts
-from plain_drafts import make_attention, plain_attention
-from test_drafts_gpu import attend, near
+from plain_drafts import make_attention, make_verify, plain_attention, plain_verify
+from test_drafts_gpu import attend, near, verify
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +139,21 @@ def test_rows_and_lengths_outside_their_bounds_count_as_if_they_ended_there(form
         near(attend(c, heads, 16, dtype, 0.2), want, weight, size, c["longest"], dtype, heads[2])
         with pytest.raises(kernels.KernelError, match="tree of drafted"):
             kernels.check_status()
+
+
+@pytest.mark.parametrize("draft", [False, True], ids=["looked up", "drawn"])
+def test_probabilities_that_are_no_positive_numbers_count_as_none(draft):
+    """In the target's rows and in the draft's, at drafted tokens too."""
+    for seed in range(30):
+        c = make_verify([12, 5, 30], 40, draft, seed=seed, near=1.0)
+        g = torch.Generator().manual_seed(seed)
+        odd = torch.tensor([float("nan"), -0.25, -float("inf"), -0.0, -1e30])
+        plain = dict(c)
+        for name in ("probs", "draft") if draft else ("probs",):
+            at = torch.rand(c[name].shape, generator=g) < 0.3
+            at[:, ::7] = False                                 # (something is left of every row)
+            c[name] = torch.where(at, odd[torch.randint(len(odd), at.shape, generator=g)], c[name])
+            plain[name] = torch.where(at, torch.zeros(()), c[name])
+        want = plain_verify(plain["probs"], c["tokens"], c["parents"].tolist(), c["row0"], c["draws"], 29, plain["draft"])
+        assert verify(c, 29) == want, seed
+    kernels.check_status()
