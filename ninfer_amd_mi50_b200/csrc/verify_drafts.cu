@@ -136,7 +136,7 @@ __device__ double sum_left(const VerifyArgs& a, Shared& sh, double* total, int r
 }
 
 // The lowest token whose running sum passes `draw` times the whole, written to `*to` by the CTA that has it; -1 where
-// nothing is left.  Called by all threads of all CTAs after sum_left.  Where rounding keeps the sums of a stretch from what
+// nothing is left, or something infinite.  Called by all threads of all CTAs after sum_left.  Where rounding keeps the sums of a stretch from what
 // they were as parts, the last token that has anything is taken.
 __device__ void draw_token(const VerifyArgs& a, Shared& sh, const double* total, int row0, int n_rejected, bool vec, double all, double draw, int* to) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -151,7 +151,7 @@ __device__ void draw_token(const VerifyArgs& a, Shared& sh, const double* total,
     }
     run += t;
   }
-  if (mine < 0) {
+  if (mine < 0 || all == INFINITY) {
     if (cluster_rank() == 0 && threadIdx.x == 0) *to = -1;
     return;
   }
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(VerifyArgs a) {
   int k = sh.n_rejected;
   if (!sh.summed) pass ^= 1, all = sum_left(a, sh, sh.total[pass], row0, k, vec);      // (where the last thing was a rejection its sums serve the draw)
   if (!(all > 0.0) && k > 0) k = 0, pass ^= 1, all = sum_left(a, sh, sh.total[pass], row0, 0, vec);
-  if (!(all > 0.0) && rank == 0 && threadIdx.x == 0) atomicCAS(&g_verify_error, 0, 1 + s);
+  if ((!(all > 0.0) || all == INFINITY) && rank == 0 && threadIdx.x == 0) atomicCAS(&g_verify_error, 0, 1 + s);
   draw_token(a, sh, sh.total[pass], row0, k, vec, all, (double)sh.draw[0], said + sh.accepted);
   if (rank == 0 && threadIdx.x == 0) a.accepted[s] = sh.accepted;
   cluster_meet();                                          // (no CTA leaves while another may still write to it)

@@ -240,8 +240,9 @@ def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tens
     the model's own, one after the other.  Sums are 64 bits wide.
 
     `path[s]` lists the accepted nodes, `said[s]` their tokens and the next one, both with -1 behind; accepted[s] counts
-    the drafted ones.  What is no positive number counts as a probability of 0; a row that holds nothing gives -1.  Nodes
-    whose token or parent makes no sense are nobody's children.  Both are reported by `check_status`."""
+    the drafted ones.  What is no positive number counts as a probability of 0; a row that holds nothing, or
+    something infinite, gives -1.  Nodes whose token or parent makes no sense are nobody's children.  Both are reported by
+    `check_status`."""
     dev, shape = probs.get_device(), probs.shape
     good = (dev >= 0 and len(shape) == 2 and shape[1] > 0 and probs.dtype is _float32 and draws.dtype is _float32 and tokens.dtype is _int32
             and parents.dtype is _int32 and row0.dtype is _int32 and tokens.get_device() == dev and parents.get_device() == dev

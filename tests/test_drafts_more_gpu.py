@@ -157,3 +157,16 @@ def test_probabilities_that_are_no_positive_numbers_count_as_none(draft):
         want = plain_verify(plain["probs"], c["tokens"], c["parents"].tolist(), c["row0"], c["draws"], 29, plain["draft"])
         assert verify(c, 29) == want, seed
     kernels.check_status()
+
+
+@pytest.mark.parametrize("draft", [False, True], ids=["looked up", "drawn"])
+@pytest.mark.parametrize("at", [0, 20000, 29999])
+def test_a_row_that_holds_something_infinite_says_nothing(at, draft):
+    c = make_verify([4, 3], 30000, draft, seed=2, shape="chain")
+    c["draws"][:] = torch.tensor([0.5, 0.0, 0.0, 0.0, 0.3, 0.0, 0.0])
+    c["probs"][3, at] = float("inf")
+    accepted, path, said = verify(c, 3)
+    assert accepted == [3, 2] and path == [[1, 2, 3], [1, 2, -1]] and said[0] == c["tokens"][1:4].tolist() + [-1]
+    assert 0 <= said[1][2] < 30000
+    with pytest.raises(kernels.KernelError, match="tree of drafted"):
+        kernels.check_status()
