@@ -11,7 +11,6 @@ positions as `places`.  Everything is on the device, so that a captured step ser
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 from typing import Optional, Tuple
 
@@ -25,6 +24,9 @@ __all__ = ["MAX_TREE_NODES", "MAX_VERIFY_NODES", "compact_cache", "copy_pages", 
 MAX_TREE_NODES = 256          # nodes of a request that tree attention takes
 MAX_VERIFY_NODES = 1024       # ... and verification
 MAX_TREE_CONTEXT = 1 << 30
+# of a scale, with which the kernels multiply as a float32 number: beyond, it or its product with log2(e) is 0 (which a hidden
+# score of -inf must not meet), infinite, or has lost bits
+LEAST_SCALE, MOST_SCALE = 2.0 ** -126, 2.0 ** 126
 
 _I, _L, _P = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
 _SIGNATURES = {
@@ -104,8 +106,8 @@ def _refuse_tree(qkv, Hq, Hkv, D, pages, block_table, page_size, lengths, row0, 
                          f"are not of one number of requests (row0: one more)")
     if mask.dim() != 2 or mask.shape[0] != T or not 1 <= mask.shape[1] <= MAX_TREE_NODES // 32:
         raise ValueError(f"{what}: mask is {tuple(mask.shape)}, not [{T}, 1 to {MAX_TREE_NODES // 32}]")
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"{what}: scale={scale} must be positive")
+    if not LEAST_SCALE <= scale <= MOST_SCALE:
+        raise ValueError(f"{what}: scale={scale} must be positive, within 2^-126 and 2^126")
     if not 1 <= max_context <= MAX_TREE_CONTEXT:
         raise ValueError(f"{what}: max_context={max_context} is not within 1 and {MAX_TREE_CONTEXT}")
     if pages.data_ptr() % 16:
@@ -141,7 +143,7 @@ def tree_attention(qkv: torch.Tensor, Hq: int, Hkv: int, D: int, pages: torch.Te
             and pages.get_device() == dev and block_table.get_device() == dev and lengths.get_device() == dev and row0.get_device() == dev
             and mask.get_device() == dev and pages.is_contiguous() and block_table.is_contiguous() and lengths.is_contiguous()
             and row0.is_contiguous() and mask.is_contiguous() and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and D % 16 == 0 and 16 <= D <= 256
-            and page_size > 0 and 1 <= max_context <= MAX_TREE_CONTEXT and 0.0 < scale < math.inf)
+            and page_size > 0 and 1 <= max_context <= MAX_TREE_CONTEXT and LEAST_SCALE <= scale <= MOST_SCALE)
     if good:
         (T, width), (S, table_width), (rows, words), (n_pages, two, heads, size, dim) = qs, bs, ms, ps
         step, one = qkv.stride()

@@ -170,3 +170,18 @@ def test_a_row_that_holds_something_infinite_says_nothing(at, draft):
     assert 0 <= said[1][2] < 30000
     with pytest.raises(kernels.KernelError, match="tree of drafted"):
         kernels.check_status()
+
+
+@pytest.mark.parametrize("form", [0, 1, 2])
+def test_scales_that_float32_does_not_hold_are_refused(form, asked):
+    asked(form)
+    heads = (4, 2, 64)
+    c = make_attention([9, 4], [40, 130], heads, 16, seed=1)
+    c["qkv"], c["pages"] = c["qkv"].bfloat16().float(), c["pages"].bfloat16().float()
+    for bad in (1e-50, 2.0 ** -127, 2.0 ** 127, 1e39, float("inf"), -1.0, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            attend(c, heads, 16, torch.bfloat16, bad)
+    # the least one: every key that is seen counts as much
+    want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], 16, c["lengths"], c["row0"], c["mask"], 2.0 ** -126)
+    near(attend(c, heads, 16, torch.bfloat16, 2.0 ** -126), want, weight, size, c["longest"], torch.bfloat16, 64)
+    kernels.check_status()
