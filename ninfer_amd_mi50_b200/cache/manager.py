@@ -187,6 +187,9 @@ class CacheManager:
     def length(self, req: Hashable) -> int:
         return self.requests[req].length
 
+    def reserved(self, req: Hashable) -> int:
+        return self.requests[req].reserved
+
     def slot(self, req: Hashable) -> int:
         return self.requests[req].slot
 
@@ -272,16 +275,17 @@ class CacheManager:
                 for i in dead:
                     table[i] = row[i] = -1
 
-    def truncate(self, req: Hashable) -> None:
-        """Drop a reservation that was never committed (a step that did not run)."""
+    def truncate(self, req: Hashable, to: int = 0) -> None:
+        """Drop a reservation that was never committed (a step that did not run), or what of it lies beyond `to` tokens."""
         ent = self.requests[req]
-        keep = self._pages_for(ent.length)
+        to = max(ent.length, to)
+        keep = self._pages_for(to)
         for g, table, row in zip(self.groups, ent.tables, ent.rows):
             extra = [p for p in table[keep:] if p >= 0]
             g.pool.give_back(extra)
             del table[keep:]
             row[keep:] = -1
-        ent.reserved = ent.length
+        ent.reserved = min(ent.reserved, to)
 
     def block_table(self, group: int, req: Hashable) -> List[int]:
         return self.requests[req].tables[group]

@@ -49,15 +49,17 @@ class ModelRunner:
 
     # ---- the step -------------------------------------------------------------------
     def reserve(self, entries: Sequence[StepEntry]) -> None:
-        """Hold pages for every entry's new tokens, or for none of them."""
-        done: List[StepEntry] = []
+        """Hold pages for every entry's new tokens, or no more of them than before: what a tree holds that may still be
+        accepted stays."""
+        done: List[Tuple[Hashable, int]] = []
         try:
             for e in entries:
+                held = self.cache.reserved(e.req)
                 self.cache.reserve(e.req, self.cache.length(e.req) + len(e.tokens))
-                done.append(e)
+                done.append((e.req, held))
         except OutOfPages:
-            for e in done:
-                self.cache.truncate(e.req)
+            for req, held in done:
+                self.cache.truncate(req, held)
             raise
 
     def step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -71,9 +73,9 @@ class ModelRunner:
             return torch.empty((0, self.model.vocab_size), dtype=torch.float32, device=self.device)
         arrays = validate_entries(entries, self.cache, self.model.vocab_size)
         adapted = self._check_adapters(entries)
+        self.reserve(entries)
         for e in entries:
             self.trees.pop(e.req, None)        # (a tree that was not accepted: its rows are written over)
-        self.reserve(entries)
         try:
             if self.graphs is not None and self.graphs.eligible(entries):
                 logits, moved = self._step_from_graph(entries, device_tokens)
@@ -119,9 +121,9 @@ class ModelRunner:
         arrays = validate_entries(steps, self.cache, self.model.vocab_size)
         parents = [tree_parents(e, kernels.MAX_TREE_NODES) for e in entries]
         adapted = self._check_adapters(steps)
+        self.reserve(steps)
         for e in entries:
             self.trees.pop(e.req, None)
-        self.reserve(steps)
         lengths = [self.cache.length(e.req) for e in entries]
         try:
             ctx = pack_step(steps, self.cache, self.dtype, self.device, arrays=arrays, adapted=adapted)
