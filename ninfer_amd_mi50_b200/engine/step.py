@@ -62,6 +62,12 @@ class ModelRunner:
                 self.cache.truncate(req, held)
             raise
 
+    def _leave_trees(self, entries: Sequence[StepEntry]) -> None:
+        """Forget trees that were not accepted and that the step is about to write over, with the pages that only they hold."""
+        for e in entries:
+            if self.trees.pop(e.req, None) is not None:
+                self.cache.truncate(e.req, self.cache.length(e.req) + len(e.tokens))
+
     def step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """float32 logits [R, vocab] on the device, R = total wanted rows, in entry order.
 
@@ -74,8 +80,7 @@ class ModelRunner:
         arrays = validate_entries(entries, self.cache, self.model.vocab_size)
         adapted = self._check_adapters(entries)
         self.reserve(entries)
-        for e in entries:
-            self.trees.pop(e.req, None)        # (a tree that was not accepted: its rows are written over)
+        self._leave_trees(entries)
         try:
             if self.graphs is not None and self.graphs.eligible(entries):
                 logits, moved = self._step_from_graph(entries, device_tokens)
@@ -122,8 +127,7 @@ class ModelRunner:
         parents = [tree_parents(e, kernels.MAX_TREE_NODES) for e in entries]
         adapted = self._check_adapters(steps)
         self.reserve(steps)
-        for e in entries:
-            self.trees.pop(e.req, None)
+        self._leave_trees(steps)
         lengths = [self.cache.length(e.req) for e in entries]
         try:
             ctx = pack_step(steps, self.cache, self.dtype, self.device, arrays=arrays, adapted=adapted)

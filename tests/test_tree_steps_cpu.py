@@ -81,3 +81,17 @@ def test_a_pass_that_fails_ends_trees(runner):
         assert free(runner) == 6
         with pytest.raises(BatchError):
             runner.accept({"a": [1]})
+
+
+def test_pages_of_a_tree_that_was_not_accepted_are_given_back(runner):
+    """With the step that writes over it, not at the session's end."""
+    start(runner, "a", 6)
+    runner.tree_step([TreeEntry("a", [1] * 20)])             # 26 places: 7 pages
+    assert free(runner) == 1
+    runner.step([StepEntry("a", [1])])
+    assert free(runner) == 6
+    runner.tree_step([TreeEntry("a", [1] * 20)])
+    runner.tree_step([TreeEntry("a", [1, 2])])
+    assert free(runner) == 5
+    runner.accept({"a": [1]})
+    assert runner.cache.length("a") == 9 and free(runner) == 5
