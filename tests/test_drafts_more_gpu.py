@@ -1,6 +1,8 @@
 """Trees of drafted tokens where a call goes from one piece of work to the next, or its operands do not fit, against plain
 forms in 64 bits."""
 
+import random
+
 import pytest
 import torch
 
@@ -184,4 +186,38 @@ def test_scales_that_float32_does_not_hold_are_refused(form, asked):
     # the least one: every key that is seen counts as much
     want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], 16, c["lengths"], c["row0"], c["mask"], 2.0 ** -126)
     near(attend(c, heads, 16, torch.bfloat16, 2.0 ** -126), want, weight, size, c["longest"], torch.bfloat16, 64)
+    kernels.check_status()
+
+
+@pytest.mark.parametrize("form", [0, 1, 2])
+def test_which_sizes_each_form_takes(form, asked):
+    """A form that is asked for serves every size that it takes, and another one the rest."""
+    asked(form)
+    for dtype in (torch.bfloat16, torch.float32):
+        for heads, page_size in [((4, 2, 64), 16), ((4, 2, 64), 32), ((4, 2, 128), 64), ((1, 1, 128), 128), ((28, 4, 128), 64), ((4, 2, 64), 48), ((2, 2, 128), 96),
+                                 ((4, 2, 128), 256), ((4, 2, 64), 8), ((4, 2, 64), 7), ((6, 2, 48), 16), ((4, 1, 256), 64), ((3, 3, 80), 64)]:
+            c = make_attention([3], [20], heads, page_size, seed=1)
+            attend(c, heads, page_size, dtype, 0.1)
+            whole = dtype == torch.bfloat16 and heads[2] in (64, 128) and page_size % 16 == 0
+            tc = whole and page_size in (16, 32, 64, 128)
+            key = next(k for k in reversed(drafts._plans) if k[2:6] == (*heads, page_size) and k[-1] == form and k[9] == (dtype == torch.bfloat16))
+            # (one request of three nodes: what form 1 does not take and whatever is little goes to form 2, the rest to CUDA cores)
+            assert drafts._plans[key][0] & 3 == (0 if form == 0 or not whole else (1 if form == 1 and tc else 2)), (dtype, heads, page_size)
+    kernels.check_status()
+
+
+@pytest.mark.parametrize("form", [1, 2])
+@pytest.mark.parametrize("heads,most,page_size", [((24, 2, 128), 30, 64), ((8, 8, 64), 40, 16), ((5, 1, 128), 64, 128)])
+def test_every_row_of_many_requests(heads, most, page_size, form, asked):
+    """More work than there are SMs, in items of one tile of rows and of two, each row against the plain form."""
+    asked(form)
+    rnd = random.Random(most)
+    sizes = [rnd.randint(0 if s else 1, most) for s in range(30)]
+    lengths = [rnd.choice([0, 1, 127, 128, 129, rnd.randint(0, 600), rnd.randint(0, 300)]) for _ in sizes]
+    c = make_attention(sizes, lengths, heads, page_size, seed=most, words=2)
+    c["qkv"], c["pages"] = c["qkv"].bfloat16().float(), c["pages"].bfloat16().float()
+    want, weight, size = plain_attention(c["qkv"], *heads, c["pages"], c["table"], page_size, c["lengths"], c["row0"], c["mask"], 0.1)
+    got = attend(c, heads, page_size, torch.bfloat16, 0.1)
+    assert form_of(c, heads, page_size) == form
+    near(got, want, weight, size, c["longest"], torch.bfloat16, heads[2])
     kernels.check_status()
