@@ -11,7 +11,8 @@
 // `chunk` keys.  Shares begin at multiples of `chunk`; each leaves an unnormalised sum with its maximum and its
 // weights' sum, and a second kernel adds a row's shares up in ascending order (with one share the first kernel writes
 // the result).  Scores, weights and sums are float32.  What bounds it is multiply-adds out of shared memory: 2 requests of 12
-// nodes behind 1,000 keys, 16 heads of 128, float32: 32 us, 4 of which the reading of keys and values would take.
+// nodes behind 1,000 keys, 16 heads of 128, float32: 32 us in a replayed graph, 4 of which the reading of keys and values would
+// take.  bfloat16, 27 nodes behind 4,097 keys, 16 query and 4 key heads of 96: 58 us; of 256: 194 (of 128, by mma.sync: 15.5).
 #include "tree_attention.cuh"
 
 namespace nf {
@@ -306,10 +307,13 @@ static bool form_takes(int form, int dtype, int Hkv, int D, int page_size, long 
 // How a call of these sizes is served: 4 times the keys of a share (of form 1: the CTAs), plus the form: 0 CUDA cores; 1
 // tcgen05, 2 mma.sync, both for bfloat16, heads of 64 or 128, pages of a multiple of 16 rows, and queries and results on
 // 16-byte boundaries.  Up to 32 pairs a request and key head on average, or where all is little, mma.sync, which is then the
-// faster: 8 requests of up to 32 nodes, 16 key heads, behind 8,192 keys 76 us and 77 to 83 with tcgen05; 32 of 8 nodes, 4
-// query heads a key head, behind 2,000 46 and 53; one of 27 nodes, 7 query heads, behind 4,097 16.4 and 22.5.  Beyond, the
-// other where pages are 16, 32, 64 or 128 rows: 4 requests of up to 64 nodes, 16 key heads, behind 30,000 142 and 305; 16 of
-// them, 7 query heads, behind 16,384 224 and 812.  `form` from 0 on asks for one; it counts where it takes the sizes.
+// faster (replayed graphs): 8 requests of up to 32 nodes, 16 key heads, behind 8,192 keys 76 to 80 us and 77 to 83 with tcgen05;
+// 32 of 8 nodes, 4 query heads a key head, behind 2,000 47.5 and 53.6; one of 27 nodes, 7 query heads, behind 4,097 16.7 and
+// 22.5.  Beyond, the other where pages are 16, 32, 64 or 128 rows: 4 requests of up to 64 nodes, 16 key heads, behind 30,000 144
+// and 317; 16 of them, 7 query heads, behind 16,384 224 and 849.  Other pages go by mma.sync with any number of pairs, which reads the cache
+// again for each 32 (8 requests of up to 64 nodes, 7 query heads, behind 8,192: pages of 96 rows 269, of 64, on tcgen05, 74);
+// what that form does not take either, to CUDA cores (8 of 32, 4 query heads of 96: 729; of 128, on tcgen05, 34).
+// `form` from 0 on asks for one; it counts where it takes the sizes.
 extern "C" long long nf_tree_attention_plan(int form, int dtype, int S, int T, int Hq, int Hkv, int D, int page_size, long long num_pages, int words,
                                             int max_context, int aligned) {
   const bool asked = form >= 0 && form_takes(form, dtype, Hkv, D, page_size, num_pages, aligned);

@@ -15,8 +15,9 @@
 // block of 128 keys; with few pairs most of that is waiting.
 //
 // What bounds it: a warp's step is a chain of ldmatrix, products, exponentials and products, 0.85 us with 32 pairs, and two CTAs
-// an SM hide some of each other's.  8 requests of up to 32 nodes behind up to 8,192 keys, 16 key heads: 75 us, 5.3 TB/s while
-// the first kernel runs (80 % of what a copy reaches); one of 27 nodes behind 4,097, 28 query heads: 16.5 us.
+// an SM hide some of each other's.  8 requests of up to 32 nodes behind up to 8,192 keys, 16 key heads: 76 us in a replayed
+// graph, 5.2 TB/s while the first kernel runs (80 % of what a copy reaches); one of 27 nodes behind 4,097, 28 query heads: 16.7 us.
+// A word a stage says which of its boxes have a page (1 to 2 % of this; found out once by all threads it was as much).
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 

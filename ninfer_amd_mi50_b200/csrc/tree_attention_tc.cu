@@ -27,7 +27,7 @@
 // What bounds it: 128 x 128 scores take a group some 3,700 cycles, of which the exponentials of both groups are 2,050 on their
 // own pipe and the products 2,060, one behind the other (the first waits for the scores, the second for the weights).  At this
 // rate the GPU draws its 1,000 W and runs at 1.7 instead of 1.97 GHz, so that what shortens the chain gains less than it
-// saves.  16 requests as above: 224 us, 0.63 PFLOP/s of what the formula asks for, a quarter of the rows being padding.
+// saves.  16 requests as below: 224 us in a replayed graph, 0.63 PFLOP/s of what the formula asks for, a quarter of the rows being padding.
 //
 // Every wait is bounded: the one that runs out records a code in `g_tree_tc_error` and sets `stop`, upon which the other
 // waits run out too, the CTA's warps leave, wait (bounded) for copies in flight, and free tensor memory.
@@ -121,10 +121,12 @@ __device__ __forceinline__ bool warp_wait(void* bar, unsigned parity, volatile i
 
 // The work of a launch lies on a line: request after request, their key heads, their units of two tiles of pairs and at the
 // end, where one tile is left, of one; a unit's length is kAround, for what comes before and behind its blocks, and kTwo or
-// kOne for each block of keys (in hundreds of cycles, as measured).  Each CTA takes as much of the line: the end of a unit that
-// another began, units as a whole, and the beginning of one.  (16 requests of 32 to 64 nodes behind 8,192 to 16,384 keys, 28
-// query heads: 224 us, and 241 with shares of one length dealt to CTAs, the longest first; one of 100 nodes behind 65,536
-// keys 130 and 140; four of up to 64 behind 30,000, 16 key heads 142 and 161.)  Block b of a unit that begins at `o` is the CTA's within whose part o + kAround + b * kTwo lies.
+// kOne for each block of keys (in hundreds of cycles, as measured with heads of 128; with heads of 64 they are no measure of
+// time, and only say how the line is shared).  Each CTA takes as much of the line: the end of a unit that another began, units
+// as a whole, and the beginning of one.  (Replayed graphs: 16 requests of 32 to 64 nodes behind 8,192 to 16,384 keys, 28 query
+// heads of 128: 224 us, and 241 with shares of one length dealt to CTAs, the longest first; one of 100 nodes behind 65,536 keys
+// 132 and 140; four of up to 64 behind 30,000, 16 key heads 144 and 161.  The first with heads of 64: 174.)  Block b of a unit
+// that begins at `o` is the CTA's within whose part o + kAround + b * kTwo lies.
 constexpr int kTwo = 37, kOne = 22, kAround = 120;
 constexpr int kLeast = 4 * kOne;          // of a CTA's part: 256 keys and more
 

@@ -15,8 +15,12 @@
 // takes time is the vocabulary's row at the walk's end, and one for a rejection of a drafted token.  A cluster of CTAs
 // takes a request: each walks by itself (the same numbers, the same steps) and reads its part of such rows, a warp a run of
 // neighbouring numbers; the runs' sums change hands in shared memory.  The drawn token is then in one CTA's part, in one
-// warp's run, which the CTA reads once more.  (151,936 tokens: a chain of 5 takes 8.9 us, 8 trees of up to 32 13.8, 64 chains of 6
-// drawn tokens 26, when the rows that are read come at 3.0 TB/s.  One CTA a request took 30 to 178.)
+// warp's run, which the CTA reads once more.  (151,936 tokens: a chain of 5 takes 8.9 us, 8 trees of up to 32 14.0, 64 chains of 6
+// drawn tokens 26.5, when the rows that are read come at 3.0 TB/s.  One CTA a request took 30 to 178.)
+//
+// What a rejection of a drawn token leaves is not kept: each pass over the vocabulary reads the target's row and those of all
+// siblings rejected so far, so that k of them cost some k^2 / 2 rows (1, 7 and 30 refused siblings of one node: 10, 110 and
+// 1,570 us; 8 trees of up to 32 nodes, drawn from a draft model near the target: 64 us).
 #include "common.cuh"
 
 namespace nf {

@@ -322,7 +322,8 @@ def compact_cache(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch
 
     so that they lie as if they alone had been run behind the root, whose row, lengths[s], stays.  pages: a cache group's
     [layers, pages, 2, heads, page_size, D] or [layers, pages, page_size, width], or one layer's; block_table int32
-    [S, width]; path int32 [S, most] (rising) and accepted int32 [S] as `verify_drafts` gives them.  A request whose path does
+    [S, width]; path int32 [S, most] (rising) and accepted int32 [S] as `verify_drafts` gives them.  No two requests may have
+    a page that rows move in, so none is listed twice.  A request whose path does
     not rise keeps its rows as they are, a row whose page is not in the pool stays: both are reported by `check_status`."""
     shape, dev = _pages("compact_cache", pages), pages.get_device()
     ts, ps = block_table.shape, path.shape
